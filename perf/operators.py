@@ -1,0 +1,363 @@
+"""The front of a gated feed-forward block as this library is measured on it: h = act(x Wg^T) * (x Wu^T) for any number
+of rows on GGUF-quantized weights, its backward pass with the weights frozen, and the single-token products on 4-bit
+weights with group scales and zero points.
+
+Shapes are those of an 8B decoder (hidden 4096, key/value 1024, feed-forward 14336) and of a 32000-token vocabulary, as
+in the benchmark and the tests, plus odd and ragged ones.  `draw` spreads sizes, formats and types over the same ranges.
+"""
+import math
+import os
+import sys
+
+import torch
+
+own = False
+
+ELEMS = {"q4_0": 32, "q8_0": 32, "q4_k": 256, "q6_k": 256}
+BYTES = {"q4_0": 18, "q8_0": 34, "q4_k": 144, "q6_k": 210}
+DTYPE = {"f32": torch.float32, "bf16": torch.bfloat16, "f16": torch.float16}
+SIZE = {"f32": 4, "bf16": 2, "f16": 2}
+LARGEST = 2048 * 14336 * 4096  # multiply-adds per matrix of the largest listed case
+
+
+def _gq():
+    path = os.path.join(os.getcwd(), "gretacore-v3_amd")
+    if path not in sys.path:
+        sys.path.insert(0, path)
+    import gq
+    return gq
+
+
+def listed():
+    return [
+        # key/value projection of one token: the smallest call of a decode step
+        {"name": "w4_kv_proj", "kind": "w4", "m": 1, "n": 1024, "k": 4096, "group": 128, "dt": "bf16"},
+        # down projection of one token
+        {"name": "w4_down", "kind": "w4", "m": 1, "n": 4096, "k": 14336, "group": 128, "dt": "f16"},
+        # output logits of two sequences, f32 in and out, finer groups
+        {"name": "w4_logits", "kind": "w4", "m": 2, "n": 32000, "k": 4096, "group": 64, "dt": "f32"},
+        # eleven sequences decoded together, the finest groups, a ragged last group and an odd row count
+        {"name": "w4_batch_ragged", "kind": "w4", "m": 11, "n": 14337, "k": 4090, "group": 32, "dt": "bf16"},
+        # the feed-forward front of one token on the same kind of weights
+        {"name": "w4_front_token", "kind": "w4_front", "m": 1, "n": 14336, "k": 4096, "group": 128, "dt": "bf16"},
+        # the same for a batch of six, tanh-GELU
+        {"name": "w4_front_batch", "kind": "w4_front", "m": 6, "n": 14336, "k": 4096, "group": 64, "dt": "f16",
+         "act": "gelu"},
+        # the front of one token on GGUF weights
+        {"name": "front_token", "kind": "front", "fmt": "q4_k", "m": 1, "n": 14336, "k": 4096, "dt": "bf16"},
+        # sixteen sequences decoded together
+        {"name": "front_batch_16", "kind": "front", "fmt": "q6_k", "m": 16, "n": 14336, "k": 4096, "dt": "f16"},
+        # a ragged prompt, odd row count of the weights, the products kept for a backward pass
+        {"name": "front_ragged_train", "kind": "front", "fmt": "q8_0", "m": 509, "n": 8191, "k": 4096, "dt": "f16",
+         "save": True, "act": "gelu"},
+        # a full 2048-token chunk of a prompt
+        {"name": "front_prompt", "kind": "front", "fmt": "q4_k", "m": 2048, "n": 14336, "k": 4096, "dt": "bf16"},
+        # backward of a short ragged sequence, with tanh-GELU
+        {"name": "front_bwd_ragged", "kind": "bwd", "fmt": "q6_k", "m": 203, "n": 5003, "k": 4096, "dt": "f16",
+         "act": "gelu"},
+        # backward of a full 2048-token step
+        {"name": "front_bwd", "kind": "bwd", "fmt": "q4_0", "m": 2048, "n": 14336, "k": 4096, "dt": "bf16"},
+    ]
+
+
+def _size(rng, lo, hi):
+    return int(round(math.exp(rng.uniform(math.log(lo), math.log(hi)))))
+
+
+def draw(rng):
+    kind = rng.choice(["w4", "w4", "w4_front", "front", "front", "bwd", "bwd"])
+    case = {"kind": kind}
+    if kind in ("w4", "w4_front"):
+        k = _size(rng, 256, 14336)
+        if rng.random() < 0.7:
+            k = -(-k // 32) * 32
+        case.update(m=rng.randint(1, 16), n=_size(rng, 64, 32000 if kind == "w4" else 14336), k=k,
+                    group=rng.choice([32, 64, 128]), dt=rng.choice(["bf16", "bf16", "f16", "f32"]))
+    else:
+        fmt = rng.choice(sorted(ELEMS))
+        m, n = _size(rng, 1, 2048), _size(rng, 64, 14336)
+        k = max(1, _size(rng, 512, 8192) // ELEMS[fmt]) * ELEMS[fmt]
+        n = max(1, min(n, LARGEST // (m * k)))
+        case.update(fmt=fmt, m=m, n=n, k=k, dt=rng.choice(["bf16", "f16"]))
+        if kind == "front":
+            case["save"] = rng.random() < 0.4
+    if kind != "w4":
+        case["act"] = rng.choice(["silu", "silu", "gelu"])
+    return case
+
+
+# ---- inputs -------------------------------------------------------------------
+def _half_bytes(t):
+    return t.to(torch.float16).reshape(-1, 1).view(torch.uint8)
+
+
+def _codes(nb, per, mean, std, lo, hi, g):
+    return torch.randn(nb, per, generator=g, device="cuda").mul_(std).add_(mean).round_().clamp_(lo, hi).to(torch.uint8)
+
+
+def _blocks(fmt, n, k, g):
+    """GGUF blocks of an n x k tensor of roughly normal weights of size 0.02."""
+    nb = n * (k // ELEMS[fmt])
+    u = 0.75 + 0.5 * torch.rand(nb, generator=g, device="cuda")
+    if fmt == "q4_0":
+        q = _codes(nb, 32, 8.0, 2.7, 0, 15, g)
+        sign = 1 - 2 * torch.randint(0, 2, (nb,), generator=g, device="cuda")
+        return torch.cat([_half_bytes(0.0074 * u * sign), q[:, :16] | (q[:, 16:] << 4)], 1)
+    if fmt == "q8_0":
+        q = _codes(nb, 32, 128.0, 42.0, 1, 255, g) ^ 128  # (two's complement)
+        return torch.cat([_half_bytes(0.00048 * u), q], 1)
+    if fmt == "q4_k":  # (d, dmin, 12 B of 6-bit scales and mins, 128 B of nibble pairs)
+        sc = torch.randint(20, 60, (nb, 8), generator=g, device="cuda")
+        mn = (sc + torch.randint(-3, 4, (nb, 8), generator=g, device="cuda")).clamp(0, 63)
+        q = _codes(nb, 256, 7.5, 3.2, 0, 15, g)
+
+        def six(v):  # four codes with the low 2 bits of the next four on top, then those codes' high nibbles
+            top = v[:, 4:] >> 2
+            return [v[:, :4] | ((v[:, 4:] & 3) << 6), top[:, 0:1] | (top[:, 1:2] << 4),
+                    top[:, 2:3] | (top[:, 3:4] << 4)]
+
+        d = (0.00016 * u).to(torch.float16)
+        return torch.cat([_half_bytes(d), _half_bytes(d.float() * 7.5),
+                          torch.cat(six(sc) + six(mn), 1).to(torch.uint8), q[:, 0::2] | (q[:, 1::2] << 4)], 1)
+    q = _codes(nb, 256, 32.0, 11.0, 0, 63, g)
+    lo, hi = q & 15, q >> 4
+    sc = torch.randint(24, 100, (nb, 16), generator=g, device="cuda")
+    sc = (sc * (1 - 2 * torch.randint(0, 2, (nb, 16), generator=g, device="cuda"))).to(torch.int8)
+    return torch.cat([lo[:, 0::2] | (lo[:, 1::2] << 4),
+                      hi[:, 0::4] | (hi[:, 1::4] << 2) | (hi[:, 2::4] << 4) | (hi[:, 3::4] << 6),
+                      sc.view(torch.uint8), _half_bytes(0.00003 * u)], 1)
+
+
+def _w4(n, k, group, g):
+    """4-bit rows: two codes a byte (even k low), one scale and one zero point a group."""
+    ng = -(-k // group)
+    q = torch.randint(0, 256, (n, -(-k // 2)), generator=g, device="cuda", dtype=torch.uint8)
+    s = 0.003 + 0.003 * torch.rand(n, ng, generator=g, device="cuda")
+    z = torch.randint(5, 11, (n, ng), generator=g, device="cuda", dtype=torch.uint8)
+    return {"q": q, "s": s.to(torch.float16), "z": z}
+
+
+def _x(m, k, g):
+    """Activations: normal, with a spread of channel sizes as a normalised hidden state has."""
+    return torch.randn(m, k, generator=g, device="cuda") * torch.exp(0.5 * torch.randn(k, generator=g, device="cuda"))
+
+
+def _inputs(case, seed):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    kind, m, n, k, dt = case["kind"], case["m"], case["n"], case["k"], DTYPE[case["dt"]]
+    if kind in ("w4", "w4_front"):
+        s = {name: _w4(n, k, case["group"], g) for name in (("w",) if kind == "w4" else ("gate", "up"))}
+    else:
+        s = {name: _blocks(case["fmt"], n, k, g) for name in ("gate", "up")}
+    if kind != "bwd":
+        s["x"] = _x(m, k, g).to(dt)
+        return s
+    # the forward pass's products, and gradients of a mean over tokens: sizes differ from token to token, and one
+    # token in eight (prompts, padding) has none
+    for name in ("g", "u"):
+        s[name] = (1.5 * torch.randn(m, n, generator=g, device="cuda")).to(dt)
+    tok = torch.exp(torch.randn(m, 1, generator=g, device="cuda"))
+    tok = tok * (torch.rand(m, 1, generator=g, device="cuda") >= 0.125)
+    s["dh"] = (1e-2 * tok * torch.randn(m, n, generator=g, device="cuda")).to(dt)
+    return s
+
+
+def prepare(case, seed):
+    s = _inputs(case, seed)
+    if own:  # the weights as a program keeps them: laid out once when they are loaded
+        gq = _gq()
+        n, k = case["n"], case["k"]
+        for name in ("w", "gate", "up"):
+            if name not in s:
+                continue
+            if case["kind"] in ("w4", "w4_front"):
+                w = s[name]
+                s[name] = gq.w4_pack(w["q"], w["s"], w["z"], n, k, case["group"])
+            else:
+                s[name] = gq.repack(gq.FORMATS[case["fmt"]], s[name], n, k)
+        s["ws"] = gq.Workspace("cuda")
+    s["case"] = case
+    return s
+
+
+# ---- the operators ---------------------------------------------------------------
+def run(s):
+    return _run_own(s) if own else _run_plain(s)
+
+
+def _run_own(s):
+    gq, c = _gq(), s["case"]
+    kind, n, k = c["kind"], c["n"], c["k"]
+    act = {"silu": gq.ACT_SILU, "gelu": gq.ACT_GELU_TANH}[c.get("act", "silu")]
+    if kind == "w4":
+        return gq.w4_gemv(s["w"], c["group"], s["x"], n, k, out_dtype=s["x"].dtype)
+    if kind == "w4_front":
+        return gq.w4_gate_up(s["gate"], s["up"], c["group"], s["x"], n, k, act=act, out_dtype=s["x"].dtype)
+    fmt = gq.FORMATS[c["fmt"]]
+    if kind == "front":
+        return gq.ffn_gate_up(fmt, s["gate"], s["up"], s["x"], n, k, act=act, save=c.get("save", False),
+                              out_dtype=s["x"].dtype, workspace=s["ws"])
+    return gq.ffn_gate_up_bwd(fmt, s["gate"], s["up"], s["dh"], s["g"], s["u"], n, k, act=act, workspace=s["ws"])
+
+
+def _plain_blocks(fmt, b, n, k):
+    """GGUF blocks -> f32 [n][k]."""
+    def half(col):
+        return b[:, col:col + 2].contiguous().view(torch.float16).float()
+
+    if fmt == "q4_0":
+        q = b[:, 2:]
+        w = (torch.cat([q & 15, q >> 4], 1).float() - 8) * half(0)
+    elif fmt == "q8_0":
+        w = b[:, 2:].contiguous().view(torch.int8).float() * half(0)
+    elif fmt == "q4_k":
+        s = b[:, 4:16].int()
+
+        def six(v):
+            hi = torch.stack([v[:, 4] & 15, v[:, 4] >> 4, v[:, 5] & 15, v[:, 5] >> 4], 1)
+            return torch.cat([v[:, :4] & 63, (v[:, :4] >> 6) | (hi << 2)], 1).float()
+
+        sc, mn = six(s[:, :6]) * half(0), six(s[:, 6:]) * half(2)
+        q = b[:, 16:]
+        q = torch.stack([q & 15, q >> 4], 2).reshape(-1, 8, 32).float()
+        w = q * sc[:, :, None] - mn[:, :, None]
+    else:
+        ql, qh = b[:, :128], b[:, 128:192]
+        lo = torch.stack([ql & 15, ql >> 4], 2).reshape(-1, 256)
+        hi = torch.stack([(qh >> (2 * j)) & 3 for j in range(4)], 2).reshape(-1, 256)
+        sc = b[:, 192:208].contiguous().view(torch.int8).float() * half(208)
+        w = ((lo | (hi << 4)).float() - 32).reshape(-1, 16, 16) * sc[:, :, None]
+    return w.reshape(n, k)
+
+
+def _plain_w4(w, n, k, group):
+    q = torch.stack([w["q"] & 15, w["q"] >> 4], 2).reshape(n, -1)[:, :k].float()
+    s = w["s"].float().repeat_interleave(group, 1)[:, :k]
+    z = w["z"].float().repeat_interleave(group, 1)[:, :k]
+    return (q - z) * s
+
+
+def _plain_act(act, g):
+    """act(g) and its derivative."""
+    if act == "silu":
+        sg = 1 / (1 + torch.exp(-g))
+        return g * sg, sg * (1 + g * (1 - sg))
+    c = math.sqrt(2 / math.pi)
+    t = torch.tanh(c * (g + 0.044715 * g * g * g))
+    return 0.5 * g * (1 + t), 0.5 * (1 + t) + 0.5 * g * (1 - t * t) * c * (1 + 3 * 0.044715 * g * g)
+
+
+def _run_plain(s):
+    c = s["case"]
+    kind, n, k, dt = c["kind"], c["n"], c["k"], DTYPE[c["dt"]]
+
+    def weights(name):
+        if kind in ("w4", "w4_front"):
+            return _plain_w4(s[name], n, k, c["group"])
+        return _plain_blocks(c["fmt"], s[name], n, k)
+
+    if kind == "w4":
+        return (s["x"].float() @ weights("w").t()).to(dt)
+    if kind == "bwd":
+        dh, g, u = s["dh"].float(), s["g"].float(), s["u"].float()
+        a, da = _plain_act(c.get("act", "silu"), g)
+        dg, du = dh * u * da, dh * a
+        dx = dg @ weights("gate") + du @ weights("up")
+        return {"dx": dx.to(dt), "dg": dg.to(dt), "du": du.to(dt)}
+    x = s["x"].float()
+    g, u = x @ weights("gate").t(), x @ weights("up").t()
+    h = (_plain_act(c.get("act", "silu"), g)[0] * u).to(dt)
+    return {"h": h, "g": g.to(dt), "u": u.to(dt)} if c.get("save") else h
+
+
+# ---- what a pass cannot do without ----------------------------------------------
+def work(case):
+    kind, m, n, k = case["kind"], case["m"], case["n"], case["k"]
+    e = SIZE[case["dt"]]
+    if kind in ("w4", "w4_front"):
+        mats = 1 if kind == "w4" else 2
+        w = n * (-(-k // 2)) + n * -(-k // case["group"]) * 5 // 2  # codes; a 2-byte scale and half a byte of zero point
+        return {"bytes": mats * w + e * m * (k + n), "flops": 2 * mats * m * n * k}
+    w = 2 * n * (k // ELEMS[case["fmt"]]) * BYTES[case["fmt"]]
+    rows = 5 * n + k if kind == "bwd" else k + (3 if case.get("save") else 1) * n
+    return {"bytes": w + e * m * rows, "flops": 4 * m * n * k}
+
+
+# ---- the same in 64 bits ---------------------------------------------------------
+def _gather(b, byte, shift, mask):
+    """Code e of every block: bits `mask` of byte[e] >> shift[e]."""
+    return (b[:, byte.cuda()].long() >> shift.cuda()) & mask
+
+
+def _exact_rows(fmt, b, n, k, r0, r1):
+    """Rows r0 .. r1 of the weight matrix, from each element's place in its block."""
+    per = k // ELEMS[fmt]
+    b = b[r0 * per:r1 * per]
+    e = torch.arange(ELEMS[fmt])
+
+    def f16(col):
+        return (b[:, col].int() | (b[:, col + 1].int() << 8)).to(torch.int16).view(torch.float16).double()[:, None]
+
+    if fmt == "q4_0":
+        w = f16(0) * (_gather(b, 2 + e % 16, 4 * (e // 16), 15) - 8)
+    elif fmt == "q8_0":
+        v = b[:, 2:].long()
+        w = f16(0) * (v - 256 * (v >= 128))
+    elif fmt == "q4_k":
+        j = e // 32
+
+        def six(base):
+            low = _gather(b, base + j % 4, torch.where(j < 4, 0, 6), 255)
+            high = _gather(b, base + 4 + (j % 4) // 2, 4 * (j % 2), 15)
+            return torch.where((j < 4).cuda(), low & 63, (low & 3) | (high << 2))
+
+        w = f16(0) * six(4) * _gather(b, 16 + e // 2, 4 * (e % 2), 15) - f16(2) * six(10)
+    else:
+        code = _gather(b, e // 2, 4 * (e % 2), 15) + 16 * _gather(b, 128 + e // 4, 2 * (e % 4), 3)
+        sc = b[:, (192 + e // 16).cuda()].long()
+        w = f16(208) * (sc - 256 * (sc >= 128)) * (code - 32)
+    return w.reshape(r1 - r0, k)
+
+
+def _exact_w4_rows(w, k, group, r0, r1):
+    e = torch.arange(k, device="cuda")
+    q = (w["q"][r0:r1][:, e // 2].long() >> (4 * (e % 2))) & 15
+    return w["s"][r0:r1].double()[:, e // group] * (q - w["z"][r0:r1].long()[:, e // group])
+
+
+def _exact_act(act, g):
+    if act == "silu":
+        sg = torch.sigmoid(g)
+        return g * sg, sg + g * sg * torch.sigmoid(-g)
+    p = math.sqrt(2 / math.pi) * (g + 0.044715 * g ** 3)
+    dp = math.sqrt(2 / math.pi) * (1 + 3 * 0.044715 * g ** 2)
+    return g * torch.sigmoid(2 * p), torch.sigmoid(2 * p) + g * 2 * dp * torch.sigmoid(2 * p) * torch.sigmoid(-2 * p)
+
+
+def exact(case, seed):
+    s = _inputs(case, seed)
+    kind, n, k = case["kind"], case["n"], case["k"]
+    step = 2048
+
+    def rows(name, r0):
+        r1 = min(r0 + step, n)
+        if kind in ("w4", "w4_front"):
+            return _exact_w4_rows(s[name], k, case["group"], r0, r1)
+        return _exact_rows(case["fmt"], s[name], n, k, r0, r1)
+
+    def product(name):
+        return torch.cat([s["x"].double() @ rows(name, r0).t().contiguous() for r0 in range(0, n, step)], 1)
+
+    if kind == "w4":
+        return product("w")
+    if kind == "bwd":
+        dh = s["dh"].double()
+        a, da = _exact_act(case.get("act", "silu"), s["g"].double())
+        dg, du = dh * s["u"].double() * da, dh * a
+        dx = torch.zeros(case["m"], k, dtype=torch.float64, device="cuda")
+        for r0 in range(0, n, step):
+            dx += dg[:, r0:r0 + step].contiguous() @ rows("gate", r0) + du[:, r0:r0 + step].contiguous() @ rows("up", r0)
+        return {"dx": dx, "dg": dg, "du": du}
+    g, u = product("gate"), product("up")
+    h = _exact_act(case.get("act", "silu"), g)[0] * u
+    return {"h": h, "g": g, "u": u} if case.get("save") else h
