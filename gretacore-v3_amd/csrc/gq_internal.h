@@ -103,6 +103,10 @@ int gq_launch_matmul_q6k(int fmt, const void *packed, const float *a, float *c, 
                          hipStream_t s);
 // fp16-weight rows of gq_gemm_f16w through the tiled GEMM (gq_gemm.hip)
 int gq_launch_gemm_f16w(const void *w, const float *a, float *c, size_t M, size_t N, size_t K, hipStream_t s);
+// A [M][K] (any activation dtype) -> fp16 [M][ldo] scaled by a power of two per row,
+// rs[m] undoing it (gq_gemm.hip); q4perm: the 4-bit B fragments' order
+int gq_launch_a_to_f16(const void *a, int a_dtype, _Float16 *o, float *rs, int M, int K, int ldo, int q4perm,
+                       hipStream_t s);
 // c[i] = the sum over p of part[p][i], in part order (gq_gemm.hip)
 int gq_launch_split_sum(const float *part, float *c, size_t n, int parts, hipStream_t s);
 // Compute units of the current device (cached per device; 0 without a device).

@@ -254,6 +254,59 @@ int gq_launch_gemm_mixed_f16f32(void *stream, const float *a, const void *b, flo
 int gq_launch_gemm_mfma_mixed_f16f32(void *stream, const float *a, const void *b, float *c, uint32_t M, uint32_t N,
                                      uint32_t K, uint32_t lda, uint32_t ldb, uint32_t ldc);
 
+/* ---- gated feed-forward front, any number of rows -----------------------------
+ * h[m][n] = act(g[m][n]) * u[m][n] with g = x W_gate^T, u = x W_up^T: gq_gemv_swiglu's
+ * block without its normalisation, for prompts, batches and training.  x is
+ * [M][K] of x_dtype, h [M][N] of h_dtype, both contiguous; W_gate and W_up are T16
+ * tensors of one format.  d_g and d_u (NULL: not wanted) receive the two products,
+ * of h_dtype, as gq_ffn_gate_up_bwd takes them.  fp16 matrix cores, fp32 sums, as
+ * gq_gemm: x is rounded to fp16 after a power-of-two scale per row, each weight once
+ * to fp16, which for fp32 outputs leaves about 3e-4 of a row's norm.  Every output is
+ * rounded once from fp32. */
+#define GQ_ACT_SILU 0      /* g / (1 + e^-g) */
+#define GQ_ACT_GELU_TANH 1 /* g / 2 (1 + tanh(sqrt(2 / pi) (g + 0.044715 g^3))) */
+/* A workspace of NULL takes scratch memory of the call's own, which needs no room
+ * from the caller and does not race with other calls; there is none while the stream
+ * is being captured, where a call without a workspace returns GQ_ERR_WORKSPACE.
+ * Calls that overlap must not share a workspace.  Rows are taken in blocks, so the
+ * workspace stops growing with M. */
+size_t gq_ffn_gate_up_workspace_bytes(int fmt, size_t M, size_t N, size_t K);
+int gq_ffn_gate_up(int fmt, const void *d_gate, const void *d_up, const void *d_x, int x_dtype, void *d_h,
+                   int h_dtype, void *d_g, void *d_u, size_t M, size_t N, size_t K, int act, void *d_workspace,
+                   size_t workspace_bytes, void *stream);
+/* Its backward pass with the weights frozen:
+ *   dg = dh * u * act'(g), du = dh * act(g), dx = dg W_gate + du W_up.
+ * dh, g, u and dg, du are [M][N] of `dtype`, dx [M][K] of dx_dtype.  dg and du (the
+ * gradients of the projections, for adapters beside them) and dx may each be NULL:
+ * not wanted.  dx is computed from dg and du as they are before their rounding, which
+ * are brought to fp16 with a power-of-two scale per row.  dg may be the same buffer
+ * as g and du the same as u or dh; no other overlap. */
+size_t gq_ffn_gate_up_bwd_workspace_bytes(int fmt, size_t M, size_t N, size_t K);
+int gq_ffn_gate_up_bwd(int fmt, const void *d_gate, const void *d_up, const void *d_dh, const void *d_g,
+                       const void *d_u, int dtype, void *d_dg, void *d_du, void *d_dx, int dx_dtype, size_t M,
+                       size_t N, size_t K, int act, void *d_workspace, size_t workspace_bytes, void *stream);
+
+/* ---- 4-bit weights with group scales and zero points ---------------------------
+ * W[n][k] = s[n][k / group] * (q[n][k] - z[n][k / group]), the form of 4-bit checkpoints
+ * outside GGUF: q 0..15, two codes a byte (even k in the low nibble, a row is
+ * ceil(K / 2) bytes), s fp16 or bf16, z one byte each (0..31; NULL: 8), a row having
+ * ceil(K / group) of both.  group is 32, 64 or 128; any K and N.  gq_w4_pack lays the
+ * three out once, at load time, in gq_w4_packed_size bytes (16-byte aligned); the
+ * values stay as they are. */
+int gq_w4_packed_size(size_t N, size_t K, int group, size_t *bytes);
+int gq_w4_pack(const uint8_t *d_q, const void *d_scales, int scale_dtype, const uint8_t *d_zeros, size_t N, size_t K,
+               int group, void *d_packed, void *stream);
+/* y[b][n] = sum_k x[b][k] W[n][k], 1 <= batch <= 16, x [batch][K] and y [batch][N] of
+ * any activation dtype.  The codes and x enter the matrix cores as they are (fp32 x
+ * as three bf16 parts), sums and scales are fp32: the error is that of fp32
+ * sums, then one rounding to y_dtype.  A row of x with an Inf or NaN comes out
+ * non-finite; finite values must stay below 2^120.  No workspace. */
+int gq_w4_gemv(const void *d_packed, int group, const void *d_x, int x_dtype, void *d_y, int y_dtype, size_t N, size_t K,
+               int batch, void *stream);
+/* h[b][n] = act(g) * u, g = x W_gate^T, u = x W_up^T: the gated form, in one launch. */
+int gq_w4_gate_up(const void *d_gate, const void *d_up, int group, const void *d_x, int x_dtype, void *d_h, int h_dtype,
+                  size_t N, size_t K, int batch, int act, void *stream);
+
 #ifdef __cplusplus
 }
 #endif
