@@ -195,8 +195,9 @@ def _run_own(s):
         return gq.w4_gate_up(s["gate"], s["up"], c["group"], s["x"], n, k, act=act, out_dtype=s["x"].dtype)
     fmt = gq.FORMATS[c["fmt"]]
     if kind == "front":
-        return gq.ffn_gate_up(fmt, s["gate"], s["up"], s["x"], n, k, act=act, save=c.get("save", False),
-                              out_dtype=s["x"].dtype, workspace=s["ws"])
+        out = gq.ffn_gate_up(fmt, s["gate"], s["up"], s["x"], n, k, act=act, save=c.get("save", False),
+                             out_dtype=s["x"].dtype, workspace=s["ws"])
+        return dict(zip("hgu", out)) if c.get("save") else out
     return gq.ffn_gate_up_bwd(fmt, s["gate"], s["up"], s["dh"], s["g"], s["u"], n, k, act=act, workspace=s["ws"])
 
 
