@@ -10,6 +10,10 @@
 //         of two 16-bit floats, 8 steps of the last place each.
 //   meta  [tile][C][16 rows][128 / group] one word: the scale as fp32 bits (fp16 and
 //         bf16 leave its low 13 bits zero) with the zero point in the low 5.
+#include <stdlib.h>
+
+#include <type_traits>
+
 #include "gq_act.h"
 #include "gq_internal.h"
 
@@ -59,32 +63,288 @@ __global__ void __launch_bounds__(256) k_w4_pack(const uint8_t *__restrict__ q, 
 struct W4Mats {
   const uint8_t *w[2];
 };
-GQ_DEV uint32_t w4_code(uint32_t w, int e) { return (__builtin_rotateright32(w, 4 * (e >> 1) + 3 + 16 * (e & 1))) & 15u; }
 
-// One wave a row; lane l takes every 64th run of 8 k.
-template <int MATS>
-__global__ void __launch_bounds__(256) k_w4(W4Mats mats, size_t meta_off, const void *x, int xdt, void *y, int ydt, int N,
-                                            int K, int C, int group, int batch, int act) {
-  const int n = 4 * (int)blockIdx.x + (threadIdx.x >> 6), lane = threadIdx.x & 63;
-  if (n >= N) return;
-  for (int b = 0; b < batch; ++b) {
-    float s[MATS] = {};
-    for (int k = 8 * lane; k < K; k += 512) {
-      const size_t tc = (size_t)(n >> 4) * C + (k >> 7);
-      for (int m = 0; m < MATS; ++m) {
-        const uint32_t w = reinterpret_cast<const uint32_t *>(
-            mats.w[m])[tc * 256 + 4 * (16 * ((k >> 3) & 3) + (n & 15)) + ((k >> 5) & 3)];
-        const uint32_t v = reinterpret_cast<const uint32_t *>(
-            mats.w[m] + meta_off)[(tc * 16 + (n & 15)) * (kW4Chunk / group) + (k & 127) / group];
-        const float sc = __uint_as_float(v & ~31u), z = (float)(v & 31u);
-        for (int e = 0; e < 8 && k + e < K; ++e)
-          s[m] += gq_ld_dt(x, xdt, (size_t)b * K + k + e) * (sc * ((float)w4_code(w, e) - z));
+// ---- the product ---------------------------------------------------------------
+// v_mfma_f32_16x16x32 on one 32-block: the weights are the B operand (column = row n of
+// W, lane 16 g + r holds its codes 8 g .. + 7), x the A operand (row = batch row).  The codes
+// enter as they are, as the 16-bit floats 16 + q (bf16) or 128 + q (f16) that one AND-OR
+// makes of them; their sum is brought back with the sum of x (a product with ones, shared by
+// the tiles of a wave), and scale and zero point are applied once a group, in fp32:
+//   y += s (sum x (OFF + q) - (OFF + z) sum x)
+// so nothing is rounded but the fp32 sums.  fp32 x goes in as three bf16 parts of 8 bits.
+// Bound by the weights' bytes: a workgroup takes R row tiles (of both matrices) with KS waves
+// that share K chunk by chunk, PD chunks in flight each.
+typedef __bf16 w4_bf8 __attribute__((ext_vector_type(8)));
+struct __attribute__((packed, aligned(2))) W4Run16 {  // 8 values at any 2-byte address
+  gq_u4 v;
+};
+struct __attribute__((packed, aligned(4))) W4Run32 {
+  gq_u4 v[2];
+};
+
+template <int XT>
+constexpr int kW4Parts = XT == GQ_DT_F32 ? 3 : 1;
+template <int XT>
+constexpr float kW4Off = XT == GQ_DT_F16 ? 128.f : 16.f;
+template <int XT>
+constexpr uint32_t kW4Magic = XT == GQ_DT_F16 ? 0x58005800u : 0x41804180u;
+template <int XT>
+constexpr uint32_t kW4Ones = XT == GQ_DT_F16 ? 0x3C003C00u : 0x3F803F80u;
+
+template <int XT>
+GQ_DEV gq_f4 w4_mfma(const gq_u4 &a, const gq_u4 &b, const gq_f4 &c) {
+  if constexpr (XT == GQ_DT_F16)
+    return gq_mfma16(__builtin_bit_cast(gq_half8, a), __builtin_bit_cast(gq_half8, b), c);
+  else
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(w4_bf8, a), __builtin_bit_cast(w4_bf8, b), c, 0, 0,
+                                                   0);
+}
+GQ_DEV gq_u4 w4_codes(uint32_t w, uint32_t mg) {
+  constexpr uint32_t m = 0x00780078u;
+  return gq_u4{(w & m) | mg, ((w >> 4) & m) | mg, ((w >> 8) & m) | mg, (__builtin_rotateright32(w, 12) & m) | mg};
+}
+
+// 8 values of a row from k on, as loaded; TAIL: zeros from K on
+template <int XT>
+struct W4Raw {
+  gq_u4 v[XT == GQ_DT_F32 ? 2 : 1];
+};
+template <int XT, bool TAIL>
+GQ_DEV void w4_load_x(const void *x, size_t row, int k, int K, W4Raw<XT> &r) {
+  if constexpr (TAIL) {
+#pragma unroll
+    for (int i = 0; i < (XT == GQ_DT_F32 ? 2 : 1); ++i) r.v[i] = gq_u4{0, 0, 0, 0};
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (k + e < K) {
+        if constexpr (XT == GQ_DT_F32)
+          r.v[e >> 2][e & 3] = reinterpret_cast<const uint32_t *>(x)[row + k + e];
+        else
+          r.v[0][e >> 1] |= (uint32_t)reinterpret_cast<const uint16_t *>(x)[row + k + e] << (16 * (e & 1));
+      }
+  } else if constexpr (XT == GQ_DT_F32) {
+    const W4Run32 t = *reinterpret_cast<const W4Run32 *>(reinterpret_cast<const uint32_t *>(x) + row + k);
+    r.v[0] = t.v[0];
+    r.v[1] = t.v[1];
+  } else {
+    r.v[0] = reinterpret_cast<const W4Run16 *>(reinterpret_cast<const uint16_t *>(x) + row + k)->v;
+  }
+}
+// The A operand's parts, the smallest first (their sum is the value: 8 bits of it each, cut
+// off, not rounded; the differences are exact)
+template <int XT>
+GQ_DEV void w4_parts(const W4Raw<XT> &r, gq_u4 (&o)[kW4Parts<XT>]) {
+  if constexpr (XT != GQ_DT_F32) {
+    o[0] = r.v[0];
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      uint32_t p[3][2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int e = 2 * j + h;
+        float v = __uint_as_float(r.v[e >> 2][e & 3]);
+#pragma unroll
+        for (int i = 0; i < 3; ++i) {
+          p[i][h] = __float_as_uint(v);
+          v -= __uint_as_float(p[i][h] & 0xFFFF0000u);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 3; ++i) o[2 - i][j] = __builtin_amdgcn_perm(p[i][1], p[i][0], 0x07060302u);
+    }
+  }
+}
+
+// FEW: up to 4 rows.  Lane 16 g + 4 b + j then loads row j of block b, one load a chunk where the
+// operand's order takes four, and rotations by 4 b lanes bring each block to rows 0..3
+// of the operand (its other rows are not read).
+template <int XT, bool FEW, int B>
+GQ_DEV void w4_operand(const gq_u4 (&p)[FEW ? 1 : 4][kW4Parts<XT>], gq_u4 (&o)[kW4Parts<XT>]) {
+#pragma unroll
+  for (int i = 0; i < kW4Parts<XT>; ++i) {
+    if constexpr (!FEW) {
+      o[i] = p[B][i];
+    } else if constexpr (B == 0) {
+      o[i] = p[0][i];
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        o[i][j] = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)p[0][i][j], 0x120 + 16 - 4 * B, 0xF, 0xF, false);
+    }
+  }
+}
+
+template <int MATS, int XT, int GW, int R, int KS, bool FEW>
+__global__ void __launch_bounds__(64 * KS)
+k_w4(W4Mats mats, size_t meta_off, const void *__restrict__ x, void *__restrict__ y, int ydt, int N, int K, int C,
+     int batch, int act) {
+  constexpr int T = MATS * R, NP = kW4Parts<XT>, NX = FEW ? 1 : 4;
+  constexpr int PD = T == 1 ? 4 : T == 2 ? 3 : 2;
+  constexpr int BPG = 4 / GW;  // 32-blocks a group
+  __shared__ gq_f4 red[KS][T][64];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int g = lane >> 4, r = lane & 15;
+  const int tile0 = (int)blockIdx.x * R, ntiles = (N + 15) >> 4;
+  const uint8_t *wp[T], *mp[T];
+#pragma unroll
+  for (int t = 0; t < T; ++t) {
+    int tile = tile0 + t % R;
+    if (tile >= ntiles) tile = ntiles - 1;  // clamped; not stored
+    const size_t tc = (size_t)tile * C;
+    wp[t] = mats.w[t / R] + tc * kW4Codes + 16 * lane;
+    mp[t] = mats.w[t / R] + meta_off + (tc * 16 + r) * (4 * GW);
+  }
+  // the row (FEW: and block) of x this lane loads; rows past the batch: any
+  const int xr = FEW ? lane & 3 : r;
+  const size_t row = (size_t)(xr < batch ? xr : 0) * K;
+  const int xk = 8 * g + (FEW ? 32 * ((lane >> 2) & 3) : 0);
+
+  gq_u4 q[PD][T];
+  uint32_t meta[PD][T][GW];
+  W4Raw<XT> xs[PD][NX];
+  auto load = [&](int c, int st) __attribute__((always_inline)) {
+#pragma unroll
+    for (int t = 0; t < T; ++t) {
+      q[st][t] = gq_ld16_nt(wp[t] + (size_t)c * kW4Codes);
+      const uint8_t *m = mp[t] + (size_t)c * (64 * GW);
+      if constexpr (GW == 1) {
+        meta[st][t][0] = *reinterpret_cast<const uint32_t *>(m);
+      } else if constexpr (GW == 2) {
+        const gq_u2 v = gq_ld8(m);
+        meta[st][t][0] = v[0];
+        meta[st][t][1] = v[1];
+      } else {
+        const gq_u4 v = gq_ld16(m);
+#pragma unroll
+        for (int i = 0; i < GW; ++i) meta[st][t][i] = v[i];
       }
     }
-    for (int m = 0; m < MATS; ++m)
-      for (int o = 32; o > 0; o >>= 1) s[m] += __shfl_xor(s[m], o, 64);
-    if (lane == 0) gq_st_dt(y, ydt, (size_t)b * N + n, MATS == 2 ? gq_act_f(act, s[0]) * s[MATS - 1] : s[0]);
+  };
+  auto load_x = [&](int c, int st, auto tail) __attribute__((always_inline)) {
+#pragma unroll
+    for (int b = 0; b < NX; ++b)
+      w4_load_x<XT, decltype(tail)::value>(x, row, kW4Chunk * c + xk + 32 * b, K, xs[st][b]);
+  };
+
+  gq_f4 acc[T];
+#pragma unroll
+  for (int t = 0; t < T; ++t) acc[t] = gq_f4{0.f, 0.f, 0.f, 0.f};
+  uint32_t mg;
+  asm volatile("v_mov_b32 %0, %1" : "=v"(mg) : "i"(kW4Magic<XT>));  // (kept in a register)
+  const gq_u4 ones = {kW4Ones<XT>, kW4Ones<XT>, kW4Ones<XT>, kW4Ones<XT>};
+  auto compute = [&](int st) __attribute__((always_inline)) {
+    gq_u4 p[NX][NP];
+#pragma unroll
+    for (int b = 0; b < NX; ++b) w4_parts<XT>(xs[st][b], p[b]);
+    gq_f4 d[T], sx;
+    auto block = [&](auto bc) __attribute__((always_inline)) {
+      constexpr int B = decltype(bc)::value;
+      gq_u4 o[NP];
+      w4_operand<XT, FEW, B>(p, o);
+      if constexpr (B % BPG == 0) {
+        sx = gq_f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int t = 0; t < T; ++t) d[t] = sx;
+      }
+#pragma unroll
+      for (int i = 0; i < NP; ++i) sx = w4_mfma<XT>(o[i], ones, sx);
+#pragma unroll
+      for (int t = 0; t < T; ++t) {
+        const gq_u4 w = w4_codes(q[st][t][B], mg);
+#pragma unroll
+        for (int i = 0; i < NP; ++i) d[t] = w4_mfma<XT>(o[i], w, d[t]);
+      }
+      if constexpr (B % BPG == BPG - 1) {
+#pragma unroll
+        for (int t = 0; t < T; ++t) {
+          const uint32_t v = meta[st][t][B / BPG];
+          const float s = __uint_as_float(v & ~31u), z = kW4Off<XT> + (float)(v & 31u);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) acc[t][i] = fmaf(s, fmaf(-z, sx[i], d[t][i]), acc[t][i]);
+        }
+      }
+    };
+    block(std::integral_constant<int, 0>{});
+    block(std::integral_constant<int, 1>{});
+    block(std::integral_constant<int, 2>{});
+    block(std::integral_constant<int, 3>{});
+  };
+
+  // this wave's whole chunks: wave, wave + KS, ...; loads past the last one repeat it
+  const int full = K / kW4Chunk, n = full > wave ? (full - wave + KS - 1) / KS : 0;
+  if (n > 0) {
+#pragma unroll
+    for (int i = 0; i < PD; ++i) {
+      const int c = wave + KS * (i < n ? i : n - 1);
+      load(c, i);
+      load_x(c, i, std::false_type{});
+    }
+    for (int j = 0; j < n; j += PD) {
+#pragma unroll
+      for (int i = 0; i < PD; ++i) {
+        if (j + i >= n) break;
+        compute(i);
+        const int c = wave + KS * (j + i + PD < n ? j + i + PD : n - 1);
+        load(c, i);
+        load_x(c, i, std::false_type{});
+      }
+    }
   }
+  if (C > full && full % KS == wave) {  // a chunk that ends behind K
+    load(full, 0);
+    load_x(full, 0, std::true_type{});
+    compute(0);
+  }
+
+#pragma unroll
+  for (int t = 0; t < T; ++t) red[wave][t][lane] = acc[t];
+  __syncthreads();
+  // D layout (16x16): lane l holds column l % 16, rows 4 (l / 16) + i
+  for (int o = threadIdx.x; o < 16 * R * batch; o += 64 * KS) {
+    const int nl = o % (16 * R), m = o / (16 * R), at = 16 * (m >> 2) + (nl & 15);
+    float s[MATS] = {};
+#pragma unroll
+    for (int k = 0; k < MATS; ++k)
+#pragma unroll
+      for (int w = 0; w < KS; ++w) s[k] += reinterpret_cast<const float *>(&red[w][k * R + (nl >> 4)][at])[m & 3];
+    const int nn = 16 * tile0 + nl;
+    if (nn < N) gq_st_dt(y, ydt, (size_t)m * N + nn, MATS == 2 ? gq_act_f(act, s[0]) * s[MATS - 1] : s[0]);
+  }
+}
+
+template <int MATS, int XT, int GW, int R, int KS>
+int launch_w4_few(W4Mats mats, const void *x, void *y, int ydt, int N, int K, int batch, int act, hipStream_t s) {
+  const dim3 grid((unsigned)((gq_tiles(N) + R - 1) / R)), block(64 * KS);
+  const size_t mo = w4_meta_off(N, K);
+  const int C = (int)w4_chunks(K);
+  if (batch <= 4)
+    hipLaunchKernelGGL((k_w4<MATS, XT, GW, R, KS, true>), grid, block, 0, s, mats, mo, x, y, ydt, N, K, C, batch, act);
+  else
+    hipLaunchKernelGGL((k_w4<MATS, XT, GW, R, KS, false>), grid, block, 0, s, mats, mo, x, y, ydt, N, K, C, batch, act);
+  return gq_last_launch();
+}
+// Row tiles a workgroup: enough workgroups first
+template <int MATS, int XT, int GW>
+int launch_w4_shape(W4Mats mats, const void *x, void *y, int ydt, int N, int K, int batch, int act, hipStream_t s) {
+  const size_t tiles = gq_tiles(N);
+  static const int force = getenv("GQ_W4_R") ? atoi(getenv("GQ_W4_R")) : 0;
+  const int R = force ? force : tiles * MATS >= 4 * 448 ? 4 : tiles * MATS >= 2 * 448 ? 2 : 1;
+  if constexpr (MATS == 1) {
+    if (R >= 4) return launch_w4_few<1, XT, GW, 4, 8>(mats, x, y, ydt, N, K, batch, act, s);
+    if (R >= 2) return launch_w4_few<1, XT, GW, 2, 8>(mats, x, y, ydt, N, K, batch, act, s);
+    return launch_w4_few<1, XT, GW, 1, 16>(mats, x, y, ydt, N, K, batch, act, s);
+  } else {
+    if (R >= 4) return launch_w4_few<2, XT, GW, 2, 8>(mats, x, y, ydt, N, K, batch, act, s);
+    return launch_w4_few<2, XT, GW, 1, 16>(mats, x, y, ydt, N, K, batch, act, s);
+  }
+}
+template <int MATS, int XT>
+int launch_w4_group(W4Mats mats, int group, const void *x, void *y, int ydt, int N, int K, int batch, int act,
+                    hipStream_t s) {
+  if (group == 128) return launch_w4_shape<MATS, XT, 1>(mats, x, y, ydt, N, K, batch, act, s);
+  if (group == 64) return launch_w4_shape<MATS, XT, 2>(mats, x, y, ydt, N, K, batch, act, s);
+  return launch_w4_shape<MATS, XT, 4>(mats, x, y, ydt, N, K, batch, act, s);
 }
 
 int check_w4(int group, size_t N, size_t K) {
@@ -102,9 +362,10 @@ int launch_w4(W4Mats mats, int group, const void *x, int x_dtype, void *y, int y
   GQ_CHECK(mats.w[0] && mats.w[MATS - 1] && x && y, GQ_ERR_INVALID_ARGS);
   if (N == 0) return GQ_OK;
   GQ_CHECK(K > 0, GQ_ERR_INVALID_ARGS);
-  hipLaunchKernelGGL(k_w4<MATS>, dim3((unsigned)((N + 3) / 4)), dim3(256), 0, s, mats, w4_meta_off(N, K), x, x_dtype, y,
-                     y_dtype, (int)N, (int)K, (int)w4_chunks(K), group, batch, act);
-  return gq_last_launch();
+  const int n = (int)N, k = (int)K;
+  if (x_dtype == GQ_DT_F32) return launch_w4_group<MATS, GQ_DT_F32>(mats, group, x, y, y_dtype, n, k, batch, act, s);
+  if (x_dtype == GQ_DT_F16) return launch_w4_group<MATS, GQ_DT_F16>(mats, group, x, y, y_dtype, n, k, batch, act, s);
+  return launch_w4_group<MATS, GQ_DT_BF16>(mats, group, x, y, y_dtype, n, k, batch, act, s);
 }
 
 }  // namespace
