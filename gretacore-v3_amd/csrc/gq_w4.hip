@@ -10,8 +10,6 @@
 //         of two 16-bit floats, 8 steps of the last place each.
 //   meta  [tile][C][16 rows][128 / group] one word: the scale as fp32 bits (fp16 and
 //         bf16 leave its low 13 bits zero) with the zero point in the low 5.
-#include <stdlib.h>
-
 #include <type_traits>
 
 #include "gq_act.h"
@@ -111,17 +109,25 @@ struct W4Raw {
 };
 template <int XT, bool TAIL>
 GQ_DEV void w4_load_x(const void *x, size_t row, int k, int K, W4Raw<XT> &r) {
-  if constexpr (TAIL) {
+  if constexpr (TAIL) {  // (addresses clamped into the row, no branch around a load)
+    uint32_t t[8];
 #pragma unroll
-    for (int i = 0; i < (XT == GQ_DT_F32 ? 2 : 1); ++i) r.v[i] = gq_u4{0, 0, 0, 0};
+    for (int e = 0; e < 8; ++e) {
+      const size_t at = row + (k + e < K ? k + e : K - 1);
+      if constexpr (XT == GQ_DT_F32) t[e] = reinterpret_cast<const uint32_t *>(x)[at];
+      else t[e] = reinterpret_cast<const uint16_t *>(x)[at];
+    }
 #pragma unroll
-    for (int e = 0; e < 8; ++e)
-      if (k + e < K) {
-        if constexpr (XT == GQ_DT_F32)
-          r.v[e >> 2][e & 3] = reinterpret_cast<const uint32_t *>(x)[row + k + e];
-        else
-          r.v[0][e >> 1] |= (uint32_t)reinterpret_cast<const uint16_t *>(x)[row + k + e] << (16 * (e & 1));
+    for (int e = 0; e < 8; ++e) t[e] = k + e < K ? t[e] : 0u;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      if constexpr (XT == GQ_DT_F32) {
+        r.v[0][e] = t[e];
+        r.v[1][e] = t[4 + e];
+      } else {
+        r.v[0][e] = t[2 * e] | t[2 * e + 1] << 16;
       }
+    }
   } else if constexpr (XT == GQ_DT_F32) {
     const W4Run32 t = *reinterpret_cast<const W4Run32 *>(reinterpret_cast<const uint32_t *>(x) + row + k);
     r.v[0] = t.v[0];
@@ -156,44 +162,59 @@ GQ_DEV void w4_parts(const W4Raw<XT> &r, gq_u4 (&o)[kW4Parts<XT>]) {
   }
 }
 
-// FEW: up to 4 rows.  Lane 16 g + 4 b + j then loads row j of block b, one load a chunk where the
-// operand's order takes four, and rotations by 4 b lanes bring each block to rows 0..3
-// of the operand (its other rows are not read).
+// FEW: up to 4 rows, and the A operand has 16.  Lane 16 g + 4 b + j then loads row j of
+// block b, one load a chunk where the operand's order takes four, and rotations by whole
+// quads bring a block to rows 0..3 of the operand; fp32's other parts go to rows 4..7 and 8..11,
+// so that they take no product of their own (their sums are added at the end).
+template <int I, int B>
+GQ_DEV uint32_t w4_quad(uint32_t old, uint32_t src) {  // quad B of each 16 lanes to quad I, the others as in old
+  constexpr int n = 4 * ((I - B + 4) % 4);
+  return (uint32_t)__builtin_amdgcn_update_dpp((int)old, (int)src, n ? 0x120 + n : 0xE4, 0xF, 1 << I, false);
+}
+template <int XT, bool FEW>
+constexpr int kW4Ops = FEW ? 1 : kW4Parts<XT>;  // products of a block
 template <int XT, bool FEW, int B>
-GQ_DEV void w4_operand(const gq_u4 (&p)[FEW ? 1 : 4][kW4Parts<XT>], gq_u4 (&o)[kW4Parts<XT>]) {
+GQ_DEV void w4_operand(const gq_u4 (&p)[FEW ? 1 : 4][kW4Parts<XT>], gq_u4 (&o)[kW4Ops<XT, FEW>]) {
 #pragma unroll
-  for (int i = 0; i < kW4Parts<XT>; ++i) {
+  for (int i = 0; i < kW4Ops<XT, FEW>; ++i)
     if constexpr (!FEW) {
       o[i] = p[B][i];
-    } else if constexpr (B == 0) {
-      o[i] = p[0][i];
     } else {
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        o[i][j] = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)p[0][i][j], 0x120 + 16 - 4 * B, 0xF, 0xF, false);
+      for (int j = 0; j < 4; ++j) {
+        if constexpr (XT == GQ_DT_F32) {
+          o[0][j] = w4_quad<0, B>(0u, p[0][0][j]);
+          o[0][j] = w4_quad<1, B>(o[0][j], p[0][1][j]);
+          o[0][j] = w4_quad<2, B>(o[0][j], p[0][2][j]);
+        } else {
+          o[0][j] = B == 0 ? p[0][0][j] : w4_quad<0, B>(p[0][0][j], p[0][0][j]);
+        }
+      }
     }
-  }
 }
 
 template <int MATS, int XT, int GW, int R, int KS, bool FEW>
 __global__ void __launch_bounds__(64 * KS)
 k_w4(W4Mats mats, size_t meta_off, const void *__restrict__ x, void *__restrict__ y, int ydt, int N, int K, int C,
      int batch, int act) {
-  constexpr int T = MATS * R, NP = kW4Parts<XT>, NX = FEW ? 1 : 4;
-  constexpr int PD = T == 1 ? 4 : T == 2 ? 3 : 2;
+  constexpr int T = MATS * R, NP = kW4Parts<XT>, NO = kW4Ops<XT, FEW>, NX = FEW ? 1 : 4;
+  constexpr int PD = T == 1 ? (XT == GQ_DT_F32 && !FEW ? 2 : 4) : T == 2 ? 3 : 2;  // (as the registers allow)
   constexpr int BPG = 4 / GW;  // 32-blocks a group
   __shared__ gq_f4 red[KS][T][64];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int g = lane >> 4, r = lane & 15;
   const int tile0 = (int)blockIdx.x * R, ntiles = (N + 15) >> 4;
-  const uint8_t *wp[T], *mp[T];
+  // A tile's codes and meta words through buffer resources of their own, which end with
+  // the tile: a load of chunk C or beyond lies out of range and fetches nothing.
+  __amdgpu_buffer_rsrc_t wr[T], mr[T];
 #pragma unroll
   for (int t = 0; t < T; ++t) {
     int tile = tile0 + t % R;
     if (tile >= ntiles) tile = ntiles - 1;  // clamped; not stored
     const size_t tc = (size_t)tile * C;
-    wp[t] = mats.w[t / R] + tc * kW4Codes + 16 * lane;
-    mp[t] = mats.w[t / R] + meta_off + (tc * 16 + r) * (4 * GW);
+    uint8_t *w = const_cast<uint8_t *>(mats.w[t / R]);
+    wr[t] = __builtin_amdgcn_make_buffer_rsrc(w + tc * kW4Codes, (short)0, C * kW4Codes, 0x00020000);
+    mr[t] = __builtin_amdgcn_make_buffer_rsrc(w + meta_off + tc * (64 * GW), (short)0, C * (64 * GW), 0x00020000);
   }
   // the row (FEW: and block) of x this lane loads; rows past the batch: any
   const int xr = FEW ? lane & 3 : r;
@@ -204,20 +225,21 @@ k_w4(W4Mats mats, size_t meta_off, const void *__restrict__ x, void *__restrict_
   uint32_t meta[PD][T][GW];
   W4Raw<XT> xs[PD][NX];
   auto load = [&](int c, int st) __attribute__((always_inline)) {
+    const uint32_t wo = (uint32_t)c * kW4Codes + 16u * (uint32_t)lane, mo = (uint32_t)c * (64 * GW) + 4 * GW * (uint32_t)r;
 #pragma unroll
     for (int t = 0; t < T; ++t) {
-      q[st][t] = gq_ld16_nt(wp[t] + (size_t)c * kW4Codes);
-      const uint8_t *m = mp[t] + (size_t)c * (64 * GW);
+      const auto v = __builtin_amdgcn_raw_buffer_load_b128(wr[t], wo, 0, 2);  // (streamed: read once)
+      q[st][t] = gq_u4{v[0], v[1], v[2], v[3]};
       if constexpr (GW == 1) {
-        meta[st][t][0] = *reinterpret_cast<const uint32_t *>(m);
+        meta[st][t][0] = __builtin_amdgcn_raw_buffer_load_b32(mr[t], mo, 0, 0);
       } else if constexpr (GW == 2) {
-        const gq_u2 v = gq_ld8(m);
-        meta[st][t][0] = v[0];
-        meta[st][t][1] = v[1];
+        const auto m = __builtin_amdgcn_raw_buffer_load_b64(mr[t], mo, 0, 0);
+        meta[st][t][0] = m[0];
+        meta[st][t][1] = m[1];
       } else {
-        const gq_u4 v = gq_ld16(m);
+        const auto m = __builtin_amdgcn_raw_buffer_load_b128(mr[t], mo, 0, 0);
 #pragma unroll
-        for (int i = 0; i < GW; ++i) meta[st][t][i] = v[i];
+        for (int i = 0; i < GW; ++i) meta[st][t][i] = m[i];
       }
     }
   };
@@ -240,7 +262,7 @@ k_w4(W4Mats mats, size_t meta_off, const void *__restrict__ x, void *__restrict_
     gq_f4 d[T], sx;
     auto block = [&](auto bc) __attribute__((always_inline)) {
       constexpr int B = decltype(bc)::value;
-      gq_u4 o[NP];
+      gq_u4 o[NO];
       w4_operand<XT, FEW, B>(p, o);
       if constexpr (B % BPG == 0) {
         sx = gq_f4{0.f, 0.f, 0.f, 0.f};
@@ -248,12 +270,12 @@ k_w4(W4Mats mats, size_t meta_off, const void *__restrict__ x, void *__restrict_
         for (int t = 0; t < T; ++t) d[t] = sx;
       }
 #pragma unroll
-      for (int i = 0; i < NP; ++i) sx = w4_mfma<XT>(o[i], ones, sx);
+      for (int i = 0; i < NO; ++i) sx = w4_mfma<XT>(o[i], ones, sx);
 #pragma unroll
       for (int t = 0; t < T; ++t) {
         const gq_u4 w = w4_codes(q[st][t][B], mg);
 #pragma unroll
-        for (int i = 0; i < NP; ++i) d[t] = w4_mfma<XT>(o[i], w, d[t]);
+        for (int i = 0; i < NO; ++i) d[t] = w4_mfma<XT>(o[i], w, d[t]);
       }
       if constexpr (B % BPG == BPG - 1) {
 #pragma unroll
@@ -271,23 +293,22 @@ k_w4(W4Mats mats, size_t meta_off, const void *__restrict__ x, void *__restrict_
     block(std::integral_constant<int, 3>{});
   };
 
-  // this wave's whole chunks: wave, wave + KS, ...; loads past the last one repeat it
+  // this wave's whole chunks: wave, wave + KS, ...; past the last one nothing is fetched of
+  // the weights, and x of the last one again
   const int full = K / kW4Chunk, n = full > wave ? (full - wave + KS - 1) / KS : 0;
   if (n > 0) {
+    auto request = [&](int j, int st) __attribute__((always_inline)) {
+      load(j < n ? wave + KS * j : C, st);
+      load_x(wave + KS * (j < n ? j : n - 1), st, std::false_type{});
+    };
 #pragma unroll
-    for (int i = 0; i < PD; ++i) {
-      const int c = wave + KS * (i < n ? i : n - 1);
-      load(c, i);
-      load_x(c, i, std::false_type{});
-    }
+    for (int i = 0; i < PD; ++i) request(i, i);
     for (int j = 0; j < n; j += PD) {
 #pragma unroll
       for (int i = 0; i < PD; ++i) {
         if (j + i >= n) break;
         compute(i);
-        const int c = wave + KS * (j + i + PD < n ? j + i + PD : n - 1);
-        load(c, i);
-        load_x(c, i, std::false_type{});
+        request(j + i + PD, i);
       }
     }
   }
@@ -307,44 +328,55 @@ k_w4(W4Mats mats, size_t meta_off, const void *__restrict__ x, void *__restrict_
 #pragma unroll
     for (int k = 0; k < MATS; ++k)
 #pragma unroll
-      for (int w = 0; w < KS; ++w) s[k] += reinterpret_cast<const float *>(&red[w][k * R + (nl >> 4)][at])[m & 3];
+      for (int w = 0; w < KS; ++w)
+#pragma unroll
+        for (int i = 0; i < (FEW ? NP : 1); ++i)
+          s[k] += reinterpret_cast<const float *>(&red[w][k * R + (nl >> 4)][at + 16 * i])[m & 3];
     const int nn = 16 * tile0 + nl;
     if (nn < N) gq_st_dt(y, ydt, (size_t)m * N + nn, MATS == 2 ? gq_act_f(act, s[0]) * s[MATS - 1] : s[0]);
   }
 }
 
-template <int MATS, int XT, int GW, int R, int KS>
-int launch_w4_few(W4Mats mats, const void *x, void *y, int ydt, int N, int K, int batch, int act, hipStream_t s) {
-  const dim3 grid((unsigned)((gq_tiles(N) + R - 1) / R)), block(64 * KS);
-  const size_t mo = w4_meta_off(N, K);
+// Row tiles and waves of a workgroup.  More tiles share one reading of x and its
+// conversion, more waves per tile start more loads at once where tiles are few:
+//  * one tile while the tiles fit the CUs (8 waves; with more than 4 rows, whose x takes four
+//    times the loads, only for long K).  us, tiles 1 / 2 / 4: 4096 x 4096 one row 4.9 / 5.9 / 9.4,
+//    8 rows 7.9 / 7.9 / 10.0; 4096 x 14336 one row 9.6 / 13.0 / 26.6, 8 rows 15.5 / 17.2 / 25.8
+//  * two tiles, on 8 waves up to 1000 tiles (8192 x 4096 one row 6.5, on 4 waves 7.3; 20000 x 4096 13.1
+//    and 12.9); more than 4 rows on 4 waves but for long K (8192 x 4096 8 rows 8.2, on 8 waves 8.5;
+//    6000 x 14336 20.1 and 17.8)
+//  * four tiles on 4 waves from where two give more than a round of workgroups: 14336 x 4096
+//    8 rows 10.7, two tiles 12.1; 32000 x 4096 two rows of fp32 18.9 and 21.1
+template <int MATS, int XT, int GW, bool FEW>
+int launch_w4_shape(W4Mats mats, const void *x, void *y, int ydt, int N, int K, int batch, int act, hipStream_t s) {
+  const size_t tiles = gq_tiles(N), tt = tiles * MATS, mo = w4_meta_off(N, K);
   const int C = (int)w4_chunks(K);
-  if (batch <= 4)
-    hipLaunchKernelGGL((k_w4<MATS, XT, GW, R, KS, true>), grid, block, 0, s, mats, mo, x, y, ydt, N, K, C, batch, act);
-  else
-    hipLaunchKernelGGL((k_w4<MATS, XT, GW, R, KS, false>), grid, block, 0, s, mats, mo, x, y, ydt, N, K, C, batch, act);
+  const size_t two = !FEW ? 600 : XT == GQ_DT_F32 ? 800 : 1400;  // the most tiles that go by twos
+#define GQ_W4(R, KS)                                                                                               \
+  hipLaunchKernelGGL((k_w4<MATS, XT, GW, R, KS, FEW>), dim3((unsigned)((tiles + (R)-1) / (R))), dim3(64 * (KS)), 0, s, mats, \
+                     mo, x, y, ydt, N, K, C, batch, act)
+  if (MATS == 1 && tt <= 256 && (FEW || C >= 64)) {
+    if constexpr (MATS == 1) GQ_W4(1, 8);
+  } else if (tt <= two) {
+    if (FEW ? tt <= 1000 : C >= 64) GQ_W4(2 / MATS, 8);
+    else GQ_W4(2 / MATS, 4);
+  } else {
+    GQ_W4(4 / MATS, 4);
+  }
+#undef GQ_W4
   return gq_last_launch();
 }
-// Row tiles a workgroup: enough workgroups first
 template <int MATS, int XT, int GW>
-int launch_w4_shape(W4Mats mats, const void *x, void *y, int ydt, int N, int K, int batch, int act, hipStream_t s) {
-  const size_t tiles = gq_tiles(N);
-  static const int force = getenv("GQ_W4_R") ? atoi(getenv("GQ_W4_R")) : 0;
-  const int R = force ? force : tiles * MATS >= 4 * 448 ? 4 : tiles * MATS >= 2 * 448 ? 2 : 1;
-  if constexpr (MATS == 1) {
-    if (R >= 4) return launch_w4_few<1, XT, GW, 4, 8>(mats, x, y, ydt, N, K, batch, act, s);
-    if (R >= 2) return launch_w4_few<1, XT, GW, 2, 8>(mats, x, y, ydt, N, K, batch, act, s);
-    return launch_w4_few<1, XT, GW, 1, 16>(mats, x, y, ydt, N, K, batch, act, s);
-  } else {
-    if (R >= 4) return launch_w4_few<2, XT, GW, 2, 8>(mats, x, y, ydt, N, K, batch, act, s);
-    return launch_w4_few<2, XT, GW, 1, 16>(mats, x, y, ydt, N, K, batch, act, s);
-  }
+int launch_w4_rows(W4Mats mats, const void *x, void *y, int ydt, int N, int K, int batch, int act, hipStream_t s) {
+  return batch <= 4 ? launch_w4_shape<MATS, XT, GW, true>(mats, x, y, ydt, N, K, batch, act, s)
+                    : launch_w4_shape<MATS, XT, GW, false>(mats, x, y, ydt, N, K, batch, act, s);
 }
 template <int MATS, int XT>
 int launch_w4_group(W4Mats mats, int group, const void *x, void *y, int ydt, int N, int K, int batch, int act,
                     hipStream_t s) {
-  if (group == 128) return launch_w4_shape<MATS, XT, 1>(mats, x, y, ydt, N, K, batch, act, s);
-  if (group == 64) return launch_w4_shape<MATS, XT, 2>(mats, x, y, ydt, N, K, batch, act, s);
-  return launch_w4_shape<MATS, XT, 4>(mats, x, y, ydt, N, K, batch, act, s);
+  if (group == 128) return launch_w4_rows<MATS, XT, 1>(mats, x, y, ydt, N, K, batch, act, s);
+  if (group == 64) return launch_w4_rows<MATS, XT, 2>(mats, x, y, ydt, N, K, batch, act, s);
+  return launch_w4_rows<MATS, XT, 4>(mats, x, y, ydt, N, K, batch, act, s);
 }
 
 int check_w4(int group, size_t N, size_t K) {
