@@ -7,12 +7,7 @@ static inline bool gq_dtype_valid(int dt) { return dt == GQ_DT_F32 || dt == GQ_D
 static inline bool gq_act_valid(int act) { return act == GQ_ACT_SILU || act == GQ_ACT_GELU_TANH; }
 static inline size_t gq_dtype_size(int dt) { return dt == GQ_DT_F32 ? 4 : 2; }
 
-GQ_DEV uint16_t gq_f32_to_bf16(float f) {
-  uint32_t u = __float_as_uint(f);
-  if ((u & 0x7F800000u) == 0x7F800000u) return (uint16_t)((u >> 16) | ((u & 0xFFFFu) ? 0x40u : 0u));
-  u += 0x7FFFu + ((u >> 16) & 1u);
-  return (uint16_t)(u >> 16);
-}
+GQ_DEV uint16_t gq_f32_to_bf16(float f) { return __builtin_bit_cast(uint16_t, (__bf16)f); }  // (to nearest even)
 GQ_DEV float gq_ld_dt(const void *p, int dt, size_t i) {
   if (dt == GQ_DT_F32) return reinterpret_cast<const float *>(p)[i];
   if (dt == GQ_DT_F16) return (float)reinterpret_cast<const _Float16 *>(p)[i];

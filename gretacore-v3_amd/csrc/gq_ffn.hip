@@ -1,7 +1,12 @@
 // gq_ffn.hip -- the gated feed-forward front h = act(x W_gate^T) * (x W_up^T) over T16
 // weights for any number of rows, and its backward pass.
+#include <stdlib.h>
+
+#include <type_traits>
+
 #include "gq_act.h"
 #include "gq_gemm_frag.h"
+#include "gq_gemv_frag.h"
 #include "gq_internal.h"
 
 namespace {
@@ -34,37 +39,628 @@ GQ_DEV float t16_weight(int fmt, const uint8_t *w, size_t sc_off, size_t n, size
   return gq_h2f(mv[0]) * (float)a * (float)q - gq_h2f(mv[0] >> 16) * (float)m;
 }
 
-// 16 x 16 outputs a workgroup, K in steps of 32 through LDS, fp32 throughout
-__global__ void __launch_bounds__(256) k_front(int fmt, const uint8_t *gate, const uint8_t *up, size_t sc_off,
-                                               const void *x, int xdt, void *h, int hdt, void *go, void *uo, int M,
-                                               int N, int K, int C, int act) {
-  __shared__ float xs[16][33], ws[2][16][33];
-  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-  const int n0 = 16 * blockIdx.x;
-  for (int m0 = 16 * (int)blockIdx.y; m0 < M; m0 += 16 * (int)gridDim.y) {
-    float g = 0.f, u = 0.f;
-    for (int k0 = 0; k0 < K; k0 += 32) {
+// ---- forward: up to 32 rows, units of 128 k ------------------------------------------
+// The weights' bytes bound these.  A workgroup takes R row tiles of both matrices, its KS waves
+// share K unit by unit (wave, wave + KS, ...) with PD units in flight each, and their sums are
+// added through LDS.  A unit is 128 k of a row tile: a chunk of Q4_0 / Q8_0, half a super-block of the
+// k-quants; it is loaded through buffer resources that end with the tile, so a unit past the
+// last one fetches nothing and needs no branch.
+template <int FMT>
+struct FUnit {
+  gq_u4 q[FMT == GQ_FMT_Q8_0 ? 2 : 1];  // codes of the two 64-k steps (lane 16 g + r: row r, k 16 g .. + 15)
+  gq_u4 s;  // Q4_0 / Q8_0: d0 d2 | d1 d3; Q4_K: meta; Q6_K: high fields of the steps | their scales
+  uint32_t d;  // Q6_K: d
+};
+template <int FMT>
+constexpr bool kSuper = FMT == GQ_FMT_Q4_K || FMT == GQ_FMT_Q6_K;
+
+template <int FMT>
+struct FTile {
+  __amdgpu_buffer_rsrc_t q, s;
+};
+template <int FMT>
+GQ_DEV FTile<FMT> ftile(const uint8_t *w, size_t sc_off, size_t tile, int C) {
+  using F = HFmt<FMT>;
+  uint8_t *p = const_cast<uint8_t *>(w);
+  return FTile<FMT>{
+      __builtin_amdgcn_make_buffer_rsrc(p + tile * (size_t)C * F::QB, (short)0, C * F::QB, 0x00020000),
+      __builtin_amdgcn_make_buffer_rsrc(p + sc_off + tile * (size_t)C * F::SB, (short)0, C * F::SB, 0x00020000)};
+}
+GQ_DEV gq_u4 ld16_r(const __amdgpu_buffer_rsrc_t &r, uint32_t o) {  // (streamed: read once)
+  const auto v = __builtin_amdgcn_raw_buffer_load_b128(r, o, 0, 2);
+  return gq_u4{v[0], v[1], v[2], v[3]};
+}
+template <int FMT>
+GQ_DEV void load_unit(const FTile<FMT> &t, int unit, int lane, FUnit<FMT> &u) {
+  using F = HFmt<FMT>;
+  const uint32_t c = (uint32_t)(kSuper<FMT> ? unit >> 1 : unit), p = kSuper<FMT> ? (uint32_t)unit & 1u : 0u;
+  const uint32_t qo = c * F::QB + 1024u * p + 16u * (uint32_t)lane, so = c * F::SB, r = (uint32_t)lane & 15u;
+  u.q[0] = ld16_r(t.q, qo);
+  if constexpr (FMT == GQ_FMT_Q8_0) u.q[1] = ld16_r(t.q, qo + 1024u);
+  if constexpr (FMT == GQ_FMT_Q4_K) {
+    const auto v = __builtin_amdgcn_raw_buffer_load_b128(t.s, so + 16u * r, 0, 0);
+    u.s = gq_u4{v[0], v[1], v[2], v[3]};
+  } else if constexpr (FMT == GQ_FMT_Q6_K) {
+    const auto h = __builtin_amdgcn_raw_buffer_load_b64(t.q, c * F::QB + 2048u + 16u * (uint32_t)lane + 8u * p, 0, 0);
+    const auto v = __builtin_amdgcn_raw_buffer_load_b64(t.s, so + 16u * r + 8u * p, 0, 0);
+    u.s = gq_u4{h[0], h[1], v[0], v[1]};
+    u.d = __builtin_amdgcn_raw_buffer_load_b16(t.s, so + 256u + 2u * r, 0, 0);
+  } else {
+    const auto v = __builtin_amdgcn_raw_buffer_load_b64(t.s, so + 8u * r, 0, 0);
+    u.s[0] = v[0];
+    u.s[1] = v[1];
+  }
+}
+// Q4_K: scale and min codes of sub-blocks i of the unit's two steps, a byte each (p: the unit's half)
+GQ_DEV void unit_codes_q4k(const FUnit<GQ_FMT_Q4_K> &u, uint32_t p, bool i, uint32_t &sc, uint32_t &mn) {
+  const uint32_t w = (i ? u.s[2] : u.s[1]) >> (16u * p), m = u.s[3] >> (16u * p + (i ? 4u : 0u));
+  sc = w & 0x3F3Fu;
+  mn = ((w >> 6) & 0x0303u) | ((m & 0x0F0Fu) << 2);
+}
+// Q6_K: the 8 codes 8 j .. + 7 of step m as bytes (byte b of the high fields' word holds slot 4 q + b at
+// bits 2 q)
+GQ_DEV void unit_codes_q6k(const FUnit<GQ_FMT_Q6_K> &u, int m, int j, uint32_t (&o)[2]) {
+  const uint32_t w = u.q[0][2 * m + j], h = u.s[m];
+  o[0] = (w & 0x0F0F0F0Fu) | ((j ? h : h << 4) & 0x30303030u);
+  o[1] = ((w >> 4) & 0x0F0F0F0Fu) | ((j ? h >> 2 : h << 2) & 0x30303030u);
+}
+// 8 values in the nibbles' order 0 2 4 6 1 3 5 7
+GQ_DEV gq_u4 nib_order(const gq_u4 &v) {
+  return gq_u4{__builtin_amdgcn_perm(v[1], v[0], 0x05040100u), __builtin_amdgcn_perm(v[3], v[2], 0x05040100u),
+               __builtin_amdgcn_perm(v[1], v[0], 0x07060302u), __builtin_amdgcn_perm(v[3], v[2], 0x07060302u)};
+}
+
+// Sums of the waves, h and where they are kept g and u.  at(k, w, t, n, m): wave k's part of output
+// (m, 16 t + n) of matrix w; rs: row scales of x
+template <int KS, int R, typename At>
+GQ_DEV void front_out(At at, const float *rs, void *h, void *go, void *uo, int dt, int M, int N, int act) {
+  for (int o = threadIdx.x; o < 16 * R * M; o += 64 * KS) {
+    const int nl = o % (16 * R), m = o / (16 * R), n = 16 * R * (int)blockIdx.x + nl;
+    float y[2] = {0.f, 0.f};
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int r = ty, k = k0 + tx + 16 * i;
-        xs[r][tx + 16 * i] = m0 + r < M ? gq_ld_dt(x, xdt, (size_t)(m0 + r) * K + k) : 0.f;
-        ws[0][r][tx + 16 * i] = n0 + r < N ? t16_weight(fmt, gate, sc_off, n0 + r, k, C) : 0.f;
-        ws[1][r][tx + 16 * i] = n0 + r < N ? t16_weight(fmt, up, sc_off, n0 + r, k, C) : 0.f;
-      }
-      __syncthreads();
-      for (int k = 0; k < 32; ++k) {
-        g += xs[ty][k] * ws[0][tx][k];
-        u += xs[ty][k] * ws[1][tx][k];
-      }
-      __syncthreads();
-    }
-    if (m0 + ty < M && n0 + tx < N) {
-      const size_t i = (size_t)(m0 + ty) * N + n0 + tx;
-      gq_st_dt(h, hdt, i, gq_act_f(act, g) * u);
-      if (go) gq_st_dt(go, hdt, i, g);
-      if (uo) gq_st_dt(uo, hdt, i, u);
+    for (int w = 0; w < 2; ++w)
+#pragma unroll
+      for (int k = 0; k < KS; ++k) y[w] += at(k, w, nl >> 4, nl & 15, m);
+    if (n < N) {
+      const float f = rs ? rs[m] : 1.f, g = y[0] * f, u = y[1] * f;
+      const size_t i = (size_t)m * N + n;
+      gq_st_dt(h, dt, i, gq_act_f(act, g) * u);
+      if (go) gq_st_dt(go, dt, i, g);
+      if (uo) gq_st_dt(uo, dt, i, u);
     }
   }
+}
+// The units of a wave: request(unit, stage) and compute(unit, stage), PD stages
+template <int PD, int KS, typename Request, typename Compute>
+GQ_DEV void walk_units(int units, int wave, Request request, Compute compute) {
+  const int n = units > wave ? (units - wave + KS - 1) / KS : 0;
+  if (n == 0) return;
+  auto req = [&](int j, int st) __attribute__((always_inline)) { request(j < n ? wave + KS * j : units, st); };
+#pragma unroll
+  for (int i = 0; i < PD; ++i) req(i, i);
+  for (int j = 0; j < n; j += PD) {
+#pragma unroll
+    for (int i = 0; i < PD; ++i) {
+      if (j + i >= n) break;
+      compute(wave + KS * (j + i), i);
+      req(j + i + PD, i);
+    }
+  }
+}
+
+// Up to 4 rows: nothing comes before the weights.  x enters the matrix cores as it is (bf16 or
+// f16, no conversion launch), and so do the codes, as the 16-bit floats OFF + q; scales and
+// minima are applied in fp32 to the sums of each scale group,
+//   y += s (sum x (OFF + q) - OFF sum x) - min sum x,  sum x from a product with ones.
+// A product of v_mfma_f32_16x16x32 spans NG scale groups (lane groups g / (4 / NG)).  The rows of the
+// A operand keep them apart: row 4 i + j holds row j of x masked to group i, and lane group i
+// of the result the sums of group i.  One load of x a unit: lane 16 g + 4 b + j takes row j, step b / 2, half
+// b % 2 of its 16 k, and moves of whole quads bring a step's half to the operand's rows (four loads
+// a unit in the operand's order: 19.4 us against 13.9 without any, 14336 x 4096 Q4_K).  MR: 1 or 4
+// rows, the components of the result that are scaled and added.
+template <int FMT>
+constexpr int kFewGroups = FMT == GQ_FMT_Q6_K ? 4 : 2;
+template <int FMT, int XT>
+constexpr float kFewOff = (FMT == GQ_FMT_Q8_0 && XT == GQ_DT_BF16 ? 0.f
+                           : XT == GQ_DT_BF16                     ? 128.f
+                                                                  : 1024.f) +
+                          (FMT == GQ_FMT_Q4_0                          ? 8.f
+                           : FMT == GQ_FMT_Q6_K                        ? 32.f
+                           : FMT == GQ_FMT_Q8_0 && XT == GQ_DT_F16 ? 128.f
+                                                                       : 0.f);
+
+typedef __bf16 few_bf8 __attribute__((ext_vector_type(8)));
+template <int XT>
+GQ_DEV gq_f4 few_mfma(const gq_u4 &a, const gq_u4 &b, const gq_f4 &c) {
+  if constexpr (XT == GQ_DT_F16) return gq_mfma16(__builtin_bit_cast(gq_half8, a), __builtin_bit_cast(gq_half8, b), c);
+  else
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(few_bf8, a), __builtin_bit_cast(few_bf8, b), c, 0, 0,
+                                                   0);
+}
+// The lane's 16 codes of step m as B operands of slots 0..7 and 8..15, the 4-bit formats in the
+// nibbles' order
+template <int FMT, int XT>
+GQ_DEV void few_codes(const FUnit<FMT> &u, int m, uint32_t mg, gq_u4 (&o)[2]) {
+  if constexpr (FMT == GQ_FMT_Q8_0 && XT == GQ_DT_BF16) {  // whole numbers of 8 bits
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t q = u.q[m][i];
+      uint32_t f[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) f[e] = __float_as_uint((float)(int8_t)(q >> (8 * e)));
+      o[i >> 1][2 * (i & 1)] = __builtin_amdgcn_perm(f[1], f[0], 0x07060302u);
+      o[i >> 1][2 * (i & 1) + 1] = __builtin_amdgcn_perm(f[3], f[2], 0x07060302u);
+    }
+  } else if constexpr (FMT == GQ_FMT_Q8_0 || FMT == GQ_FMT_Q6_K) {  // bytes: Q8_0 1024 + 128 + q
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      uint32_t c[2];
+      if constexpr (FMT == GQ_FMT_Q6_K) {
+        unit_codes_q6k(u, m, j, c);
+      } else {
+        c[0] = u.q[m][2 * j] ^ 0x80808080u;
+        c[1] = u.q[m][2 * j + 1] ^ 0x80808080u;
+      }
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        o[j][2 * i] = __builtin_amdgcn_perm(mg, c[i], 0x05010500u);
+        o[j][2 * i + 1] = __builtin_amdgcn_perm(mg, c[i], 0x05030502u);
+      }
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) o[j][i] = ((u.q[0][2 * m + j] >> (4 * i)) & 0x000F000Fu) | mg;
+  }
+}
+// Scale and minimum (Q4_K) of the lane's row for scale group i of the two steps
+template <int FMT>
+GQ_DEV void few_scales(const FUnit<FMT> &u, int unit, int i, float (&s)[2], float (&mn)[2]) {
+  if constexpr (FMT == GQ_FMT_Q4_K) {
+    uint32_t sc, mc;
+    unit_codes_q4k(u, (uint32_t)unit & 1u, i, sc, mc);
+    const float d = (float)bits_h(u.s[0]), dm = (float)bits_h(u.s[0] >> 16);
+    s[0] = d * (float)(sc & 255u);
+    s[1] = d * (float)(sc >> 8);
+    mn[0] = dm * (float)(mc & 255u);
+    mn[1] = dm * (float)(mc >> 8);
+  } else {
+#pragma unroll
+    for (int m = 0; m < 2; ++m) {
+      mn[m] = 0.f;
+      if constexpr (FMT == GQ_FMT_Q6_K) s[m] = (float)bits_h(u.d) * (float)(int8_t)(u.s[2 + m] >> (8 * i));
+      else s[m] = (float)bits_h((i ? u.s[1] : u.s[0]) >> (16 * m));
+    }
+  }
+}
+// Rows 4 I + j of the operand: quad Q of x in the lane groups of scale group I, the others as in old
+template <int NG, int I, int Q>
+GQ_DEV uint32_t few_quad(uint32_t old, uint32_t src) {
+  constexpr int n = 4 * ((I - Q + 4) % 4), rows = NG == 4 ? 1 << I : 3 << (2 * I);
+  return (uint32_t)__builtin_amdgcn_update_dpp((int)old, (int)src, n ? 0x120 + n : 0xE4, rows, 1 << I, false);
+}
+template <int NG, int Q>
+GQ_DEV gq_u4 few_operand(const gq_u4 &x) {
+  gq_u4 o;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    uint32_t v = few_quad<NG, 1, Q>(few_quad<NG, 0, Q>(0u, x[e]), x[e]);
+    if constexpr (NG == 4) v = few_quad<NG, 3, Q>(few_quad<NG, 2, Q>(v, x[e]), x[e]);
+    o[e] = v;
+  }
+  return o;
+}
+
+template <int FMT, int XT, int MR, int R, int KS>
+__global__ void __launch_bounds__(64 * KS)
+k_front_few(const uint8_t *__restrict__ wg, const uint8_t *__restrict__ wu, size_t sc_off, const void *__restrict__ x,
+            const float *__restrict__ rs, void *__restrict__ h, void *__restrict__ go, void *__restrict__ uo, int dt, int M,
+            int N, int K, int C, int units, int act) {
+  constexpr int NG = kFewGroups<FMT>, T = 2 * R, PD = R == 1 ? 3 : 2;
+  constexpr float OFF = kFewOff<FMT, XT>;
+  __shared__ float red[KS][T][MR][64];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int g = lane >> 4, ntiles = (int)gq_tiles(N);
+  FTile<FMT> tl[T];
+#pragma unroll
+  for (int t = 0; t < T; ++t) {
+    const int tile = (int)blockIdx.x * R + t % R;
+    tl[t] = ftile<FMT>(t < R ? wg : wu, sc_off, (size_t)(tile < ntiles ? tile : ntiles - 1), C);  // (clamped: not stored)
+  }
+  const __amdgpu_buffer_rsrc_t xr =
+      __builtin_amdgcn_make_buffer_rsrc(const_cast<void *>(x), (short)0, (int)(2u * (uint32_t)M * (uint32_t)K), 0x00020000);
+  const int xrow = lane & 3, xk = 64 * ((lane >> 3) & 1) + 16 * g + 8 * ((lane >> 2) & 1);
+  FUnit<FMT> us[PD][T];
+  gq_u4 xs[PD];
+  auto request = [&](int unit, int st) __attribute__((always_inline)) {
+#pragma unroll
+    for (int t = 0; t < T; ++t) load_unit<FMT>(tl[t], unit, lane, us[st][t]);
+    const uint32_t k = 128u * (uint32_t)unit + (uint32_t)xk;  // (K is whole 32-blocks: a run is wholly in or out)
+    const bool in = xrow < M && k < (uint32_t)K;
+    const auto v = __builtin_amdgcn_raw_buffer_load_b128(xr, in ? 2u * ((uint32_t)xrow * (uint32_t)K + k) : 0xFFFFFFF0u, 0, 0);
+    xs[st] = gq_u4{v[0], v[1], v[2], v[3]};
+  };
+  float acc[T][MR] = {};
+  uint32_t mg;  // (kept in a register)
+  if constexpr (XT == GQ_DT_F16) asm volatile("v_mov_b32 %0, 0x64006400" : "=v"(mg));
+  else asm volatile("v_mov_b32 %0, 0x43004300" : "=v"(mg));
+  constexpr uint32_t one = XT == GQ_DT_F16 ? 0x3C003C00u : 0x3F803F80u;
+  const gq_u4 ones = {one, one, one, one};
+  const gq_f4 zero = {0.f, 0.f, 0.f, 0.f};
+  auto compute = [&](int unit, int st) __attribute__((always_inline)) {
+    const gq_u4 xv = kNibOrder<FMT> ? nib_order(xs[st]) : xs[st];
+    float s[T][2], mn[T][2];
+#pragma unroll
+    for (int t = 0; t < T; ++t) few_scales<FMT>(us[st][t], unit, g & (NG - 1), s[t], mn[t]);
+    auto step = [&](auto mc) __attribute__((always_inline)) {
+      constexpr int m = decltype(mc)::value;
+      const gq_u4 a0 = few_operand<NG, 2 * m>(xv), a1 = few_operand<NG, 2 * m + 1>(xv);
+      gq_f4 sx = zero;
+      if constexpr (OFF != 0.f || FMT == GQ_FMT_Q4_K) sx = few_mfma<XT>(a1, ones, few_mfma<XT>(a0, ones, zero));
+#pragma unroll
+      for (int t = 0; t < T; ++t) {
+        gq_u4 b[2];
+        few_codes<FMT, XT>(us[st][t], m, mg, b);
+        const gq_f4 d = few_mfma<XT>(a1, b[1], few_mfma<XT>(a0, b[0], zero));
+        const float o = FMT == GQ_FMT_Q4_K ? fmaf(s[t][m], OFF, mn[t][m]) : 0.f;
+#pragma unroll
+        for (int v = 0; v < MR; ++v) {
+          if constexpr (FMT == GQ_FMT_Q4_K) acc[t][v] = fmaf(s[t][m], d[v], fmaf(-o, sx[v], acc[t][v]));
+          else acc[t][v] = fmaf(s[t][m], OFF != 0.f ? fmaf(-OFF, sx[v], d[v]) : d[v], acc[t][v]);
+        }
+      }
+    };
+    step(std::integral_constant<int, 0>{});
+    step(std::integral_constant<int, 1>{});
+  };
+  walk_units<PD, KS>(units, wave, request, compute);
+#pragma unroll
+  for (int t = 0; t < T; ++t)
+#pragma unroll
+    for (int v = 0; v < MR; ++v) red[wave][t][v][lane] = acc[t][v];
+  __syncthreads();
+  front_out<KS, R>(
+      [&](int k, int w, int t, int n, int m) {
+        float y = 0.f;
+#pragma unroll
+        for (int i = 0; i < NG; ++i) y += red[k][w * R + t][MR == 1 ? 0 : m][16 * i + n];
+        return y;
+      },
+      rs, h, go, uo, dt, M, N, act);
+}
+
+// More rows: the sums of the scale groups would cost more than folding the scale into the
+// weights, 13 to 24 operations for 8 weights with one rounding to fp16; the matrix cores then
+// add over all of K.  x comes as fp16 with a power-of-two scale per row (gq_launch_a_to_f16, for the
+// 4-bit formats in their nibbles' order), MT tiles of 16 rows.
+template <int FMT>
+GQ_DEV void rows_frags(const FUnit<FMT> &u, int unit, int g, uint32_t mg, gq_half8 (&o)[2][2]) {
+  uint32_t sc = 0, mc = 0;
+  if constexpr (FMT == GQ_FMT_Q4_K) unit_codes_q4k(u, (uint32_t)unit & 1u, g >> 1, sc, mc);
+#pragma unroll
+  for (int m = 0; m < 2; ++m) {
+    gq_half2 d2, a1, b1, m1, m16;  // Q4_K: (1024 + q) a1 + b1 = sc q, exact; then one rounding of d sc q - dmin m
+    if constexpr (FMT == GQ_FMT_Q4_K) {
+      const _Float16 d = bits_h(u.s[0]), ndm = -bits_h(u.s[0] >> 16);
+      const _Float16 s = (_Float16)(float)((sc >> (8 * m)) & 255u), c = (_Float16)(float)((mc >> (8 * m)) & 255u);
+      const _Float16 ns = s * (_Float16)-1024.0f, hm = c * ndm, hm16 = hm * (_Float16)16.0f;
+      d2 = gq_half2{d, d};
+      a1 = gq_half2{s, s};
+      b1 = gq_half2{ns, ns};
+      m1 = gq_half2{hm, hm};
+      m16 = gq_half2{hm16, hm16};
+    } else if constexpr (FMT == GQ_FMT_Q6_K) {
+      const _Float16 s = (_Float16)((float)bits_h(u.d) * (float)(int8_t)(u.s[2 + m] >> (8 * g)));
+      d2 = gq_half2{s, s};
+    } else {
+      d2 = splat_h((g >> 1 ? u.s[1] : u.s[0]) >> (16 * m));
+    }
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      gq_half2 p[4];
+      if constexpr (FMT == GQ_FMT_Q8_0) {
+        magic4(u.q[m][2 * j] ^ 0x80808080u, p[0], p[1]);
+        magic4(u.q[m][2 * j + 1] ^ 0x80808080u, p[2], p[3]);
+      } else if constexpr (FMT == GQ_FMT_Q6_K) {
+        uint32_t c[2];
+        unit_codes_q6k(u, m, j, c);
+        magic4(c[0], p[0], p[1]);
+        magic4(c[1], p[2], p[3]);
+      } else {
+        gq_nib_halves(u.q[0][2 * m + j], mg, p);
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if constexpr (FMT == GQ_FMT_Q4_K) {
+          p[i] = __builtin_elementwise_fma(__builtin_elementwise_fma(p[i], a1, b1), d2, i & 1 ? m16 : m1);
+        } else {
+          const float off = FMT == GQ_FMT_Q8_0 ? -1152.f : FMT == GQ_FMT_Q6_K ? -1056.f : i & 1 ? -1152.f : -1032.f;
+          p[i] = (p[i] + gq_half2{(_Float16)off, (_Float16)off}) * d2;  // (the sum is exact)
+        }
+        o[m][j][2 * i] = p[i][0];
+        o[m][j][2 * i + 1] = p[i][1];
+      }
+    }
+  }
+}
+
+template <int FMT, int MT, int R, int KS>
+__global__ void __launch_bounds__(64 * KS)
+k_front_rows(const uint8_t *__restrict__ wg, const uint8_t *__restrict__ wu, size_t sc_off,
+             const _Float16 *__restrict__ a16, int lda, const float *__restrict__ rs, void *__restrict__ h,
+             void *__restrict__ go, void *__restrict__ uo, int dt, int M, int N, int C, int units, int act) {
+  constexpr int T = 2 * R, PD = R == 1 ? 3 : 2;
+  __shared__ gq_f4 red[KS][T][MT][64];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int g = lane >> 4, r = lane & 15, ntiles = (int)gq_tiles(N);
+  FTile<FMT> tl[T];
+#pragma unroll
+  for (int t = 0; t < T; ++t) {
+    const int tile = (int)blockIdx.x * R + t % R;
+    tl[t] = ftile<FMT>(t < R ? wg : wu, sc_off, (size_t)(tile < ntiles ? tile : ntiles - 1), C);  // (clamped: not stored)
+  }
+  const __amdgpu_buffer_rsrc_t xr = __builtin_amdgcn_make_buffer_rsrc(
+      const_cast<_Float16 *>(a16), (short)0, (int)(2u * (uint32_t)M * (uint32_t)lda), 0x00020000);
+  uint32_t xo[MT];
+#pragma unroll
+  for (int t = 0; t < MT; ++t) {
+    const int row = 16 * t + r;
+    xo[t] = 2u * ((uint32_t)(row < M ? row : M - 1) * (uint32_t)lda + 16u * (uint32_t)g);  // (rows past M: not stored)
+  }
+  FUnit<FMT> us[PD][T];
+  gq_half8 xs[PD][MT][4];
+  auto request = [&](int unit, int st) __attribute__((always_inline)) {
+#pragma unroll
+    for (int t = 0; t < T; ++t) load_unit<FMT>(tl[t], unit, lane, us[st][t]);
+#pragma unroll
+    for (int t = 0; t < MT; ++t) {
+      const uint32_t o = unit < units ? xo[t] + 256u * (uint32_t)unit : 0xFFFFFF00u;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const auto v = __builtin_amdgcn_raw_buffer_load_b128(xr, o, 128u * (i >> 1) + 16u * (i & 1), 0);
+        xs[st][t][i] = __builtin_bit_cast(gq_half8, gq_u4{v[0], v[1], v[2], v[3]});
+      }
+    }
+  };
+  gq_f4 acc[T][MT];
+#pragma unroll
+  for (int t = 0; t < T; ++t)
+#pragma unroll
+    for (int i = 0; i < MT; ++i) acc[t][i] = gq_f4{0.f, 0.f, 0.f, 0.f};
+  const uint32_t mg = gq_nib_magic();
+  auto compute = [&](int unit, int st) __attribute__((always_inline)) {
+#pragma unroll
+    for (int t = 0; t < T; ++t) {
+      gq_half8 b[2][2];
+      rows_frags<FMT>(us[st][t], unit, g, mg, b);
+#pragma unroll
+      for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int f = 0; f < 4; ++f) acc[t][i] = gq_mfma16(xs[st][i][f], b[f >> 1][f & 1], acc[t][i]);
+    }
+  };
+  walk_units<PD, KS>(units, wave, request, compute);
+#pragma unroll
+  for (int t = 0; t < T; ++t)
+#pragma unroll
+    for (int i = 0; i < MT; ++i) red[wave][t][i][lane] = acc[t][i];
+  __syncthreads();
+  front_out<KS, R>(
+      [&](int k, int w, int t, int n, int m) {
+        return reinterpret_cast<const float *>(&red[k][w * R + t][m >> 4][16 * ((m >> 2) & 3) + n])[m & 3];
+      },
+      rs, h, go, uo, dt, M, N, act);
+}
+
+// ---- forward: register-B tiles ---------------------------------------------------
+// gq_gemm's register-B kernel on two matrices at once: a wave owns NJ 32-column blocks of
+// W_gate and the same of W_up, so one activation fragment read from LDS feeds the products of
+// both, and the epilogue has g and u of an output in the same lane: h (and g, u where they
+// are kept) goes out once, nothing comes back.  Operand order, swizzle and pipeline are those
+// of gq_gemm_frag.h: fp16 activations by LDS DMA PD - 1 steps of 64 k ahead, weights PD steps
+// ahead in registers.  KG: groups of waves that share the tile and take every KG-th step,
+// their sums added through LDS at the end.
+template <int DT>
+GQ_DEV void front_put(const __amdgpu_buffer_rsrc_t &r, uint32_t vo, uint32_t so, int dt, float v) {
+  if constexpr (DT == GQ_DT_F32)
+    __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(v), r, vo, so, 0);
+  else
+    __builtin_amdgcn_raw_buffer_store_b16(
+        dt == GQ_DT_BF16 ? gq_f32_to_bf16(v) : __builtin_bit_cast(uint16_t, (_Float16)v), r, vo, so, 0);
+}
+
+// waves per SIMD: what a workgroup brings, at least two but where the sums of 256 rows take
+// the registers of both
+constexpr int front_wpe(int waves, int bm) { return waves > 4 ? waves / 4 : bm > 128 ? 1 : 2; }
+
+template <int FMT, int BM, int WM, int WN, int NJ, int PD, int KG>
+__global__ void __launch_bounds__(64 * WM * WN * KG)
+__attribute__((amdgpu_waves_per_eu(front_wpe(WM *WN *KG, BM), front_wpe(WM *WN *KG, BM))))
+k_front_rb(const uint8_t *__restrict__ wg, const uint8_t *__restrict__ wu, uint32_t sc_off,
+           const _Float16 *__restrict__ a16, int lda, const float *__restrict__ rs, void *__restrict__ h,
+           void *__restrict__ go, void *__restrict__ uo, int dt, int M, int N, int C, int nsteps, int tiles_m, int act) {
+  constexpr int KS = BK / 16, NW = WM * WN, TM = BM / WM / 32, BN = 32 * NJ * WN;
+  __shared__ __attribute__((aligned(16))) _Float16 As_0[KG * BM * BK];
+  __shared__ __attribute__((aligned(16))) _Float16 As_1[KG * BM * BK];
+  __shared__ __attribute__((aligned(16))) _Float16 As_2[PD >= 3 ? KG * BM * BK : 8];
+  __shared__ __attribute__((aligned(16))) _Float16 As_3[PD >= 4 ? KG * BM * BK : 8];
+  __shared__ __attribute__((aligned(16))) float rs_s[BM];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int kg = KG == 1 ? 0 : __builtin_amdgcn_readfirstlane((tid >> 6) / NW);
+  const int wave = __builtin_amdgcn_readfirstlane((tid >> 6) % NW);
+  const int wm = wave / WN, wn = wave % WN;
+  auto As_of = [&](auto b) -> _Float16 * {
+    constexpr int v = decltype(b)::value;
+    return (v == 0 ? As_0 : v == 1 ? As_1 : v == 2 ? As_2 : As_3) + kg * (BM * BK);
+  };
+  using B0 = std::integral_constant<int, 0>;
+  using B1 = std::integral_constant<int, 1>;
+  using B2 = std::integral_constant<int, 2>;
+  using B3 = std::integral_constant<int, 3>;
+  // loads a step may leave in flight: activations of steps s + 2 .. s + PD - 1, weights of s + 2 .. s + PD
+  constexpr int NA = BM / (8 * NW), pend = (PD - 2) * NA + (PD - 1) * 2 * kRLoads<FMT> * NJ;
+  static_assert(pend <= 63, "vmcnt immediate");
+  constexpr int kWaitPend = 0x0F70 | (pend & 15) | ((pend >> 4) << 14);
+  int mt, nt;
+  tile_of_g(blockIdx.x, gridDim.x, tiles_m, (N + BN - 1) / BN, 4, mt, nt);
+  const int m0 = mt * BM, n0 = nt * BN, nl = nsteps / KG;
+  const int ntiles = (int)gq_tiles(N), kh = lane >> 5, r = lane & 15;
+  uint32_t qo[NJ], so[NJ];  // byte offsets of this lane's codes (slot kh) and scales, chunk 0
+#pragma unroll
+  for (int j = 0; j < NJ; ++j) {
+    int t = (n0 + 32 * (NJ * wn + j) + (lane & 31)) >> 4;
+    if (t >= ntiles) t = ntiles - 1;  // clamped; those columns are never stored
+    const uint32_t tc = (uint32_t)t * (uint32_t)C;
+    qo[j] = tc * (uint32_t)gq_chunk_qs_bytes(FMT) + 16u * (16u * (uint32_t)kh + (uint32_t)r);
+    so[j] = sc_off + tc * (uint32_t)gq_chunk_sc_bytes(FMT) + (FMT == GQ_FMT_Q4_0 || FMT == GQ_FMT_Q8_0 ? 8u : 16u) * r;
+  }
+  gq_f16v acc[2][TM][NJ];
+#pragma unroll
+  for (int w = 0; w < 2; ++w)
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+#pragma unroll
+      for (int j = 0; j < NJ; ++j)
+#pragma unroll
+        for (int v = 0; v < 16; ++v) acc[w][i][j][v] = 0.f;
+  RStep<FMT, NJ> st[2][PD];
+  const uint32_t mg = gq_nib_magic();
+  uint32_t ao[NA];
+  a_offsets<BM, NW>(lda, M, m0, wave, lane, ao);
+  const int arow = (BM / WM) * wm + (lane & 31), sw = a_swz(lane & 31);
+  auto gstep = [&](int l) { return (l < nl ? l : nl - 1) * KG + kg; };
+  auto run_step = [&](int l, auto buf_c) __attribute__((always_inline)) {
+    constexpr int BUF = decltype(buf_c)::value;
+    using NB = std::integral_constant<int, (BUF + PD - 1) % PD>;
+    const int step = l * KG + kg, s1 = gstep(l + PD - 1), s2 = gstep(l + PD);
+    load_a_lds_b<BM, NW>(a16, ao, s1, wave, As_of(NB{}));
+    __builtin_amdgcn_sched_barrier(0);
+    const _Float16 *As = As_of(buf_c) + arow * BK;
+    gq_half8 af[2][TM];
+    auto read_a = [&](int ks, int fb) __attribute__((always_inline)) {
+      const int ch = (4 * (ks >> 1) + 2 * kh + (ks & 1)) ^ sw;
+#pragma unroll
+      for (int i = 0; i < TM; ++i) af[fb][i] = *reinterpret_cast<const gq_half8 *>(As + 32 * i * BK + 8 * ch);
+    };
+    read_a(0, 0);
+    QKf qk[2][NJ][2];
+    gq_half2 q6[2][NJ][2];
+#pragma unroll
+    for (int w = 0; w < 2; ++w) {
+      if constexpr (FMT == GQ_FMT_Q4_K) q4k_factors<NJ>(st[w][BUF], step, qk[w]);
+      if constexpr (FMT == GQ_FMT_Q6_K) q6k_factors<NJ>(st[w][BUF], kh, q6[w]);
+    }
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      if (ks + 1 < KS) read_a(ks + 1, (ks + 1) & 1);
+#pragma unroll
+      for (int j = 0; j < NJ; ++j)
+#pragma unroll
+        for (int w = 0; w < 2; ++w) {
+          const gq_half8 bf = rfrag<FMT, NJ>(st[w][BUF], j, ks, step, qk[w][j], q6[w][j], mg);
+#pragma unroll
+          for (int i = 0; i < TM; ++i) acc[w][i][j] = gq_mfma32(af[ks & 1][i], bf, acc[w][i][j]);
+        }
+    }
+    load_rstep<FMT, NJ>(wg, qo, so, s2, st[0][BUF]);
+    load_rstep<FMT, NJ>(wu, qo, so, s2, st[1][BUF]);
+    __builtin_amdgcn_s_waitcnt(kWaitPend);
+    __syncthreads();
+  };
+  auto prime = [&](auto b) __attribute__((always_inline)) {
+    constexpr int i = decltype(b)::value;
+    const int s = gstep(i);
+    if constexpr (i < PD - 1) load_a_lds_b<BM, NW>(a16, ao, s, wave, As_of(b));
+    load_rstep<FMT, NJ>(wg, qo, so, s, st[0][i]);
+    load_rstep<FMT, NJ>(wu, qo, so, s, st[1][i]);
+  };
+  const gq_f4 rs4 = *reinterpret_cast<const gq_f4 *>(rs + m0 + 4 * (tid % (BM / 4)));  // (padded past M)
+  prime(B0{});
+  prime(B1{});
+  if constexpr (PD >= 3) prime(B2{});
+  if constexpr (PD >= 4) prime(B3{});
+  __builtin_amdgcn_s_waitcnt(kWaitPend);
+  if (tid < BM / 4) *reinterpret_cast<gq_f4 *>(rs_s + 4 * tid) = rs4;
+  __syncthreads();
+  for (int l = 0; l < nl; l += PD) {
+    run_step(l, B0{});
+    if (l + 1 < nl) run_step(l + 1, B1{});
+    if constexpr (PD >= 3)
+      if (l + 2 < nl) run_step(l + 2, B2{});
+    if constexpr (PD >= 4)
+      if (l + 3 < nl) run_step(l + 3, B3{});
+  }
+  if constexpr (KG > 1) {
+    __shared__ __attribute__((aligned(16))) gq_f4 xs[(KG - 1) * NW * 4 * 64];
+#pragma unroll
+    for (int w = 0; w < 2; ++w)
+#pragma unroll
+      for (int i = 0; i < TM; ++i)
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) {
+          gq_f16v &a = acc[w][i][j];
+          if (kg > 0) {
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+              xs[(((kg - 1) * NW + wave) * 4 + q) * 64 + lane] = gq_f4{a[4 * q], a[4 * q + 1], a[4 * q + 2], a[4 * q + 3]};
+          }
+          __syncthreads();
+          if (kg == 0) {
+#pragma unroll
+            for (int g = 0; g < KG - 1; ++g)
+#pragma unroll
+              for (int q = 0; q < 4; ++q) {
+                const gq_f4 t = xs[((g * NW + wave) * 4 + q) * 64 + lane];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) a[4 * q + e] += t[e];
+              }
+          }
+          __syncthreads();
+        }
+    if (kg > 0) return;
+  }
+  // D layout (32x32): lane l holds column l % 32, rows 8 (v / 4) + 4 (l / 32) + v % 4.  A store's
+  // row is a scalar offset from the lane's; rows >= M lie past the resource's end (host: a
+  // tile's rows span less than 2 GiB).
+  auto store = [&](auto dtc) __attribute__((always_inline)) {
+    constexpr int DT = decltype(dtc)::value;
+    constexpr uint32_t ES = DT == GQ_DT_F32 ? 4u : 2u;
+    const size_t left = (size_t)(M - m0) * (size_t)N * ES;
+    const int range = (int)(uint32_t)(left < 0xFFFFFFFFu ? left : 0xFFFFFFFFu);
+    auto rsrc = [&](void *p) {
+      return __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<uint8_t *>(p) + (p ? (size_t)m0 * N * ES : 0), (short)0,
+                                               p ? range : 0, 0x00020000);
+    };
+    const __amdgpu_buffer_rsrc_t hr = rsrc(h), gr = rsrc(go), ur = rsrc(uo);  // (an output not wanted: no range)
+#pragma unroll
+    for (int i = 0; i < TM; ++i) {
+      const int mb = (BM / WM) * wm + 32 * i + 4 * (lane >> 5);
+      float rsv[16];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const gq_f4 t = *reinterpret_cast<const gq_f4 *>(rs_s + mb + 8 * q);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) rsv[4 * q + e] = t[e];
+      }
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) {
+        const int n = n0 + 32 * (NJ * wn + j) + (lane & 31);
+        if (n >= N) continue;
+        const uint32_t vo = ((uint32_t)mb * (uint32_t)N + (uint32_t)n) * ES;
+#pragma unroll
+        for (int v = 0; v < 16; ++v) {
+          const uint32_t ro = (uint32_t)(8 * (v >> 2) + (v & 3)) * (uint32_t)N * ES;
+          const float g = acc[0][i][j][v] * rsv[v], u = acc[1][i][j][v] * rsv[v];
+          front_put<DT>(hr, vo, ro, dt, gq_act_f(act, g) * u);
+          if (go) front_put<DT>(gr, vo, ro, dt, g);
+          if (uo) front_put<DT>(ur, vo, ro, dt, u);
+        }
+      }
+    }
+  };
+  if (dt == GQ_DT_F32) store(std::integral_constant<int, GQ_DT_F32>{});
+  else store(std::integral_constant<int, GQ_DT_BF16>{});
 }
 
 GQ_DEV void front_grads(int act, float dh, float g, float u, float &dg, float &du) {
@@ -108,6 +704,114 @@ __global__ void __launch_bounds__(256) k_front_dgu(const void *dh, const void *g
   }
 }
 
+template <int FMT, int BM, int WM, int WN, int NJ, int PD, int KG>
+int launch_front_rb(const void *wg, const void *wu, const _Float16 *a16, int lda, const float *rs, void *h, void *go,
+                    void *uo, int dt, int M, int N, int K, int act, hipStream_t s) {
+  const int tiles_m = (M + BM - 1) / BM, tiles_n = (N + 32 * NJ * WN - 1) / (32 * NJ * WN);
+  GQ_CHECK((size_t)tiles_m * (size_t)tiles_n <= 0x7FFFFFFFu, GQ_ERR_INVALID_ARGS);  // (one grid dimension)
+  hipLaunchKernelGGL((k_front_rb<FMT, BM, WM, WN, NJ, PD, KG>), dim3((unsigned)(tiles_m * tiles_n)), dim3(64 * WM * WN * KG),
+                     0, s, (const uint8_t *)wg, (const uint8_t *)wu, (uint32_t)gq_sc_plane_offset(FMT, N, K), a16, lda, rs,
+                     h, go, uo, dt, M, N, (int)gq_chunks(FMT, K), (int)(gq_kpad(FMT, K) / BK), tiles_m, act);
+  return gq_last_launch();
+}
+template <int FMT, int XT>
+int launch_front_few_t(const void *wg, const void *wu, const void *x, const float *rs, void *h, void *go, void *uo, int dt,
+                       int M, int N, int K, int act, hipStream_t s) {
+#ifndef FKS
+#define FKS 4
+#define FRS 4
+#endif
+  const int units = (int)(gq_kpad(FMT, K) / 128);
+#define GQ_FEW(MR, R, KS)                                                                                             \
+  hipLaunchKernelGGL((k_front_few<FMT, XT, MR, R, KS>), dim3((unsigned)((gq_tiles(N) + (R)-1) / (R))), dim3(64 * (KS)), 0, s, \
+                     (const uint8_t *)wg, (const uint8_t *)wu, gq_sc_plane_offset(FMT, N, K), x, rs, h, go, uo, dt, M, N, K,  \
+                     (int)gq_chunks(FMT, K), units, act)
+#ifdef GQ_TUNE
+  if (getenv("GQ_R2")) {
+  if (M == 1) GQ_FEW(1, 2, FKS);
+  else GQ_FEW(4, 2, FKS);
+  return 0;
+  }
+#endif
+  if (M == 1) GQ_FEW(1, 1, FKS);
+  else GQ_FEW(4, 1, FKS);
+#undef GQ_FEW
+  return gq_last_launch();
+}
+// x of xt (f16 or bf16), 4-byte aligned
+int launch_front_few(int fmt, const void *wg, const void *wu, const void *x, int xt, const float *rs, void *h, void *go,
+                     void *uo, int dt, int M, int N, int K, int act, hipStream_t s) {
+#define GQ_FMT_X(F)                                                                                          \
+  (xt == GQ_DT_F16 ? launch_front_few_t<F, GQ_DT_F16>(wg, wu, x, rs, h, go, uo, dt, M, N, K, act, s)         \
+                   : launch_front_few_t<F, GQ_DT_BF16>(wg, wu, x, rs, h, go, uo, dt, M, N, K, act, s))
+  if (fmt == GQ_FMT_Q4_0) return GQ_FMT_X(GQ_FMT_Q4_0);
+  if (fmt == GQ_FMT_Q8_0) return GQ_FMT_X(GQ_FMT_Q8_0);
+  if (gq_fmt_is_q6k(fmt)) return GQ_FMT_X(GQ_FMT_Q6_K);
+  return GQ_FMT_X(GQ_FMT_Q4_K);
+#undef GQ_FMT_X
+}
+template <int FMT>
+int launch_front_rows_t(const void *wg, const void *wu, const _Float16 *a16, int lda, const float *rs, void *h, void *go,
+                        void *uo, int dt, int M, int N, int K, int act, hipStream_t s) {
+  const int units = (int)(gq_kpad(FMT, K) / 128);
+#define GQ_ROWS(MT, R, KS)                                                                                           \
+  hipLaunchKernelGGL((k_front_rows<FMT, MT, R, KS>), dim3((unsigned)((gq_tiles(N) + (R)-1) / (R))), dim3(64 * (KS)), 0, s, \
+                     (const uint8_t *)wg, (const uint8_t *)wu, gq_sc_plane_offset(FMT, N, K), a16, lda, rs, h, go, uo, dt, \
+                     M, N, (int)gq_chunks(FMT, K), units, act)
+#ifdef GQ_TUNE
+  if (getenv("GQ_R2")) {
+  if (M <= 16) GQ_ROWS(1, 2, FRS);
+  else GQ_ROWS(2, 2, FRS);
+  return 0;
+  }
+#endif
+  if (M <= 16) GQ_ROWS(1, 1, FRS);
+  else GQ_ROWS(2, 1, FRS);
+#undef GQ_ROWS
+  return gq_last_launch();
+}
+int launch_front_rows(int fmt, const void *wg, const void *wu, const _Float16 *a16, int lda, const float *rs, void *h,
+                      void *go, void *uo, int dt, int M, int N, int K, int act, hipStream_t s) {
+  if (fmt == GQ_FMT_Q4_0) return launch_front_rows_t<GQ_FMT_Q4_0>(wg, wu, a16, lda, rs, h, go, uo, dt, M, N, K, act, s);
+  if (fmt == GQ_FMT_Q8_0) return launch_front_rows_t<GQ_FMT_Q8_0>(wg, wu, a16, lda, rs, h, go, uo, dt, M, N, K, act, s);
+  if (gq_fmt_is_q6k(fmt)) return launch_front_rows_t<GQ_FMT_Q6_K>(wg, wu, a16, lda, rs, h, go, uo, dt, M, N, K, act, s);
+  return launch_front_rows_t<GQ_FMT_Q4_K>(wg, wu, a16, lda, rs, h, go, uo, dt, M, N, K, act, s);
+}
+template <int FMT>
+int launch_front_fmt(const void *wg, const void *wu, const _Float16 *a16, int lda, const float *rs, void *h, void *go,
+                     void *uo, int dt, int M, int N, int K, int act, hipStream_t s) {
+#define GQ_FRONT(...) launch_front_rb<FMT, __VA_ARGS__>(wg, wu, a16, lda, rs, h, go, uo, dt, M, N, K, act, s)
+#ifdef GQ_TUNE
+  const char *e = getenv("GQ_FT");
+  switch (e ? atoi(e) : 0) {
+  case 1: return GQ_FRONT(128, 1, 4, 1, 2, 1);
+  case 2: return GQ_FRONT(128, 1, 4, 1, 3, 2);
+  case 3: return GQ_FRONT(64, 1, 4, 1, 3, 2);
+  case 4: return GQ_FRONT(64, 1, 2, 1, 3, 4);
+  case 5: return GQ_FRONT(32, 1, 2, 1, 4, 4);
+  case 6: return GQ_FRONT(32, 1, 4, 1, 4, 4);
+  case 7: return GQ_FRONT(64, 1, 2, 1, 4, 4);
+  default: break;
+  }
+#endif
+  auto wgs = [&](int bm, int bn) { return (size_t)((M + bm - 1) / bm) * (size_t)((N + bn - 1) / bn); };
+  const int nsteps = (int)(gq_kpad(FMT, K) / BK);
+  if (wgs(64, 64) <= 288 && nsteps % 4 == 0) return GQ_FRONT(64, 1, 2, 1, 3, 4);
+  if (wgs(64, 128) <= 288) return GQ_FRONT(64, 1, 4, 1, 3, 2);
+  if (wgs(128, 128) <= 288) return GQ_FRONT(128, 1, 4, 1, 3, 2);
+  return GQ_FRONT(128, 1, 4, 1, 2, 1);
+#undef GQ_FRONT
+}
+int launch_front(int fmt, const void *wg, const void *wu, const _Float16 *a16, int lda, const float *rs, void *h, void *go,
+                 void *uo, int dt, int M, int N, int K, int act, hipStream_t s) {
+  if (fmt == GQ_FMT_Q4_0) return launch_front_fmt<GQ_FMT_Q4_0>(wg, wu, a16, lda, rs, h, go, uo, dt, M, N, K, act, s);
+#ifndef ONLYQ4
+  if (fmt == GQ_FMT_Q8_0) return launch_front_fmt<GQ_FMT_Q8_0>(wg, wu, a16, lda, rs, h, go, uo, dt, M, N, K, act, s);
+  if (gq_fmt_is_q6k(fmt)) return launch_front_fmt<GQ_FMT_Q6_K>(wg, wu, a16, lda, rs, h, go, uo, dt, M, N, K, act, s);
+#endif
+  return launch_front_fmt<GQ_FMT_Q4_K>(wg, wu, a16, lda, rs, h, go, uo, dt, M, N, K, act, s);
+}
+
 int check_front(int fmt, const void *gate, const void *up, size_t M, size_t N, size_t K, int act) {
   GQ_TRY(gq_check_shape(fmt, N, K));
   GQ_CHECK(M <= GQ_MAX_DIM, GQ_ERR_INVALID_ARGS);
@@ -120,7 +824,24 @@ int check_front(int fmt, const void *gate, const void *up, size_t M, size_t N, s
 
 }  // namespace
 
-extern "C" size_t gq_ffn_gate_up_workspace_bytes(int fmt, size_t M, size_t N, size_t K) { return 0; }
+
+constexpr size_t kFewRows = 4;
+// Rows that go into the few-row kernel without a conversion
+static bool front_as_it_is(const void *x, int x_dtype, size_t M) {
+  return M <= kFewRows && x_dtype != GQ_DT_F32 && (uintptr_t)x % 4 == 0;
+}
+// Rows a call takes at a time: their fp16 copies stay below 64 MiB (and 32-bit offsets)
+static size_t front_rows(int fmt, size_t M, size_t K) {
+  const size_t fit = (((size_t)64 << 20) / (2 * gq_kpad(fmt, K))) & ~(size_t)255;
+  const size_t mb = fit < 256 ? 256 : fit;
+  return M < mb ? M : mb;
+}
+
+extern "C" size_t gq_ffn_gate_up_workspace_bytes(int fmt, size_t M, size_t N, size_t K) {
+  if (!gq_fmt_valid(fmt) || M > GQ_MAX_DIM || N > GQ_MAX_DIM || K > GQ_MAX_DIM) return 0;
+  const size_t mb = front_rows(fmt, M, K);
+  return gq_align256(mb * (gq_kpad(fmt, K) + 8) * 2) + gq_align256((mb + 256) * 4);
+}
 
 extern "C" int gq_ffn_gate_up(int fmt, const void *gate, const void *up, const void *x, int x_dtype, void *h,
                               int h_dtype, void *g, void *u, size_t M, size_t N, size_t K, int act, void *ws,
@@ -130,11 +851,35 @@ extern "C" int gq_ffn_gate_up(int fmt, const void *gate, const void *up, const v
   GQ_CHECK(x && h, GQ_ERR_INVALID_ARGS);
   if (M == 0 || N == 0) return GQ_OK;
   GQ_CHECK(K > 0, GQ_ERR_INVALID_ARGS);
-  const dim3 grid((unsigned)gq_tiles(N), (unsigned)(M < 65536 ? (M + 15) / 16 : 4096));
-  hipLaunchKernelGGL(k_front, grid, dim3(256), 0, (hipStream_t)stream, fmt, (const uint8_t *)gate,
-                     (const uint8_t *)up, gq_sc_plane_offset(fmt, N, K), x, x_dtype, h, h_dtype, g, u, (int)M, (int)N,
-                     (int)K, (int)gq_chunks(fmt, K), act);
-  return gq_last_launch();
+  GQ_CHECK(N * 256 * gq_dtype_size(h_dtype) < ((size_t)1 << 31), GQ_ERR_INVALID_ARGS);  // (a tile's rows of outputs)
+  hipStream_t s = (hipStream_t)stream;
+  if (front_as_it_is(x, x_dtype, M))
+    return launch_front_few(fmt, gate, up, x, x_dtype, nullptr, h, g, u, h_dtype, (int)M, (int)N, (int)K, act, s);
+  const size_t need = gq_ffn_gate_up_workspace_bytes(fmt, M, N, K), mb = front_rows(fmt, M, K), Kp = gq_kpad(fmt, K);
+  GqScratch sc(ws ? 0 : need, s);
+  if (ws) GQ_CHECK(ws_bytes >= need, GQ_ERR_WORKSPACE);
+  else ws = sc.ptr;
+  GQ_CHECK(ws, GQ_ERR_WORKSPACE);
+  _Float16 *a16 = (_Float16 *)ws;
+  float *rs = (float *)((uint8_t *)ws + gq_align256(mb * (Kp + 8) * 2));
+  const int q4 = fmt == GQ_FMT_Q4_0 || gq_fmt_is_q4k(fmt);
+  if (M <= kFewRows) {  // (x in fp32, or at an odd address)
+    GQ_TRY(gq_launch_a_to_f16(x, x_dtype, a16, rs, (int)M, (int)K, (int)K, 0, s));
+    return launch_front_few(fmt, gate, up, a16, GQ_DT_F16, rs, h, g, u, h_dtype, (int)M, (int)N, (int)K, act, s);
+  }
+  if (M <= 32) {  // rows 16 bytes longer than a multiple of 4 KiB, where 16 of them would collide
+    const int ld = (int)Kp + 8;
+    GQ_TRY(gq_launch_a_to_f16(x, x_dtype, a16, rs, (int)M, (int)K, ld, q4, s));
+    return launch_front_rows(fmt, gate, up, a16, ld, rs, h, g, u, h_dtype, (int)M, (int)N, (int)K, act, s);
+  }
+  const size_t xs = gq_dtype_size(x_dtype) * K, hs = gq_dtype_size(h_dtype) * N;
+  for (size_t m0 = 0; m0 < M; m0 += mb) {
+    const int m = (int)(M - m0 < mb ? M - m0 : mb);
+    GQ_TRY(gq_launch_a_to_f16((const uint8_t *)x + m0 * xs, x_dtype, a16, rs, m, (int)K, (int)Kp, q4, s));
+    auto at = [&](void *p) { return p ? (void *)((uint8_t *)p + m0 * hs) : nullptr; };
+    GQ_TRY(launch_front(fmt, gate, up, a16, (int)Kp, rs, at(h), at(g), at(u), h_dtype, m, (int)N, (int)K, act, s));
+  }
+  return GQ_OK;
 }
 
 extern "C" size_t gq_ffn_gate_up_bwd_workspace_bytes(int fmt, size_t M, size_t N, size_t K) { return 0; }

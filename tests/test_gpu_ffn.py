@@ -3,8 +3,9 @@
 Tolerances.  A product over K is a sum of independent terms, so its error, as a share of a row's norm, is that of one
 term: x to fp16 (2^-11 at most, f32 and bf16 inputs scaled by a power of two first) and the weight to fp16 (2^-11;
 the k-quants with a minimum round twice, and there to 2^-11 of a product up to three times the weight's size) -- under 1e-3,
-the bound of every product of this library.  h multiplies two such products: 2e-3.  A rounding of the output adds
-finfo.eps / 2.  dg and du are fp32 arithmetic: ten roundings of 2^-24 and a 2^-21 exponential."""
+the bound of every product of this library.  Such an error has one size along a row, whatever the value it falls
+on, so in h = act(g) u it counts as dh = u act'(g) dg + act(g) du with dg, du of 1e-3 of the rms of their row: a row whose gates
+are mostly closed is small itself while u act'(g) dg is not.  A rounding of the output adds finfo.eps / 2.  dg and du are fp32 arithmetic: ten roundings of 2^-24 and a 2^-21 exponential."""
 import numpy as np
 import pytest
 import torch
@@ -20,10 +21,6 @@ PRODUCT = 1e-3
 
 def half_step(dtype):
     return torch.finfo(dtype).eps / 2
-
-
-def rel(a, b):
-    return float((a.double() - b).norm() / b.norm().clamp_min(1e-300))
 
 
 def worst_row(a, b):
@@ -64,7 +61,10 @@ class Case:
 
 def check_front(c, act, out, dtype):
     h, g, u = c.front(act)
-    assert worst_row(out[0], h) <= 2 * PRODUCT + half_step(dtype)
+    f, d = act_grad(act, g)
+    rms = [t.pow(2).mean(1).sqrt() for t in (g, u)]
+    bound = PRODUCT * (rms[0] * (u * d).norm(dim=1) + rms[1] * f.norm(dim=1)) + half_step(dtype) * h.norm(dim=1)
+    assert bool(((out[0].double() - h).norm(dim=1) <= bound + 1e-30).all())
     for o, r in ((out[1], g), (out[2], u)):
         if o is not None:
             assert worst_row(o, r) <= PRODUCT + half_step(dtype)
@@ -366,6 +366,7 @@ def test_block_trains_and_decodes(dev):
     for i in (0, 33, 69):
         one = gq.ffn_gate_up(fmt, *c.packed, c.x[i], n, k, out_dtype=torch.float32)
         dec = gq.gemv_swiglu(fmt, *c.packed, c.x[i].float(), n, k)
-        ref = c.front(0)[0][i:i + 1]
-        assert rel(one, ref) <= 2 * PRODUCT and rel(dec, ref) <= 2 * PRODUCT
-        assert rel(h[i:i + 1], ref) <= 2 * PRODUCT + half_step(torch.bfloat16)
+        c1 = Case.__new__(Case)
+        c1.w, c1.x = c.w, c.x[i:i + 1]
+        for t in (one, dec, h[i:i + 1]):
+            check_front(c1, 0, (t, None, None), t.dtype)
