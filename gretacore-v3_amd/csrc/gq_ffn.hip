@@ -1,7 +1,5 @@
 // gq_ffn.hip -- the gated feed-forward front h = act(x W_gate^T) * (x W_up^T) over T16
 // weights for any number of rows, and its backward pass.
-#include <stdlib.h>
-
 #include <type_traits>
 
 #include "gq_act.h"
@@ -110,12 +108,12 @@ GQ_DEV gq_u4 nib_order(const gq_u4 &v) {
                __builtin_amdgcn_perm(v[1], v[0], 0x07060302u), __builtin_amdgcn_perm(v[3], v[2], 0x07060302u)};
 }
 
-// Sums of the waves, h and where they are kept g and u.  at(k, w, t, n, m): wave k's part of output
+// Sums of the waves, h and where they are kept g and u, of the R tiles `block`.  at(k, w, t, n, m): wave k's part of output
 // (m, 16 t + n) of matrix w; rs: row scales of x
 template <int KS, int R, typename At>
-GQ_DEV void front_out(At at, const float *rs, void *h, void *go, void *uo, int dt, int M, int N, int act) {
+GQ_DEV void front_out(At at, const float *rs, void *h, void *go, void *uo, int dt, int M, int N, int act, int block) {
   for (int o = threadIdx.x; o < 16 * R * M; o += 64 * KS) {
-    const int nl = o % (16 * R), m = o / (16 * R), n = 16 * R * (int)blockIdx.x + nl;
+    const int nl = o % (16 * R), m = o / (16 * R), n = 16 * R * block + nl;
     float y[2] = {0.f, 0.f};
 #pragma unroll
     for (int w = 0; w < 2; ++w)
@@ -327,7 +325,7 @@ k_front_few(const uint8_t *__restrict__ wg, const uint8_t *__restrict__ wu, size
         for (int i = 0; i < NG; ++i) y += red[k][w * R + t][MR == 1 ? 0 : m][16 * i + n];
         return y;
       },
-      rs, h, go, uo, dt, M, N, act);
+      rs, h, go, uo, dt, M, N, act, (int)blockIdx.x);
 }
 
 // More rows: the sums of the scale groups would cost more than folding the scale into the
@@ -450,7 +448,280 @@ k_front_rows(const uint8_t *__restrict__ wg, const uint8_t *__restrict__ wu, siz
       [&](int k, int w, int t, int n, int m) {
         return reinterpret_cast<const float *>(&red[k][w * R + t][m >> 4][16 * ((m >> 2) & 3) + n])[m & 3];
       },
-      rs, h, go, uo, dt, M, N, act);
+      rs, h, go, uo, dt, M, N, act, (int)blockIdx.x);
+}
+
+// K up to 4096: x stays in registers.  A wave's share of K is the same for every row tile, so a
+// workgroup of 8 waves reads (and converts) x once and walks the tiles blockIdx.x, + gridDim.x, ...; while a
+// unit of one tile is computed the same unit of the next tile is requested, NU units in
+// flight a wave.  14336 x 4096, 16 rows, Q4_K / Q6_K: x read for every tile 27.5 / 31.3 us, so 21.8 / 26.2.
+constexpr int kPxWaves = 8;
+struct __attribute__((packed, aligned(2))) FRun16 {  // 8 values at any 2-byte address
+  gq_u4 v;
+};
+struct __attribute__((packed, aligned(4))) FRun32 {
+  gq_f4 v[2];
+};
+// a run of 8 values of x as it lies in memory, and as floats (zeros where !in)
+template <int XT>
+struct FRaw {
+  gq_u4 v[XT == GQ_DT_F32 ? 2 : 1];
+};
+template <int XT>
+GQ_DEV void px_load(const void *x, size_t at, FRaw<XT> &r) {
+  if constexpr (XT == GQ_DT_F32) {
+    const FRun32 t = *reinterpret_cast<const FRun32 *>(reinterpret_cast<const float *>(x) + at);
+    r.v[0] = __builtin_bit_cast(gq_u4, t.v[0]);
+    r.v[1] = __builtin_bit_cast(gq_u4, t.v[1]);
+  } else {
+    r.v[0] = reinterpret_cast<const FRun16 *>(reinterpret_cast<const uint16_t *>(x) + at)->v;
+  }
+}
+template <int XT>
+GQ_DEV void px_floats(const FRaw<XT> &r, bool in, float (&o)[8]) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    float f;
+    if constexpr (XT == GQ_DT_F32) f = __uint_as_float(r.v[e >> 2][e & 3]);
+    else if constexpr (XT == GQ_DT_BF16) f = __uint_as_float(e & 1 ? r.v[0][e >> 1] & 0xFFFF0000u : r.v[0][e >> 1] << 16);
+    else f = (float)gq_bits_h2(r.v[0][e >> 1])[e & 1];
+    o[e] = in ? f : 0.f;
+  }
+}
+// The tiles of a workgroup: request(tile, slot) ahead, compute(slot), then finish(tile) with the sums
+template <int NU, typename Load, typename Request, typename Begin, typename Compute, typename Finish>
+GQ_DEV void walk_tiles(int ntiles, Load load_x, Request request, Begin begin, Compute compute, Finish finish) {
+  int tile = blockIdx.x;
+  load_x();  // (before the first requests: behind them its loads would wait for theirs)
+  __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+  for (int i = 0; i < NU; ++i) request(tile, i);
+  __builtin_amdgcn_sched_barrier(0);
+  begin();
+  int buf = 0;
+  for (; tile < ntiles; tile += gridDim.x) {
+#pragma unroll
+    for (int i = 0; i < NU; ++i) {
+      compute(i);
+      request(tile + (int)gridDim.x, i);  // (past the last tile: nothing is fetched)
+    }
+    finish(tile, buf);
+    buf ^= 1;
+  }
+}
+
+// Up to 4 rows of 16-bit x (the sums of k_front_few).  The operands made of x and its sums stay in
+// registers too: 14336 x 4096 Q4_K one row 17.3 us with them made for every tile, 15.4 so.
+template <int FMT, int XT, int MR, int NU>
+__global__ void __launch_bounds__(64 * kPxWaves) __attribute__((amdgpu_waves_per_eu(2)))
+k_front_few_px(const uint8_t *__restrict__ wg, const uint8_t *__restrict__ wu, size_t sc_off, const void *__restrict__ x,
+               void *__restrict__ h, void *__restrict__ go, void *__restrict__ uo, int dt, int M, int N, int K, int C,
+               int units, int act) {
+  constexpr int NG = kFewGroups<FMT>;
+  constexpr float OFF = kFewOff<FMT, XT>;
+  __shared__ float red[2][kPxWaves][2][MR][64];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int g = lane >> 4, ntiles = (int)gq_tiles(N);
+  constexpr bool SUMS = OFF != 0.f || FMT == GQ_FMT_Q4_K;
+  gq_u4 ops[NU][4];
+  float sums[NU][2][MR];
+  constexpr uint32_t one = XT == GQ_DT_F16 ? 0x3C003C00u : 0x3F803F80u;
+  const gq_u4 ones = {one, one, one, one};
+  const gq_f4 zero = {0.f, 0.f, 0.f, 0.f};
+  auto operands = [&](const gq_u4 &v, gq_u4 (&o)[4], float (&sx)[2][MR]) __attribute__((always_inline)) {
+    o[0] = few_operand<NG, 0>(v);
+    o[1] = few_operand<NG, 1>(v);
+    o[2] = few_operand<NG, 2>(v);
+    o[3] = few_operand<NG, 3>(v);
+#pragma unroll
+    for (int m = 0; m < 2; ++m) {
+      const gq_f4 t = SUMS ? few_mfma<XT>(o[2 * m + 1], ones, few_mfma<XT>(o[2 * m], ones, zero)) : zero;
+#pragma unroll
+      for (int e = 0; e < MR; ++e) sx[m][e] = t[e];
+    }
+  };
+  const int row = lane & 3, xk = 128 * wave + 64 * ((lane >> 3) & 1) + 16 * g + 8 * ((lane >> 2) & 1);
+  auto xin = [&](int i) { return row < M && xk + 128 * kPxWaves * i < K; };  // (whole 32-blocks: a run is wholly in or out)
+  FRaw<XT> raw[NU];
+  auto load_x = [&]() __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < NU; ++i) px_load<XT>(x, xin(i) ? (size_t)row * K + xk + 128 * kPxWaves * i : 0, raw[i]);
+  };
+  auto begin = [&]() __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < NU; ++i) {
+      gq_u4 v = raw[i].v[0];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = xin(i) ? v[e] : 0u;
+      operands(kNibOrder<FMT> ? nib_order(v) : v, ops[i], sums[i]);
+    }
+  };
+  FUnit<FMT> us[NU][2];
+  auto request = [&](int tile, int i) __attribute__((always_inline)) {
+#pragma unroll
+    for (int w = 0; w < 2; ++w)
+      load_unit<FMT>(ftile<FMT>(w ? wu : wg, sc_off, (size_t)tile, tile < ntiles ? C : 0), wave + kPxWaves * i, lane, us[i][w]);
+  };
+  float acc[2][MR] = {};
+  uint32_t mg;  // (kept in a register)
+  if constexpr (XT == GQ_DT_F16) asm volatile("v_mov_b32 %0, 0x64006400" : "=v"(mg));
+  else asm volatile("v_mov_b32 %0, 0x43004300" : "=v"(mg));
+  auto compute = [&](int i) __attribute__((always_inline)) {
+    float s[2][2], mn[2][2];
+#pragma unroll
+    for (int w = 0; w < 2; ++w) few_scales<FMT>(us[i][w], wave, g & (NG - 1), s[w], mn[w]);  // (8 i units on: the same half)
+#pragma unroll
+    for (int m = 0; m < 2; ++m)
+#pragma unroll
+      for (int w = 0; w < 2; ++w) {
+        gq_u4 b[2];
+        few_codes<FMT, XT>(us[i][w], m, mg, b);
+        const gq_f4 d = few_mfma<XT>(ops[i][2 * m + 1], b[1], few_mfma<XT>(ops[i][2 * m], b[0], zero));
+        const float o = FMT == GQ_FMT_Q4_K ? fmaf(s[w][m], OFF, mn[w][m]) : 0.f;
+#pragma unroll
+        for (int v = 0; v < MR; ++v) {
+          if constexpr (FMT == GQ_FMT_Q4_K) acc[w][v] = fmaf(s[w][m], d[v], fmaf(-o, sums[i][m][v], acc[w][v]));
+          else acc[w][v] = fmaf(s[w][m], SUMS ? fmaf(-OFF, sums[i][m][v], d[v]) : d[v], acc[w][v]);
+        }
+      }
+  };
+  auto finish = [&](int tile, int buf) __attribute__((always_inline)) {
+#pragma unroll
+    for (int w = 0; w < 2; ++w)
+#pragma unroll
+      for (int v = 0; v < MR; ++v) {
+        red[buf][wave][w][v][lane] = acc[w][v];
+        acc[w][v] = 0.f;
+      }
+    __syncthreads();
+    front_out<kPxWaves, 1>(
+        [&](int k, int w, int t, int n, int m) {
+          float y = 0.f;
+#pragma unroll
+          for (int i = 0; i < NG; ++i) y += red[buf][k][w][MR == 1 ? 0 : m][16 * i + n];
+          return y;
+        },
+        nullptr, h, go, uo, dt, M, N, act, tile);
+  };
+  walk_tiles<NU>(ntiles, load_x, request, begin, compute, finish);
+}
+
+// Up to 32 rows of any x (the weights of k_front_rows).  x to fp16 with a power-of-two scale per
+// row and wave: the largest of the wave's share of a row is brought into [2^14, 2^15), one rounding
+// to fp16, and the wave's sums are scaled back in fp32 before they are added to the other waves'.
+template <int FMT, int XT, int MT, int NU>
+__global__ void __launch_bounds__(64 * kPxWaves) __attribute__((amdgpu_waves_per_eu(2)))
+k_front_rows_px(const uint8_t *__restrict__ wg, const uint8_t *__restrict__ wu, size_t sc_off, const void *__restrict__ x,
+                void *__restrict__ h, void *__restrict__ go, void *__restrict__ uo, int dt, int M, int N, int K, int C,
+                int units, int act) {
+  __shared__ gq_f4 red[2][kPxWaves][2][MT][64];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int g = lane >> 4, r = lane & 15, ntiles = (int)gq_tiles(N);
+  FUnit<FMT> us[NU][2];
+  auto request = [&](int tile, int i) __attribute__((always_inline)) {
+#pragma unroll
+    for (int w = 0; w < 2; ++w)
+      load_unit<FMT>(ftile<FMT>(w ? wu : wg, sc_off, (size_t)tile, tile < ntiles ? C : 0), wave + kPxWaves * i, lane, us[i][w]);
+  };
+  gq_half8 xs[MT][NU][4];
+  float back[MT][4];  // what undoes the scales of this lane's rows of the result, 16 t + 4 g + v
+  auto xin = [&](int t, int i, int f) {
+    return 16 * t + r < M && 128 * (wave + kPxWaves * i) + 64 * (f >> 1) + 16 * g + 8 * (f & 1) < K;
+  };
+  auto load_run = [&](int t, int i, int f, FRaw<XT> &o) __attribute__((always_inline)) {
+    const int k = 128 * (wave + kPxWaves * i) + 64 * (f >> 1) + 16 * g + 8 * (f & 1);
+    px_load<XT>(x, xin(t, i, f) ? (size_t)(16 * t + r) * K + k : 0, o);
+  };
+  // (as loaded where the registers hold that, else read again for the conversion)
+  constexpr bool ONCE = MT * NU * (XT == GQ_DT_F32 ? 2 : 1) <= 8;
+  FRaw<XT> raw[ONCE ? MT : 1][ONCE ? NU : 1][4];
+  auto load_x = [&]() __attribute__((always_inline)) {
+    if constexpr (ONCE) {
+#pragma unroll
+      for (int t = 0; t < MT; ++t)
+#pragma unroll
+        for (int i = 0; i < NU; ++i)
+#pragma unroll
+          for (int f = 0; f < 4; ++f) load_run(t, i, f, raw[t][i][f]);
+    }
+  };
+  auto run = [&](int t, int i, int f, float (&v)[8]) __attribute__((always_inline)) {
+    if constexpr (ONCE) {
+      px_floats<XT>(raw[t][i][f], xin(t, i, f), v);
+    } else {
+      FRaw<XT> o;
+      load_run(t, i, f, o);
+      px_floats<XT>(o, xin(t, i, f), v);
+    }
+  };
+  auto begin = [&]() __attribute__((always_inline)) {
+#pragma unroll
+    for (int t = 0; t < MT; ++t) {
+      float top = 0.f;
+#pragma unroll
+      for (int i = 0; i < NU; ++i)
+#pragma unroll
+        for (int f = 0; f < 4; ++f) {
+          float v[8];
+          run(t, i, f, v);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(v[e]));
+        }
+      top = fmaxf(top, __shfl_xor(top, 16, 64));
+      top = fmaxf(top, __shfl_xor(top, 32, 64));
+      // 2^s, s = 14 - floor(log2(top)) cut to +-100 (0, Inf: any)
+      const int sh = 14 + 127 - (int)((__float_as_uint(top) >> 23) & 0xFFu), cut = sh < -100 ? -100 : sh > 100 ? 100 : sh;
+      const float f2 = __uint_as_float((uint32_t)(127 + cut) << 23), inv = __uint_as_float((uint32_t)(127 - cut) << 23);
+#pragma unroll
+      for (int v = 0; v < 4; ++v) back[t][v] = __shfl(inv, 4 * g + v, 64);
+#pragma unroll
+      for (int i = 0; i < NU; ++i)
+#pragma unroll
+        for (int f = 0; f < 4; ++f) {
+          float v[8];
+          run(t, i, f, v);
+          constexpr int perm[8] = {0, 2, 4, 6, 1, 3, 5, 7};  // the nibbles' order, their 16 x divided out
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            xs[t][i][f][e] = (_Float16)(kNibOrder<FMT> ? ((e & 2) ? v[perm[e]] * 0.0625f : v[perm[e]]) * f2 : v[e] * f2);
+        }
+    }
+  };
+  gq_f4 acc[2][MT];
+#pragma unroll
+  for (int w = 0; w < 2; ++w)
+#pragma unroll
+    for (int t = 0; t < MT; ++t) acc[w][t] = gq_f4{0.f, 0.f, 0.f, 0.f};
+  const uint32_t mg = gq_nib_magic();
+  auto compute = [&](int i) __attribute__((always_inline)) {
+#pragma unroll
+    for (int w = 0; w < 2; ++w) {
+      gq_half8 b[2][2];
+      rows_frags<FMT>(us[i][w], wave, g, mg, b);  // (8 i units on: the same half of a super-block)
+#pragma unroll
+      for (int t = 0; t < MT; ++t)
+#pragma unroll
+        for (int f = 0; f < 4; ++f) acc[w][t] = gq_mfma16(xs[t][i][f], b[f >> 1][f & 1], acc[w][t]);
+    }
+  };
+  auto finish = [&](int tile, int buf) __attribute__((always_inline)) {
+#pragma unroll
+    for (int w = 0; w < 2; ++w)
+#pragma unroll
+      for (int t = 0; t < MT; ++t) {
+#pragma unroll
+        for (int v = 0; v < 4; ++v) acc[w][t][v] *= back[t][v];
+        red[buf][wave][w][t][lane] = acc[w][t];
+        acc[w][t] = gq_f4{0.f, 0.f, 0.f, 0.f};
+      }
+    __syncthreads();
+    front_out<kPxWaves, 1>(
+        [&](int k, int w, int t, int n, int m) {
+          return reinterpret_cast<const float *>(&red[buf][k][w][m >> 4][16 * ((m >> 2) & 3) + n])[m & 3];
+        },
+        nullptr, h, go, uo, dt, M, N, act, tile);
+  };
+  walk_tiles<NU>(ntiles, load_x, request, begin, compute, finish);
 }
 
 // ---- forward: register-B tiles ---------------------------------------------------
@@ -717,27 +988,82 @@ int launch_front_rb(const void *wg, const void *wu, const _Float16 *a16, int lda
 template <int FMT, int XT>
 int launch_front_few_t(const void *wg, const void *wu, const void *x, const float *rs, void *h, void *go, void *uo, int dt,
                        int M, int N, int K, int act, hipStream_t s) {
-#ifndef FKS
-#define FKS 4
-#define FRS 4
-#endif
   const int units = (int)(gq_kpad(FMT, K) / 128);
 #define GQ_FEW(MR, R, KS)                                                                                             \
   hipLaunchKernelGGL((k_front_few<FMT, XT, MR, R, KS>), dim3((unsigned)((gq_tiles(N) + (R)-1) / (R))), dim3(64 * (KS)), 0, s, \
                      (const uint8_t *)wg, (const uint8_t *)wu, gq_sc_plane_offset(FMT, N, K), x, rs, h, go, uo, dt, M, N, K,  \
                      (int)gq_chunks(FMT, K), units, act)
-#ifdef GQ_TUNE
-  if (getenv("GQ_R2")) {
-  if (M == 1) GQ_FEW(1, 2, FKS);
-  else GQ_FEW(4, 2, FKS);
-  return 0;
-  }
-#endif
-  if (M == 1) GQ_FEW(1, 1, FKS);
-  else GQ_FEW(4, 1, FKS);
+  const size_t tiles = gq_tiles(N);
+#define GQ_FEW_M(R, KS)          \
+  do {                           \
+    if (M == 1) GQ_FEW(1, R, KS); \
+    else GQ_FEW(4, R, KS);       \
+  } while (0)
+  // (14336 x 4096 Q4_K one row: 17.6 us by one tile, 16.9 by two; 4096 x 4096 7.3 and 10.1)
+  if (tiles <= 256) GQ_FEW_M(1, 8);
+  else if (tiles <= 448) GQ_FEW_M(1, 4);
+  else GQ_FEW_M(2, 4);
+#undef GQ_FEW_M
 #undef GQ_FEW
   return gq_last_launch();
 }
+// x in registers (K <= 8192): any dtype and alignment of x, no workspace
+template <int FMT, int XT, int NU>
+int launch_front_px_n(const void *wg, const void *wu, const void *x, void *h, void *go, void *uo, int dt, int M, int N,
+                      int K, int act, hipStream_t s) {
+  const int tiles = (int)gq_tiles(N), cus = gq_device_cus();
+  const int C = (int)gq_chunks(FMT, K), units = (int)(gq_kpad(FMT, K) / 128);
+  const size_t so = gq_sc_plane_offset(FMT, N, K);
+  const uint8_t *g8 = (const uint8_t *)wg, *u8 = (const uint8_t *)wu;
+    const dim3 grid((unsigned)(cus > 0 && tiles > cus ? cus : tiles)), block(64 * kPxWaves);
+#define GQ_PX(KERN) hipLaunchKernelGGL(KERN, grid, block, 0, s, g8, u8, so, x, h, go, uo, dt, M, N, K, C, units, act)
+  if constexpr (XT != GQ_DT_F32) {
+    if (M == 1) {
+      GQ_PX((k_front_few_px<FMT, XT, 1, NU>));
+      return gq_last_launch();
+    }
+    if (M <= 4) {
+      GQ_PX((k_front_few_px<FMT, XT, 4, NU>));
+      return gq_last_launch();
+    }
+  }
+  if (M <= 16) {
+    GQ_PX((k_front_rows_px<FMT, XT, 1, NU>));
+  } else {
+    if constexpr (NU <= 2) GQ_PX((k_front_rows_px<FMT, XT, 2, NU>));
+  }
+#undef GQ_PX
+  return gq_last_launch();
+}
+template <int FMT, int XT>
+int launch_front_px_t(const void *wg, const void *wu, const void *x, void *h, void *go, void *uo, int dt, int M, int N,
+                      int K, int act, hipStream_t s) {
+  const size_t units = gq_kpad(FMT, K) / 128;
+  if (units <= kPxWaves) return launch_front_px_n<FMT, XT, 1>(wg, wu, x, h, go, uo, dt, M, N, K, act, s);
+  if (units <= 2 * kPxWaves) return launch_front_px_n<FMT, XT, 2>(wg, wu, x, h, go, uo, dt, M, N, K, act, s);
+  return launch_front_px_n<FMT, XT, 4>(wg, wu, x, h, go, uo, dt, M, N, K, act, s);
+}
+template <int FMT>
+int launch_front_px_x(const void *wg, const void *wu, const void *x, int xt, void *h, void *go, void *uo, int dt, int M,
+                      int N, int K, int act, hipStream_t s) {
+  if (xt == GQ_DT_F32) return launch_front_px_t<FMT, GQ_DT_F32>(wg, wu, x, h, go, uo, dt, M, N, K, act, s);
+  if (xt == GQ_DT_F16) return launch_front_px_t<FMT, GQ_DT_F16>(wg, wu, x, h, go, uo, dt, M, N, K, act, s);
+  return launch_front_px_t<FMT, GQ_DT_BF16>(wg, wu, x, h, go, uo, dt, M, N, K, act, s);
+}
+// Up to 16 rows of K <= 4096, and 32 of K <= 2048 (with more units the registers spill: 16 rows of
+// 8192 x 8192 Q4_K 40.6 us, x read for every tile 28.3; one row 20.0 and 18.6)
+bool front_px(int fmt, size_t M, size_t K) {
+  const size_t units = gq_kpad(fmt, K) / 128;
+  return M <= 16 ? units <= 4 * kPxWaves : M <= 32 && units <= 2 * kPxWaves;
+}
+int launch_front_px(int fmt, const void *wg, const void *wu, const void *x, int xt, void *h, void *go, void *uo, int dt,
+                    int M, int N, int K, int act, hipStream_t s) {
+  if (fmt == GQ_FMT_Q4_0) return launch_front_px_x<GQ_FMT_Q4_0>(wg, wu, x, xt, h, go, uo, dt, M, N, K, act, s);
+  if (fmt == GQ_FMT_Q8_0) return launch_front_px_x<GQ_FMT_Q8_0>(wg, wu, x, xt, h, go, uo, dt, M, N, K, act, s);
+  if (gq_fmt_is_q6k(fmt)) return launch_front_px_x<GQ_FMT_Q6_K>(wg, wu, x, xt, h, go, uo, dt, M, N, K, act, s);
+  return launch_front_px_x<GQ_FMT_Q4_K>(wg, wu, x, xt, h, go, uo, dt, M, N, K, act, s);
+}
+
 // x of xt (f16 or bf16), 4-byte aligned
 int launch_front_few(int fmt, const void *wg, const void *wu, const void *x, int xt, const float *rs, void *h, void *go,
                      void *uo, int dt, int M, int N, int K, int act, hipStream_t s) {
@@ -758,15 +1084,10 @@ int launch_front_rows_t(const void *wg, const void *wu, const _Float16 *a16, int
   hipLaunchKernelGGL((k_front_rows<FMT, MT, R, KS>), dim3((unsigned)((gq_tiles(N) + (R)-1) / (R))), dim3(64 * (KS)), 0, s, \
                      (const uint8_t *)wg, (const uint8_t *)wu, gq_sc_plane_offset(FMT, N, K), a16, lda, rs, h, go, uo, dt, \
                      M, N, (int)gq_chunks(FMT, K), units, act)
-#ifdef GQ_TUNE
-  if (getenv("GQ_R2")) {
-  if (M <= 16) GQ_ROWS(1, 2, FRS);
-  else GQ_ROWS(2, 2, FRS);
-  return 0;
-  }
-#endif
-  if (M <= 16) GQ_ROWS(1, 1, FRS);
-  else GQ_ROWS(2, 1, FRS);
+  // (as k_front_few; 17..32 rows by one tile, the host sends large N to the tiled kernel)
+  if (M > 16) GQ_ROWS(2, 1, 4);
+  else if (gq_tiles(N) <= 448) GQ_ROWS(1, 1, 4);
+  else GQ_ROWS(1, 2, 4);
 #undef GQ_ROWS
   return gq_last_launch();
 }
@@ -781,21 +1102,14 @@ template <int FMT>
 int launch_front_fmt(const void *wg, const void *wu, const _Float16 *a16, int lda, const float *rs, void *h, void *go,
                      void *uo, int dt, int M, int N, int K, int act, hipStream_t s) {
 #define GQ_FRONT(...) launch_front_rb<FMT, __VA_ARGS__>(wg, wu, a16, lda, rs, h, go, uo, dt, M, N, K, act, s)
-#ifdef GQ_TUNE
-  const char *e = getenv("GQ_FT");
-  switch (e ? atoi(e) : 0) {
-  case 1: return GQ_FRONT(128, 1, 4, 1, 2, 1);
-  case 2: return GQ_FRONT(128, 1, 4, 1, 3, 2);
-  case 3: return GQ_FRONT(64, 1, 4, 1, 3, 2);
-  case 4: return GQ_FRONT(64, 1, 2, 1, 3, 4);
-  case 5: return GQ_FRONT(32, 1, 2, 1, 4, 4);
-  case 6: return GQ_FRONT(32, 1, 4, 1, 4, 4);
-  case 7: return GQ_FRONT(64, 1, 2, 1, 4, 4);
-  default: break;
-  }
-#endif
   auto wgs = [&](int bm, int bn) { return (size_t)((M + bm - 1) / bm) * (size_t)((N + bn - 1) / bn); };
   const int nsteps = (int)(gq_kpad(FMT, K) / BK);
+  // About one workgroup per CU first, with K groups where the tiles alone give fewer waves
+  // (Q4_K, K = 4096, us by 32 x 64 / 64 x 64 / 64 x 128 / 128 x 128 tiles: 32 x 14336 24.5 / 30.8 / 39.7 / -,
+  // 64 x 14336 43.0 / 31.2 / 40.6 / 57.2, 128 x 14336 79.5 / 56.3 / 46.3 / 57.8, 256 x 4096 - / 31.5 / 40.6 / 56.2); 128
+  // x 128 without groups, two workgroups a CU, for the rest: 2048 x 14336 450 us (with K groups 492,
+  // 256 x 128 on 8 waves 470, on 4 waves of 256 rows 503)
+  if (M <= 32 && nsteps % 4 == 0) return GQ_FRONT(32, 1, 2, 1, 4, 4);
   if (wgs(64, 64) <= 288 && nsteps % 4 == 0) return GQ_FRONT(64, 1, 2, 1, 3, 4);
   if (wgs(64, 128) <= 288) return GQ_FRONT(64, 1, 4, 1, 3, 2);
   if (wgs(128, 128) <= 288) return GQ_FRONT(128, 1, 4, 1, 3, 2);
@@ -853,6 +1167,8 @@ extern "C" int gq_ffn_gate_up(int fmt, const void *gate, const void *up, const v
   GQ_CHECK(K > 0, GQ_ERR_INVALID_ARGS);
   GQ_CHECK(N * 256 * gq_dtype_size(h_dtype) < ((size_t)1 << 31), GQ_ERR_INVALID_ARGS);  // (a tile's rows of outputs)
   hipStream_t s = (hipStream_t)stream;
+  if (front_px(fmt, M, K))
+    return launch_front_px(fmt, gate, up, x, x_dtype, h, g, u, h_dtype, (int)M, (int)N, (int)K, act, s);
   if (front_as_it_is(x, x_dtype, M))
     return launch_front_few(fmt, gate, up, x, x_dtype, nullptr, h, g, u, h_dtype, (int)M, (int)N, (int)K, act, s);
   const size_t need = gq_ffn_gate_up_workspace_bytes(fmt, M, N, K), mb = front_rows(fmt, M, K), Kp = gq_kpad(fmt, K);
@@ -867,7 +1183,7 @@ extern "C" int gq_ffn_gate_up(int fmt, const void *gate, const void *up, const v
     GQ_TRY(gq_launch_a_to_f16(x, x_dtype, a16, rs, (int)M, (int)K, (int)K, 0, s));
     return launch_front_few(fmt, gate, up, a16, GQ_DT_F16, rs, h, g, u, h_dtype, (int)M, (int)N, (int)K, act, s);
   }
-  if (M <= 32) {  // rows 16 bytes longer than a multiple of 4 KiB, where 16 of them would collide
+  if (M <= 16 || (M <= 32 && gq_tiles(N) <= 400)) {  // rows 16 bytes longer than a multiple of 4 KiB, where 16 of them would collide
     const int ld = (int)Kp + 8;
     GQ_TRY(gq_launch_a_to_f16(x, x_dtype, a16, rs, (int)M, (int)K, ld, q4, s));
     return launch_front_rows(fmt, gate, up, a16, ld, rs, h, g, u, h_dtype, (int)M, (int)N, (int)K, act, s);
