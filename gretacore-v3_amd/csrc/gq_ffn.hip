@@ -9,34 +9,6 @@
 
 namespace {
 
-// One weight of a T16 tensor, dequantized in fp32.
-GQ_DEV float t16_weight(int fmt, const uint8_t *w, size_t sc_off, size_t n, size_t k, size_t C) {
-  const uint8_t *sc = w + sc_off;
-  const size_t blk = k >> 5;
-  const int eh = (int)(k >> 4) & 1, s = (int)k & 15;
-  const int b = 4 * (s >> 3) + (s & 3), sh = 4 * ((s >> 2) & 1);  // the slot's byte and nibble in its code group
-  if (fmt == GQ_FMT_Q4_0) {
-    const int q = (w[gq_q4_0_grp_off(n, blk, eh, C) + b] >> sh) & 15;
-    return (float)(q - 8) * gq_h2f(gq_rd16(sc + gq_q4_0_d_off(n, blk, C)));
-  }
-  if (fmt == GQ_FMT_Q8_0)
-    return (float)(int8_t)w[gq_q8_0_half_off(n, blk, eh, C) + s] * gq_h2f(gq_rd16(sc + gq_q4_0_d_off(n, blk, C)));
-  const size_t sb = k >> 8;
-  const int j = (int)blk & 7;
-  if (gq_fmt_is_q6k(fmt)) {
-    const uint32_t hw = *reinterpret_cast<const uint32_t *>(w + gq_q6k_hi_off(n, sb, j, eh, C));
-    const int q = ((w[gq_q6k_grp_off(n, sb, j, eh, C) + b] >> sh) & 15) | (int)(gq_q6k_hi_of(hw, s) << 4);
-    return gq_h2f(gq_rd16(sc + gq_q6k_d_off(n, sb, C))) * (float)(int8_t)sc[gq_q6k_sc_off(n, sb, C) + 2 * j + eh] *
-           (float)(q - 32);
-  }
-  const uint32_t *meta = reinterpret_cast<const uint32_t *>(sc + gq_q4k_meta_off(n, sb, C));
-  const uint32_t mv[4] = {meta[0], meta[1], meta[2], meta[3]};
-  uint32_t a, m;
-  gq_q4k_meta_codes(mv, j, &a, &m);
-  const int q = (w[gq_q4k_grp_off(n, sb, j, eh, C) + b] >> sh) & 15;
-  return gq_h2f(mv[0]) * (float)a * (float)q - gq_h2f(mv[0] >> 16) * (float)m;
-}
-
 // ---- forward: up to 32 rows, units of 128 k ------------------------------------------
 // The weights' bytes bound these.  A workgroup takes R row tiles of both matrices, its KS waves
 // share K unit by unit (wave, wave + KS, ...) with PD units in flight each, and their sums are
@@ -862,6 +834,7 @@ k_front_rb(const uint8_t *__restrict__ wg, const uint8_t *__restrict__ wu, uint3
     if constexpr (PD >= 4)
       if (l + 3 < nl) run_step(l + 3, B3{});
   }
+  __builtin_amdgcn_s_waitcnt(0x0F70);  // (loads of no step still on their way to LDS)
   if constexpr (KG > 1) {
     __shared__ __attribute__((aligned(16))) gq_f4 xs[(KG - 1) * NW * 4 * 64];
 #pragma unroll
@@ -934,45 +907,469 @@ k_front_rb(const uint8_t *__restrict__ wg, const uint8_t *__restrict__ wu, uint3
   else store(std::integral_constant<int, GQ_DT_BF16>{});
 }
 
+// ---- backward --------------------------------------------------------------------
+// dg = dh u act'(g), du = dh act(g): one pass over dh, g, u, a workgroup a row.  The products
+// go out in their own type where they are wanted, and, as they are before that rounding, to fp16
+// [dg | du] with one power-of-two scale per row (the row's largest to [2^14, 2^15)), the A operand of
+// dx, each half padded with zeros to np columns (whole steps of 64).  The first 4096 x 4 columns of a
+// row stay in registers between the maximum and the conversion, the rest is computed twice.
 GQ_DEV void front_grads(int act, float dh, float g, float u, float &dg, float &du) {
   float f, d;
   gq_act_fd(act, g, f, d);
   dg = dh * u * d;
   du = dh * f;
 }
-__global__ void __launch_bounds__(256) k_front_dx(int fmt, const uint8_t *gate, const uint8_t *up, size_t sc_off,
-                                                  const void *dh, const void *g, const void *u, int dt, void *dx,
-                                                  int xdt, int M, int N, int K, int C, int act) {
-  __shared__ float as[2][16][17], ws[2][16][17];
-  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-  const int k0 = 16 * blockIdx.x;
-  for (int m0 = 16 * (int)blockIdx.y; m0 < M; m0 += 16 * (int)gridDim.y) {
-    float s = 0.f;
-    for (int n0 = 0; n0 < N; n0 += 16) {
-      float dg = 0.f, du = 0.f;
-      if (m0 + ty < M && n0 + tx < N) {
-        const size_t i = (size_t)(m0 + ty) * N + n0 + tx;
-        front_grads(act, gq_ld_dt(dh, dt, i), gq_ld_dt(g, dt, i), gq_ld_dt(u, dt, i), dg, du);
-      }
-      as[0][ty][tx] = dg;
-      as[1][ty][tx] = du;
-      ws[0][ty][tx] = n0 + ty < N ? t16_weight(fmt, gate, sc_off, n0 + ty, k0 + tx, C) : 0.f;
-      ws[1][ty][tx] = n0 + ty < N ? t16_weight(fmt, up, sc_off, n0 + ty, k0 + tx, C) : 0.f;
-      __syncthreads();
-      for (int n = 0; n < 16; ++n) s += as[0][ty][n] * ws[0][n][tx] + as[1][ty][n] * ws[1][n][tx];
-      __syncthreads();
-    }
-    if (m0 + ty < M) gq_st_dt(dx, xdt, (size_t)(m0 + ty) * K + k0 + tx, s);
+constexpr int kDguThreads = 512, kDguRuns = 4;
+struct __attribute__((packed, aligned(2))) FStore16 {
+  gq_u4 v;
+};
+// 8 values of a row of n from column k on (zeros behind it)
+template <int DT>
+GQ_DEV void dgu_load(const void *p, size_t row, int k, int n, float (&o)[8]) {
+  if (k + 8 <= n) {
+    FRaw<DT> r;
+    px_load<DT>(p, row + k, r);
+    px_floats<DT>(r, true, o);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) o[e] = k + e < n ? gq_ld_dt(p, DT, row + k + e) : 0.f;
   }
 }
-__global__ void __launch_bounds__(256) k_front_dgu(const void *dh, const void *g, const void *u, int dt, void *dgo,
-                                                   void *duo, size_t mn, int act) {
-  for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < mn; i += (size_t)gridDim.x * 256) {
-    float dg, du;
-    front_grads(act, gq_ld_dt(dh, dt, i), gq_ld_dt(g, dt, i), gq_ld_dt(u, dt, i), dg, du);
-    if (dgo) gq_st_dt(dgo, dt, i, dg);
-    if (duo) gq_st_dt(duo, dt, i, du);
+template <int DT>
+GQ_DEV void dgu_store(void *p, size_t row, int k, int n, const float (&v)[8]) {
+  if (k + 8 <= n) {
+    if constexpr (DT == GQ_DT_F32) {
+      FRun32 r;
+      r.v[0] = gq_f4{v[0], v[1], v[2], v[3]};
+      r.v[1] = gq_f4{v[4], v[5], v[6], v[7]};
+      *reinterpret_cast<FRun32 *>(reinterpret_cast<float *>(p) + row + k) = r;
+    } else {
+      FStore16 r;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const uint32_t lo = DT == GQ_DT_BF16 ? gq_f32_to_bf16(v[2 * e]) : __builtin_bit_cast(uint16_t, (_Float16)v[2 * e]);
+        const uint32_t hi =
+            DT == GQ_DT_BF16 ? gq_f32_to_bf16(v[2 * e + 1]) : __builtin_bit_cast(uint16_t, (_Float16)v[2 * e + 1]);
+        r.v[e] = lo | hi << 16;
+      }
+      *reinterpret_cast<FStore16 *>(reinterpret_cast<uint16_t *>(p) + row + k) = r;
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (k + e < n) gq_st_dt(p, DT, row + k + e, v[e]);
   }
+}
+// (no __restrict__: dg may be g, du may be u or dh; every element is read by the thread that writes it, before)
+template <int DT>
+__global__ void __launch_bounds__(kDguThreads) k_front_dgu(const void *dh, const void *g, const void *u, void *dgo, void *duo,
+                                                           _Float16 *a16, float *rs, int N, int np, int act) {
+  __shared__ float top_s[kDguThreads / 64];
+  const int tid = threadIdx.x;
+  const size_t row = (size_t)blockIdx.x * (size_t)N;
+  _Float16 *ar = a16 + (size_t)blockIdx.x * 2 * (size_t)np;
+  float dg[kDguRuns][8], du[kDguRuns][8], top = 0.f;
+  auto grads = [&](int k, float (&a)[8], float (&b)[8]) __attribute__((always_inline)) {
+    float x[8], y[8], z[8];
+    dgu_load<DT>(dh, row, k, N, x);
+    dgu_load<DT>(g, row, k, N, y);
+    dgu_load<DT>(u, row, k, N, z);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) front_grads(act, x[e], y[e], z[e], a[e], b[e]);
+  };
+  auto put = [&](int k, const float (&a)[8], const float (&b)[8]) __attribute__((always_inline)) {
+    if (k >= N) return;
+    if (dgo) dgu_store<DT>(dgo, row, k, N, a);
+    if (duo) dgu_store<DT>(duo, row, k, N, b);
+  };
+#pragma unroll
+  for (int i = 0; i < kDguRuns; ++i) {
+    const int k = 8 * (tid + kDguThreads * i);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) dg[i][e] = du[i][e] = 0.f;
+    if (k < N) grads(k, dg[i], du[i]);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) top = fmaxf(top, fmaxf(fabsf(dg[i][e]), fabsf(du[i][e])));
+  }
+  constexpr int SPAN = 8 * kDguThreads * kDguRuns;
+  if (a16)
+    for (int k = SPAN + 8 * tid; k < N; k += 8 * kDguThreads) {
+      float a[8], b[8];
+      grads(k, a, b);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) top = fmaxf(top, fmaxf(fabsf(a[e]), fabsf(b[e])));
+    }
+  float f2 = 0.f;
+  if (a16) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
+    if ((tid & 63) == 0) top_s[tid >> 6] = top;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kDguThreads / 64; ++w) top = fmaxf(top, top_s[w]);
+    const int sh = 14 + 127 - (int)((__float_as_uint(top) >> 23) & 0xFFu), cut = sh < -100 ? -100 : sh > 100 ? 100 : sh;
+    f2 = __uint_as_float((uint32_t)(127 + cut) << 23);
+    if (tid == 0) rs[blockIdx.x] = __uint_as_float((uint32_t)(127 - cut) << 23);
+  }
+  auto put16 = [&](int k, const float (&a)[8], const float (&b)[8]) __attribute__((always_inline)) {
+    if (!a16 || k >= np) return;
+    gq_half8 x, y;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      x[e] = (_Float16)(a[e] * f2);
+      y[e] = (_Float16)(b[e] * f2);
+    }
+    *reinterpret_cast<gq_half8 *>(ar + k) = x;
+    *reinterpret_cast<gq_half8 *>(ar + np + k) = y;
+  };
+#pragma unroll
+  for (int i = 0; i < kDguRuns; ++i) {
+    const int k = 8 * (tid + kDguThreads * i);
+    put(k, dg[i], du[i]);
+    put16(k, dg[i], du[i]);
+  }
+  for (int k = SPAN + 8 * tid; k < (a16 ? np : N); k += 8 * kDguThreads) {
+    float a[8], b[8];
+    grads(k, a, b);
+    put(k, a, b);
+    put16(k, a, b);
+  }
+}
+
+// dx[m][k] = sum over n of dg[m][n] W_gate[n][k] + du[m][n] W_up[n][k]: the sum runs over the weights'
+// rows, while a T16 record holds 16 rows of 128 k, each row's codes side by side.  Steps of 64 n (four row
+// tiles), gate's before up's.  The records go to LDS as they are (by DMA, the slots of a 64-lane
+// record XOR-swizzled), and a lane collects for its four columns the codes of 8 rows, 16 bits (Q8_0
+// 32) a row: joined in pairs of rows they are masked into fp16 pairs that run along n, B
+// fragments of v_mfma_f32_32x32x16_f16 without a transposition.  Lane c of 32 owns columns
+//   4-bit and Q6_K: 32 (c / 8) + 16 (c / 4 % 2) + 8 (c / 2 % 2) + 2 (c % 2) + {0, 4, 1, 5}  Q8_0: 4 c + {0, 1, 2, 3}
+// of 128, one per fragment; the second and fourth of the former come out 16 x (nibbles masked in place) and
+// the sums are divided by 16 at the end.  Scales vary along n: a wave brings the step's 64 rows'
+// scales to LDS as fp16 [group of columns][16 rows], a lane's 8 rows one 16-byte read.  (Q4_K: d sc and
+// dmin m rounded to fp16 each, then one rounding of their combination.)
+template <int FMT>
+constexpr int kDxGroups = FMT == GQ_FMT_Q6_K ? 8 : 4;  // scale groups of 128 columns
+template <int FMT>
+constexpr int kDxRecs = FMT == GQ_FMT_Q8_0 || FMT == GQ_FMT_Q6_K ? 2 : 1;  // 1 KiB records of 128 columns and a row tile
+template <int FMT>
+constexpr int kDxTables = FMT == GQ_FMT_Q4_K ? 2 : 1;
+
+// scales of row r (of a tile) for 128 columns, as loaded
+template <int FMT>
+GQ_DEV gq_u4 dx_load_scales(const __amdgpu_buffer_rsrc_t &w, uint32_t sc_off, uint32_t tc, uint32_t p, uint32_t r, bool in) {
+  const uint32_t o = in ? sc_off + tc * HFmt<FMT>::SB : 0xFFFFF000u;  // (outside: zeros)
+  gq_u4 v = {0, 0, 0, 0};
+  if constexpr (FMT == GQ_FMT_Q4_K) {
+    const auto t = __builtin_amdgcn_raw_buffer_load_b128(w, o + 16u * r, 0, 0);
+    v = gq_u4{t[0], t[1], t[2], t[3]};
+  } else if constexpr (FMT == GQ_FMT_Q6_K) {
+    const auto t = __builtin_amdgcn_raw_buffer_load_b64(w, o + 16u * r + 8u * p, 0, 0);
+    v[0] = t[0];
+    v[1] = t[1];
+    v[2] = __builtin_amdgcn_raw_buffer_load_b16(w, o + 256u + 2u * r, 0, 0);
+  } else {
+    const auto t = __builtin_amdgcn_raw_buffer_load_b64(w, o + 8u * r, 0, 0);
+    v[0] = t[0];
+    v[1] = t[1];
+  }
+  return v;
+}
+// -> the tables [table][group][16 rows] of the row's tile
+template <int FMT>
+GQ_DEV void dx_store_scales(const gq_u4 &v, uint32_t p, int r, _Float16 *t) {
+  constexpr int G = kDxGroups<FMT>;
+  if constexpr (FMT == GQ_FMT_Q4_K) {
+    const float d = (float)bits_h(v[0]), dm = (float)bits_h(v[0] >> 16);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {  // sub-block 4 p + j
+      const uint32_t sh = 16u * p + 8u * (j >> 1), b = ((j & 1) ? v[2] : v[1]) >> sh, m = v[3] >> (sh + 4u * (j & 1));
+      t[16 * j + r] = (_Float16)(d * (float)(b & 63u));
+      t[16 * (G + j) + r] = (_Float16)(-(dm * (float)(((b >> 6) & 3u) | ((m & 15u) << 2))));
+    }
+  } else if constexpr (FMT == GQ_FMT_Q6_K) {
+    const float d = (float)bits_h(v[2]);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) t[16 * j + r] = (_Float16)(d * (float)(int8_t)(v[j >> 2] >> (8 * (j & 3))));
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) t[16 * j + r] = bits_h(v[j & 1] >> (16 * (j >> 1)));  // (d0 d2 | d1 d3)
+  }
+}
+
+template <int FMT, int WM, int WN, int KG, int TM, int PD>
+__global__ void __launch_bounds__(64 * WM * WN * KG)
+__attribute__((amdgpu_waves_per_eu(WM *WN *KG / 4, TM >= 4 ? WM *WN *KG / 4 : 8)))
+k_front_dx(const uint8_t *__restrict__ wg, const uint8_t *__restrict__ wu, uint32_t w_bytes, uint32_t sc_off,
+           const _Float16 *__restrict__ a16, const float *__restrict__ rs, void *__restrict__ y, int dt, int M, int K,
+           int C, int ntiles, int nsteps, int sps, int tiles_m) {
+  constexpr int NW = WM * WN, BM = 32 * TM * WM, BN = 128 * WN, G = kDxGroups<FMT>, RECS = kDxRecs<FMT>, TB = kDxTables<FMT>;
+  constexpr int NREC = 4 * WN * RECS, RPW = (NREC + NW - 1) / NW;  // records a step, per wave
+  static_assert(NREC % NW == 0, "records");
+  constexpr int A_B = BM * BK * 2, W_B = NREC * 1024, S_H = WN * 4 * TB * G * 16, STAGE = A_B + W_B;
+  static_assert(PD == 2 || PD == 3, "pipeline depth");
+  static_assert(KG * PD * (STAGE + 2 * S_H) <= 160 * 1024, "LDS");
+  // an array a stage, and the scales in one of their own: no wait for a DMA into another stage
+  __shared__ __attribute__((aligned(1024))) uint8_t lds_0[KG * STAGE], lds_1[KG * STAGE], lds_2[PD == 3 ? KG * STAGE : 16];
+  __shared__ __attribute__((aligned(16))) _Float16 sc_s[KG * PD * S_H];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int kg = KG == 1 ? 0 : __builtin_amdgcn_readfirstlane((tid >> 6) / NW);
+  const int wave = __builtin_amdgcn_readfirstlane((tid >> 6) % NW);
+  const int wm = wave / WN, wn = wave % WN;
+  int mt, nt;
+  tile_of_g(blockIdx.x, gridDim.x, tiles_m, (K + BN - 1) / BN, 4, mt, nt);
+  const int m0 = mt * BM, kc0 = nt * WN;
+  // this workgroup's steps of 64 n (part blockIdx.y), this group's every KG-th
+  const int s0 = (int)blockIdx.y * sps, s1 = s0 + sps < nsteps ? s0 + sps : nsteps;
+  const int nl = (s1 - s0 + KG - 1) / KG;
+  const int lda = 64 * nsteps;
+  auto stage = [&](int i) { return (i == 0 ? lds_0 : i == 1 ? lds_1 : lds_2) + kg * STAGE; };
+  auto table = [&](int i) { return sc_s + (kg * PD + i) * S_H; };
+  uint32_t ao[BM / (8 * NW)];
+  a_offsets<BM, NW>(lda, M, m0, wave, lane, ao);
+  const __amdgpu_buffer_rsrc_t rg = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t *>(wg), (short)0, (int)w_bytes, 0x00020000);
+  const __amdgpu_buffer_rsrc_t ru = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t *>(wu), (short)0, (int)w_bytes, 0x00020000);
+  // the record's slot a lane fetches: 16 g + (rho ^ 2 g), Q8_0's second half-record (64 k on) ^ 1 more
+  const uint32_t slot = 16u * (16u * (uint32_t)(lane >> 4) + (uint32_t)((lane & 15) ^ (2 * (lane >> 4))));
+  auto step_of = [&](int l) { return s0 + l * KG + kg; };  // (past the part's end: skipped by the sums, A zero or not used)
+  auto request = [&](int l, int st) __attribute__((always_inline)) {
+    int s = step_of(l);
+    s = s < s1 ? s : s1 - 1;
+    load_a_lds_b<BM, NW>(a16, ao, s, wave, reinterpret_cast<_Float16 *>(stage(st)));
+    const bool up = 2 * s >= nsteps;
+    const uint32_t t0 = 4u * (uint32_t)(up ? s - nsteps / 2 : s);
+    uint8_t *wl = stage(st) + A_B;
+#pragma unroll
+    for (int i = 0; i < RPW; ++i) {
+      const int rec = wave * RPW + i;  // [column block][tile][record]
+      const int b = rec / (4 * RECS), t = rec / RECS % 4, h = rec % RECS;
+      const uint32_t kc = (uint32_t)(kc0 + b), c = kSuper<FMT> ? kc >> 1 : kc, p = kSuper<FMT> ? kc & 1u : 0u;
+      uint32_t o = ((t0 + (uint32_t)t) * (uint32_t)C + c) * HFmt<FMT>::QB;
+      uint32_t v = slot;
+      if constexpr (FMT == GQ_FMT_Q8_0) {
+        o += 1024u * (uint32_t)h;
+        v ^= h ? 16u : 0u;
+      } else if constexpr (FMT == GQ_FMT_Q6_K) {
+        o += h ? 2048u : 1024u * p;
+      } else {
+        o += 1024u * p;
+      }
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(up ? ru : rg, (__attribute__((address_space(3))) void *)(wl + 1024 * rec), 16, v,
+                                               o, 0, 0);
+    }
+  };
+  // scales: wave w (below WN) of the group those of column block w, a row a lane
+  const int srow = lane & 15, stile = lane >> 4;
+  auto load_scales = [&](int l) __attribute__((always_inline)) {
+    int s = step_of(l);
+    s = s < s1 ? s : s1 - 1;
+    const bool up = 2 * s >= nsteps;
+    const uint32_t t = 4u * (uint32_t)(up ? s - nsteps / 2 : s) + (uint32_t)stile, kc = (uint32_t)(kc0 + wave);
+    const uint32_t c = kSuper<FMT> ? kc >> 1 : kc;
+    return dx_load_scales<FMT>(up ? ru : rg, sc_off, t * (uint32_t)C + c, kSuper<FMT> ? kc & 1u : 0u, (uint32_t)srow,
+                               t < (uint32_t)ntiles && c < (uint32_t)C);
+  };
+  auto store_scales = [&](const gq_u4 &v, int st) __attribute__((always_inline)) {
+    _Float16 *t = table(st) + (wave * 4 + stile) * (TB * G * 16);
+    dx_store_scales<FMT>(v, kSuper<FMT> ? (uint32_t)(kc0 + wave) & 1u : 0u, srow, t);
+  };
+
+  gq_f16v acc[TM][4];
+#pragma unroll
+  for (int i = 0; i < TM; ++i)
+#pragma unroll
+    for (int f = 0; f < 4; ++f)
+#pragma unroll
+      for (int v = 0; v < 16; ++v) acc[i][f][v] = 0.f;
+  const int c = lane & 31, kh = lane >> 5, sw = a_swz(lane & 31);
+  // where this lane's codes lie in a record: slot group, byte in the slot; its scale group
+  const bool q8 = FMT == GQ_FMT_Q8_0;
+  const int cg = q8 ? (c >> 2) & 3 : 2 * ((c >> 3) & 1) + ((c >> 2) & 1), cm = c >> 4;
+  const int cb = q8 ? 4 * (c & 3) : 8 * cm + 4 * ((c >> 1) & 1) + 2 * (c & 1);
+  const int grp = FMT == GQ_FMT_Q6_K ? 4 * cm + cg : 2 * cm + (cg >> 1);
+  const uint32_t mg = gq_nib_magic();
+  const int par = FMT == GQ_FMT_Q6_K ? (kc0 + wn) & 1 : 0;
+  // byte offset of row 8 kh + e: slot 16 cg + ((8 kh + e) ^ 2 cg ^ (Q8_0: cm))
+  auto row_at = [&](int e) { return 16 * (16 * cg + ((8 * kh + e) ^ (2 * cg) ^ (q8 ? cm : 0))) + (q8 ? 1024 * cm : 0); };
+
+  auto compute = [&](int st) __attribute__((always_inline)) {
+    const _Float16 *As = reinterpret_cast<const _Float16 *>(stage(st)) + (32 * TM * wm + (lane & 31)) * BK;
+    const uint8_t *Ws = stage(st) + A_B + wn * (4 * RECS * 1024);
+    const _Float16 *Ss = table(st) + wn * (4 * TB * G * 16) + 16 * grp + 8 * kh;
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      gq_half8 af[TM];
+#pragma unroll
+      for (int i = 0; i < TM; ++i) af[i] = *reinterpret_cast<const gq_half8 *>(As + 32 * i * BK + 8 * ((2 * t + kh) ^ sw));
+      const gq_half8 d8 = *reinterpret_cast<const gq_half8 *>(Ss + t * (TB * G * 16));
+      gq_half8 m8 = d8;
+      if constexpr (FMT == GQ_FMT_Q4_K) m8 = *reinterpret_cast<const gq_half8 *>(Ss + t * (TB * G * 16) + G * 16);
+      const uint8_t *W = Ws + t * (RECS * 1024) + cb;
+      gq_half8 bf[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {  // rows 2 j, 2 j + 1
+        uint32_t q[4];               // fp16 pairs 1024 + code (4-bit, Q6_K: of the second and fourth 16 x the code)
+        if constexpr (FMT == GQ_FMT_Q8_0) {
+          const uint32_t w0 = *reinterpret_cast<const uint32_t *>(W + row_at(2 * j));
+          const uint32_t w1 = *reinterpret_cast<const uint32_t *>(W + row_at(2 * j + 1));
+#pragma unroll
+          for (int f = 0; f < 4; ++f)
+            q[f] = __builtin_amdgcn_perm(w1, w0, 0x0C040C00u + 0x00010001u * (uint32_t)f) ^ 0x64806480u;
+        } else {
+          const uint32_t lo = *reinterpret_cast<const uint16_t *>(W + row_at(2 * j));
+          const uint32_t hi = *reinterpret_cast<const uint16_t *>(W + row_at(2 * j + 1));
+          const uint32_t v = lo | hi << 16, v8 = v >> 8;
+          q[0] = (v & 0x000F000Fu) | mg;
+          q[1] = (v & 0x00F000F0u) | mg;
+          q[2] = (v8 & 0x000F000Fu) | mg;
+          q[3] = (v8 & 0x00F000F0u) | mg;
+          if constexpr (FMT == GQ_FMT_Q6_K) {
+            // the high fields: bytes 2 hw, 2 hw + 1 of the step's word, the word's half w in bits 4 w .. + 3
+            const uint8_t *H = Ws + t * (RECS * 1024) + 1024 + 4 * (2 * par + cm) + 2 * (c & 1);
+            const uint32_t hl = *reinterpret_cast<const uint16_t *>(H + row_at(2 * j));
+            const uint32_t hh = *reinterpret_cast<const uint16_t *>(H + row_at(2 * j + 1));
+            const uint32_t h = (hl | hh << 16) >> (4 * ((c >> 1) & 1)), h8 = h >> 8;
+            q[0] |= (h << 4) & 0x00300030u;
+            q[1] |= (h << 6) & 0x03000300u;
+            q[2] |= (h8 << 4) & 0x00300030u;
+            q[3] |= (h8 << 6) & 0x03000300u;
+          }
+        }
+        const gq_half2 d2 = {d8[2 * j], d8[2 * j + 1]};
+        gq_half2 m2 = {m8[2 * j], m8[2 * j + 1]}, m16 = m2;
+        if constexpr (FMT == GQ_FMT_Q4_K) m16 = m2 * gq_half2{(_Float16)16.0f, (_Float16)16.0f};
+#pragma unroll
+        for (int f = 0; f < 4; ++f) {
+          const bool x16 = !q8 && (f & 1);
+          const float off = q8                     ? -1152.f
+                            : FMT == GQ_FMT_Q4_0 ? (x16 ? -1152.f : -1032.f)
+                            : FMT == GQ_FMT_Q6_K ? (x16 ? -1536.f : -1056.f)
+                                                 : -1024.f;
+          const gq_half2 o2 = {(_Float16)off, (_Float16)off};
+          gq_half2 r = gq_bits_h2(q[f]) + o2;  // (exact)
+          if constexpr (FMT == GQ_FMT_Q4_K) r = __builtin_elementwise_fma(r, d2, x16 ? m16 : m2);
+          else r = r * d2;
+          bf[f][2 * j] = r[0];
+          bf[f][2 * j + 1] = r[1];
+        }
+      }
+#pragma unroll
+      for (int f = 0; f < 4; ++f)
+#pragma unroll
+        for (int i = 0; i < TM; ++i) acc[i][f] = gq_mfma32(af[i], bf[f], acc[i][f]);
+    }
+  };
+
+  // Step l computes from stage l % PD; the loads of step l + PD - 1 go into the stage step l - 1 has
+  // left, the scales of l + 2 into registers, those of l + 1 to LDS
+  constexpr int ND = BM / (8 * NW) + RPW, pend = (PD - 2) * ND;
+  static_assert(pend <= 63, "vmcnt immediate");
+  constexpr int kWaitPend = 0x0F70 | (pend & 15) | ((pend >> 4) << 14);
+  const bool scales = wave < WN;
+  gq_u4 sv = {0, 0, 0, 0};
+  if (scales) {
+    store_scales(load_scales(0), 0);
+    sv = load_scales(1);
+  }
+#pragma unroll
+  for (int i = 0; i < PD - 1; ++i) request(i, i);
+  __builtin_amdgcn_s_waitcnt(kWaitPend);
+  __syncthreads();
+  for (int l = 0; l < nl; l += PD) {
+#pragma unroll
+    for (int i = 0; i < PD; ++i) {
+      if (l + i >= nl) break;
+      request(l + i + PD - 1, (i + PD - 1) % PD);
+      gq_u4 nv = sv;
+      if (scales) nv = load_scales(l + i + 2);
+      __builtin_amdgcn_sched_barrier(0);
+      // (the last group's step may lie past the part: nothing to add, the barriers are everyone's)
+      if (KG == 1 || step_of(l + i) < s1) compute(i);
+      if (scales) store_scales(sv, (i + 1) % PD);
+      sv = nv;
+      __builtin_amdgcn_s_waitcnt(kWaitPend);
+      __syncthreads();
+    }
+  }
+  __builtin_amdgcn_s_waitcnt(0x0F70);  // (loads of no step still on their way into the stages)
+  if constexpr (KG > 1) {  // the groups' sums through LDS, an MFMA tile at a time, in group order
+    static_assert((KG - 1) * NW * 4096 <= KG * STAGE, "LDS");
+    gq_f4 *xs = reinterpret_cast<gq_f4 *>(lds_0);
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+#pragma unroll
+      for (int f = 0; f < 4; ++f) {
+        gq_f16v &a = acc[i][f];
+        if (kg > 0) {
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+            xs[(((kg - 1) * NW + wave) * 4 + q) * 64 + lane] = gq_f4{a[4 * q], a[4 * q + 1], a[4 * q + 2], a[4 * q + 3]};
+        }
+        __syncthreads();
+        if (kg == 0) {
+#pragma unroll
+          for (int g = 0; g < KG - 1; ++g)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              const gq_f4 t = xs[((g * NW + wave) * 4 + q) * 64 + lane];
+#pragma unroll
+              for (int e = 0; e < 4; ++e) a[4 * q + e] += t[e];
+            }
+        }
+        __syncthreads();
+      }
+    if (kg > 0) return;
+  }
+  // parts: fp32 sums [part][M][K], scaled by k_dx_sum; else dx itself
+  const bool parts = gridDim.y > 1;
+  if (parts) y = reinterpret_cast<float *>(y) + (size_t)blockIdx.y * (size_t)M * (size_t)K;
+  const int k0 = 128 * (kc0 + wn) + (q8 ? 4 * c : 32 * (c >> 3) + 16 * ((c >> 2) & 1) + 8 * ((c >> 1) & 1) + 2 * (c & 1));
+  if (k0 >= K) return;  // (K is whole 32-blocks: a lane's columns are wholly in or out)
+#pragma unroll
+  for (int i = 0; i < TM; ++i)
+#pragma unroll
+    for (int v = 0; v < 16; ++v) {
+      const int m = m0 + 32 * (TM * wm + i) + 8 * (v >> 2) + 4 * kh + (v & 3);
+      if (m >= M) continue;
+      const float s = parts ? 1.f : rs[m], s16 = q8 ? s : s * 0.0625f;
+      const size_t at = (size_t)m * K + k0;
+      // columns k0, k0 + 1 and k0 + 4, + 5 (Q8_0: + 2, + 3)
+      const float o[4] = {acc[i][0][v] * s, q8 ? acc[i][1][v] * s : acc[i][2][v] * s, q8 ? acc[i][2][v] * s : acc[i][1][v] * s16,
+                          acc[i][3][v] * s16};
+      const size_t at2 = at + (q8 ? 2 : 4);
+      if (parts || dt == GQ_DT_F32) {
+        float *p = reinterpret_cast<float *>(y);
+        p[at] = o[0];
+        p[at + 1] = o[1];
+        p[at2] = o[2];
+        p[at2 + 1] = o[3];
+      } else {
+        uint16_t *p = reinterpret_cast<uint16_t *>(y);
+        uint16_t b[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          b[e] = dt == GQ_DT_BF16 ? gq_f32_to_bf16(o[e]) : __builtin_bit_cast(uint16_t, (_Float16)o[e]);
+        p[at] = b[0];
+        p[at + 1] = b[1];
+        p[at2] = b[2];
+        p[at2 + 1] = b[3];
+      }
+    }
+}
+// dx = rs[m] * the parts' sums, in part order
+__global__ void __launch_bounds__(256) k_dx_sum(const float *__restrict__ part, const float *__restrict__ rs, void *__restrict__ y,
+                                                int dt, size_t mk, int K, int parts) {
+  const size_t i = ((size_t)blockIdx.x * 256 + threadIdx.x) * 4;  // (K % 32 == 0: four of one row)
+  if (i >= mk) return;
+  gq_f4 v = *reinterpret_cast<const gq_f4 *>(part + i);
+  for (int p = 1; p < parts; ++p) {
+    const gq_f4 t = *reinterpret_cast<const gq_f4 *>(part + (size_t)p * mk + i);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] += t[e];
+  }
+  const float s = rs[i / (size_t)K];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) gq_st_dt(y, dt, i + e, v[e] * s);
 }
 
 template <int FMT, int BM, int WM, int WN, int NJ, int PD, int KG>
@@ -1119,10 +1516,8 @@ int launch_front_fmt(const void *wg, const void *wu, const _Float16 *a16, int ld
 int launch_front(int fmt, const void *wg, const void *wu, const _Float16 *a16, int lda, const float *rs, void *h, void *go,
                  void *uo, int dt, int M, int N, int K, int act, hipStream_t s) {
   if (fmt == GQ_FMT_Q4_0) return launch_front_fmt<GQ_FMT_Q4_0>(wg, wu, a16, lda, rs, h, go, uo, dt, M, N, K, act, s);
-#ifndef ONLYQ4
   if (fmt == GQ_FMT_Q8_0) return launch_front_fmt<GQ_FMT_Q8_0>(wg, wu, a16, lda, rs, h, go, uo, dt, M, N, K, act, s);
   if (gq_fmt_is_q6k(fmt)) return launch_front_fmt<GQ_FMT_Q6_K>(wg, wu, a16, lda, rs, h, go, uo, dt, M, N, K, act, s);
-#endif
   return launch_front_fmt<GQ_FMT_Q4_K>(wg, wu, a16, lda, rs, h, go, uo, dt, M, N, K, act, s);
 }
 
@@ -1198,7 +1593,93 @@ extern "C" int gq_ffn_gate_up(int fmt, const void *gate, const void *up, const v
   return GQ_OK;
 }
 
-extern "C" size_t gq_ffn_gate_up_bwd_workspace_bytes(int fmt, size_t M, size_t N, size_t K) { return 0; }
+// The backward pass's plan: rows at a time, the kernel's shape and the parts of the sum over n
+namespace {
+struct DxPlan {
+  size_t mb, np;  // rows a block; columns of each half of A
+  int shape, parts, sps;
+};
+struct DxShape {
+  int bm, bn, kg;
+};
+constexpr DxShape kDxShapes[4] = {{32, 128, 4}, {64, 128, 4}, {128, 256, 2}, {256, 256, 1}};
+
+DxPlan dx_plan(size_t M, size_t N, size_t K) {
+  DxPlan p;
+  p.np = (gq_tiles(N) * 16 + 63) & ~(size_t)63;
+  // A below 96 MiB (and 32-bit offsets), whole tiles of rows
+  const size_t fit = (((size_t)96 << 20) / (4 * p.np)) & ~(size_t)255;
+  p.mb = fit < 256 ? 256 : fit;
+  if (M < p.mb) p.mb = M;
+  const size_t nsteps = 2 * p.np / 64;
+  p.shape = p.mb <= 32 ? 0 : p.mb <= 96 ? 1 : 2;
+#ifdef GQ_TUNE
+  if (getenv("GQ_BT")) p.shape = atoi(getenv("GQ_BT")) % 10;
+#endif
+  const DxShape &t = kDxShapes[p.shape];
+  const size_t wgs = ((p.mb + t.bm - 1) / t.bm) * ((K + t.bn - 1) / t.bn);
+  size_t want = wgs >= 192 ? 1 : 256 / wgs;
+#ifdef GQ_TUNE
+  if (getenv("GQ_BT") && atoi(getenv("GQ_BT")) >= 10) want = atoi(getenv("GQ_BT")) / 10;
+#endif
+  const size_t most = nsteps / (4 * t.kg);  // at least four steps a group
+  if (want > most) want = most < 1 ? 1 : most;
+  p.sps = (int)((nsteps + want - 1) / want);
+  p.parts = (int)((nsteps + p.sps - 1) / p.sps);
+  // the parts' sums below 64 MiB
+  while (p.parts > 1 && (size_t)p.parts * p.mb * K * 4 > ((size_t)64 << 20)) {
+    p.sps = (int)((nsteps + p.parts - 2) / (p.parts - 1));
+    p.parts = (int)((nsteps + p.sps - 1) / p.sps);
+  }
+  return p;
+}
+size_t dx_a_bytes(const DxPlan &p) { return gq_align256(p.mb * 2 * p.np * 2); }
+size_t dx_rs_bytes(const DxPlan &p) { return gq_align256((p.mb + 256) * 4); }
+size_t dx_bytes(const DxPlan &p, size_t K) {
+  return dx_a_bytes(p) + dx_rs_bytes(p) + (p.parts > 1 ? gq_align256((size_t)p.parts * p.mb * K * 4) : 0);
+}
+
+template <int FMT, int WM, int WN, int KG, int TM, int PD>
+int launch_dx_t(const DxPlan &p, const void *wg, const void *wu, const _Float16 *a16, const float *rs, void *y, int dt, int M,
+                size_t N, size_t K, hipStream_t s) {
+  const int tiles_m = (M + 32 * TM * WM - 1) / (32 * TM * WM), tiles_k = (int)((K + 128 * WN - 1) / (128 * WN));
+  GQ_CHECK((size_t)tiles_m * (size_t)tiles_k <= 0x7FFFFFFFu, GQ_ERR_INVALID_ARGS);  // (one grid dimension)
+  hipLaunchKernelGGL((k_front_dx<FMT, WM, WN, KG, TM, PD>), dim3((unsigned)(tiles_m * tiles_k), (unsigned)p.parts),
+                     dim3(64 * WM * WN * KG), 0, s, (const uint8_t *)wg, (const uint8_t *)wu,
+                     (uint32_t)gq_packed_bytes(FMT, N, K), (uint32_t)gq_sc_plane_offset(FMT, N, K), a16, rs, y, dt, M, (int)K,
+                     (int)gq_chunks(FMT, K), (int)gq_tiles(N), (int)(2 * p.np / 64), p.sps, tiles_m);
+  return gq_last_launch();
+}
+template <int FMT>
+int launch_dx(const DxPlan &p, const void *wg, const void *wu, const _Float16 *a16, const float *rs, void *y, int dt, int M,
+              size_t N, size_t K, hipStream_t s) {
+#define GQ_DX(...) launch_dx_t<FMT, __VA_ARGS__>(p, wg, wu, a16, rs, y, dt, M, N, K, s)
+  switch (p.shape) {
+  case 0: return GQ_DX(1, 1, 4, 1, 3);
+  case 1: return GQ_DX(1, 1, 4, 2, FMT == GQ_FMT_Q8_0 || FMT == GQ_FMT_Q6_K ? 2 : 3);
+  case 2: return GQ_DX(1, 2, 2, 4, FMT == GQ_FMT_Q8_0 || FMT == GQ_FMT_Q6_K ? 2 : 3);
+  default: return GQ_DX(2, 2, 1, 4, 3);
+  }
+#undef GQ_DX
+}
+template <int DT>
+int launch_dgu(const void *dh, const void *g, const void *u, void *dg, void *du, _Float16 *a16, float *rs, int M, int N, int np,
+               int act, hipStream_t s) {
+  hipLaunchKernelGGL(k_front_dgu<DT>, dim3((unsigned)M), dim3(kDguThreads), 0, s, dh, g, u, dg, du, a16, rs, N, np, act);
+  return gq_last_launch();
+}
+}  // namespace
+
+extern "C" size_t gq_ffn_gate_up_bwd_workspace_bytes(int fmt, size_t M, size_t N, size_t K) {
+  if (!gq_fmt_valid(fmt) || M == 0 || M > GQ_MAX_DIM || N > GQ_MAX_DIM || K > GQ_MAX_DIM || K == 0) return 0;
+  // (never less for more rows: a block of fewer rows may have more parts)
+  size_t most = 0;
+  for (size_t m = M; m > 0; m /= 2) {
+    const size_t b = dx_bytes(dx_plan(m, N, K), K);
+    most = b > most ? b : most;
+  }
+  return most;
+}
 
 extern "C" int gq_ffn_gate_up_bwd(int fmt, const void *gate, const void *up, const void *dh, const void *g,
                                   const void *u, int dtype, void *dg, void *du, void *dx, int dx_dtype, size_t M,
@@ -1206,17 +1687,37 @@ extern "C" int gq_ffn_gate_up_bwd(int fmt, const void *gate, const void *up, con
   GQ_TRY(check_front(fmt, gate, up, M, N, K, act));
   GQ_CHECK(gq_dtype_valid(dtype) && gq_dtype_valid(dx_dtype), GQ_ERR_UNSUPPORTED);
   GQ_CHECK(dh && g && u, GQ_ERR_INVALID_ARGS);
-  if (M == 0 || K == 0) return GQ_OK;
-  if (dx) {
-    const dim3 grid((unsigned)(K / 16), (unsigned)(M < 65536 ? (M + 15) / 16 : 4096));
-    hipLaunchKernelGGL(k_front_dx, grid, dim3(256), 0, (hipStream_t)stream, fmt, (const uint8_t *)gate,
-                       (const uint8_t *)up, gq_sc_plane_offset(fmt, N, K), dh, g, u, dtype, dx, dx_dtype, (int)M, (int)N,
-                       (int)K, (int)gq_chunks(fmt, K), act);
-    GQ_TRY(gq_last_launch());
-  }
-  if ((dg || du) && N > 0) {
-    hipLaunchKernelGGL(k_front_dgu, dim3(4096), dim3(256), 0, (hipStream_t)stream, dh, g, u, dtype, dg, du, M * N, act);
-    GQ_TRY(gq_last_launch());
+  if (M == 0 || K == 0 || (!dg && !du && !dx)) return GQ_OK;
+  hipStream_t s = (hipStream_t)stream;
+  const DxPlan plan = dx_plan(M, N, K);
+  const size_t need = dx ? gq_ffn_gate_up_bwd_workspace_bytes(fmt, M, N, K) : 0;
+  GqScratch sc(ws ? 0 : need, s);
+  if (ws) GQ_CHECK(ws_bytes >= need, GQ_ERR_WORKSPACE);
+  else ws = sc.ptr;
+  GQ_CHECK(ws || !dx, GQ_ERR_WORKSPACE);
+  _Float16 *a16 = dx ? (_Float16 *)ws : nullptr;
+  float *rs = dx ? (float *)((uint8_t *)ws + dx_a_bytes(plan)) : nullptr;
+  float *part = dx ? (float *)((uint8_t *)rs + dx_rs_bytes(plan)) : nullptr;
+  const size_t es = gq_dtype_size(dtype) * N, xs = gq_dtype_size(dx_dtype) * K;
+  const size_t step = dx ? plan.mb : (size_t)1 << 20;
+  for (size_t m0 = 0; m0 < M; m0 += step) {
+    const int m = (int)(M - m0 < step ? M - m0 : step);
+    auto at = [&](const void *p) { return p ? (void *)((uint8_t *)p + m0 * es) : nullptr; };
+    if (dtype == GQ_DT_F32) GQ_TRY(launch_dgu<GQ_DT_F32>(at(dh), at(g), at(u), at(dg), at(du), a16, rs, m, (int)N, (int)plan.np, act, s));
+    else if (dtype == GQ_DT_F16) GQ_TRY(launch_dgu<GQ_DT_F16>(at(dh), at(g), at(u), at(dg), at(du), a16, rs, m, (int)N, (int)plan.np, act, s));
+    else GQ_TRY(launch_dgu<GQ_DT_BF16>(at(dh), at(g), at(u), at(dg), at(du), a16, rs, m, (int)N, (int)plan.np, act, s));
+    if (!dx) continue;
+    void *y = (uint8_t *)dx + m0 * xs, *to = plan.parts > 1 ? (void *)part : y;
+    if (fmt == GQ_FMT_Q4_0) GQ_TRY(launch_dx<GQ_FMT_Q4_0>(plan, gate, up, a16, rs, to, dx_dtype, m, N, K, s));
+    else if (fmt == GQ_FMT_Q8_0) GQ_TRY(launch_dx<GQ_FMT_Q8_0>(plan, gate, up, a16, rs, to, dx_dtype, m, N, K, s));
+    else if (gq_fmt_is_q6k(fmt)) GQ_TRY(launch_dx<GQ_FMT_Q6_K>(plan, gate, up, a16, rs, to, dx_dtype, m, N, K, s));
+    else GQ_TRY(launch_dx<GQ_FMT_Q4_K>(plan, gate, up, a16, rs, to, dx_dtype, m, N, K, s));
+    if (plan.parts > 1) {
+      const size_t mk = (size_t)m * K;
+      hipLaunchKernelGGL(k_dx_sum, dim3((unsigned)((mk / 4 + 255) / 256)), dim3(256), 0, s, part, rs, y, dx_dtype, mk, (int)K,
+                         plan.parts);
+      GQ_TRY(gq_last_launch());
+    }
   }
   return GQ_OK;
 }
