@@ -713,6 +713,18 @@ GQ_DEV void front_put(const __amdgpu_buffer_rsrc_t &r, uint32_t vo, uint32_t so,
         dt == GQ_DT_BF16 ? gq_f32_to_bf16(v) : __builtin_bit_cast(uint16_t, (_Float16)v), r, vo, so, 0);
 }
 
+// A step's end.  Waits for this wave's LDS DMAs but the VM youngest loads (which the caller counts) and for its
+// LDS operations, then for the other waves.  __syncthreads would wait for every DMA, those of later
+// steps too: its fence counts them as writes to LDS.
+template <int VM>
+GQ_DEV void step_barrier() {
+  static_assert(VM <= 63, "vmcnt immediate");
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt(0x0070 | (VM & 15) | ((VM >> 4) << 14));  // vmcnt(VM) lgkmcnt(0)
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
 // waves per SIMD: what a workgroup brings, at least two but where the sums of 256 rows take
 // the registers of both
 constexpr int front_wpe(int waves, int bm) { return waves > 4 ? waves / 4 : bm > 128 ? 1 : 2; }
@@ -743,8 +755,6 @@ k_front_rb(const uint8_t *__restrict__ wg, const uint8_t *__restrict__ wu, uint3
   using B3 = std::integral_constant<int, 3>;
   // loads a step may leave in flight: activations of steps s + 2 .. s + PD - 1, weights of s + 2 .. s + PD
   constexpr int NA = BM / (8 * NW), pend = (PD - 2) * NA + (PD - 1) * 2 * kRLoads<FMT> * NJ;
-  static_assert(pend <= 63, "vmcnt immediate");
-  constexpr int kWaitPend = 0x0F70 | (pend & 15) | ((pend >> 4) << 14);
   int mt, nt;
   tile_of_g(blockIdx.x, gridDim.x, tiles_m, (N + BN - 1) / BN, 4, mt, nt);
   const int m0 = mt * BM, n0 = nt * BN, nl = nsteps / KG;
@@ -808,8 +818,7 @@ k_front_rb(const uint8_t *__restrict__ wg, const uint8_t *__restrict__ wu, uint3
     }
     load_rstep<FMT, NJ>(wg, qo, so, s2, st[0][BUF]);
     load_rstep<FMT, NJ>(wu, qo, so, s2, st[1][BUF]);
-    __builtin_amdgcn_s_waitcnt(kWaitPend);
-    __syncthreads();
+    step_barrier<pend>();
   };
   auto prime = [&](auto b) __attribute__((always_inline)) {
     constexpr int i = decltype(b)::value;
@@ -823,9 +832,8 @@ k_front_rb(const uint8_t *__restrict__ wg, const uint8_t *__restrict__ wu, uint3
   prime(B1{});
   if constexpr (PD >= 3) prime(B2{});
   if constexpr (PD >= 4) prime(B3{});
-  __builtin_amdgcn_s_waitcnt(kWaitPend);
   if (tid < BM / 4) *reinterpret_cast<gq_f4 *>(rs_s + 4 * tid) = rs4;
-  __syncthreads();
+  step_barrier<pend>();
   for (int l = 0; l < nl; l += PD) {
     run_step(l, B0{});
     if (l + 1 < nl) run_step(l + 1, B1{});
@@ -1096,25 +1104,22 @@ GQ_DEV void dx_store_scales(const gq_u4 &v, uint32_t p, int r, _Float16 *t) {
   }
 }
 
-template <int FMT, int WM, int WN, int KG, int TM, int PD>
-__global__ void __launch_bounds__(64 * WM * WN * KG)
-__attribute__((amdgpu_waves_per_eu(WM *WN *KG / 4, TM >= 4 ? WM *WN *KG / 4 : 8)))
-k_front_dx(const uint8_t *__restrict__ wg, const uint8_t *__restrict__ wu, uint32_t w_bytes, uint32_t sc_off,
+template <int FMT, int WN, int KG, int TM, int PD>
+__global__ void __launch_bounds__(64 * WN * KG) k_front_dx(const uint8_t *__restrict__ wg, const uint8_t *__restrict__ wu, uint32_t w_bytes, uint32_t sc_off,
            const _Float16 *__restrict__ a16, const float *__restrict__ rs, void *__restrict__ y, int dt, int M, int K,
            int C, int ntiles, int nsteps, int sps, int tiles_m) {
-  constexpr int NW = WM * WN, BM = 32 * TM * WM, BN = 128 * WN, G = kDxGroups<FMT>, RECS = kDxRecs<FMT>, TB = kDxTables<FMT>;
+  constexpr int NW = WN, BM = 32 * TM, BN = 128 * WN, G = kDxGroups<FMT>, RECS = kDxRecs<FMT>, TB = kDxTables<FMT>;
   constexpr int NREC = 4 * WN * RECS, RPW = (NREC + NW - 1) / NW;  // records a step, per wave
   static_assert(NREC % NW == 0, "records");
-  constexpr int A_B = BM * BK * 2, W_B = NREC * 1024, S_H = WN * 4 * TB * G * 16, STAGE = A_B + W_B;
+  constexpr int A_B = BM * BK * 2, W_B = NREC * 1024, S_B = WN * 4 * TB * G * 32, STAGE = A_B + W_B + S_B;
   static_assert(PD == 2 || PD == 3, "pipeline depth");
-  static_assert(KG * PD * (STAGE + 2 * S_H) <= 160 * 1024, "LDS");
-  // an array a stage, and the scales in one of their own: no wait for a DMA into another stage
+  static_assert(KG * PD * STAGE <= 160 * 1024, "LDS");
+  // an array a stage (activations, records, scales): no wait for a DMA into another one
   __shared__ __attribute__((aligned(1024))) uint8_t lds_0[KG * STAGE], lds_1[KG * STAGE], lds_2[PD == 3 ? KG * STAGE : 16];
-  __shared__ __attribute__((aligned(16))) _Float16 sc_s[KG * PD * S_H];
   const int tid = threadIdx.x, lane = tid & 63;
   const int kg = KG == 1 ? 0 : __builtin_amdgcn_readfirstlane((tid >> 6) / NW);
   const int wave = __builtin_amdgcn_readfirstlane((tid >> 6) % NW);
-  const int wm = wave / WN, wn = wave % WN;
+  const int wn = wave;
   int mt, nt;
   tile_of_g(blockIdx.x, gridDim.x, tiles_m, (K + BN - 1) / BN, 4, mt, nt);
   const int m0 = mt * BM, kc0 = nt * WN;
@@ -1123,7 +1128,7 @@ k_front_dx(const uint8_t *__restrict__ wg, const uint8_t *__restrict__ wu, uint3
   const int nl = (s1 - s0 + KG - 1) / KG;
   const int lda = 64 * nsteps;
   auto stage = [&](int i) { return (i == 0 ? lds_0 : i == 1 ? lds_1 : lds_2) + kg * STAGE; };
-  auto table = [&](int i) { return sc_s + (kg * PD + i) * S_H; };
+  auto table = [&](int i) { return reinterpret_cast<_Float16 *>(stage(i) + A_B + W_B); };
   uint32_t ao[BM / (8 * NW)];
   a_offsets<BM, NW>(lda, M, m0, wave, lane, ao);
   const __amdgpu_buffer_rsrc_t rg = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t *>(wg), (short)0, (int)w_bytes, 0x00020000);
@@ -1157,7 +1162,7 @@ k_front_dx(const uint8_t *__restrict__ wg, const uint8_t *__restrict__ wu, uint3
                                                o, 0, 0);
     }
   };
-  // scales: wave w (below WN) of the group those of column block w, a row a lane
+  // scales: a wave those of its own column block, a row a lane
   const int srow = lane & 15, stile = lane >> 4;
   auto load_scales = [&](int l) __attribute__((always_inline)) {
     int s = step_of(l);
@@ -1192,51 +1197,60 @@ k_front_dx(const uint8_t *__restrict__ wg, const uint8_t *__restrict__ wu, uint3
   auto row_at = [&](int e) { return 16 * (16 * cg + ((8 * kh + e) ^ (2 * cg) ^ (q8 ? cm : 0))) + (q8 ? 1024 * cm : 0); };
 
   auto compute = [&](int st) __attribute__((always_inline)) {
-    const _Float16 *As = reinterpret_cast<const _Float16 *>(stage(st)) + (32 * TM * wm + (lane & 31)) * BK;
+    const _Float16 *As = reinterpret_cast<const _Float16 *>(stage(st)) + (lane & 31) * BK;
     const uint8_t *Ws = stage(st) + A_B + wn * (4 * RECS * 1024);
     const _Float16 *Ss = table(st) + wn * (4 * TB * G * 16) + 16 * grp + 8 * kh;
+    // a row tile's operands as they lie in LDS, one tile ahead of the products
+    gq_half8 af[2][TM], d8[2], m8[2];
+    uint32_t cw[2][8], hw[2][8];
+    auto read = [&](int t, int x) __attribute__((always_inline)) {
+      const uint8_t *W = Ws + t * (RECS * 1024) + cb;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        if constexpr (FMT == GQ_FMT_Q8_0) cw[x][e] = *reinterpret_cast<const uint32_t *>(W + row_at(e));
+        else cw[x][e] = *reinterpret_cast<const uint16_t *>(W + row_at(e));
+        // (Q6_K's high fields: bytes 2 hw, 2 hw + 1 of the step's word)
+        if constexpr (FMT == GQ_FMT_Q6_K)
+          hw[x][e] = *reinterpret_cast<const uint16_t *>(Ws + t * (RECS * 1024) + 1024 + 4 * (2 * par + cm) + 2 * (c & 1) + row_at(e));
+      }
+      d8[x] = *reinterpret_cast<const gq_half8 *>(Ss + t * (TB * G * 16));
+      if constexpr (FMT == GQ_FMT_Q4_K) m8[x] = *reinterpret_cast<const gq_half8 *>(Ss + t * (TB * G * 16) + G * 16);
+#pragma unroll
+      for (int i = 0; i < TM; ++i) af[x][i] = *reinterpret_cast<const gq_half8 *>(As + 32 * i * BK + 8 * ((2 * t + kh) ^ sw));
+    };
+    read(0, 0);
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
-      gq_half8 af[TM];
-#pragma unroll
-      for (int i = 0; i < TM; ++i) af[i] = *reinterpret_cast<const gq_half8 *>(As + 32 * i * BK + 8 * ((2 * t + kh) ^ sw));
-      const gq_half8 d8 = *reinterpret_cast<const gq_half8 *>(Ss + t * (TB * G * 16));
-      gq_half8 m8 = d8;
-      if constexpr (FMT == GQ_FMT_Q4_K) m8 = *reinterpret_cast<const gq_half8 *>(Ss + t * (TB * G * 16) + G * 16);
-      const uint8_t *W = Ws + t * (RECS * 1024) + cb;
+      const int x = t & 1;
+      if (t < 3) read(t + 1, x ^ 1);
       gq_half8 bf[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {  // rows 2 j, 2 j + 1
         uint32_t q[4];               // fp16 pairs 1024 + code (4-bit, Q6_K: of the second and fourth 16 x the code)
         if constexpr (FMT == GQ_FMT_Q8_0) {
-          const uint32_t w0 = *reinterpret_cast<const uint32_t *>(W + row_at(2 * j));
-          const uint32_t w1 = *reinterpret_cast<const uint32_t *>(W + row_at(2 * j + 1));
 #pragma unroll
           for (int f = 0; f < 4; ++f)
-            q[f] = __builtin_amdgcn_perm(w1, w0, 0x0C040C00u + 0x00010001u * (uint32_t)f) ^ 0x64806480u;
+            q[f] = __builtin_amdgcn_perm(cw[x][2 * j + 1], cw[x][2 * j], 0x0C040C00u + 0x00010001u * (uint32_t)f) ^ 0x64806480u;
         } else {
-          const uint32_t lo = *reinterpret_cast<const uint16_t *>(W + row_at(2 * j));
-          const uint32_t hi = *reinterpret_cast<const uint16_t *>(W + row_at(2 * j + 1));
-          const uint32_t v = lo | hi << 16, v8 = v >> 8;
+          const uint32_t v = cw[x][2 * j] | cw[x][2 * j + 1] << 16, v8 = v >> 8;
           q[0] = (v & 0x000F000Fu) | mg;
           q[1] = (v & 0x00F000F0u) | mg;
           q[2] = (v8 & 0x000F000Fu) | mg;
           q[3] = (v8 & 0x00F000F0u) | mg;
-          if constexpr (FMT == GQ_FMT_Q6_K) {
-            // the high fields: bytes 2 hw, 2 hw + 1 of the step's word, the word's half w in bits 4 w .. + 3
-            const uint8_t *H = Ws + t * (RECS * 1024) + 1024 + 4 * (2 * par + cm) + 2 * (c & 1);
-            const uint32_t hl = *reinterpret_cast<const uint16_t *>(H + row_at(2 * j));
-            const uint32_t hh = *reinterpret_cast<const uint16_t *>(H + row_at(2 * j + 1));
-            const uint32_t h = (hl | hh << 16) >> (4 * ((c >> 1) & 1)), h8 = h >> 8;
+          if constexpr (FMT == GQ_FMT_Q6_K) {  // (the word's half w in bits 4 w .. + 3 of a byte)
+            const uint32_t h = (hw[x][2 * j] | hw[x][2 * j + 1] << 16) >> (4 * ((c >> 1) & 1)), h8 = h >> 8;
             q[0] |= (h << 4) & 0x00300030u;
             q[1] |= (h << 6) & 0x03000300u;
             q[2] |= (h8 << 4) & 0x00300030u;
             q[3] |= (h8 << 6) & 0x03000300u;
           }
         }
-        const gq_half2 d2 = {d8[2 * j], d8[2 * j + 1]};
-        gq_half2 m2 = {m8[2 * j], m8[2 * j + 1]}, m16 = m2;
-        if constexpr (FMT == GQ_FMT_Q4_K) m16 = m2 * gq_half2{(_Float16)16.0f, (_Float16)16.0f};
+        const gq_half2 d2 = {d8[x][2 * j], d8[x][2 * j + 1]};
+        gq_half2 m2 = d2, m16 = d2;
+        if constexpr (FMT == GQ_FMT_Q4_K) {
+          m2 = gq_half2{m8[x][2 * j], m8[x][2 * j + 1]};
+          m16 = m2 * gq_half2{(_Float16)16.0f, (_Float16)16.0f};
+        }
 #pragma unroll
         for (int f = 0; f < 4; ++f) {
           const bool x16 = !q8 && (f & 1);
@@ -1255,39 +1269,31 @@ k_front_dx(const uint8_t *__restrict__ wg, const uint8_t *__restrict__ wu, uint3
 #pragma unroll
       for (int f = 0; f < 4; ++f)
 #pragma unroll
-        for (int i = 0; i < TM; ++i) acc[i][f] = gq_mfma32(af[i], bf[f], acc[i][f]);
+        for (int i = 0; i < TM; ++i) acc[i][f] = gq_mfma32(af[x][i], bf[f], acc[i][f]);
     }
   };
 
   // Step l computes from stage l % PD; the loads of step l + PD - 1 go into the stage step l - 1 has
-  // left, the scales of l + 2 into registers, those of l + 1 to LDS
-  constexpr int ND = BM / (8 * NW) + RPW, pend = (PD - 2) * ND;
-  static_assert(pend <= 63, "vmcnt immediate");
-  constexpr int kWaitPend = 0x0F70 | (pend & 15) | ((pend >> 4) << 14);
-  const bool scales = wave < WN;
-  gq_u4 sv = {0, 0, 0, 0};
-  if (scales) {
-    store_scales(load_scales(0), 0);
-    sv = load_scales(1);
-  }
+  // left, the scales of l + 2 into registers, those of l + 1 from there to LDS.  At its end the DMA of l + 1
+  // must have landed: of what was issued behind it the scales of l + 2 (l + 1) and later DMAs may be open.
+  constexpr int ND = BM / (8 * NW) + RPW, SL = FMT == GQ_FMT_Q6_K ? 2 : 1, pend = (PD - 2) * ND + (PD - 1) * SL;
+  gq_u4 sv[PD];
+  store_scales(load_scales(0), 0);
+  sv[1] = load_scales(1);
 #pragma unroll
   for (int i = 0; i < PD - 1; ++i) request(i, i);
-  __builtin_amdgcn_s_waitcnt(kWaitPend);
-  __syncthreads();
+  step_barrier<(PD - 2) * ND>();
   for (int l = 0; l < nl; l += PD) {
 #pragma unroll
     for (int i = 0; i < PD; ++i) {
       if (l + i >= nl) break;
       request(l + i + PD - 1, (i + PD - 1) % PD);
-      gq_u4 nv = sv;
-      if (scales) nv = load_scales(l + i + 2);
+      sv[(i + 2) % PD] = load_scales(l + i + 2);
       __builtin_amdgcn_sched_barrier(0);
       // (the last group's step may lie past the part: nothing to add, the barriers are everyone's)
       if (KG == 1 || step_of(l + i) < s1) compute(i);
-      if (scales) store_scales(sv, (i + 1) % PD);
-      sv = nv;
-      __builtin_amdgcn_s_waitcnt(kWaitPend);
-      __syncthreads();
+      store_scales(sv[(i + 1) % PD], (i + 1) % PD);
+      step_barrier<pend>();
     }
   }
   __builtin_amdgcn_s_waitcnt(0x0F70);  // (loads of no step still on their way into the stages)
@@ -1329,7 +1335,7 @@ k_front_dx(const uint8_t *__restrict__ wg, const uint8_t *__restrict__ wu, uint3
   for (int i = 0; i < TM; ++i)
 #pragma unroll
     for (int v = 0; v < 16; ++v) {
-      const int m = m0 + 32 * (TM * wm + i) + 8 * (v >> 2) + 4 * kh + (v & 3);
+      const int m = m0 + 32 * i + 8 * (v >> 2) + 4 * kh + (v & 3);
       if (m >= M) continue;
       const float s = parts ? 1.f : rs[m], s16 = q8 ? s : s * 0.0625f;
       const size_t at = (size_t)m * K + k0;
@@ -1602,13 +1608,13 @@ struct DxPlan {
 struct DxShape {
   int bm, bn, kg;
 };
-constexpr DxShape kDxShapes[4] = {{32, 128, 4}, {64, 128, 4}, {128, 256, 2}, {256, 256, 1}};
+constexpr DxShape kDxShapes[3] = {{32, 128, 4}, {64, 128, 4}, {128, 256, 2}};
 
 DxPlan dx_plan(size_t M, size_t N, size_t K) {
   DxPlan p;
   p.np = (gq_tiles(N) * 16 + 63) & ~(size_t)63;
-  // A below 96 MiB (and 32-bit offsets), whole tiles of rows
-  const size_t fit = (((size_t)96 << 20) / (4 * p.np)) & ~(size_t)255;
+  // A below 120 MiB (and 32-bit offsets), whole tiles of rows
+  const size_t fit = (((size_t)120 << 20) / (4 * p.np)) & ~(size_t)255;
   p.mb = fit < 256 ? 256 : fit;
   if (M < p.mb) p.mb = M;
   const size_t nsteps = 2 * p.np / 64;
@@ -1626,8 +1632,9 @@ DxPlan dx_plan(size_t M, size_t N, size_t K) {
   if (want > most) want = most < 1 ? 1 : most;
   p.sps = (int)((nsteps + want - 1) / want);
   p.parts = (int)((nsteps + p.sps - 1) / p.sps);
-  // the parts' sums below 64 MiB
-  while (p.parts > 1 && (size_t)p.parts * p.mb * K * 4 > ((size_t)64 << 20)) {
+  // all of it below what one scratch block holds
+  const size_t held = gq_align256(p.mb * 4 * p.np) + gq_align256((p.mb + 256) * 4);
+  while (p.parts > 1 && held + (size_t)p.parts * p.mb * K * 4 + 256 > kGqScratchMax) {
     p.sps = (int)((nsteps + p.parts - 2) / (p.parts - 1));
     p.parts = (int)((nsteps + p.sps - 1) / p.sps);
   }
@@ -1639,13 +1646,13 @@ size_t dx_bytes(const DxPlan &p, size_t K) {
   return dx_a_bytes(p) + dx_rs_bytes(p) + (p.parts > 1 ? gq_align256((size_t)p.parts * p.mb * K * 4) : 0);
 }
 
-template <int FMT, int WM, int WN, int KG, int TM, int PD>
+template <int FMT, int WN, int KG, int TM, int PD>
 int launch_dx_t(const DxPlan &p, const void *wg, const void *wu, const _Float16 *a16, const float *rs, void *y, int dt, int M,
                 size_t N, size_t K, hipStream_t s) {
-  const int tiles_m = (M + 32 * TM * WM - 1) / (32 * TM * WM), tiles_k = (int)((K + 128 * WN - 1) / (128 * WN));
+  const int tiles_m = (M + 32 * TM - 1) / (32 * TM), tiles_k = (int)((K + 128 * WN - 1) / (128 * WN));
   GQ_CHECK((size_t)tiles_m * (size_t)tiles_k <= 0x7FFFFFFFu, GQ_ERR_INVALID_ARGS);  // (one grid dimension)
-  hipLaunchKernelGGL((k_front_dx<FMT, WM, WN, KG, TM, PD>), dim3((unsigned)(tiles_m * tiles_k), (unsigned)p.parts),
-                     dim3(64 * WM * WN * KG), 0, s, (const uint8_t *)wg, (const uint8_t *)wu,
+  hipLaunchKernelGGL((k_front_dx<FMT, WN, KG, TM, PD>), dim3((unsigned)(tiles_m * tiles_k), (unsigned)p.parts),
+                     dim3(64 * WN * KG), 0, s, (const uint8_t *)wg, (const uint8_t *)wu,
                      (uint32_t)gq_packed_bytes(FMT, N, K), (uint32_t)gq_sc_plane_offset(FMT, N, K), a16, rs, y, dt, M, (int)K,
                      (int)gq_chunks(FMT, K), (int)gq_tiles(N), (int)(2 * p.np / 64), p.sps, tiles_m);
   return gq_last_launch();
@@ -1655,10 +1662,9 @@ int launch_dx(const DxPlan &p, const void *wg, const void *wu, const _Float16 *a
               size_t N, size_t K, hipStream_t s) {
 #define GQ_DX(...) launch_dx_t<FMT, __VA_ARGS__>(p, wg, wu, a16, rs, y, dt, M, N, K, s)
   switch (p.shape) {
-  case 0: return GQ_DX(1, 1, 4, 1, 3);
-  case 1: return GQ_DX(1, 1, 4, 2, FMT == GQ_FMT_Q8_0 || FMT == GQ_FMT_Q6_K ? 2 : 3);
-  case 2: return GQ_DX(1, 2, 2, 4, FMT == GQ_FMT_Q8_0 || FMT == GQ_FMT_Q6_K ? 2 : 3);
-  default: return GQ_DX(2, 2, 1, 4, 3);
+  case 0: return GQ_DX(1, 4, 1, 3);
+  case 1: return GQ_DX(1, 4, 2, FMT == GQ_FMT_Q8_0 || FMT == GQ_FMT_Q6_K ? 2 : 3);
+  default: return GQ_DX(2, 2, 4, FMT == GQ_FMT_Q8_0 || FMT == GQ_FMT_Q6_K ? 2 : 3);
   }
 #undef GQ_DX
 }
