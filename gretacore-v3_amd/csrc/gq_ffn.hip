@@ -1278,10 +1278,12 @@ __global__ void __launch_bounds__(64 * WN * KG) k_front_dx(const uint8_t *__rest
   // must have landed: of what was issued behind it the scales of l + 2 (l + 1) and later DMAs may be open.
   constexpr int ND = BM / (8 * NW) + RPW, SL = FMT == GQ_FMT_Q6_K ? 2 : 1, pend = (PD - 2) * ND + (PD - 1) * SL;
   gq_u4 sv[PD];
-  store_scales(load_scales(0), 0);
+  const gq_u4 first = load_scales(0);
   sv[1] = load_scales(1);
 #pragma unroll
   for (int i = 0; i < PD - 1; ++i) request(i, i);
+  __builtin_amdgcn_sched_barrier(0);  // (no wait for the scales before all of it is requested)
+  store_scales(first, 0);
   step_barrier<(PD - 2) * ND>();
   for (int l = 0; l < nl; l += PD) {
 #pragma unroll
@@ -1297,33 +1299,35 @@ __global__ void __launch_bounds__(64 * WN * KG) k_front_dx(const uint8_t *__rest
     }
   }
   __builtin_amdgcn_s_waitcnt(0x0F70);  // (loads of no step still on their way into the stages)
-  if constexpr (KG > 1) {  // the groups' sums through LDS, an MFMA tile at a time, in group order
-    static_assert((KG - 1) * NW * 4096 <= KG * STAGE, "LDS");
+  if constexpr (KG > 1) {  // the groups' sums through LDS, a fragment's tiles at a time, in group order
+    static_assert((KG - 1) * NW * TM * 4096 <= KG * STAGE, "LDS");
     gq_f4 *xs = reinterpret_cast<gq_f4 *>(lds_0);
+    auto at = [&](int g, int i, int q) { return (((g * NW + wave) * TM + i) * 4 + q) * 64 + lane; };
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < TM; ++i)
+    for (int f = 0; f < 4; ++f) {
+      if (kg > 0) {
 #pragma unroll
-      for (int f = 0; f < 4; ++f) {
-        gq_f16v &a = acc[i][f];
-        if (kg > 0) {
+        for (int i = 0; i < TM; ++i)
 #pragma unroll
           for (int q = 0; q < 4; ++q)
-            xs[(((kg - 1) * NW + wave) * 4 + q) * 64 + lane] = gq_f4{a[4 * q], a[4 * q + 1], a[4 * q + 2], a[4 * q + 3]};
-        }
-        __syncthreads();
-        if (kg == 0) {
+            xs[at(kg - 1, i, q)] = gq_f4{acc[i][f][4 * q], acc[i][f][4 * q + 1], acc[i][f][4 * q + 2], acc[i][f][4 * q + 3]};
+      }
+      __syncthreads();
+      if (kg == 0) {
 #pragma unroll
-          for (int g = 0; g < KG - 1; ++g)
+        for (int g = 0; g < KG - 1; ++g)
+#pragma unroll
+          for (int i = 0; i < TM; ++i)
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
-              const gq_f4 t = xs[((g * NW + wave) * 4 + q) * 64 + lane];
+              const gq_f4 t = xs[at(g, i, q)];
 #pragma unroll
-              for (int e = 0; e < 4; ++e) a[4 * q + e] += t[e];
+              for (int e = 0; e < 4; ++e) acc[i][f][4 * q + e] += t[e];
             }
-        }
-        __syncthreads();
       }
+      __syncthreads();
+    }
     if (kg > 0) return;
   }
   // parts: fp32 sums [part][M][K], scaled by k_dx_sum; else dx itself

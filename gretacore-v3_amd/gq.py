@@ -529,53 +529,64 @@ def gemv_swiglu_plan(fmt: int, n: int, k: int, batch: int):
 
 
 # ---- gated feed-forward front, 4-bit weights with group scales --------------------
-_dts = None  # torch dtype -> DT_*
+# These calls take whole contiguous tensors on the current device and refuse others.  The checks are few
+# attribute reads (a 4-bit GEMV's kernel runs 4 us); the messages are made only when one fails.
+_dts = {}  # torch dtype -> DT_*
+_empty = _current_device = None
+
+
+def _init_torch():
+    global _empty, _current_device
+    import torch
+    _dts.update({torch.float32: DT_F32, torch.float16: DT_F16, torch.bfloat16: DT_BF16})
+    _empty, _current_device = torch.empty, torch.cuda.current_device
 
 
 def _dt(dtype):
-    global _dts
-    if _dts is None:
-        import torch
-        _dts = {torch.float32: DT_F32, torch.float16: DT_F16, torch.bfloat16: DT_BF16}
+    if not _dts:
+        _init_torch()
     dt = _dts.get(dtype)
     if dt is None:
         raise GQError(f"float32, float16 or bfloat16 expected, not {dtype}")
     return dt
 
 
-def _operand(t, shape, what, dtype=None):
-    """The calls below take whole contiguous tensors on the current device."""
+def _refuse(t, shape, what, dtype):
     if not t.is_cuda:
         raise GQError(f"{what}: device tensor expected (libgq has no CPU path)")
-    if t.shape != shape or not t.is_contiguous():
-        raise GQError(f"{what}: contiguous {list(shape)} expected, not {list(t.shape)} with strides {list(t.stride())}")
+    if t.get_device() != _current_device():
+        raise GQError(f"{what}: on {t.device}, but the current device is {_current_device()}")
     if dtype is not None and t.dtype != dtype:
         raise GQError(f"{what}: {dtype} expected, not {t.dtype}")
+    raise GQError(f"{what}: contiguous {list(shape)} expected, not {list(t.shape)} with strides {list(t.stride())}")
+
+
+def _operand(t, shape, what, device, dtype=None):
+    if t.get_device() != device or t.shape != shape or not t.is_contiguous() or (dtype is not None and t.dtype != dtype):
+        _refuse(t, shape, what, dtype)
 
 
 def _packed_operand(t, nbytes, what, device):
-    if not t.is_cuda or t.device != device:
-        raise GQError(f"{what}: a tensor on {device} expected")
-    if not t.is_contiguous() or t.numel() * t.element_size() < nbytes:
-        raise GQError(f"{what}: {nbytes} contiguous bytes of packed weights expected")
+    if t.get_device() != device or not t.is_contiguous() or t.nbytes < nbytes:
+        raise GQError(f"{what}: {nbytes} contiguous bytes of packed weights on device {device} expected")
 
 
-def _on_current(t):
-    import torch
-    if t.is_cuda and t.device.index != torch.cuda.current_device():
-        raise GQError(f"tensors on {t.device}, but the current device is {torch.cuda.current_device()}")
-
-
-def _front_sizes(x, n, k, what):
-    if x.dim() not in (1, 2):
+def _rows(x, k, what):
+    """(rows, device) of x [k] or [rows][k]"""
+    if _current_device is None:
+        _init_torch()
+    if not x.is_cuda:
+        raise GQError(f"{what}: device tensor expected (libgq has no CPU path)")
+    device, shape = _current_device(), x.shape
+    n = len(shape)
+    if n not in (1, 2):
         raise GQError(f"{what}: [k] or [rows][k] expected")
-    m = 1 if x.dim() == 1 else x.shape[0]
-    _operand(x, (k,) if x.dim() == 1 else (m, k), what)
-    _on_current(x)
-    return m
+    if x.get_device() != device or shape[-1] != k or not x.is_contiguous():
+        _refuse(x, (k,) if n == 1 else (shape[0], k), what, None)
+    return (1 if n == 1 else shape[0]), device
 
 
-_sizes = {}  # packed sizes asked for so far
+_sizes = {}  # sizes asked for so far
 
 
 def _size_of(key, fn, *args):
@@ -593,26 +604,31 @@ def ffn_gate_up(fmt: int, gate, up, x, n: int, k: int, act: int = ACT_SILU, save
                 out_dtype=None, workspace: Workspace | None = None, stream=None):
     """h = act(x Wg^T) * (x Wu^T) over T16 weights, any number of rows of x [m][k] (f32/f16/bf16).  h is of out_dtype
     (default: x's) or the tensor given; with save (or g, u given) the two products come back too: (h, g, u)."""
-    import torch
-    m = _front_sizes(x, n, k, "x")
+    m, device = _rows(x, k, "x")
     dtype = h.dtype if h is not None else out_dtype or x.dtype
     nbytes = _size_of((fmt, n, k), packed_size, fmt, n, k)
-    _packed_operand(gate, nbytes, "gate", x.device)
-    _packed_operand(up, nbytes, "up", x.device)
-    outs = [h, g, u]
-    for i, t in enumerate(outs):
-        if t is not None:
-            _operand(t, (m, n), ("h", "g", "u")[i], dtype)
-            _on_current(t)
-        elif i == 0 or save:
-            outs[i] = torch.empty((m, n), dtype=dtype, device=x.device)
-    h, g, u = outs
+    _packed_operand(gate, nbytes, "gate", device)
+    _packed_operand(up, nbytes, "up", device)
+    if h is None:
+        h = _empty((m, n), dtype=dtype, device=x.device)
+    else:
+        _operand(h, (m, n), "h", device)
+    if g is not None:
+        _operand(g, (m, n), "g", device, dtype)
+    elif save:
+        g = _empty((m, n), dtype=dtype, device=x.device)
+    if u is not None:
+        _operand(u, (m, n), "u", device, dtype)
+    elif save:
+        u = _empty((m, n), dtype=dtype, device=x.device)
     ws_ptr, ws_n = None, 0
     if workspace is not None:
-        buf = workspace.ensure(ffn_gate_up_workspace_bytes(fmt, m, n, k))
-        ws_ptr, ws_n = _ptr(buf), buf.numel()
-    check(load().gq_ffn_gate_up(fmt, _ptr(gate), _ptr(up), _ptr(x), _dt(x.dtype), _ptr(h), _dt(dtype), _ptr(g), _ptr(u), m,
-                                n, k, act, ws_ptr, ws_n, _stream(stream)), "gq_ffn_gate_up")
+        buf = workspace.ensure(_size_of((fmt, m, n, k, "front"), ffn_gate_up_workspace_bytes, fmt, m, n, k))
+        ws_ptr, ws_n = buf.data_ptr(), buf.numel()
+    st = load().gq_ffn_gate_up(fmt, gate.data_ptr(), up.data_ptr(), x.data_ptr(), _dt(x.dtype), h.data_ptr(), _dt(dtype),
+                               _ptr(g), _ptr(u), m, n, k, act, ws_ptr, ws_n, _stream(stream))
+    if st:
+        check(st, "gq_ffn_gate_up")
     return h if g is None and u is None else (h, g, u)
 
 
@@ -625,34 +641,34 @@ def ffn_gate_up_bwd(fmt: int, gate, up, dh, g, u, n: int, k: int, act: int = ACT
                     stream=None):
     """Gradients of ffn_gate_up with the weights frozen: {"dx", "dg", "du"} for dh [m][n] and the g, u it saved.  dg and
     du are the gradients of the two projections, None where not wanted."""
-    import torch
-    m = _front_sizes(dh, k, n, "dh")
+    m, device = _rows(dh, n, "dh")
     dtype = dh.dtype
-    for t, what in ((g, "g"), (u, "u")):
-        _operand(t, dh.shape, what, dtype)
+    _operand(g, dh.shape, "g", device, dtype)
+    _operand(u, dh.shape, "u", device, dtype)
     nbytes = _size_of((fmt, n, k), packed_size, fmt, n, k)
-    _packed_operand(gate, nbytes, "gate", dh.device)
-    _packed_operand(up, nbytes, "up", dh.device)
+    _packed_operand(gate, nbytes, "gate", device)
+    _packed_operand(up, nbytes, "up", device)
     if dx is not None:
-        _operand(dx, (m, k), "dx")
+        _operand(dx, (m, k), "dx", device)
     elif want_dx:
-        dx = torch.empty((m, k), dtype=dx_dtype or dtype, device=dh.device)
-    for t, what in ((dg, "dg"), (du, "du")):
-        if t is not None:
-            _operand(t, (m, n), what, dtype)
-    if want_dgu:
-        dg = torch.empty((m, n), dtype=dtype, device=dh.device) if dg is None else dg
-        du = torch.empty((m, n), dtype=dtype, device=dh.device) if du is None else du
-    for t in (g, u, dx, dg, du):
-        if t is not None:
-            _on_current(t)
+        dx = _empty((m, k), dtype=dx_dtype or dtype, device=dh.device)
+    if dg is not None:
+        _operand(dg, (m, n), "dg", device, dtype)
+    elif want_dgu:
+        dg = _empty((m, n), dtype=dtype, device=dh.device)
+    if du is not None:
+        _operand(du, (m, n), "du", device, dtype)
+    elif want_dgu:
+        du = _empty((m, n), dtype=dtype, device=dh.device)
     ws_ptr, ws_n = None, 0
     if workspace is not None:
-        buf = workspace.ensure(ffn_gate_up_bwd_workspace_bytes(fmt, m, n, k))
-        ws_ptr, ws_n = _ptr(buf), buf.numel()
-    check(load().gq_ffn_gate_up_bwd(fmt, _ptr(gate), _ptr(up), _ptr(dh), _ptr(g), _ptr(u), _dt(dtype), _ptr(dg), _ptr(du),
-                                    _ptr(dx), _dt(dx.dtype if dx is not None else dtype), m, n, k, act, ws_ptr, ws_n,
-                                    _stream(stream)), "gq_ffn_gate_up_bwd")
+        buf = workspace.ensure(_size_of((fmt, m, n, k, "bwd"), ffn_gate_up_bwd_workspace_bytes, fmt, m, n, k))
+        ws_ptr, ws_n = buf.data_ptr(), buf.numel()
+    st = load().gq_ffn_gate_up_bwd(fmt, gate.data_ptr(), up.data_ptr(), dh.data_ptr(), g.data_ptr(), u.data_ptr(), _dt(dtype),
+                                   _ptr(dg), _ptr(du), _ptr(dx), _dt(dx.dtype if dx is not None else dtype), m, n, k, act,
+                                   ws_ptr, ws_n, _stream(stream))
+    if st:
+        check(st, "gq_ffn_gate_up_bwd")
     return {"dx": dx, "dg": dg, "du": du}
 
 
@@ -666,15 +682,14 @@ def w4_pack(q, scales, zeros, n: int, k: int, group: int, stream=None):
     """4-bit rows q uint8 [n][ceil(k/2)] (even k in the low nibble), scales f16/bf16 and zeros uint8 (None: 8)
     [n][ceil(k/group)] -> the packed weights of w4_gemv / w4_gate_up."""
     import torch
-    ng = -(-k // group) if group > 0 else 0
     nbytes = w4_packed_size(n, k, group)
-    _operand(q, (n, -(-k // 2)), "q", torch.uint8)
-    _operand(scales, (n, ng), "scales")
+    ng = -(-k // group)
+    _dt(scales.dtype)
+    device = _current_device() if q.is_cuda else -2
+    _operand(q, (n, -(-k // 2)), "q", device, torch.uint8)
+    _operand(scales, (n, ng), "scales", device)
     if zeros is not None:
-        _operand(zeros, (n, ng), "zeros", torch.uint8)
-    for t in (q, scales, zeros):
-        if t is not None:
-            _on_current(t)
+        _operand(zeros, (n, ng), "zeros", device, torch.uint8)
     out = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
     check(load().gq_w4_pack(_ptr(q), _ptr(scales), _dt(scales.dtype), _ptr(zeros), n, k, group, _ptr(out),
                             _stream(stream)), "gq_w4_pack")
@@ -684,33 +699,33 @@ def w4_pack(q, scales, zeros, n: int, k: int, group: int, stream=None):
 def w4_gemv(w, group: int, x, n: int, k: int, y=None, out_dtype=None, stream=None):
     """y[b][n] = sum_k x[b][k] * W[n][k] over w4_pack's weights; x f32/f16/bf16 [k] or [1..16][k], y of out_dtype
     (default: x's) or the tensor given."""
-    import torch
-    m = _front_sizes(x, n, k, "x")
-    _packed_operand(w, _size_of((n, k, group, "w4"), w4_packed_size, n, k, group), "w", x.device)
+    m, device = _rows(x, k, "x")
+    _packed_operand(w, _size_of((n, k, group, "w4"), w4_packed_size, n, k, group), "w", device)
     if y is None:
-        y = torch.empty((m, n), dtype=out_dtype or x.dtype, device=x.device)
+        y = _empty((m, n), dtype=out_dtype or x.dtype, device=x.device)
     else:
-        _operand(y, (m, n), "y")
-        _on_current(y)
-    check(load().gq_w4_gemv(_ptr(w), group, _ptr(x), _dt(x.dtype), _ptr(y), _dt(y.dtype), n, k, m, _stream(stream)),
-          "gq_w4_gemv")
+        _operand(y, (m, n), "y", device)
+    st = load().gq_w4_gemv(w.data_ptr(), group, x.data_ptr(), _dt(x.dtype), y.data_ptr(), _dt(y.dtype), n, k, m,
+                           _stream(stream))
+    if st:
+        check(st, "gq_w4_gemv")
     return y
 
 
 def w4_gate_up(gate, up, group: int, x, n: int, k: int, act: int = ACT_SILU, h=None, out_dtype=None, stream=None):
     """h = act(x Wg^T) * (x Wu^T) over two matrices of w4_pack, 1..16 rows of x, in one launch."""
-    import torch
-    m = _front_sizes(x, n, k, "x")
+    m, device = _rows(x, k, "x")
     nbytes = _size_of((n, k, group, "w4"), w4_packed_size, n, k, group)
-    _packed_operand(gate, nbytes, "gate", x.device)
-    _packed_operand(up, nbytes, "up", x.device)
+    _packed_operand(gate, nbytes, "gate", device)
+    _packed_operand(up, nbytes, "up", device)
     if h is None:
-        h = torch.empty((m, n), dtype=out_dtype or x.dtype, device=x.device)
+        h = _empty((m, n), dtype=out_dtype or x.dtype, device=x.device)
     else:
-        _operand(h, (m, n), "h")
-        _on_current(h)
-    check(load().gq_w4_gate_up(_ptr(gate), _ptr(up), group, _ptr(x), _dt(x.dtype), _ptr(h), _dt(h.dtype), n, k, m, act,
-                               _stream(stream)), "gq_w4_gate_up")
+        _operand(h, (m, n), "h", device)
+    st = load().gq_w4_gate_up(gate.data_ptr(), up.data_ptr(), group, x.data_ptr(), _dt(x.dtype), h.data_ptr(), _dt(h.dtype), n,
+                              k, m, act, _stream(stream))
+    if st:
+        check(st, "gq_w4_gate_up")
     return h
 
 
