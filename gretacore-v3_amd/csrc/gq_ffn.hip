@@ -1044,6 +1044,12 @@ __global__ void __launch_bounds__(kDguThreads) k_front_dgu(const void *dh, const
   }
 }
 
+struct __attribute__((packed, aligned(2))) FRun16h {  // 4 values
+  gq_u2 v;
+};
+struct __attribute__((packed, aligned(4))) FRun32h {
+  gq_f4 v;
+};
 // dx[m][k] = sum over n of dg[m][n] W_gate[n][k] + du[m][n] W_up[n][k]: the sum runs over the weights'
 // rows, while a T16 record holds 16 rows of 128 k, each row's codes side by side.  Steps of 64 n (four row
 // tiles), gate's before up's.  The records go to LDS as they are (by DMA, the slots of a 64-lane
@@ -1299,70 +1305,60 @@ __global__ void __launch_bounds__(64 * WN * KG) k_front_dx(const uint8_t *__rest
     }
   }
   __builtin_amdgcn_s_waitcnt(0x0F70);  // (loads of no step still on their way into the stages)
-  if constexpr (KG > 1) {  // the groups' sums through LDS, a fragment's tiles at a time, in group order
-    static_assert((KG - 1) * NW * TM * 4096 <= KG * STAGE, "LDS");
-    gq_f4 *xs = reinterpret_cast<gq_f4 *>(lds_0);
-    auto at = [&](int g, int i, int q) { return (((g * NW + wave) * TM + i) * 4 + q) * 64 + lane; };
-    __syncthreads();
-#pragma unroll
-    for (int f = 0; f < 4; ++f) {
-      if (kg > 0) {
-#pragma unroll
-        for (int i = 0; i < TM; ++i)
-#pragma unroll
-          for (int q = 0; q < 4; ++q)
-            xs[at(kg - 1, i, q)] = gq_f4{acc[i][f][4 * q], acc[i][f][4 * q + 1], acc[i][f][4 * q + 2], acc[i][f][4 * q + 3]};
-      }
-      __syncthreads();
-      if (kg == 0) {
-#pragma unroll
-        for (int g = 0; g < KG - 1; ++g)
-#pragma unroll
-          for (int i = 0; i < TM; ++i)
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-              const gq_f4 t = xs[at(g, i, q)];
-#pragma unroll
-              for (int e = 0; e < 4; ++e) acc[i][f][4 * q + e] += t[e];
-            }
-      }
-      __syncthreads();
-    }
-    if (kg > 0) return;
-  }
-  // parts: fp32 sums [part][M][K], scaled by k_dx_sum; else dx itself
+  // Out through LDS, 16 rows of the tile at a time: every wave puts its sums there by row, then the
+  // groups' waves of a column block add them in group order, a share of the rows each, and store whole
+  // runs.  (From the lanes that hold them, 8 bytes every 16 of a row, the stores took 12 of 46 us, 200 x
+  // 5003 x 4096 Q4_K in 8 parts.)  Parts: fp32 sums [part][M][K], scaled by k_dx_sum; else dx itself.
+  constexpr int LD = 132, ROWS = 16 / KG;
+  static_assert(KG * NW * 16 * LD * 4 <= KG * STAGE, "LDS");
+  float *xs = reinterpret_cast<float *>(lds_0);
   const bool parts = gridDim.y > 1;
   if (parts) y = reinterpret_cast<float *>(y) + (size_t)blockIdx.y * (size_t)M * (size_t)K;
-  const int k0 = 128 * (kc0 + wn) + (q8 ? 4 * c : 32 * (c >> 3) + 16 * ((c >> 2) & 1) + 8 * ((c >> 1) & 1) + 2 * (c & 1));
-  if (k0 >= K) return;  // (K is whole 32-blocks: a lane's columns are wholly in or out)
+  const int kl = q8 ? 4 * c : 32 * (c >> 3) + 16 * ((c >> 2) & 1) + 8 * ((c >> 1) & 1) + 2 * (c & 1);
+  const int k0 = 128 * (kc0 + wn) + 4 * (lane & 31);  // the run of 4 this lane stores
 #pragma unroll
   for (int i = 0; i < TM; ++i)
 #pragma unroll
-    for (int v = 0; v < 16; ++v) {
-      const int m = m0 + 32 * i + 8 * (v >> 2) + 4 * kh + (v & 3);
-      if (m >= M) continue;
-      const float s = parts ? 1.f : rs[m], s16 = q8 ? s : s * 0.0625f;
-      const size_t at = (size_t)m * K + k0;
-      // columns k0, k0 + 1 and k0 + 4, + 5 (Q8_0: + 2, + 3)
-      const float o[4] = {acc[i][0][v] * s, q8 ? acc[i][1][v] * s : acc[i][2][v] * s, q8 ? acc[i][2][v] * s : acc[i][1][v] * s16,
-                          acc[i][3][v] * s16};
-      const size_t at2 = at + (q8 ? 2 : 4);
-      if (parts || dt == GQ_DT_F32) {
-        float *p = reinterpret_cast<float *>(y);
-        p[at] = o[0];
-        p[at + 1] = o[1];
-        p[at2] = o[2];
-        p[at2 + 1] = o[3];
-      } else {
-        uint16_t *p = reinterpret_cast<uint16_t *>(y);
-        uint16_t b[4];
+    for (int half = 0; half < 2; ++half) {
+      __syncthreads();
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          b[e] = dt == GQ_DT_BF16 ? gq_f32_to_bf16(o[e]) : __builtin_bit_cast(uint16_t, (_Float16)o[e]);
-        p[at] = b[0];
-        p[at + 1] = b[1];
-        p[at2] = b[2];
-        p[at2 + 1] = b[3];
+      for (int w = 0; w < 8; ++w) {
+        const int v = 8 * half + w;
+        float *row = xs + ((kg * NW + wn) * 16 + 8 * (w >> 2) + 4 * kh + (w & 3)) * LD + kl;
+        if constexpr (FMT == GQ_FMT_Q8_0) {
+          *reinterpret_cast<gq_f4 *>(row) = gq_f4{acc[i][0][v], acc[i][1][v], acc[i][2][v], acc[i][3][v]};
+        } else {  // (columns + 0, + 1 and + 4, + 5)
+          *reinterpret_cast<float2 *>(row) = make_float2(acc[i][0][v], acc[i][2][v]);
+          *reinterpret_cast<float2 *>(row + 4) = make_float2(acc[i][1][v] * 0.0625f, acc[i][3][v] * 0.0625f);
+        }
+      }
+      __syncthreads();
+#pragma unroll
+      for (int j = 0; j < ROWS; j += 2) {
+        const int r = kg * ROWS + j + (lane >> 5), m = m0 + 32 * i + 16 * half + r;
+        gq_f4 t = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int g = 0; g < KG; ++g) {
+          const gq_f4 u = *reinterpret_cast<const gq_f4 *>(xs + ((g * NW + wn) * 16 + r) * LD + 4 * (lane & 31));
+#pragma unroll
+          for (int e = 0; e < 4; ++e) t[e] += u[e];
+        }
+        if (m >= M || k0 >= K) continue;  // (K is whole 32-blocks)
+        const size_t at = (size_t)m * K + k0;
+        const float f = parts ? 1.f : rs[m];
+        if (parts || dt == GQ_DT_F32) {
+          FRun32h o;
+          o.v = gq_f4{t[0] * f, t[1] * f, t[2] * f, t[3] * f};
+          *reinterpret_cast<FRun32h *>(reinterpret_cast<float *>(y) + at) = o;
+        } else {
+          uint32_t b[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            b[e] = dt == GQ_DT_BF16 ? gq_f32_to_bf16(t[e] * f) : __builtin_bit_cast(uint16_t, (_Float16)(t[e] * f));
+          FRun16h o;
+          o.v = gq_u2{b[0] | b[1] << 16, b[2] | b[3] << 16};
+          *reinterpret_cast<FRun16h *>(reinterpret_cast<uint16_t *>(y) + at) = o;
+        }
       }
     }
 }
