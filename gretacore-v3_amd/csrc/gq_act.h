@@ -19,8 +19,8 @@ GQ_DEV void gq_st_dt(void *p, int dt, size_t i, float v) {
   else reinterpret_cast<uint16_t *>(p)[i] = gq_f32_to_bf16(v);
 }
 
-// 1 / (1 + e^-x); e^-x overflows to Inf below -88 and the result is then 0
-GQ_DEV float gq_sigmoid(float x) { return 1.0f / (1.0f + __expf(-x)); }
+// 1 / (1 + e^-x), the reciprocal of one step's error; e^-x overflows to Inf below -88 and the result is then 0
+GQ_DEV float gq_sigmoid(float x) { return __builtin_amdgcn_rcpf(1.0f + __expf(-x)); }
 
 // Both activations are g * sigmoid(p): p = g for SiLU, and for the tanh form of
 // GELU 1/2 (1 + tanh t) = sigmoid(2 t), so p = 2 sqrt(2 / pi) (g + 0.044715 g^3).  There

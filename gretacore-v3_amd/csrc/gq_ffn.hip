@@ -725,17 +725,15 @@ GQ_DEV void step_barrier() {
   asm volatile("" ::: "memory");
 }
 
-// waves per SIMD: what a workgroup brings, at least two but where the sums of 256 rows take
-// the registers of both
-constexpr int front_wpe(int waves, int bm) { return waves > 4 ? waves / 4 : bm > 128 ? 1 : 2; }
+// waves per SIMD: what a workgroup brings, at least two
+constexpr int front_wpe(int waves) { return waves > 4 ? waves / 4 : 2; }
 
-template <int FMT, int BM, int WM, int WN, int NJ, int PD, int KG>
-__global__ void __launch_bounds__(64 * WM * WN * KG)
-__attribute__((amdgpu_waves_per_eu(front_wpe(WM *WN *KG, BM), front_wpe(WM *WN *KG, BM))))
+template <int FMT, int BM, int WN, int NJ, int PD, int KG>
+__global__ void __launch_bounds__(64 * WN * KG) __attribute__((amdgpu_waves_per_eu(front_wpe(WN *KG), front_wpe(WN *KG))))
 k_front_rb(const uint8_t *__restrict__ wg, const uint8_t *__restrict__ wu, uint32_t sc_off,
            const _Float16 *__restrict__ a16, int lda, const float *__restrict__ rs, void *__restrict__ h,
            void *__restrict__ go, void *__restrict__ uo, int dt, int M, int N, int C, int nsteps, int tiles_m, int act) {
-  constexpr int KS = BK / 16, NW = WM * WN, TM = BM / WM / 32, BN = 32 * NJ * WN;
+  constexpr int KS = BK / 16, NW = WN, TM = BM / 32, BN = 32 * NJ * WN;
   __shared__ __attribute__((aligned(16))) _Float16 As_0[KG * BM * BK];
   __shared__ __attribute__((aligned(16))) _Float16 As_1[KG * BM * BK];
   __shared__ __attribute__((aligned(16))) _Float16 As_2[PD >= 3 ? KG * BM * BK : 8];
@@ -744,7 +742,7 @@ k_front_rb(const uint8_t *__restrict__ wg, const uint8_t *__restrict__ wu, uint3
   const int tid = threadIdx.x, lane = tid & 63;
   const int kg = KG == 1 ? 0 : __builtin_amdgcn_readfirstlane((tid >> 6) / NW);
   const int wave = __builtin_amdgcn_readfirstlane((tid >> 6) % NW);
-  const int wm = wave / WN, wn = wave % WN;
+  const int wn = wave;
   auto As_of = [&](auto b) -> _Float16 * {
     constexpr int v = decltype(b)::value;
     return (v == 0 ? As_0 : v == 1 ? As_1 : v == 2 ? As_2 : As_3) + kg * (BM * BK);
@@ -781,7 +779,7 @@ k_front_rb(const uint8_t *__restrict__ wg, const uint8_t *__restrict__ wu, uint3
   const uint32_t mg = gq_nib_magic();
   uint32_t ao[NA];
   a_offsets<BM, NW>(lda, M, m0, wave, lane, ao);
-  const int arow = (BM / WM) * wm + (lane & 31), sw = a_swz(lane & 31);
+  const int arow = lane & 31, sw = a_swz(lane & 31);
   auto gstep = [&](int l) { return (l < nl ? l : nl - 1) * KG + kg; };
   auto run_step = [&](int l, auto buf_c) __attribute__((always_inline)) {
     constexpr int BUF = decltype(buf_c)::value;
@@ -887,7 +885,7 @@ k_front_rb(const uint8_t *__restrict__ wg, const uint8_t *__restrict__ wu, uint3
     const __amdgpu_buffer_rsrc_t hr = rsrc(h), gr = rsrc(go), ur = rsrc(uo);  // (an output not wanted: no range)
 #pragma unroll
     for (int i = 0; i < TM; ++i) {
-      const int mb = (BM / WM) * wm + 32 * i + 4 * (lane >> 5);
+      const int mb = 32 * i + 4 * (lane >> 5);
       float rsv[16];
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
@@ -1378,12 +1376,12 @@ __global__ void __launch_bounds__(256) k_dx_sum(const float *__restrict__ part, 
   for (int e = 0; e < 4; ++e) gq_st_dt(y, dt, i + e, v[e] * s);
 }
 
-template <int FMT, int BM, int WM, int WN, int NJ, int PD, int KG>
+template <int FMT, int BM, int WN, int NJ, int PD, int KG>
 int launch_front_rb(const void *wg, const void *wu, const _Float16 *a16, int lda, const float *rs, void *h, void *go,
                     void *uo, int dt, int M, int N, int K, int act, hipStream_t s) {
   const int tiles_m = (M + BM - 1) / BM, tiles_n = (N + 32 * NJ * WN - 1) / (32 * NJ * WN);
   GQ_CHECK((size_t)tiles_m * (size_t)tiles_n <= 0x7FFFFFFFu, GQ_ERR_INVALID_ARGS);  // (one grid dimension)
-  hipLaunchKernelGGL((k_front_rb<FMT, BM, WM, WN, NJ, PD, KG>), dim3((unsigned)(tiles_m * tiles_n)), dim3(64 * WM * WN * KG),
+  hipLaunchKernelGGL((k_front_rb<FMT, BM, WN, NJ, PD, KG>), dim3((unsigned)(tiles_m * tiles_n)), dim3(64 * WN * KG),
                      0, s, (const uint8_t *)wg, (const uint8_t *)wu, (uint32_t)gq_sc_plane_offset(FMT, N, K), a16, lda, rs,
                      h, go, uo, dt, M, N, (int)gq_chunks(FMT, K), (int)(gq_kpad(FMT, K) / BK), tiles_m, act);
   return gq_last_launch();
@@ -1512,11 +1510,11 @@ int launch_front_fmt(const void *wg, const void *wu, const _Float16 *a16, int ld
   // 64 x 14336 43.0 / 31.2 / 40.6 / 57.2, 128 x 14336 79.5 / 56.3 / 46.3 / 57.8, 256 x 4096 - / 31.5 / 40.6 / 56.2); 128
   // x 128 without groups, two workgroups a CU, for the rest: 2048 x 14336 450 us (with K groups 492,
   // 256 x 128 on 8 waves 470, on 4 waves of 256 rows 503)
-  if (M <= 32 && nsteps % 4 == 0) return GQ_FRONT(32, 1, 2, 1, 4, 4);
-  if (wgs(64, 64) <= 288 && nsteps % 4 == 0) return GQ_FRONT(64, 1, 2, 1, 3, 4);
-  if (wgs(64, 128) <= 288) return GQ_FRONT(64, 1, 4, 1, 3, 2);
-  if (wgs(128, 128) <= 288) return GQ_FRONT(128, 1, 4, 1, 3, 2);
-  return GQ_FRONT(128, 1, 4, 1, 2, 1);
+  if (M <= 32 && nsteps % 4 == 0) return GQ_FRONT(32, 2, 1, 4, 4);
+  if (wgs(64, 64) <= 288 && nsteps % 4 == 0) return GQ_FRONT(64, 2, 1, 3, 4);
+  if (wgs(64, 128) <= 288) return GQ_FRONT(64, 4, 1, 3, 2);
+  if (wgs(128, 128) <= 288) return GQ_FRONT(128, 4, 1, 3, 2);
+  return GQ_FRONT(128, 4, 1, 2, 1);
 #undef GQ_FRONT
 }
 int launch_front(int fmt, const void *wg, const void *wu, const _Float16 *a16, int lda, const float *rs, void *h, void *go,
