@@ -301,27 +301,26 @@ k_front_few(const uint8_t *__restrict__ wg, const uint8_t *__restrict__ wu, size
 }
 
 // More rows: the sums of the scale groups would cost more than folding the scale into the
-// weights, 13 to 24 operations for 8 weights with one rounding to fp16; the matrix cores then
-// add over all of K.  x comes as fp16 with a power-of-two scale per row (gq_launch_a_to_f16, for the
-// 4-bit formats in their nibbles' order), MT tiles of 16 rows.
+// weights; the matrix cores then add over a unit or all of K.  Q4_0 and Q8_0: d (q - bias), rounded once
+// to fp16.  The k-quants keep their d (and dmin) out, one of each to a row and unit, applied in fp32
+// to the unit's sums: sc q is exact in fp16, sc (q - 32) but for the few beyond 2048, and the minima
+// are a product of their own, of x with their codes.  x comes as fp16 with a power-of-two scale per row (for the
+// 4-bit formats in their nibbles' order, where every other pair is x / 16 and its weight 16 x).
 template <int FMT>
-GQ_DEV void rows_frags(const FUnit<FMT> &u, int unit, int g, uint32_t mg, gq_half8 (&o)[2][2]) {
+GQ_DEV void rows_frags(const FUnit<FMT> &u, int unit, int g, uint32_t mg, gq_half8 (&o)[2][2], gq_half8 (&mins)[2]) {
   uint32_t sc = 0, mc = 0;
   if constexpr (FMT == GQ_FMT_Q4_K) unit_codes_q4k(u, (uint32_t)unit & 1u, g >> 1, sc, mc);
 #pragma unroll
   for (int m = 0; m < 2; ++m) {
-    gq_half2 d2, a1, b1, m1, m16;  // Q4_K: (1024 + q) a1 + b1 = sc q, exact; then one rounding of d sc q - dmin m
+    gq_half2 d2, b1;
     if constexpr (FMT == GQ_FMT_Q4_K) {
-      const _Float16 d = bits_h(u.s[0]), ndm = -bits_h(u.s[0] >> 16);
       const _Float16 s = (_Float16)(float)((sc >> (8 * m)) & 255u), c = (_Float16)(float)((mc >> (8 * m)) & 255u);
-      const _Float16 ns = s * (_Float16)-1024.0f, hm = c * ndm, hm16 = hm * (_Float16)16.0f;
-      d2 = gq_half2{d, d};
-      a1 = gq_half2{s, s};
+      const _Float16 ns = s * (_Float16)-1024.0f, c16 = c * (_Float16)16.0f;
+      d2 = gq_half2{s, s};
       b1 = gq_half2{ns, ns};
-      m1 = gq_half2{hm, hm};
-      m16 = gq_half2{hm16, hm16};
+      mins[m] = gq_half8{c, c, c16, c16, c, c, c16, c16};
     } else if constexpr (FMT == GQ_FMT_Q6_K) {
-      const _Float16 s = (_Float16)((float)bits_h(u.d) * (float)(int8_t)(u.s[2 + m] >> (8 * g)));
+      const _Float16 s = (_Float16)(float)(int8_t)(u.s[2 + m] >> (8 * g));
       d2 = gq_half2{s, s};
     } else {
       d2 = splat_h((g >> 1 ? u.s[1] : u.s[0]) >> (16 * m));
@@ -343,13 +342,39 @@ GQ_DEV void rows_frags(const FUnit<FMT> &u, int unit, int g, uint32_t mg, gq_hal
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         if constexpr (FMT == GQ_FMT_Q4_K) {
-          p[i] = __builtin_elementwise_fma(__builtin_elementwise_fma(p[i], a1, b1), d2, i & 1 ? m16 : m1);
+          p[i] = __builtin_elementwise_fma(p[i], d2, b1);  // sc q (or 16 sc q), exact
         } else {
           const float off = FMT == GQ_FMT_Q8_0 ? -1152.f : FMT == GQ_FMT_Q6_K ? -1056.f : i & 1 ? -1152.f : -1032.f;
           p[i] = (p[i] + gq_half2{(_Float16)off, (_Float16)off}) * d2;  // (the sum is exact)
         }
         o[m][j][2 * i] = p[i][0];
         o[m][j][2 * i + 1] = p[i][1];
+      }
+    }
+  }
+}
+// acc += the unit's products with x (its four fragments xs[t])
+template <int FMT, int MT>
+GQ_DEV void rows_add(const FUnit<FMT> &u, int unit, int g, uint32_t mg, const gq_half8 (&xs)[MT][4], gq_f4 (&acc)[MT]) {
+  gq_half8 b[2][2], mins[2];
+  rows_frags<FMT>(u, unit, g, mg, b, mins);
+#pragma unroll
+  for (int t = 0; t < MT; ++t) {
+    if constexpr (!kSuper<FMT>) {
+#pragma unroll
+      for (int f = 0; f < 4; ++f) acc[t] = gq_mfma16(xs[t][f], b[f >> 1][f & 1], acc[t]);
+    } else {
+      const float d = (float)bits_h(FMT == GQ_FMT_Q4_K ? u.s[0] : u.d);
+      gq_f4 y = {0.f, 0.f, 0.f, 0.f}, z = y;
+#pragma unroll
+      for (int f = 0; f < 4; ++f) {
+        y = gq_mfma16(xs[t][f], b[f >> 1][f & 1], y);
+        if constexpr (FMT == GQ_FMT_Q4_K) z = gq_mfma16(xs[t][f], mins[f >> 1], z);
+      }
+#pragma unroll
+      for (int v = 0; v < 4; ++v) {
+        acc[t][v] = fmaf(d, y[v], acc[t][v]);
+        if constexpr (FMT == GQ_FMT_Q4_K) acc[t][v] = fmaf(-(float)bits_h(u.s[0] >> 16), z[v], acc[t][v]);
       }
     }
   }
@@ -401,14 +426,7 @@ k_front_rows(const uint8_t *__restrict__ wg, const uint8_t *__restrict__ wu, siz
   const uint32_t mg = gq_nib_magic();
   auto compute = [&](int unit, int st) __attribute__((always_inline)) {
 #pragma unroll
-    for (int t = 0; t < T; ++t) {
-      gq_half8 b[2][2];
-      rows_frags<FMT>(us[st][t], unit, g, mg, b);
-#pragma unroll
-      for (int i = 0; i < MT; ++i)
-#pragma unroll
-        for (int f = 0; f < 4; ++f) acc[t][i] = gq_mfma16(xs[st][i][f], b[f >> 1][f & 1], acc[t][i]);
-    }
+    for (int t = 0; t < T; ++t) rows_add<FMT, MT>(us[st][t], unit, g, mg, xs[st], acc[t]);
   };
   walk_units<PD, KS>(units, wave, request, compute);
 #pragma unroll
@@ -595,7 +613,7 @@ k_front_rows_px(const uint8_t *__restrict__ wg, const uint8_t *__restrict__ wu, 
     for (int w = 0; w < 2; ++w)
       load_unit<FMT>(ftile<FMT>(w ? wu : wg, sc_off, (size_t)tile, tile < ntiles ? C : 0), wave + kPxWaves * i, lane, us[i][w]);
   };
-  gq_half8 xs[MT][NU][4];
+  gq_half8 xs[NU][MT][4];
   float back[MT][4];  // what undoes the scales of this lane's rows of the result, 16 t + 4 g + v
   auto xin = [&](int t, int i, int f) {
     return 16 * t + r < M && 128 * (wave + kPxWaves * i) + 64 * (f >> 1) + 16 * g + 8 * (f & 1) < K;
@@ -655,7 +673,7 @@ k_front_rows_px(const uint8_t *__restrict__ wg, const uint8_t *__restrict__ wu, 
           constexpr int perm[8] = {0, 2, 4, 6, 1, 3, 5, 7};  // the nibbles' order, their 16 x divided out
 #pragma unroll
           for (int e = 0; e < 8; ++e)
-            xs[t][i][f][e] = (_Float16)(kNibOrder<FMT> ? ((e & 2) ? v[perm[e]] * 0.0625f : v[perm[e]]) * f2 : v[e] * f2);
+            xs[i][t][f][e] = (_Float16)(kNibOrder<FMT> ? ((e & 2) ? v[perm[e]] * 0.0625f : v[perm[e]]) * f2 : v[e] * f2);
         }
     }
   };
@@ -667,14 +685,8 @@ k_front_rows_px(const uint8_t *__restrict__ wg, const uint8_t *__restrict__ wu, 
   const uint32_t mg = gq_nib_magic();
   auto compute = [&](int i) __attribute__((always_inline)) {
 #pragma unroll
-    for (int w = 0; w < 2; ++w) {
-      gq_half8 b[2][2];
-      rows_frags<FMT>(us[i][w], wave, g, mg, b);  // (8 i units on: the same half of a super-block)
-#pragma unroll
-      for (int t = 0; t < MT; ++t)
-#pragma unroll
-        for (int f = 0; f < 4; ++f) acc[w][t] = gq_mfma16(xs[t][i][f], b[f >> 1][f & 1], acc[w][t]);
-    }
+    for (int w = 0; w < 2; ++w)
+      rows_add<FMT, MT>(us[i][w], wave, g, mg, xs[i], acc[w]);  // (8 i units on: the same half of a super-block)
   };
   auto finish = [&](int tile, int buf) __attribute__((always_inline)) {
 #pragma unroll
@@ -1057,14 +1069,14 @@ struct __attribute__((packed, aligned(4))) FRun32h {
 //   4-bit and Q6_K: 32 (c / 8) + 16 (c / 4 % 2) + 8 (c / 2 % 2) + 2 (c % 2) + {0, 4, 1, 5}  Q8_0: 4 c + {0, 1, 2, 3}
 // of 128, one per fragment; the second and fourth of the former come out 16 x (nibbles masked in place) and
 // the sums are divided by 16 at the end.  Scales vary along n: a wave brings the step's 64 rows'
-// scales to LDS as fp16 [group of columns][16 rows], a lane's 8 rows one 16-byte read.  (Q4_K: d sc and
-// dmin m rounded to fp16 each, then one rounding of their combination.)
+// scales to LDS as fp16 [group of columns][16 rows], a lane's 8 rows one 16-byte read.  (Q4_K: sc, -dmin m
+// rounded to fp16, and d apart, so that sc q is exact and d sc q - dmin m rounded once.)
 template <int FMT>
 constexpr int kDxGroups = FMT == GQ_FMT_Q6_K ? 8 : 4;  // scale groups of 128 columns
 template <int FMT>
 constexpr int kDxRecs = FMT == GQ_FMT_Q8_0 || FMT == GQ_FMT_Q6_K ? 2 : 1;  // 1 KiB records of 128 columns and a row tile
 template <int FMT>
-constexpr int kDxTables = FMT == GQ_FMT_Q4_K ? 2 : 1;
+constexpr int kDxRows = FMT == GQ_FMT_Q4_K ? 9 : kDxGroups<FMT>;  // [16 rows] of a tile's table: 4 sc, 4 minima, d; else the scales
 
 // scales of row r (of a tile) for 128 columns, as loaded
 template <int FMT>
@@ -1089,15 +1101,15 @@ GQ_DEV gq_u4 dx_load_scales(const __amdgpu_buffer_rsrc_t &w, uint32_t sc_off, ui
 // -> the tables [table][group][16 rows] of the row's tile
 template <int FMT>
 GQ_DEV void dx_store_scales(const gq_u4 &v, uint32_t p, int r, _Float16 *t) {
-  constexpr int G = kDxGroups<FMT>;
   if constexpr (FMT == GQ_FMT_Q4_K) {
-    const float d = (float)bits_h(v[0]), dm = (float)bits_h(v[0] >> 16);
+    const float dm = (float)bits_h(v[0] >> 16);
 #pragma unroll
     for (int j = 0; j < 4; ++j) {  // sub-block 4 p + j
       const uint32_t sh = 16u * p + 8u * (j >> 1), b = ((j & 1) ? v[2] : v[1]) >> sh, m = v[3] >> (sh + 4u * (j & 1));
-      t[16 * j + r] = (_Float16)(d * (float)(b & 63u));
-      t[16 * (G + j) + r] = (_Float16)(-(dm * (float)(((b >> 6) & 3u) | ((m & 15u) << 2))));
+      t[16 * j + r] = (_Float16)(float)(b & 63u);
+      t[16 * (4 + j) + r] = (_Float16)(-(dm * (float)(((b >> 6) & 3u) | ((m & 15u) << 2))));
     }
+    t[16 * 8 + r] = bits_h(v[0]);
   } else if constexpr (FMT == GQ_FMT_Q6_K) {
     const float d = (float)bits_h(v[2]);
 #pragma unroll
@@ -1112,10 +1124,10 @@ template <int FMT, int WN, int KG, int TM, int PD>
 __global__ void __launch_bounds__(64 * WN * KG) k_front_dx(const uint8_t *__restrict__ wg, const uint8_t *__restrict__ wu, uint32_t w_bytes, uint32_t sc_off,
            const _Float16 *__restrict__ a16, const float *__restrict__ rs, void *__restrict__ y, int dt, int M, int K,
            int C, int ntiles, int nsteps, int sps, int tiles_m) {
-  constexpr int NW = WN, BM = 32 * TM, BN = 128 * WN, G = kDxGroups<FMT>, RECS = kDxRecs<FMT>, TB = kDxTables<FMT>;
+  constexpr int NW = WN, BM = 32 * TM, BN = 128 * WN, ROWS_T = 16 * kDxRows<FMT>, RECS = kDxRecs<FMT>;
   constexpr int NREC = 4 * WN * RECS, RPW = (NREC + NW - 1) / NW;  // records a step, per wave
   static_assert(NREC % NW == 0, "records");
-  constexpr int A_B = BM * BK * 2, W_B = NREC * 1024, S_B = WN * 4 * TB * G * 32, STAGE = A_B + W_B + S_B;
+  constexpr int A_B = BM * BK * 2, W_B = NREC * 1024, S_B = WN * 4 * ROWS_T * 2, STAGE = A_B + W_B + S_B;
   static_assert(PD == 2 || PD == 3, "pipeline depth");
   static_assert(KG * PD * STAGE <= 160 * 1024, "LDS");
   // an array a stage (activations, records, scales): no wait for a DMA into another one
@@ -1178,7 +1190,7 @@ __global__ void __launch_bounds__(64 * WN * KG) k_front_dx(const uint8_t *__rest
                                t < (uint32_t)ntiles && c < (uint32_t)C);
   };
   auto store_scales = [&](const gq_u4 &v, int st) __attribute__((always_inline)) {
-    _Float16 *t = table(st) + (wave * 4 + stile) * (TB * G * 16);
+    _Float16 *t = table(st) + (wave * 4 + stile) * ROWS_T;
     dx_store_scales<FMT>(v, kSuper<FMT> ? (uint32_t)(kc0 + wave) & 1u : 0u, srow, t);
   };
 
@@ -1203,9 +1215,9 @@ __global__ void __launch_bounds__(64 * WN * KG) k_front_dx(const uint8_t *__rest
   auto compute = [&](int st) __attribute__((always_inline)) {
     const _Float16 *As = reinterpret_cast<const _Float16 *>(stage(st)) + (lane & 31) * BK;
     const uint8_t *Ws = stage(st) + A_B + wn * (4 * RECS * 1024);
-    const _Float16 *Ss = table(st) + wn * (4 * TB * G * 16) + 16 * grp + 8 * kh;
+    const _Float16 *Ss = table(st) + wn * (4 * ROWS_T) + 8 * kh;
     // a row tile's operands as they lie in LDS, one tile ahead of the products
-    gq_half8 af[2][TM], d8[2], m8[2];
+    gq_half8 af[2][TM], s8[2], m8[2], d8[2];
     uint32_t cw[2][8], hw[2][8];
     auto read = [&](int t, int x) __attribute__((always_inline)) {
       const uint8_t *W = Ws + t * (RECS * 1024) + cb;
@@ -1217,8 +1229,12 @@ __global__ void __launch_bounds__(64 * WN * KG) k_front_dx(const uint8_t *__rest
         if constexpr (FMT == GQ_FMT_Q6_K)
           hw[x][e] = *reinterpret_cast<const uint16_t *>(Ws + t * (RECS * 1024) + 1024 + 4 * (2 * par + cm) + 2 * (c & 1) + row_at(e));
       }
-      d8[x] = *reinterpret_cast<const gq_half8 *>(Ss + t * (TB * G * 16));
-      if constexpr (FMT == GQ_FMT_Q4_K) m8[x] = *reinterpret_cast<const gq_half8 *>(Ss + t * (TB * G * 16) + G * 16);
+      const _Float16 *S = Ss + t * ROWS_T;
+      s8[x] = *reinterpret_cast<const gq_half8 *>(S + 16 * grp);
+      if constexpr (FMT == GQ_FMT_Q4_K) {
+        m8[x] = *reinterpret_cast<const gq_half8 *>(S + 16 * (4 + grp));
+        d8[x] = *reinterpret_cast<const gq_half8 *>(S + 16 * 8);
+      }
 #pragma unroll
       for (int i = 0; i < TM; ++i) af[x][i] = *reinterpret_cast<const gq_half8 *>(As + 32 * i * BK + 8 * ((2 * t + kh) ^ sw));
     };
@@ -1249,23 +1265,25 @@ __global__ void __launch_bounds__(64 * WN * KG) k_front_dx(const uint8_t *__rest
             q[3] |= (h8 << 6) & 0x03000300u;
           }
         }
-        const gq_half2 d2 = {d8[x][2 * j], d8[x][2 * j + 1]};
-        gq_half2 m2 = d2, m16 = d2;
+        const gq_half2 s2 = {s8[x][2 * j], s8[x][2 * j + 1]};
+        gq_half2 m2 = s2, m16 = s2, d2 = s2, n2 = s2;
         if constexpr (FMT == GQ_FMT_Q4_K) {
           m2 = gq_half2{m8[x][2 * j], m8[x][2 * j + 1]};
           m16 = m2 * gq_half2{(_Float16)16.0f, (_Float16)16.0f};
+          d2 = gq_half2{d8[x][2 * j], d8[x][2 * j + 1]};
+          n2 = s2 * gq_half2{(_Float16)-1024.0f, (_Float16)-1024.0f};
         }
 #pragma unroll
         for (int f = 0; f < 4; ++f) {
           const bool x16 = !q8 && (f & 1);
           const float off = q8                     ? -1152.f
                             : FMT == GQ_FMT_Q4_0 ? (x16 ? -1152.f : -1032.f)
-                            : FMT == GQ_FMT_Q6_K ? (x16 ? -1536.f : -1056.f)
-                                                 : -1024.f;
-          const gq_half2 o2 = {(_Float16)off, (_Float16)off};
-          gq_half2 r = gq_bits_h2(q[f]) + o2;  // (exact)
-          if constexpr (FMT == GQ_FMT_Q4_K) r = __builtin_elementwise_fma(r, d2, x16 ? m16 : m2);
-          else r = r * d2;
+                                                 : (x16 ? -1536.f : -1056.f);
+          gq_half2 r;
+          if constexpr (FMT == GQ_FMT_Q4_K)  // (sc q or 16 sc q, exact; then one rounding)
+            r = __builtin_elementwise_fma(__builtin_elementwise_fma(gq_bits_h2(q[f]), s2, n2), d2, x16 ? m16 : m2);
+          else
+            r = (gq_bits_h2(q[f]) + gq_half2{(_Float16)off, (_Float16)off}) * s2;  // (the sum is exact)
           bf[f][2 * j] = r[0];
           bf[f][2 * j + 1] = r[1];
         }
@@ -1307,7 +1325,7 @@ __global__ void __launch_bounds__(64 * WN * KG) k_front_dx(const uint8_t *__rest
   // groups' waves of a column block add them in group order, a share of the rows each, and store whole
   // runs.  (From the lanes that hold them, 8 bytes every 16 of a row, the stores took 12 of 46 us, 200 x
   // 5003 x 4096 Q4_K in 8 parts.)  Parts: fp32 sums [part][M][K], scaled by k_dx_sum; else dx itself.
-  constexpr int LD = 132, ROWS = 16 / KG;
+  constexpr int LD = 132, SHARE = 16 / KG;
   static_assert(KG * NW * 16 * LD * 4 <= KG * STAGE, "LDS");
   float *xs = reinterpret_cast<float *>(lds_0);
   const bool parts = gridDim.y > 1;
@@ -1332,8 +1350,8 @@ __global__ void __launch_bounds__(64 * WN * KG) k_front_dx(const uint8_t *__rest
       }
       __syncthreads();
 #pragma unroll
-      for (int j = 0; j < ROWS; j += 2) {
-        const int r = kg * ROWS + j + (lane >> 5), m = m0 + 32 * i + 16 * half + r;
+      for (int j = 0; j < SHARE; j += 2) {
+        const int r = kg * SHARE + j + (lane >> 5), m = m0 + 32 * i + 16 * half + r;
         gq_f4 t = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int g = 0; g < KG; ++g) {
@@ -1360,18 +1378,18 @@ __global__ void __launch_bounds__(64 * WN * KG) k_front_dx(const uint8_t *__rest
       }
     }
 }
-// dx = rs[m] * the parts' sums, in part order
+// dx = rs[m] * the parts' sums, in part order (no parts: zeros)
 __global__ void __launch_bounds__(256) k_dx_sum(const float *__restrict__ part, const float *__restrict__ rs, void *__restrict__ y,
                                                 int dt, size_t mk, int K, int parts) {
   const size_t i = ((size_t)blockIdx.x * 256 + threadIdx.x) * 4;  // (K % 32 == 0: four of one row)
   if (i >= mk) return;
-  gq_f4 v = *reinterpret_cast<const gq_f4 *>(part + i);
-  for (int p = 1; p < parts; ++p) {
+  gq_f4 v = {0.f, 0.f, 0.f, 0.f};
+  for (int p = 0; p < parts; ++p) {
     const gq_f4 t = *reinterpret_cast<const gq_f4 *>(part + (size_t)p * mk + i);
 #pragma unroll
     for (int e = 0; e < 4; ++e) v[e] += t[e];
   }
-  const float s = rs[i / (size_t)K];
+  const float s = parts ? rs[i / (size_t)K] : 0.f;
 #pragma unroll
   for (int e = 0; e < 4; ++e) gq_st_dt(y, dt, i + e, v[e] * s);
 }
@@ -1408,7 +1426,7 @@ int launch_front_few_t(const void *wg, const void *wu, const void *x, const floa
 #undef GQ_FEW
   return gq_last_launch();
 }
-// x in registers (K <= 8192): any dtype and alignment of x, no workspace
+// x in registers (front_px): any dtype and alignment of x, no workspace
 template <int FMT, int XT, int NU>
 int launch_front_px_n(const void *wg, const void *wu, const void *x, void *h, void *go, void *uo, int dt, int M, int N,
                       int K, int act, hipStream_t s) {
@@ -1416,7 +1434,7 @@ int launch_front_px_n(const void *wg, const void *wu, const void *x, void *h, vo
   const int C = (int)gq_chunks(FMT, K), units = (int)(gq_kpad(FMT, K) / 128);
   const size_t so = gq_sc_plane_offset(FMT, N, K);
   const uint8_t *g8 = (const uint8_t *)wg, *u8 = (const uint8_t *)wu;
-    const dim3 grid((unsigned)(cus > 0 && tiles > cus ? cus : tiles)), block(64 * kPxWaves);
+  const dim3 grid((unsigned)(cus > 0 && tiles > cus ? cus : tiles)), block(64 * kPxWaves);
 #define GQ_PX(KERN) hipLaunchKernelGGL(KERN, grid, block, 0, s, g8, u8, so, x, h, go, uo, dt, M, N, K, C, units, act)
   if constexpr (XT != GQ_DT_F32) {
     if (M == 1) {
@@ -1529,7 +1547,7 @@ int check_front(int fmt, const void *gate, const void *up, size_t M, size_t N, s
   GQ_TRY(gq_check_shape(fmt, N, K));
   GQ_CHECK(M <= GQ_MAX_DIM, GQ_ERR_INVALID_ARGS);
   GQ_CHECK(gq_act_valid(act), GQ_ERR_UNSUPPORTED);
-  GQ_CHECK(gate && up, GQ_ERR_INVALID_ARGS);
+  GQ_CHECK((gate && up) || M == 0 || N == 0, GQ_ERR_INVALID_ARGS);
   // the kernels address a packed tensor with 32-bit offsets
   GQ_CHECK(N == 0 || K == 0 || gq_packed_bytes(fmt, N, K) < ((size_t)1 << 32), GQ_ERR_INVALID_ARGS);
   return GQ_OK;
@@ -1537,21 +1555,22 @@ int check_front(int fmt, const void *gate, const void *up, size_t M, size_t N, s
 
 }  // namespace
 
-
 constexpr size_t kFewRows = 4;
 // Rows that go into the few-row kernel without a conversion
 static bool front_as_it_is(const void *x, int x_dtype, size_t M) {
   return M <= kFewRows && x_dtype != GQ_DT_F32 && (uintptr_t)x % 4 == 0;
 }
-// Rows a call takes at a time: their fp16 copies stay below 64 MiB (and 32-bit offsets)
+// Rows a call takes at a time: their fp16 copies stay below 64 MiB, but for the rows that the kernels
+// of few rows take at once (32 of at most 2^24 columns: 1 GiB, 32-bit offsets still)
+constexpr size_t kOneBlock = 32;
 static size_t front_rows(int fmt, size_t M, size_t K) {
-  const size_t fit = (((size_t)64 << 20) / (2 * gq_kpad(fmt, K))) & ~(size_t)255;
-  const size_t mb = fit < 256 ? 256 : fit;
+  const size_t fit = ((size_t)64 << 20) / (2 * gq_kpad(fmt, K));
+  const size_t mb = fit >= 256 ? fit & ~(size_t)255 : fit > kOneBlock ? fit : kOneBlock;
   return M < mb ? M : mb;
 }
 
 extern "C" size_t gq_ffn_gate_up_workspace_bytes(int fmt, size_t M, size_t N, size_t K) {
-  if (!gq_fmt_valid(fmt) || M > GQ_MAX_DIM || N > GQ_MAX_DIM || K > GQ_MAX_DIM) return 0;
+  if (!gq_fmt_valid(fmt) || M > GQ_MAX_DIM || N > GQ_MAX_DIM || K > GQ_MAX_DIM || K == 0) return 0;
   const size_t mb = front_rows(fmt, M, K);
   return gq_align256(mb * (gq_kpad(fmt, K) + 8) * 2) + gq_align256((mb + 256) * 4);
 }
@@ -1561,10 +1580,9 @@ extern "C" int gq_ffn_gate_up(int fmt, const void *gate, const void *up, const v
                               size_t ws_bytes, void *stream) {
   GQ_TRY(check_front(fmt, gate, up, M, N, K, act));
   GQ_CHECK(gq_dtype_valid(x_dtype) && gq_dtype_valid(h_dtype), GQ_ERR_UNSUPPORTED);
-  GQ_CHECK(x && h, GQ_ERR_INVALID_ARGS);
   if (M == 0 || N == 0) return GQ_OK;
-  GQ_CHECK(K > 0, GQ_ERR_INVALID_ARGS);
-  GQ_CHECK(N * 256 * gq_dtype_size(h_dtype) < ((size_t)1 << 31), GQ_ERR_INVALID_ARGS);  // (a tile's rows of outputs)
+  GQ_CHECK(x && h && K > 0, GQ_ERR_INVALID_ARGS);
+  GQ_CHECK(N * 128 * gq_dtype_size(h_dtype) < ((size_t)1 << 31), GQ_ERR_INVALID_ARGS);  // (a tile's rows of outputs)
   hipStream_t s = (hipStream_t)stream;
   if (front_px(fmt, M, K))
     return launch_front_px(fmt, gate, up, x, x_dtype, h, g, u, h_dtype, (int)M, (int)N, (int)K, act, s);
@@ -1582,7 +1600,7 @@ extern "C" int gq_ffn_gate_up(int fmt, const void *gate, const void *up, const v
     GQ_TRY(gq_launch_a_to_f16(x, x_dtype, a16, rs, (int)M, (int)K, (int)K, 0, s));
     return launch_front_few(fmt, gate, up, a16, GQ_DT_F16, rs, h, g, u, h_dtype, (int)M, (int)N, (int)K, act, s);
   }
-  if (M <= 16 || (M <= 32 && gq_tiles(N) <= 400)) {  // rows 16 bytes longer than a multiple of 4 KiB, where 16 of them would collide
+  if (M <= 16 || (M <= kOneBlock && gq_tiles(N) <= 400)) {  // rows 16 bytes longer than a multiple of 4 KiB, where 16 of them would collide
     const int ld = (int)Kp + 8;
     GQ_TRY(gq_launch_a_to_f16(x, x_dtype, a16, rs, (int)M, (int)K, ld, q4, s));
     return launch_front_rows(fmt, gate, up, a16, ld, rs, h, g, u, h_dtype, (int)M, (int)N, (int)K, act, s);
@@ -1611,21 +1629,16 @@ constexpr DxShape kDxShapes[3] = {{32, 128, 4}, {64, 128, 4}, {128, 256, 2}};
 DxPlan dx_plan(size_t M, size_t N, size_t K) {
   DxPlan p;
   p.np = (gq_tiles(N) * 16 + 63) & ~(size_t)63;
-  // A below 120 MiB (and 32-bit offsets), whole tiles of rows
-  const size_t fit = (((size_t)120 << 20) / (4 * p.np)) & ~(size_t)255;
-  p.mb = fit < 256 ? 256 : fit;
+  // A below 120 MiB (what a scratch block holds with the rest), whole tiles of rows where they fit
+  const size_t fit = ((size_t)120 << 20) / (4 * p.np);  // (np <= 2^24: at least 1)
+  p.mb = fit < 256 ? fit : fit & ~(size_t)255;
   if (M < p.mb) p.mb = M;
   const size_t nsteps = 2 * p.np / 64;
-  p.shape = p.mb <= 32 ? 0 : p.mb <= 96 ? 1 : 2;
-#ifdef GQ_TUNE
-  if (getenv("GQ_BT")) p.shape = atoi(getenv("GQ_BT")) % 10;
-#endif
+  // (Q4_K, K = 4096: 128 x 14336 by the second shape 73.4 us, the third 94.5; 128 x 5003 41.4 and 54.8)
+  p.shape = p.mb <= 32 ? 0 : p.mb <= 128 ? 1 : 2;
   const DxShape &t = kDxShapes[p.shape];
   const size_t wgs = ((p.mb + t.bm - 1) / t.bm) * ((K + t.bn - 1) / t.bn);
   size_t want = wgs >= 192 ? 1 : 256 / wgs;
-#ifdef GQ_TUNE
-  if (getenv("GQ_BT") && atoi(getenv("GQ_BT")) >= 10) want = atoi(getenv("GQ_BT")) / 10;
-#endif
   const size_t most = nsteps / (4 * t.kg);  // at least four steps a group
   if (want > most) want = most < 1 ? 1 : most;
   p.sps = (int)((nsteps + want - 1) / want);
@@ -1666,6 +1679,12 @@ int launch_dx(const DxPlan &p, const void *wg, const void *wu, const _Float16 *a
   }
 #undef GQ_DX
 }
+int launch_dx_sum(const float *part, const float *rs, void *y, int dt, size_t M, size_t K, int parts, hipStream_t s) {
+  const size_t mk = M * K, wgs = (mk / 4 + 255) / 256;
+  GQ_CHECK(wgs <= 0x7FFFFFFFu, GQ_ERR_INVALID_ARGS);  // (one grid dimension)
+  hipLaunchKernelGGL(k_dx_sum, dim3((unsigned)wgs), dim3(256), 0, s, part, rs, y, dt, mk, (int)K, parts);
+  return gq_last_launch();
+}
 template <int DT>
 int launch_dgu(const void *dh, const void *g, const void *u, void *dg, void *du, _Float16 *a16, float *rs, int M, int N, int np,
                int act, hipStream_t s) {
@@ -1675,7 +1694,7 @@ int launch_dgu(const void *dh, const void *g, const void *u, void *dg, void *du,
 }  // namespace
 
 extern "C" size_t gq_ffn_gate_up_bwd_workspace_bytes(int fmt, size_t M, size_t N, size_t K) {
-  if (!gq_fmt_valid(fmt) || M == 0 || M > GQ_MAX_DIM || N > GQ_MAX_DIM || K > GQ_MAX_DIM || K == 0) return 0;
+  if (!gq_fmt_valid(fmt) || M > GQ_MAX_DIM || N > GQ_MAX_DIM || K > GQ_MAX_DIM || N == 0 || K == 0) return 0;
   // (never less for more rows: a block of fewer rows may have more parts)
   size_t most = 0;
   for (size_t m = M; m > 0; m /= 2) {
@@ -1690,9 +1709,11 @@ extern "C" int gq_ffn_gate_up_bwd(int fmt, const void *gate, const void *up, con
                                   size_t N, size_t K, int act, void *ws, size_t ws_bytes, void *stream) {
   GQ_TRY(check_front(fmt, gate, up, M, N, K, act));
   GQ_CHECK(gq_dtype_valid(dtype) && gq_dtype_valid(dx_dtype), GQ_ERR_UNSUPPORTED);
-  GQ_CHECK(dh && g && u, GQ_ERR_INVALID_ARGS);
-  if (M == 0 || K == 0 || (!dg && !du && !dx)) return GQ_OK;
+  if (M == 0 || (!dg && !du && !dx)) return GQ_OK;
+  GQ_CHECK(K > 0, GQ_ERR_INVALID_ARGS);
   hipStream_t s = (hipStream_t)stream;
+  if (N == 0) return dx ? launch_dx_sum(nullptr, nullptr, dx, dx_dtype, M, K, 0, s) : GQ_OK;  // (sums of nothing)
+  GQ_CHECK(dh && g && u, GQ_ERR_INVALID_ARGS);
   const DxPlan plan = dx_plan(M, N, K);
   const size_t need = dx ? gq_ffn_gate_up_bwd_workspace_bytes(fmt, M, N, K) : 0;
   GqScratch sc(ws ? 0 : need, s);
@@ -1716,12 +1737,7 @@ extern "C" int gq_ffn_gate_up_bwd(int fmt, const void *gate, const void *up, con
     else if (fmt == GQ_FMT_Q8_0) GQ_TRY(launch_dx<GQ_FMT_Q8_0>(plan, gate, up, a16, rs, to, dx_dtype, m, N, K, s));
     else if (gq_fmt_is_q6k(fmt)) GQ_TRY(launch_dx<GQ_FMT_Q6_K>(plan, gate, up, a16, rs, to, dx_dtype, m, N, K, s));
     else GQ_TRY(launch_dx<GQ_FMT_Q4_K>(plan, gate, up, a16, rs, to, dx_dtype, m, N, K, s));
-    if (plan.parts > 1) {
-      const size_t mk = (size_t)m * K;
-      hipLaunchKernelGGL(k_dx_sum, dim3((unsigned)((mk / 4 + 255) / 256)), dim3(256), 0, s, part, rs, y, dx_dtype, mk, (int)K,
-                         plan.parts);
-      GQ_TRY(gq_last_launch());
-    }
+    if (plan.parts > 1) GQ_TRY(launch_dx_sum(part, rs, y, dx_dtype, (size_t)m, K, plan.parts, s));
   }
   return GQ_OK;
 }

@@ -267,9 +267,11 @@ int gq_launch_gemm_mfma_mixed_f16f32(void *stream, const float *a, const void *b
 #define GQ_ACT_GELU_TANH 1 /* g / 2 (1 + tanh(sqrt(2 / pi) (g + 0.044715 g^3))) */
 /* A workspace of NULL takes scratch memory of the call's own, which needs no room
  * from the caller and does not race with other calls; there is none while the stream
- * is being captured, where a call without a workspace returns GQ_ERR_WORKSPACE.
- * Calls that overlap must not share a workspace.  Rows are taken in blocks, so the
- * workspace stops growing with M. */
+ * is being captured, where a call that needs one (up to 16 rows of K <= 4096 and 32 of
+ * K <= 2048 do not) returns GQ_ERR_WORKSPACE, as does one of K above 2^21.
+ * Calls that overlap must not share a workspace, and neither may two captured graphs
+ * whose replays overlap.  Rows are taken in blocks, so the workspace stops growing
+ * with M.  N * 128 outputs stay below 2^31 bytes; K == 0 is refused. */
 size_t gq_ffn_gate_up_workspace_bytes(int fmt, size_t M, size_t N, size_t K);
 int gq_ffn_gate_up(int fmt, const void *d_gate, const void *d_up, const void *d_x, int x_dtype, void *d_h,
                    int h_dtype, void *d_g, void *d_u, size_t M, size_t N, size_t K, int act, void *d_workspace,

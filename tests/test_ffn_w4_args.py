@@ -46,13 +46,19 @@ def test_front_refuses(call, bad, status):
 def test_front_refuses_its_own():
     assert front(hdt=7) == UNSUPPORTED
     assert front(x=None) == INVALID and front(h=None) == INVALID and front(k=0) == INVALID
+    assert front(n=1 << 22, k=32, hdt=gq.DT_F32) == INVALID  # (offsets of a tile's outputs)
+    assert bwd(k=0) == INVALID
     assert bwd(dt=7) == UNSUPPORTED
     assert bwd(dh=None) == INVALID and bwd(g=None) == INVALID and bwd(u=None) == INVALID
 
 
 def test_empty_calls():
     assert front(m=0) == OK and front(n=0) == OK
-    assert bwd(m=0) == OK and bwd(k=0) == OK
+    assert bwd(m=0) == OK and bwd(n=0, dx=None) == OK and bwd(n=0, gate=None, up=None, dh=None, g=None, u=None, dx=None) == OK
+    assert front(m=0, x=None, h=None) == OK and front(n=0, gate=None, up=None, h=None) == OK and bwd(m=0, dh=None, dx=P) == OK
+    for size in (gq.ffn_gate_up_workspace_bytes, gq.ffn_gate_up_bwd_workspace_bytes):
+        assert size(gq.FMT_Q4_0, 5, 64, 0) == 0
+    assert gq.ffn_gate_up_bwd_workspace_bytes(gq.FMT_Q4_0, 5, 0, 64) == 0
     assert bwd(dg=None, du=None, dx=None) == OK  # nothing wanted
     assert w4(n=0) == OK and w4_front(n=0) == OK
 
@@ -98,6 +104,17 @@ def test_workspaces_stop_growing(fmt):
         at = [size(fmt, m, 14336, 4096) for m in (1, 16, 64, 300, 2048, 20000, 1 << 20)]
         assert at == sorted(at) and at[-1] <= 1 << 30
         assert size(99, 16, 64, 256) == 0 and size(fmt, BIG, 64, 256) == 0
+
+
+@pytest.mark.parametrize("fmt", sorted(set(gq.FORMATS.values())))
+@pytest.mark.parametrize("m", [1, 17, 33, 300, 5000])
+def test_scratch_suffices_for_long_rows(fmt, m):
+    """Blocks of rows get shorter as the rows get longer: a call without a workspace fits what it may take by itself
+    (128 MiB), up to a front's K of 2^21 and any N of a backward pass."""
+    for k in (256, 4096, 1 << 17, 1 << 20):
+        assert 0 < gq.ffn_gate_up_workspace_bytes(fmt, m, 64, k) <= 128 << 20
+    for n in (16, 14336, 1 << 20, 1 << 22, 1 << 24):
+        assert 0 < gq.ffn_gate_up_bwd_workspace_bytes(fmt, m, n, 256) <= 128 << 20
 
 
 def test_binding_refuses_host_tensors_and_shapes():

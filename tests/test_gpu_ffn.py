@@ -349,6 +349,55 @@ def test_small_workspace_is_refused(dev):
         torch.cuda.synchronize()
 
 
+def test_blocks_of_fewer_rows(dev):
+    """Rows so long that a block holds fewer than 256 of them: three blocks, the last one ragged, scratch of the call's own."""
+    import gq
+    m, n, k = 300, 20, 1 << 18
+    c = Case(dev, O.Q4_K, m, n, k, seed=1)
+    check_front(c, 0, gq.ffn_gate_up(O.Q4_K, *c.packed, c.x, n, k, save=True), torch.bfloat16)
+    m, n, k = 500, 1 << 17, 32
+    c = Case(dev, O.Q4_0, m, n, k, seed=2)
+    check_grads(c, 0, gq.ffn_gate_up_bwd(O.Q4_0, *c.packed, c.dh, c.g, c.u, n, k), torch.bfloat16)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_no_columns_between(dev, dtype):
+    """N = 0: dx is a sum of nothing."""
+    import gq
+    m, k = 5, 256
+    e, w = torch.empty(m, 0, dtype=dtype, device=dev), torch.empty(0, dtype=torch.uint8, device=dev)
+    dx = torch.full((m + 1, k), 7.0, dtype=dtype, device=dev)
+    out = gq.ffn_gate_up_bwd(O.Q8_0, w, w, e, e, e, 0, k, dx=dx[:m])
+    assert bool((dx[:m] == 0).all()) and bool((dx[m:] == 7).all()) and out["dg"].shape == (m, 0)
+    assert gq.ffn_gate_up(O.Q8_0, w, w, dx[:m], 0, k).shape == (m, 0)
+    x = torch.empty(0, k, dtype=dtype, device=dev)
+    full = Case(dev, O.Q8_0, 1, 16, k).packed
+    assert gq.ffn_gate_up(O.Q8_0, *full, x, 16, k).shape == (0, 16)
+
+
+def test_capture_without_a_workspace(dev):
+    """A call that needs a workspace takes none of its own while its stream is captured; one that needs none is captured."""
+    import gq
+    fmt, n, k = O.Q4_K, 64, 512
+    c, few = Case(dev, fmt, 40, n, k), Case(dev, fmt, 3, n, k)
+    h = torch.empty(3, n, dtype=torch.bfloat16, device=dev)
+    ref = gq.ffn_gate_up(fmt, *few.packed, few.x, n, k)
+    out, dx = torch.empty(40, n, dtype=torch.bfloat16, device=dev), torch.empty_like(c.x)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        with pytest.raises(gq.GQError):
+            gq.ffn_gate_up(fmt, *c.packed, c.x, n, k, h=out)
+        with pytest.raises(gq.GQError):
+            gq.ffn_gate_up_bwd(fmt, *c.packed, c.dh, c.g, c.u, n, k, dx=dx, want_dgu=False)
+        gq.ffn_gate_up(fmt, *few.packed, few.x, n, k, h=h)
+    for _ in range(3):
+        h.fill_(float("nan"))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(h, ref)
+
+
 def test_block_trains_and_decodes(dev):
     """The operators as they are used together: a prompt through the block's front and the down projection, the
     backward pass of both ends, then single tokens that agree with the prompt's rows and with the f32 decode front."""
