@@ -659,8 +659,8 @@ k_front_rows_px(const uint8_t *__restrict__ wg, const uint8_t *__restrict__ wu, 
         }
       top = fmaxf(top, __shfl_xor(top, 16, 64));
       top = fmaxf(top, __shfl_xor(top, 32, 64));
-      // 2^s, s = 14 - floor(log2(top)) cut to +-100 (0, Inf: any)
-      const int sh = 14 + 127 - (int)((__float_as_uint(top) >> 23) & 0xFFu), cut = sh < -100 ? -100 : sh > 100 ? 100 : sh;
+      // 2^s, s = 14 - floor(log2(top)) at most 126 (at least -114: both have a normal inverse)
+      const int sh = 14 + 127 - (int)((__float_as_uint(top) >> 23) & 0xFFu), cut = sh > 126 ? 126 : sh;
       const float f2 = __uint_as_float((uint32_t)(127 + cut) << 23), inv = __uint_as_float((uint32_t)(127 - cut) << 23);
 #pragma unroll
       for (int v = 0; v < 4; ++v) back[t][v] = __shfl(inv, 4 * g + v, 64);
@@ -928,7 +928,7 @@ k_front_rb(const uint8_t *__restrict__ wg, const uint8_t *__restrict__ wu, uint3
 // ---- backward --------------------------------------------------------------------
 // dg = dh u act'(g), du = dh act(g): one pass over dh, g, u, a workgroup a row.  The products
 // go out in their own type where they are wanted, and, as they are before that rounding, to fp16
-// [dg | du] with one power-of-two scale per row (the row's largest to [2^14, 2^15)), the A operand of
+// [dg | du] with one power-of-two scale per row (the row's largest to [2^14, 2^15); 2^-114 to 2^126), the A operand of
 // dx, each half padded with zeros to np columns (whole steps of 64).  The first 4096 x 4 columns of a
 // row stay in registers between the maximum and the conversion, the rest is computed twice.
 GQ_DEV void front_grads(int act, float dh, float g, float u, float &dg, float &du) {
@@ -1025,7 +1025,7 @@ __global__ void __launch_bounds__(kDguThreads) k_front_dgu(const void *dh, const
     __syncthreads();
 #pragma unroll
     for (int w = 0; w < kDguThreads / 64; ++w) top = fmaxf(top, top_s[w]);
-    const int sh = 14 + 127 - (int)((__float_as_uint(top) >> 23) & 0xFFu), cut = sh < -100 ? -100 : sh > 100 ? 100 : sh;
+    const int sh = 14 + 127 - (int)((__float_as_uint(top) >> 23) & 0xFFu), cut = sh > 126 ? 126 : sh;
     f2 = __uint_as_float((uint32_t)(127 + cut) << 23);
     if (tid == 0) rs[blockIdx.x] = __uint_as_float((uint32_t)(127 - cut) << 23);
   }
@@ -1164,8 +1164,9 @@ __global__ void __launch_bounds__(64 * WN * KG) k_front_dx(const uint8_t *__rest
       const int rec = wave * RPW + i;  // [column block][tile][record]
       const int b = rec / (4 * RECS), t = rec / RECS % 4, h = rec % RECS;
       const uint32_t kc = (uint32_t)(kc0 + b), c = kSuper<FMT> ? kc >> 1 : kc, p = kSuper<FMT> ? kc & 1u : 0u;
-      uint32_t o = ((t0 + (uint32_t)t) * (uint32_t)C + c) * HFmt<FMT>::QB;
-      uint32_t v = slot;
+      uint32_t v = slot, o = t0 + (uint32_t)t < (uint32_t)ntiles && c < (uint32_t)C  // (outside: any record, its scales are zero)
+                                 ? ((t0 + (uint32_t)t) * (uint32_t)C + c) * HFmt<FMT>::QB
+                                 : 0u;
       if constexpr (FMT == GQ_FMT_Q8_0) {
         o += 1024u * (uint32_t)h;
         v ^= h ? 16u : 0u;
@@ -1548,8 +1549,9 @@ int check_front(int fmt, const void *gate, const void *up, size_t M, size_t N, s
   GQ_CHECK(M <= GQ_MAX_DIM, GQ_ERR_INVALID_ARGS);
   GQ_CHECK(gq_act_valid(act), GQ_ERR_UNSUPPORTED);
   GQ_CHECK((gate && up) || M == 0 || N == 0, GQ_ERR_INVALID_ARGS);
-  // the kernels address a packed tensor with 32-bit offsets
-  GQ_CHECK(N == 0 || K == 0 || gq_packed_bytes(fmt, N, K) < ((size_t)1 << 32), GQ_ERR_INVALID_ARGS);
+  GQ_CHECK((((uintptr_t)gate | (uintptr_t)up) & 15) == 0, GQ_ERR_INVALID_ARGS);  // (16-byte loads)
+  // the kernels address a packed tensor with 32-bit offsets (the last 4 KiB: those that lie outside)
+  GQ_CHECK(N == 0 || K == 0 || gq_packed_bytes(fmt, N, K) <= 0xFFFFF000u, GQ_ERR_INVALID_ARGS);
   return GQ_OK;
 }
 
@@ -1593,6 +1595,7 @@ extern "C" int gq_ffn_gate_up(int fmt, const void *gate, const void *up, const v
   if (ws) GQ_CHECK(ws_bytes >= need, GQ_ERR_WORKSPACE);
   else ws = sc.ptr;
   GQ_CHECK(ws, GQ_ERR_WORKSPACE);
+  GQ_CHECK(((uintptr_t)ws & 15) == 0, GQ_ERR_INVALID_ARGS);
   _Float16 *a16 = (_Float16 *)ws;
   float *rs = (float *)((uint8_t *)ws + gq_align256(mb * (Kp + 8) * 2));
   const int q4 = fmt == GQ_FMT_Q4_0 || gq_fmt_is_q4k(fmt);
@@ -1720,6 +1723,7 @@ extern "C" int gq_ffn_gate_up_bwd(int fmt, const void *gate, const void *up, con
   if (ws) GQ_CHECK(ws_bytes >= need, GQ_ERR_WORKSPACE);
   else ws = sc.ptr;
   GQ_CHECK(ws || !dx, GQ_ERR_WORKSPACE);
+  GQ_CHECK(((uintptr_t)ws & 15) == 0, GQ_ERR_INVALID_ARGS);
   _Float16 *a16 = dx ? (_Float16 *)ws : nullptr;
   float *rs = dx ? (float *)((uint8_t *)ws + dx_a_bytes(plan)) : nullptr;
   float *part = dx ? (float *)((uint8_t *)rs + dx_rs_bytes(plan)) : nullptr;

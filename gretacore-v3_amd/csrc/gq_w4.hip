@@ -26,6 +26,9 @@ size_t w4_bytes(size_t N, size_t K, int group) {
   return w4_meta_off(N, K) + gq_tiles(N) * w4_chunks(K) * (size_t)(16 * 4 * (kW4Chunk / group));
 }
 
+struct __attribute__((packed, aligned(1))) W4Bytes4 {
+  uint32_t v;
+};
 // one word of codes, or one meta word, a thread
 __global__ void __launch_bounds__(256) k_w4_pack(const uint8_t *__restrict__ q, const uint16_t *__restrict__ s, int sbf16,
                                                  const uint8_t *__restrict__ z, size_t N, size_t K, int group,
@@ -36,14 +39,20 @@ __global__ void __launch_bounds__(256) k_w4_pack(const uint8_t *__restrict__ q, 
   if (i < n_code) {
     const size_t lane = (i >> 2) & 63, tc = i >> 8;
     const size_t n = (tc / C) * 16 + (lane & 15), k = (tc % C) * kW4Chunk + 32 * (i & 3) + 8 * (lane >> 4);
+    uint32_t v = 0;  // the row's four bytes, even k in the low nibbles
+    if (n < N && k + 8 <= K) {
+      v = reinterpret_cast<const W4Bytes4 *>(q + n * rb + k / 2)->v;
+    } else if (n < N) {
+      for (int e = 0; e < 8; ++e)
+        if (k + e < K) v |= (uint32_t)((q[n * rb + ((k + e) >> 1)] >> (4 * (e & 1))) & 15u) << (4 * e);
+    }
+    // code e to bit 3 + 16 (e % 2) + 4 (e / 2) of 32
     uint32_t w = 0;
-    for (int e = 0; e < 8; ++e)
-      if (n < N && k + e < K) {
-        const uint32_t c = (q[n * rb + ((k + e) >> 1)] >> (4 * (e & 1))) & 15u;
-        const int at = 3 + 16 * (e & 1) + 4 * (e >> 1);
-        w |= at < 32 ? c << at : 0u;
-        w |= at > 28 ? c >> (32 - at) : 0u;
-      }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const int at = 3 + 16 * (e & 1) + 4 * (e >> 1);
+      w |= __builtin_rotateleft32((v >> (4 * e)) & 15u, at & 31);
+    }
     codes[i] = w;
   } else if (i - n_code < n_meta) {
     const size_t j = i - n_code, per = kW4Chunk / group;
@@ -391,9 +400,9 @@ int launch_w4(W4Mats mats, int group, const void *x, int x_dtype, void *y, int y
   GQ_CHECK(gq_dtype_valid(x_dtype) && gq_dtype_valid(y_dtype), GQ_ERR_UNSUPPORTED);
   GQ_CHECK(MATS == 1 || gq_act_valid(act), GQ_ERR_UNSUPPORTED);
   GQ_CHECK(batch >= 1 && batch <= GQ_MAX_BATCH, GQ_ERR_UNSUPPORTED);
-  GQ_CHECK(mats.w[0] && mats.w[MATS - 1] && x && y, GQ_ERR_INVALID_ARGS);
   if (N == 0) return GQ_OK;
-  GQ_CHECK(K > 0, GQ_ERR_INVALID_ARGS);
+  GQ_CHECK(mats.w[0] && mats.w[MATS - 1] && x && y && K > 0, GQ_ERR_INVALID_ARGS);
+  GQ_CHECK((((uintptr_t)mats.w[0] | (uintptr_t)mats.w[MATS - 1]) & 15) == 0, GQ_ERR_INVALID_ARGS);  // (16-byte loads)
   const int n = (int)N, k = (int)K;
   if (x_dtype == GQ_DT_F32) return launch_w4_group<MATS, GQ_DT_F32>(mats, group, x, y, y_dtype, n, k, batch, act, s);
   if (x_dtype == GQ_DT_F16) return launch_w4_group<MATS, GQ_DT_F16>(mats, group, x, y, y_dtype, n, k, batch, act, s);
@@ -414,8 +423,8 @@ extern "C" int gq_w4_pack(const uint8_t *q, const void *scales, int scale_dtype,
   GQ_TRY(check_w4(group, N, K));
   // (an fp32 scale would have to be rounded)
   GQ_CHECK(scale_dtype == GQ_DT_F16 || scale_dtype == GQ_DT_BF16, GQ_ERR_UNSUPPORTED);
-  GQ_CHECK(q && scales && packed, GQ_ERR_INVALID_ARGS);
   if (N == 0 || K == 0) return GQ_OK;
+  GQ_CHECK(q && scales && packed && ((uintptr_t)packed & 15) == 0, GQ_ERR_INVALID_ARGS);
   const size_t codes = w4_meta_off(N, K) / 4, meta = w4_bytes(N, K, group) / 4 - codes;
   GQ_CHECK((codes + meta + 255) / 256 <= 0x7FFFFFFFu, GQ_ERR_INVALID_ARGS);
   hipLaunchKernelGGL(k_w4_pack, dim3((unsigned)((codes + meta + 255) / 256)), dim3(256), 0, (hipStream_t)stream, q,

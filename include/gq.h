@@ -258,7 +258,7 @@ int gq_launch_gemm_mfma_mixed_f16f32(void *stream, const float *a, const void *b
  * h[m][n] = act(g[m][n]) * u[m][n] with g = x W_gate^T, u = x W_up^T: gq_gemv_swiglu's
  * block without its normalisation, for prompts, batches and training.  x is
  * [M][K] of x_dtype, h [M][N] of h_dtype, both contiguous; W_gate and W_up are T16
- * tensors of one format.  d_g and d_u (NULL: not wanted) receive the two products,
+ * tensors of one format (they and the workspace 16-byte aligned).  d_g and d_u (NULL: not wanted) receive the two products,
  * of h_dtype, as gq_ffn_gate_up_bwd takes them.  fp16 matrix cores, fp32 sums, as
  * gq_gemm: x is rounded to fp16 after a power-of-two scale per row, each weight once
  * to fp16, which for fp32 outputs leaves about 3e-4 of a row's norm.  Every output is

@@ -38,6 +38,8 @@ BIG = (1 << 24) + 32
     (dict(k=BIG), INVALID), (dict(m=BIG), INVALID), (dict(gate=None), INVALID), (dict(up=None), INVALID),
     # a packed tensor of 4 GiB and more
     (dict(fmt=gq.FMT_Q8_0, n=1 << 20, k=4096), INVALID),
+    # packed tensors that are not 16-byte aligned
+    (dict(gate=P + 8), INVALID), (dict(up=P + 1), INVALID),
 ])
 def test_front_refuses(call, bad, status):
     assert call(**bad) == status
@@ -60,7 +62,7 @@ def test_empty_calls():
         assert size(gq.FMT_Q4_0, 5, 64, 0) == 0
     assert gq.ffn_gate_up_bwd_workspace_bytes(gq.FMT_Q4_0, 5, 0, 64) == 0
     assert bwd(dg=None, du=None, dx=None) == OK  # nothing wanted
-    assert w4(n=0) == OK and w4_front(n=0) == OK
+    assert w4(n=0) == OK and w4_front(n=0) == OK and w4(n=0, w=None, y=None) == OK
 
 
 @pytest.mark.parametrize("call", [w4, w4_front])
@@ -74,6 +76,7 @@ def test_w4_refuses(call, bad, status):
 
 
 def test_w4_refuses_its_own():
+    assert w4(w=P + 4) == INVALID and w4_front(up=P + 8) == INVALID and w4_front(gate=P + 1) == INVALID
     assert w4(w=None) == INVALID and w4(y=None) == INVALID and w4(ydt=9) == UNSUPPORTED
     assert w4_front(gate=None) == INVALID and w4_front(up=None) == INVALID and w4_front(h=None) == INVALID
     assert w4_front(act=5) == UNSUPPORTED and w4_front(hdt=9) == UNSUPPORTED
@@ -84,6 +87,7 @@ def test_w4_refuses_its_own():
         args = [P, P, gq.DT_F16, P, 16, 128, 128, P, None]
         args[i] = None
         assert pack(*args) == INVALID
+    assert pack(P, P, gq.DT_F16, P, 16, 128, 128, P + 4, None) == INVALID
     assert pack(P, P, gq.DT_F16, None, 0, 128, 128, P, None) == OK
     size = ctypes.c_size_t(0)
     assert gq.load().gq_w4_packed_size(16, 128, 128, None) == INVALID

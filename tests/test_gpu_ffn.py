@@ -204,6 +204,19 @@ def test_sizes_of_rows(dev, m):
     assert worst_row(dx, c.grads(0)[0]) <= PRODUCT
 
 
+@pytest.mark.parametrize("m", [3, 40, 200])
+@pytest.mark.parametrize("size", [-112, -60, 60, 117])
+def test_sizes_of_gradients(dev, m, size):
+    """dh of any size that leaves dx a normal fp32: its row's power of two takes it into fp16 and back.  2^size times 0.1 e^N(0,1),
+    u act'(g) of 1.5: dg 2^-115 (normal: 2^-126) to 2^120; dx of one to a few times that."""
+    import gq
+    fmt, n, k = O.Q8_0, 200, 256
+    c = Case(dev, fmt, m, n, k, seed=11, dtype=torch.float32)
+    c.dh *= 2.0 ** size
+    out = gq.ffn_gate_up_bwd(fmt, *c.packed, c.dh, c.g, c.u, n, k, want_dgu=False)
+    assert worst_row(out["dx"], c.grads(0)[0]) <= PRODUCT + half_step(torch.float32)
+
+
 @pytest.mark.parametrize("m", [2, 16, 40, 200])
 @pytest.mark.parametrize("bad", [np.nan, np.inf, -np.inf])
 def test_nonfinite_rows(dev, m, bad):
