@@ -262,7 +262,7 @@ int gq_launch_gemm_mfma_mixed_f16f32(void *stream, const float *a, const void *b
  * of h_dtype, as gq_ffn_gate_up_bwd takes them.  fp16 matrix cores, fp32 sums, as
  * gq_gemm: x is rounded to fp16 after a power-of-two scale per row, each weight once
  * to fp16, which for fp32 outputs leaves about 3e-4 of a row's norm.  Every output is
- * rounded once from fp32. */
+ * rounded once from fp32.  h, g and u overlap nothing else. */
 #define GQ_ACT_SILU 0      /* g / (1 + e^-g) */
 #define GQ_ACT_GELU_TANH 1 /* g / 2 (1 + tanh(sqrt(2 / pi) (g + 0.044715 g^3))) */
 /* A workspace of NULL takes scratch memory of the call's own, which needs no room
