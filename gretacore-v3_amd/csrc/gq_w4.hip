@@ -357,6 +357,9 @@ k_w4(W4Mats mats, size_t meta_off, const void *__restrict__ x, void *__restrict_
 //    6000 x 14336 20.1 and 17.8)
 //  * four tiles on 4 waves from where two give more than a round of workgroups: 14336 x 4096
 //    8 rows 10.7, two tiles 12.1; 32000 x 4096 two rows of fp32 18.9 and 21.1
+//  * these on 8 waves where one round of workgroups holds them and a chunk's work is long (groups of 32) or K
+//    is: 8 rows of 14336 x 4096, group 32, 11.5, on 4 waves 13.3; 11008 x 8192 17.9 and 21.6, group 64 fp32 22.3 and
+//    25.3; but 32000 x 4096 group 32 22.3 and 20.4, 14336 x 4096 group 128 16 rows 11.1 and 10.9
 template <int MATS, int XT, int GW, bool FEW>
 int launch_w4_shape(W4Mats mats, const void *x, void *y, int ydt, int N, int K, int batch, int act, hipStream_t s) {
   const size_t tiles = gq_tiles(N), tt = tiles * MATS, mo = w4_meta_off(N, K);
@@ -370,6 +373,8 @@ int launch_w4_shape(W4Mats mats, const void *x, void *y, int ydt, int N, int K, 
   } else if (tt <= two) {
     if (FEW ? tt <= 1000 : C >= 64) GQ_W4(2 / MATS, 8);
     else GQ_W4(2 / MATS, 4);
+  } else if (MATS == 1 && !FEW && tt <= 1024 && (GW == 4 || C >= 64)) {
+    if constexpr (MATS == 1 && !FEW) GQ_W4(4, 8);
   } else {
     GQ_W4(4 / MATS, 4);
   }

@@ -78,6 +78,22 @@ def test_gate_up(dev, group, dtype, m, n, k):
         check(h, act_grad(act, g)[0] * u, extra=8.0)
 
 
+# matrices of so many rows that workgroups take four tiles, on four waves and on eight; K with and without a tail
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("m,n,k", [(3, 22500, 130), (7, 9700, 300), (16, 16401, 256), (12, 9650, 8200), (5, 17000, 129)])
+def test_wide(dev, group, dtype, m, n, k):
+    import gq
+    print(f"m={m} n={n} k={k} group={group} {dtype}", flush=True)
+    p, w = make(dev, n, k, group, seed=n)
+    x = make_x(dev, m, k, dtype, n)
+    check(gq.w4_gemv(p, group, x, n, k), x.double() @ w.t().contiguous())
+    if k < 1000:
+        h = gq.w4_gate_up(p, p, group, (x.double() / k ** 0.5 * 20).to(dtype), n, k)
+        g = (x.double() / k ** 0.5 * 20).to(dtype).double() @ w.t().contiguous()
+        check(h, act_grad(0, g)[0] * g, extra=8.0)
+
+
 @pytest.mark.parametrize("xdt", DTYPES)
 @pytest.mark.parametrize("ydt", DTYPES)
 @pytest.mark.parametrize("m", [1, 6, 16])
