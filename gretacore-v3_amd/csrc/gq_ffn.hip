@@ -938,9 +938,6 @@ GQ_DEV void front_grads(int act, float dh, float g, float u, float &dg, float &d
   du = dh * f;
 }
 constexpr int kDguThreads = 512, kDguRuns = 4;
-struct __attribute__((packed, aligned(2))) FStore16 {
-  gq_u4 v;
-};
 // 8 values of a row of n from column k on (zeros behind it)
 template <int DT>
 GQ_DEV void dgu_load(const void *p, size_t row, int k, int n, float (&o)[8]) {
@@ -962,7 +959,7 @@ GQ_DEV void dgu_store(void *p, size_t row, int k, int n, const float (&v)[8]) {
       r.v[1] = gq_f4{v[4], v[5], v[6], v[7]};
       *reinterpret_cast<FRun32 *>(reinterpret_cast<float *>(p) + row + k) = r;
     } else {
-      FStore16 r;
+      FRun16 r;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const uint32_t lo = DT == GQ_DT_BF16 ? gq_f32_to_bf16(v[2 * e]) : __builtin_bit_cast(uint16_t, (_Float16)v[2 * e]);
@@ -970,7 +967,7 @@ GQ_DEV void dgu_store(void *p, size_t row, int k, int n, const float (&v)[8]) {
             DT == GQ_DT_BF16 ? gq_f32_to_bf16(v[2 * e + 1]) : __builtin_bit_cast(uint16_t, (_Float16)v[2 * e + 1]);
         r.v[e] = lo | hi << 16;
       }
-      *reinterpret_cast<FStore16 *>(reinterpret_cast<uint16_t *>(p) + row + k) = r;
+      *reinterpret_cast<FRun16 *>(reinterpret_cast<uint16_t *>(p) + row + k) = r;
     }
   } else {
 #pragma unroll
