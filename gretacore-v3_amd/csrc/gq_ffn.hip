@@ -1139,13 +1139,15 @@ __global__ void __launch_bounds__(64 * WN * KG) k_front_dx(const uint8_t *__rest
   // this workgroup's steps of 64 n (part blockIdx.y), this group's every KG-th
   const int s0 = (int)blockIdx.y * sps, s1 = s0 + sps < nsteps ? s0 + sps : nsteps;
   const int nl = (s1 - s0 + KG - 1) / KG;
+  __builtin_assume(nl > 0);  // (no part is empty; under a branch around the loop the loads in front of it may sink)
   const int lda = 64 * nsteps;
   auto stage = [&](int i) { return (i == 0 ? lds_0 : i == 1 ? lds_1 : lds_2) + kg * STAGE; };
   auto table = [&](int i) { return reinterpret_cast<_Float16 *>(stage(i) + A_B + W_B); };
   uint32_t ao[BM / (8 * NW)];
   a_offsets<BM, NW>(lda, M, m0, wave, lane, ao);
-  const __amdgpu_buffer_rsrc_t rg = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t *>(wg), (short)0, (int)w_bytes, 0x00020000);
-  const __amdgpu_buffer_rsrc_t ru = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t *>(wu), (short)0, (int)w_bytes, 0x00020000);
+  auto mat = [&](bool up) __attribute__((always_inline)) {  // (the pointer is chosen, not one of two resources in memory)
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t *>(up ? wu : wg), (short)0, (int)w_bytes, 0x00020000);
+  };
   // the record's slot a lane fetches: 16 g + (rho ^ 2 g), Q8_0's second half-record (64 k on) ^ 1 more
   const uint32_t slot = 16u * (16u * (uint32_t)(lane >> 4) + (uint32_t)((lane & 15) ^ (2 * (lane >> 4))));
   auto step_of = [&](int l) { return s0 + l * KG + kg; };  // (past the part's end: skipped by the sums, A zero or not used)
@@ -1154,6 +1156,7 @@ __global__ void __launch_bounds__(64 * WN * KG) k_front_dx(const uint8_t *__rest
     s = s < s1 ? s : s1 - 1;
     load_a_lds_b<BM, NW>(a16, ao, s, wave, reinterpret_cast<_Float16 *>(stage(st)));
     const bool up = 2 * s >= nsteps;
+    const __amdgpu_buffer_rsrc_t wr = mat(up);
     const uint32_t t0 = 4u * (uint32_t)(up ? s - nsteps / 2 : s);
     uint8_t *wl = stage(st) + A_B;
 #pragma unroll
@@ -1161,9 +1164,9 @@ __global__ void __launch_bounds__(64 * WN * KG) k_front_dx(const uint8_t *__rest
       const int rec = wave * RPW + i;  // [column block][tile][record]
       const int b = rec / (4 * RECS), t = rec / RECS % 4, h = rec % RECS;
       const uint32_t kc = (uint32_t)(kc0 + b), c = kSuper<FMT> ? kc >> 1 : kc, p = kSuper<FMT> ? kc & 1u : 0u;
-      uint32_t v = slot, o = t0 + (uint32_t)t < (uint32_t)ntiles && c < (uint32_t)C  // (outside: any record, its scales are zero)
-                                 ? ((t0 + (uint32_t)t) * (uint32_t)C + c) * HFmt<FMT>::QB
-                                 : 0u;
+      // (outside: the last record, its scales are zero; clamped without a branch, which would copy the DMAs)
+      const uint32_t tt = min(t0 + (uint32_t)t, (uint32_t)ntiles - 1u), cc = min(c, (uint32_t)C - 1u);
+      uint32_t v = slot, o = (tt * (uint32_t)C + cc) * HFmt<FMT>::QB;
       if constexpr (FMT == GQ_FMT_Q8_0) {
         o += 1024u * (uint32_t)h;
         v ^= h ? 16u : 0u;
@@ -1172,8 +1175,7 @@ __global__ void __launch_bounds__(64 * WN * KG) k_front_dx(const uint8_t *__rest
       } else {
         o += 1024u * p;
       }
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(up ? ru : rg, (__attribute__((address_space(3))) void *)(wl + 1024 * rec), 16, v,
-                                               o, 0, 0);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(wr, (__attribute__((address_space(3))) void *)(wl + 1024 * rec), 16, v, o, 0, 0);
     }
   };
   // scales: a wave those of its own column block, a row a lane
@@ -1184,7 +1186,7 @@ __global__ void __launch_bounds__(64 * WN * KG) k_front_dx(const uint8_t *__rest
     const bool up = 2 * s >= nsteps;
     const uint32_t t = 4u * (uint32_t)(up ? s - nsteps / 2 : s) + (uint32_t)stile, kc = (uint32_t)(kc0 + wave);
     const uint32_t c = kSuper<FMT> ? kc >> 1 : kc;
-    return dx_load_scales<FMT>(up ? ru : rg, sc_off, t * (uint32_t)C + c, kSuper<FMT> ? kc & 1u : 0u, (uint32_t)srow,
+    return dx_load_scales<FMT>(mat(up), sc_off, t * (uint32_t)C + c, kSuper<FMT> ? kc & 1u : 0u, (uint32_t)srow,
                                t < (uint32_t)ntiles && c < (uint32_t)C);
   };
   auto store_scales = [&](const gq_u4 &v, int st) __attribute__((always_inline)) {
@@ -1295,13 +1297,17 @@ __global__ void __launch_bounds__(64 * WN * KG) k_front_dx(const uint8_t *__rest
 
   // Step l computes from stage l % PD; the loads of step l + PD - 1 go into the stage step l - 1 has
   // left, the scales of l + 2 into registers, those of l + 1 from there to LDS.  At its end the DMA of l + 1
-  // must have landed: of what was issued behind it the scales of l + 2 (l + 1) and later DMAs may be open.
+  // must have landed.  Every step issues its DMAs first and its scales behind them (kept so by the
+  // sched_barriers: the count is of that order), so behind the DMA of l + 1 come, PD = 2, the scales of l + 2; PD =
+  // 3, those of l + 1, the DMA of l + 2 and the scales of l + 2.
   constexpr int ND = BM / (8 * NW) + RPW, SL = FMT == GQ_FMT_Q6_K ? 2 : 1, pend = (PD - 2) * ND + (PD - 1) * SL;
   gq_u4 sv[PD];
   const gq_u4 first = load_scales(0);
-  sv[1] = load_scales(1);
+  __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
   for (int i = 0; i < PD - 1; ++i) request(i, i);
+  __builtin_amdgcn_sched_barrier(0);
+  sv[1] = load_scales(1);
   __builtin_amdgcn_sched_barrier(0);  // (no wait for the scales before all of it is requested)
   store_scales(first, 0);
   step_barrier<(PD - 2) * ND>();
@@ -1310,6 +1316,7 @@ __global__ void __launch_bounds__(64 * WN * KG) k_front_dx(const uint8_t *__rest
     for (int i = 0; i < PD; ++i) {
       if (l + i >= nl) break;
       request(l + i + PD - 1, (i + PD - 1) % PD);
+      __builtin_amdgcn_sched_barrier(0);
       sv[(i + 2) % PD] = load_scales(l + i + 2);
       __builtin_amdgcn_sched_barrier(0);
       // (the last group's step may lie past the part: nothing to add, the barriers are everyone's)

@@ -1,0 +1,79 @@
+"""The order of loads in the built kernels of the gated front whose step barriers wait for a counted number of them.
+
+A step ends with a wait that leaves the youngest `pend` loads open, counted by hand for one order of issue: an LDS DMA that
+the compiler put behind loads it should precede would be left open, and other waves would read LDS before it has
+landed.  The GPU code of the built library is listed with llvm-objdump and its loads are read off between the barriers."""
+import os
+import re
+import shutil
+import subprocess
+
+import pytest
+
+import gq
+
+OBJDUMP = "/opt/rocm/llvm/bin/llvm-objdump"
+Q4_0, Q8_0, Q4_K, Q6_K = gq.FMT_Q4_0, gq.FMT_Q8_0, gq.FMT_Q4_K, gq.FMT_Q6_K
+
+pytestmark = pytest.mark.skipif(not os.path.exists(OBJDUMP), reason="no llvm-objdump")
+
+
+@pytest.fixture(scope="module")
+def kernels(tmp_path_factory):
+    """{mangled name: instruction lines} of the gated front's kernels."""
+    tmp = tmp_path_factory.mktemp("code")
+    lib = shutil.copy(gq.LIB_PATH, tmp)
+    subprocess.run([OBJDUMP, "--offloading", lib], check=True, capture_output=True, cwd=tmp)
+    out = {}
+    for f in sorted(tmp.iterdir()):
+        if not f.name.endswith("gfx950"):
+            continue
+        names = subprocess.run([OBJDUMP, "-t", f], check=True, capture_output=True, text=True).stdout
+        if "k_front_dx" not in names:
+            continue
+        text = subprocess.run([OBJDUMP, "-d", "--no-show-raw-insn", f], check=True, capture_output=True, text=True).stdout
+        lines = []
+        for line in text.splitlines():
+            m = re.match(r"[0-9a-f]+ <(.*)>:", line)
+            if m:
+                lines = out.setdefault(m[1], [])
+            else:
+                lines.append(line.strip())
+    return {n: t for n, t in out.items() if "k_front_" in n}
+
+
+def instances(kernels, name):
+    """(template arguments, lines) of every instantiation."""
+    found = []
+    for n, lines in kernels.items():
+        m = re.search(name + r"I((?:Li\d+E)+)E", n)
+        if m:
+            found.append((tuple(int(v) for v in re.findall(r"Li(\d+)E", m[1])), lines))
+    assert found
+    return found
+
+
+def loads(lines):
+    """The vector memory loads between the barriers, in order: D an LDS DMA, v a load into registers."""
+    parts = [""]
+    for line in lines:
+        if line.startswith("s_barrier"):
+            parts.append("")
+        elif re.match(r"(buffer|global|flat)_load", line):
+            parts[-1] += "D" if re.search(r"\blds\b", line) else "v"
+    return parts
+
+
+def test_backward_loads(kernels):
+    seen = set()
+    for (fmt, wn, kg, tm, pd), lines in instances(kernels, "k_front_dx"):
+        nd = 32 * tm // (8 * wn) + 4 * (2 if fmt in (Q8_0, Q6_K) else 1)
+        sl = 2 if fmt == Q6_K else 1
+        parts = loads(lines)
+        what = f"k_front_dx<{fmt},{wn},{kg},{tm},{pd}>: {parts[:pd + 1]}"
+        assert parts[0] == "v" * sl + "D" * (nd * (pd - 1)) + "v" * sl, what
+        for p in parts[1:pd + 1]:
+            assert p == "D" * nd + "v" * sl, what
+        assert not any("D" in p for p in parts[pd + 1:]), what
+        seen.add(fmt)
+    assert seen == {Q4_0, Q8_0, Q4_K, Q6_K}
