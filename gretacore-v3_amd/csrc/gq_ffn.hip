@@ -834,8 +834,10 @@ k_front_rb(const uint8_t *__restrict__ wg, const uint8_t *__restrict__ wu, uint3
     constexpr int i = decltype(b)::value;
     const int s = gstep(i);
     if constexpr (i < PD - 1) load_a_lds_b<BM, NW>(a16, ao, s, wave, As_of(b));
+    __builtin_amdgcn_sched_barrier(0);  // (pend counts this order)
     load_rstep<FMT, NJ>(wg, qo, so, s, st[0][i]);
     load_rstep<FMT, NJ>(wu, qo, so, s, st[1][i]);
+    __builtin_amdgcn_sched_barrier(0);
   };
   const gq_f4 rs4 = *reinterpret_cast<const gq_f4 *>(rs + m0 + 4 * (tid % (BM / 4)));  // (padded past M)
   prime(B0{});

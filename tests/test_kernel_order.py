@@ -77,3 +77,20 @@ def test_backward_loads(kernels):
         assert not any("D" in p for p in parts[pd + 1:]), what
         seen.add(fmt)
     assert seen == {Q4_0, Q8_0, Q4_K, Q6_K}
+
+
+def test_forward_loads(kernels):
+    per_column = {Q4_0: 3, Q8_0: 3, Q4_K: 3, Q6_K: 6}  # loads of a weight column block and step
+    seen = set()
+    for (fmt, bm, wn, nj, pd, kg), lines in instances(kernels, "k_front_rb"):
+        na, nw = bm // (8 * wn), 2 * per_column[fmt] * nj
+        parts = loads(lines)
+        what = f"k_front_rb<{fmt},{bm},{wn},{nj},{pd},{kg}>: {parts[:pd + 1]}"
+        # (one more load: the row scales, whose place is free, since the wait for them comes before the first barrier)
+        first = ("D" * na + "v" * nw) * (pd - 1) + "v" * nw
+        assert parts[0] in ("v" + first, first + "v"), what
+        for p in parts[1:pd + 1]:
+            assert p == "D" * na + "v" * nw, what
+        assert not any("D" in p for p in parts[pd + 1:]), what
+        seen.add(fmt)
+    assert seen == {Q4_0, Q8_0, Q4_K, Q6_K}
