@@ -717,12 +717,12 @@ k_front_rows_px(const uint8_t *__restrict__ wg, const uint8_t *__restrict__ wu, 
 // ahead in registers.  KG: groups of waves that share the tile and take every KG-th step,
 // their sums added through LDS at the end.
 template <int DT>
-GQ_DEV void front_put(const __amdgpu_buffer_rsrc_t &r, uint32_t vo, uint32_t so, int dt, float v) {
+GQ_DEV void front_put(const __amdgpu_buffer_rsrc_t &r, uint32_t o, int dt, float v) {
   if constexpr (DT == GQ_DT_F32)
-    __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(v), r, vo, so, 0);
+    __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(v), r, o, 0, 0);
   else
     __builtin_amdgcn_raw_buffer_store_b16(
-        dt == GQ_DT_BF16 ? gq_f32_to_bf16(v) : __builtin_bit_cast(uint16_t, (_Float16)v), r, vo, so, 0);
+        dt == GQ_DT_BF16 ? gq_f32_to_bf16(v) : __builtin_bit_cast(uint16_t, (_Float16)v), r, o, 0, 0);
 }
 
 // A step's end.  Waits for this wave's LDS DMAs but the VM youngest loads (which the caller counts) and for its
@@ -884,9 +884,9 @@ k_front_rb(const uint8_t *__restrict__ wg, const uint8_t *__restrict__ wu, uint3
         }
     if (kg > 0) return;
   }
-  // D layout (32x32): lane l holds column l % 32, rows 8 (v / 4) + 4 (l / 32) + v % 4.  A store's
-  // row is a scalar offset from the lane's; rows >= M lie past the resource's end (host: a
-  // tile's rows span less than 2 GiB).
+  // D layout (32x32): lane l holds column l % 32, rows 8 (v / 4) + 4 (l / 32) + v % 4.  Rows >= M lie
+  // past the resource's end, whose check need not count a scalar offset: all of it is in the lane's
+  // (host: a tile's rows span less than 2 GiB).
   auto store = [&](auto dtc) __attribute__((always_inline)) {
     constexpr int DT = decltype(dtc)::value;
     constexpr uint32_t ES = DT == GQ_DT_F32 ? 4u : 2u;
@@ -914,11 +914,11 @@ k_front_rb(const uint8_t *__restrict__ wg, const uint8_t *__restrict__ wu, uint3
         const uint32_t vo = ((uint32_t)mb * (uint32_t)N + (uint32_t)n) * ES;
 #pragma unroll
         for (int v = 0; v < 16; ++v) {
-          const uint32_t ro = (uint32_t)(8 * (v >> 2) + (v & 3)) * (uint32_t)N * ES;
+          const uint32_t o = vo + (uint32_t)(8 * (v >> 2) + (v & 3)) * (uint32_t)N * ES;
           const float g = acc[0][i][j][v] * rsv[v], u = acc[1][i][j][v] * rsv[v];
-          front_put<DT>(hr, vo, ro, dt, gq_act_f(act, g) * u);
-          if (go) front_put<DT>(gr, vo, ro, dt, g);
-          if (uo) front_put<DT>(ur, vo, ro, dt, u);
+          front_put<DT>(hr, o, dt, gq_act_f(act, g) * u);
+          if (go) front_put<DT>(gr, o, dt, g);
+          if (uo) front_put<DT>(ur, o, dt, u);
         }
       }
     }

@@ -1,4 +1,5 @@
-"""The order of loads in the built kernels of the gated front whose step barriers wait for a counted number of them.
+"""What the built kernels of the gated front rely on without a value to show for it: the order of loads where a step barrier
+waits for a counted number of them, and stores whose range check has to see their whole offset.
 
 A step ends with a wait that leaves the youngest `pend` loads open, counted by hand for one order of issue: an LDS DMA that
 the compiler put behind loads it should precede would be left open, and other waves would read LDS before it has
@@ -94,3 +95,17 @@ def test_forward_loads(kernels):
         assert not any("D" in p for p in parts[pd + 1:]), what
         seen.add(fmt)
     assert seen == {Q4_0, Q8_0, Q4_K, Q6_K}
+
+
+def test_store_offsets(kernels):
+    """Rows past the last are kept out of memory by a buffer's range, which is only sure to count the lane's offset: no
+    store of the front has a scalar one."""
+    n = 0
+    for (fmt, bm, wn, nj, pd, kg), lines in instances(kernels, "k_front_rb"):
+        for line in lines:
+            m = re.match(r"buffer_store_\w+ \w+, v\d+, s\[\d+:\d+\], (\S+) ", line)
+            assert m or not line.startswith("buffer_store"), line
+            if m:
+                n += 1
+                assert m[1] == "0", f"k_front_rb<{fmt},{bm},{wn},{nj},{pd},{kg}>: {line}"
+    assert n > 0
