@@ -1,5 +1,6 @@
 // gq_ffn.hip -- the gated feed-forward front h = act(x W_gate^T) * (x W_up^T) over T16
 // weights for any number of rows, and its backward pass.
+#include <algorithm>
 #include <type_traits>
 
 #include "gq_act.h"
@@ -1632,8 +1633,10 @@ struct DxPlan {
 };
 struct DxShape {
   int bm, bn, kg;
+  size_t rows;  // the largest block it is taken for
 };
-constexpr DxShape kDxShapes[3] = {{32, 128, 4}, {64, 128, 4}, {128, 256, 2}};
+// (Q4_K, K = 4096: 128 x 14336 by the second shape 73.4 us, the third 94.5; 128 x 5003 41.4 and 54.8)
+constexpr DxShape kDxShapes[3] = {{32, 128, 4, 32}, {64, 128, 4, 128}, {128, 256, 2, ~(size_t)0}};
 
 DxPlan dx_plan(size_t M, size_t N, size_t K) {
   DxPlan p;
@@ -1643,8 +1646,8 @@ DxPlan dx_plan(size_t M, size_t N, size_t K) {
   p.mb = fit < 256 ? fit : fit & ~(size_t)255;
   if (M < p.mb) p.mb = M;
   const size_t nsteps = 2 * p.np / 64;
-  // (Q4_K, K = 4096: 128 x 14336 by the second shape 73.4 us, the third 94.5; 128 x 5003 41.4 and 54.8)
-  p.shape = p.mb <= 32 ? 0 : p.mb <= 128 ? 1 : 2;
+  p.shape = 0;
+  while (p.mb > kDxShapes[p.shape].rows) ++p.shape;
   const DxShape &t = kDxShapes[p.shape];
   const size_t wgs = ((p.mb + t.bm - 1) / t.bm) * ((K + t.bn - 1) / t.bn);
   size_t want = wgs >= 192 ? 1 : 256 / wgs;
@@ -1664,6 +1667,27 @@ size_t dx_a_bytes(const DxPlan &p) { return gq_align256(p.mb * 2 * p.np * 2); }
 size_t dx_rs_bytes(const DxPlan &p) { return gq_align256((p.mb + 256) * 4); }
 size_t dx_bytes(const DxPlan &p, size_t K) {
   return dx_a_bytes(p) + dx_rs_bytes(p) + (p.parts > 1 ? gq_align256((size_t)p.parts * p.mb * K * 4) : 0);
+}
+
+// No less than dx_bytes of any call of at most M rows, and never less for more rows (a call of fewer rows
+// may have more parts, so its own bytes may be more than M's).  A plan with parts has at most 256 / workgroups of
+// them, so parts * (rows, up to whole tiles) * (columns, up to whole tiles) <= 256 tiles; it has them only
+// while its workgroups are at most 128.
+size_t dx_most_bytes(size_t M, size_t N, size_t K) {
+  const DxPlan p = dx_plan(M, N, K);
+  size_t most = dx_a_bytes(p) + dx_rs_bytes(p);  // (of the block of most rows)
+  const size_t nsteps = 2 * p.np / 64;
+  for (int i = 0; i <= p.shape; ++i) {
+    const DxShape &t = kDxShapes[i];
+    const size_t tk = (K + t.bn - 1) / t.bn, tiles = 128 / tk, parts = std::min(nsteps / (4 * t.kg), 256 / tk);
+    DxPlan q = p;  // the most rows of this shape that have parts
+    q.mb = std::min({p.mb, t.rows, tiles * t.bm});
+    if (q.mb <= (i ? kDxShapes[i - 1].rows : 0) || parts < 2) continue;
+    const size_t sums = std::min((size_t)256 * t.bm * t.bn, parts * q.mb * K);
+    // (dx_plan keeps plans with parts below kGqScratchMax)
+    most = std::max(most, std::min(dx_a_bytes(q) + dx_rs_bytes(q) + gq_align256(4 * sums), kGqScratchMax));
+  }
+  return most;
 }
 
 template <int FMT, int WN, int KG, int TM, int PD>
@@ -1703,14 +1727,8 @@ int launch_dgu(const void *dh, const void *g, const void *u, void *dg, void *du,
 }  // namespace
 
 extern "C" size_t gq_ffn_gate_up_bwd_workspace_bytes(int fmt, size_t M, size_t N, size_t K) {
-  if (!gq_fmt_valid(fmt) || M > GQ_MAX_DIM || N > GQ_MAX_DIM || K > GQ_MAX_DIM || N == 0 || K == 0) return 0;
-  // (never less for more rows: a block of fewer rows may have more parts)
-  size_t most = 0;
-  for (size_t m = M; m > 0; m /= 2) {
-    const size_t b = dx_bytes(dx_plan(m, N, K), K);
-    most = b > most ? b : most;
-  }
-  return most;
+  if (!gq_fmt_valid(fmt) || M > GQ_MAX_DIM || N > GQ_MAX_DIM || K > GQ_MAX_DIM || M == 0 || N == 0 || K == 0) return 0;
+  return dx_most_bytes(M, N, K);
 }
 
 extern "C" int gq_ffn_gate_up_bwd(int fmt, const void *gate, const void *up, const void *dh, const void *g,
@@ -1725,7 +1743,7 @@ extern "C" int gq_ffn_gate_up_bwd(int fmt, const void *gate, const void *up, con
   GQ_CHECK(dh && g && u, GQ_ERR_INVALID_ARGS);
   const DxPlan plan = dx_plan(M, N, K);
   const size_t need = dx ? gq_ffn_gate_up_bwd_workspace_bytes(fmt, M, N, K) : 0;
-  GqScratch sc(ws ? 0 : need, s);
+  GqScratch sc(ws || !dx ? 0 : dx_bytes(plan, K), s);
   if (ws) GQ_CHECK(ws_bytes >= need, GQ_ERR_WORKSPACE);
   else ws = sc.ptr;
   GQ_CHECK(ws || !dx, GQ_ERR_WORKSPACE);

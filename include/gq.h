@@ -271,7 +271,7 @@ int gq_launch_gemm_mfma_mixed_f16f32(void *stream, const float *a, const void *b
  * K <= 2048 do not) returns GQ_ERR_WORKSPACE, as does one of K above 2^21.
  * Calls that overlap must not share a workspace, and neither may two captured graphs
  * whose replays overlap.  Rows are taken in blocks, so the workspace stops growing
- * with M.  N * 128 outputs stay below 2^31 bytes; K == 0 is refused. */
+ * with M; the bytes for M rows are enough for every call of fewer.  N * 128 outputs stay below 2^31 bytes; K == 0 is refused. */
 size_t gq_ffn_gate_up_workspace_bytes(int fmt, size_t M, size_t N, size_t K);
 int gq_ffn_gate_up(int fmt, const void *d_gate, const void *d_up, const void *d_x, int x_dtype, void *d_h,
                    int h_dtype, void *d_g, void *d_u, size_t M, size_t N, size_t K, int act, void *d_workspace,

@@ -110,6 +110,15 @@ def test_workspaces_stop_growing(fmt):
         assert size(99, 16, 64, 256) == 0 and size(fmt, BIG, 64, 256) == 0
 
 
+@pytest.mark.parametrize("n,k", [(14336, 4096), (5003, 4096), (520, 130 * 32), (64, 256), (200, 14336), (100000, 64), (4096, 14336)])
+def test_a_workspace_of_more_rows_suffices_for_fewer(n, k):
+    """What is made for M rows is enough for every call of fewer: no size is below that of a smaller M, one by one up to
+    1200 rows and in odd steps beyond."""
+    for size in (gq.ffn_gate_up_workspace_bytes, gq.ffn_gate_up_bwd_workspace_bytes):
+        at = [size(gq.FMT_Q4_0, m, n, k) for m in [*range(0, 1201), *range(1201, 200000, 997)]]
+        assert all(a <= b for a, b in zip(at, at[1:]))
+
+
 @pytest.mark.parametrize("fmt", sorted(set(gq.FORMATS.values())))
 @pytest.mark.parametrize("m", [1, 17, 33, 300, 5000])
 def test_scratch_suffices_for_long_rows(fmt, m):
