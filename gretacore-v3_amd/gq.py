@@ -8,6 +8,7 @@ or a call fails, an exception is raised.
 from __future__ import annotations
 
 import ctypes
+import functools
 import os
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
@@ -586,14 +587,20 @@ def _rows(x, k, what):
     return (1 if n == 1 else shape[0]), device
 
 
-_sizes = {}  # sizes asked for so far
+# Sizes of the last calls (a prompt's length is part of a workspace's: the number of them is bounded)
+@functools.lru_cache(maxsize=512)
+def _packed_bytes(fmt, n, k):
+    return packed_size(fmt, n, k)
 
 
-def _size_of(key, fn, *args):
-    v = _sizes.get(key)
-    if v is None:
-        v = _sizes[key] = fn(*args)
-    return v
+@functools.lru_cache(maxsize=512)
+def _w4_packed_bytes(n, k, group):
+    return w4_packed_size(n, k, group)
+
+
+@functools.lru_cache(maxsize=512)
+def _front_bytes(backward, fmt, m, n, k):
+    return (ffn_gate_up_bwd_workspace_bytes if backward else ffn_gate_up_workspace_bytes)(fmt, m, n, k)
 
 
 def ffn_gate_up_workspace_bytes(fmt: int, m: int, n: int, k: int) -> int:
@@ -606,7 +613,7 @@ def ffn_gate_up(fmt: int, gate, up, x, n: int, k: int, act: int = ACT_SILU, save
     (default: x's) or the tensor given; with save (or g, u given) the two products come back too: (h, g, u)."""
     m, device = _rows(x, k, "x")
     dtype = h.dtype if h is not None else out_dtype or x.dtype
-    nbytes = _size_of((fmt, n, k), packed_size, fmt, n, k)
+    nbytes = _packed_bytes(fmt, n, k)
     _packed_operand(gate, nbytes, "gate", device)
     _packed_operand(up, nbytes, "up", device)
     if h is None:
@@ -623,7 +630,7 @@ def ffn_gate_up(fmt: int, gate, up, x, n: int, k: int, act: int = ACT_SILU, save
         u = _empty((m, n), dtype=dtype, device=x.device)
     ws_ptr, ws_n = None, 0
     if workspace is not None:
-        buf = workspace.ensure(_size_of((fmt, m, n, k, "front"), ffn_gate_up_workspace_bytes, fmt, m, n, k))
+        buf = workspace.ensure(_front_bytes(False, fmt, m, n, k))
         ws_ptr, ws_n = buf.data_ptr(), buf.numel()
     st = load().gq_ffn_gate_up(fmt, gate.data_ptr(), up.data_ptr(), x.data_ptr(), _dt(x.dtype), h.data_ptr(), _dt(dtype),
                                _ptr(g), _ptr(u), m, n, k, act, ws_ptr, ws_n, _stream(stream))
@@ -645,7 +652,7 @@ def ffn_gate_up_bwd(fmt: int, gate, up, dh, g, u, n: int, k: int, act: int = ACT
     dtype = dh.dtype
     _operand(g, dh.shape, "g", device, dtype)
     _operand(u, dh.shape, "u", device, dtype)
-    nbytes = _size_of((fmt, n, k), packed_size, fmt, n, k)
+    nbytes = _packed_bytes(fmt, n, k)
     _packed_operand(gate, nbytes, "gate", device)
     _packed_operand(up, nbytes, "up", device)
     if dx is not None:
@@ -662,7 +669,7 @@ def ffn_gate_up_bwd(fmt: int, gate, up, dh, g, u, n: int, k: int, act: int = ACT
         du = _empty((m, n), dtype=dtype, device=dh.device)
     ws_ptr, ws_n = None, 0
     if workspace is not None:
-        buf = workspace.ensure(_size_of((fmt, m, n, k, "bwd"), ffn_gate_up_bwd_workspace_bytes, fmt, m, n, k))
+        buf = workspace.ensure(_front_bytes(True, fmt, m, n, k))
         ws_ptr, ws_n = buf.data_ptr(), buf.numel()
     st = load().gq_ffn_gate_up_bwd(fmt, gate.data_ptr(), up.data_ptr(), dh.data_ptr(), g.data_ptr(), u.data_ptr(), _dt(dtype),
                                    _ptr(dg), _ptr(du), _ptr(dx), _dt(dx.dtype if dx is not None else dtype), m, n, k, act,
@@ -700,7 +707,7 @@ def w4_gemv(w, group: int, x, n: int, k: int, y=None, out_dtype=None, stream=Non
     """y[b][n] = sum_k x[b][k] * W[n][k] over w4_pack's weights; x f32/f16/bf16 [k] or [1..16][k], y of out_dtype
     (default: x's) or the tensor given."""
     m, device = _rows(x, k, "x")
-    _packed_operand(w, _size_of((n, k, group, "w4"), w4_packed_size, n, k, group), "w", device)
+    _packed_operand(w, _w4_packed_bytes(n, k, group), "w", device)
     if y is None:
         y = _empty((m, n), dtype=out_dtype or x.dtype, device=x.device)
     else:
@@ -715,7 +722,7 @@ def w4_gemv(w, group: int, x, n: int, k: int, y=None, out_dtype=None, stream=Non
 def w4_gate_up(gate, up, group: int, x, n: int, k: int, act: int = ACT_SILU, h=None, out_dtype=None, stream=None):
     """h = act(x Wg^T) * (x Wu^T) over two matrices of w4_pack, 1..16 rows of x, in one launch."""
     m, device = _rows(x, k, "x")
-    nbytes = _size_of((n, k, group, "w4"), w4_packed_size, n, k, group)
+    nbytes = _w4_packed_bytes(n, k, group)
     _packed_operand(gate, nbytes, "gate", device)
     _packed_operand(up, nbytes, "up", device)
     if h is None:

@@ -432,3 +432,19 @@ def test_block_trains_and_decodes(dev):
         c1.w, c1.x = c.w, c.x[i:i + 1]
         for t in (one, dec, h[i:i + 1]):
             check_front(c1, 0, (t, None, None), t.dtype)
+
+
+def test_sizes_kept_are_bounded(dev):
+    """Calls of ever new lengths leave no record of each behind."""
+    import gq
+
+    def held():
+        return sum(len(v) for v in vars(gq).values() if isinstance(v, (dict, list, set))) + sum(
+            v.cache_info().currsize for v in vars(gq).values() if hasattr(v, "cache_info"))
+
+    fmt, n, k = O.Q4_0, 16, 64
+    c = Case(dev, fmt, 2500, n, k)
+    ws, before = gq.Workspace(dev), held()
+    for m in range(1, 2501):
+        gq.ffn_gate_up(fmt, *c.packed, c.x[:m], n, k, workspace=ws)
+    assert held() - before <= 1024
