@@ -530,7 +530,8 @@ def gemv_swiglu_plan(fmt: int, n: int, k: int, batch: int):
 
 
 # ---- gated feed-forward front, 4-bit weights with group scales --------------------
-# These calls take whole contiguous tensors on the current device and refuse others.  The checks are few
+# These calls take whole contiguous tensors on the current device and refuse others, and run on the current stream or the
+# one given (inputs of other streams are the caller's to order, as for torch's own).  The checks are few
 # attribute reads (a 4-bit GEMV's kernel runs 4 us); the messages are made only when one fails.
 _dts = {}  # torch dtype -> DT_*
 _empty = _current_device = None
@@ -541,6 +542,21 @@ def _init_torch():
     import torch
     _dts.update({torch.float32: DT_F32, torch.float16: DT_F16, torch.bfloat16: DT_BF16})
     _empty, _current_device = torch.empty, torch.cuda.current_device
+
+
+def _on(stream, call, *args):
+    """The call with `stream` as the current stream.  Outputs made there are that stream's memory: made on the current one
+    they could be what work still queued on it uses.  Freed, they wait for the current stream too, which reads them."""
+    import torch
+    current = torch.cuda.current_stream()
+    if stream.device != current.device:
+        raise GQError(f"stream of {stream.device}, but the current device is {current.device}")
+    with torch.cuda.stream(stream):
+        out = call(*args)
+    for t in out.values() if isinstance(out, dict) else out if isinstance(out, tuple) else (out,):
+        if t is not None:
+            t.record_stream(current)
+    return out
 
 
 def _dt(dtype):
@@ -611,6 +627,8 @@ def ffn_gate_up(fmt: int, gate, up, x, n: int, k: int, act: int = ACT_SILU, save
                 out_dtype=None, workspace: Workspace | None = None, stream=None):
     """h = act(x Wg^T) * (x Wu^T) over T16 weights, any number of rows of x [m][k] (f32/f16/bf16).  h is of out_dtype
     (default: x's) or the tensor given; with save (or g, u given) the two products come back too: (h, g, u)."""
+    if stream is not None:
+        return _on(stream, ffn_gate_up, fmt, gate, up, x, n, k, act, save, h, g, u, out_dtype, workspace)
     m, device = _rows(x, k, "x")
     dtype = h.dtype if h is not None else out_dtype or x.dtype
     nbytes = _packed_bytes(fmt, n, k)
@@ -633,7 +651,7 @@ def ffn_gate_up(fmt: int, gate, up, x, n: int, k: int, act: int = ACT_SILU, save
         buf = workspace.ensure(_front_bytes(False, fmt, m, n, k))
         ws_ptr, ws_n = buf.data_ptr(), buf.numel()
     st = load().gq_ffn_gate_up(fmt, gate.data_ptr(), up.data_ptr(), x.data_ptr(), _dt(x.dtype), h.data_ptr(), _dt(dtype),
-                               _ptr(g), _ptr(u), m, n, k, act, ws_ptr, ws_n, _stream(stream))
+                               _ptr(g), _ptr(u), m, n, k, act, ws_ptr, ws_n, _stream())
     if st:
         check(st, "gq_ffn_gate_up")
     return h if g is None and u is None else (h, g, u)
@@ -648,6 +666,8 @@ def ffn_gate_up_bwd(fmt: int, gate, up, dh, g, u, n: int, k: int, act: int = ACT
                     stream=None):
     """Gradients of ffn_gate_up with the weights frozen: {"dx", "dg", "du"} for dh [m][n] and the g, u it saved.  dg and
     du are the gradients of the two projections, None where not wanted."""
+    if stream is not None:
+        return _on(stream, ffn_gate_up_bwd, fmt, gate, up, dh, g, u, n, k, act, want_dx, want_dgu, dx, dg, du, dx_dtype, workspace)
     m, device = _rows(dh, n, "dh")
     dtype = dh.dtype
     _operand(g, dh.shape, "g", device, dtype)
@@ -673,7 +693,7 @@ def ffn_gate_up_bwd(fmt: int, gate, up, dh, g, u, n: int, k: int, act: int = ACT
         ws_ptr, ws_n = buf.data_ptr(), buf.numel()
     st = load().gq_ffn_gate_up_bwd(fmt, gate.data_ptr(), up.data_ptr(), dh.data_ptr(), g.data_ptr(), u.data_ptr(), _dt(dtype),
                                    _ptr(dg), _ptr(du), _ptr(dx), _dt(dx.dtype if dx is not None else dtype), m, n, k, act,
-                                   ws_ptr, ws_n, _stream(stream))
+                                   ws_ptr, ws_n, _stream())
     if st:
         check(st, "gq_ffn_gate_up_bwd")
     return {"dx": dx, "dg": dg, "du": du}
@@ -688,6 +708,8 @@ def w4_packed_size(n: int, k: int, group: int) -> int:
 def w4_pack(q, scales, zeros, n: int, k: int, group: int, stream=None):
     """4-bit rows q uint8 [n][ceil(k/2)] (even k in the low nibble), scales f16/bf16 and zeros uint8 (None: 8)
     [n][ceil(k/group)] -> the packed weights of w4_gemv / w4_gate_up."""
+    if stream is not None:
+        return _on(stream, w4_pack, q, scales, zeros, n, k, group)
     import torch
     nbytes = w4_packed_size(n, k, group)
     ng = -(-k // group)
@@ -699,13 +721,15 @@ def w4_pack(q, scales, zeros, n: int, k: int, group: int, stream=None):
         _operand(zeros, (n, ng), "zeros", device, torch.uint8)
     out = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
     check(load().gq_w4_pack(_ptr(q), _ptr(scales), _dt(scales.dtype), _ptr(zeros), n, k, group, _ptr(out),
-                            _stream(stream)), "gq_w4_pack")
+                            _stream()), "gq_w4_pack")
     return out
 
 
 def w4_gemv(w, group: int, x, n: int, k: int, y=None, out_dtype=None, stream=None):
     """y[b][n] = sum_k x[b][k] * W[n][k] over w4_pack's weights; x f32/f16/bf16 [k] or [1..16][k], y of out_dtype
     (default: x's) or the tensor given."""
+    if stream is not None:
+        return _on(stream, w4_gemv, w, group, x, n, k, y, out_dtype)
     m, device = _rows(x, k, "x")
     _packed_operand(w, _w4_packed_bytes(n, k, group), "w", device)
     if y is None:
@@ -713,7 +737,7 @@ def w4_gemv(w, group: int, x, n: int, k: int, y=None, out_dtype=None, stream=Non
     else:
         _operand(y, (m, n), "y", device)
     st = load().gq_w4_gemv(w.data_ptr(), group, x.data_ptr(), _dt(x.dtype), y.data_ptr(), _dt(y.dtype), n, k, m,
-                           _stream(stream))
+                           _stream())
     if st:
         check(st, "gq_w4_gemv")
     return y
@@ -721,6 +745,8 @@ def w4_gemv(w, group: int, x, n: int, k: int, y=None, out_dtype=None, stream=Non
 
 def w4_gate_up(gate, up, group: int, x, n: int, k: int, act: int = ACT_SILU, h=None, out_dtype=None, stream=None):
     """h = act(x Wg^T) * (x Wu^T) over two matrices of w4_pack, 1..16 rows of x, in one launch."""
+    if stream is not None:
+        return _on(stream, w4_gate_up, gate, up, group, x, n, k, act, h, out_dtype)
     m, device = _rows(x, k, "x")
     nbytes = _w4_packed_bytes(n, k, group)
     _packed_operand(gate, nbytes, "gate", device)
@@ -730,7 +756,7 @@ def w4_gate_up(gate, up, group: int, x, n: int, k: int, act: int = ACT_SILU, h=N
     else:
         _operand(h, (m, n), "h", device)
     st = load().gq_w4_gate_up(gate.data_ptr(), up.data_ptr(), group, x.data_ptr(), _dt(x.dtype), h.data_ptr(), _dt(h.dtype), n,
-                              k, m, act, _stream(stream))
+                              k, m, act, _stream())
     if st:
         check(st, "gq_w4_gate_up")
     return h

@@ -448,3 +448,44 @@ def test_sizes_kept_are_bounded(dev):
     for m in range(1, 2501):
         gq.ffn_gate_up(fmt, *c.packed, c.x[:m], n, k, workspace=ws)
     assert held() - before <= 1024
+
+
+def test_a_given_stream_owns_the_outputs(dev):
+    """Outputs made for a call on another stream do not lie in memory that queued work of the current one still writes."""
+    import gq
+    fmt, m, n, k = O.Q8_0, 64, 2048, 512
+    c = Case(dev, fmt, m, n, k, seed=31)
+    ref = gq.ffn_gate_up(fmt, *c.packed, c.x, n, k, save=True)
+    gref = gq.ffn_gate_up_bwd(fmt, *c.packed, c.dh, c.g, c.u, n, k)
+    q, s = torch.full((n, k // 2), 0x5A, dtype=torch.uint8, device=dev), torch.ones(n, k // 128, dtype=torch.float16, device=dev)
+    wref = gq.w4_pack(q, s, None, n, k, 128)
+    yref, href = gq.w4_gemv(wref, 128, c.x[:16], n, k), gq.w4_gate_up(wref, wref, 128, c.x[:16], n, k)
+    side, a = torch.cuda.Stream(), torch.randn(8192, 8192, device=dev).to(torch.bfloat16)
+    calls = [(lambda: gq.ffn_gate_up(fmt, *c.packed, c.x, n, k, save=True, stream=side), ref),
+             (lambda: tuple(gq.ffn_gate_up_bwd(fmt, *c.packed, c.dh, c.g, c.u, n, k, stream=side).values()), tuple(gref.values())),
+             (lambda: (gq.w4_pack(q, s, None, n, k, 128, stream=side),), (wref,)),
+             (lambda: (gq.w4_gemv(wref, 128, c.x[:16], n, k, stream=side),), (yref,)),
+             (lambda: (gq.w4_gate_up(wref, wref, 128, c.x[:16], n, k, stream=side),), (href,))]
+    for call, want in calls:
+        b = torch.mm(a, a)
+        torch.cuda.synchronize()
+        old = [torch.empty_like(t) for t in want for _ in range(2)]
+        for _ in range(20):
+            torch.mm(a, a, out=b)  # (some milliseconds of work in front of the writes)
+        for t in old:
+            t.fill_(77)
+        del old, t
+        got = call()
+        side.synchronize()
+        torch.cuda.synchronize()
+        for x, y in zip(got, want):
+            assert torch.equal(x, y)
+
+
+def test_a_stream_of_another_device_is_refused(dev):
+    import types
+
+    import gq
+    c = Case(dev, O.Q8_0, 4, 64, 256)
+    with pytest.raises(gq.GQError, match="cuda:7"):
+        gq.ffn_gate_up(O.Q8_0, *c.packed, c.x, 64, 256, stream=types.SimpleNamespace(device=torch.device("cuda:7"), cuda_stream=0))
