@@ -619,6 +619,13 @@ def _front_bytes(backward, fmt, m, n, k):
     return (ffn_gate_up_bwd_workspace_bytes if backward else ffn_gate_up_workspace_bytes)(fmt, m, n, k)
 
 
+def _room(workspace, nbytes, device):
+    buf = workspace.ensure(nbytes)
+    if buf.get_device() != device:
+        raise GQError(f"workspace: on {buf.device}, but the current device is {device}")
+    return buf.data_ptr(), buf.numel()
+
+
 def ffn_gate_up_workspace_bytes(fmt: int, m: int, n: int, k: int) -> int:
     return load().gq_ffn_gate_up_workspace_bytes(fmt, m, n, k)
 
@@ -648,8 +655,7 @@ def ffn_gate_up(fmt: int, gate, up, x, n: int, k: int, act: int = ACT_SILU, save
         u = _empty((m, n), dtype=dtype, device=x.device)
     ws_ptr, ws_n = None, 0
     if workspace is not None:
-        buf = workspace.ensure(_front_bytes(False, fmt, m, n, k))
-        ws_ptr, ws_n = buf.data_ptr(), buf.numel()
+        ws_ptr, ws_n = _room(workspace, _front_bytes(False, fmt, m, n, k), device)
     st = load().gq_ffn_gate_up(fmt, gate.data_ptr(), up.data_ptr(), x.data_ptr(), _dt(x.dtype), h.data_ptr(), _dt(dtype),
                                _ptr(g), _ptr(u), m, n, k, act, ws_ptr, ws_n, _stream())
     if st:
@@ -689,8 +695,7 @@ def ffn_gate_up_bwd(fmt: int, gate, up, dh, g, u, n: int, k: int, act: int = ACT
         du = _empty((m, n), dtype=dtype, device=dh.device)
     ws_ptr, ws_n = None, 0
     if workspace is not None:
-        buf = workspace.ensure(_front_bytes(True, fmt, m, n, k))
-        ws_ptr, ws_n = buf.data_ptr(), buf.numel()
+        ws_ptr, ws_n = _room(workspace, _front_bytes(True, fmt, m, n, k), device)
     st = load().gq_ffn_gate_up_bwd(fmt, gate.data_ptr(), up.data_ptr(), dh.data_ptr(), g.data_ptr(), u.data_ptr(), _dt(dtype),
                                    _ptr(dg), _ptr(du), _ptr(dx), _dt(dx.dtype if dx is not None else dtype), m, n, k, act,
                                    ws_ptr, ws_n, _stream())

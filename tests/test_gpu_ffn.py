@@ -489,3 +489,15 @@ def test_a_stream_of_another_device_is_refused(dev):
     c = Case(dev, O.Q8_0, 4, 64, 256)
     with pytest.raises(gq.GQError, match="cuda:7"):
         gq.ffn_gate_up(O.Q8_0, *c.packed, c.x, 64, 256, stream=types.SimpleNamespace(device=torch.device("cuda:7"), cuda_stream=0))
+
+
+def test_a_workspace_elsewhere_is_refused(dev):
+    """No kernel gets the address of host memory, or of another device's."""
+    import gq
+    fmt, n, k = O.Q8_0, 64, 256
+    for m in (4, 40):
+        c = Case(dev, fmt, m, n, k)
+        with pytest.raises(gq.GQError, match="workspace"):
+            gq.ffn_gate_up(fmt, *c.packed, c.x, n, k, workspace=gq.Workspace("cpu"))
+        with pytest.raises(gq.GQError, match="workspace"):
+            gq.ffn_gate_up_bwd(fmt, *c.packed, c.dh, c.g, c.u, n, k, workspace=gq.Workspace("cpu"))
