@@ -276,17 +276,28 @@ def dequant_packed(fmt: int, d_packed, n: int, k: int, stream=None):
 
 
 class Workspace:
-    """Caller-owned device workspace reused across calls."""
+    """Caller-owned device workspace reused across calls.  It grows with the calls: a buffer that a captured call used is
+    kept when it is outgrown (the graph's replays use it), any other is free again once the work queued on the current
+    stream is done."""
 
     def __init__(self, device, nbytes: int = 0):
         self.device = device
         self.buf = None
+        self.captured = False  # buf is in a graph
+        self.outgrown = []     # buffers that graphs use
         self.ensure(nbytes)
 
     def ensure(self, nbytes: int):
         import torch
         if self.buf is None or self.buf.numel() < nbytes:
+            if self.captured:
+                self.outgrown.append(self.buf)
+            elif self.buf is not None and self.buf.is_cuda:
+                self.buf.record_stream(torch.cuda.current_stream(self.buf.device))
+            self.captured = False
             self.buf = torch.empty(max(nbytes, 1 << 20), dtype=torch.uint8, device=self.device)
+        if not self.captured and self.buf.is_cuda and torch.cuda.is_current_stream_capturing():
+            self.captured = True
         return self.buf
 
 

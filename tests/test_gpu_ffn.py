@@ -501,3 +501,37 @@ def test_a_workspace_elsewhere_is_refused(dev):
             gq.ffn_gate_up(fmt, *c.packed, c.x, n, k, workspace=gq.Workspace("cpu"))
         with pytest.raises(gq.GQError, match="workspace"):
             gq.ffn_gate_up_bwd(fmt, *c.packed, c.dh, c.g, c.u, n, k, workspace=gq.Workspace("cpu"))
+
+
+def test_a_workspace_outgrown_after_a_capture(dev):
+    """A captured call's workspace is not given to others when a later call needs a larger one."""
+    import gq
+    fmt, m, n, k = O.Q4_K, 64, 512, 4096
+    c, big = Case(dev, fmt, m, n, k, seed=1), Case(dev, fmt, 900, n, k, seed=2)
+    need = max(gq.ffn_gate_up_workspace_bytes(fmt, m, n, k), gq.ffn_gate_up_bwd_workspace_bytes(fmt, m, n, k))
+    ws = gq.Workspace(dev, need)
+    h, dx = torch.empty(m, n, dtype=torch.bfloat16, device=dev), torch.empty(m, k, dtype=torch.bfloat16, device=dev)
+
+    def step():
+        gq.ffn_gate_up(fmt, *c.packed, c.x, n, k, h=h, workspace=ws)
+        gq.ffn_gate_up_bwd(fmt, *c.packed, c.dh, c.g, c.u, n, k, dx=dx, want_dgu=False, workspace=ws)
+
+    step()
+    torch.cuda.synchronize()
+    ref = h.clone(), dx.clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+    size = ws.buf.numel()
+    gq.ffn_gate_up(fmt, *big.packed, big.x, n, k, workspace=ws)
+    gq.ffn_gate_up_bwd(fmt, *big.packed, big.dh, big.g, big.u, n, k, workspace=ws)
+    assert ws.buf.numel() > size
+    torch.cuda.synchronize()
+    others = [torch.full((size,), 7, dtype=torch.uint8, device=dev) for _ in range(3)]
+    for _ in range(3):
+        h.fill_(float("nan"))
+        dx.fill_(float("nan"))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(h, ref[0]) and torch.equal(dx, ref[1])
+        assert all(bool((t == 7).all()) for t in others)
