@@ -288,17 +288,23 @@ class Workspace:
         self.ensure(nbytes)
 
     def ensure(self, nbytes: int):
-        import torch
         if self.buf is None or self.buf.numel() < nbytes:
-            if self.captured:
-                self.outgrown.append(self.buf)
-            elif self.buf is not None and self.buf.is_cuda:
-                self.buf.record_stream(torch.cuda.current_stream(self.buf.device))
-            self.captured = False
-            self.buf = torch.empty(max(nbytes, 1 << 20), dtype=torch.uint8, device=self.device)
-        if not self.captured and self.buf.is_cuda and torch.cuda.is_current_stream_capturing():
+            self._grow(nbytes)
+        if self._capturing is not None and not self.captured and self._capturing():
             self.captured = True
         return self.buf
+
+    def _grow(self, nbytes):
+        import torch
+        if self.captured:
+            self.outgrown.append(self.buf)
+        elif self.buf is not None and self.buf.is_cuda:
+            self.buf.record_stream(torch.cuda.current_stream(self.buf.device))
+        self.captured = False
+        self.buf = torch.empty(max(nbytes, 1 << 20), dtype=torch.uint8, device=self.device)
+        self._capturing = None  # (asked at every call: without torch's Python layer where it has the plain function)
+        if self.buf.is_cuda:
+            self._capturing = getattr(torch._C, "_cuda_isCurrentStreamCapturing", torch.cuda.is_current_stream_capturing)
 
 
 def gemv_plan(fmt: int, n: int, k: int, batch: int):
