@@ -290,7 +290,8 @@ class Workspace:
     def ensure(self, nbytes: int):
         if self.buf is None or self.buf.numel() < nbytes:
             self._grow(nbytes)
-        if self._capturing is not None and not self.captured and self._capturing():
+        # (the default stream, whose handle is 0, is never captured: seen in 0.04 us, the question itself takes 0.3)
+        if self._index is not None and not self.captured and _raw_stream(self._index) and self._capturing():
             self.captured = True
         return self.buf
 
@@ -302,9 +303,10 @@ class Workspace:
             self.buf.record_stream(torch.cuda.current_stream(self.buf.device))
         self.captured = False
         self.buf = torch.empty(max(nbytes, 1 << 20), dtype=torch.uint8, device=self.device)
-        self._capturing = None  # (asked at every call: without torch's Python layer where it has the plain function)
+        self._index, self._capturing = None, torch.cuda.is_current_stream_capturing
         if self.buf.is_cuda:
-            self._capturing = getattr(torch._C, "_cuda_isCurrentStreamCapturing", torch.cuda.is_current_stream_capturing)
+            _stream()  # (initialises _raw_stream)
+            self._index = self.buf.get_device()
 
 
 def gemv_plan(fmt: int, n: int, k: int, batch: int):
