@@ -619,31 +619,17 @@ k_front_rows_px(const uint8_t *__restrict__ wg, const uint8_t *__restrict__ wu, 
   auto xin = [&](int t, int i, int f) {
     return 16 * t + r < M && 128 * (wave + kPxWaves * i) + 64 * (f >> 1) + 16 * g + 8 * (f & 1) < K;
   };
-  auto load_run = [&](int t, int i, int f, FRaw<XT> &o) __attribute__((always_inline)) {
-    const int k = 128 * (wave + kPxWaves * i) + 64 * (f >> 1) + 16 * g + 8 * (f & 1);
-    px_load<XT>(x, xin(t, i, f) ? (size_t)(16 * t + r) * K + k : 0, o);
-  };
-  // (as loaded where the registers hold that, else read again for the conversion)
-  constexpr bool ONCE = MT * NU * (XT == GQ_DT_F32 ? 2 : 1) <= 8;
-  FRaw<XT> raw[ONCE ? MT : 1][ONCE ? NU : 1][4];
+  FRaw<XT> raw[MT][NU][4];  // x as loaded
   auto load_x = [&]() __attribute__((always_inline)) {
-    if constexpr (ONCE) {
 #pragma unroll
-      for (int t = 0; t < MT; ++t)
+    for (int t = 0; t < MT; ++t)
 #pragma unroll
-        for (int i = 0; i < NU; ++i)
+      for (int i = 0; i < NU; ++i)
 #pragma unroll
-          for (int f = 0; f < 4; ++f) load_run(t, i, f, raw[t][i][f]);
-    }
-  };
-  auto run = [&](int t, int i, int f, float (&v)[8]) __attribute__((always_inline)) {
-    if constexpr (ONCE) {
-      px_floats<XT>(raw[t][i][f], xin(t, i, f), v);
-    } else {
-      FRaw<XT> o;
-      load_run(t, i, f, o);
-      px_floats<XT>(o, xin(t, i, f), v);
-    }
+        for (int f = 0; f < 4; ++f) {
+          const int k = 128 * (wave + kPxWaves * i) + 64 * (f >> 1) + 16 * g + 8 * (f & 1);
+          px_load<XT>(x, xin(t, i, f) ? (size_t)(16 * t + r) * K + k : 0, raw[t][i][f]);
+        }
   };
   auto begin = [&]() __attribute__((always_inline)) {
 #pragma unroll
@@ -654,7 +640,7 @@ k_front_rows_px(const uint8_t *__restrict__ wg, const uint8_t *__restrict__ wu, 
 #pragma unroll
         for (int f = 0; f < 4; ++f) {
           float v[8];
-          run(t, i, f, v);
+          px_floats<XT>(raw[t][i][f], xin(t, i, f), v);
 #pragma unroll
           for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(v[e]));
         }
@@ -670,7 +656,7 @@ k_front_rows_px(const uint8_t *__restrict__ wg, const uint8_t *__restrict__ wu, 
 #pragma unroll
         for (int f = 0; f < 4; ++f) {
           float v[8];
-          run(t, i, f, v);
+          px_floats<XT>(raw[t][i][f], xin(t, i, f), v);
           constexpr int perm[8] = {0, 2, 4, 6, 1, 3, 5, 7};  // the nibbles' order, their 16 x divided out
 #pragma unroll
           for (int e = 0; e < 8; ++e)

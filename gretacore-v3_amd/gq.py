@@ -692,7 +692,8 @@ def ffn_gate_up_bwd(fmt: int, gate, up, dh, g, u, n: int, k: int, act: int = ACT
     """Gradients of ffn_gate_up with the weights frozen: {"dx", "dg", "du"} for dh [m][n] and the g, u it saved.  dg and
     du are the gradients of the two projections, None where not wanted."""
     if stream is not None:
-        return _on(stream, ffn_gate_up_bwd, fmt, gate, up, dh, g, u, n, k, act, want_dx, want_dgu, dx, dg, du, dx_dtype, workspace)
+        return _on(stream, ffn_gate_up_bwd, fmt, gate, up, dh, g, u, n, k, act, want_dx, want_dgu, dx, dg, du, dx_dtype,
+                   workspace)
     m, device = _rows(dh, n, "dh")
     dtype = dh.dtype
     _operand(g, dh.shape, "g", device, dtype)
