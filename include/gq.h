@@ -262,7 +262,9 @@ int gq_launch_gemm_mfma_mixed_f16f32(void *stream, const float *a, const void *b
  * of h_dtype, as gq_ffn_gate_up_bwd takes them.  fp16 matrix cores, fp32 sums, as
  * gq_gemm: x is rounded to fp16 after a power-of-two scale per row, each weight once
  * to fp16, which for fp32 outputs leaves about 3e-4 of a row's norm.  Every output is
- * rounded once from fp32.  h, g and u overlap nothing else. */
+ * rounded once from fp32.  One to four rows of bf16 enter the matrix cores as they
+ * are, so their finite values must stay below 2^115; more rows, and fp32, may have any.
+ * h, g and u overlap nothing else. */
 #define GQ_ACT_SILU 0      /* g / (1 + e^-g) */
 #define GQ_ACT_GELU_TANH 1 /* g / 2 (1 + tanh(sqrt(2 / pi) (g + 0.044715 g^3))) */
 /* A workspace of NULL takes scratch memory of the call's own, which needs no room
@@ -302,7 +304,8 @@ int gq_w4_pack(const uint8_t *d_q, const void *d_scales, int scale_dtype, const 
  * any activation dtype.  The codes and x enter the matrix cores as they are (fp32 x
  * as three bf16 parts), sums and scales are fp32: the error is that of fp32
  * sums, then one rounding to y_dtype.  A row of x with an Inf or NaN comes out
- * non-finite; finite values must stay below 2^120.  No workspace. */
+ * non-finite; finite values must stay below 2^115 (a
+ * group's sum of 128 values times codes of up to 47, the offset included, is fp32).  No workspace. */
 int gq_w4_gemv(const void *d_packed, int group, const void *d_x, int x_dtype, void *d_y, int y_dtype, size_t N, size_t K,
                int batch, void *stream);
 /* h[b][n] = act(g) * u, g = x W_gate^T, u = x W_up^T: the gated form, in one launch. */
