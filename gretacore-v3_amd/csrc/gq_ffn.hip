@@ -701,7 +701,9 @@ k_front_rows_px(const uint8_t *__restrict__ wg, const uint8_t *__restrict__ wu, 
 // both, and the epilogue has g and u of an output in the same lane: h (and g, u where they
 // are kept) goes out once, nothing comes back.  Operand order, swizzle and pipeline are those
 // of gq_gemm_frag.h: fp16 activations by LDS DMA PD - 1 steps of 64 k ahead, weights PD steps
-// ahead in registers.  KG: groups of waves that share the tile and take every KG-th step,
+// ahead in registers.  So are the weights' roundings to fp16: Q4_0 and Q8_0 once (1.7e-4 and 2.1e-4 of a product's row), Q6_K
+// d sc first (2.9e-4), Q4_K dmin m first (5.4e-4 where minima are 7.5 scales, as in weights about zero; as d sc (q - 8) + c, c
+// rounded, 2.3e-4 there, but 2.8e-4 against 2.1e-4 where they are not).  KG: groups of waves that share the tile and take every KG-th step,
 // their sums added through LDS at the end.
 template <int DT>
 GQ_DEV void front_put(const __amdgpu_buffer_rsrc_t &r, uint32_t o, int dt, float v) {
@@ -714,7 +716,9 @@ GQ_DEV void front_put(const __amdgpu_buffer_rsrc_t &r, uint32_t o, int dt, float
 
 // A step's end.  Waits for this wave's LDS DMAs but the VM youngest loads (which the caller counts) and for its
 // LDS operations, then for the other waves.  __syncthreads would wait for every DMA, those of later
-// steps too: its fence counts them as writes to LDS.
+// steps too: its fence counts them as writes to LDS.  (k_front_dx in Q4_K and Q6_K still waits for
+// them in some of its steps: the compiler does so between two stores of the scale tables, which lie in the
+// DMAs' arrays and are too many for it to tell apart.)
 template <int VM>
 GQ_DEV void step_barrier() {
   static_assert(VM <= 63, "vmcnt immediate");

@@ -258,19 +258,27 @@ int gq_launch_gemm_mfma_mixed_f16f32(void *stream, const float *a, const void *b
  * h[m][n] = act(g[m][n]) * u[m][n] with g = x W_gate^T, u = x W_up^T: gq_gemv_swiglu's
  * block without its normalisation, for prompts, batches and training.  x is
  * [M][K] of x_dtype, h [M][N] of h_dtype, both contiguous; W_gate and W_up are T16
- * tensors of one format (they and the workspace 16-byte aligned).  d_g and d_u (NULL: not wanted) receive the two products,
- * of h_dtype, as gq_ffn_gate_up_bwd takes them.  fp16 matrix cores, fp32 sums, as
- * gq_gemm: x is rounded to fp16 after a power-of-two scale per row, each weight once
- * to fp16, which for fp32 outputs leaves about 3e-4 of a row's norm.  Every output is
- * rounded once from fp32.  One to four rows of bf16 enter the matrix cores as they
- * are, so their finite values must stay below 2^115; more rows, and fp32, may have any.
- * h, g and u overlap nothing else. */
+ * tensors of one format (they and the workspace 16-byte aligned).  d_g and d_u (NULL:
+ * not wanted) receive the two products, of h_dtype, as gq_ffn_gate_up_bwd takes them.
+ * h, g and u overlap nothing else.
+ * Sums are fp32 and every output is rounded once from them.  One to four rows of
+ * 16-bit x enter the matrix cores as they are, the scales apply to fp32 sums: 2e-5 of a
+ * product's row (bf16: 2e-6); of such bf16 rows the
+ * finite values must stay below 2^115, more rows, and fp32, may have any.  All other
+ * calls round x to fp16 after a power-of-two scale per row (nothing lost of 16-bit
+ * values near the row's largest, 2e-4 of fp32's) and the weights as follows.  Q4_0, Q8_0:
+ * once, 2e-4.  k-quants in the kernels of few rows (to 16; to 32 for K <= 2048 or N <=
+ * 6400): d (and dmin) stay apart in fp32, Q4_K nothing, Q6_K 1e-4.  k-quants above, as in
+ * gq_gemm: Q4_K's dmin m and then the weight, 5e-4; Q6_K's d sc and then the weight, 3e-4.
+ * (One to four fp32 rows with SiLU and no products kept: gq_gemv_swiglu without gamma has
+ * 2e-5 and is quicker, 13.2 us against 19.2 for Q4_K 14336 x 4096.) */
 #define GQ_ACT_SILU 0      /* g / (1 + e^-g) */
 #define GQ_ACT_GELU_TANH 1 /* g / 2 (1 + tanh(sqrt(2 / pi) (g + 0.044715 g^3))) */
 /* A workspace of NULL takes scratch memory of the call's own, which needs no room
  * from the caller and does not race with other calls; there is none while the stream
- * is being captured, where a call that needs one (up to 16 rows of K <= 4096 and 32 of
- * K <= 2048 do not) returns GQ_ERR_WORKSPACE, as does one of K above 2^21.
+ * is being captured, where a call that needs one (up to 16 rows of K <= 4096, 32 of
+ * K <= 2048 and four of 4-byte aligned 16-bit x do not) returns GQ_ERR_WORKSPACE, as does
+ * one that needs more than 128 MiB (32 rows and more of K = 2^21 and longer).
  * Calls that overlap must not share a workspace, and neither may two captured graphs
  * whose replays overlap.  Rows are taken in blocks, so the workspace stops growing
  * with M; the bytes for M rows are enough for every call of fewer.  N * 128 outputs stay below 2^31 bytes; K == 0 is refused. */
@@ -283,7 +291,8 @@ int gq_ffn_gate_up(int fmt, const void *d_gate, const void *d_up, const void *d_
  * dh, g, u and dg, du are [M][N] of `dtype`, dx [M][K] of dx_dtype.  dg and du (the
  * gradients of the projections, for adapters beside them) and dx may each be NULL:
  * not wanted.  dx is computed from dg and du as they are before their rounding, which
- * are brought to fp16 with a power-of-two scale per row.  dg may be the same buffer
+ * are brought to fp16 with a power-of-two scale per row; the weights are rounded as in
+ * the calls of many rows above: 3e-4 of a row of dx, Q4_K 6e-4.  dg may be the same buffer
  * as g and du the same as u or dh; no other overlap. */
 size_t gq_ffn_gate_up_bwd_workspace_bytes(int fmt, size_t M, size_t N, size_t K);
 int gq_ffn_gate_up_bwd(int fmt, const void *d_gate, const void *d_up, const void *d_dh, const void *d_g,
