@@ -703,7 +703,8 @@ k_front_rows_px(const uint8_t *__restrict__ wg, const uint8_t *__restrict__ wu, 
 // of gq_gemm_frag.h: fp16 activations by LDS DMA PD - 1 steps of 64 k ahead, weights PD steps
 // ahead in registers.  So are the weights' roundings to fp16: Q4_0 and Q8_0 once (1.7e-4 and 2.1e-4 of a product's row), Q6_K
 // d sc first (2.9e-4), Q4_K dmin m first (5.4e-4 where minima are 7.5 scales, as in weights about zero; as d sc (q - 8) + c, c
-// rounded, 2.3e-4 there, but 2.8e-4 against 2.1e-4 where they are not).  KG: groups of waves that share the tile and take every KG-th step,
+// rounded, 2.3e-4 there, but 2.8e-4 against 2.1e-4 where they are not).
+// KG: groups of waves that share the tile and take every KG-th step,
 // their sums added through LDS at the end.
 template <int DT>
 GQ_DEV void front_put(const __amdgpu_buffer_rsrc_t &r, uint32_t o, int dt, float v) {
