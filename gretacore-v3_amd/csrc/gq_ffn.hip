@@ -662,7 +662,7 @@ __global__ void __launch_bounds__(kDguThreads) k_front_dgu(const void *dh, const
 
 // dx[m][k] = sum over n of dg[m][n] W_gate[n][k] + du[m][n] W_up[n][k]: the sum runs over the weights'
 // rows, while a T16 record holds 16 rows of 128 k, each row's codes side by side.  Steps of 64 n (four row
-// tiles), gate's before up's.  The records go to LDS as they are (by DMA, the slots of a 64-lane
+// tiles), the first matrix's before the second's (`half` steps each; or one matrix alone, half = nsteps).  The records go to LDS as they are (by DMA, the slots of a 64-lane
 // record XOR-swizzled), and a lane collects for its four columns the codes of 8 rows, 16 bits (Q8_0
 // 32) a row: joined in pairs of rows they are masked into fp16 pairs that run along n, B
 // fragments of v_mfma_f32_32x32x16_f16 without a transposition.  Lane c of 32 owns columns
@@ -723,7 +723,7 @@ GQ_DEV void dx_store_scales(const gq_u4 &v, uint32_t p, int r, _Float16 *t) {
 template <int FMT, int WN, int KG, int TM, int PD>
 __global__ void __launch_bounds__(64 * WN * KG) k_front_dx(const uint8_t *__restrict__ wg, const uint8_t *__restrict__ wu, uint32_t w_bytes, uint32_t sc_off,
            const _Float16 *__restrict__ a16, const float *__restrict__ rs, void *__restrict__ y, int dt, int M, int K,
-           int C, int ntiles, int nsteps, int sps, int tiles_m) {
+           int C, int ntiles, int nsteps, int half, int sps, int tiles_m) {
   constexpr int NW = WN, BM = 32 * TM, BN = 128 * WN, ROWS_T = 16 * kDxRows<FMT>, RECS = kDxRecs<FMT>;
   constexpr int NREC = 4 * WN * RECS, RPW = (NREC + NW - 1) / NW;  // records a step, per wave
   static_assert(NREC % NW == 0, "records");
@@ -758,9 +758,9 @@ __global__ void __launch_bounds__(64 * WN * KG) k_front_dx(const uint8_t *__rest
     int s = step_of(l);
     s = s < s1 ? s : s1 - 1;
     load_a_lds_b<BM, NW>(a16, ao, s, wave, reinterpret_cast<_Float16 *>(stage(st)));
-    const bool up = 2 * s >= nsteps;
+    const bool up = s >= half;
     const __amdgpu_buffer_rsrc_t wr = mat(up);
-    const uint32_t t0 = 4u * (uint32_t)(up ? s - nsteps / 2 : s);
+    const uint32_t t0 = 4u * (uint32_t)(up ? s - half : s);
     uint8_t *wl = stage(st) + A_B;
 #pragma unroll
     for (int i = 0; i < RPW; ++i) {
@@ -786,8 +786,8 @@ __global__ void __launch_bounds__(64 * WN * KG) k_front_dx(const uint8_t *__rest
   auto load_scales = [&](int l) __attribute__((always_inline)) {
     int s = step_of(l);
     s = s < s1 ? s : s1 - 1;
-    const bool up = 2 * s >= nsteps;
-    const uint32_t t = 4u * (uint32_t)(up ? s - nsteps / 2 : s) + (uint32_t)stile, kc = (uint32_t)(kc0 + wave);
+    const bool up = s >= half;
+    const uint32_t t = 4u * (uint32_t)(up ? s - half : s) + (uint32_t)stile, kc = (uint32_t)(kc0 + wave);
     const uint32_t c = kSuper<FMT> ? kc >> 1 : kc;
     return dx_load_scales<FMT>(mat(up), sc_off, t * (uint32_t)C + c, kSuper<FMT> ? kc & 1u : 0u, (uint32_t)srow,
                                t < (uint32_t)ntiles && c < (uint32_t)C);
@@ -1225,12 +1225,8 @@ extern "C" int gq_ffn_gate_up(int fmt, const void *gate, const void *up, const v
   return GQ_OK;
 }
 
-// The backward pass's plan: rows at a time, the kernel's shape and the parts of the sum over n
+// The plan of sums over the weights' rows: rows at a time, the kernel's shape and the parts of the sum over n (gq_internal.h)
 namespace {
-struct DxPlan {
-  size_t mb, np;  // rows a block; columns of each half of A
-  int shape, parts, sps;
-};
 struct DxShape {
   int bm, bn, kg;
   size_t rows;  // the largest block it is taken for
@@ -1238,14 +1234,15 @@ struct DxShape {
 // (Q4_K, K = 4096: 128 x 14336 by the second shape 73.4 us, the third 94.5; 128 x 5003 41.4 and 54.8)
 constexpr DxShape kDxShapes[3] = {{32, 128, 4, 32}, {64, 128, 4, 128}, {128, 256, 2, ~(size_t)0}};
 
-DxPlan dx_plan(size_t M, size_t N, size_t K) {
-  DxPlan p;
+GqDxPlan dx_plan(size_t M, size_t N, size_t K, int mats) {
+  GqDxPlan p;
+  p.mats = mats;
   p.np = (gq_tiles(N) * 16 + 63) & ~(size_t)63;
   // A below 120 MiB (what a scratch block holds with the rest), whole tiles of rows where they fit
-  const size_t fit = ((size_t)120 << 20) / (4 * p.np);  // (np <= 2^24: at least 1)
+  const size_t fit = ((size_t)120 << 20) / (2 * mats * p.np);  // (np <= 2^24: at least 1)
   p.mb = fit < 256 ? fit : fit & ~(size_t)255;
   if (M < p.mb) p.mb = M;
-  const size_t nsteps = 2 * p.np / 64;
+  const size_t nsteps = mats * p.np / 64;
   p.shape = 0;
   while (p.mb > kDxShapes[p.shape].rows) ++p.shape;
   const DxShape &t = kDxShapes[p.shape];
@@ -1256,16 +1253,16 @@ DxPlan dx_plan(size_t M, size_t N, size_t K) {
   p.sps = (int)((nsteps + want - 1) / want);
   p.parts = (int)((nsteps + p.sps - 1) / p.sps);
   // all of it below what one scratch block holds
-  const size_t held = gq_align256(p.mb * 4 * p.np) + gq_align256((p.mb + 256) * 4);
+  const size_t held = gq_align256(p.mb * 2 * mats * p.np) + gq_align256((p.mb + 256) * 4);
   while (p.parts > 1 && held + (size_t)p.parts * p.mb * K * 4 + 256 > kGqScratchMax) {
     p.sps = (int)((nsteps + p.parts - 2) / (p.parts - 1));
     p.parts = (int)((nsteps + p.sps - 1) / p.sps);
   }
   return p;
 }
-size_t dx_a_bytes(const DxPlan &p) { return gq_align256(p.mb * 2 * p.np * 2); }
-size_t dx_rs_bytes(const DxPlan &p) { return gq_align256((p.mb + 256) * 4); }
-size_t dx_bytes(const DxPlan &p, size_t K) {
+size_t dx_a_bytes(const GqDxPlan &p) { return gq_align256(p.mb * p.mats * p.np * 2); }
+size_t dx_rs_bytes(const GqDxPlan &p) { return gq_align256((p.mb + 256) * 4); }
+size_t dx_bytes(const GqDxPlan &p, size_t K) {
   return dx_a_bytes(p) + dx_rs_bytes(p) + (p.parts > 1 ? gq_align256((size_t)p.parts * p.mb * K * 4) : 0);
 }
 
@@ -1273,14 +1270,14 @@ size_t dx_bytes(const DxPlan &p, size_t K) {
 // may have more parts, so its own bytes may be more than M's).  A plan with parts has at most 256 / workgroups of
 // them, so parts * (rows, up to whole tiles) * (columns, up to whole tiles) <= 256 tiles; it has them only
 // while its workgroups are at most 128.
-size_t dx_most_bytes(size_t M, size_t N, size_t K) {
-  const DxPlan p = dx_plan(M, N, K);
+size_t dx_most_bytes(size_t M, size_t N, size_t K, int mats) {
+  const GqDxPlan p = dx_plan(M, N, K, mats);
   size_t most = dx_a_bytes(p) + dx_rs_bytes(p);  // (of the block of most rows)
-  const size_t nsteps = 2 * p.np / 64;
+  const size_t nsteps = mats * p.np / 64;
   for (int i = 0; i <= p.shape; ++i) {
     const DxShape &t = kDxShapes[i];
     const size_t tk = (K + t.bn - 1) / t.bn, tiles = 128 / tk, parts = std::min(nsteps / (4 * t.kg), 256 / tk);
-    DxPlan q = p;  // the most rows of this shape that have parts
+    GqDxPlan q = p;  // the most rows of this shape that have parts
     q.mb = std::min({p.mb, t.rows, tiles * t.bm});
     if (q.mb <= (i ? kDxShapes[i - 1].rows : 0) || parts < 2) continue;
     const size_t sums = std::min((size_t)256 * t.bm * t.bn, parts * q.mb * K);
@@ -1291,18 +1288,19 @@ size_t dx_most_bytes(size_t M, size_t N, size_t K) {
 }
 
 template <int FMT, int WN, int KG, int TM, int PD>
-int launch_dx_t(const DxPlan &p, const void *wg, const void *wu, const _Float16 *a16, const float *rs, void *y, int dt, int M,
+int launch_dx_t(const GqDxPlan &p, const void *wg, const void *wu, const _Float16 *a16, const float *rs, void *y, int dt, int M,
                 size_t N, size_t K, hipStream_t s) {
   const int tiles_m = (M + 32 * TM - 1) / (32 * TM), tiles_k = (int)((K + 128 * WN - 1) / (128 * WN));
   GQ_CHECK((size_t)tiles_m * (size_t)tiles_k <= 0x7FFFFFFFu, GQ_ERR_INVALID_ARGS);  // (one grid dimension)
   hipLaunchKernelGGL((k_front_dx<FMT, WN, KG, TM, PD>), dim3((unsigned)(tiles_m * tiles_k), (unsigned)p.parts),
                      dim3(64 * WN * KG), 0, s, (const uint8_t *)wg, (const uint8_t *)wu,
                      (uint32_t)gq_packed_bytes(FMT, N, K), (uint32_t)gq_sc_plane_offset(FMT, N, K), a16, rs, y, dt, M, (int)K,
-                     (int)gq_chunks(FMT, K), (int)gq_tiles(N), (int)(2 * p.np / 64), p.sps, tiles_m);
+                     (int)gq_chunks(FMT, K), (int)gq_tiles(N), (int)(p.mats * p.np / 64),
+                     (int)(p.np / 64), p.sps, tiles_m);
   return gq_last_launch();
 }
 template <int FMT>
-int launch_dx(const DxPlan &p, const void *wg, const void *wu, const _Float16 *a16, const float *rs, void *y, int dt, int M,
+int launch_dx(const GqDxPlan &p, const void *wg, const void *wu, const _Float16 *a16, const float *rs, void *y, int dt, int M,
               size_t N, size_t K, hipStream_t s) {
 #define GQ_DX(...) launch_dx_t<FMT, __VA_ARGS__>(p, wg, wu, a16, rs, y, dt, M, N, K, s)
   switch (p.shape) {
@@ -1326,9 +1324,27 @@ int launch_dgu(const void *dh, const void *g, const void *u, void *dg, void *du,
 }
 }  // namespace
 
+GqDxPlan gq_dx_plan(size_t M, size_t N, size_t K, int mats) { return dx_plan(M, N, K, mats); }
+size_t gq_dx_a_bytes(const GqDxPlan &p) { return dx_a_bytes(p); }
+size_t gq_dx_rs_bytes(const GqDxPlan &p) { return dx_rs_bytes(p); }
+size_t gq_dx_bytes(const GqDxPlan &p, size_t K) { return dx_bytes(p, K); }
+size_t gq_dx_most_bytes(size_t M, size_t N, size_t K, int mats) { return dx_most_bytes(M, N, K, mats); }
+int gq_launch_dx(int fmt, const GqDxPlan &p, const void *w0, const void *w1, const _Float16 *a16, const float *rs, float *part,
+                 void *y, int dt, int M, size_t N, size_t K, hipStream_t s) {
+  void *to = p.parts > 1 ? (void *)part : y;
+  if (fmt == GQ_FMT_Q4_0) GQ_TRY(launch_dx<GQ_FMT_Q4_0>(p, w0, w1, a16, rs, to, dt, M, N, K, s));
+  else if (fmt == GQ_FMT_Q8_0) GQ_TRY(launch_dx<GQ_FMT_Q8_0>(p, w0, w1, a16, rs, to, dt, M, N, K, s));
+  else if (gq_fmt_is_q6k(fmt)) GQ_TRY(launch_dx<GQ_FMT_Q6_K>(p, w0, w1, a16, rs, to, dt, M, N, K, s));
+  else GQ_TRY(launch_dx<GQ_FMT_Q4_K>(p, w0, w1, a16, rs, to, dt, M, N, K, s));
+  return p.parts > 1 ? launch_dx_sum(part, rs, y, dt, (size_t)M, K, p.parts, s) : GQ_OK;
+}
+int gq_launch_zeros(void *y, int dt, size_t M, size_t K, hipStream_t s) {
+  return launch_dx_sum(nullptr, nullptr, y, dt, M, K, 0, s);
+}
+
 extern "C" size_t gq_ffn_gate_up_bwd_workspace_bytes(int fmt, size_t M, size_t N, size_t K) {
   if (!gq_fmt_valid(fmt) || M > GQ_MAX_DIM || N > GQ_MAX_DIM || K > GQ_MAX_DIM || M == 0 || N == 0 || K == 0) return 0;
-  return dx_most_bytes(M, N, K);
+  return dx_most_bytes(M, N, K, 2);
 }
 
 extern "C" int gq_ffn_gate_up_bwd(int fmt, const void *gate, const void *up, const void *dh, const void *g,
@@ -1341,7 +1357,7 @@ extern "C" int gq_ffn_gate_up_bwd(int fmt, const void *gate, const void *up, con
   hipStream_t s = (hipStream_t)stream;
   if (N == 0) return dx ? launch_dx_sum(nullptr, nullptr, dx, dx_dtype, M, K, 0, s) : GQ_OK;  // (sums of nothing)
   GQ_CHECK(dh && g && u, GQ_ERR_INVALID_ARGS);
-  const DxPlan plan = dx_plan(M, N, K);
+  const GqDxPlan plan = dx_plan(M, N, K, 2);
   const size_t need = dx ? gq_ffn_gate_up_bwd_workspace_bytes(fmt, M, N, K) : 0;
   GqScratch sc(ws || !dx ? 0 : dx_bytes(plan, K), s);
   if (ws) GQ_CHECK(ws_bytes >= need, GQ_ERR_WORKSPACE);
@@ -1360,12 +1376,7 @@ extern "C" int gq_ffn_gate_up_bwd(int fmt, const void *gate, const void *up, con
     else if (dtype == GQ_DT_F16) GQ_TRY(launch_dgu<GQ_DT_F16>(at(dh), at(g), at(u), at(dg), at(du), a16, rs, m, (int)N, (int)plan.np, act, s));
     else GQ_TRY(launch_dgu<GQ_DT_BF16>(at(dh), at(g), at(u), at(dg), at(du), a16, rs, m, (int)N, (int)plan.np, act, s));
     if (!dx) continue;
-    void *y = (uint8_t *)dx + m0 * xs, *to = plan.parts > 1 ? (void *)part : y;
-    if (fmt == GQ_FMT_Q4_0) GQ_TRY(launch_dx<GQ_FMT_Q4_0>(plan, gate, up, a16, rs, to, dx_dtype, m, N, K, s));
-    else if (fmt == GQ_FMT_Q8_0) GQ_TRY(launch_dx<GQ_FMT_Q8_0>(plan, gate, up, a16, rs, to, dx_dtype, m, N, K, s));
-    else if (gq_fmt_is_q6k(fmt)) GQ_TRY(launch_dx<GQ_FMT_Q6_K>(plan, gate, up, a16, rs, to, dx_dtype, m, N, K, s));
-    else GQ_TRY(launch_dx<GQ_FMT_Q4_K>(plan, gate, up, a16, rs, to, dx_dtype, m, N, K, s));
-    if (plan.parts > 1) GQ_TRY(launch_dx_sum(part, rs, y, dx_dtype, (size_t)m, K, plan.parts, s));
+    GQ_TRY(gq_launch_dx(fmt, plan, gate, up, a16, rs, part, (uint8_t *)dx + m0 * xs, dx_dtype, m, N, K, s));
   }
   return GQ_OK;
 }

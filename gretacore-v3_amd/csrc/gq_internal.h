@@ -109,5 +109,22 @@ int gq_launch_a_to_f16(const void *a, int a_dtype, _Float16 *o, float *rs, int M
                        hipStream_t s);
 // c[i] = the sum over p of part[p][i], in part order (gq_gemm.hip)
 int gq_launch_split_sum(const float *part, float *c, size_t n, int parts, hipStream_t s);
+// Sums over the weights' rows, y[m][k] = sum over n of a0[m][n] W0[n][k] (+ a1[m][n] W1[n][k], mats = 2), of up to mb rows
+// at a time (gq_ffn.hip).  A is fp16 [m][mats * np], each half padded with zeros to np columns, rs its row
+// scales; part: the parts' sums, behind dx_a_bytes and dx_rs_bytes in a workspace of dx_bytes (dx_most_bytes: enough
+// for every call of at most M rows).
+struct GqDxPlan {
+  size_t mb, np;
+  int shape, parts, sps, mats;
+};
+GqDxPlan gq_dx_plan(size_t M, size_t N, size_t K, int mats);
+size_t gq_dx_a_bytes(const GqDxPlan &p);
+size_t gq_dx_rs_bytes(const GqDxPlan &p);
+size_t gq_dx_bytes(const GqDxPlan &p, size_t K);
+size_t gq_dx_most_bytes(size_t M, size_t N, size_t K, int mats);
+int gq_launch_dx(int fmt, const GqDxPlan &p, const void *w0, const void *w1, const _Float16 *a16, const float *rs, float *part,
+                 void *y, int dt, int M, size_t N, size_t K, hipStream_t s);
+// zeros [M][K] of an activation dtype (K % 32 == 0)
+int gq_launch_zeros(void *y, int dt, size_t M, size_t K, hipStream_t s);
 // Compute units of the current device (cached per device; 0 without a device).
 int gq_device_cus(void);

@@ -1,0 +1,445 @@
+// gq_linear.hip -- the product with bias, activation and residual in its epilogue over T16 weights,
+// any number of rows (few rows here, tiles in gq_linear_rb.hip), and its backward pass.
+#include <algorithm>
+#include <type_traits>
+
+#include "gq_internal.h"
+#include "gq_linear.h"
+#include "gq_rows_frag.h"
+
+namespace {
+
+// ---- forward: up to 64 rows, units of 128 k ------------------------------------------
+// The weights' bytes bound these: a workgroup takes R row tiles, its KS waves share K unit by unit with PD units in
+// flight each, and their sums are added through LDS.
+template <int KS, int R, typename At>
+GQ_DEV void lin_out(At at, const float *rs, const LinEpi &e, int M, int N, int block) {
+  for (int o = threadIdx.x; o < 16 * R * M; o += 64 * KS) {
+    const int nl = o % (16 * R), m = o / (16 * R), n = 16 * R * block + nl;
+    float y = 0.f;
+#pragma unroll
+    for (int k = 0; k < KS; ++k) y += at(k, nl >> 4, nl & 15, m);
+    if (n < N) lin_put(e, (size_t)m, n, N, rs ? y * rs[m] : y);
+  }
+}
+
+// Up to 4 rows of 16-bit x: codes and x as they are, scales in fp32 (gq_rows_frag.h)
+template <int FMT, int XT, int MR, int R, int KS, int PD>
+__global__ void __launch_bounds__(64 * KS)
+k_lin_few(const uint8_t *__restrict__ w, size_t sc_off, const void *__restrict__ x, const float *__restrict__ rs, LinEpi e,
+          int M, int N, int K, int C, int units) {
+  constexpr int NG = kFewGroups<FMT>;
+  constexpr float OFF = kFewOff<FMT, XT>;
+  __shared__ float red[KS][R][MR][64];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int g = lane >> 4, ntiles = (int)gq_tiles(N);
+  FTile<FMT> tl[R];
+#pragma unroll
+  for (int t = 0; t < R; ++t) {
+    const int tile = (int)blockIdx.x * R + t;
+    tl[t] = ftile<FMT>(w, sc_off, (size_t)(tile < ntiles ? tile : ntiles - 1), C);  // (clamped: not stored)
+  }
+  const __amdgpu_buffer_rsrc_t xr =
+      __builtin_amdgcn_make_buffer_rsrc(const_cast<void *>(x), (short)0, (int)(2u * (uint32_t)M * (uint32_t)K), 0x00020000);
+  const int xrow = lane & 3, xk = 64 * ((lane >> 3) & 1) + 16 * g + 8 * ((lane >> 2) & 1);
+  FUnit<FMT> us[PD][R];
+  gq_u4 xs[PD];
+  auto request = [&](int unit, int st) __attribute__((always_inline)) {
+#pragma unroll
+    for (int t = 0; t < R; ++t) load_unit<FMT>(tl[t], unit, lane, us[st][t]);
+    const uint32_t k = 128u * (uint32_t)unit + (uint32_t)xk;  // (K is whole 32-blocks: a run is wholly in or out)
+    const bool in = xrow < M && k < (uint32_t)K;
+    const auto v = __builtin_amdgcn_raw_buffer_load_b128(xr, in ? 2u * ((uint32_t)xrow * (uint32_t)K + k) : 0xFFFFFFF0u, 0, 0);
+    xs[st] = gq_u4{v[0], v[1], v[2], v[3]};
+  };
+  float acc[R][MR] = {};
+  uint32_t mg;  // (kept in a register)
+  if constexpr (XT == GQ_DT_F16) asm volatile("v_mov_b32 %0, 0x64006400" : "=v"(mg));
+  else asm volatile("v_mov_b32 %0, 0x43004300" : "=v"(mg));
+  constexpr uint32_t one = XT == GQ_DT_F16 ? 0x3C003C00u : 0x3F803F80u;
+  const gq_u4 ones = {one, one, one, one};
+  const gq_f4 zero = {0.f, 0.f, 0.f, 0.f};
+  auto compute = [&](int unit, int st) __attribute__((always_inline)) {
+    const gq_u4 xv = kNibOrder<FMT> ? nib_order(xs[st]) : xs[st];
+    float s[R][2], mn[R][2];
+#pragma unroll
+    for (int t = 0; t < R; ++t) few_scales<FMT>(us[st][t], unit, g & (NG - 1), s[t], mn[t]);
+    auto step = [&](auto mc) __attribute__((always_inline)) {
+      constexpr int m = decltype(mc)::value;
+      const gq_u4 a0 = few_operand<NG, 2 * m>(xv), a1 = few_operand<NG, 2 * m + 1>(xv);
+      gq_f4 sx = zero;
+      if constexpr (OFF != 0.f || FMT == GQ_FMT_Q4_K) sx = few_mfma<XT>(a1, ones, few_mfma<XT>(a0, ones, zero));
+#pragma unroll
+      for (int t = 0; t < R; ++t) {
+        gq_u4 b[2];
+        few_codes<FMT, XT>(us[st][t], m, mg, b);
+        const gq_f4 d = few_mfma<XT>(a1, b[1], few_mfma<XT>(a0, b[0], zero));
+        const float o = FMT == GQ_FMT_Q4_K ? fmaf(s[t][m], OFF, mn[t][m]) : 0.f;
+#pragma unroll
+        for (int v = 0; v < MR; ++v) {
+          if constexpr (FMT == GQ_FMT_Q4_K) acc[t][v] = fmaf(s[t][m], d[v], fmaf(-o, sx[v], acc[t][v]));
+          else acc[t][v] = fmaf(s[t][m], OFF != 0.f ? fmaf(-OFF, sx[v], d[v]) : d[v], acc[t][v]);
+        }
+      }
+    };
+    step(std::integral_constant<int, 0>{});
+    step(std::integral_constant<int, 1>{});
+  };
+  walk_units<PD, KS>(units, wave, request, compute);
+#pragma unroll
+  for (int t = 0; t < R; ++t)
+#pragma unroll
+    for (int v = 0; v < MR; ++v) red[wave][t][v][lane] = acc[t][v];
+  __syncthreads();
+  lin_out<KS, R>(
+      [&](int k, int t, int n, int m) {
+        float y = 0.f;
+#pragma unroll
+        for (int i = 0; i < NG; ++i) y += red[k][t][MR == 1 ? 0 : m][16 * i + n];
+        return y;
+      },
+      rs, e, M, N, (int)blockIdx.x);
+}
+
+// More rows: fp16 rows of x with a power-of-two scale each, the scale groups folded into the weights (gq_rows_frag.h)
+template <int FMT, int MT, int R, int KS, int PD>
+__global__ void __launch_bounds__(64 * KS)
+k_lin_rows(const uint8_t *__restrict__ w, size_t sc_off, const _Float16 *__restrict__ a16, int lda,
+           const float *__restrict__ rs, LinEpi e, int M, int N, int C, int units) {
+  __shared__ gq_f4 red[KS][R][MT][64];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int g = lane >> 4, r = lane & 15, ntiles = (int)gq_tiles(N);
+  FTile<FMT> tl[R];
+#pragma unroll
+  for (int t = 0; t < R; ++t) {
+    const int tile = (int)blockIdx.x * R + t;
+    tl[t] = ftile<FMT>(w, sc_off, (size_t)(tile < ntiles ? tile : ntiles - 1), C);  // (clamped: not stored)
+  }
+  const __amdgpu_buffer_rsrc_t xr = __builtin_amdgcn_make_buffer_rsrc(
+      const_cast<_Float16 *>(a16), (short)0, (int)(2u * (uint32_t)M * (uint32_t)lda), 0x00020000);
+  uint32_t xo[MT];
+#pragma unroll
+  for (int t = 0; t < MT; ++t) {
+    const int row = 16 * t + r;
+    xo[t] = 2u * ((uint32_t)(row < M ? row : M - 1) * (uint32_t)lda + 16u * (uint32_t)g);  // (rows past M: not stored)
+  }
+  FUnit<FMT> us[PD][R];
+  gq_half8 xs[PD][MT][4];
+  auto request = [&](int unit, int st) __attribute__((always_inline)) {
+#pragma unroll
+    for (int t = 0; t < R; ++t) load_unit<FMT>(tl[t], unit, lane, us[st][t]);
+#pragma unroll
+    for (int t = 0; t < MT; ++t) {
+      const uint32_t o = unit < units ? xo[t] + 256u * (uint32_t)unit : 0xFFFFFF00u;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const auto v = __builtin_amdgcn_raw_buffer_load_b128(xr, o + 128u * (i >> 1) + 16u * (i & 1), 0, 0);
+        xs[st][t][i] = __builtin_bit_cast(gq_half8, gq_u4{v[0], v[1], v[2], v[3]});
+      }
+    }
+  };
+  gq_f4 acc[R][MT];
+#pragma unroll
+  for (int t = 0; t < R; ++t)
+#pragma unroll
+    for (int i = 0; i < MT; ++i) acc[t][i] = gq_f4{0.f, 0.f, 0.f, 0.f};
+  const uint32_t mg = gq_nib_magic();
+  auto compute = [&](int unit, int st) __attribute__((always_inline)) {
+#pragma unroll
+    for (int t = 0; t < R; ++t) rows_add<FMT, MT>(us[st][t], unit, g, mg, xs[st], acc[t]);
+  };
+  walk_units<PD, KS>(units, wave, request, compute);
+#pragma unroll
+  for (int t = 0; t < R; ++t)
+#pragma unroll
+    for (int i = 0; i < MT; ++i) red[wave][t][i][lane] = acc[t][i];
+  __syncthreads();
+  lin_out<KS, R>(
+      [&](int k, int t, int n, int m) {
+        return reinterpret_cast<const float *>(&red[k][t][m >> 4][16 * ((m >> 2) & 3) + n])[m & 3];
+      },
+      rs, e, M, N, (int)blockIdx.x);
+}
+
+template <int FMT, int XT>
+int launch_few_t(const void *w, const void *x, const float *rs, const LinEpi &e, int M, int N, int K, hipStream_t s) {
+  const int units = (int)(gq_kpad(FMT, K) / 128);
+  const size_t tiles = gq_tiles(N);
+#define GQ_FEW(MR, R, KS, PD)                                                                                               \
+  hipLaunchKernelGGL((k_lin_few<FMT, XT, MR, R, KS, PD>), dim3((unsigned)((tiles + (R)-1) / (R))), dim3(64 * (KS)), 0, s,     \
+                     (const uint8_t *)w, gq_sc_plane_offset(FMT, N, K), x, rs, e, M, N, K, (int)gq_chunks(FMT, K), units)
+#define GQ_FEW_M(R, KS, PD)           \
+  do {                                \
+    if (M == 1) GQ_FEW(1, R, KS, PD); \
+    else GQ_FEW(4, R, KS, PD);        \
+  } while (0)
+  if (tiles <= 512) GQ_FEW_M(1, 8, 4);
+  else GQ_FEW_M(2, 4, 3);
+#undef GQ_FEW_M
+#undef GQ_FEW
+  return gq_last_launch();
+}
+template <int FMT>
+int launch_rows_t(const void *w, const _Float16 *a16, int lda, const float *rs, const LinEpi &e, int M, int N, int K,
+                  hipStream_t s) {
+  const int units = (int)(gq_kpad(FMT, K) / 128);
+  const size_t tiles = gq_tiles(N);
+#define GQ_ROWS(MT, R, KS, PD)                                                                                              \
+  hipLaunchKernelGGL((k_lin_rows<FMT, MT, R, KS, PD>), dim3((unsigned)((tiles + (R)-1) / (R))), dim3(64 * (KS)), 0, s,        \
+                     (const uint8_t *)w, gq_sc_plane_offset(FMT, N, K), a16, lda, rs, e, M, N, (int)gq_chunks(FMT, K), units)
+  if (M > 32) GQ_ROWS(4, 1, 8, 2);
+  else if (M > 16) GQ_ROWS(2, 1, 8, 2);
+  else GQ_ROWS(1, 1, 8, 3);
+#undef GQ_ROWS
+  return gq_last_launch();
+}
+
+// ---- backward ----------------------------------------------------------------------
+// dz = dy act'(z): one pass over dy and z, a workgroup a row at a time (row blockIdx.x, + gridDim.x, ...).  dz goes out in its own
+// type where it is wanted, and, as it is before that rounding, to fp16 with one power-of-two scale per row (the row's
+// largest to [2^14, 2^15); 2^-114 to 2^126), padded with zeros to np columns: the A operand of dx.  The workgroup's rows are summed
+// by column into its row of `part` (dbias), which a last kernel adds over the workgroups in their order.  The first kDzRuns
+// * 4096 columns of a row and their sums stay in registers, the rest is computed twice and summed in `part`.
+constexpr int kDzThreads = 512, kDzRuns = 4;
+template <int DT>
+__global__ void __launch_bounds__(kDzThreads) k_lin_dz(const void *dy, const void *z, void *dzo, _Float16 *a16, float *rs,
+                                                       float *part, int add, int M, int N, int np, int act) {
+  __shared__ float top_s[2][kDzThreads / 64];
+  const int tid = threadIdx.x;
+  constexpr int SPAN = 8 * kDzThreads * kDzRuns;
+  float sum[kDzRuns][8];
+  float *pr = part ? part + (size_t)blockIdx.x * (size_t)N : nullptr;
+#pragma unroll
+  for (int i = 0; i < kDzRuns; ++i)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const int n = 8 * (tid + kDzThreads * i) + e;
+      sum[i][e] = part && add && n < N ? pr[n] : 0.f;
+    }
+  int buf = 0;
+  for (int m = (int)blockIdx.x; m < M; m += (int)gridDim.x, buf ^= 1) {
+    const size_t row = (size_t)m * (size_t)N;
+    auto grads = [&](int k, float (&o)[8]) __attribute__((always_inline)) {
+      float a[8], b[8];
+      dgu_load<DT>(dy, row, k, N, a);
+      if (act == GQ_ACT_NONE) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) o[e] = a[e];
+        return;
+      }
+      dgu_load<DT>(z, row, k, N, b);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) o[e] = k + e < N ? a[e] * lin_act_d(act, b[e]) : 0.f;
+    };
+    float d[kDzRuns][8], top = 0.f;
+#pragma unroll
+    for (int i = 0; i < kDzRuns; ++i) {
+      const int k = 8 * (tid + kDzThreads * i);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) d[i][e] = 0.f;
+      if (k < N) grads(k, d[i]);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        top = fmaxf(top, fabsf(d[i][e]));
+        sum[i][e] += d[i][e];
+      }
+    }
+    if (a16)
+      for (int k = SPAN + 8 * tid; k < N; k += 8 * kDzThreads) {
+        float a[8];
+        grads(k, a);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(a[e]));
+      }
+    float f2 = 0.f;
+    if (a16) {
+#pragma unroll
+      for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
+      if ((tid & 63) == 0) top_s[buf][tid >> 6] = top;
+      __syncthreads();  // (two buffers: a row's maxima are read before the next row's barrier, the one after writes them)
+#pragma unroll
+      for (int w = 0; w < kDzThreads / 64; ++w) top = fmaxf(top, top_s[buf][w]);
+      const int sh = 14 + 127 - (int)((__float_as_uint(top) >> 23) & 0xFFu), cut = sh > 126 ? 126 : sh;
+      f2 = __uint_as_float((uint32_t)(127 + cut) << 23);
+      if (tid == 0) rs[m] = __uint_as_float((uint32_t)(127 - cut) << 23);
+    }
+    auto put = [&](int k, const float (&a)[8]) __attribute__((always_inline)) {
+      if (dzo && k < N) dgu_store<DT>(dzo, row, k, N, a);
+      if (!a16 || k >= np) return;
+      gq_half8 x;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] = (_Float16)(a[e] * f2);
+      *reinterpret_cast<gq_half8 *>(a16 + (size_t)m * (size_t)np + k) = x;
+    };
+#pragma unroll
+    for (int i = 0; i < kDzRuns; ++i) put(8 * (tid + kDzThreads * i), d[i]);
+    for (int k = SPAN + 8 * tid; k < (a16 ? np : N); k += 8 * kDzThreads) {
+      float a[8] = {};
+      if (k < N) grads(k, a);
+      put(k, a);
+      if (part)
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (k + e < N) pr[k + e] = (add || m != (int)blockIdx.x ? pr[k + e] : 0.f) + a[e];
+    }
+  }
+  if (!part) return;
+#pragma unroll
+  for (int i = 0; i < kDzRuns; ++i)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const int n = 8 * (tid + kDzThreads * i) + e;
+      if (n < N) pr[n] = sum[i][e];
+    }
+}
+// dbias = the workgroups' sums, in their order (none: zeros)
+__global__ void __launch_bounds__(256) k_lin_dbias(const float *__restrict__ part, float *__restrict__ db, int N, int parts) {
+  const int n = (int)blockIdx.x * 256 + (int)threadIdx.x;
+  if (n >= N) return;
+  double v = 0.0;
+  for (int p = 0; p < parts; ++p) v += (double)part[(size_t)p * (size_t)N + n];
+  db[n] = (float)v;
+}
+int launch_dbias(const float *part, float *db, size_t N, int parts, hipStream_t s) {
+  hipLaunchKernelGGL(k_lin_dbias, dim3((unsigned)((N + 255) / 256)), dim3(256), 0, s, part, db, (int)N, parts);
+  return gq_last_launch();
+}
+template <int DT>
+int launch_dz(const void *dy, const void *z, void *dz, _Float16 *a16, float *rs, float *part, int add, int wgs, int M, int N,
+              int np, int act, hipStream_t s) {
+  hipLaunchKernelGGL(k_lin_dz<DT>, dim3((unsigned)wgs), dim3(kDzThreads), 0, s, dy, z, dz, a16, rs, part, add, M, N, np, act);
+  return gq_last_launch();
+}
+
+bool lin_act_valid(int act) { return act >= GQ_ACT_SILU && act <= GQ_ACT_GELU; }
+
+int check_linear(int fmt, const void *w, size_t M, size_t N, size_t K, int act) {
+  GQ_TRY(gq_check_shape(fmt, N, K));
+  GQ_CHECK(M <= GQ_MAX_DIM, GQ_ERR_INVALID_ARGS);
+  GQ_CHECK(lin_act_valid(act), GQ_ERR_UNSUPPORTED);
+  GQ_CHECK(w || M == 0 || N == 0, GQ_ERR_INVALID_ARGS);
+  GQ_CHECK(((uintptr_t)w & 15) == 0, GQ_ERR_INVALID_ARGS);  // (16-byte loads)
+  // the kernels address a packed tensor with 32-bit offsets (the last 4 KiB: those that lie outside)
+  GQ_CHECK(N == 0 || K == 0 || gq_packed_bytes(fmt, N, K) <= 0xFFFFF000u, GQ_ERR_INVALID_ARGS);
+  return GQ_OK;
+}
+
+constexpr size_t kFew = 4, kRows = 64;
+// Rows a call takes at a time: their fp16 copies stay below 64 MiB, but for the rows that the kernels of few rows take at
+// once (64 of at most 2^24 columns: 2 GiB, 32-bit offsets still)
+size_t linear_rows(int fmt, size_t M, size_t K) {
+  const size_t fit = ((size_t)64 << 20) / (2 * gq_kpad(fmt, K));
+  const size_t mb = fit >= 256 ? fit & ~(size_t)255 : fit > kRows ? fit : kRows;
+  return M < mb ? M : mb;
+}
+
+}  // namespace
+
+extern "C" size_t gq_linear_workspace_bytes(int fmt, size_t M, size_t N, size_t K) {
+  if (!gq_fmt_valid(fmt) || M > GQ_MAX_DIM || N > GQ_MAX_DIM || K > GQ_MAX_DIM || K == 0) return 0;
+  const size_t mb = linear_rows(fmt, M, K);
+  return gq_align256(mb * (gq_kpad(fmt, K) + 8) * 2) + gq_align256((mb + 256) * 4);
+}
+
+extern "C" int gq_linear(int fmt, const void *w, const void *x, int x_dtype, const void *bias, int bias_dtype, int act,
+                         const void *resid, void *y, int y_dtype, void *z, size_t M, size_t N, size_t K, void *ws,
+                         size_t ws_bytes, void *stream) {
+  GQ_TRY(check_linear(fmt, w, M, N, K, act));
+  GQ_CHECK(gq_dtype_valid(x_dtype) && gq_dtype_valid(y_dtype) && (!bias || gq_dtype_valid(bias_dtype)), GQ_ERR_UNSUPPORTED);
+  if (M == 0 || N == 0) return GQ_OK;
+  GQ_CHECK(x && y && K > 0, GQ_ERR_INVALID_ARGS);
+  GQ_CHECK(N * 256 * gq_dtype_size(y_dtype) < ((size_t)1 << 31), GQ_ERR_INVALID_ARGS);  // (a tile's rows of outputs)
+  hipStream_t s = (hipStream_t)stream;
+  LinEpi e = {bias, resid, y, z, bias_dtype, y_dtype, act};
+  auto few = [&](const void *xp, int xt, const float *rs) -> int {
+#define GQ_FMT_X(F)                                                                             \
+  (xt == GQ_DT_F16 ? launch_few_t<F, GQ_DT_F16>(w, xp, rs, e, (int)M, (int)N, (int)K, s)         \
+                   : launch_few_t<F, GQ_DT_BF16>(w, xp, rs, e, (int)M, (int)N, (int)K, s))
+    if (fmt == GQ_FMT_Q4_0) return GQ_FMT_X(GQ_FMT_Q4_0);
+    if (fmt == GQ_FMT_Q8_0) return GQ_FMT_X(GQ_FMT_Q8_0);
+    if (gq_fmt_is_q6k(fmt)) return GQ_FMT_X(GQ_FMT_Q6_K);
+    return GQ_FMT_X(GQ_FMT_Q4_K);
+#undef GQ_FMT_X
+  };
+  if (M <= kFew && x_dtype != GQ_DT_F32 && (uintptr_t)x % 4 == 0) return few(x, x_dtype, nullptr);
+  const size_t need = gq_linear_workspace_bytes(fmt, M, N, K), mb = linear_rows(fmt, M, K), Kp = gq_kpad(fmt, K);
+  GqScratch sc(ws ? 0 : need, s);
+  if (ws) GQ_CHECK(ws_bytes >= need, GQ_ERR_WORKSPACE);
+  else ws = sc.ptr;
+  GQ_CHECK(ws, GQ_ERR_WORKSPACE);
+  GQ_CHECK(((uintptr_t)ws & 15) == 0, GQ_ERR_INVALID_ARGS);
+  _Float16 *a16 = (_Float16 *)ws;
+  float *rs = (float *)((uint8_t *)ws + gq_align256(mb * (Kp + 8) * 2));
+  const int q4 = fmt == GQ_FMT_Q4_0 || gq_fmt_is_q4k(fmt);
+  if (M <= kFew) {  // (x in fp32, or at an odd address)
+    GQ_TRY(gq_launch_a_to_f16(x, x_dtype, a16, rs, (int)M, (int)K, (int)K, 0, s));
+    return few(a16, GQ_DT_F16, rs);
+  }
+  if (M <= kRows) {  // rows 16 bytes longer than a multiple of 4 KiB, where 16 of them would collide
+    const int ld = (int)Kp + 8;
+    GQ_TRY(gq_launch_a_to_f16(x, x_dtype, a16, rs, (int)M, (int)K, ld, q4, s));
+#define GQ_ROWS_F(F) launch_rows_t<F>(w, a16, ld, rs, e, (int)M, (int)N, (int)K, s)
+    if (fmt == GQ_FMT_Q4_0) return GQ_ROWS_F(GQ_FMT_Q4_0);
+    if (fmt == GQ_FMT_Q8_0) return GQ_ROWS_F(GQ_FMT_Q8_0);
+    if (gq_fmt_is_q6k(fmt)) return GQ_ROWS_F(GQ_FMT_Q6_K);
+    return GQ_ROWS_F(GQ_FMT_Q4_K);
+#undef GQ_ROWS_F
+  }
+  const size_t xs = gq_dtype_size(x_dtype) * K, ys = gq_dtype_size(y_dtype) * N;
+  for (size_t m0 = 0; m0 < M; m0 += mb) {
+    const int m = (int)(M - m0 < mb ? M - m0 : mb);
+    GQ_TRY(gq_launch_a_to_f16((const uint8_t *)x + m0 * xs, x_dtype, a16, rs, m, (int)K, (int)Kp, q4, s));
+    LinEpi b = e;
+    b.resid = resid ? (const uint8_t *)resid + m0 * ys : nullptr;
+    b.y = (uint8_t *)y + m0 * ys;
+    b.z = z ? (uint8_t *)z + m0 * ys : nullptr;
+    GQ_TRY(gq_launch_linear_rb(fmt, w, a16, rs, &b, m, (int)N, (int)K, s));
+  }
+  return GQ_OK;
+}
+
+// Workgroups that share the rows of dz (and so the sums in `part`): one a CU, of 64 MiB of sums together at most (N <= 2^24)
+static size_t dz_groups(size_t M, size_t N) { return std::min({M, (size_t)256, ((size_t)1 << 24) / N}); }
+static size_t dbias_bytes(size_t M, size_t N) { return gq_align256(dz_groups(M, N) * N * 4); }
+
+extern "C" size_t gq_linear_bwd_workspace_bytes(int fmt, size_t M, size_t N, size_t K) {
+  if (!gq_fmt_valid(fmt) || M > GQ_MAX_DIM || N > GQ_MAX_DIM || K > GQ_MAX_DIM || M == 0 || N == 0 || K == 0) return 0;
+  return dbias_bytes(M, N) + gq_dx_most_bytes(M, N, K, 1);
+}
+
+extern "C" int gq_linear_bwd(int fmt, const void *w, const void *dy, const void *z, int dtype, int act, void *dz, void *dx,
+                             int dx_dtype, float *dbias, size_t M, size_t N, size_t K, void *ws, size_t ws_bytes,
+                             void *stream) {
+  GQ_TRY(check_linear(fmt, w, M, N, K, act));
+  GQ_CHECK(gq_dtype_valid(dtype) && gq_dtype_valid(dx_dtype), GQ_ERR_UNSUPPORTED);
+  hipStream_t s = (hipStream_t)stream;
+  if (M == 0) return dbias && N ? launch_dbias(nullptr, dbias, N, 0, s) : GQ_OK;  // (sums of nothing)
+  if (!dz && !dx && !dbias) return GQ_OK;
+  GQ_CHECK(K > 0, GQ_ERR_INVALID_ARGS);
+  if (N == 0) return dx ? gq_launch_zeros(dx, dx_dtype, M, K, s) : GQ_OK;
+  GQ_CHECK(dy && (z || act == GQ_ACT_NONE), GQ_ERR_INVALID_ARGS);
+  const GqDxPlan plan = gq_dx_plan(M, N, K, 1);
+  const size_t db = dbias ? dbias_bytes(M, N) : 0;
+  GqScratch sc0(ws ? 0 : db, s), sc1(ws || !dx ? 0 : gq_dx_bytes(plan, K), s);  // (two blocks: each fits one)
+  if (ws) GQ_CHECK(ws_bytes >= gq_linear_bwd_workspace_bytes(fmt, M, N, K), GQ_ERR_WORKSPACE);
+  GQ_CHECK(((uintptr_t)ws & 15) == 0, GQ_ERR_INVALID_ARGS);
+  float *sums = dbias ? (float *)(ws ? ws : sc0.ptr) : nullptr;
+  uint8_t *at16 = dx ? (ws ? (uint8_t *)ws + db : (uint8_t *)sc1.ptr) : nullptr;
+  GQ_CHECK((sums || !dbias) && (at16 || !dx), GQ_ERR_WORKSPACE);
+  _Float16 *a16 = dx ? (_Float16 *)at16 : nullptr;
+  float *rs = dx ? (float *)(at16 + gq_dx_a_bytes(plan)) : nullptr;
+  float *part = dx ? (float *)((uint8_t *)rs + gq_dx_rs_bytes(plan)) : nullptr;
+  const size_t es = gq_dtype_size(dtype) * N, xs = gq_dtype_size(dx_dtype) * K;
+  const size_t step = dx ? plan.mb : (size_t)1 << 20, wgs = dz_groups(M < step ? M : step, N);
+  for (size_t m0 = 0; m0 < M; m0 += step) {
+    const int m = (int)(M - m0 < step ? M - m0 : step);
+    auto at = [&](const void *p) { return p ? (void *)((uint8_t *)p + m0 * es) : nullptr; };
+#define GQ_DZ(DT) launch_dz<DT>(at(dy), at(z), at(dz), a16, rs, sums, m0 > 0, (int)wgs, m, (int)N, (int)plan.np, act, s)
+    if (dtype == GQ_DT_F32) GQ_TRY(GQ_DZ(GQ_DT_F32));
+    else if (dtype == GQ_DT_F16) GQ_TRY(GQ_DZ(GQ_DT_F16));
+    else GQ_TRY(GQ_DZ(GQ_DT_BF16));
+#undef GQ_DZ
+    if (dx) GQ_TRY(gq_launch_dx(fmt, plan, w, w, a16, rs, part, (uint8_t *)dx + m0 * xs, dx_dtype, m, N, K, s));
+  }
+  return dbias ? launch_dbias(sums, dbias, N, (int)wgs, s) : GQ_OK;
+}

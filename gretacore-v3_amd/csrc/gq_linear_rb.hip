@@ -1,0 +1,259 @@
+// gq_linear_rb.hip -- the tiled product with bias, activation and residual in its epilogue over T16 weights.
+#include <type_traits>
+
+#include "gq_gemm_frag.h"
+#include "gq_internal.h"
+#include "gq_linear.h"
+#include "gq_rows_frag.h"
+
+namespace {
+
+// The register-B tile of gq_gemm_frag.h: a wave owns NJ 32-column blocks of W over all BM rows, fp16 activations by LDS DMA PD - 1
+// steps of 64 k ahead, weights PD steps ahead in registers, one counted barrier a step.  KG: groups of waves that share the
+// tile and take every KG-th step, their sums added through LDS at the end.  gridDim.y parts of the steps: each part's fp32 sums go to
+// `part` [part][M][N], and k_lin_sum finishes them.
+template <int FMT, int BM, int WN, int NJ, int PD, int KG>
+__global__ void __launch_bounds__(64 * WN * KG) __attribute__((amdgpu_waves_per_eu(front_wpe(WN *KG), front_wpe(WN *KG))))
+k_lin_rb(const uint8_t *__restrict__ w, uint32_t sc_off, const _Float16 *__restrict__ a16, int lda, const float *__restrict__ rs,
+         LinEpi e, float *__restrict__ part, int M, int N, int C, int nsteps, int sps, int tiles_m) {
+  constexpr int KS = BK / 16, NW = WN, TM = BM / 32, BN = 32 * NJ * WN;
+  __shared__ __attribute__((aligned(16))) _Float16 As_0[KG * BM * BK];
+  __shared__ __attribute__((aligned(16))) _Float16 As_1[KG * BM * BK];
+  __shared__ __attribute__((aligned(16))) _Float16 As_2[PD >= 3 ? KG * BM * BK : 8];
+  __shared__ __attribute__((aligned(16))) _Float16 As_3[PD >= 4 ? KG * BM * BK : 8];
+  __shared__ __attribute__((aligned(16))) float rs_s[BM];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int kg = KG == 1 ? 0 : __builtin_amdgcn_readfirstlane((tid >> 6) / NW);
+  const int wave = __builtin_amdgcn_readfirstlane((tid >> 6) % NW);
+  const int wn = wave;
+  auto As_of = [&](auto b) -> _Float16 * {
+    constexpr int v = decltype(b)::value;
+    return (v == 0 ? As_0 : v == 1 ? As_1 : v == 2 ? As_2 : As_3) + kg * (BM * BK);
+  };
+  using B0 = std::integral_constant<int, 0>;
+  using B1 = std::integral_constant<int, 1>;
+  using B2 = std::integral_constant<int, 2>;
+  using B3 = std::integral_constant<int, 3>;
+  // loads a step may leave in flight: activations of steps s + 2 .. s + PD - 1, weights of s + 2 .. s + PD
+  constexpr int NA = BM / (8 * NW), pend = (PD - 2) * NA + (PD - 1) * kRLoads<FMT> * NJ;
+  int mt, nt;
+  tile_of_g(blockIdx.x, gridDim.x, tiles_m, (N + BN - 1) / BN, 4, mt, nt);
+  const int m0 = mt * BM, n0 = nt * BN;
+  // this part's steps s0 .. s1 (whole rounds of the groups)
+  const int s0 = (int)blockIdx.y * sps, s1 = s0 + sps < nsteps ? s0 + sps : nsteps, nl = (s1 - s0) / KG;
+  const int ntiles = (int)gq_tiles(N), kh = lane >> 5, r = lane & 15;
+  uint32_t qo[NJ], so[NJ];  // byte offsets of this lane's codes (slot kh) and scales, chunk 0
+#pragma unroll
+  for (int j = 0; j < NJ; ++j) {
+    int t = (n0 + 32 * (NJ * wn + j) + (lane & 31)) >> 4;
+    if (t >= ntiles) t = ntiles - 1;  // clamped; those columns are never stored
+    const uint32_t tc = (uint32_t)t * (uint32_t)C;
+    qo[j] = tc * (uint32_t)gq_chunk_qs_bytes(FMT) + 16u * (16u * (uint32_t)kh + (uint32_t)r);
+    so[j] = sc_off + tc * (uint32_t)gq_chunk_sc_bytes(FMT) + (FMT == GQ_FMT_Q4_0 || FMT == GQ_FMT_Q8_0 ? 8u : 16u) * r;
+  }
+  gq_f16v acc[TM][NJ];
+#pragma unroll
+  for (int i = 0; i < TM; ++i)
+#pragma unroll
+    for (int j = 0; j < NJ; ++j)
+#pragma unroll
+      for (int v = 0; v < 16; ++v) acc[i][j][v] = 0.f;
+  RStep<FMT, NJ> st[PD];
+  const uint32_t mg = gq_nib_magic();
+  uint32_t ao[NA];
+  a_offsets<BM, NW>(lda, M, m0, wave, lane, ao);
+  const int arow = lane & 31, sw = a_swz(lane & 31);
+  auto gstep = [&](int l) { return s0 + (l < nl ? l : nl - 1) * KG + kg; };
+  auto run_step = [&](int l, auto buf_c) __attribute__((always_inline)) {
+    constexpr int BUF = decltype(buf_c)::value;
+    using NB = std::integral_constant<int, (BUF + PD - 1) % PD>;
+    const int step = s0 + l * KG + kg, sa = gstep(l + PD - 1), sb = gstep(l + PD);
+    load_a_lds_b<BM, NW>(a16, ao, sa, wave, As_of(NB{}));
+    __builtin_amdgcn_sched_barrier(0);
+    const _Float16 *As = As_of(buf_c) + arow * BK;
+    gq_half8 af[2][TM];
+    auto read_a = [&](int ks, int fb) __attribute__((always_inline)) {
+      const int ch = (4 * (ks >> 1) + 2 * kh + (ks & 1)) ^ sw;
+#pragma unroll
+      for (int i = 0; i < TM; ++i) af[fb][i] = *reinterpret_cast<const gq_half8 *>(As + 32 * i * BK + 8 * ch);
+    };
+    read_a(0, 0);
+    QKf qk[NJ][2];
+    gq_half2 q6[NJ][2];
+    if constexpr (FMT == GQ_FMT_Q4_K) q4k_factors<NJ>(st[BUF], step, qk);
+    if constexpr (FMT == GQ_FMT_Q6_K) q6k_factors<NJ>(st[BUF], kh, q6);
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      if (ks + 1 < KS) read_a(ks + 1, (ks + 1) & 1);
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) {
+        const gq_half8 bf = rfrag<FMT, NJ>(st[BUF], j, ks, step, qk[j], q6[j], mg);
+#pragma unroll
+        for (int i = 0; i < TM; ++i) acc[i][j] = gq_mfma32(af[ks & 1][i], bf, acc[i][j]);
+      }
+    }
+    load_rstep<FMT, NJ>(w, qo, so, sb, st[BUF]);
+    step_barrier<pend>();
+  };
+  auto prime = [&](auto b) __attribute__((always_inline)) {
+    constexpr int i = decltype(b)::value;
+    const int s = gstep(i);
+    if constexpr (i < PD - 1) load_a_lds_b<BM, NW>(a16, ao, s, wave, As_of(b));
+    __builtin_amdgcn_sched_barrier(0);  // (pend counts this order)
+    load_rstep<FMT, NJ>(w, qo, so, s, st[i]);
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  const gq_f4 rs4 = *reinterpret_cast<const gq_f4 *>(rs + m0 + 4 * (tid % (BM / 4)));  // (padded past M)
+  prime(B0{});
+  prime(B1{});
+  if constexpr (PD >= 3) prime(B2{});
+  if constexpr (PD >= 4) prime(B3{});
+  if (tid < BM / 4) *reinterpret_cast<gq_f4 *>(rs_s + 4 * tid) = rs4;
+  step_barrier<pend>();
+  for (int l = 0; l < nl; l += PD) {
+    run_step(l, B0{});
+    if (l + 1 < nl) run_step(l + 1, B1{});
+    if constexpr (PD >= 3)
+      if (l + 2 < nl) run_step(l + 2, B2{});
+    if constexpr (PD >= 4)
+      if (l + 3 < nl) run_step(l + 3, B3{});
+  }
+  __builtin_amdgcn_s_waitcnt(0x0F70);  // (loads of no step still on their way to LDS)
+  if constexpr (KG > 1) {
+    __shared__ __attribute__((aligned(16))) gq_f4 xs[(KG - 1) * NW * 4 * 64];
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) {
+        gq_f16v &a = acc[i][j];
+        if (kg > 0) {
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+            xs[(((kg - 1) * NW + wave) * 4 + q) * 64 + lane] = gq_f4{a[4 * q], a[4 * q + 1], a[4 * q + 2], a[4 * q + 3]};
+        }
+        __syncthreads();
+        if (kg == 0) {
+#pragma unroll
+          for (int g = 0; g < KG - 1; ++g)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              const gq_f4 t = xs[((g * NW + wave) * 4 + q) * 64 + lane];
+#pragma unroll
+              for (int u = 0; u < 4; ++u) a[4 * q + u] += t[u];
+            }
+        }
+        __syncthreads();
+      }
+    if (kg > 0) return;
+  }
+  // D layout (32x32): lane l holds column l % 32, rows 8 (v / 4) + 4 (l / 32) + v % 4.  Rows >= M lie
+  // past the resource's end, whose check need not count a scalar offset: all of it is in the lane's
+  // (host: a tile's rows span less than 2 GiB).
+  auto range = [&](uint32_t es) {
+    const size_t left = (size_t)(M - m0) * (size_t)N * es;
+    return (int)(uint32_t)(left < 0xFFFFFFFFu ? left : 0xFFFFFFFFu);
+  };
+  auto row_scales = [&](int i, float (&rsv)[16]) __attribute__((always_inline)) {
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const gq_f4 t = *reinterpret_cast<const gq_f4 *>(rs_s + 32 * i + 4 * (lane >> 5) + 8 * q);
+#pragma unroll
+      for (int u = 0; u < 4; ++u) rsv[4 * q + u] = t[u];
+    }
+  };
+  if (part) {
+    const __amdgpu_buffer_rsrc_t pr = __builtin_amdgcn_make_buffer_rsrc(
+        part + ((size_t)blockIdx.y * (size_t)M + m0) * (size_t)N, (short)0, range(4u), 0x00020000);
+#pragma unroll
+    for (int i = 0; i < TM; ++i) {
+      float rsv[16];
+      row_scales(i, rsv);
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) {
+        const int n = n0 + 32 * (NJ * wn + j) + (lane & 31);
+        if (n >= N) continue;
+#pragma unroll
+        for (int v = 0; v < 16; ++v)
+          front_put<GQ_DT_F32>(pr, ((uint32_t)(32 * i + 4 * (lane >> 5) + 8 * (v >> 2) + (v & 3)) * (uint32_t)N + (uint32_t)n) * 4u,
+                               GQ_DT_F32, acc[i][j][v] * rsv[v]);
+      }
+    }
+    return;
+  }
+  auto store = [&](auto dtc) __attribute__((always_inline)) {
+    constexpr int DT = decltype(dtc)::value;
+    constexpr uint32_t ES = DT == GQ_DT_F32 ? 4u : 2u;
+    auto rsrc = [&](const void *p) {
+      return __builtin_amdgcn_make_buffer_rsrc(
+          const_cast<uint8_t *>(reinterpret_cast<const uint8_t *>(p)) + (p ? (size_t)m0 * N * ES : 0), (short)0,
+          p ? range(ES) : 0, 0x00020000);
+    };
+    const __amdgpu_buffer_rsrc_t yr = rsrc(e.y), zr = rsrc(e.z), rr = rsrc(e.resid);  // (none: no range)
+#pragma unroll
+    for (int i = 0; i < TM; ++i) {
+      float rsv[16];
+      row_scales(i, rsv);
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) {
+        const int n = n0 + 32 * (NJ * wn + j) + (lane & 31);
+        if (n >= N) continue;
+        const float b = e.bias ? gq_ld_dt(e.bias, e.bias_dt, n) : 0.f;
+        const uint32_t vo = ((uint32_t)(32 * i + 4 * (lane >> 5)) * (uint32_t)N + (uint32_t)n) * ES;
+        auto at = [&](int v) { return vo + (uint32_t)(8 * (v >> 2) + (v & 3)) * (uint32_t)N * ES; };
+        float res[16] = {};
+        if (e.resid) {  // (all of it before the first store: resid may be y)
+#pragma unroll
+          for (int v = 0; v < 16; ++v) {
+            if constexpr (DT == GQ_DT_F32) {
+              res[v] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(rr, at(v), 0, 0));
+            } else {
+              const uint16_t t = __builtin_amdgcn_raw_buffer_load_b16(rr, at(v), 0, 0);
+              res[v] = e.dt == GQ_DT_BF16 ? __uint_as_float((uint32_t)t << 16) : (float)__builtin_bit_cast(_Float16, t);
+            }
+          }
+        }
+#pragma unroll
+        for (int v = 0; v < 16; ++v) {
+          const float z = fmaf(acc[i][j][v], rsv[v], b);
+          if (e.z) front_put<DT>(zr, at(v), e.dt, z);
+          front_put<DT>(yr, at(v), e.dt, lin_act(e.act, z) + res[v]);
+        }
+      }
+    }
+  };
+  if (e.dt == GQ_DT_F32) store(std::integral_constant<int, GQ_DT_F32>{});
+  else store(std::integral_constant<int, GQ_DT_BF16>{});
+}
+
+template <int FMT, int BM, int WN, int NJ, int PD, int KG>
+int launch_rb(const void *w, const _Float16 *a16, const float *rs, const LinEpi &e, int M, int N, int K, hipStream_t s) {
+  const int tiles_m = (M + BM - 1) / BM, tiles_n = (N + 32 * NJ * WN - 1) / (32 * NJ * WN);
+  GQ_CHECK((size_t)tiles_m * (size_t)tiles_n <= 0x7FFFFFFFu, GQ_ERR_INVALID_ARGS);  // (one grid dimension)
+  const int nsteps = (int)(gq_kpad(FMT, K) / BK);
+  hipLaunchKernelGGL((k_lin_rb<FMT, BM, WN, NJ, PD, KG>), dim3((unsigned)(tiles_m * tiles_n)), dim3(64 * WN * KG), 0, s,
+                     (const uint8_t *)w, (uint32_t)gq_sc_plane_offset(FMT, N, K), a16, (int)gq_kpad(FMT, K), rs, e, (float *)nullptr,
+                     M, N, (int)gq_chunks(FMT, K), nsteps, nsteps, tiles_m);
+  return gq_last_launch();
+}
+template <int FMT>
+int launch_fmt(const void *w, const _Float16 *a16, const float *rs, const LinEpi &e, int M, int N, int K, hipStream_t s) {
+#define GQ_RB(...) launch_rb<FMT, __VA_ARGS__>(w, a16, rs, e, M, N, K, s)
+  auto wgs = [&](int bm, int bn) { return (size_t)((M + bm - 1) / bm) * (size_t)((N + bn - 1) / bn); };
+  const int nsteps = (int)(gq_kpad(FMT, K) / BK);
+  if (wgs(256, 256) >= 384) return GQ_RB(256, 8, 1, 3, 1);
+  if (wgs(128, 256) >= 192) return GQ_RB(128, 8, 1, 4, 1);
+  if (wgs(128, 128) >= 192 || nsteps % 4) return GQ_RB(128, 4, 1, 4, 2);  // (a step count is even)
+  return GQ_RB(64, 4, 1, 3, 4);
+#undef GQ_RB
+}
+
+}  // namespace
+
+int gq_launch_linear_rb(int fmt, const void *w, const _Float16 *a16, const float *rs, const void *epi, int M, int N, int K,
+                        hipStream_t s) {
+  const LinEpi &e = *reinterpret_cast<const LinEpi *>(epi);
+  if (fmt == GQ_FMT_Q4_0) return launch_fmt<GQ_FMT_Q4_0>(w, a16, rs, e, M, N, K, s);
+  if (fmt == GQ_FMT_Q8_0) return launch_fmt<GQ_FMT_Q8_0>(w, a16, rs, e, M, N, K, s);
+  if (gq_fmt_is_q6k(fmt)) return launch_fmt<GQ_FMT_Q6_K>(w, a16, rs, e, M, N, K, s);
+  return launch_fmt<GQ_FMT_Q4_K>(w, a16, rs, e, M, N, K, s);
+}

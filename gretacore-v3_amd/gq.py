@@ -26,6 +26,7 @@ FORMATS = {"q4_0": FMT_Q4_0, "q8_0": FMT_Q8_0, "q4_k": FMT_Q4_K, "q4_k_ggml": FM
 
 DT_F32, DT_F16, DT_BF16 = 0, 1, 2
 ACT_SILU, ACT_GELU_TANH = 0, 1
+ACT_NONE, ACT_RELU, ACT_GELU = 2, 3, 4  # linear only
 MAX_BATCH = 16
 
 _c_size = ctypes.c_size_t
@@ -90,6 +91,12 @@ _SIGS = {
                                   _vp]),
     "gq_w4_gate_up": (ctypes.c_int, [_vp, _vp, ctypes.c_int, _vp, ctypes.c_int, _vp, ctypes.c_int, _c_size, _c_size,
                                      ctypes.c_int, ctypes.c_int, _vp]),
+    "gq_linear_workspace_bytes": (_c_size, [ctypes.c_int, _c_size, _c_size, _c_size]),
+    "gq_linear": (ctypes.c_int, [ctypes.c_int, _vp, _vp, ctypes.c_int, _vp, ctypes.c_int, ctypes.c_int, _vp, _vp,
+                                 ctypes.c_int, _vp, _c_size, _c_size, _c_size, _vp, _c_size, _vp]),
+    "gq_linear_bwd_workspace_bytes": (_c_size, [ctypes.c_int, _c_size, _c_size, _c_size]),
+    "gq_linear_bwd": (ctypes.c_int, [ctypes.c_int, _vp, _vp, _vp, ctypes.c_int, ctypes.c_int, _vp, _vp, ctypes.c_int, _vp,
+                                     _c_size, _c_size, _c_size, _vp, _c_size, _vp]),
     "gq_launch_gemm_mfma_int8_wt_fp32_acc32": (
         ctypes.c_int, [_vp, _vp, _vp, _vp, _vp] + [ctypes.c_uint32] * 7),
     "gq_launch_gemm_mfma_int4_wt_fp32_acc32": (
@@ -553,12 +560,13 @@ def gemv_swiglu_plan(fmt: int, n: int, k: int, batch: int):
 # one given (inputs of other streams are the caller's to order, as for torch's own).  The checks are few
 # attribute reads (a 4-bit GEMV's kernel runs 4 us); the messages are made only when one fails.
 _dts = {}  # torch dtype -> DT_*
-_empty = _current_device = None
+_empty = _current_device = _f32 = None
 
 
 def _init_torch():
-    global _empty, _current_device
+    global _empty, _current_device, _f32
     import torch
+    _f32 = torch.float32
     _dts.update({torch.float32: DT_F32, torch.float16: DT_F16, torch.bfloat16: DT_BF16})
     _empty, _current_device = torch.empty, torch.cuda.current_device
 
@@ -722,6 +730,90 @@ def ffn_gate_up_bwd(fmt: int, gate, up, dh, g, u, n: int, k: int, act: int = ACT
     if st:
         check(st, "gq_ffn_gate_up_bwd")
     return {"dx": dx, "dg": dg, "du": du}
+
+
+# ---- product with bias, activation and residual ------------------------------------
+@functools.lru_cache(maxsize=512)
+def _linear_bytes(backward, fmt, m, n, k):
+    return (linear_bwd_workspace_bytes if backward else linear_workspace_bytes)(fmt, m, n, k)
+
+
+def linear_workspace_bytes(fmt: int, m: int, n: int, k: int) -> int:
+    return load().gq_linear_workspace_bytes(fmt, m, n, k)
+
+
+def linear(fmt: int, w, x, n: int, k: int, bias=None, act: int = ACT_NONE, resid=None, y=None, z=None, save: bool = False,
+           out_dtype=None, workspace: Workspace | None = None, stream=None):
+    """y = act(x W^T + bias) + resid over a T16 tensor, any number of rows of x [m][k] (f32/f16/bf16).  y is of out_dtype
+    (default: x's) or the tensor given (resid itself, to add in place); bias [n] of any of the three dtypes, resid [m][n] of
+    y's.  With save (or z given) the sums before the activation come back too: (y, z)."""
+    if stream is not None:
+        return _on(stream, linear, fmt, w, x, n, k, bias, act, resid, y, z, save, out_dtype, workspace)
+    m, device = _rows(x, k, "x")
+    dtype = y.dtype if y is not None else out_dtype or x.dtype
+    _packed_operand(w, _packed_bytes(fmt, n, k), "w", device)
+    bias_dt = 0
+    if bias is not None:
+        _operand(bias, (n,), "bias", device)
+        bias_dt = _dt(bias.dtype)
+    if resid is not None:
+        _operand(resid, (m, n), "resid", device, dtype)
+    if y is None:
+        y = _empty((m, n), dtype=dtype, device=x.device)
+    else:
+        _operand(y, (m, n), "y", device)
+    if z is not None:
+        _operand(z, (m, n), "z", device, dtype)
+    elif save:
+        z = _empty((m, n), dtype=dtype, device=x.device)
+    ws_ptr, ws_n = None, 0
+    if workspace is not None:
+        ws_ptr, ws_n = _room(workspace, _linear_bytes(False, fmt, m, n, k), device)
+    st = load().gq_linear(fmt, w.data_ptr(), x.data_ptr(), _dt(x.dtype), _ptr(bias), bias_dt, act, _ptr(resid), y.data_ptr(),
+                          _dt(dtype), _ptr(z), m, n, k, ws_ptr, ws_n, _stream())
+    if st:
+        check(st, "gq_linear")
+    return y if z is None else (y, z)
+
+
+def linear_bwd_workspace_bytes(fmt: int, m: int, n: int, k: int) -> int:
+    return load().gq_linear_bwd_workspace_bytes(fmt, m, n, k)
+
+
+def linear_bwd(fmt: int, w, dy, z, n: int, k: int, act: int = ACT_NONE, want_dx: bool = True, want_dz: bool = True,
+               want_dbias: bool = False, dx=None, dz=None, dbias=None, dx_dtype=None, workspace: Workspace | None = None,
+               stream=None):
+    """Gradients of linear with the weights frozen: {"dx", "dz", "dbias"} for dy [m][n] and the z it saved (None with
+    ACT_NONE), None where not wanted.  dbias is float32; the residual's gradient is dy itself."""
+    if stream is not None:
+        return _on(stream, linear_bwd, fmt, w, dy, z, n, k, act, want_dx, want_dz, want_dbias, dx, dz, dbias, dx_dtype,
+                   workspace)
+    m, device = _rows(dy, n, "dy")
+    dtype = dy.dtype
+    if z is not None:
+        _operand(z, dy.shape, "z", device, dtype)
+    _packed_operand(w, _packed_bytes(fmt, n, k), "w", device)
+    if dx is not None:
+        _operand(dx, (m, k), "dx", device)
+    elif want_dx:
+        dx = _empty((m, k), dtype=dx_dtype or dtype, device=dy.device)
+    if dz is not None:
+        _operand(dz, (m, n), "dz", device, dtype)
+    elif want_dz:
+        dz = _empty((m, n), dtype=dtype, device=dy.device)
+    if dbias is not None or want_dbias:
+        if dbias is None:
+            dbias = _empty((n,), dtype=_f32, device=dy.device)
+        else:
+            _operand(dbias, (n,), "dbias", device, _f32)
+    ws_ptr, ws_n = None, 0
+    if workspace is not None:
+        ws_ptr, ws_n = _room(workspace, _linear_bytes(True, fmt, m, n, k), device)
+    st = load().gq_linear_bwd(fmt, w.data_ptr(), dy.data_ptr(), _ptr(z), _dt(dtype), act, _ptr(dz), _ptr(dx),
+                              _dt(dx.dtype if dx is not None else dtype), _ptr(dbias), m, n, k, ws_ptr, ws_n, _stream())
+    if st:
+        check(st, "gq_linear_bwd")
+    return {"dx": dx, "dz": dz, "dbias": dbias}
 
 
 def w4_packed_size(n: int, k: int, group: int) -> int:

@@ -321,6 +321,40 @@ int gq_w4_gemv(const void *d_packed, int group, const void *d_x, int x_dtype, vo
 int gq_w4_gate_up(const void *d_gate, const void *d_up, int group, const void *d_x, int x_dtype, void *d_h, int h_dtype,
                   size_t N, size_t K, int batch, int act, void *stream);
 
+/* ---- product with bias, activation and residual, any number of rows -------------------
+ * z[m][n] = sum_k x[m][k] W[n][k] + bias[n], y = act(z) + resid: gq_matmul's product with what
+ * follows it in a block (the biases of q/k/v, an ungated feed-forward block's first product, the output
+ * and down projections added to the hidden state).  x is [M][K] of x_dtype; y, resid and
+ * z [M][N] of y_dtype, bias [N] of bias_dtype, all contiguous; W a T16 tensor (it and the
+ * workspace 16-byte aligned).  bias and resid may be NULL (none), d_z NULL (not
+ * wanted; gq_linear_bwd takes it).  resid may be y itself; y and z overlap nothing else.
+ * Sums are fp32, bias, activation and residual are applied to them in fp32, and
+ * y and z are rounded once.  x and the weights enter the matrix cores as in gq_ffn_gate_up: one to four rows
+ * of 16-bit x as they are (of bf16 rows the finite values stay below 2^115), all others rounded to fp16
+ * after a power-of-two scale per row; up to 64 rows keep the k-quants' d (and dmin) in fp32, more
+ * fold them into fp16 weights. */
+#define GQ_ACT_NONE 2 /* z */
+#define GQ_ACT_RELU 3 /* max(z, 0) */
+#define GQ_ACT_GELU 4 /* z Phi(z), Phi the normal distribution; beside these GQ_ACT_SILU and GQ_ACT_GELU_TANH */
+/* A workspace of NULL takes scratch memory of the call's own, as in gq_ffn_gate_up; calls that need none (up to
+ * four 4-byte aligned rows of 16-bit x) run without under capture too.  The bytes for M rows are enough for every call of
+ * fewer.  N * 256 outputs stay below 2^31 bytes; K == 0 is refused. */
+size_t gq_linear_workspace_bytes(int fmt, size_t M, size_t N, size_t K);
+int gq_linear(int fmt, const void *d_packed, const void *d_x, int x_dtype, const void *d_bias, int bias_dtype, int act,
+              const void *d_resid, void *d_y, int y_dtype, void *d_z, size_t M, size_t N, size_t K, void *d_workspace,
+              size_t workspace_bytes, void *stream);
+/* Its backward pass with the weights frozen:
+ *   dz = dy * act'(z), dbias[n] = sum_m dz[m][n], dx = dz W  (resid's gradient is dy).
+ * dy, z and dz are [M][N] of `dtype`, dx [M][K] of dx_dtype, dbias [N] fp32.  dz, dx and
+ * dbias may each be NULL: not wanted; z may be with GQ_ACT_NONE.  dx and dbias are computed from dz as it
+ * is before its rounding; dx rounds it to fp16 with a power-of-two scale per row, and the weights as
+ * gq_ffn_gate_up_bwd does.  dbias is summed in one order whatever the device does.  dz may be the same buffer as
+ * dy or z; no other overlap. */
+size_t gq_linear_bwd_workspace_bytes(int fmt, size_t M, size_t N, size_t K);
+int gq_linear_bwd(int fmt, const void *d_packed, const void *d_dy, const void *d_z, int dtype, int act, void *d_dz,
+                  void *d_dx, int dx_dtype, float *d_dbias, size_t M, size_t N, size_t K, void *d_workspace,
+                  size_t workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif
