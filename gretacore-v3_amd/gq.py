@@ -27,6 +27,8 @@ FORMATS = {"q4_0": FMT_Q4_0, "q8_0": FMT_Q8_0, "q4_k": FMT_Q4_K, "q4_k_ggml": FM
 DT_F32, DT_F16, DT_BF16 = 0, 1, 2
 ACT_SILU, ACT_GELU_TANH = 0, 1
 ACT_NONE, ACT_RELU, ACT_GELU = 2, 3, 4  # linear only
+SCORE_SOFTMAX, SCORE_SIGMOID = 0, 1
+MOE_MAX_TOKENS, MOE_MAX_EXPERTS, MOE_MAX_TOP = 64, 1024, 16
 MAX_BATCH = 16
 
 _c_size = ctypes.c_size_t
@@ -97,6 +99,11 @@ _SIGS = {
     "gq_linear_bwd_workspace_bytes": (_c_size, [ctypes.c_int, _c_size, _c_size, _c_size]),
     "gq_linear_bwd": (ctypes.c_int, [ctypes.c_int, _vp, _vp, _vp, ctypes.c_int, ctypes.c_int, _vp, _vp, ctypes.c_int, _vp,
                                      _c_size, _c_size, _c_size, _vp, _c_size, _vp]),
+    "gq_moe_route_workspace_bytes": (_c_size, [_vp, _c_size]),
+    "gq_moe_route": (ctypes.c_int, [_vp, _vp, ctypes.c_int, _vp, _vp, _c_size, _vp, _c_size, _vp]),
+    "gq_moe_workspace_bytes": (_c_size, [_vp, _c_size]),
+    "gq_moe_ffn": (ctypes.c_int, [_vp, _vp, ctypes.c_int, _vp, _vp, _vp, _vp, ctypes.c_int, _c_size, _vp, _c_size, _vp]),
+    "gq_moe_layer": (ctypes.c_int, [_vp, _vp, ctypes.c_int, _vp, _vp, ctypes.c_int, _vp, _vp, _c_size, _vp, _c_size, _vp]),
     "gq_launch_gemm_mfma_int8_wt_fp32_acc32": (
         ctypes.c_int, [_vp, _vp, _vp, _vp, _vp] + [ctypes.c_uint32] * 7),
     "gq_launch_gemm_mfma_int4_wt_fp32_acc32": (
@@ -132,6 +139,14 @@ _SIGS_GGUF = {
     "gq_greta_load": (ctypes.c_int, [_vp, ctypes.c_char_p, _vp, _c_size, _vp, _c_size, _vp, _c_size]),
 }
 _SIGS.update(_SIGS_GGUF)
+
+
+class MoeLayer(ctypes.Structure):
+    """gq_moe (include/gq.h)."""
+    _fields_ = [("fmt", ctypes.c_int), ("fmt_down", ctypes.c_int), ("act", ctypes.c_int), ("top_k", ctypes.c_int),
+                ("gate", _vp), ("up", _vp), ("down", _vp), ("n_experts", _c_size), ("N", _c_size), ("K", _c_size),
+                ("router", _vp), ("router_bias", _vp), ("router_dtype", ctypes.c_int), ("score", ctypes.c_int),
+                ("renorm", ctypes.c_int), ("scale", ctypes.c_float)]
 
 
 class ChainOp(ctypes.Structure):
@@ -814,6 +829,126 @@ def linear_bwd(fmt: int, w, dy, z, n: int, k: int, act: int = ACT_NONE, want_dx:
     if st:
         check(st, "gq_linear_bwd")
     return {"dx": dx, "dz": dz, "dbias": dbias}
+
+
+# ---- mixture-of-experts layer of a few tokens -----------------------------------------
+@functools.lru_cache(maxsize=512)
+def _moe_bytes(fmt, fmt_down, m, n, k, n_experts, top_k):
+    return moe_workspace_bytes(fmt, fmt_down, m, n, k, n_experts, top_k)
+
+
+def moe_workspace_bytes(fmt: int, fmt_down: int, m: int, n: int, k: int, n_experts: int, top_k: int) -> int:
+    """Workspace bytes of moe_ffn and moe_layer of up to m tokens."""
+    layer = MoeLayer(fmt, fmt_down, ACT_SILU, top_k, None, None, None, n_experts, n, k)
+    return load().gq_moe_workspace_bytes(ctypes.addressof(layer), m)
+
+
+def _router_operands(router, router_bias, n_experts, k, device):
+    _operand(router, (n_experts, k), "router", device)
+    if router_bias is not None:
+        _operand(router_bias, (n_experts,), "router_bias", device, _f32)
+
+
+def _expert_operands(fmt, gate, up, fmt_down, down, n, k, n_experts, device):
+    nbytes = _packed_bytes(fmt, n_experts * n, k)
+    _packed_operand(gate, nbytes, "gate", device)
+    _packed_operand(up, nbytes, "up", device)
+    _packed_operand(down, _packed_bytes(fmt_down, n_experts * k, n), "down", device)
+
+
+def _choice(ids, weights, m, top_k, x, device):
+    import torch
+    if ids is None:
+        ids = _empty((m, top_k), dtype=torch.int32, device=x.device)
+    else:
+        _operand(ids, (m, top_k), "ids", device, torch.int32)
+    if weights is None:
+        weights = _empty((m, top_k), dtype=_f32, device=x.device)
+    else:
+        _operand(weights, (m, top_k), "weights", device, _f32)
+    return ids, weights
+
+
+def moe_route(router, x, k: int, n_experts: int, top_k: int, score: int = SCORE_SOFTMAX, renorm: bool = True,
+              scale: float = 1.0, router_bias=None, ids=None, weights=None, workspace: Workspace | None = None, stream=None):
+    """The experts of 1..64 tokens x [m][k]: (ids int32, weights float32), [m][top_k] each, for a router [n_experts][k] of any
+    activation dtype.  router_bias (float32) is added to the scores for the choice alone."""
+    if stream is not None:
+        return _on(stream, moe_route, router, x, k, n_experts, top_k, score, renorm, scale, router_bias, ids, weights, workspace)
+    m, device = _rows(x, k, "x")
+    _router_operands(router, router_bias, n_experts, k, device)
+    ids, weights = _choice(ids, weights, m, top_k, x, device)
+    layer = MoeLayer(0, 0, 0, top_k, None, None, None, n_experts, 0, k, router.data_ptr(), _ptr(router_bias), _dt(router.dtype),
+                     score, renorm, scale)
+    ws_ptr, ws_n = None, 0
+    if workspace is not None:
+        ws_ptr, ws_n = _room(workspace, load().gq_moe_route_workspace_bytes(ctypes.addressof(layer), m), device)
+    st = load().gq_moe_route(ctypes.addressof(layer), x.data_ptr(), _dt(x.dtype), ids.data_ptr(), weights.data_ptr(), m, ws_ptr,
+                             ws_n, _stream())
+    if st:
+        check(st, "gq_moe_route")
+    return ids, weights
+
+
+def moe_ffn(fmt: int, gate, up, fmt_down: int, down, x, ids, weights, n: int, k: int, n_experts: int, act: int = ACT_SILU,
+            resid=None, y=None, out_dtype=None, workspace: Workspace | None = None, stream=None):
+    """y = resid + the weighted sum of the experts ids [m][top_k] (int32; others than 0..n_experts - 1: none) with weights
+    [m][top_k] (float32) over T16 expert tensors: gate and up [n_experts * n][k] of fmt, down [n_experts * k][n] of fmt_down.
+    1..64 tokens x [m][k]; y of out_dtype (default: x's) or the tensor given (resid itself, to add in place)."""
+    if stream is not None:
+        return _on(stream, moe_ffn, fmt, gate, up, fmt_down, down, x, ids, weights, n, k, n_experts, act, resid, y, out_dtype,
+                   workspace)
+    m, device = _rows(x, k, "x")
+    if ids.dim() != 2:
+        raise GQError("ids: [m][top_k] expected")
+    top_k = ids.shape[1]
+    ids, weights = _choice(ids, weights, m, top_k, x, device)
+    return _moe_call(False, fmt, gate, up, fmt_down, down, None, x, n, k, n_experts, top_k, act, 0, False, 1.0, None, resid, y, ids,
+                     weights, out_dtype, workspace, m, device)
+
+
+def moe_layer(fmt: int, gate, up, fmt_down: int, down, router, x, n: int, k: int, n_experts: int, top_k: int,
+              act: int = ACT_SILU, score: int = SCORE_SOFTMAX, renorm: bool = True, scale: float = 1.0, router_bias=None,
+              resid=None, y=None, ids=None, weights=None, save: bool = False, out_dtype=None,
+              workspace: Workspace | None = None, stream=None):
+    """moe_route and moe_ffn in one call.  With save (or ids, weights given) the choice comes back too: (y, ids, weights)."""
+    if stream is not None:
+        return _on(stream, moe_layer, fmt, gate, up, fmt_down, down, router, x, n, k, n_experts, top_k, act, score, renorm, scale,
+                   router_bias, resid, y, ids, weights, save, out_dtype, workspace)
+    m, device = _rows(x, k, "x")
+    _router_operands(router, router_bias, n_experts, k, device)
+    if save or ids is not None or weights is not None:
+        ids, weights = _choice(ids, weights, m, top_k, x, device)
+    y = _moe_call(True, fmt, gate, up, fmt_down, down, router, x, n, k, n_experts, top_k, act, score, renorm, scale, router_bias,
+                  resid, y, ids, weights, out_dtype, workspace, m, device)
+    return y if ids is None else (y, ids, weights)
+
+
+def _moe_call(route, fmt, gate, up, fmt_down, down, router, x, n, k, n_experts, top_k, act, score, renorm, scale, router_bias, resid,
+              y, ids, weights, out_dtype, workspace, m, device):
+    _expert_operands(fmt, gate, up, fmt_down, down, n, k, n_experts, device)
+    dtype = y.dtype if y is not None else out_dtype or x.dtype
+    if resid is not None:
+        _operand(resid, (m, k), "resid", device, dtype)
+    if y is None:
+        y = _empty((m, k), dtype=dtype, device=x.device)
+    else:
+        _operand(y, (m, k), "y", device)
+    layer = MoeLayer(fmt, fmt_down, act, top_k, gate.data_ptr(), up.data_ptr(), down.data_ptr(), n_experts, n, k, _ptr(router),
+                     _ptr(router_bias), _dt(router.dtype) if router is not None else 0, score, renorm, scale)
+    ws_ptr, ws_n = None, 0
+    if workspace is not None:
+        ws_ptr, ws_n = _room(workspace, _moe_bytes(fmt, fmt_down, m, n, k, n_experts, top_k), device)
+    at = ctypes.addressof(layer)
+    if route:
+        st = load().gq_moe_layer(at, x.data_ptr(), _dt(x.dtype), _ptr(resid), y.data_ptr(), _dt(dtype), _ptr(ids), _ptr(weights),
+                                 m, ws_ptr, ws_n, _stream())
+    else:
+        st = load().gq_moe_ffn(at, x.data_ptr(), _dt(x.dtype), ids.data_ptr(), weights.data_ptr(), _ptr(resid), y.data_ptr(),
+                               _dt(dtype), m, ws_ptr, ws_n, _stream())
+    if st:
+        check(st, "gq_moe_layer" if route else "gq_moe_ffn")
+    return y
 
 
 def w4_packed_size(n: int, k: int, group: int) -> int:

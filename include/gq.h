@@ -355,6 +355,49 @@ int gq_linear_bwd(int fmt, const void *d_packed, const void *d_dy, const void *d
                   void *d_dx, int dx_dtype, float *d_dbias, size_t M, size_t N, size_t K, void *d_workspace,
                   size_t workspace_bytes, void *stream);
 
+/* ---- mixture-of-experts layer of a few tokens ------------------------------------------
+ * y_m = resid_m + sum over the experts e that token m takes of w_me W_down,e h, h = act(W_gate,e x_m) * (W_up,e x_m): the
+ * sparse counterpart of gq_ffn_gate_up and the down projection.  An expert tensor is one T16 tensor of the experts'
+ * rows one behind the other, gate and up [n_experts * N][K], down [n_experts * K][N]: what gq_repack and the loader make of a
+ * GGUF file's three-dimensional ffn_*_exps tensors.  The struct is read during the call alone. */
+#define GQ_MOE_MAX_TOKENS 64
+#define GQ_MOE_MAX_EXPERTS 1024
+#define GQ_MOE_MAX_TOP 16
+#define GQ_MOE_SOFTMAX 0 /* scores s = softmax over all experts of the logits */
+#define GQ_MOE_SIGMOID 1 /* s = 1 / (1 + e^-logit) */
+typedef struct gq_moe {
+  int fmt, fmt_down;             /* of gate and up, and of down */
+  int act, top_k;                /* GQ_ACT_SILU or GQ_ACT_GELU_TANH; experts a token takes, 1 .. 16 */
+  const void *gate, *up, *down;  /* 16-byte aligned */
+  size_t n_experts, N, K;        /* N: feed-forward size of an expert */
+  const void *router;            /* [n_experts][K], row-major, of router_dtype */
+  const float *router_bias;      /* [n_experts], added to the scores for the choice alone; NULL: none */
+  int router_dtype, score;
+  int renorm;                    /* not 0: the weights of a token's experts are divided by their sum */
+  float scale;                   /* and multiplied by this */
+} gq_moe;
+/* The router: token m takes the top_k experts of the largest logits (with a bias: of s + bias), of equal ones the lower
+ * number, in that order: ids [M][top_k], weights [M][top_k] = s (renormalised, scaled).  Logits and scores are
+ * computed in 64 bits.  An expert whose logit (with a bias: s + bias) is -Inf is never taken: where fewer than top_k are left, the last
+ * slots are expert -1 with weight 0.  A NaN counts as the largest.  1 <= M <= 64. */
+size_t gq_moe_route_workspace_bytes(const gq_moe *layer, size_t M);
+int gq_moe_route(const gq_moe *layer, const void *d_x, int x_dtype, int32_t *d_ids, float *d_weights, size_t M,
+                 void *d_workspace, size_t workspace_bytes, void *stream);
+/* The experts' products for a given choice (the router is not read): ids outside 0 .. n_experts - 1 name no expert (one
+ * that another device holds, an empty slot), an expert named twice counts with both weights.  x is [M][K] of
+ * x_dtype, y and resid (NULL: none; it may be y) [M][K] of y_dtype, all contiguous.  Sums, h and the weighted sum are
+ * fp32, y is rounded once; x and h enter the matrix cores in fp16 after a power-of-two scale per row (one to
+ * four tokens: x as it is, h with a scale per row and 128 values), weights as in gq_ffn_gate_up's kernels of few rows. */
+int gq_moe_ffn(const gq_moe *layer, const void *d_x, int x_dtype, const int32_t *d_ids, const float *d_weights,
+               const void *d_resid, void *d_y, int y_dtype, size_t M, void *d_workspace, size_t workspace_bytes,
+               void *stream);
+/* Both; ids and weights may be NULL (not wanted).  A workspace of NULL takes scratch memory of the call's own (not under capture,
+ * and up to 128 MiB), else gq_moe_workspace_bytes serve gq_moe_ffn and gq_moe_layer of up to M tokens.  Calls that overlap must not
+ * share a workspace, and neither may two captured graphs whose replays overlap. */
+size_t gq_moe_workspace_bytes(const gq_moe *layer, size_t M);
+int gq_moe_layer(const gq_moe *layer, const void *d_x, int x_dtype, const void *d_resid, void *d_y, int y_dtype, int32_t *d_ids,
+                 float *d_weights, size_t M, void *d_workspace, size_t workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif
