@@ -292,16 +292,25 @@ __global__ void __launch_bounds__(kDzThreads) k_lin_dz(const void *dy, const voi
       if (n < N) pr[n] = sum[i][e];
     }
 }
-// dbias = the workgroups' sums, in their order (none: zeros)
-__global__ void __launch_bounds__(256) k_lin_dbias(const float *__restrict__ part, float *__restrict__ db, int N, int parts) {
-  const int n = (int)blockIdx.x * 256 + (int)threadIdx.x;
-  if (n >= N) return;
+// dbias = the workgroups' sums, in an order of their own (none: zeros): 64 columns a workgroup, wave w adds parts w, w + 16, ...
+constexpr int kDbWaves = 16;
+__global__ void __launch_bounds__(64 * kDbWaves) k_lin_dbias(const float *__restrict__ part, float *__restrict__ db, int N, int parts) {
+  __shared__ double red[kDbWaves][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = 64 * (int)blockIdx.x + lane;
   double v = 0.0;
-  for (int p = 0; p < parts; ++p) v += (double)part[(size_t)p * (size_t)N + n];
+  if (n < N) {
+#pragma unroll 8
+    for (int p = wave; p < parts; p += kDbWaves) v += (double)part[(size_t)p * (size_t)N + n];
+  }
+  red[wave][lane] = v;
+  __syncthreads();
+  if (wave > 0 || n >= N) return;
+#pragma unroll
+  for (int w = 1; w < kDbWaves; ++w) v += red[w][lane];
   db[n] = (float)v;
 }
 int launch_dbias(const float *part, float *db, size_t N, int parts, hipStream_t s) {
-  hipLaunchKernelGGL(k_lin_dbias, dim3((unsigned)((N + 255) / 256)), dim3(256), 0, s, part, db, (int)N, parts);
+  hipLaunchKernelGGL(k_lin_dbias, dim3((unsigned)((N + 63) / 64)), dim3(64 * kDbWaves), 0, s, part, db, (int)N, parts);
   return gq_last_launch();
 }
 template <int DT>

@@ -17,49 +17,54 @@ namespace {
 
 constexpr int kMoeFew = 4;  // tokens that the kernels of few rows take
 
-// A block of an expert's work: up to 16 of its pairs (token * top + slot); few tokens (M <= 4): pair[m] is token m's, -1 none
+// A block of an expert's work: up to 16 of its pairs (token * top + slot); few tokens (M <= 4): pair[m] is token m's, -1 none,
+// and w[m] its weight.  expert -1: no block.
 struct MoeBlk {
   int expert, count;
   int pair[16];
+  float w[kMoeFew];
 };
 struct MoePlan {
   int *nblk;
-  MoeBlk *blk;
-  float *wsum;  // [pair] the weight (of the first pair of an expert that a token names twice: their sum)
+  MoeBlk *blk;  // [maxblk], the blocks that there are first
+  float *wsum;  // [pair] the weight (of the first pair of an expert that a token names twice: their sum); not for few tokens
+  int maxblk;
 };
 
 // ---- router --------------------------------------------------------------------------
-// Workgroup (e, b): logits of expert e for tokens 4 b .. 4 b + 3.  Products of two fp32 values are exact in 64 bits.
-constexpr int kLogThreads = 256, kLogTok = 4;
-template <int XT, int RT>
+// Workgroup (e, b): logits of expert e for tokens TOK b .. TOK b + TOK - 1.  Products of two fp32 values are exact in 64 bits.
+constexpr int kLogThreads = 256;
+template <int XT, int RT, int TOK>
 __global__ void __launch_bounds__(kLogThreads) k_moe_logits(const void *__restrict__ x, const void *__restrict__ wr,
                                                             double *__restrict__ logits, int M, int E, int K) {
-  __shared__ double red[kLogThreads / 64][kLogTok];
-  const int tid = threadIdx.x, e = blockIdx.x, m0 = kLogTok * (int)blockIdx.y;
-  double acc[kLogTok] = {};
-  for (int k = 8 * tid; k < K; k += 8 * kLogThreads) {  // (K is whole 32-blocks)
+  __shared__ double red[kLogThreads / 64][TOK];
+  const int tid = threadIdx.x, e = blockIdx.x, m0 = TOK * (int)blockIdx.y;
+  double acc[TOK] = {};
+#pragma unroll 2
+  for (int k = 8 * tid; k < K; k += 8 * kLogThreads) {  // (K is whole 8s)
     FRaw<RT> wv;
-    FRaw<XT> xv[kLogTok];
+    FRaw<XT> xv[TOK];
     px_load<RT>(wr, (size_t)e * K + k, wv);
 #pragma unroll
-    for (int t = 0; t < kLogTok; ++t) px_load<XT>(x, (size_t)(m0 + t < M ? m0 + t : M - 1) * K + k, xv[t]);
+    for (int t = 0; t < TOK; ++t) px_load<XT>(x, (size_t)(m0 + t < M ? m0 + t : M - 1) * K + k, xv[t]);
     float wf[8], xf[8];
     px_floats<RT>(wv, true, wf);
 #pragma unroll
-    for (int t = 0; t < kLogTok; ++t) {
+    for (int t = 0; t < TOK; ++t) {
       px_floats<XT>(xv[t], true, xf);
 #pragma unroll
       for (int i = 0; i < 8; ++i) acc[t] = fma((double)wf[i], (double)xf[i], acc[t]);
     }
   }
 #pragma unroll
-  for (int t = 0; t < kLogTok; ++t) {
+  for (int o = 32; o > 0; o >>= 1)
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) acc[t] += __shfl_xor(acc[t], o, 64);
-    if ((tid & 63) == 0) red[tid >> 6][t] = acc[t];
-  }
+    for (int t = 0; t < TOK; ++t) acc[t] += __shfl_xor(acc[t], o, 64);
+  if ((tid & 63) == 0)
+#pragma unroll
+    for (int t = 0; t < TOK; ++t) red[tid >> 6][t] = acc[t];
   __syncthreads();
-  if (tid < kLogTok && m0 + tid < M) {
+  if (tid < TOK && m0 + tid < M) {
     double v = 0.0;
 #pragma unroll
     for (int w = 0; w < kLogThreads / 64; ++w) v += red[w][tid];
@@ -75,122 +80,147 @@ struct RouteArgs {
   int score, renorm;
   float scale;
 };
-// One wave chooses the experts of token m; lane 0 writes them.  Keys are compared as (value, lower index first), a NaN above
-// all; -Inf is never taken: its slots get expert -1 and weight 0.
+// The largest of a wave's values, in all lanes
+GQ_DEV uint32_t wave_max(uint32_t v) {
+#define GQ_DPP_MAX(CTRL, ROWS) v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xF, false))
+  GQ_DPP_MAX(0x111, 0xF);  // row_shr 1, 2, 4, 8: lane 15 of each row has its largest
+  GQ_DPP_MAX(0x112, 0xF);
+  GQ_DPP_MAX(0x114, 0xF);
+  GQ_DPP_MAX(0x118, 0xF);
+  GQ_DPP_MAX(0x142, 0xA);  // row_bcast 15, 31: lane 63 the wave's
+  GQ_DPP_MAX(0x143, 0xC);
+#undef GQ_DPP_MAX
+  return (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
+}
+GQ_DEV double lane_d(double v, int lane) {  // (lane: the same in all lanes)
+  const uint64_t b = __builtin_bit_cast(uint64_t, v);
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)b, lane);
+  const uint32_t hi = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(b >> 32), lane);
+  return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+// One wave chooses the experts of token m; lane j writes slot j.  A key is a 64-bit number in the values' order, 0 what is
+// never taken (-Inf, none there, taken before): the largest's high word, then its low word, then the lowest
+// expert that has both.
+template <int NE>
 GQ_DEV void moe_choose(const RouteArgs &a, int m, int E, int top, int lane, int *ids_s, float *w_s) {
-  constexpr int NE = GQ_MOE_MAX_EXPERTS / 64;
   const double ninf = -__builtin_inf();
-  double l[NE], lmax = ninf;
-  const int ne = (E + 63) / 64;
+  const bool sm = a.score == GQ_MOE_SOFTMAX;
+  double l[NE], lmax = ninf, sum = 0.0;
 #pragma unroll
   for (int i = 0; i < NE; ++i) {
     const int e = 64 * i + lane;
-    l[i] = i < ne && e < E ? a.logits[(size_t)m * E + e] : ninf;
-    lmax = fmax(lmax, l[i]);  // (not of NaNs: such a row's sum is one)
+    l[i] = e < E ? a.logits[(size_t)m * E + e] : ninf;
+    lmax = fmax(lmax, l[i]);  // (of those that are numbers)
   }
-  double sum = 0.0;
-  const bool sm = a.score == GQ_MOE_SOFTMAX;
   if (sm) {
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) lmax = fmax(lmax, __shfl_xor(lmax, o, 64));
+    if (!a.renorm || a.bias) {  // (renormalised weights do without the sum over all experts)
 #pragma unroll
-    for (int i = 0; i < NE; ++i)
-      if (i < ne) sum += 64 * i + lane < E && l[i] != ninf ? exp(l[i] - lmax) : 0.0;
+      for (int i = 0; i < NE; ++i) sum += l[i] == ninf ? 0.0 : exp(l[i] - lmax);
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
+      for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
+    } else {
+      sum = 1.0;
+    }
   }
   auto score = [&](double v) { return sm ? (v == ninf ? 0.0 : exp(v - lmax) / sum) : 1.0 / (1.0 + exp(-v)); };
-  uint32_t taken = 0;
-  double key[NE];
+  uint32_t kh[NE], kl[NE];
 #pragma unroll
   for (int i = 0; i < NE; ++i) {
     const int e = 64 * i + lane;
-    key[i] = l[i];
-    if (i < ne && e < E && a.bias) key[i] = score(l[i]) + (double)a.bias[e];
-    if (key[i] != key[i]) key[i] = __builtin_inf();
+    double key = l[i];
+    if (a.bias && e < E) key = score(l[i]) + (double)a.bias[e];
+    if (key != key) key = __builtin_inf();
+    const uint64_t b = __builtin_bit_cast(uint64_t, key);
+    const uint64_t o = e >= E || key == ninf ? 0 : b >> 63 ? ~b : b | (uint64_t)1 << 63;
+    kh[i] = (uint32_t)(o >> 32);
+    kl[i] = (uint32_t)o;
   }
-  double total = 0.0, mine = 0.0;  // lane j: the score of slot j
+  double mine = ninf;  // lane j: the logit of slot j
   int id = -1;
   for (int j = 0; j < top; ++j) {
-    double bk = ninf, bl = 0.0;
-    int be = 0x7FFFFFFF;
+    uint32_t h = 0, w = 0;
 #pragma unroll
-    for (int i = 0; i < NE; ++i)
-      if (i < ne && !(taken >> i & 1) && key[i] > bk) {
-        bk = key[i];
-        bl = l[i];
-        be = 64 * i + lane;
-      }
+    for (int i = 0; i < NE; ++i) h = max(h, kh[i]);
+    const uint32_t mh = wave_max(h);
+    if (mh == 0) break;
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) {
-      const double ok = __shfl_xor(bk, o, 64), ol = __shfl_xor(bl, o, 64);
-      const int oe = __shfl_xor(be, o, 64);
-      if (ok > bk || (ok == bk && oe < be)) {
-        bk = ok;
-        bl = ol;
-        be = oe;
+    for (int i = 0; i < NE; ++i) w = max(w, kh[i] == mh ? kl[i] : 0u);
+    const uint32_t mw = wave_max(w);
+    bool found = false;
+#pragma unroll
+    for (int i = 0; i < NE; ++i) {
+      const uint64_t at = found ? 0 : __ballot(kh[i] == mh && kl[i] == mw);
+      if (at == 0) continue;
+      found = true;
+      const int ln = __builtin_ctzll(at);
+      const double v = lane_d(l[i], ln);
+      if (lane == ln) kh[i] = kl[i] = 0;
+      if (lane == j) {
+        id = 64 * i + ln;
+        mine = v;
       }
-    }
-    if (be == 0x7FFFFFFF) break;  // (the same in all lanes)
-    if ((be & 63) == lane) taken |= 1u << (be >> 6);
-    const double s = score(bl);
-    total += s;
-    if (lane == j) {
-      id = be;
-      mine = s;
     }
   }
+  double w = id < 0 ? 0.0 : score(mine), total = 0.0;
+  if (a.renorm) {
+    for (int j = 0; j < top; ++j) total += lane_d(w, j);
+    w = total == 0.0 ? 0.0 : w / total;
+  }
   if (lane < top) {
-    double w = id < 0 ? 0.0 : mine;
-    if (id >= 0 && a.renorm) w = total == 0.0 ? 0.0 : w / total;
-    const float f = (float)(w * (double)a.scale);
+    const float f = id < 0 ? 0.f : (float)(w * (double)a.scale);
     ids_s[m * top + lane] = id;
-    w_s[m * top + lane] = id < 0 ? 0.f : f;
+    w_s[m * top + lane] = f;
     if (a.ids) a.ids[m * top + lane] = id;
-    if (a.weights) a.weights[m * top + lane] = id < 0 ? 0.f : f;
+    if (a.weights) a.weights[m * top + lane] = f;
   }
 }
 
 // ---- plan: one workgroup ------------------------------------------------------------
-// The choice (ROUTE) or the given ids, each expert's pairs in order of their tokens, in blocks.  Ids outside 0 .. E - 1 name no
-// expert; an expert that a token names twice gets one pair with both weights.
+// The choice (NE: experts a lane; 0: ids and weights are given), each expert's pairs in order of their tokens, in blocks of `per`.
+// Ids outside 0 .. E - 1 name no expert; an expert that a token names twice gets one pair with both weights.
 constexpr int kPlanThreads = 1024;
-template <bool ROUTE>
+template <int NE>
 __global__ void __launch_bounds__(kPlanThreads) k_moe_plan(RouteArgs a, const int *__restrict__ ids, const float *__restrict__ weights,
                                                            MoePlan p, int M, int E, int top, int per) {
-  constexpr int MP = GQ_MOE_MAX_TOKENS * GQ_MOE_MAX_TOP;
+  constexpr int MP = GQ_MOE_MAX_TOKENS * GQ_MOE_MAX_TOP, FB = kMoeFew * GQ_MOE_MAX_TOP;
   static_assert(MP <= kPlanThreads && GQ_MOE_MAX_EXPERTS <= kPlanThreads, "a thread a pair, a thread an expert");
-  __shared__ int id_s[MP], key_s[MP], cnt_s[kPlanThreads], base_s[kPlanThreads], tot_s[kPlanThreads / 64];
-  __shared__ float w_s[MP];
+  __shared__ int id_s[MP], base_s[kPlanThreads], tot_s[kPlanThreads / 64], pair_s[FB][kMoeFew];
+  __shared__ uint32_t tok_s[2][kPlanThreads];  // the tokens of an expert, a bit each
+  __shared__ float w_s[MP], wsum_s[FB];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, P = M * top;
-  cnt_s[tid] = 0;
-  if constexpr (ROUTE) {
-    for (int m = wave; m < M; m += kPlanThreads / 64) moe_choose(a, m, E, top, lane, id_s, w_s);
+  const bool few = M <= kMoeFew;
+  tok_s[0][tid] = tok_s[1][tid] = 0;
+  if (tid < FB * kMoeFew) pair_s[tid / kMoeFew][tid % kMoeFew] = -1;
+  if constexpr (NE > 0) {
+    for (int m = wave; m < M; m += kPlanThreads / 64) moe_choose<NE>(a, m, E, top, lane, id_s, w_s);
   } else if (tid < P) {
     id_s[tid] = ids[tid];
     w_s[tid] = weights[tid];
   }
-  if (!p.nblk) return;  // (the choice alone)
+  if (!p.blk) return;  // (the choice alone)
   __syncthreads();
+  const int tok = tid / top;
   int id = -1;
   if (tid < P) {
-    const int t0 = tid / top * top;
     id = id_s[tid];
     if (id < 0 || id >= E) id = -1;
-    float w = 0.f;
-    for (int j = t0; j < t0 + top; ++j) {
-      if (id_s[j] != id) continue;
-      if (j < tid) id = -1;
-      else w += w_s[j];
+    float w = w_s[tid];
+    if constexpr (NE == 0) {
+      w = 0.f;
+      for (int j = tok * top; j < tok * top + top; ++j) {
+        if (id_s[j] != id) continue;
+        if (j < tid) id = -1;  // (the first pair's)
+        else w += w_s[j];
+      }
     }
-    p.wsum[tid] = w;
-    key_s[tid] = id;
-    if (id >= 0) atomicAdd(&cnt_s[id], 1);
+    if (few) wsum_s[tid] = w;
+    else p.wsum[tid] = w;
+    if (id >= 0) atomicOr(&tok_s[tok >> 5][id], 1u << (tok & 31));
   }
   __syncthreads();
-  int rank = 0;
-  for (int q = 0; q < P; ++q) rank += q < tid && key_s[q] == id;
-  const int c = cnt_s[tid], nb = (c + per - 1) / per;
+  const int c = __popc(tok_s[0][tid]) + __popc(tok_s[1][tid]), nb = (c + per - 1) / per;
   int inc = nb;
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) {
@@ -200,29 +230,33 @@ __global__ void __launch_bounds__(kPlanThreads) k_moe_plan(RouteArgs a, const in
   if (lane == 63) tot_s[wave] = inc;
   __syncthreads();
   int base = inc - nb, all = 0;
+#pragma unroll
   for (int w = 0; w < kPlanThreads / 64; ++w) {
-    if (w < wave) base += tot_s[w];
-    all += tot_s[w];
+    const int v = tot_s[w];
+    if (w < wave) base += v;
+    all += v;
   }
   base_s[tid] = base;
-  if (tid == 0) *p.nblk = all;
-  const bool few = M <= kMoeFew;
   for (int b = 0; b < nb; ++b) {
-    MoeBlk &k = p.blk[base + b];
-    k.expert = tid;
-    k.count = c - per * b < per ? c - per * b : per;
-    if (few) {
-#pragma unroll
-      for (int m = 0; m < kMoeFew; ++m) {
-        int pr = -1;
-        for (int j = 0; j < top && m < M; ++j)
-          if (key_s[m * top + j] == tid) pr = m * top + j;
-        k.pair[m] = pr;
-      }
-    }
+    p.blk[base + b].expert = tid;
+    p.blk[base + b].count = c - per * b < per ? c - per * b : per;
   }
+  for (int b = all + tid; b < p.maxblk; b += kPlanThreads) p.blk[b].expert = -1;
+  if (tid == 0) *p.nblk = all;
   __syncthreads();
-  if (!few && id >= 0) p.blk[base_s[id] + rank / per].pair[rank % per] = tid;
+  if (id >= 0) {
+    const uint32_t below = (1u << (tok & 31)) - 1u, w0 = tok_s[0][id], w1 = tok_s[1][id];
+    const int rank = tok < 32 ? __popc(w0 & below) : __popc(w0) + __popc(w1 & below);
+    if (few) pair_s[base_s[id]][tok] = tid;
+    else p.blk[base_s[id] + rank / per].pair[rank % per] = tid;
+  }
+  if (!few) return;
+  __syncthreads();
+  if (tid < all * kMoeFew) {
+    const int b = tid / kMoeFew, m = tid % kMoeFew, q = pair_s[b][m];
+    p.blk[b].pair[m] = q;
+    p.blk[b].w[m] = q < 0 ? 0.f : wsum_s[q];
+  }
 }
 
 // ---- gate and up -----------------------------------------------------------------------
@@ -249,11 +283,12 @@ k_moe_gu_few(const uint8_t *__restrict__ wg, const uint8_t *__restrict__ wu, siz
   constexpr int NG = kFewGroups<FMT>, T = 2 * R;
   constexpr float OFF = kFewOff<FMT, XT>;
   __shared__ float red[KS][T][MR][64];
-  if ((int)blockIdx.y >= *p.nblk) return;
   const MoeBlk &blk = p.blk[blockIdx.y];
+  const int expert = __builtin_amdgcn_readfirstlane(blk.expert);
+  if (expert < 0) return;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int g = lane >> 4, ntiles = N / 16;
-  const size_t tile0 = (size_t)__builtin_amdgcn_readfirstlane(blk.expert) * (size_t)ntiles;
+  const size_t tile0 = (size_t)expert * (size_t)ntiles;
   FTile<FMT> tl[T];
 #pragma unroll
   for (int t = 0; t < T; ++t) {
@@ -330,11 +365,12 @@ k_moe_gu_rows(const uint8_t *__restrict__ wg, const uint8_t *__restrict__ wu, si
               int top) {
   constexpr int T = 2 * R;
   __shared__ gq_f4 red[KS][T][64];
-  if ((int)blockIdx.y >= *p.nblk) return;
   const MoeBlk &blk = p.blk[blockIdx.y];
+  const int expert = __builtin_amdgcn_readfirstlane(blk.expert);
+  if (expert < 0) return;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int g = lane >> 4, r = lane & 15, ntiles = N / 16;
-  const size_t tile0 = (size_t)__builtin_amdgcn_readfirstlane(blk.expert) * (size_t)ntiles;
+  const size_t tile0 = (size_t)expert * (size_t)ntiles;
   FTile<FMT> tl[T];
 #pragma unroll
   for (int t = 0; t < T; ++t) {
@@ -423,14 +459,14 @@ k_moe_down_few(const uint8_t *__restrict__ wd, size_t sc_off, const float *__res
   __shared__ int e_s[MB], p_s[MB][kMoeFew];
   __shared__ float w_s[MB][kMoeFew];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int g = lane >> 4, ntiles = K / 16, nblk = __builtin_amdgcn_readfirstlane(*p.nblk);
-  if (tid < nblk) {
+  const int g = lane >> 4, ntiles = K / 16;
+  const int nblk = __builtin_amdgcn_readfirstlane(*p.nblk);
+  if (tid < p.maxblk) {  // (not nblk, which would have to arrive first)
     e_s[tid] = p.blk[tid].expert;
 #pragma unroll
     for (int m = 0; m < kMoeFew; ++m) {
-      const int q = p.blk[tid].pair[m];
-      p_s[tid][m] = q;
-      w_s[tid][m] = q < 0 ? 0.f : p.wsum[q];
+      p_s[tid][m] = p.blk[tid].pair[m];
+      w_s[tid][m] = p.blk[tid].w[m];
     }
   }
   __syncthreads();
@@ -534,13 +570,14 @@ k_moe_down_rows(const uint8_t *__restrict__ wd, size_t sc_off, const _Float16 *_
   uint16_t *e_s = p_s + 16 * maxblk;                                     // [maxblk]
   uint8_t *t_s = reinterpret_cast<uint8_t *>(e_s + maxblk);              // [P]: token of a pair
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int g = lane >> 4, r = lane & 15, ntiles = K / 16, nblk = __builtin_amdgcn_readfirstlane(*p.nblk);
+  const int g = lane >> 4, r = lane & 15, ntiles = K / 16;
+  const int nblk = __builtin_amdgcn_readfirstlane(*p.nblk);
   for (int i = tid; i < KS * M * 16; i += 64 * KS) sum_s[i] = 0.f;
   for (int i = tid; i < P; i += 64 * KS) {
     f_s[i] = p.wsum[i] * hs[i];
     t_s[i] = (uint8_t)(i / top);
   }
-  for (int i = tid; i < 16 * nblk; i += 64 * KS) {
+  for (int i = tid; i < 16 * maxblk; i += 64 * KS) {
     const MoeBlk &b = p.blk[i >> 4];
     p_s[i] = (i & 15) < b.count ? (uint16_t)b.pair[i & 15] : (uint16_t)0xFFFF;
     if ((i & 15) == 0) e_s[i >> 4] = (uint16_t)b.expert;
@@ -656,15 +693,33 @@ MoeWs moe_ws(const gq_moe &l, size_t M) {
   return w;
 }
 
+template <int XT, int RT>
+int launch_logits_t(const gq_moe &l, const void *x, double *logits, int M, hipStream_t s) {
+#define GQ_LOG(TOK)                                                                                                            \
+  hipLaunchKernelGGL((k_moe_logits<XT, RT, TOK>), dim3((unsigned)l.n_experts, (unsigned)((M + (TOK)-1) / (TOK))), dim3(kLogThreads), \
+                     0, s, x, l.router, logits, M, (int)l.n_experts, (int)l.K)
+  if (M == 1) GQ_LOG(1);
+  else GQ_LOG(4);
+#undef GQ_LOG
+  return gq_last_launch();
+}
 template <int XT>
 int launch_logits_x(const gq_moe &l, const void *x, double *logits, int M, hipStream_t s) {
-  const dim3 grid((unsigned)l.n_experts, (unsigned)((M + kLogTok - 1) / kLogTok)), block(kLogThreads);
-#define GQ_LOG(RT) \
-  hipLaunchKernelGGL((k_moe_logits<XT, RT>), grid, block, 0, s, x, l.router, logits, M, (int)l.n_experts, (int)l.K)
-  if (l.router_dtype == GQ_DT_F32) GQ_LOG(GQ_DT_F32);
-  else if (l.router_dtype == GQ_DT_F16) GQ_LOG(GQ_DT_F16);
-  else GQ_LOG(GQ_DT_BF16);
-#undef GQ_LOG
+  if (l.router_dtype == GQ_DT_F32) return launch_logits_t<XT, GQ_DT_F32>(l, x, logits, M, s);
+  if (l.router_dtype == GQ_DT_F16) return launch_logits_t<XT, GQ_DT_F16>(l, x, logits, M, s);
+  return launch_logits_t<XT, GQ_DT_BF16>(l, x, logits, M, s);
+}
+int launch_plan(const gq_moe &l, const RouteArgs &a, const int *ids, const float *weights, const MoePlan &plan, int M,
+                hipStream_t s) {
+  const int E = (int)l.n_experts;
+#define GQ_PLAN(NE)                                                                                                       \
+  hipLaunchKernelGGL(k_moe_plan<NE>, dim3(1), dim3(kPlanThreads), 0, s, a, ids, weights, plan, M, E, l.top_k, M <= kMoeFew ? kMoeFew : 16)
+  if (!a.logits) GQ_PLAN(0);
+  else if (E <= 64) GQ_PLAN(1);
+  else if (E <= 128) GQ_PLAN(2);
+  else if (E <= 256) GQ_PLAN(4);
+  else GQ_PLAN(16);
+#undef GQ_PLAN
   return gq_last_launch();
 }
 int launch_route(const gq_moe &l, const void *x, int xt, int M, double *logits, int *ids, float *weights, const MoePlan &plan,
@@ -673,9 +728,7 @@ int launch_route(const gq_moe &l, const void *x, int xt, int M, double *logits, 
   else if (xt == GQ_DT_F16) GQ_TRY(launch_logits_x<GQ_DT_F16>(l, x, logits, M, s));
   else GQ_TRY(launch_logits_x<GQ_DT_BF16>(l, x, logits, M, s));
   const RouteArgs a = {logits, l.router_bias, ids, weights, l.score, l.renorm, l.scale};
-  hipLaunchKernelGGL(k_moe_plan<true>, dim3(1), dim3(kPlanThreads), 0, s, a, (const int *)nullptr, (const float *)nullptr, plan, M,
-                     (int)l.n_experts, l.top_k, M <= kMoeFew ? kMoeFew : 16);
-  return gq_last_launch();
+  return launch_plan(l, a, nullptr, nullptr, plan, M, s);
 }
 
 template <int FMT, int XT>
@@ -767,7 +820,7 @@ struct MoeRoom {
   }
 };
 MoePlan plan_of(const MoeWs &w, uint8_t *ws) {
-  return MoePlan{(int *)(ws + w.nblk), (MoeBlk *)(ws + w.blk), (float *)(ws + w.wsum)};
+  return MoePlan{(int *)(ws + w.nblk), (MoeBlk *)(ws + w.blk), (float *)(ws + w.wsum), w.maxblk};
 }
 
 }  // namespace
@@ -805,9 +858,7 @@ extern "C" int gq_moe_ffn(const gq_moe *l, const void *x, int x_dtype, const int
   MoeRoom room(ws, ws_bytes, w.bytes, s);
   GQ_TRY(room.status);
   const MoePlan plan = plan_of(w, room.ptr);
-  hipLaunchKernelGGL(k_moe_plan<false>, dim3(1), dim3(kPlanThreads), 0, s, RouteArgs{}, (const int *)ids, weights, plan, (int)M,
-                     (int)l->n_experts, l->top_k, M <= (size_t)kMoeFew ? kMoeFew : 16);
-  GQ_TRY(gq_last_launch());
+  GQ_TRY(launch_plan(*l, RouteArgs{}, (const int *)ids, weights, plan, (int)M, s));
   return moe_ffn(*l, x, x_dtype, plan, w, room.ptr, resid, y, y_dtype, (int)M, s);
 }
 
