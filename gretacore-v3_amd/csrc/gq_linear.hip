@@ -216,13 +216,26 @@ __global__ void __launch_bounds__(kDzThreads) k_lin_dz(const void *dy, const voi
       const int n = 8 * (tid + kDzThreads * i) + e;
       sum[i][e] = part && add && n < N ? pr[n] : 0.f;
     }
+  // whole runs of the next row are requested before a row's are used (whole: the row's last, ragged run is loaded in its turn)
+  FRaw<DT> ra[kDzRuns], rb[kDzRuns];
+  const bool gated = act != GQ_ACT_NONE;
+  auto request = [&](int m) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < kDzRuns; ++i) {
+      const int k = 8 * (tid + kDzThreads * i);
+      if (m >= M || k + 8 > N) continue;
+      px_load<DT>(dy, (size_t)m * (size_t)N + k, ra[i]);
+      if (gated) px_load<DT>(z, (size_t)m * (size_t)N + k, rb[i]);
+    }
+  };
+  request((int)blockIdx.x);
   int buf = 0;
   for (int m = (int)blockIdx.x; m < M; m += (int)gridDim.x, buf ^= 1) {
     const size_t row = (size_t)m * (size_t)N;
     auto grads = [&](int k, float (&o)[8]) __attribute__((always_inline)) {
       float a[8], b[8];
       dgu_load<DT>(dy, row, k, N, a);
-      if (act == GQ_ACT_NONE) {
+      if (!gated) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) o[e] = a[e];
         return;
@@ -237,13 +250,24 @@ __global__ void __launch_bounds__(kDzThreads) k_lin_dz(const void *dy, const voi
       const int k = 8 * (tid + kDzThreads * i);
 #pragma unroll
       for (int e = 0; e < 8; ++e) d[i][e] = 0.f;
-      if (k < N) grads(k, d[i]);
+      if (k + 8 <= N) {
+        float b[8];
+        px_floats<DT>(ra[i], true, d[i]);
+        if (gated) {
+          px_floats<DT>(rb[i], true, b);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) d[i][e] *= lin_act_d(act, b[e]);
+        }
+      } else if (k < N) {
+        grads(k, d[i]);
+      }
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         top = fmaxf(top, fabsf(d[i][e]));
         sum[i][e] += d[i][e];
       }
     }
+    request(m + (int)gridDim.x);
     if (a16)
       for (int k = SPAN + 8 * tid; k < N; k += 8 * kDzThreads) {
         float a[8];

@@ -32,13 +32,56 @@ struct MoePlan {
 };
 
 // ---- router --------------------------------------------------------------------------
+// Where the rows of x go as fp16 with a power-of-two scale each (gq_launch_a_to_f16's), a16 NULL: nowhere
+struct MoeConv {
+  _Float16 *a16;
+  float *rs;
+  int lda, q4;
+};
+// One wave, one row
+template <int XT>
+GQ_DEV void moe_convert(const void *x, const MoeConv &c, int m, int K, int lane) {
+  float top = 0.f;
+  for (int k = 8 * lane; k < K; k += 512) {
+    FRaw<XT> r;
+    float v[8];
+    px_load<XT>(x, (size_t)m * K + k, r);
+    px_floats<XT>(r, true, v);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(v[i]));
+  }
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
+  // s = 14 - floor(log2(top)) within +-100, 0 for a row of zeros or with an Inf
+  const int eb = (int)((__float_as_uint(top) >> 23) & 0xFFu);
+  const int sh = eb == 0 || eb == 0xFF ? 0 : min(max(14 + 127 - eb, -100), 100);
+  const float f = __uint_as_float((uint32_t)(127 + sh) << 23);
+  if (lane == 0) c.rs[m] = __uint_as_float((uint32_t)(127 - sh) << 23);
+  for (int k = 8 * lane; k < c.lda; k += 512) {
+    FRaw<XT> r;
+    float v[8];
+    px_load<XT>(x, (size_t)m * K + (k < K ? k : 0), r);
+    px_floats<XT>(r, k < K, v);
+    gq_half8 h;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) h[i] = (_Float16)((c.q4 ? (kQ4Div16[i] ? v[kQ4Perm[i]] * 0.0625f : v[kQ4Perm[i]]) : v[i]) * f);
+    *reinterpret_cast<gq_half8 *>(c.a16 + (size_t)m * c.lda + k) = h;
+  }
+}
 // Workgroup (e, b): logits of expert e for tokens TOK b .. TOK b + TOK - 1.  Products of two fp32 values are exact in 64 bits.
+// Workgroup (E, b): the conversion of those tokens' rows, a wave a row.
 constexpr int kLogThreads = 256;
 template <int XT, int RT, int TOK>
 __global__ void __launch_bounds__(kLogThreads) k_moe_logits(const void *__restrict__ x, const void *__restrict__ wr,
-                                                            double *__restrict__ logits, int M, int E, int K) {
+                                                            double *__restrict__ logits, MoeConv conv, int M, int E, int K) {
+  static_assert(TOK <= kLogThreads / 64, "a wave a row");
   __shared__ double red[kLogThreads / 64][TOK];
   const int tid = threadIdx.x, e = blockIdx.x, m0 = TOK * (int)blockIdx.y;
+  if (e == E) {
+    const int w = tid >> 6;
+    if (w < TOK && m0 + w < M) moe_convert<XT>(x, conv, m0 + w, K, tid & 63);
+    return;
+  }
   double acc[TOK] = {};
 #pragma unroll 2
   for (int k = 8 * tid; k < K; k += 8 * kLogThreads) {  // (K is whole 8s)
@@ -98,7 +141,7 @@ GQ_DEV double lane_d(double v, int lane) {  // (lane: the same in all lanes)
   const uint32_t hi = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(b >> 32), lane);
   return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
 }
-// One wave chooses the experts of token m; lane j writes slot j.  A key is a 64-bit number in the values' order, 0 what is
+// One wave chooses the experts of token m; lane j writes slot j (ids_s: in LDS, at the token's place).  A key is a 64-bit number in the values' order, 0 what is
 // never taken (-Inf, none there, taken before): the largest's high word, then its low word, then the lowest
 // expert that has both.
 template <int NE>
@@ -170,11 +213,18 @@ GQ_DEV void moe_choose(const RouteArgs &a, int m, int E, int top, int lane, int 
   }
   if (lane < top) {
     const float f = id < 0 ? 0.f : (float)(w * (double)a.scale);
-    ids_s[m * top + lane] = id;
-    w_s[m * top + lane] = f;
+    if (ids_s) {
+      ids_s[m * top + lane] = id;
+      w_s[m * top + lane] = f;
+    }
     if (a.ids) a.ids[m * top + lane] = id;
     if (a.weights) a.weights[m * top + lane] = f;
   }
+}
+
+template <int NE>
+__global__ void __launch_bounds__(64) k_moe_choose(RouteArgs a, int E, int top) {
+  moe_choose<NE>(a, (int)blockIdx.x, E, top, (int)threadIdx.x, nullptr, nullptr);
 }
 
 // ---- plan: one workgroup ------------------------------------------------------------
@@ -199,7 +249,6 @@ __global__ void __launch_bounds__(kPlanThreads) k_moe_plan(RouteArgs a, const in
     id_s[tid] = ids[tid];
     w_s[tid] = weights[tid];
   }
-  if (!p.blk) return;  // (the choice alone)
   __syncthreads();
   const int tok = tid / top;
   int id = -1;
@@ -260,27 +309,26 @@ __global__ void __launch_bounds__(kPlanThreads) k_moe_plan(RouteArgs a, const in
 }
 
 // ---- gate and up -----------------------------------------------------------------------
-template <int KS, int R, int MR, typename At>
-GQ_DEV void moe_gu_out(At at, float *__restrict__ h, int N, int act, int group, int rows, const int *pair, const float *rs, int top) {
-  for (int o = threadIdx.x; o < 16 * R * rows; o += 64 * KS) {
-    const int nl = o % (16 * R), m = o / (16 * R), n = 16 * R * group + nl, p = pair[m];
-    if (n >= N || p < 0) continue;
-    float y[2] = {0.f, 0.f};
+// Output (m, 16 t + n) of the R tiles `group` in both matrices from the waves' parts at(k, w, t, n, m)
+template <int KS, int R, typename At>
+GQ_DEV float moe_gu_h(At at, int nl, int m, float f, int act) {
+  float y[2] = {0.f, 0.f};
 #pragma unroll
-    for (int w = 0; w < 2; ++w)
+  for (int w = 0; w < 2; ++w)
 #pragma unroll
-      for (int k = 0; k < KS; ++k) y[w] += at(k, w, nl >> 4, nl & 15, m);
-    const float f = rs ? rs[p / top] : 1.f, g = y[0] * f, u = y[1] * f;
-    h[(size_t)p * N + n] = gq_act_f(act, g) * u;
-  }
+    for (int k = 0; k < KS; ++k) y[w] += at(k, w, nl >> 4, nl & 15, m);
+  return gq_act_f(act, y[0] * f) * (y[1] * f);
 }
 
-// Up to 4 tokens of 16-bit x: codes and x as they are, scales in fp32 (gq_rows_frag.h); row j is token j.
-template <int FMT, int XT, int MR, int R, int KS, int PD>
+// Up to 4 tokens of 16-bit x: codes and x as they are, scales in fp32 (gq_rows_frag.h); row j is token j.  h goes out in fp16 (nib:
+// in the nibbles' order) with a power-of-two scale for each 32 of a row, the scale groups of W_down's products; the inverse of block
+// 2 m + i of 128 values to hs[pair][128s][i][m].
+template <int FMT, int XT, int MR, int KS, int PD>
 __global__ void __launch_bounds__(64 * KS)
 k_moe_gu_few(const uint8_t *__restrict__ wg, const uint8_t *__restrict__ wu, size_t sc_off, const void *__restrict__ x,
-             const float *__restrict__ rs, MoePlan p, float *__restrict__ h, int M, int N, int K, int C, int units, int act, int top) {
-  constexpr int NG = kFewGroups<FMT>, T = 2 * R;
+             const float *__restrict__ rs, MoePlan p, _Float16 *__restrict__ h, float *__restrict__ hs, int nib, int M, int N, int K,
+             int C, int units, int act, int top) {
+  constexpr int NG = kFewGroups<FMT>, R = 2, T = 2 * R;
   constexpr float OFF = kFewOff<FMT, XT>;
   __shared__ float red[KS][T][MR][64];
   const MoeBlk &blk = p.blk[blockIdx.y];
@@ -347,14 +395,31 @@ k_moe_gu_few(const uint8_t *__restrict__ wg, const uint8_t *__restrict__ wu, siz
 #pragma unroll
     for (int v = 0; v < MR; ++v) red[wave][t][v][lane] = acc[t][v];
   __syncthreads();
-  moe_gu_out<KS, R, MR>(
-      [&](int k, int w, int t, int n, int m) {
+  const int m = threadIdx.x >> 5, nl = threadIdx.x & 31, n0 = 32 * (int)blockIdx.x;  // (N is whole 32-blocks)
+  const int q = m < M ? blk.pair[m] : -1;
+  if (q < 0) return;  // (whole half-waves)
+  const float v = moe_gu_h<KS, R>(
+      [&](int k, int w, int t, int n, int mm) {
         float y = 0.f;
 #pragma unroll
-        for (int i = 0; i < NG; ++i) y += red[k][w * R + t][MR == 1 ? 0 : m][16 * i + n];
+        for (int i = 0; i < NG; ++i) y += red[k][w * R + t][MR == 1 ? 0 : mm][16 * i + n];
         return y;
       },
-      h, N, act, (int)blockIdx.x, M, blk.pair, rs, top);
+      nl, m, rs ? rs[m] : 1.f, act);
+  float t = fabsf(v);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) t = fmaxf(t, __shfl_xor(t, o, 32));
+  // 2^s, s = 14 - floor(log2(t)) at most 126 (at least -114: both have a normal inverse)
+  const int sh = 14 + 127 - (int)((__float_as_uint(t) >> 23) & 0xFFu), cut = sh > 126 ? 126 : sh;
+  const int e = nl & 7, to = nib ? (e & 1 ? 4 + (e >> 1) : e >> 1) : e;
+  h[(size_t)q * N + n0 + (nl & 24) + to] = (_Float16)(v * __uint_as_float((uint32_t)(127 + cut) << 23));
+  if (nl == 0) {
+    const int c = (n0 >> 5) & 3;
+    float *o = hs + ((size_t)q * ((N + 127) / 128) + (n0 >> 7)) * 4;
+    o[2 * (c & 1) + (c >> 1)] = __uint_as_float((uint32_t)(127 - cut) << 23);
+    if (n0 + 32 == N)
+      for (int d = c + 1; d < 4; ++d) o[2 * (d & 1) + (d >> 1)] = 0.f;  // (blocks behind the row)
+  }
 }
 
 // More tokens: a block's rows are its pairs, fp16 rows of x gathered, the scale groups folded into the weights.
@@ -405,11 +470,15 @@ k_moe_gu_rows(const uint8_t *__restrict__ wg, const uint8_t *__restrict__ wu, si
 #pragma unroll
   for (int t = 0; t < T; ++t) red[wave][t][lane] = acc[t][0];
   __syncthreads();
-  moe_gu_out<KS, R, 4>(
-      [&](int k, int w, int t, int n, int m) {
-        return reinterpret_cast<const float *>(&red[k][w * R + t][16 * (m >> 2) + n])[m & 3];
-      },
-      h, N, act, (int)blockIdx.x, blk.count, blk.pair, rs, top);
+  for (int o = threadIdx.x; o < 16 * R * blk.count; o += 64 * KS) {
+    const int nl = o % (16 * R), m = o / (16 * R), n = 16 * R * (int)blockIdx.x + nl, q = blk.pair[m];
+    if (n >= N) continue;
+    h[(size_t)q * N + n] = moe_gu_h<KS, R>(
+        [&](int k, int w, int t, int nn, int mm) {
+          return reinterpret_cast<const float *>(&red[k][w * R + t][16 * (mm >> 2) + nn])[mm & 3];
+        },
+        nl, m, rs[q / top], act);
+  }
 }
 
 // ---- down ------------------------------------------------------------------------------
@@ -426,8 +495,8 @@ struct ItemAt {
   }
 };
 template <int PD, int KS, typename Request, typename Compute>
-GQ_DEV void walk_items(int nblk, int units, int wave, Request request, Compute compute) {
-  ItemAt rq = {0, 0}, at = {0, 0};
+GQ_DEV void walk_items(int b0, int nblk, int units, int wave, Request request, Compute compute) {
+  ItemAt rq = {b0, 0}, at;
   rq.next(wave, units);
   at = rq;
 #pragma unroll
@@ -447,12 +516,11 @@ GQ_DEV void walk_items(int nblk, int units, int wave, Request request, Compute c
   }
 }
 
-// Up to 4 tokens: rows are the tokens, h comes in fp32 and is rounded to fp16 after a power-of-two scale per row and unit; the
-// scale's inverse and the expert's weight go onto the unit's fp32 sums.
+// Up to 4 tokens: rows are the tokens; the scale groups' fp32 sums take the inverse scales of h and the expert's weight.
 template <int FMT, int MR, int KS, int PD>
 __global__ void __launch_bounds__(64 * KS)
-k_moe_down_few(const uint8_t *__restrict__ wd, size_t sc_off, const float *__restrict__ h, MoePlan p, const void *resid, void *y,
-               int dt, int M, int N, int K, int C, int units, int top) {
+k_moe_down_few(const uint8_t *__restrict__ wd, size_t sc_off, const _Float16 *__restrict__ h, const float *__restrict__ hs, MoePlan p,
+               const void *resid, void *y, int dt, int M, int N, int K, int C, int units, int top) {
   constexpr int NG = kFewGroups<FMT>, XT = GQ_DT_F16, MB = kMoeFew * GQ_MOE_MAX_TOP;
   constexpr float OFF = kFewOff<FMT, XT>;
   __shared__ float red[KS][MR][64];
@@ -471,21 +539,29 @@ k_moe_down_few(const uint8_t *__restrict__ wd, size_t sc_off, const float *__res
   }
   __syncthreads();
   const __amdgpu_buffer_rsrc_t hr = __builtin_amdgcn_make_buffer_rsrc(
-      const_cast<float *>(h), (short)0, (int)(4u * (uint32_t)(M * top) * (uint32_t)N), 0x00020000);
+      const_cast<_Float16 *>(h), (short)0, (int)(2u * (uint32_t)(M * top) * (uint32_t)N), 0x00020000);
+  const __amdgpu_buffer_rsrc_t sr = __builtin_amdgcn_make_buffer_rsrc(
+      const_cast<float *>(hs), (short)0, (int)(16u * (uint32_t)(M * top) * (uint32_t)units), 0x00020000);
   const int xrow = lane & 3, xk = 64 * ((lane >> 3) & 1) + 16 * g + 8 * ((lane >> 2) & 1);
+  const uint32_t gi = NG == 2 ? (uint32_t)g & 1u : (uint32_t)g >> 1;  // the 32-block of a step that this lane's sums are of
   FUnit<FMT> us[PD];
-  gq_f4 xs[PD][2];
+  gq_u4 xs[PD];
+  float2 is[PD][MR];
   auto request = [&](const ItemAt &at, int st) __attribute__((always_inline)) {
     const bool on = at.b < nblk;
     const int b = on ? at.b : 0;
     const size_t tile = (size_t)__builtin_amdgcn_readfirstlane(e_s[b]) * (size_t)ntiles + blockIdx.x;
     load_unit<FMT>(ftile<FMT>(wd, sc_off, tile, on ? C : 0), at.u, lane, us[st]);
     const int q = p_s[b][xrow], k = 128 * at.u + xk;  // (N is whole 32-blocks: a run is wholly in or out)
-    const uint32_t o = on && q >= 0 && k < N ? 4u * ((uint32_t)q * (uint32_t)N + (uint32_t)k) : 0xFFFFFFE0u;
+    const uint32_t o = on && q >= 0 && k < N ? 2u * ((uint32_t)q * (uint32_t)N + (uint32_t)k) : 0xFFFFFFF0u;
+    const auto v = __builtin_amdgcn_raw_buffer_load_b128(hr, o, 0, 0);
+    xs[st] = gq_u4{v[0], v[1], v[2], v[3]};
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const auto v = __builtin_amdgcn_raw_buffer_load_b128(hr, o + 16u * i, 0, 0);
-      xs[st][i] = __builtin_bit_cast(gq_f4, v);
+    for (int r = 0; r < MR; ++r) {
+      const int qr = p_s[b][r];
+      const uint32_t so = on && qr >= 0 ? 8u * (2u * ((uint32_t)qr * (uint32_t)units + (uint32_t)at.u) + gi) : 0xFFFFFFF0u;
+      const auto f = __builtin_amdgcn_raw_buffer_load_b64(sr, so, 0, 0);  // (none: 0)
+      is[st][r] = make_float2(__uint_as_float(f[0]), __uint_as_float(f[1]));
     }
   };
   float acc[MR] = {};
@@ -494,22 +570,10 @@ k_moe_down_few(const uint8_t *__restrict__ wd, size_t sc_off, const float *__res
   const gq_u4 ones = {0x3C003C00u, 0x3C003C00u, 0x3C003C00u, 0x3C003C00u};
   const gq_f4 zero = {0.f, 0.f, 0.f, 0.f};
   auto compute = [&](const ItemAt &at, int st) __attribute__((always_inline)) {
-    float v[8], t = 0.f;
+    const gq_u4 xv = xs[st];
+    float s[2], mn[2], w[MR];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      v[i] = xs[st][i >> 2][i & 3];
-      t = fmaxf(t, fabsf(v[i]));
-    }
-#pragma unroll
-    for (int o = 4; o < 64; o <<= 1) t = fmaxf(t, __shfl_xor(t, o, 64));
-    // 2^s, s = 14 - floor(log2(t)) at most 126 (at least -114: both have a normal inverse)
-    const int sh = 14 + 127 - (int)((__float_as_uint(t) >> 23) & 0xFFu), cut = sh > 126 ? 126 : sh;
-    const float f2 = __uint_as_float((uint32_t)(127 + cut) << 23), inv = __uint_as_float((uint32_t)(127 - cut) << 23);
-    gq_u4 xv;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) xv[i] = gq_h2_bits(gq_half2{(_Float16)(v[2 * i] * f2), (_Float16)(v[2 * i + 1] * f2)});
-    if (kNibOrder<FMT>) xv = nib_order(xv);
-    float s[2], mn[2], sum[MR] = {};
+    for (int r = 0; r < MR; ++r) w[r] = w_s[at.b][r];
     few_scales<FMT>(us[st], at.u, g & (NG - 1), s, mn);
     auto step = [&](auto mc) __attribute__((always_inline)) {
       constexpr int m = decltype(mc)::value;
@@ -518,28 +582,15 @@ k_moe_down_few(const uint8_t *__restrict__ wd, size_t sc_off, const float *__res
       gq_u4 b[2];
       few_codes<FMT, XT>(us[st], m, mg, b);
       const gq_f4 d = few_mfma<XT>(a1, b[1], few_mfma<XT>(a0, b[0], zero));
-      const float o = FMT == GQ_FMT_Q4_K ? fmaf(s[m], OFF, mn[m]) : 0.f;
+      const float o = FMT == GQ_FMT_Q4_K ? fmaf(s[m], OFF, mn[m]) : s[m] * OFF;
 #pragma unroll
-      for (int r = 0; r < MR; ++r) {
-        if constexpr (FMT == GQ_FMT_Q4_K) sum[r] = fmaf(s[m], d[r], fmaf(-o, sx[r], sum[r]));
-        else sum[r] = fmaf(s[m], fmaf(-OFF, sx[r], d[r]), sum[r]);
-      }
+      for (int r = 0; r < MR; ++r)
+        acc[r] = fmaf(w[r] * (m ? is[st][r].y : is[st][r].x), fmaf(s[m], d[r], -o * sx[r]), acc[r]);
     };
     step(std::integral_constant<int, 0>{});
     step(std::integral_constant<int, 1>{});
-    // (each quad of lanes holds the four rows' scales)
-    const float inv0 = __uint_as_float((uint32_t)__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(inv), 0x00, 15, 15, true));
-    acc[0] = fmaf(w_s[at.b][0] * inv0, sum[0], acc[0]);
-    if constexpr (MR == 4) {
-      const float inv1 = __uint_as_float((uint32_t)__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(inv), 0x55, 15, 15, true));
-      const float inv2 = __uint_as_float((uint32_t)__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(inv), 0xAA, 15, 15, true));
-      const float inv3 = __uint_as_float((uint32_t)__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(inv), 0xFF, 15, 15, true));
-      acc[1] = fmaf(w_s[at.b][1] * inv1, sum[1], acc[1]);
-      acc[2] = fmaf(w_s[at.b][2] * inv2, sum[2], acc[2]);
-      acc[3] = fmaf(w_s[at.b][3] * inv3, sum[3], acc[3]);
-    }
   };
-  if (nblk > 0) walk_items<PD, KS>(nblk, units, wave, request, compute);
+  if (nblk > 0) walk_items<PD, KS>(0, nblk, units, wave, request, compute);
 #pragma unroll
   for (int r = 0; r < MR; ++r) red[wave][r][lane] = acc[r];
   __syncthreads();
@@ -557,11 +608,12 @@ k_moe_down_few(const uint8_t *__restrict__ wd, size_t sc_off, const float *__res
 }
 
 // More tokens: a block's rows are its pairs (fp16 rows of h with a power-of-two scale each); a block's sums go, with the
-// scale's inverse and the expert's weight, to the wave's own sums of the tokens in LDS.
+// scale's inverse and the expert's weight, to the wave's own sums of the tokens in LDS.  gridDim.y parts of the blocks: their sums go to part
+// [part][M][K] in fp32, which k_moe_sum adds.
 template <int FMT, int KS, int PD>
 __global__ void __launch_bounds__(64 * KS)
 k_moe_down_rows(const uint8_t *__restrict__ wd, size_t sc_off, const _Float16 *__restrict__ h16, int ldh, const float *__restrict__ hs,
-                MoePlan p, const void *resid, void *y, int dt, int M, int K, int C, int units, int top, int maxblk) {
+                MoePlan p, const void *resid, void *y, int dt, float *__restrict__ part, int M, int K, int C, int units, int top, int maxblk) {
   extern __shared__ float lds[];
   const int P = M * top;
   float *sum_s = lds;                                                    // [KS][M][16]
@@ -571,7 +623,8 @@ k_moe_down_rows(const uint8_t *__restrict__ wd, size_t sc_off, const _Float16 *_
   uint8_t *t_s = reinterpret_cast<uint8_t *>(e_s + maxblk);              // [P]: token of a pair
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int g = lane >> 4, r = lane & 15, ntiles = K / 16;
-  const int nblk = __builtin_amdgcn_readfirstlane(*p.nblk);
+  const int all = __builtin_amdgcn_readfirstlane(*p.nblk);
+  const int b0 = all * (int)blockIdx.y / (int)gridDim.y, nblk = all * ((int)blockIdx.y + 1) / (int)gridDim.y;
   for (int i = tid; i < KS * M * 16; i += 64 * KS) sum_s[i] = 0.f;
   for (int i = tid; i < P; i += 64 * KS) {
     f_s[i] = p.wsum[i] * hs[i];
@@ -589,7 +642,7 @@ k_moe_down_rows(const uint8_t *__restrict__ wd, size_t sc_off, const _Float16 *_
   gq_half8 xs[PD][1][4];
   auto request = [&](const ItemAt &at, int st) __attribute__((always_inline)) {
     const bool on = at.b < nblk;
-    const int b = on ? at.b : 0;
+    const int b = on ? at.b : b0;
     const size_t tile = (size_t)__builtin_amdgcn_readfirstlane((int)e_s[b]) * (size_t)ntiles + blockIdx.x;
     load_unit<FMT>(ftile<FMT>(wd, sc_off, tile, on ? C : 0), at.u, lane, us[st]);
     const uint32_t q = p_s[16 * b + r];
@@ -619,7 +672,7 @@ k_moe_down_rows(const uint8_t *__restrict__ wd, size_t sc_off, const _Float16 *_
     }
     rows_add<FMT, 1>(us[st], at.u, g, mg, xs[st], acc);
   };
-  if (nblk > 0) walk_items<PD, KS>(nblk, units, wave, request, compute);
+  if (b0 < nblk) walk_items<PD, KS>(b0, nblk, units, wave, request, compute);
   flush();
   __syncthreads();
   for (int i = tid; i < 16 * M; i += 64 * KS) {
@@ -627,9 +680,21 @@ k_moe_down_rows(const uint8_t *__restrict__ wd, size_t sc_off, const _Float16 *_
     float v = 0.f;
     for (int w = 0; w < KS; ++w) v += sum_s[(w * M + m) * 16 + n];
     const size_t o = (size_t)m * K + 16 * blockIdx.x + n;
+    if (part) {
+      part[(size_t)blockIdx.y * M * K + o] = v;
+      continue;
+    }
     if (resid) v += gq_ld_dt(resid, dt, o);
     gq_st_dt(y, dt, o, v);
   }
+}
+__global__ void __launch_bounds__(256) k_moe_sum(const float *__restrict__ part, const void *resid, void *y, int dt, int n, int parts) {
+  const int i = (int)blockIdx.x * 256 + (int)threadIdx.x;
+  if (i >= n) return;
+  float v = 0.f;
+  for (int p = 0; p < parts; ++p) v += part[(size_t)p * n + i];
+  if (resid) v += gq_ld_dt(resid, dt, i);
+  gq_st_dt(y, dt, i, v);
 }
 
 // ---- host ----------------------------------------------------------------------------
@@ -663,8 +728,8 @@ int check_moe(const gq_moe *l, size_t M, bool route, bool ffn) {
 
 // Where a call's intermediate values lie in its workspace
 struct MoeWs {
-  size_t logits, ids, weights, nblk, blk, wsum, a16, rs, h, h16, hs, bytes;
-  int maxblk;
+  size_t logits, ids, weights, nblk, blk, wsum, a16, rs, h, h16, hs, part, bytes;
+  int maxblk, parts;
 };
 MoeWs moe_ws(const gq_moe &l, size_t M) {
   MoeWs w;
@@ -686,28 +751,33 @@ MoeWs moe_ws(const gq_moe &l, size_t M) {
   w.wsum = take(P * 4);
   w.a16 = take(M * (gq_kpad(l.fmt, l.K) + 8) * 2);
   w.rs = take((M + 256) * 4);
-  w.h = take(P * l.N * 4);
+  w.h = take(few ? 0 : P * l.N * 4);
   w.h16 = take(P * (gq_kpad(l.fmt_down, l.N) + 8) * 2);
-  w.hs = take((P + 256) * 4);
+  w.hs = take(few ? P * ((l.N + 127) / 128) * 16 : (P + 256) * 4);
+  // W_down's row tiles, a workgroup each, in parts where they would leave CUs idle
+  const size_t tiles = l.K / 16;
+  w.parts = few || tiles >= 192 ? 1 : (int)std::min({(size_t)4, 320 / tiles, (size_t)w.maxblk});
+  w.part = take(w.parts > 1 ? w.parts * M * l.K * 4 : 0);
   w.bytes = at;
   return w;
 }
 
 template <int XT, int RT>
-int launch_logits_t(const gq_moe &l, const void *x, double *logits, int M, hipStream_t s) {
-#define GQ_LOG(TOK)                                                                                                            \
-  hipLaunchKernelGGL((k_moe_logits<XT, RT, TOK>), dim3((unsigned)l.n_experts, (unsigned)((M + (TOK)-1) / (TOK))), dim3(kLogThreads), \
-                     0, s, x, l.router, logits, M, (int)l.n_experts, (int)l.K)
+int launch_logits_t(const gq_moe &l, const void *x, double *logits, const MoeConv &conv, int M, hipStream_t s) {
+#define GQ_LOG(TOK)                                                                                                       \
+  hipLaunchKernelGGL((k_moe_logits<XT, RT, TOK>), dim3((unsigned)(l.n_experts + (conv.a16 != nullptr)),                  \
+                                                       (unsigned)((M + (TOK)-1) / (TOK))),                               \
+                     dim3(kLogThreads), 0, s, x, l.router, logits, conv, M, (int)l.n_experts, (int)l.K)
   if (M == 1) GQ_LOG(1);
   else GQ_LOG(4);
 #undef GQ_LOG
   return gq_last_launch();
 }
 template <int XT>
-int launch_logits_x(const gq_moe &l, const void *x, double *logits, int M, hipStream_t s) {
-  if (l.router_dtype == GQ_DT_F32) return launch_logits_t<XT, GQ_DT_F32>(l, x, logits, M, s);
-  if (l.router_dtype == GQ_DT_F16) return launch_logits_t<XT, GQ_DT_F16>(l, x, logits, M, s);
-  return launch_logits_t<XT, GQ_DT_BF16>(l, x, logits, M, s);
+int launch_logits_x(const gq_moe &l, const void *x, double *logits, const MoeConv &conv, int M, hipStream_t s) {
+  if (l.router_dtype == GQ_DT_F32) return launch_logits_t<XT, GQ_DT_F32>(l, x, logits, conv, M, s);
+  if (l.router_dtype == GQ_DT_F16) return launch_logits_t<XT, GQ_DT_F16>(l, x, logits, conv, M, s);
+  return launch_logits_t<XT, GQ_DT_BF16>(l, x, logits, conv, M, s);
 }
 int launch_plan(const gq_moe &l, const RouteArgs &a, const int *ids, const float *weights, const MoePlan &plan, int M,
                 hipStream_t s) {
@@ -722,89 +792,120 @@ int launch_plan(const gq_moe &l, const RouteArgs &a, const int *ids, const float
 #undef GQ_PLAN
   return gq_last_launch();
 }
-int launch_route(const gq_moe &l, const void *x, int xt, int M, double *logits, int *ids, float *weights, const MoePlan &plan,
-                 hipStream_t s) {
-  if (xt == GQ_DT_F32) GQ_TRY(launch_logits_x<GQ_DT_F32>(l, x, logits, M, s));
-  else if (xt == GQ_DT_F16) GQ_TRY(launch_logits_x<GQ_DT_F16>(l, x, logits, M, s));
-  else GQ_TRY(launch_logits_x<GQ_DT_BF16>(l, x, logits, M, s));
-  const RouteArgs a = {logits, l.router_bias, ids, weights, l.score, l.renorm, l.scale};
+int launch_choose(const gq_moe &l, const RouteArgs &a, int M, hipStream_t s) {
+  const int E = (int)l.n_experts;
+#define GQ_CHOOSE(NE) hipLaunchKernelGGL(k_moe_choose<NE>, dim3((unsigned)M), dim3(64), 0, s, a, E, l.top_k)
+  if (E <= 64) GQ_CHOOSE(1);
+  else if (E <= 128) GQ_CHOOSE(2);
+  else if (E <= 256) GQ_CHOOSE(4);
+  else GQ_CHOOSE(16);
+#undef GQ_CHOOSE
+  return gq_last_launch();
+}
+// plan.blk NULL: the choice alone.  A wave a token, in the plan's workgroup where each of its 16 waves has one at most (in turn by four
+// tokens a wave 22 us for 64 tokens of 128 experts, in a launch of their own XX).
+int launch_route(const gq_moe &l, const void *x, int xt, int M, double *logits, const MoeConv &conv, int *ids, float *weights,
+                 const MoePlan &plan, hipStream_t s) {
+  if (xt == GQ_DT_F32) GQ_TRY(launch_logits_x<GQ_DT_F32>(l, x, logits, conv, M, s));
+  else if (xt == GQ_DT_F16) GQ_TRY(launch_logits_x<GQ_DT_F16>(l, x, logits, conv, M, s));
+  else GQ_TRY(launch_logits_x<GQ_DT_BF16>(l, x, logits, conv, M, s));
+  RouteArgs a = {logits, l.router_bias, ids, weights, l.score, l.renorm, l.scale};
+  if (M > kPlanThreads / 64 || !plan.blk) {
+    GQ_TRY(launch_choose(l, a, M, s));
+    if (!plan.blk) return GQ_OK;
+    a.logits = nullptr;
+    return launch_plan(l, a, ids, weights, plan, M, s);
+  }
   return launch_plan(l, a, nullptr, nullptr, plan, M, s);
 }
 
+// Intermediate values of a call
+struct MoeMid {
+  _Float16 *a16, *h16;
+  float *rs, *h, *hs, *part;
+  int lda, ldh, parts;
+};
 template <int FMT, int XT>
-int launch_gu_few_t(const gq_moe &l, const void *x, const float *rs, const MoePlan &p, float *h, int M, int maxblk, hipStream_t s) {
-  const int N = (int)l.N, K = (int)l.K, units = (int)(gq_kpad(FMT, K) / 128), tiles = N / 16;
-#define GQ_GU(MR, R, KS, PD)                                                                                              \
-  hipLaunchKernelGGL((k_moe_gu_few<FMT, XT, MR, R, KS, PD>), dim3((unsigned)((tiles + (R)-1) / (R)), (unsigned)maxblk),    \
-                     dim3(64 * (KS)), 0, s, (const uint8_t *)l.gate, (const uint8_t *)l.up,                               \
-                     gq_sc_plane_offset(FMT, l.n_experts * l.N, K), x, rs, p, h, M, N, K, (int)gq_chunks(FMT, K), units,  \
-                     l.act, l.top_k)
-  if (M == 1) GQ_GU(1, 1, 4, 3);
-  else GQ_GU(4, 1, 4, 3);
+int launch_gu_few_t(const gq_moe &l, const void *x, const float *rs, const MoePlan &p, const MoeMid &b, int M, hipStream_t s) {
+  const int N = (int)l.N, K = (int)l.K, units = (int)(gq_kpad(FMT, K) / 128), nib = l.fmt_down == GQ_FMT_Q4_0 || gq_fmt_is_q4k(l.fmt_down);
+#define GQ_GU(MR, KS, PD)                                                                                                  \
+  hipLaunchKernelGGL((k_moe_gu_few<FMT, XT, MR, KS, PD>), dim3((unsigned)(N / 32), (unsigned)p.maxblk), dim3(64 * (KS)), 0, s, \
+                     (const uint8_t *)l.gate, (const uint8_t *)l.up, gq_sc_plane_offset(FMT, l.n_experts * l.N, K), x, rs, p, b.h16, \
+                     b.hs, nib, M, N, K, (int)gq_chunks(FMT, K), units, l.act, l.top_k)
+  if (M == 1) GQ_GU(1, 4, 2);
+  else GQ_GU(4, 4, 2);
 #undef GQ_GU
   return gq_last_launch();
 }
 template <int FMT>
-int launch_gu_t(const gq_moe &l, const void *x, int xt, const _Float16 *a16, int lda, const float *rs, const MoePlan &p, float *h,
-                int M, int maxblk, hipStream_t s) {
+int launch_gu_t(const gq_moe &l, const void *x, int xt, const float *rs, const MoePlan &p, const MoeMid &b, int M, hipStream_t s) {
   if (M <= kMoeFew)
-    return xt == GQ_DT_F16 ? launch_gu_few_t<FMT, GQ_DT_F16>(l, x, rs, p, h, M, maxblk, s)
-                           : launch_gu_few_t<FMT, GQ_DT_BF16>(l, x, rs, p, h, M, maxblk, s);
-  const int N = (int)l.N, K = (int)l.K, units = (int)(gq_kpad(FMT, K) / 128), tiles = N / 16;
-  hipLaunchKernelGGL((k_moe_gu_rows<FMT, 1, 4, 3>), dim3((unsigned)tiles, (unsigned)maxblk), dim3(256), 0, s,
-                     (const uint8_t *)l.gate, (const uint8_t *)l.up, gq_sc_plane_offset(FMT, l.n_experts * l.N, K), a16, lda, rs, p,
-                     h, M, N, (int)gq_chunks(FMT, K), units, l.act, l.top_k);
+    return xt == GQ_DT_F16 ? launch_gu_few_t<FMT, GQ_DT_F16>(l, x, rs, p, b, M, s)
+                           : launch_gu_few_t<FMT, GQ_DT_BF16>(l, x, rs, p, b, M, s);
+  const int N = (int)l.N, K = (int)l.K, units = (int)(gq_kpad(FMT, K) / 128);
+  hipLaunchKernelGGL((k_moe_gu_rows<FMT, 1, 4, 3>), dim3((unsigned)(N / 16), (unsigned)p.maxblk), dim3(256), 0, s,
+                     (const uint8_t *)l.gate, (const uint8_t *)l.up, gq_sc_plane_offset(FMT, l.n_experts * l.N, K), b.a16, b.lda, rs, p,
+                     b.h, M, N, (int)gq_chunks(FMT, K), units, l.act, l.top_k);
   return gq_last_launch();
 }
 template <int FMT>
-int launch_down_t(const gq_moe &l, const float *h, const _Float16 *h16, int ldh, const float *hs, const MoePlan &p,
-                  const void *resid, void *y, int dt, int M, int maxblk, hipStream_t s) {
+int launch_down_t(const gq_moe &l, const MoePlan &p, const MoeMid &b, const void *resid, void *y, int dt, int M, hipStream_t s) {
   const int N = (int)l.N, K = (int)l.K, units = (int)(gq_kpad(FMT, N) / 128), C = (int)gq_chunks(FMT, N);
   const size_t so = gq_sc_plane_offset(FMT, l.n_experts * l.K, N);
-  const dim3 grid((unsigned)(K / 16));
-  constexpr int KS = 8;
+  const unsigned tiles = (unsigned)(K / 16);
   if (M <= kMoeFew) {
-#define GQ_DOWN(MR)                                                                                                    \
-  hipLaunchKernelGGL((k_moe_down_few<FMT, MR, KS, 4>), grid, dim3(64 * KS), 0, s, (const uint8_t *)l.down, so, h, p, resid, y, \
-                     dt, M, N, K, C, units, l.top_k)
-    if (M == 1) GQ_DOWN(1);
-    else GQ_DOWN(4);
+#define GQ_DOWN(MR, KS, PD)                                                                                              \
+  hipLaunchKernelGGL((k_moe_down_few<FMT, MR, KS, PD>), dim3(tiles), dim3(64 * (KS)), 0, s, (const uint8_t *)l.down, so, b.h16, b.hs, p, \
+                     resid, y, dt, M, N, K, C, units, l.top_k)
+    if (M == 1) GQ_DOWN(1, 16, 3);
+    else GQ_DOWN(4, 16, 2);
 #undef GQ_DOWN
     return gq_last_launch();
   }
-  const size_t P = (size_t)M * l.top_k, lds = (size_t)KS * M * 64 + P * 4 + (size_t)maxblk * 34 + P + 16;
-  hipLaunchKernelGGL((k_moe_down_rows<FMT, KS, 3>), grid, dim3(64 * KS), lds, s, (const uint8_t *)l.down, so, h16, ldh, hs, p, resid,
-                     y, dt, M, K, C, units, l.top_k, maxblk);
+  constexpr int KS = 8;
+  const size_t P = (size_t)M * l.top_k, lds = (size_t)KS * M * 64 + P * 4 + (size_t)p.maxblk * 34 + P + 16;
+  hipLaunchKernelGGL((k_moe_down_rows<FMT, KS, 3>), dim3(tiles, (unsigned)b.parts), dim3(64 * KS), lds, s, (const uint8_t *)l.down, so,
+                     b.h16, b.ldh, b.hs, p, resid, y, dt, b.parts > 1 ? b.part : nullptr, M, K, C, units, l.top_k, p.maxblk);
   return gq_last_launch();
 }
 
-int moe_ffn(const gq_moe &l, const void *x, int xt, const MoePlan &plan, const MoeWs &w, uint8_t *ws, const void *resid, void *y,
-            int dt, int M, hipStream_t s) {
-  _Float16 *a16 = (_Float16 *)(ws + w.a16), *h16 = (_Float16 *)(ws + w.h16);
-  float *rs = (float *)(ws + w.rs), *h = (float *)(ws + w.h), *hs = (float *)(ws + w.hs);
-  const bool few = M <= kMoeFew;
-  const int q4 = l.fmt == GQ_FMT_Q4_0 || gq_fmt_is_q4k(l.fmt), q4d = l.fmt_down == GQ_FMT_Q4_0 || gq_fmt_is_q4k(l.fmt_down);
-  const int lda = few ? (int)l.K : (int)gq_kpad(l.fmt, l.K) + 8, ldh = (int)gq_kpad(l.fmt_down, l.N) + 8;
-  const float *xs = nullptr;
-  if (!few || xt == GQ_DT_F32 || (uintptr_t)x % 4) {  // (few rows of 16-bit x go in as they are)
-    GQ_TRY(gq_launch_a_to_f16(x, xt, a16, rs, M, (int)l.K, lda, few ? 0 : q4, s));
-    x = a16;
+bool moe_few(int M) { return M <= kMoeFew; }
+// x goes in as it is: few rows of 16-bit values
+bool moe_as_it_is(const void *x, int xt, int M) { return moe_few(M) && xt != GQ_DT_F32 && (uintptr_t)x % 4 == 0; }
+MoeMid moe_mid(const gq_moe &l, const MoeWs &w, uint8_t *ws, int M) {
+  return MoeMid{(_Float16 *)(ws + w.a16), (_Float16 *)(ws + w.h16), (float *)(ws + w.rs), (float *)(ws + w.h), (float *)(ws + w.hs),
+                (float *)(ws + w.part), moe_few(M) ? (int)l.K : (int)gq_kpad(l.fmt, l.K) + 8, (int)gq_kpad(l.fmt_down, l.N) + 8, w.parts};
+}
+int moe_x_order(const gq_moe &l, int M) { return !moe_few(M) && (l.fmt == GQ_FMT_Q4_0 || gq_fmt_is_q4k(l.fmt)); }
+
+// The products, x converted already where it has to be
+int moe_products(const gq_moe &l, const void *x, int xt, const MoePlan &plan, const MoeMid &b, const void *resid, void *y, int dt, int M,
+                 hipStream_t s) {
+  const float *rs = nullptr;
+  if (!moe_as_it_is(x, xt, M)) {
+    x = b.a16;
     xt = GQ_DT_F16;
-    xs = rs;
+    rs = b.rs;
   }
-#define GQ_GU_F(F) launch_gu_t<F>(l, x, xt, a16, lda, xs, plan, h, M, w.maxblk, s)
+#define GQ_GU_F(F) launch_gu_t<F>(l, x, xt, rs, plan, b, M, s)
   if (l.fmt == GQ_FMT_Q4_0) GQ_TRY(GQ_GU_F(GQ_FMT_Q4_0));
   else if (l.fmt == GQ_FMT_Q8_0) GQ_TRY(GQ_GU_F(GQ_FMT_Q8_0));
   else if (gq_fmt_is_q6k(l.fmt)) GQ_TRY(GQ_GU_F(GQ_FMT_Q6_K));
   else GQ_TRY(GQ_GU_F(GQ_FMT_Q4_K));
 #undef GQ_GU_F
-  if (!few) GQ_TRY(gq_launch_a_to_f16(h, GQ_DT_F32, h16, hs, M * l.top_k, (int)l.N, ldh, q4d, s));
-#define GQ_DOWN_F(F) launch_down_t<F>(l, h, h16, ldh, hs, plan, resid, y, dt, M, w.maxblk, s)
-  if (l.fmt_down == GQ_FMT_Q4_0) return GQ_DOWN_F(GQ_FMT_Q4_0);
-  if (l.fmt_down == GQ_FMT_Q8_0) return GQ_DOWN_F(GQ_FMT_Q8_0);
-  if (gq_fmt_is_q6k(l.fmt_down)) return GQ_DOWN_F(GQ_FMT_Q6_K);
-  return GQ_DOWN_F(GQ_FMT_Q4_K);
+  if (!moe_few(M))
+    GQ_TRY(gq_launch_a_to_f16(b.h, GQ_DT_F32, b.h16, b.hs, M * l.top_k, (int)l.N, b.ldh,
+                              l.fmt_down == GQ_FMT_Q4_0 || gq_fmt_is_q4k(l.fmt_down), s));
+#define GQ_DOWN_F(F) launch_down_t<F>(l, plan, b, resid, y, dt, M, s)
+  if (l.fmt_down == GQ_FMT_Q4_0) GQ_TRY(GQ_DOWN_F(GQ_FMT_Q4_0));
+  else if (l.fmt_down == GQ_FMT_Q8_0) GQ_TRY(GQ_DOWN_F(GQ_FMT_Q8_0));
+  else if (gq_fmt_is_q6k(l.fmt_down)) GQ_TRY(GQ_DOWN_F(GQ_FMT_Q6_K));
+  else GQ_TRY(GQ_DOWN_F(GQ_FMT_Q4_K));
 #undef GQ_DOWN_F
+  if (b.parts == 1) return GQ_OK;
+  const int n = M * (int)l.K;
+  hipLaunchKernelGGL(k_moe_sum, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, s, b.part, resid, y, dt, n, b.parts);
+  return gq_last_launch();
 }
 
 // The workspace of a call: the caller's, or scratch memory of its own
@@ -844,7 +945,7 @@ extern "C" int gq_moe_route(const gq_moe *l, const void *x, int x_dtype, int32_t
   hipStream_t s = (hipStream_t)stream;
   MoeRoom room(ws, ws_bytes, M * l->n_experts * 8, s);
   GQ_TRY(room.status);
-  return launch_route(*l, x, x_dtype, (int)M, (double *)room.ptr, ids, weights, MoePlan{}, s);
+  return launch_route(*l, x, x_dtype, (int)M, (double *)room.ptr, MoeConv{}, ids, weights, MoePlan{}, s);
 }
 
 extern "C" int gq_moe_ffn(const gq_moe *l, const void *x, int x_dtype, const int32_t *ids, const float *weights,
@@ -858,8 +959,11 @@ extern "C" int gq_moe_ffn(const gq_moe *l, const void *x, int x_dtype, const int
   MoeRoom room(ws, ws_bytes, w.bytes, s);
   GQ_TRY(room.status);
   const MoePlan plan = plan_of(w, room.ptr);
+  const MoeMid mid = moe_mid(*l, w, room.ptr, (int)M);
   GQ_TRY(launch_plan(*l, RouteArgs{}, (const int *)ids, weights, plan, (int)M, s));
-  return moe_ffn(*l, x, x_dtype, plan, w, room.ptr, resid, y, y_dtype, (int)M, s);
+  if (!moe_as_it_is(x, x_dtype, (int)M))
+    GQ_TRY(gq_launch_a_to_f16(x, x_dtype, mid.a16, mid.rs, (int)M, (int)l->K, mid.lda, moe_x_order(*l, (int)M), s));
+  return moe_products(*l, x, x_dtype, plan, mid, resid, y, y_dtype, (int)M, s);
 }
 
 extern "C" int gq_moe_layer(const gq_moe *l, const void *x, int x_dtype, const void *resid, void *y, int y_dtype, int32_t *ids,
@@ -873,6 +977,11 @@ extern "C" int gq_moe_layer(const gq_moe *l, const void *x, int x_dtype, const v
   MoeRoom room(ws, ws_bytes, w.bytes, s);
   GQ_TRY(room.status);
   const MoePlan plan = plan_of(w, room.ptr);
-  GQ_TRY(launch_route(*l, x, x_dtype, (int)M, (double *)(room.ptr + w.logits), ids, weights, plan, s));
-  return moe_ffn(*l, x, x_dtype, plan, w, room.ptr, resid, y, y_dtype, (int)M, s);
+  const MoeMid mid = moe_mid(*l, w, room.ptr, (int)M);
+  const MoeConv conv = moe_as_it_is(x, x_dtype, (int)M) ? MoeConv{} : MoeConv{mid.a16, mid.rs, mid.lda, moe_x_order(*l, (int)M)};
+  // (the choice passes through memory where it has a launch of its own)
+  if (!ids) ids = (int32_t *)(room.ptr + w.ids);
+  if (!weights) weights = (float *)(room.ptr + w.weights);
+  GQ_TRY(launch_route(*l, x, x_dtype, (int)M, (double *)(room.ptr + w.logits), conv, ids, weights, plan, s));
+  return moe_products(*l, x, x_dtype, plan, mid, resid, y, y_dtype, (int)M, s);
 }
