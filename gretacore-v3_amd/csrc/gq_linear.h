@@ -29,14 +29,18 @@ GQ_DEV float lin_act_d(int act, float z) {
   gq_act_fd(act, z, f, d);
   return d;
 }
-// output (m, n) of a product's sum v
-GQ_DEV void lin_put(const LinEpi &e, size_t m, int n, int N, float v) {
+// bias and residual of output (m, n), loaded ahead of the sums; the output of a product's sum v
+struct LinTail {
+  float bias, resid;
+};
+GQ_DEV LinTail lin_tail(const LinEpi &e, size_t m, int n, int N) {
+  return LinTail{e.bias ? gq_ld_dt(e.bias, e.bias_dt, n) : 0.f, e.resid ? gq_ld_dt(e.resid, e.dt, m * (size_t)N + n) : 0.f};
+}
+GQ_DEV void lin_put(const LinEpi &e, size_t m, int n, int N, float v, const LinTail &t) {
   const size_t i = m * (size_t)N + n;
-  if (e.bias) v += gq_ld_dt(e.bias, e.bias_dt, n);
+  v += t.bias;
   if (e.z) gq_st_dt(e.z, e.dt, i, v);
-  float y = lin_act(e.act, v);
-  if (e.resid) y += gq_ld_dt(e.resid, e.dt, i);
-  gq_st_dt(e.y, e.dt, i, y);
+  gq_st_dt(e.y, e.dt, i, lin_act(e.act, v) + t.resid);
 }
 
 }  // namespace

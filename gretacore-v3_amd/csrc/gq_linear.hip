@@ -1,6 +1,7 @@
 // gq_linear.hip -- the product with bias, activation and residual in its epilogue over T16 weights,
 // any number of rows (few rows here, tiles in gq_linear_rb.hip), and its backward pass.
 #include <algorithm>
+#include <stdlib.h>
 #include <type_traits>
 
 #include "gq_internal.h"
@@ -12,18 +13,46 @@ namespace {
 // ---- forward: up to 64 rows, units of 128 k ------------------------------------------
 // The weights' bytes bound these: a workgroup takes R row tiles, its KS waves share K unit by unit with PD units in
 // flight each, and their sums are added through LDS.
-template <int KS, int R, typename At>
-GQ_DEV void lin_out(At at, const float *rs, const LinEpi &e, int M, int N, int block) {
-  for (int o = threadIdx.x; o < 16 * R * M; o += 64 * KS) {
-    const int nl = o % (16 * R), m = o / (16 * R), n = 16 * R * block + nl;
-    float y = 0.f;
+// Outputs of R tiles and up to ROWS rows, several a thread: their biases and residuals (which may be y, and are read before any
+// output is written) are loaded first of all, so that nothing waits for them at the end.
+template <int KS, int R, int ROWS>
+struct LinOut {
+  static constexpr int EACH = (16 * R * ROWS + 64 * KS - 1) / (64 * KS);
+  LinTail t[EACH];
+  __device__ __forceinline__ void ahead(const LinEpi &e, int M, int N, int block) {
 #pragma unroll
-    for (int k = 0; k < KS; ++k) y += at(k, nl >> 4, nl & 15, m);
-    if (n < N) lin_put(e, (size_t)m, n, N, rs ? y * rs[m] : y);
+    for (int i = 0; i < EACH; ++i) {
+      const int o = threadIdx.x + 64 * KS * i, m = o / (16 * R), n = 16 * R * block + o % (16 * R);
+      t[i] = m < M && n < N ? lin_tail(e, m, n, N) : LinTail{0.f, 0.f};
+    }
   }
-}
+  template <typename At>
+  __device__ __forceinline__ void put(At at, const float *rs, const LinEpi &e, int M, int N, int block) {
+#pragma unroll
+    for (int i = 0; i < EACH; ++i) {
+      const int o = threadIdx.x + 64 * KS * i, nl = o % (16 * R), m = o / (16 * R), n = 16 * R * block + nl;
+      if (m >= M || n >= N) continue;
+      float y = 0.f;
+#pragma unroll
+      for (int k = 0; k < KS; ++k) y += at(k, nl >> 4, nl & 15, m);
+      lin_put(e, m, n, N, rs ? y * rs[m] : y, t[i]);
+    }
+  }
+  // a part's sums, fp32 [M][N]
+  template <typename At>
+  __device__ __forceinline__ void put_part(At at, const float *rs, float *part, int M, int N, int block) {
+    for (int o = threadIdx.x; o < 16 * R * M; o += 64 * KS) {
+      const int nl = o % (16 * R), m = o / (16 * R), n = 16 * R * block + nl;
+      if (n >= N) continue;
+      float y = 0.f;
+#pragma unroll
+      for (int k = 0; k < KS; ++k) y += at(k, nl >> 4, nl & 15, m);
+      part[(size_t)m * (size_t)N + n] = y * rs[m];
+    }
+  }
+};
 
-// Up to 4 rows of 16-bit x: codes and x as they are, scales in fp32 (gq_rows_frag.h)
+// Up to 4 rows of 16-bit x: codes and x as they are, scales in fp32 (gq_rows_frag.h), x through LDS
 template <int FMT, int XT, int MR, int R, int KS, int PD>
 __global__ void __launch_bounds__(64 * KS)
 k_lin_few(const uint8_t *__restrict__ w, size_t sc_off, const void *__restrict__ x, const float *__restrict__ rs, LinEpi e,
@@ -31,7 +60,8 @@ k_lin_few(const uint8_t *__restrict__ w, size_t sc_off, const void *__restrict__
   constexpr int NG = kFewGroups<FMT>;
   constexpr float OFF = kFewOff<FMT, XT>;
   __shared__ float red[KS][R][MR][64];
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  extern __shared__ __attribute__((aligned(16))) uint8_t xs_s[];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int g = lane >> 4, ntiles = (int)gq_tiles(N);
   FTile<FMT> tl[R];
 #pragma unroll
@@ -39,18 +69,13 @@ k_lin_few(const uint8_t *__restrict__ w, size_t sc_off, const void *__restrict__
     const int tile = (int)blockIdx.x * R + t;
     tl[t] = ftile<FMT>(w, sc_off, (size_t)(tile < ntiles ? tile : ntiles - 1), C);  // (clamped: not stored)
   }
-  const __amdgpu_buffer_rsrc_t xr =
-      __builtin_amdgcn_make_buffer_rsrc(const_cast<void *>(x), (short)0, (int)(2u * (uint32_t)M * (uint32_t)K), 0x00020000);
-  const int xrow = lane & 3, xk = 64 * ((lane >> 3) & 1) + 16 * g + 8 * ((lane >> 2) & 1);
+  const int np = 128 * units, stride = (int)few_lds_stride(np);
+  const bool mine = few_mine<FMT>(lane) && (lane & 3) < M;
+  const uint32_t x0 = mine ? (uint32_t)((lane & 3) * stride + 32 * g) : (uint32_t)(M * stride), xd = mine ? 256u : 0u;
   FUnit<FMT> us[PD][R];
-  gq_u4 xs[PD];
   auto request = [&](int unit, int st) __attribute__((always_inline)) {
 #pragma unroll
     for (int t = 0; t < R; ++t) load_unit<FMT>(tl[t], unit, lane, us[st][t]);
-    const uint32_t k = 128u * (uint32_t)unit + (uint32_t)xk;  // (K is whole 32-blocks: a run is wholly in or out)
-    const bool in = xrow < M && k < (uint32_t)K;
-    const auto v = __builtin_amdgcn_raw_buffer_load_b128(xr, in ? 2u * ((uint32_t)xrow * (uint32_t)K + k) : 0xFFFFFFF0u, 0, 0);
-    xs[st] = gq_u4{v[0], v[1], v[2], v[3]};
   };
   float acc[R][MR] = {};
   uint32_t mg;  // (kept in a register)
@@ -60,13 +85,13 @@ k_lin_few(const uint8_t *__restrict__ w, size_t sc_off, const void *__restrict__
   const gq_u4 ones = {one, one, one, one};
   const gq_f4 zero = {0.f, 0.f, 0.f, 0.f};
   auto compute = [&](int unit, int st) __attribute__((always_inline)) {
-    const gq_u4 xv = kNibOrder<FMT> ? nib_order(xs[st]) : xs[st];
+    const uint32_t at = x0 + xd * (uint32_t)unit;
     float s[R][2], mn[R][2];
 #pragma unroll
     for (int t = 0; t < R; ++t) few_scales<FMT>(us[st][t], unit, g & (NG - 1), s[t], mn[t]);
-    auto step = [&](auto mc) __attribute__((always_inline)) {
-      constexpr int m = decltype(mc)::value;
-      const gq_u4 a0 = few_operand<NG, 2 * m>(xv), a1 = few_operand<NG, 2 * m + 1>(xv);
+#pragma unroll
+    for (int m = 0; m < 2; ++m) {
+      const gq_u4 a0 = few_lds(xs_s, at, m, 0), a1 = few_lds(xs_s, at, m, 1);
       gq_f4 sx = zero;
       if constexpr (OFF != 0.f || FMT == GQ_FMT_Q4_K) sx = few_mfma<XT>(a1, ones, few_mfma<XT>(a0, ones, zero));
 #pragma unroll
@@ -81,17 +106,21 @@ k_lin_few(const uint8_t *__restrict__ w, size_t sc_off, const void *__restrict__
           else acc[t][v] = fmaf(s[t][m], OFF != 0.f ? fmaf(-OFF, sx[v], d[v]) : d[v], acc[t][v]);
         }
       }
-    };
-    step(std::integral_constant<int, 0>{});
-    step(std::integral_constant<int, 1>{});
+    }
   };
-  walk_units<PD, KS>(units, wave, request, compute);
+  LinOut<KS, R, MR> out;
+  out.ahead(e, M, N, (int)blockIdx.x);
+  // (x's loads go out before the weights': behind them they would wait for theirs)
+  few_stage<64 * KS>(x, M, K, np, stride, kNibOrder<FMT>, xs_s, tid,
+                     [&]() __attribute__((always_inline)) { walk_requests<PD, KS>(units, wave, request); });
+  step_barrier<63>();  // (of LDS alone)
+  walk_computes<PD, KS>(units, wave, request, compute);
 #pragma unroll
   for (int t = 0; t < R; ++t)
 #pragma unroll
     for (int v = 0; v < MR; ++v) red[wave][t][v][lane] = acc[t][v];
   __syncthreads();
-  lin_out<KS, R>(
+  out.put(
       [&](int k, int t, int n, int m) {
         float y = 0.f;
 #pragma unroll
@@ -105,8 +134,9 @@ k_lin_few(const uint8_t *__restrict__ w, size_t sc_off, const void *__restrict__
 template <int FMT, int MT, int R, int KS, int PD>
 __global__ void __launch_bounds__(64 * KS)
 k_lin_rows(const uint8_t *__restrict__ w, size_t sc_off, const _Float16 *__restrict__ a16, int lda,
-           const float *__restrict__ rs, LinEpi e, int M, int N, int C, int units) {
+           const float *__restrict__ rs, LinEpi e, float *__restrict__ part, int M, int N, int C, int units) {
   __shared__ gq_f4 red[KS][R][MT][64];
+  const int u0 = units * (int)blockIdx.y / (int)gridDim.y, un = units * ((int)blockIdx.y + 1) / (int)gridDim.y - u0;  // this part's
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int g = lane >> 4, r = lane & 15, ntiles = (int)gq_tiles(N);
   FTile<FMT> tl[R];
@@ -127,10 +157,10 @@ k_lin_rows(const uint8_t *__restrict__ w, size_t sc_off, const _Float16 *__restr
   gq_half8 xs[PD][MT][4];
   auto request = [&](int unit, int st) __attribute__((always_inline)) {
 #pragma unroll
-    for (int t = 0; t < R; ++t) load_unit<FMT>(tl[t], unit, lane, us[st][t]);
+    for (int t = 0; t < R; ++t) load_unit<FMT>(tl[t], unit < un ? u0 + unit : units, lane, us[st][t]);
 #pragma unroll
     for (int t = 0; t < MT; ++t) {
-      const uint32_t o = unit < units ? xo[t] + 256u * (uint32_t)unit : 0xFFFFFF00u;
+      const uint32_t o = unit < un ? xo[t] + 256u * (uint32_t)(u0 + unit) : 0xFFFFFF00u;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const auto v = __builtin_amdgcn_raw_buffer_load_b128(xr, o + 128u * (i >> 1) + 16u * (i & 1), 0, 0);
@@ -146,52 +176,90 @@ k_lin_rows(const uint8_t *__restrict__ w, size_t sc_off, const _Float16 *__restr
   const uint32_t mg = gq_nib_magic();
   auto compute = [&](int unit, int st) __attribute__((always_inline)) {
 #pragma unroll
-    for (int t = 0; t < R; ++t) rows_add<FMT, MT>(us[st][t], unit, g, mg, xs[st], acc[t]);
+    for (int t = 0; t < R; ++t) rows_add<FMT, MT>(us[st][t], u0 + unit, g, mg, xs[st], acc[t]);
   };
-  walk_units<PD, KS>(units, wave, request, compute);
+  LinOut<KS, R, 16 * MT> out;
+  if (!part) out.ahead(e, M, N, (int)blockIdx.x);
+  walk_units<PD, KS>(un, wave, request, compute);
 #pragma unroll
   for (int t = 0; t < R; ++t)
 #pragma unroll
     for (int i = 0; i < MT; ++i) red[wave][t][i][lane] = acc[t][i];
   __syncthreads();
-  lin_out<KS, R>(
-      [&](int k, int t, int n, int m) {
-        return reinterpret_cast<const float *>(&red[k][t][m >> 4][16 * ((m >> 2) & 3) + n])[m & 3];
-      },
-      rs, e, M, N, (int)blockIdx.x);
+  auto at = [&](int k, int t, int n, int m) {
+    return reinterpret_cast<const float *>(&red[k][t][m >> 4][16 * ((m >> 2) & 3) + n])[m & 3];
+  };
+  if (part) out.put_part(at, rs, part + (size_t)blockIdx.y * (size_t)M * (size_t)N, M, N, (int)blockIdx.x);
+  else out.put(at, rs, e, M, N, (int)blockIdx.x);
+}
+
+// the parts' sums, in their order, and the epilogue; a thread takes outputs of one row
+__global__ void __launch_bounds__(256) k_lin_sum(const float *__restrict__ part, LinEpi e, int M, int N, int parts) {
+  const int n = (int)blockIdx.x * 256 + (int)threadIdx.x, m = (int)blockIdx.y;
+  if (n >= N) return;
+  const LinTail t = lin_tail(e, m, n, N);
+  float v = 0.f;
+  for (int p = 0; p < parts; ++p) v += part[((size_t)p * M + m) * (size_t)N + n];
+  lin_put(e, m, n, N, v, t);
+}
+int launch_sum(const float *part, const LinEpi &e, int M, int N, int parts, hipStream_t s) {
+  hipLaunchKernelGGL(k_lin_sum, dim3((unsigned)((N + 255) / 256), (unsigned)M), dim3(256), 0, s, part, e, M, N, parts);
+  return gq_last_launch();
 }
 
 template <int FMT, int XT>
 int launch_few_t(const void *w, const void *x, const float *rs, const LinEpi &e, int M, int N, int K, hipStream_t s) {
   const int units = (int)(gq_kpad(FMT, K) / 128);
-  const size_t tiles = gq_tiles(N);
+  const size_t tiles = gq_tiles(N), lds = few_lds_bytes(M, 128 * (size_t)units);
 #define GQ_FEW(MR, R, KS, PD)                                                                                               \
-  hipLaunchKernelGGL((k_lin_few<FMT, XT, MR, R, KS, PD>), dim3((unsigned)((tiles + (R)-1) / (R))), dim3(64 * (KS)), 0, s,     \
+  hipLaunchKernelGGL((k_lin_few<FMT, XT, MR, R, KS, PD>), dim3((unsigned)((tiles + (R)-1) / (R))), dim3(64 * (KS)), lds, s,   \
                      (const uint8_t *)w, gq_sc_plane_offset(FMT, N, K), x, rs, e, M, N, K, (int)gq_chunks(FMT, K), units)
 #define GQ_FEW_M(R, KS, PD)           \
   do {                                \
     if (M == 1) GQ_FEW(1, R, KS, PD); \
     else GQ_FEW(4, R, KS, PD);        \
   } while (0)
-  if (tiles <= 512) GQ_FEW_M(1, 8, 4);
-  else GQ_FEW_M(2, 4, 3);
+  // (Q4_K, one row: 4096 x 14336 by one tile 9.6 us, by two 12.5; Q4_0 14336 x 4096 11.1 and 9.0)
+  if (tiles <= 320) GQ_FEW_M(1, 16, 2);
+  else GQ_FEW_M(2, 8, 2);
 #undef GQ_FEW_M
 #undef GQ_FEW
   return gq_last_launch();
 }
 template <int FMT>
-int launch_rows_t(const void *w, const _Float16 *a16, int lda, const float *rs, const LinEpi &e, int M, int N, int K,
+int launch_rows_t(const void *w, const _Float16 *a16, int lda, const float *rs, const LinEpi &e, float *part, int parts, int M, int N, int K,
                   hipStream_t s) {
   const int units = (int)(gq_kpad(FMT, K) / 128);
   const size_t tiles = gq_tiles(N);
 #define GQ_ROWS(MT, R, KS, PD)                                                                                              \
-  hipLaunchKernelGGL((k_lin_rows<FMT, MT, R, KS, PD>), dim3((unsigned)((tiles + (R)-1) / (R))), dim3(64 * (KS)), 0, s,        \
-                     (const uint8_t *)w, gq_sc_plane_offset(FMT, N, K), a16, lda, rs, e, M, N, (int)gq_chunks(FMT, K), units)
-  if (M > 32) GQ_ROWS(4, 1, 8, 2);
-  else if (M > 16) GQ_ROWS(2, 1, 8, 2);
-  else GQ_ROWS(1, 1, 8, 3);
+  hipLaunchKernelGGL((k_lin_rows<FMT, MT, R, KS, PD>), dim3((unsigned)((tiles + (R)-1) / (R)), (unsigned)parts), dim3(64 * (KS)), 0, s, \
+                     (const uint8_t *)w, gq_sc_plane_offset(FMT, N, K), a16, lda, rs, e, parts > 1 ? part : nullptr, M, N,   \
+                     (int)gq_chunks(FMT, K), units)
+  const char *ev = getenv("GQ_DEV"); const int v = ev ? atoi(ev) : 0;
+  if (M > 32) {
+    if (v == 1) GQ_ROWS(4, 2, 4, 2);
+    else if (v == 2) GQ_ROWS(4, 2, 4, 1);
+    else if (v == 3) GQ_ROWS(4, 2, 8, 1);
+    else if (v == 4) GQ_ROWS(4, 1, 4, 2);
+    else if (v == 5) GQ_ROWS(4, 1, 8, 1);
+    else GQ_ROWS(4, 1, 8, 2);
+  } else if (M > 16) {
+    if (v == 1) GQ_ROWS(2, 2, 4, 2);
+    else if (v == 2) GQ_ROWS(2, 2, 4, 1);
+    else if (v == 3) GQ_ROWS(2, 2, 8, 2);
+    else if (v == 4) GQ_ROWS(2, 1, 4, 2);
+    else if (v == 5) GQ_ROWS(2, 1, 4, 4);
+    else GQ_ROWS(2, 1, 8, 2);
+  } else {
+    if (v == 1) GQ_ROWS(1, 2, 4, 2);
+    else if (v == 2) GQ_ROWS(1, 2, 8, 2);
+    else if (v == 3) GQ_ROWS(1, 1, 8, 2);
+    else if (v == 4) GQ_ROWS(1, 1, 16, 2);
+    else GQ_ROWS(1, 1, 4, 4);
+  }
 #undef GQ_ROWS
-  return gq_last_launch();
+  GQ_TRY(gq_last_launch());
+  return parts > 1 ? launch_sum(part, e, M, N, parts, s) : GQ_OK;
 }
 
 // ---- backward ----------------------------------------------------------------------
@@ -358,6 +426,7 @@ int check_linear(int fmt, const void *w, size_t M, size_t N, size_t K, int act) 
 }
 
 constexpr size_t kFew = 4, kRows = 64;
+constexpr size_t kFewLds = 65536;  // values of x that LDS takes beside the waves' sums
 // Rows a call takes at a time: their fp16 copies stay below 64 MiB, but for the rows that the kernels of few rows take at
 // once (64 of at most 2^24 columns: 2 GiB, 32-bit offsets still)
 size_t linear_rows(int fmt, size_t M, size_t K) {
@@ -366,12 +435,18 @@ size_t linear_rows(int fmt, size_t M, size_t K) {
   return M < mb ? M : mb;
 }
 
+// Parts of K for rows that the kernels of few rows take
+int row_parts(size_t M, size_t N, size_t K, int units) {
+  const char *ev = getenv("GQ_PARTS");
+  return ev ? atoi(ev) : 1;
+}
+
 }  // namespace
 
 extern "C" size_t gq_linear_workspace_bytes(int fmt, size_t M, size_t N, size_t K) {
   if (!gq_fmt_valid(fmt) || M > GQ_MAX_DIM || N > GQ_MAX_DIM || K > GQ_MAX_DIM || K == 0) return 0;
   const size_t mb = linear_rows(fmt, M, K);
-  return gq_align256(mb * (gq_kpad(fmt, K) + 8) * 2) + gq_align256((mb + 256) * 4);
+  return gq_align256(mb * (gq_kpad(fmt, K) + 8) * 2) + gq_align256((mb + 256) * 4) + (M <= 64 ? 8 * M * N * 4 : 0);
 }
 
 extern "C" int gq_linear(int fmt, const void *w, const void *x, int x_dtype, const void *bias, int bias_dtype, int act,
@@ -394,7 +469,8 @@ extern "C" int gq_linear(int fmt, const void *w, const void *x, int x_dtype, con
     return GQ_FMT_X(GQ_FMT_Q4_K);
 #undef GQ_FMT_X
   };
-  if (M <= kFew && x_dtype != GQ_DT_F32 && (uintptr_t)x % 4 == 0) return few(x, x_dtype, nullptr);
+  const bool is_few = M <= kFew && M * gq_kpad(fmt, K) <= kFewLds;
+  if (is_few && x_dtype != GQ_DT_F32) return few(x, x_dtype, nullptr);
   const size_t need = gq_linear_workspace_bytes(fmt, M, N, K), mb = linear_rows(fmt, M, K), Kp = gq_kpad(fmt, K);
   GqScratch sc(ws ? 0 : need, s);
   if (ws) GQ_CHECK(ws_bytes >= need, GQ_ERR_WORKSPACE);
@@ -404,14 +480,16 @@ extern "C" int gq_linear(int fmt, const void *w, const void *x, int x_dtype, con
   _Float16 *a16 = (_Float16 *)ws;
   float *rs = (float *)((uint8_t *)ws + gq_align256(mb * (Kp + 8) * 2));
   const int q4 = fmt == GQ_FMT_Q4_0 || gq_fmt_is_q4k(fmt);
-  if (M <= kFew) {  // (x in fp32, or at an odd address)
+  if (is_few) {
     GQ_TRY(gq_launch_a_to_f16(x, x_dtype, a16, rs, (int)M, (int)K, (int)K, 0, s));
     return few(a16, GQ_DT_F16, rs);
   }
   if (M <= kRows) {  // rows 16 bytes longer than a multiple of 4 KiB, where 16 of them would collide
     const int ld = (int)Kp + 8;
     GQ_TRY(gq_launch_a_to_f16(x, x_dtype, a16, rs, (int)M, (int)K, ld, q4, s));
-#define GQ_ROWS_F(F) launch_rows_t<F>(w, a16, ld, rs, e, (int)M, (int)N, (int)K, s)
+    float *part = (float *)((uint8_t *)rs + gq_align256((mb + 256) * 4));
+    const int parts = row_parts(M, N, K, (int)(Kp / 128));
+#define GQ_ROWS_F(F) launch_rows_t<F>(w, a16, ld, rs, e, part, parts, (int)M, (int)N, (int)K, s)
     if (fmt == GQ_FMT_Q4_0) return GQ_ROWS_F(GQ_FMT_Q4_0);
     if (fmt == GQ_FMT_Q8_0) return GQ_ROWS_F(GQ_FMT_Q8_0);
     if (gq_fmt_is_q6k(fmt)) return GQ_ROWS_F(GQ_FMT_Q6_K);

@@ -13,21 +13,21 @@
 #include "gq_internal.h"
 #include "gq_rows_frag.h"
 
+#define GQ_DEV_M __device__ __forceinline__
+
 namespace {
 
 constexpr int kMoeFew = 4;  // tokens that the kernels of few rows take
 
-// A block of an expert's work: up to 16 of its pairs (token * top + slot); few tokens (M <= 4): pair[m] is token m's, -1 none,
-// and w[m] its weight.  expert -1: no block.
+// A block of an expert's work: up to 16 of its pairs (token * top + slot).  expert -1: no block.
 struct MoeBlk {
   int expert, count;
   int pair[16];
-  float w[kMoeFew];
 };
 struct MoePlan {
   int *nblk;
   MoeBlk *blk;  // [maxblk], the blocks that there are first
-  float *wsum;  // [pair] the weight (of the first pair of an expert that a token names twice: their sum); not for few tokens
+  float *wsum;  // [pair] the weight (of the first pair of an expert that a token names twice: their sum)
   int maxblk;
 };
 
@@ -141,13 +141,14 @@ GQ_DEV double lane_d(double v, int lane) {  // (lane: the same in all lanes)
   const uint32_t hi = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(b >> 32), lane);
   return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
 }
+constexpr int kFewNE = 2;  // experts a lane of the choice within k_moe_gu_few
 // One wave chooses the experts of token m; lane j writes slot j (ids_s: in LDS, at the token's place).  A key is a 64-bit number in the values' order, 0 what is
 // never taken (-Inf, none there, taken before): the largest's high word, then its low word, then the lowest
 // expert that has both.
 template <int NE>
 GQ_DEV void moe_choose(const RouteArgs &a, int m, int E, int top, int lane, int *ids_s, float *w_s) {
   const double ninf = -__builtin_inf();
-  const bool sm = a.score == GQ_MOE_SOFTMAX;
+  const bool sm = a.score == GQ_MOE_SOFTMAX, weighed = w_s || a.weights;  // (else the ids alone)
   double l[NE], lmax = ninf, sum = 0.0;
 #pragma unroll
   for (int i = 0; i < NE; ++i) {
@@ -155,7 +156,7 @@ GQ_DEV void moe_choose(const RouteArgs &a, int m, int E, int top, int lane, int 
     l[i] = e < E ? a.logits[(size_t)m * E + e] : ninf;
     lmax = fmax(lmax, l[i]);  // (of those that are numbers)
   }
-  if (sm) {
+  if (sm && (weighed || a.bias)) {
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) lmax = fmax(lmax, __shfl_xor(lmax, o, 64));
     if (!a.renorm || a.bias) {  // (renormalised weights do without the sum over all experts)
@@ -188,13 +189,19 @@ GQ_DEV void moe_choose(const RouteArgs &a, int m, int E, int top, int lane, int 
     for (int i = 0; i < NE; ++i) h = max(h, kh[i]);
     const uint32_t mh = wave_max(h);
     if (mh == 0) break;
+    int same = 0;
 #pragma unroll
-    for (int i = 0; i < NE; ++i) w = max(w, kh[i] == mh ? kl[i] : 0u);
-    const uint32_t mw = wave_max(w);
+    for (int i = 0; i < NE; ++i) same += __builtin_popcountll(__ballot(kh[i] == mh));
+    uint32_t mw = 0;
+    if (same > 1) {  // (low words count)
+#pragma unroll
+      for (int i = 0; i < NE; ++i) w = max(w, kh[i] == mh ? kl[i] : 0u);
+      mw = wave_max(w);
+    }
     bool found = false;
 #pragma unroll
     for (int i = 0; i < NE; ++i) {
-      const uint64_t at = found ? 0 : __ballot(kh[i] == mh && kl[i] == mw);
+      const uint64_t at = found ? 0 : __ballot(kh[i] == mh && kl[i] >= mw);
       if (at == 0) continue;
       found = true;
       const int ln = __builtin_ctzll(at);
@@ -206,6 +213,11 @@ GQ_DEV void moe_choose(const RouteArgs &a, int m, int E, int top, int lane, int 
       }
     }
   }
+  if (lane < top) {
+    if (ids_s) ids_s[m * top + lane] = id;
+    if (a.ids) a.ids[m * top + lane] = id;
+  }
+  if (!weighed) return;
   double w = id < 0 ? 0.0 : score(mine), total = 0.0;
   if (a.renorm) {
     for (int j = 0; j < top; ++j) total += lane_d(w, j);
@@ -213,11 +225,7 @@ GQ_DEV void moe_choose(const RouteArgs &a, int m, int E, int top, int lane, int 
   }
   if (lane < top) {
     const float f = id < 0 ? 0.f : (float)(w * (double)a.scale);
-    if (ids_s) {
-      ids_s[m * top + lane] = id;
-      w_s[m * top + lane] = f;
-    }
-    if (a.ids) a.ids[m * top + lane] = id;
+    if (w_s) w_s[m * top + lane] = f;
     if (a.weights) a.weights[m * top + lane] = f;
   }
 }
@@ -228,21 +236,19 @@ __global__ void __launch_bounds__(64) k_moe_choose(RouteArgs a, int E, int top) 
 }
 
 // ---- plan: one workgroup ------------------------------------------------------------
-// The choice (NE: experts a lane; 0: ids and weights are given), each expert's pairs in order of their tokens, in blocks of `per`.
+// The choice (NE: experts a lane; 0: ids and weights are given), each expert's pairs in order of their tokens, in blocks of 16.
 // Ids outside 0 .. E - 1 name no expert; an expert that a token names twice gets one pair with both weights.
-constexpr int kPlanThreads = 1024;
+constexpr int kPlanThreads = 1024, kBlkRows = 16;
 template <int NE>
 __global__ void __launch_bounds__(kPlanThreads) k_moe_plan(RouteArgs a, const int *__restrict__ ids, const float *__restrict__ weights,
-                                                           MoePlan p, int M, int E, int top, int per) {
-  constexpr int MP = GQ_MOE_MAX_TOKENS * GQ_MOE_MAX_TOP, FB = kMoeFew * GQ_MOE_MAX_TOP;
+                                                           MoePlan p, int M, int E, int top) {
+  constexpr int MP = GQ_MOE_MAX_TOKENS * GQ_MOE_MAX_TOP;
   static_assert(MP <= kPlanThreads && GQ_MOE_MAX_EXPERTS <= kPlanThreads, "a thread a pair, a thread an expert");
-  __shared__ int id_s[MP], base_s[kPlanThreads], tot_s[kPlanThreads / 64], pair_s[FB][kMoeFew];
+  __shared__ int id_s[MP], base_s[kPlanThreads], tot_s[kPlanThreads / 64];
   __shared__ uint32_t tok_s[2][kPlanThreads];  // the tokens of an expert, a bit each
-  __shared__ float w_s[MP], wsum_s[FB];
+  __shared__ float w_s[MP];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, P = M * top;
-  const bool few = M <= kMoeFew;
   tok_s[0][tid] = tok_s[1][tid] = 0;
-  if (tid < FB * kMoeFew) pair_s[tid / kMoeFew][tid % kMoeFew] = -1;
   if constexpr (NE > 0) {
     for (int m = wave; m < M; m += kPlanThreads / 64) moe_choose<NE>(a, m, E, top, lane, id_s, w_s);
   } else if (tid < P) {
@@ -264,12 +270,11 @@ __global__ void __launch_bounds__(kPlanThreads) k_moe_plan(RouteArgs a, const in
         else w += w_s[j];
       }
     }
-    if (few) wsum_s[tid] = w;
-    else p.wsum[tid] = w;
+    p.wsum[tid] = w;
     if (id >= 0) atomicOr(&tok_s[tok >> 5][id], 1u << (tok & 31));
   }
   __syncthreads();
-  const int c = __popc(tok_s[0][tid]) + __popc(tok_s[1][tid]), nb = (c + per - 1) / per;
+  const int c = __popc(tok_s[0][tid]) + __popc(tok_s[1][tid]), nb = (c + kBlkRows - 1) / kBlkRows;
   int inc = nb;
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) {
@@ -288,7 +293,7 @@ __global__ void __launch_bounds__(kPlanThreads) k_moe_plan(RouteArgs a, const in
   base_s[tid] = base;
   for (int b = 0; b < nb; ++b) {
     p.blk[base + b].expert = tid;
-    p.blk[base + b].count = c - per * b < per ? c - per * b : per;
+    p.blk[base + b].count = min(c - kBlkRows * b, kBlkRows);
   }
   for (int b = all + tid; b < p.maxblk; b += kPlanThreads) p.blk[b].expert = -1;
   if (tid == 0) *p.nblk = all;
@@ -296,17 +301,25 @@ __global__ void __launch_bounds__(kPlanThreads) k_moe_plan(RouteArgs a, const in
   if (id >= 0) {
     const uint32_t below = (1u << (tok & 31)) - 1u, w0 = tok_s[0][id], w1 = tok_s[1][id];
     const int rank = tok < 32 ? __popc(w0 & below) : __popc(w0) + __popc(w1 & below);
-    if (few) pair_s[base_s[id]][tok] = tid;
-    else p.blk[base_s[id] + rank / per].pair[rank % per] = tid;
-  }
-  if (!few) return;
-  __syncthreads();
-  if (tid < all * kMoeFew) {
-    const int b = tid / kMoeFew, m = tid % kMoeFew, q = pair_s[b][m];
-    p.blk[b].pair[m] = q;
-    p.blk[b].w[m] = q < 0 ? 0.f : wsum_s[q];
+    p.blk[base_s[id] + rank / kBlkRows].pair[rank % kBlkRows] = tid;
   }
 }
+
+// ---- few tokens: no plan --------------------------------------------------------------
+// At most 64 pairs, a lane each.  An expert's block is that of the first pair that names it; row m is token m's first pair with it (-1:
+// none), with the weights of all of that token's.
+struct FewPairs {
+  int id;       // this lane's pair
+  uint64_t of;  // the pairs of the expert asked for
+  GQ_DEV_M int expert(int q) const { return __builtin_amdgcn_readlane(id, q); }
+  GQ_DEV_M bool leads(int q) {  // is q the first of its expert's
+    const int e = expert(q);
+    of = e < 0 ? 0 : __ballot(id == e);
+    return e >= 0 && __builtin_ctzll(of) == q;
+  }
+  GQ_DEV_M uint64_t mine(int m, int top) const { return of & (((1ull << top) - 1ull) << (m * top)); }
+  GQ_DEV_M int pair(int m, int top) const { return mine(m, top) ? __builtin_ctzll(mine(m, top)) : -1; }
+};
 
 // ---- gate and up -----------------------------------------------------------------------
 // Output (m, 16 t + n) of the R tiles `group` in both matrices from the waves' parts at(k, w, t, n, m)
@@ -323,19 +336,34 @@ GQ_DEV float moe_gu_h(At at, int nl, int m, float f, int act) {
 // Up to 4 tokens of 16-bit x: codes and x as they are, scales in fp32 (gq_rows_frag.h); row j is token j.  h goes out in fp16 (nib:
 // in the nibbles' order) with a power-of-two scale for each 32 of a row, the scale groups of W_down's products; the inverse of block
 // 2 m + i of 128 values to hs[pair][128s][i][m].
-template <int FMT, int XT, int MR, int KS, int PD>
+// Workgroup (j, q): 32 columns of the expert that pair q names first.  ROUTE: the choice is made here, by every workgroup for itself (a
+// launch of its own cost XX us more); the first one keeps it.
+template <int FMT, int XT, int MR, int KS, int PD, bool ROUTE>
 __global__ void __launch_bounds__(64 * KS)
 k_moe_gu_few(const uint8_t *__restrict__ wg, const uint8_t *__restrict__ wu, size_t sc_off, const void *__restrict__ x,
-             const float *__restrict__ rs, MoePlan p, _Float16 *__restrict__ h, float *__restrict__ hs, int nib, int M, int N, int K,
-             int C, int units, int act, int top) {
+             const float *__restrict__ rs, RouteArgs a, const int *__restrict__ ids, _Float16 *__restrict__ h, float *__restrict__ hs,
+             int nib, int M, int N, int K, int C, int units, int act, int E, int top) {
+  static_assert(KS >= kMoeFew, "a wave a token");
   constexpr int NG = kFewGroups<FMT>, R = 2, T = 2 * R;
   constexpr float OFF = kFewOff<FMT, XT>;
   __shared__ float red[KS][T][MR][64];
-  const MoeBlk &blk = p.blk[blockIdx.y];
-  const int expert = __builtin_amdgcn_readfirstlane(blk.expert);
-  if (expert < 0) return;
+  extern __shared__ __attribute__((aligned(16))) uint8_t xs_s[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int g = lane >> 4, ntiles = N / 16;
+  const int np = 128 * units, stride = (int)few_lds_stride(np);
+  __shared__ int id_s[64];
+  few_stage<64 * KS>(x, M, K, np, stride, kNibOrder<FMT>, xs_s, (int)threadIdx.x, [&]() __attribute__((always_inline)) {
+    if constexpr (ROUTE) {  // (the weights are the first workgroup's alone)
+      if (blockIdx.x > 0 || blockIdx.y > 0) a.ids = nullptr, a.weights = nullptr;
+      if (wave < M) moe_choose<kFewNE>(a, wave, E, top, lane, id_s, nullptr);
+    }
+  });
+  __syncthreads();
+  FewPairs pairs;
+  pairs.id = lane < M * top ? (ROUTE ? id_s[lane] : ids[lane]) : -1;
+  if (pairs.id >= E) pairs.id = -1;
+  const int expert = pairs.expert((int)blockIdx.y);
+  if (!pairs.leads((int)blockIdx.y)) return;
   const size_t tile0 = (size_t)expert * (size_t)ntiles;
   FTile<FMT> tl[T];
 #pragma unroll
@@ -343,18 +371,12 @@ k_moe_gu_few(const uint8_t *__restrict__ wg, const uint8_t *__restrict__ wu, siz
     const int tile = (int)blockIdx.x * R + t % R;
     tl[t] = ftile<FMT>(t < R ? wg : wu, sc_off, tile0 + (size_t)(tile < ntiles ? tile : ntiles - 1), C);  // (clamped: not stored)
   }
-  const __amdgpu_buffer_rsrc_t xr =
-      __builtin_amdgcn_make_buffer_rsrc(const_cast<void *>(x), (short)0, (int)(2u * (uint32_t)M * (uint32_t)K), 0x00020000);
-  const int xrow = lane & 3, xk = 64 * ((lane >> 3) & 1) + 16 * g + 8 * ((lane >> 2) & 1);
+  const bool mine = few_mine<FMT>(lane) && (lane & 3) < M;
+  const uint32_t x0 = mine ? (uint32_t)((lane & 3) * stride + 32 * g) : (uint32_t)(M * stride), xd = mine ? 256u : 0u;
   FUnit<FMT> us[PD][T];
-  gq_u4 xs[PD];
   auto request = [&](int unit, int st) __attribute__((always_inline)) {
 #pragma unroll
     for (int t = 0; t < T; ++t) load_unit<FMT>(tl[t], unit, lane, us[st][t]);
-    const uint32_t k = 128u * (uint32_t)unit + (uint32_t)xk;  // (K is whole 32-blocks: a run is wholly in or out)
-    const bool in = xrow < M && k < (uint32_t)K;
-    const auto v = __builtin_amdgcn_raw_buffer_load_b128(xr, in ? 2u * ((uint32_t)xrow * (uint32_t)K + k) : 0xFFFFFFF0u, 0, 0);
-    xs[st] = gq_u4{v[0], v[1], v[2], v[3]};
   };
   float acc[T][MR] = {};
   uint32_t mg;  // (kept in a register)
@@ -364,13 +386,13 @@ k_moe_gu_few(const uint8_t *__restrict__ wg, const uint8_t *__restrict__ wu, siz
   const gq_u4 ones = {one, one, one, one};
   const gq_f4 zero = {0.f, 0.f, 0.f, 0.f};
   auto compute = [&](int unit, int st) __attribute__((always_inline)) {
-    const gq_u4 xv = kNibOrder<FMT> ? nib_order(xs[st]) : xs[st];
+    const uint32_t at = x0 + xd * (uint32_t)unit;
     float s[T][2], mn[T][2];
 #pragma unroll
     for (int t = 0; t < T; ++t) few_scales<FMT>(us[st][t], unit, g & (NG - 1), s[t], mn[t]);
-    auto step = [&](auto mc) __attribute__((always_inline)) {
-      constexpr int m = decltype(mc)::value;
-      const gq_u4 a0 = few_operand<NG, 2 * m>(xv), a1 = few_operand<NG, 2 * m + 1>(xv);
+#pragma unroll
+    for (int m = 0; m < 2; ++m) {
+      const gq_u4 a0 = few_lds(xs_s, at, m, 0), a1 = few_lds(xs_s, at, m, 1);
       gq_f4 sx = zero;
       if constexpr (OFF != 0.f || FMT == GQ_FMT_Q4_K) sx = few_mfma<XT>(a1, ones, few_mfma<XT>(a0, ones, zero));
 #pragma unroll
@@ -385,9 +407,7 @@ k_moe_gu_few(const uint8_t *__restrict__ wg, const uint8_t *__restrict__ wu, siz
           else acc[t][v] = fmaf(s[t][m], OFF != 0.f ? fmaf(-OFF, sx[v], d[v]) : d[v], acc[t][v]);
         }
       }
-    };
-    step(std::integral_constant<int, 0>{});
-    step(std::integral_constant<int, 1>{});
+    }
   };
   walk_units<PD, KS>(units, wave, request, compute);
 #pragma unroll
@@ -396,7 +416,7 @@ k_moe_gu_few(const uint8_t *__restrict__ wg, const uint8_t *__restrict__ wu, siz
     for (int v = 0; v < MR; ++v) red[wave][t][v][lane] = acc[t][v];
   __syncthreads();
   const int m = threadIdx.x >> 5, nl = threadIdx.x & 31, n0 = 32 * (int)blockIdx.x;  // (N is whole 32-blocks)
-  const int q = m < M ? blk.pair[m] : -1;
+  const int q = m < M ? pairs.pair(m, top) : -1;
   if (q < 0) return;  // (whole half-waves)
   const float v = moe_gu_h<KS, R>(
       [&](int k, int w, int t, int n, int mm) {
@@ -486,7 +506,7 @@ k_moe_gu_rows(const uint8_t *__restrict__ wg, const uint8_t *__restrict__ wu, si
 // (block by block, unit by unit), so that the sum over a token's experts stays in the workgroup, in one order.
 struct ItemAt {
   int b, u;
-  __device__ __forceinline__ void next(int by, int units) {
+  GQ_DEV_M void next(int by, int units) {
     u += by;
     while (u >= units) {
       u -= units;
@@ -494,75 +514,90 @@ struct ItemAt {
     }
   }
 };
-template <int PD, int KS, typename Request, typename Compute>
-GQ_DEV void walk_items(int b0, int nblk, int units, int wave, Request request, Compute compute) {
-  ItemAt rq = {b0, 0}, at;
-  rq.next(wave, units);
-  at = rq;
+// The items of a wave, PD requested ahead (rq: the next to request), and a group of PD at a time: a group requests the next
+// one's unless it is the last.
+template <int PD, int KS, typename Request>
+GQ_DEV void items_requests(ItemAt &rq, int units, Request request) {
 #pragma unroll
   for (int i = 0; i < PD; ++i) {
     request(rq, i);
     rq.next(KS, units);
   }
-  while (at.b < nblk) {
+}
+template <int PD, int KS, typename Request, typename Compute>
+GQ_DEV void items_computes(ItemAt at, ItemAt rq, int nblk, int units, Request request, Compute compute) {
+  while (rq.b < nblk) {
 #pragma unroll
     for (int i = 0; i < PD; ++i) {
-      if (at.b >= nblk) break;
       compute(at, i);
       at.next(KS, units);
       request(rq, i);
       rq.next(KS, units);
     }
   }
+#pragma unroll
+  for (int i = 0; i < PD; ++i) {
+    if (at.b < nblk) compute(at, i);
+    at.next(KS, units);
+  }
 }
 
-// Up to 4 tokens: rows are the tokens; the scale groups' fp32 sums take the inverse scales of h and the expert's weight.
+// Up to 4 tokens: rows are the tokens; the scale groups' fp32 sums take the inverse scales of h and the expert's weight.  h and its
+// scales go through LDS.
 template <int FMT, int MR, int KS, int PD>
 __global__ void __launch_bounds__(64 * KS)
-k_moe_down_few(const uint8_t *__restrict__ wd, size_t sc_off, const _Float16 *__restrict__ h, const float *__restrict__ hs, MoePlan p,
-               const void *resid, void *y, int dt, int M, int N, int K, int C, int units, int top) {
+k_moe_down_few(const uint8_t *__restrict__ wd, size_t sc_off, const _Float16 *__restrict__ h, const float *__restrict__ hs,
+               const int *__restrict__ ids, const float *__restrict__ weights, const void *resid, void *y, int dt, int M, int N, int K,
+               int C, int units, int E, int top) {
   constexpr int NG = kFewGroups<FMT>, XT = GQ_DT_F16, MB = kMoeFew * GQ_MOE_MAX_TOP;
   constexpr float OFF = kFewOff<FMT, XT>;
   __shared__ float red[KS][MR][64];
-  __shared__ int e_s[MB], p_s[MB][kMoeFew];
+  static_assert(MB <= 64, "a lane a pair");
+  __shared__ int p_s[MB][kMoeFew];
   __shared__ float w_s[MB][kMoeFew];
+  extern __shared__ __attribute__((aligned(16))) uint8_t xs_s[];  // [pair] rows of h, then [pair][unit][i][m] inverse scales
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int g = lane >> 4, ntiles = K / 16;
-  const int nblk = __builtin_amdgcn_readfirstlane(*p.nblk);
-  if (tid < p.maxblk) {  // (not nblk, which would have to arrive first)
-    e_s[tid] = p.blk[tid].expert;
+  // lane q: its expert's first pair of each token, and that token's weight; lane b then: block b's expert
+  int id = lane < M * top ? ids[lane] : -1;
+  if (id >= E) id = -1;
+  const float weight = lane < M * top ? weights[lane] : 0.f;
+  int pair[MR], lead = 64;
+  float w[MR];
 #pragma unroll
-    for (int m = 0; m < kMoeFew; ++m) {
-      p_s[tid][m] = p.blk[tid].pair[m];
-      w_s[tid][m] = p.blk[tid].w[m];
+  for (int m = 0; m < MR; ++m) {
+    pair[m] = -1;
+    w[m] = 0.f;
+    if (m >= M) continue;
+    for (int q = m * top; q < m * top + top; ++q) {
+      const bool same = __builtin_amdgcn_readlane(id, q) == id;
+      const float f = __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(weight), q));
+      if (same && pair[m] < 0) pair[m] = q;
+      if (same) w[m] += f;
     }
+    if (pair[m] >= 0) lead = min(lead, pair[m]);
   }
-  __syncthreads();
-  const __amdgpu_buffer_rsrc_t hr = __builtin_amdgcn_make_buffer_rsrc(
-      const_cast<_Float16 *>(h), (short)0, (int)(2u * (uint32_t)(M * top) * (uint32_t)N), 0x00020000);
-  const __amdgpu_buffer_rsrc_t sr = __builtin_amdgcn_make_buffer_rsrc(
-      const_cast<float *>(hs), (short)0, (int)(16u * (uint32_t)(M * top) * (uint32_t)units), 0x00020000);
-  const int xrow = lane & 3, xk = 64 * ((lane >> 3) & 1) + 16 * g + 8 * ((lane >> 2) & 1);
-  const uint32_t gi = NG == 2 ? (uint32_t)g & 1u : (uint32_t)g >> 1;  // the 32-block of a step that this lane's sums are of
+  const bool leads = id >= 0 && lead == lane;
+  const uint64_t all = __ballot(leads);
+  const int nblk = __builtin_popcountll(all), b0 = __builtin_popcountll(all & ((1ull << lane) - 1ull));
+  // (no two lanes to one place: the others go to the places behind the blocks, whose number is that of the lanes)
+  const int expert = __builtin_amdgcn_ds_permute(4 * (leads ? b0 : nblk + lane - b0), id);
+  if (tid < 64 && leads)
+#pragma unroll
+    for (int m = 0; m < MR; ++m) {
+      p_s[b0][m] = pair[m];
+      w_s[b0][m] = w[m];
+    }
+  const int np = 128 * units, stride = (int)few_lds_stride(np), P = M * top;
+  const bool mine = few_mine<FMT>(lane) && (lane & 3) < M;
+  const uint32_t zero_at = (uint32_t)(P * stride);
+  const float2 *f_s = reinterpret_cast<const float2 *>(xs_s + P * stride + 160);
+  const int gi = NG == 2 ? g & 1 : g >> 1;  // the 32-block of a step that this lane's sums are of
   FUnit<FMT> us[PD];
-  gq_u4 xs[PD];
-  float2 is[PD][MR];
   auto request = [&](const ItemAt &at, int st) __attribute__((always_inline)) {
     const bool on = at.b < nblk;
-    const int b = on ? at.b : 0;
-    const size_t tile = (size_t)__builtin_amdgcn_readfirstlane(e_s[b]) * (size_t)ntiles + blockIdx.x;
+    const size_t tile = (size_t)__builtin_amdgcn_readlane(expert, on ? at.b : 0) * (size_t)ntiles + blockIdx.x;
     load_unit<FMT>(ftile<FMT>(wd, sc_off, tile, on ? C : 0), at.u, lane, us[st]);
-    const int q = p_s[b][xrow], k = 128 * at.u + xk;  // (N is whole 32-blocks: a run is wholly in or out)
-    const uint32_t o = on && q >= 0 && k < N ? 2u * ((uint32_t)q * (uint32_t)N + (uint32_t)k) : 0xFFFFFFF0u;
-    const auto v = __builtin_amdgcn_raw_buffer_load_b128(hr, o, 0, 0);
-    xs[st] = gq_u4{v[0], v[1], v[2], v[3]};
-#pragma unroll
-    for (int r = 0; r < MR; ++r) {
-      const int qr = p_s[b][r];
-      const uint32_t so = on && qr >= 0 ? 8u * (2u * ((uint32_t)qr * (uint32_t)units + (uint32_t)at.u) + gi) : 0xFFFFFFF0u;
-      const auto f = __builtin_amdgcn_raw_buffer_load_b64(sr, so, 0, 0);  // (none: 0)
-      is[st][r] = make_float2(__uint_as_float(f[0]), __uint_as_float(f[1]));
-    }
   };
   float acc[MR] = {};
   uint32_t mg;  // (kept in a register)
@@ -570,14 +605,21 @@ k_moe_down_few(const uint8_t *__restrict__ wd, size_t sc_off, const _Float16 *__
   const gq_u4 ones = {0x3C003C00u, 0x3C003C00u, 0x3C003C00u, 0x3C003C00u};
   const gq_f4 zero = {0.f, 0.f, 0.f, 0.f};
   auto compute = [&](const ItemAt &at, int st) __attribute__((always_inline)) {
-    const gq_u4 xv = xs[st];
-    float s[2], mn[2], w[MR];
+    const int b = at.b, q = p_s[b][MR == 1 ? 0 : lane & 3];
+    const uint32_t xo = mine && q >= 0 ? (uint32_t)(q * stride + 256 * at.u + 32 * g) : zero_at;
+    float s[2], mn[2];
+    float2 f[MR];
 #pragma unroll
-    for (int r = 0; r < MR; ++r) w[r] = w_s[at.b][r];
+    for (int r = 0; r < MR; ++r) {
+      const int qr = p_s[b][r];
+      const float w = w_s[b][r];
+      f[r] = f_s[2 * (max(qr, 0) * units + at.u) + gi];
+      f[r] = qr < 0 ? make_float2(0.f, 0.f) : make_float2(f[r].x * w, f[r].y * w);  // (a token without the expert)
+    }
     few_scales<FMT>(us[st], at.u, g & (NG - 1), s, mn);
-    auto step = [&](auto mc) __attribute__((always_inline)) {
-      constexpr int m = decltype(mc)::value;
-      const gq_u4 a0 = few_operand<NG, 2 * m>(xv), a1 = few_operand<NG, 2 * m + 1>(xv);
+#pragma unroll
+    for (int m = 0; m < 2; ++m) {
+      const gq_u4 a0 = few_lds(xs_s, xo, m, 0), a1 = few_lds(xs_s, xo, m, 1);
       const gq_f4 sx = few_mfma<XT>(a1, ones, few_mfma<XT>(a0, ones, zero));
       gq_u4 b[2];
       few_codes<FMT, XT>(us[st], m, mg, b);
@@ -585,12 +627,19 @@ k_moe_down_few(const uint8_t *__restrict__ wd, size_t sc_off, const _Float16 *__
       const float o = FMT == GQ_FMT_Q4_K ? fmaf(s[m], OFF, mn[m]) : s[m] * OFF;
 #pragma unroll
       for (int r = 0; r < MR; ++r)
-        acc[r] = fmaf(w[r] * (m ? is[st][r].y : is[st][r].x), fmaf(s[m], d[r], -o * sx[r]), acc[r]);
-    };
-    step(std::integral_constant<int, 0>{});
-    step(std::integral_constant<int, 1>{});
+        acc[r] = fmaf(m ? f[r].y : f[r].x, fmaf(s[m], d[r], -o * sx[r]), acc[r]);
+    }
   };
-  if (nblk > 0) walk_items<PD, KS>(0, nblk, units, wave, request, compute);
+  ItemAt rq = {0, 0};
+  rq.next(wave, units);
+  ItemAt first = rq;
+  for (int i = tid; i < P * units; i += 64 * KS)  // (of pairs that name no expert too: not used)
+    *reinterpret_cast<gq_f4 *>(xs_s + P * stride + 160 + 16 * i) = *reinterpret_cast<const gq_f4 *>(hs + 4 * (size_t)i);
+  few_stage<64 * KS>(h, P, N, np, stride, false, xs_s, tid, [&]() __attribute__((always_inline)) {
+    if (nblk > 0) items_requests<PD, KS>(rq, units, request);
+  });
+  step_barrier<63>();  // (of LDS alone)
+  items_computes<PD, KS>(first, rq, nblk, units, request, compute);
 #pragma unroll
   for (int r = 0; r < MR; ++r) red[wave][r][lane] = acc[r];
   __syncthreads();
@@ -610,14 +659,14 @@ k_moe_down_few(const uint8_t *__restrict__ wd, size_t sc_off, const _Float16 *__
 // More tokens: a block's rows are its pairs (fp16 rows of h with a power-of-two scale each); a block's sums go, with the
 // scale's inverse and the expert's weight, to the wave's own sums of the tokens in LDS.  gridDim.y parts of the blocks: their sums go to part
 // [part][M][K] in fp32, which k_moe_sum adds.
-template <int FMT, int KS, int PD>
+template <int FMT, int R, int KS, int PD>
 __global__ void __launch_bounds__(64 * KS)
 k_moe_down_rows(const uint8_t *__restrict__ wd, size_t sc_off, const _Float16 *__restrict__ h16, int ldh, const float *__restrict__ hs,
                 MoePlan p, const void *resid, void *y, int dt, float *__restrict__ part, int M, int K, int C, int units, int top, int maxblk) {
   extern __shared__ float lds[];
   const int P = M * top;
-  float *sum_s = lds;                                                    // [KS][M][16]
-  float *f_s = sum_s + KS * M * 16;                                      // [P]: weight and scale of a pair
+  float *sum_s = lds;                                                    // [KS][M][16 R]
+  float *f_s = sum_s + KS * M * 16 * R;                                    // [P]: weight and scale of a pair
   uint16_t *p_s = reinterpret_cast<uint16_t *>(f_s + P);                 // [maxblk][16]: pairs, 0xFFFF none
   uint16_t *e_s = p_s + 16 * maxblk;                                     // [maxblk]
   uint8_t *t_s = reinterpret_cast<uint8_t *>(e_s + maxblk);              // [P]: token of a pair
@@ -625,7 +674,7 @@ k_moe_down_rows(const uint8_t *__restrict__ wd, size_t sc_off, const _Float16 *_
   const int g = lane >> 4, r = lane & 15, ntiles = K / 16;
   const int all = __builtin_amdgcn_readfirstlane(*p.nblk);
   const int b0 = all * (int)blockIdx.y / (int)gridDim.y, nblk = all * ((int)blockIdx.y + 1) / (int)gridDim.y;
-  for (int i = tid; i < KS * M * 16; i += 64 * KS) sum_s[i] = 0.f;
+  for (int i = tid; i < KS * M * 16 * R; i += 64 * KS) sum_s[i] = 0.f;
   for (int i = tid; i < P; i += 64 * KS) {
     f_s[i] = p.wsum[i] * hs[i];
     t_s[i] = (uint8_t)(i / top);
@@ -638,13 +687,17 @@ k_moe_down_rows(const uint8_t *__restrict__ wd, size_t sc_off, const _Float16 *_
   __syncthreads();
   const __amdgpu_buffer_rsrc_t xr = __builtin_amdgcn_make_buffer_rsrc(
       const_cast<_Float16 *>(h16), (short)0, (int)(2u * (uint32_t)P * (uint32_t)ldh), 0x00020000);
-  FUnit<FMT> us[PD];
+  FUnit<FMT> us[PD][R];
   gq_half8 xs[PD][1][4];
   auto request = [&](const ItemAt &at, int st) __attribute__((always_inline)) {
     const bool on = at.b < nblk;
     const int b = on ? at.b : b0;
-    const size_t tile = (size_t)__builtin_amdgcn_readfirstlane((int)e_s[b]) * (size_t)ntiles + blockIdx.x;
-    load_unit<FMT>(ftile<FMT>(wd, sc_off, tile, on ? C : 0), at.u, lane, us[st]);
+    const size_t tile0 = (size_t)__builtin_amdgcn_readfirstlane((int)e_s[b]) * (size_t)ntiles;
+#pragma unroll
+    for (int t = 0; t < R; ++t) {
+      const int tile = (int)blockIdx.x * R + t;  // (clamped: not stored)
+      load_unit<FMT>(ftile<FMT>(wd, sc_off, tile0 + (size_t)min(tile, ntiles - 1), on ? C : 0), at.u, lane, us[st][t]);
+    }
     const uint32_t q = p_s[16 * b + r];
     const uint32_t o = on && q != 0xFFFFu ? 2u * (q * (uint32_t)ldh + 16u * (uint32_t)g) + 256u * (uint32_t)at.u : 0xFFFFFF00u;
 #pragma unroll
@@ -653,7 +706,9 @@ k_moe_down_rows(const uint8_t *__restrict__ wd, size_t sc_off, const _Float16 *_
       xs[st][0][i] = __builtin_bit_cast(gq_half8, gq_u4{v[0], v[1], v[2], v[3]});
     }
   };
-  gq_f4 acc[1] = {{0.f, 0.f, 0.f, 0.f}};
+  gq_f4 acc[R][1];
+#pragma unroll
+  for (int t = 0; t < R; ++t) acc[t][0] = gq_f4{0.f, 0.f, 0.f, 0.f};
   const uint32_t mg = gq_nib_magic();
   int cur = -1;
   auto flush = [&]() __attribute__((always_inline)) {
@@ -661,25 +716,36 @@ k_moe_down_rows(const uint8_t *__restrict__ wd, size_t sc_off, const _Float16 *_
 #pragma unroll
     for (int v = 0; v < 4; ++v) {
       const uint32_t q = p_s[16 * cur + 4 * g + v];
-      if (q != 0xFFFFu) sum_s[(wave * M + t_s[q]) * 16 + r] += f_s[q] * acc[0][v];  // (a block's tokens differ)
-      acc[0][v] = 0.f;
+      if (q == 0xFFFFu) continue;
+      float *s = sum_s + (wave * M + t_s[q]) * (16 * R) + r;  // (a block's tokens differ)
+#pragma unroll
+      for (int t = 0; t < R; ++t) s[16 * t] += f_s[q] * acc[t][0][v];
     }
+#pragma unroll
+    for (int t = 0; t < R; ++t) acc[t][0] = gq_f4{0.f, 0.f, 0.f, 0.f};
   };
   auto compute = [&](const ItemAt &at, int st) __attribute__((always_inline)) {
     if (at.b != cur) {
       flush();
       cur = at.b;
     }
-    rows_add<FMT, 1>(us[st], at.u, g, mg, xs[st], acc);
+#pragma unroll
+    for (int t = 0; t < R; ++t) rows_add<FMT, 1>(us[st][t], at.u, g, mg, xs[st], acc[t]);
   };
-  if (b0 < nblk) walk_items<PD, KS>(b0, nblk, units, wave, request, compute);
+  ItemAt rq = {b0, 0};
+  rq.next(wave, units);
+  const ItemAt first = rq;
+  items_requests<PD, KS>(rq, units, request);
+  items_computes<PD, KS>(first, rq, nblk, units, request, compute);
   flush();
   __syncthreads();
-  for (int i = tid; i < 16 * M; i += 64 * KS) {
-    const int n = i & 15, m = i >> 4;
+  for (int i = tid; i < 16 * R * M; i += 64 * KS) {
+    const int n = i % (16 * R), m = i / (16 * R), k = 16 * R * (int)blockIdx.x + n;
+    if (k >= K) continue;
     float v = 0.f;
-    for (int w = 0; w < KS; ++w) v += sum_s[(w * M + m) * 16 + n];
-    const size_t o = (size_t)m * K + 16 * blockIdx.x + n;
+#pragma unroll
+    for (int w = 0; w < KS; ++w) v += sum_s[(w * M + m) * (16 * R) + n];
+    const size_t o = (size_t)m * K + k;
     if (part) {
       part[(size_t)blockIdx.y * M * K + o] = v;
       continue;
@@ -726,6 +792,12 @@ int check_moe(const gq_moe *l, size_t M, bool route, bool ffn) {
   return GQ_OK;
 }
 
+// Up to 4 tokens whose rows of x, and of h with their scales, fit LDS (beside 20 KiB of the kernels' own)
+bool moe_few(const gq_moe &l, size_t M) {
+  constexpr size_t kLds = (160 - 20) * 1024;
+  const size_t P = M * (size_t)l.top_k, nk = (gq_kpad(l.fmt, l.K) + 127) & ~(size_t)127, nn = (gq_kpad(l.fmt_down, l.N) + 127) & ~(size_t)127;
+  return M <= (size_t)kMoeFew && few_lds_bytes(M, nk) <= kLds && few_lds_bytes(P, nn) + P * nn / 8 <= kLds;
+}
 // Where a call's intermediate values lie in its workspace
 struct MoeWs {
   size_t logits, ids, weights, nblk, blk, wsum, a16, rs, h, h16, hs, part, bytes;
@@ -740,7 +812,7 @@ MoeWs moe_ws(const gq_moe &l, size_t M) {
     return o;
   };
   const size_t P = M * (size_t)l.top_k;
-  const bool few = M <= (size_t)kMoeFew;
+  const bool few = moe_few(l, M);
   // (an expert's last block may be short: at most a block an expert beyond whole ones)
   w.maxblk = (int)(few ? std::min(P, l.n_experts) : std::min(P, l.n_experts + P / 16));
   w.logits = take(M * l.n_experts * 8);
@@ -754,9 +826,9 @@ MoeWs moe_ws(const gq_moe &l, size_t M) {
   w.h = take(few ? 0 : P * l.N * 4);
   w.h16 = take(P * (gq_kpad(l.fmt_down, l.N) + 8) * 2);
   w.hs = take(few ? P * ((l.N + 127) / 128) * 16 : (P + 256) * 4);
-  // W_down's row tiles, a workgroup each, in parts where they would leave CUs idle
-  const size_t tiles = l.K / 16;
-  w.parts = few || tiles >= 192 ? 1 : (int)std::min({(size_t)4, 320 / tiles, (size_t)w.maxblk});
+  // W_down's row tiles, two a workgroup, in parts as far as a workgroup a CU goes (64 tokens, 128 experts of 768 x 2048, in 2 / 3 / 4
+  // parts: 147 / 127 / 117 us the layer; 37 tokens, 61 of 1376 x 2080, whose four are more than that, 100 / 92 / 98)
+  w.parts = few ? 1 : (int)std::min(std::max((size_t)1, 256 / ((l.K + 31) / 32)), std::min((size_t)8, (size_t)w.maxblk));
   w.part = take(w.parts > 1 ? w.parts * M * l.K * 4 : 0);
   w.bytes = at;
   return w;
@@ -783,7 +855,7 @@ int launch_plan(const gq_moe &l, const RouteArgs &a, const int *ids, const float
                 hipStream_t s) {
   const int E = (int)l.n_experts;
 #define GQ_PLAN(NE)                                                                                                       \
-  hipLaunchKernelGGL(k_moe_plan<NE>, dim3(1), dim3(kPlanThreads), 0, s, a, ids, weights, plan, M, E, l.top_k, M <= kMoeFew ? kMoeFew : 16)
+  hipLaunchKernelGGL(k_moe_plan<NE>, dim3(1), dim3(kPlanThreads), 0, s, a, ids, weights, plan, M, E, l.top_k)
   if (!a.logits) GQ_PLAN(0);
   else if (E <= 64) GQ_PLAN(1);
   else if (E <= 128) GQ_PLAN(2);
@@ -802,21 +874,10 @@ int launch_choose(const gq_moe &l, const RouteArgs &a, int M, hipStream_t s) {
 #undef GQ_CHOOSE
   return gq_last_launch();
 }
-// plan.blk NULL: the choice alone.  A wave a token, in the plan's workgroup where each of its 16 waves has one at most (in turn by four
-// tokens a wave 22 us for 64 tokens of 128 experts, in a launch of their own XX).
-int launch_route(const gq_moe &l, const void *x, int xt, int M, double *logits, const MoeConv &conv, int *ids, float *weights,
-                 const MoePlan &plan, hipStream_t s) {
-  if (xt == GQ_DT_F32) GQ_TRY(launch_logits_x<GQ_DT_F32>(l, x, logits, conv, M, s));
-  else if (xt == GQ_DT_F16) GQ_TRY(launch_logits_x<GQ_DT_F16>(l, x, logits, conv, M, s));
-  else GQ_TRY(launch_logits_x<GQ_DT_BF16>(l, x, logits, conv, M, s));
-  RouteArgs a = {logits, l.router_bias, ids, weights, l.score, l.renorm, l.scale};
-  if (M > kPlanThreads / 64 || !plan.blk) {
-    GQ_TRY(launch_choose(l, a, M, s));
-    if (!plan.blk) return GQ_OK;
-    a.logits = nullptr;
-    return launch_plan(l, a, ids, weights, plan, M, s);
-  }
-  return launch_plan(l, a, nullptr, nullptr, plan, M, s);
+int launch_logits(const gq_moe &l, const void *x, int xt, double *logits, const MoeConv &conv, int M, hipStream_t s) {
+  if (xt == GQ_DT_F32) return launch_logits_x<GQ_DT_F32>(l, x, logits, conv, M, s);
+  if (xt == GQ_DT_F16) return launch_logits_x<GQ_DT_F16>(l, x, logits, conv, M, s);
+  return launch_logits_x<GQ_DT_BF16>(l, x, logits, conv, M, s);
 }
 
 // Intermediate values of a call
@@ -826,77 +887,100 @@ struct MoeMid {
   int lda, ldh, parts;
 };
 template <int FMT, int XT>
-int launch_gu_few_t(const gq_moe &l, const void *x, const float *rs, const MoePlan &p, const MoeMid &b, int M, hipStream_t s) {
+int launch_gu_few_t(const gq_moe &l, const void *x, const float *rs, const RouteArgs *a, const int *ids, const MoeMid &b, int M,
+                    hipStream_t s) {
   const int N = (int)l.N, K = (int)l.K, units = (int)(gq_kpad(FMT, K) / 128), nib = l.fmt_down == GQ_FMT_Q4_0 || gq_fmt_is_q4k(l.fmt_down);
-#define GQ_GU(MR, KS, PD)                                                                                                  \
-  hipLaunchKernelGGL((k_moe_gu_few<FMT, XT, MR, KS, PD>), dim3((unsigned)(N / 32), (unsigned)p.maxblk), dim3(64 * (KS)), 0, s, \
-                     (const uint8_t *)l.gate, (const uint8_t *)l.up, gq_sc_plane_offset(FMT, l.n_experts * l.N, K), x, rs, p, b.h16, \
-                     b.hs, nib, M, N, K, (int)gq_chunks(FMT, K), units, l.act, l.top_k)
-  if (M == 1) GQ_GU(1, 4, 2);
-  else GQ_GU(4, 4, 2);
+#define GQ_GU_R(MR, KS, PD, ROUTE)                                                                                         \
+  hipLaunchKernelGGL((k_moe_gu_few<FMT, XT, MR, KS, PD, ROUTE>), dim3((unsigned)(N / 32), (unsigned)(M * l.top_k)), dim3(64 * (KS)), \
+                     few_lds_bytes(M, 128 * (size_t)units), s, (const uint8_t *)l.gate, (const uint8_t *)l.up,            \
+                     gq_sc_plane_offset(FMT, l.n_experts * l.N, K), x, rs, a ? *a : RouteArgs{}, ids, b.h16, b.hs, nib, M, N, K,    \
+                     (int)gq_chunks(FMT, K), units, l.act, (int)l.n_experts, l.top_k)
+#define GQ_GU(MR, KS, PD)                  \
+  do {                                     \
+    if (a) GQ_GU_R(MR, KS, PD, true);      \
+    else GQ_GU_R(MR, KS, PD, false);       \
+  } while (0)
+  // (one token, Q4_K: 256 workgroups, 64 experts of 1024 x 2048, by 8 waves 20.5 us the layer, by 4 20.8; 896, 8 of 14336 x 4096, 51.7 and 51.1)
+  const bool wide = (size_t)(N / 32) * (size_t)(M * l.top_k) > 512;
+  if (M == 1) {
+    if (wide) GQ_GU(1, 4, 2);
+    else GQ_GU(1, 8, 1);
+  } else {
+    if (wide) GQ_GU(4, 4, 2);
+    else GQ_GU(4, 8, 1);
+  }
 #undef GQ_GU
+#undef GQ_GU_R
   return gq_last_launch();
 }
 template <int FMT>
-int launch_gu_t(const gq_moe &l, const void *x, int xt, const float *rs, const MoePlan &p, const MoeMid &b, int M, hipStream_t s) {
-  if (M <= kMoeFew)
-    return xt == GQ_DT_F16 ? launch_gu_few_t<FMT, GQ_DT_F16>(l, x, rs, p, b, M, s)
-                           : launch_gu_few_t<FMT, GQ_DT_BF16>(l, x, rs, p, b, M, s);
-  const int N = (int)l.N, K = (int)l.K, units = (int)(gq_kpad(FMT, K) / 128);
-  hipLaunchKernelGGL((k_moe_gu_rows<FMT, 1, 4, 3>), dim3((unsigned)(N / 16), (unsigned)p.maxblk), dim3(256), 0, s,
+int launch_gu_t(const gq_moe &l, const void *x, int xt, const float *rs, const RouteArgs *a, const int *ids, const MoePlan &p,
+                const MoeMid &b, int M, hipStream_t s) {
+  if (moe_few(l, M))
+    return xt == GQ_DT_F16 ? launch_gu_few_t<FMT, GQ_DT_F16>(l, x, rs, a, ids, b, M, s)
+                           : launch_gu_few_t<FMT, GQ_DT_BF16>(l, x, rs, a, ids, b, M, s);
+  const int N = (int)l.N, K = (int)l.K, units = (int)(gq_kpad(FMT, K) / 128), tiles = N / 16;
+  // (16 tokens, 8 experts of 14336 x 4096, Q4_0, by one tile 190 us the layer, by two 167; 64 tokens, 128 experts of 768 x 2048, 143 and 128)
+  constexpr int R = 2, KS = 4;
+  hipLaunchKernelGGL((k_moe_gu_rows<FMT, R, KS, 2>), dim3((unsigned)((tiles + R - 1) / R), (unsigned)p.maxblk), dim3(64 * KS), 0, s,
                      (const uint8_t *)l.gate, (const uint8_t *)l.up, gq_sc_plane_offset(FMT, l.n_experts * l.N, K), b.a16, b.lda, rs, p,
                      b.h, M, N, (int)gq_chunks(FMT, K), units, l.act, l.top_k);
   return gq_last_launch();
 }
 template <int FMT>
-int launch_down_t(const gq_moe &l, const MoePlan &p, const MoeMid &b, const void *resid, void *y, int dt, int M, hipStream_t s) {
+int launch_down_t(const gq_moe &l, const int *ids, const float *weights, const MoePlan &p, const MoeMid &b, const void *resid, void *y,
+                  int dt, int M, hipStream_t s) {
   const int N = (int)l.N, K = (int)l.K, units = (int)(gq_kpad(FMT, N) / 128), C = (int)gq_chunks(FMT, N);
   const size_t so = gq_sc_plane_offset(FMT, l.n_experts * l.K, N);
   const unsigned tiles = (unsigned)(K / 16);
-  if (M <= kMoeFew) {
+  if (moe_few(l, M)) {
+    const size_t rows = (size_t)M * l.top_k, lds = few_lds_bytes(rows, 128 * (size_t)units) + rows * units * 16;
 #define GQ_DOWN(MR, KS, PD)                                                                                              \
-  hipLaunchKernelGGL((k_moe_down_few<FMT, MR, KS, PD>), dim3(tiles), dim3(64 * (KS)), 0, s, (const uint8_t *)l.down, so, b.h16, b.hs, p, \
-                     resid, y, dt, M, N, K, C, units, l.top_k)
-    if (M == 1) GQ_DOWN(1, 16, 3);
+  hipLaunchKernelGGL((k_moe_down_few<FMT, MR, KS, PD>), dim3(tiles), dim3(64 * (KS)), lds, s, (const uint8_t *)l.down, so, b.h16, b.hs, ids, \
+                     weights, resid, y, dt, M, N, K, C, units, (int)l.n_experts, l.top_k)
+    if (M == 1) GQ_DOWN(1, 16, 2);
     else GQ_DOWN(4, 16, 2);
 #undef GQ_DOWN
     return gq_last_launch();
   }
-  constexpr int KS = 8;
-  const size_t P = (size_t)M * l.top_k, lds = (size_t)KS * M * 64 + P * 4 + (size_t)p.maxblk * 34 + P + 16;
-  hipLaunchKernelGGL((k_moe_down_rows<FMT, KS, 3>), dim3(tiles, (unsigned)b.parts), dim3(64 * KS), lds, s, (const uint8_t *)l.down, so,
-                     b.h16, b.ldh, b.hs, p, resid, y, dt, b.parts > 1 ? b.part : nullptr, M, K, C, units, l.top_k, p.maxblk);
+  // Two tiles a workgroup, which share the rows of h: four of six loads a unit.  (16 tokens, 8 experts of 14336 x 4096, Q4_0, by one tile 167 us
+  // the layer, by two in two parts 152, by four in four parts 147 - 149; 64 tokens, 128 experts of 768 x 2048, 127, 117 and 139 - 159.)
+  constexpr int R = 2, KS = 8;
+  const size_t P = (size_t)M * l.top_k, lds = (size_t)KS * M * 64 * R + P * 4 + (size_t)p.maxblk * 34 + P + 16;
+  hipLaunchKernelGGL((k_moe_down_rows<FMT, R, KS, 2>), dim3((tiles + R - 1) / R, (unsigned)b.parts), dim3(64 * KS), lds, s,
+                     (const uint8_t *)l.down, so, b.h16, b.ldh, b.hs, p, resid, y, dt, b.parts > 1 ? b.part : nullptr, M, K, C, units,
+                     l.top_k, p.maxblk);
   return gq_last_launch();
 }
 
-bool moe_few(int M) { return M <= kMoeFew; }
 // x goes in as it is: few rows of 16-bit values
-bool moe_as_it_is(const void *x, int xt, int M) { return moe_few(M) && xt != GQ_DT_F32 && (uintptr_t)x % 4 == 0; }
+bool moe_as_it_is(const gq_moe &l, int xt, int M) { return moe_few(l, M) && xt != GQ_DT_F32; }
 MoeMid moe_mid(const gq_moe &l, const MoeWs &w, uint8_t *ws, int M) {
   return MoeMid{(_Float16 *)(ws + w.a16), (_Float16 *)(ws + w.h16), (float *)(ws + w.rs), (float *)(ws + w.h), (float *)(ws + w.hs),
-                (float *)(ws + w.part), moe_few(M) ? (int)l.K : (int)gq_kpad(l.fmt, l.K) + 8, (int)gq_kpad(l.fmt_down, l.N) + 8, w.parts};
+                (float *)(ws + w.part), moe_few(l, M) ? (int)l.K : (int)gq_kpad(l.fmt, l.K) + 8, (int)gq_kpad(l.fmt_down, l.N) + 8, w.parts};
 }
-int moe_x_order(const gq_moe &l, int M) { return !moe_few(M) && (l.fmt == GQ_FMT_Q4_0 || gq_fmt_is_q4k(l.fmt)); }
+int moe_x_order(const gq_moe &l, int M) { return !moe_few(l, M) && (l.fmt == GQ_FMT_Q4_0 || gq_fmt_is_q4k(l.fmt)); }
 
-// The products, x converted already where it has to be
-int moe_products(const gq_moe &l, const void *x, int xt, const MoePlan &plan, const MoeMid &b, const void *resid, void *y, int dt, int M,
-                 hipStream_t s) {
+// The products, x converted already where it has to be.  Few tokens: of the experts ids, or (a) of those that the logits choose, whose ids and
+// weights come out in a->ids, a->weights.
+int moe_products(const gq_moe &l, const void *x, int xt, const RouteArgs *a, const int *ids, const float *weights, const MoePlan &plan,
+                 const MoeMid &b, const void *resid, void *y, int dt, int M, hipStream_t s) {
   const float *rs = nullptr;
-  if (!moe_as_it_is(x, xt, M)) {
+  if (!moe_as_it_is(l, xt, M)) {
     x = b.a16;
     xt = GQ_DT_F16;
     rs = b.rs;
   }
-#define GQ_GU_F(F) launch_gu_t<F>(l, x, xt, rs, plan, b, M, s)
+#define GQ_GU_F(F) launch_gu_t<F>(l, x, xt, rs, a, ids, plan, b, M, s)
   if (l.fmt == GQ_FMT_Q4_0) GQ_TRY(GQ_GU_F(GQ_FMT_Q4_0));
   else if (l.fmt == GQ_FMT_Q8_0) GQ_TRY(GQ_GU_F(GQ_FMT_Q8_0));
   else if (gq_fmt_is_q6k(l.fmt)) GQ_TRY(GQ_GU_F(GQ_FMT_Q6_K));
   else GQ_TRY(GQ_GU_F(GQ_FMT_Q4_K));
 #undef GQ_GU_F
-  if (!moe_few(M))
+  if (!moe_few(l, M))
     GQ_TRY(gq_launch_a_to_f16(b.h, GQ_DT_F32, b.h16, b.hs, M * l.top_k, (int)l.N, b.ldh,
                               l.fmt_down == GQ_FMT_Q4_0 || gq_fmt_is_q4k(l.fmt_down), s));
-#define GQ_DOWN_F(F) launch_down_t<F>(l, plan, b, resid, y, dt, M, s)
+#define GQ_DOWN_F(F) launch_down_t<F>(l, ids, weights, plan, b, resid, y, dt, M, s)
   if (l.fmt_down == GQ_FMT_Q4_0) GQ_TRY(GQ_DOWN_F(GQ_FMT_Q4_0));
   else if (l.fmt_down == GQ_FMT_Q8_0) GQ_TRY(GQ_DOWN_F(GQ_FMT_Q8_0));
   else if (gq_fmt_is_q6k(l.fmt_down)) GQ_TRY(GQ_DOWN_F(GQ_FMT_Q6_K));
@@ -945,7 +1029,9 @@ extern "C" int gq_moe_route(const gq_moe *l, const void *x, int x_dtype, int32_t
   hipStream_t s = (hipStream_t)stream;
   MoeRoom room(ws, ws_bytes, M * l->n_experts * 8, s);
   GQ_TRY(room.status);
-  return launch_route(*l, x, x_dtype, (int)M, (double *)room.ptr, MoeConv{}, ids, weights, MoePlan{}, s);
+  double *logits = (double *)room.ptr;
+  GQ_TRY(launch_logits(*l, x, x_dtype, logits, MoeConv{}, (int)M, s));
+  return launch_choose(*l, RouteArgs{logits, l->router_bias, ids, weights, l->score, l->renorm, l->scale}, (int)M, s);
 }
 
 extern "C" int gq_moe_ffn(const gq_moe *l, const void *x, int x_dtype, const int32_t *ids, const float *weights,
@@ -960,10 +1046,10 @@ extern "C" int gq_moe_ffn(const gq_moe *l, const void *x, int x_dtype, const int
   GQ_TRY(room.status);
   const MoePlan plan = plan_of(w, room.ptr);
   const MoeMid mid = moe_mid(*l, w, room.ptr, (int)M);
-  GQ_TRY(launch_plan(*l, RouteArgs{}, (const int *)ids, weights, plan, (int)M, s));
-  if (!moe_as_it_is(x, x_dtype, (int)M))
+  if (!moe_few(*l, M)) GQ_TRY(launch_plan(*l, RouteArgs{}, ids, weights, plan, (int)M, s));
+  if (!moe_as_it_is(*l, x_dtype, (int)M))
     GQ_TRY(gq_launch_a_to_f16(x, x_dtype, mid.a16, mid.rs, (int)M, (int)l->K, mid.lda, moe_x_order(*l, (int)M), s));
-  return moe_products(*l, x, x_dtype, plan, mid, resid, y, y_dtype, (int)M, s);
+  return moe_products(*l, x, x_dtype, nullptr, ids, weights, plan, mid, resid, y, y_dtype, (int)M, s);
 }
 
 extern "C" int gq_moe_layer(const gq_moe *l, const void *x, int x_dtype, const void *resid, void *y, int y_dtype, int32_t *ids,
@@ -978,10 +1064,19 @@ extern "C" int gq_moe_layer(const gq_moe *l, const void *x, int x_dtype, const v
   GQ_TRY(room.status);
   const MoePlan plan = plan_of(w, room.ptr);
   const MoeMid mid = moe_mid(*l, w, room.ptr, (int)M);
-  const MoeConv conv = moe_as_it_is(x, x_dtype, (int)M) ? MoeConv{} : MoeConv{mid.a16, mid.rs, mid.lda, moe_x_order(*l, (int)M)};
-  // (the choice passes through memory where it has a launch of its own)
+  const MoeConv conv = moe_as_it_is(*l, x_dtype, (int)M) ? MoeConv{} : MoeConv{mid.a16, mid.rs, mid.lda, moe_x_order(*l, (int)M)};
   if (!ids) ids = (int32_t *)(room.ptr + w.ids);
   if (!weights) weights = (float *)(room.ptr + w.weights);
-  GQ_TRY(launch_route(*l, x, x_dtype, (int)M, (double *)(room.ptr + w.logits), conv, ids, weights, plan, s));
-  return moe_products(*l, x, x_dtype, plan, mid, resid, y, y_dtype, (int)M, s);
+  RouteArgs a = {(double *)(room.ptr + w.logits), l->router_bias, ids, weights, l->score, l->renorm, l->scale};
+  GQ_TRY(launch_logits(*l, x, x_dtype, (double *)(room.ptr + w.logits), conv, (int)M, s));
+  // The choice, a wave a token: few tokens with the gate and up products, in the plan's workgroup where each of its 16 waves has one at most
+  // (four tokens a wave, 64 of 128 experts: 22 us, against 5 and 5 of two launches), else in a launch of its own.
+  const bool few = moe_few(*l, M), within = few && l->n_experts <= 64 * kFewNE, own = !within && (few || M > kPlanThreads / 64);
+  if (own) GQ_TRY(launch_choose(*l, a, (int)M, s));
+  if (!few) {
+    RouteArgs b = a;
+    if (own) b.logits = nullptr;
+    GQ_TRY(launch_plan(*l, b, ids, weights, plan, (int)M, s));
+  }
+  return moe_products(*l, x, x_dtype, within ? &a : nullptr, ids, weights, plan, mid, resid, y, y_dtype, (int)M, s);
 }

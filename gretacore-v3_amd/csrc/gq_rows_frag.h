@@ -74,24 +74,38 @@ GQ_DEV gq_u4 nib_order(const gq_u4 &v) {
                __builtin_amdgcn_perm(v[1], v[0], 0x07060302u), __builtin_amdgcn_perm(v[3], v[2], 0x07060302u)};
 }
 
-// The units of a wave: request(unit, stage) and compute(unit, stage), PD stages
-template <int PD, int KS, typename Request, typename Compute>
-GQ_DEV void walk_units(int units, int wave, Request request, Compute compute) {
-  const int n = units > wave ? (units - wave + KS - 1) / KS : 0;
-  if (n == 0) return;
-  auto req = [&](int j, int st) __attribute__((always_inline)) { request(j < n ? wave + KS * j : units, st); };
+// The units of a wave: request(unit, stage) and compute(unit, stage), PD stages, the first requests
+// apart from the rest.  A group of PD units requests the next one unless it is the last: no branch within a group, around which the
+// compiler would wait for every load.
+template <int PD, int KS, typename Request>
+GQ_DEV void walk_requests(int units, int wave, Request request) {
 #pragma unroll
-  for (int i = 0; i < PD; ++i) req(i, i);
-  for (int j = 0; j < n; j += PD) {
+  for (int i = 0; i < PD; ++i) request(min(wave + KS * i, units), i);
+}
+template <int PD, int KS, typename Request, typename Compute>
+GQ_DEV void walk_computes(int units, int wave, Request request, Compute compute) {
+  const int n = units > wave ? (units - wave + KS - 1) / KS : 0;
+  int j = 0;
+  for (; j + PD < n; j += PD) {
 #pragma unroll
     for (int i = 0; i < PD; ++i) {
-      if (j + i >= n) break;
       compute(wave + KS * (j + i), i);
-      req(j + i + PD, i);
+      request(min(wave + KS * (j + i + PD), units), i);
     }
   }
+#pragma unroll
+  for (int i = 0; i < PD; ++i)
+    if (j + i < n) compute(wave + KS * (j + i), i);
+}
+template <int PD, int KS, typename Request, typename Compute>
+GQ_DEV void walk_units(int units, int wave, Request request, Compute compute) {
+  walk_requests<PD, KS>(units, wave, request);
+  walk_computes<PD, KS>(units, wave, request, compute);
 }
 
+struct __attribute__((packed, aligned(2))) FRun16 {  // 8 values at any 2-byte address
+  gq_u4 v;
+};
 // Up to 4 rows: nothing comes before the weights.  x enters the matrix cores as it is (bf16 or
 // f16, no conversion launch), and so do the codes, as the 16-bit floats OFF + q; scales and
 // minima are applied in fp32 to the sums of each scale group,
@@ -196,6 +210,58 @@ GQ_DEV gq_u4 few_operand(const gq_u4 &x) {
   return o;
 }
 
+// The same operands from x in LDS, where the rows fit it: a lane whose row and group do not belong together reads zeros.  Rows of 16-bit
+// values (for the 4-bit formats in the nibbles' order) lie `stride` bytes apart, `zero` is the offset of 160 zero bytes behind them.
+// (Moves between lanes for every unit: 32 or 64 instructions of 131 to 180 a unit of one row.)
+template <int FMT>
+GQ_DEV bool few_mine(int lane) {  // row lane % 4 is of this lane's scale group
+  const int i = (lane >> 2) & 3, g = lane >> 4;
+  return kFewGroups<FMT> == 4 ? i == g : i == g >> 1;
+}
+// operand of step m, half j of the unit whose 128 values start at offset `at` (of lane group 0)
+GQ_DEV gq_u4 few_lds(const uint8_t *xs, uint32_t at, int m, int j) {
+  return *reinterpret_cast<const gq_u4 *>(xs + at + 128 * m + 16 * j);
+}
+// Copies rows of `n` 16-bit values (n % 32 == 0, row r at src + r * n) to LDS, zeros up to np, nib: in the nibbles' order, by T threads.
+// ahead() is called between the last loads and their stores: what it requests is under way while they are waited for.
+template <int T, typename Ahead>
+GQ_DEV void few_stage(const void *src, int rows, int n, int np, int stride, bool nib, uint8_t *xs, int tid, Ahead ahead) {
+  constexpr int RUNS = 4;
+  const int per = np / 8, all = rows * per;  // (below 2^20: i / per from a float is exact)
+  const float inv = 1.0f / (float)per;
+  auto at = [&](int i, int &r, int &k) __attribute__((always_inline)) {
+    r = (int)(((float)i + 0.5f) * inv);
+    k = 8 * (i - r * per);
+  };
+  if (tid < 40) *reinterpret_cast<uint32_t *>(xs + (size_t)rows * stride + 4 * tid) = 0;
+  for (int i0 = 0; i0 < all; i0 += T * RUNS) {
+    FRun16 v[RUNS];
+#pragma unroll
+    for (int u = 0; u < RUNS; ++u) {
+      const int i = i0 + tid + T * u;
+      int r, k;
+      at(i, r, k);
+      v[u] = *reinterpret_cast<const FRun16 *>(reinterpret_cast<const uint16_t *>(src) +
+                                               (i < all && k < n ? (size_t)r * (size_t)n + k : 0));
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    if (i0 + T * RUNS >= all) ahead();
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int u = 0; u < RUNS; ++u) {
+      const int i = i0 + tid + T * u;
+      int r, k;
+      at(i, r, k);
+      gq_u4 o = nib ? nib_order(v[u].v) : v[u].v;
+      if (k >= n) o = gq_u4{0, 0, 0, 0};
+      if (i < all) *reinterpret_cast<gq_u4 *>(xs + (size_t)r * stride + 2 * k) = o;
+    }
+  }
+}
+// bytes of LDS they take
+GQ_LHD size_t few_lds_stride(size_t np) { return 2 * np + 16; }
+GQ_LHD size_t few_lds_bytes(size_t rows, size_t np) { return rows * few_lds_stride(np) + 160; }
+
 // More rows: the sums of the scale groups would cost more than folding the scale into the
 // weights; the matrix cores then add over a unit or all of K.  Q4_0 and Q8_0: d (q - bias), rounded once
 // to fp16.  The k-quants keep their d (and dmin) out, one of each to a row and unit, applied in fp32
@@ -276,9 +342,6 @@ GQ_DEV void rows_add(const FUnit<FMT> &u, int unit, int g, uint32_t mg, const gq
   }
 }
 
-struct __attribute__((packed, aligned(2))) FRun16 {  // 8 values at any 2-byte address
-  gq_u4 v;
-};
 struct __attribute__((packed, aligned(4))) FRun32 {
   gq_f4 v[2];
 };
