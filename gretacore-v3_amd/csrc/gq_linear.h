@@ -45,6 +45,12 @@ GQ_DEV void lin_put(const LinEpi &e, size_t m, int n, int N, float v, const LinT
 
 }  // namespace
 
-// the tiled kernels (gq_linear_rb.hip): a16 fp16 [M][gq_kpad(K)] in the B fragments' order, rs its row scales (padded by 256)
-int gq_launch_linear_rb(int fmt, const void *w, const _Float16 *a16, const float *rs, const void *epi, int M, int N, int K,
+// The tiled kernels (gq_linear_rb.hip): a16 fp16 [M][gq_kpad(K)] in the B fragments' order, rs its row scales (padded by 256), part: room for
+// parts of K, kLinPartBytes
+int gq_launch_linear_rb(int fmt, const void *w, const _Float16 *a16, const float *rs, const void *epi, float *part, int M, int N, int K,
                         hipStream_t s);
+// the epilogue epi of the parts' sums [parts][M][N] (gq_linear.hip)
+int gq_launch_linear_sum(const float *part, const void *epi, int M, int N, int parts, hipStream_t s);
+// Parts are taken only as far as a workgroup a CU goes, each with an fp32 tile of at most 128 x 256 outputs, and at most 8
+constexpr int kLinParts = 8;
+constexpr size_t kLinPartBytes = (size_t)256 * 128 * 256 * 4;

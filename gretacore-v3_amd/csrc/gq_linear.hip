@@ -1,7 +1,6 @@
 // gq_linear.hip -- the product with bias, activation and residual in its epilogue over T16 weights,
 // any number of rows (few rows here, tiles in gq_linear_rb.hip), and its backward pass.
 #include <algorithm>
-#include <stdlib.h>
 #include <type_traits>
 
 #include "gq_internal.h"
@@ -10,7 +9,7 @@
 
 namespace {
 
-// ---- forward: up to 64 rows, units of 128 k ------------------------------------------
+// ---- forward: up to 16 rows, units of 128 k ------------------------------------------
 // The weights' bytes bound these: a workgroup takes R row tiles, its KS waves share K unit by unit with PD units in
 // flight each, and their sums are added through LDS.
 // Outputs of R tiles and up to ROWS rows, several a thread: their biases and residuals (which may be y, and are read before any
@@ -36,18 +35,6 @@ struct LinOut {
 #pragma unroll
       for (int k = 0; k < KS; ++k) y += at(k, nl >> 4, nl & 15, m);
       lin_put(e, m, n, N, rs ? y * rs[m] : y, t[i]);
-    }
-  }
-  // a part's sums, fp32 [M][N]
-  template <typename At>
-  __device__ __forceinline__ void put_part(At at, const float *rs, float *part, int M, int N, int block) {
-    for (int o = threadIdx.x; o < 16 * R * M; o += 64 * KS) {
-      const int nl = o % (16 * R), m = o / (16 * R), n = 16 * R * block + nl;
-      if (n >= N) continue;
-      float y = 0.f;
-#pragma unroll
-      for (int k = 0; k < KS; ++k) y += at(k, nl >> 4, nl & 15, m);
-      part[(size_t)m * (size_t)N + n] = y * rs[m];
     }
   }
 };
@@ -134,9 +121,8 @@ k_lin_few(const uint8_t *__restrict__ w, size_t sc_off, const void *__restrict__
 template <int FMT, int MT, int R, int KS, int PD>
 __global__ void __launch_bounds__(64 * KS)
 k_lin_rows(const uint8_t *__restrict__ w, size_t sc_off, const _Float16 *__restrict__ a16, int lda,
-           const float *__restrict__ rs, LinEpi e, float *__restrict__ part, int M, int N, int C, int units) {
+           const float *__restrict__ rs, LinEpi e, int M, int N, int C, int units) {
   __shared__ gq_f4 red[KS][R][MT][64];
-  const int u0 = units * (int)blockIdx.y / (int)gridDim.y, un = units * ((int)blockIdx.y + 1) / (int)gridDim.y - u0;  // this part's
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int g = lane >> 4, r = lane & 15, ntiles = (int)gq_tiles(N);
   FTile<FMT> tl[R];
@@ -157,10 +143,10 @@ k_lin_rows(const uint8_t *__restrict__ w, size_t sc_off, const _Float16 *__restr
   gq_half8 xs[PD][MT][4];
   auto request = [&](int unit, int st) __attribute__((always_inline)) {
 #pragma unroll
-    for (int t = 0; t < R; ++t) load_unit<FMT>(tl[t], unit < un ? u0 + unit : units, lane, us[st][t]);
+    for (int t = 0; t < R; ++t) load_unit<FMT>(tl[t], unit, lane, us[st][t]);
 #pragma unroll
     for (int t = 0; t < MT; ++t) {
-      const uint32_t o = unit < un ? xo[t] + 256u * (uint32_t)(u0 + unit) : 0xFFFFFF00u;
+      const uint32_t o = unit < units ? xo[t] + 256u * (uint32_t)unit : 0xFFFFFF00u;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const auto v = __builtin_amdgcn_raw_buffer_load_b128(xr, o + 128u * (i >> 1) + 16u * (i & 1), 0, 0);
@@ -176,11 +162,11 @@ k_lin_rows(const uint8_t *__restrict__ w, size_t sc_off, const _Float16 *__restr
   const uint32_t mg = gq_nib_magic();
   auto compute = [&](int unit, int st) __attribute__((always_inline)) {
 #pragma unroll
-    for (int t = 0; t < R; ++t) rows_add<FMT, MT>(us[st][t], u0 + unit, g, mg, xs[st], acc[t]);
+    for (int t = 0; t < R; ++t) rows_add<FMT, MT>(us[st][t], unit, g, mg, xs[st], acc[t]);
   };
   LinOut<KS, R, 16 * MT> out;
-  if (!part) out.ahead(e, M, N, (int)blockIdx.x);
-  walk_units<PD, KS>(un, wave, request, compute);
+  out.ahead(e, M, N, (int)blockIdx.x);
+  walk_units<PD, KS>(units, wave, request, compute);
 #pragma unroll
   for (int t = 0; t < R; ++t)
 #pragma unroll
@@ -189,8 +175,7 @@ k_lin_rows(const uint8_t *__restrict__ w, size_t sc_off, const _Float16 *__restr
   auto at = [&](int k, int t, int n, int m) {
     return reinterpret_cast<const float *>(&red[k][t][m >> 4][16 * ((m >> 2) & 3) + n])[m & 3];
   };
-  if (part) out.put_part(at, rs, part + (size_t)blockIdx.y * (size_t)M * (size_t)N, M, N, (int)blockIdx.x);
-  else out.put(at, rs, e, M, N, (int)blockIdx.x);
+  out.put(at, rs, e, M, N, (int)blockIdx.x);
 }
 
 // the parts' sums, in their order, and the epilogue; a thread takes outputs of one row
@@ -202,11 +187,6 @@ __global__ void __launch_bounds__(256) k_lin_sum(const float *__restrict__ part,
   for (int p = 0; p < parts; ++p) v += part[((size_t)p * M + m) * (size_t)N + n];
   lin_put(e, m, n, N, v, t);
 }
-int launch_sum(const float *part, const LinEpi &e, int M, int N, int parts, hipStream_t s) {
-  hipLaunchKernelGGL(k_lin_sum, dim3((unsigned)((N + 255) / 256), (unsigned)M), dim3(256), 0, s, part, e, M, N, parts);
-  return gq_last_launch();
-}
-
 template <int FMT, int XT>
 int launch_few_t(const void *w, const void *x, const float *rs, const LinEpi &e, int M, int N, int K, hipStream_t s) {
   const int units = (int)(gq_kpad(FMT, K) / 128);
@@ -227,39 +207,19 @@ int launch_few_t(const void *w, const void *x, const float *rs, const LinEpi &e,
   return gq_last_launch();
 }
 template <int FMT>
-int launch_rows_t(const void *w, const _Float16 *a16, int lda, const float *rs, const LinEpi &e, float *part, int parts, int M, int N, int K,
-                  hipStream_t s) {
+int launch_rows_t(const void *w, const _Float16 *a16, int lda, const float *rs, const LinEpi &e, int M, int N, int K, hipStream_t s) {
   const int units = (int)(gq_kpad(FMT, K) / 128);
   const size_t tiles = gq_tiles(N);
-#define GQ_ROWS(MT, R, KS, PD)                                                                                              \
-  hipLaunchKernelGGL((k_lin_rows<FMT, MT, R, KS, PD>), dim3((unsigned)((tiles + (R)-1) / (R)), (unsigned)parts), dim3(64 * (KS)), 0, s, \
-                     (const uint8_t *)w, gq_sc_plane_offset(FMT, N, K), a16, lda, rs, e, parts > 1 ? part : nullptr, M, N,   \
-                     (int)gq_chunks(FMT, K), units)
-  const char *ev = getenv("GQ_DEV"); const int v = ev ? atoi(ev) : 0;
-  if (M > 32) {
-    if (v == 1) GQ_ROWS(4, 2, 4, 2);
-    else if (v == 2) GQ_ROWS(4, 2, 4, 1);
-    else if (v == 3) GQ_ROWS(4, 2, 8, 1);
-    else if (v == 4) GQ_ROWS(4, 1, 4, 2);
-    else if (v == 5) GQ_ROWS(4, 1, 8, 1);
-    else GQ_ROWS(4, 1, 8, 2);
-  } else if (M > 16) {
-    if (v == 1) GQ_ROWS(2, 2, 4, 2);
-    else if (v == 2) GQ_ROWS(2, 2, 4, 1);
-    else if (v == 3) GQ_ROWS(2, 2, 8, 2);
-    else if (v == 4) GQ_ROWS(2, 1, 4, 2);
-    else if (v == 5) GQ_ROWS(2, 1, 4, 4);
-    else GQ_ROWS(2, 1, 8, 2);
-  } else {
-    if (v == 1) GQ_ROWS(1, 2, 4, 2);
-    else if (v == 2) GQ_ROWS(1, 2, 8, 2);
-    else if (v == 3) GQ_ROWS(1, 1, 8, 2);
-    else if (v == 4) GQ_ROWS(1, 1, 16, 2);
-    else GQ_ROWS(1, 1, 4, 4);
-  }
+#define GQ_ROWS(R, KS, PD)                                                                                               \
+  hipLaunchKernelGGL((k_lin_rows<FMT, 1, R, KS, PD>), dim3((unsigned)((tiles + (R)-1) / (R))), dim3(64 * (KS)), 0, s,      \
+                     (const uint8_t *)w, gq_sc_plane_offset(FMT, N, K), a16, lda, rs, e, M, N, (int)gq_chunks(FMT, K), units)
+  // Two tiles share the rows of x where there are workgroups enough; long rows by few waves (16 rows, us by two tiles and 4 waves / one
+  // and 8 / one and 4, deeper: 14336 x 4096 Q4_K 15.6 / 22 / 19.6; 4096 x 14336 24.4 / 21.8 / 19.5; 4096 x 4096 Q4_0 9.6 / 8.1 / 8.4)
+  if (tiles > 512) GQ_ROWS(2, 4, 2);
+  else if (units > 64) GQ_ROWS(1, 4, 4);
+  else GQ_ROWS(1, 8, 2);
 #undef GQ_ROWS
-  GQ_TRY(gq_last_launch());
-  return parts > 1 ? launch_sum(part, e, M, N, parts, s) : GQ_OK;
+  return gq_last_launch();
 }
 
 // ---- backward ----------------------------------------------------------------------
@@ -425,28 +385,28 @@ int check_linear(int fmt, const void *w, size_t M, size_t N, size_t K, int act) 
   return GQ_OK;
 }
 
-constexpr size_t kFew = 4, kRows = 64;
+constexpr size_t kFew = 4, kRows = 16;
 constexpr size_t kFewLds = 65536;  // values of x that LDS takes beside the waves' sums
 // Rows a call takes at a time: their fp16 copies stay below 64 MiB, but for the rows that the kernels of few rows take at
-// once (64 of at most 2^24 columns: 2 GiB, 32-bit offsets still)
+// once (16 of at most 2^24 columns: 512 MiB)
 size_t linear_rows(int fmt, size_t M, size_t K) {
   const size_t fit = ((size_t)64 << 20) / (2 * gq_kpad(fmt, K));
   const size_t mb = fit >= 256 ? fit & ~(size_t)255 : fit > kRows ? fit : kRows;
   return M < mb ? M : mb;
 }
 
-// Parts of K for rows that the kernels of few rows take
-int row_parts(size_t M, size_t N, size_t K, int units) {
-  const char *ev = getenv("GQ_PARTS");
-  return ev ? atoi(ev) : 1;
-}
-
 }  // namespace
+
+int gq_launch_linear_sum(const float *part, const void *epi, int M, int N, int parts, hipStream_t s) {
+  hipLaunchKernelGGL(k_lin_sum, dim3((unsigned)((N + 255) / 256), (unsigned)M), dim3(256), 0, s, part,
+                     *reinterpret_cast<const LinEpi *>(epi), M, N, parts);
+  return gq_last_launch();
+}
 
 extern "C" size_t gq_linear_workspace_bytes(int fmt, size_t M, size_t N, size_t K) {
   if (!gq_fmt_valid(fmt) || M > GQ_MAX_DIM || N > GQ_MAX_DIM || K > GQ_MAX_DIM || K == 0) return 0;
   const size_t mb = linear_rows(fmt, M, K);
-  return gq_align256(mb * (gq_kpad(fmt, K) + 8) * 2) + gq_align256((mb + 256) * 4) + (M <= 64 ? 8 * M * N * 4 : 0);
+  return gq_align256(mb * (gq_kpad(fmt, K) + 8) * 2) + gq_align256((mb + 256) * 4) + std::min(kLinParts * mb * N * 4, kLinPartBytes);
 }
 
 extern "C" int gq_linear(int fmt, const void *w, const void *x, int x_dtype, const void *bias, int bias_dtype, int act,
@@ -484,12 +444,11 @@ extern "C" int gq_linear(int fmt, const void *w, const void *x, int x_dtype, con
     GQ_TRY(gq_launch_a_to_f16(x, x_dtype, a16, rs, (int)M, (int)K, (int)K, 0, s));
     return few(a16, GQ_DT_F16, rs);
   }
+  float *part = (float *)((uint8_t *)rs + gq_align256((mb + 256) * 4));
   if (M <= kRows) {  // rows 16 bytes longer than a multiple of 4 KiB, where 16 of them would collide
     const int ld = (int)Kp + 8;
     GQ_TRY(gq_launch_a_to_f16(x, x_dtype, a16, rs, (int)M, (int)K, ld, q4, s));
-    float *part = (float *)((uint8_t *)rs + gq_align256((mb + 256) * 4));
-    const int parts = row_parts(M, N, K, (int)(Kp / 128));
-#define GQ_ROWS_F(F) launch_rows_t<F>(w, a16, ld, rs, e, part, parts, (int)M, (int)N, (int)K, s)
+#define GQ_ROWS_F(F) launch_rows_t<F>(w, a16, ld, rs, e, (int)M, (int)N, (int)K, s)
     if (fmt == GQ_FMT_Q4_0) return GQ_ROWS_F(GQ_FMT_Q4_0);
     if (fmt == GQ_FMT_Q8_0) return GQ_ROWS_F(GQ_FMT_Q8_0);
     if (gq_fmt_is_q6k(fmt)) return GQ_ROWS_F(GQ_FMT_Q6_K);
@@ -504,7 +463,7 @@ extern "C" int gq_linear(int fmt, const void *w, const void *x, int x_dtype, con
     b.resid = resid ? (const uint8_t *)resid + m0 * ys : nullptr;
     b.y = (uint8_t *)y + m0 * ys;
     b.z = z ? (uint8_t *)z + m0 * ys : nullptr;
-    GQ_TRY(gq_launch_linear_rb(fmt, w, a16, rs, &b, m, (int)N, (int)K, s));
+    GQ_TRY(gq_launch_linear_rb(fmt, w, a16, rs, &b, part, m, (int)N, (int)K, s));
   }
   return GQ_OK;
 }

@@ -1,4 +1,5 @@
 // gq_linear_rb.hip -- the tiled product with bias, activation and residual in its epilogue over T16 weights.
+#include <algorithm>
 #include <type_traits>
 
 #include "gq_gemm_frag.h"
@@ -226,34 +227,57 @@ k_lin_rb(const uint8_t *__restrict__ w, uint32_t sc_off, const _Float16 *__restr
 }
 
 template <int FMT, int BM, int WN, int NJ, int PD, int KG>
-int launch_rb(const void *w, const _Float16 *a16, const float *rs, const LinEpi &e, int M, int N, int K, hipStream_t s) {
+int launch_rb(const void *w, const _Float16 *a16, const float *rs, const LinEpi &e, float *part, int parts, int M, int N, int K,
+              hipStream_t s) {
   const int tiles_m = (M + BM - 1) / BM, tiles_n = (N + 32 * NJ * WN - 1) / (32 * NJ * WN);
   GQ_CHECK((size_t)tiles_m * (size_t)tiles_n <= 0x7FFFFFFFu, GQ_ERR_INVALID_ARGS);  // (one grid dimension)
   const int nsteps = (int)(gq_kpad(FMT, K) / BK);
-  hipLaunchKernelGGL((k_lin_rb<FMT, BM, WN, NJ, PD, KG>), dim3((unsigned)(tiles_m * tiles_n)), dim3(64 * WN * KG), 0, s,
-                     (const uint8_t *)w, (uint32_t)gq_sc_plane_offset(FMT, N, K), a16, (int)gq_kpad(FMT, K), rs, e, (float *)nullptr,
-                     M, N, (int)gq_chunks(FMT, K), nsteps, nsteps, tiles_m);
-  return gq_last_launch();
+  parts = (int)std::min((size_t)parts, kLinPartBytes / ((size_t)M * (size_t)N * 4));  // (what their sums have room for)
+  const int sps = parts > 1 ? ((nsteps + parts - 1) / parts + KG - 1) / KG * KG : nsteps;
+  const int np = (nsteps + sps - 1) / sps;  // (no part is empty)
+  hipLaunchKernelGGL((k_lin_rb<FMT, BM, WN, NJ, PD, KG>), dim3((unsigned)(tiles_m * tiles_n), (unsigned)np), dim3(64 * WN * KG), 0, s,
+                     (const uint8_t *)w, (uint32_t)gq_sc_plane_offset(FMT, N, K), a16, (int)gq_kpad(FMT, K), rs, e,
+                     np > 1 ? part : (float *)nullptr, M, N, (int)gq_chunks(FMT, K), nsteps, sps, tiles_m);
+  GQ_TRY(gq_last_launch());
+  return np > 1 ? gq_launch_linear_sum(part, &e, M, N, np, s) : GQ_OK;
 }
 template <int FMT>
-int launch_fmt(const void *w, const _Float16 *a16, const float *rs, const LinEpi &e, int M, int N, int K, hipStream_t s) {
-#define GQ_RB(...) launch_rb<FMT, __VA_ARGS__>(w, a16, rs, e, M, N, K, s)
+int launch_fmt(const void *w, const _Float16 *a16, const float *rs, const LinEpi &e, float *part, int M, int N, int K, hipStream_t s) {
   auto wgs = [&](int bm, int bn) { return (size_t)((M + bm - 1) / bm) * (size_t)((N + bn - 1) / bn); };
-  const int nsteps = (int)(gq_kpad(FMT, K) / BK);
-  if (wgs(256, 256) >= 384) return GQ_RB(256, 8, 1, 3, 1);
-  if (wgs(128, 256) >= 192) return GQ_RB(128, 8, 1, 4, 1);
-  if (wgs(128, 128) >= 192 || nsteps % 4) return GQ_RB(128, 4, 1, 4, 2);  // (a step count is even)
-  return GQ_RB(64, 4, 1, 3, 4);
+  const int nsteps = (int)(gq_kpad(FMT, K) / BK);  // (even)
+  // parts of K as far as a workgroup a CU and at least four rounds of the groups a part go
+  auto parts = [&](size_t tiles, int kg) {
+    return (int)std::max((size_t)1, std::min({256 / std::max(tiles, (size_t)1), (size_t)(nsteps / (4 * kg)), (size_t)kLinParts}));
+  };
+#define GQ_RB(P, ...) launch_rb<FMT, __VA_ARGS__>(w, a16, rs, e, part, P, M, N, K, s)
+  // About one workgroup a CU, by tiles of 256 x 256, 128 x 256, 64 x 256 in two K groups, 64 x 128 in four, 32 x 64 in four, us with the conversion
+  // of x (Q4_K, bf16; the 64-row tiles in two and four groups of M x 4096 x 14336 within 3 %):
+  //   2048 x 4096 x 14336                251 by 128 x 256, one round
+  //   512 x 4096 x 14336 (Q6_K)          86 by 128 x 256 in 4 parts, 101 by 64 x 256 in 2, 98 by 64 x 128
+  //   256 x 14336 x 4096                 46 by 64 x 256 (and by 128 x 128), 53 by 64 x 128
+  //   128 x 14336 x 4096                 39 by 64 x 256, 29 by 64 x 128, 51 by 32 x 64
+  //   256 x 4096 x 14336                 63, 49 by 64 x 128 in 1, 2 parts; 72 by 32 x 64
+  //   64 x 4096 x 14336                  56, 35, 25 by 64 x 128 in 1, 2, 4 parts; 36, 25, 27 by 32 x 64
+  //   64 x 4096 x 4096 (Q4_0)            23, 17, 15.5; 15.2, 13.5, 16.6
+  //   32 x 4096 x 14336                  56, 34, 24; 35, 23, 18.7 (16-row fragments as for fewer rows: 23)
+  //   64 x 14336 x 4096                  25.6 by 64 x 128, 27.8 by 32 x 64
+  if (wgs(256, 256) >= 384) return GQ_RB(1, 256, 8, 1, 3, 1);
+  const size_t wide = wgs(128, 256);
+  if (wide >= 192 || (wide >= 64 && M >= 256 && nsteps >= 128)) return GQ_RB(parts(wide, 1), 128, 8, 1, 4, 1);
+  if (wgs(64, 256) >= 192) return GQ_RB(1, 64, 8, 1, 4, 2);
+  if (nsteps % 4) return GQ_RB(parts(wgs(64, 128), 2), 64, 4, 1, 4, 2);
+  if (M <= 64 && wgs(32, 64) <= 256) return GQ_RB(parts(wgs(32, 64), 4), 32, 2, 1, 4, 4);
+  return GQ_RB(parts(wgs(64, 128), 4), 64, 4, 1, 3, 4);
 #undef GQ_RB
 }
 
 }  // namespace
 
-int gq_launch_linear_rb(int fmt, const void *w, const _Float16 *a16, const float *rs, const void *epi, int M, int N, int K,
+int gq_launch_linear_rb(int fmt, const void *w, const _Float16 *a16, const float *rs, const void *epi, float *part, int M, int N, int K,
                         hipStream_t s) {
   const LinEpi &e = *reinterpret_cast<const LinEpi *>(epi);
-  if (fmt == GQ_FMT_Q4_0) return launch_fmt<GQ_FMT_Q4_0>(w, a16, rs, e, M, N, K, s);
-  if (fmt == GQ_FMT_Q8_0) return launch_fmt<GQ_FMT_Q8_0>(w, a16, rs, e, M, N, K, s);
-  if (gq_fmt_is_q6k(fmt)) return launch_fmt<GQ_FMT_Q6_K>(w, a16, rs, e, M, N, K, s);
-  return launch_fmt<GQ_FMT_Q4_K>(w, a16, rs, e, M, N, K, s);
+  if (fmt == GQ_FMT_Q4_0) return launch_fmt<GQ_FMT_Q4_0>(w, a16, rs, e, part, M, N, K, s);
+  if (fmt == GQ_FMT_Q8_0) return launch_fmt<GQ_FMT_Q8_0>(w, a16, rs, e, part, M, N, K, s);
+  if (gq_fmt_is_q6k(fmt)) return launch_fmt<GQ_FMT_Q6_K>(w, a16, rs, e, part, M, N, K, s);
+  return launch_fmt<GQ_FMT_Q4_K>(w, a16, rs, e, part, M, N, K, s);
 }
