@@ -1234,6 +1234,9 @@ struct DxShape {
 // (Q4_K, K = 4096: 128 x 14336 by the second shape 73.4 us, the third 94.5; 128 x 5003 41.4 and 54.8)
 constexpr DxShape kDxShapes[3] = {{32, 128, 4, 32}, {64, 128, 4, 128}, {128, 256, 2, ~(size_t)0}};
 
+size_t dx_tiles(const DxShape &t, size_t rows, size_t K) {
+  return ((rows + t.bm - 1) / t.bm) * ((K + t.bn - 1) / t.bn);
+}
 GqDxPlan dx_plan(size_t M, size_t N, size_t K, int mats) {
   GqDxPlan p;
   p.mats = mats;
@@ -1245,8 +1248,11 @@ GqDxPlan dx_plan(size_t M, size_t N, size_t K, int mats) {
   const size_t nsteps = mats * p.np / 64;
   p.shape = 0;
   while (p.mb > kDxShapes[p.shape].rows) ++p.shape;
+  // One matrix has half the steps to go round: the second shape also where it gives no more than a workgroup a CU (us by the second / the
+  // third: 512 rows, 4096 x 4096 Q8_0 40.6 / 49.7; 203, 5003 x 4096 Q6_K 43.4 / 44.8; 256, 4096 x 14336 Q4_K 69.6 / 63.6)
+  if (mats == 1 && p.shape == 2 && dx_tiles(kDxShapes[1], p.mb, K) <= 256) p.shape = 1;
   const DxShape &t = kDxShapes[p.shape];
-  const size_t wgs = ((p.mb + t.bm - 1) / t.bm) * ((K + t.bn - 1) / t.bn);
+  const size_t wgs = dx_tiles(t, p.mb, K);
   size_t want = wgs >= 192 ? 1 : 256 / wgs;
   const size_t most = nsteps / (4 * t.kg);  // at least four steps a group
   if (want > most) want = most < 1 ? 1 : most;
@@ -1278,7 +1284,7 @@ size_t dx_most_bytes(size_t M, size_t N, size_t K, int mats) {
     const DxShape &t = kDxShapes[i];
     const size_t tk = (K + t.bn - 1) / t.bn, tiles = 128 / tk, parts = std::min(nsteps / (4 * t.kg), 256 / tk);
     GqDxPlan q = p;  // the most rows of this shape that have parts
-    q.mb = std::min({p.mb, t.rows, tiles * t.bm});
+    q.mb = std::min({p.mb, mats == 1 && i == 1 ? p.mb : t.rows, tiles * t.bm});
     if (q.mb <= (i ? kDxShapes[i - 1].rows : 0) || parts < 2) continue;
     const size_t sums = std::min((size_t)256 * t.bm * t.bn, parts * q.mb * K);
     // (dx_plan keeps plans with parts below kGqScratchMax)

@@ -10,23 +10,31 @@ struct LinEpi {
   int bias_dt, dt, act;      // dt: of resid, y and z
 };
 
-// x / sqrt(2) with the error function: Phi(x) = erfc(-x / sqrt(2)) / 2 keeps its relative accuracy where it is small
-GQ_DEV float lin_phi(float x) { return 0.5f * erfcf(-0.7071067811865476f * x); }
-GQ_DEV float lin_act(int act, float z) {
-  if (act == GQ_ACT_NONE) return z;
-  if (act == GQ_ACT_RELU) return z < 0.f ? 0.f : z;  // (a NaN stays one)
-  if (act == GQ_ACT_GELU) return z * lin_phi(z);
-  return gq_act_f(act, z);
+// act(z) = z gate(z): 1, z > 0, or as in gq_act.h sigmoid(p(z)), p = a z + b z^3 = z for SiLU and 2 sqrt(2 / pi) (z + 0.044715 z^3) for the
+// tanh form of GELU, |z| cut at 100, where the sigmoid is 0 or 1 in fp32, so that no power overflows.  One code for
+// both sigmoids: a tile's epilogue is unrolled over its outputs, and every case of an activation is fetched with it.
+struct LinAct {
+  float a, b;
+  bool relu;
+};
+GQ_DEV LinAct lin_act_of(int act) {
+  const bool g = act == GQ_ACT_GELU_TANH;
+  return LinAct{g ? kGelu1 : 1.f, g ? kGelu1 * kGelu3 : 0.f, act == GQ_ACT_RELU};
 }
-GQ_DEV float lin_act_d(int act, float z) {
-  if (act == GQ_ACT_NONE) return 1.f;
-  if (act == GQ_ACT_RELU) return z <= 0.f ? 0.f : 1.f;
-  if (act == GQ_ACT_GELU) {
-    // Phi(z) + z phi(z), phi the normal density
-    return lin_phi(z) + z * 0.3989422804014327f * __expf(-0.5f * fminf(z * z, 1e30f));
-  }
+GQ_DEV float lin_cut(float z) { return fminf(fmaxf(z, -100.f), 100.f); }
+// (not GQ_ACT_NONE; a NaN stays one)
+GQ_DEV float lin_act_f(const LinAct &t, float z) {
+  const float c = lin_cut(z), s = gq_sigmoid(c * fmaf(t.b * c, c, t.a));
+  return t.relu ? (z < 0.f ? 0.f : z) : z * s;
+}
+GQ_DEV float lin_act(int act, float z) { return act == GQ_ACT_NONE ? z : lin_act_f(lin_act_of(act), z); }
+// act'(z): s + c p' s (1 - s)
+template <int ACT>
+GQ_DEV float lin_act_d(float z) {
+  if constexpr (ACT == GQ_ACT_NONE) return 1.f;
+  if constexpr (ACT == GQ_ACT_RELU) return z <= 0.f ? 0.f : 1.f;
   float f, d;
-  gq_act_fd(act, z, f, d);
+  gq_act_fd(ACT, z, f, d);
   return d;
 }
 // bias and residual of output (m, n), loaded ahead of the sums; the output of a product's sum v

@@ -226,34 +226,36 @@ int launch_rows_t(const void *w, const _Float16 *a16, int lda, const float *rs, 
 // dz = dy act'(z): one pass over dy and z, a workgroup a row at a time (row blockIdx.x, + gridDim.x, ...).  dz goes out in its own
 // type where it is wanted, and, as it is before that rounding, to fp16 with one power-of-two scale per row (the row's
 // largest to [2^14, 2^15); 2^-114 to 2^126), padded with zeros to np columns: the A operand of dx.  The workgroup's rows are summed
-// by column into its row of `part` (dbias), which a last kernel adds over the workgroups in their order.  The first kDzRuns
-// * 4096 columns of a row and their sums stay in registers, the rest is computed twice and summed in `part`.
-constexpr int kDzThreads = 512, kDzRuns = 4;
-template <int DT>
+// by column into its row of `part` (dbias), which a last kernel adds over the workgroups in their order.  The first RUNS * 4096
+// columns of a row and their sums stay in registers, the rest (RUNS = 4 alone) is computed twice and summed in `part`.  The row's last,
+// ragged run is one thread's, on a path of its own: a launch starts with its code to be fetched, and every unrolled run's
+// copy of it counts (203 x 5003 fp16, tanh-GELU: 13.3 us with all activations and runs in one kernel, 8.0 so;
+// 2048 x 14336 bf16, ReLU, 44 us, 250 MB).
+constexpr int kDzThreads = 512;
+template <int DT, int ACT, int RUNS>
 __global__ void __launch_bounds__(kDzThreads) k_lin_dz(const void *dy, const void *z, void *dzo, _Float16 *a16, float *rs,
-                                                       float *part, int add, int M, int N, int np, int act) {
+                                                       float *part, int add, int M, int N, int np) {
   __shared__ float top_s[2][kDzThreads / 64];
+  constexpr int SPAN = 8 * kDzThreads * RUNS;
+  constexpr bool GATED = ACT != GQ_ACT_NONE, LONG = RUNS == 4;
   const int tid = threadIdx.x;
-  constexpr int SPAN = 8 * kDzThreads * kDzRuns;
-  float sum[kDzRuns][8];
+  auto run = [&](int i) { return 8 * (tid + kDzThreads * i); };
+  const int kt = N & ~7, it = kt / (8 * kDzThreads);  // the ragged run, and which of its thread's it is
+  const bool last = kt < N && kt < SPAN && kt / 8 % kDzThreads == tid;
+  float sum[RUNS][8];
   float *pr = part ? part + (size_t)blockIdx.x * (size_t)N : nullptr;
 #pragma unroll
-  for (int i = 0; i < kDzRuns; ++i)
+  for (int i = 0; i < RUNS; ++i)
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const int n = 8 * (tid + kDzThreads * i) + e;
-      sum[i][e] = part && add && n < N ? pr[n] : 0.f;
-    }
-  // whole runs of the next row are requested before a row's are used (whole: the row's last, ragged run is loaded in its turn)
-  FRaw<DT> ra[kDzRuns], rb[kDzRuns];
-  const bool gated = act != GQ_ACT_NONE;
+    for (int e = 0; e < 8; ++e) sum[i][e] = pr && add && run(i) + e < N ? pr[run(i) + e] : 0.f;
+  // whole runs of the next row are requested before a row's are used
+  FRaw<DT> ra[RUNS], rb[RUNS];
   auto request = [&](int m) __attribute__((always_inline)) {
 #pragma unroll
-    for (int i = 0; i < kDzRuns; ++i) {
-      const int k = 8 * (tid + kDzThreads * i);
-      if (m >= M || k + 8 > N) continue;
-      px_load<DT>(dy, (size_t)m * (size_t)N + k, ra[i]);
-      if (gated) px_load<DT>(z, (size_t)m * (size_t)N + k, rb[i]);
+    for (int i = 0; i < RUNS; ++i) {
+      if (m >= M || run(i) + 8 > N) continue;
+      px_load<DT>(dy, (size_t)m * (size_t)N + run(i), ra[i]);
+      if (GATED) px_load<DT>(z, (size_t)m * (size_t)N + run(i), rb[i]);
     }
   };
   request((int)blockIdx.x);
@@ -261,33 +263,28 @@ __global__ void __launch_bounds__(kDzThreads) k_lin_dz(const void *dy, const voi
   for (int m = (int)blockIdx.x; m < M; m += (int)gridDim.x, buf ^= 1) {
     const size_t row = (size_t)m * (size_t)N;
     auto grads = [&](int k, float (&o)[8]) __attribute__((always_inline)) {
-      float a[8], b[8];
-      dgu_load<DT>(dy, row, k, N, a);
-      if (!gated) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) o[e] = a[e];
-        return;
-      }
+      float b[8];
+      dgu_load<DT>(dy, row, k, N, o);
+      if (!GATED) return;
       dgu_load<DT>(z, row, k, N, b);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) o[e] = k + e < N ? a[e] * lin_act_d(act, b[e]) : 0.f;
+      for (int e = 0; e < 8; ++e) o[e] = k + e < N ? o[e] * lin_act_d<ACT>(b[e]) : 0.f;
     };
-    float d[kDzRuns][8], top = 0.f;
+    float d[RUNS][8], tail[8] = {}, top = 0.f;
+    if (last) grads(kt, tail);
 #pragma unroll
-    for (int i = 0; i < kDzRuns; ++i) {
-      const int k = 8 * (tid + kDzThreads * i);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) d[i][e] = 0.f;
-      if (k + 8 <= N) {
+    for (int i = 0; i < RUNS; ++i) {
+      if (run(i) + 8 <= N) {
         float b[8];
         px_floats<DT>(ra[i], true, d[i]);
-        if (gated) {
+        if (GATED) {
           px_floats<DT>(rb[i], true, b);
 #pragma unroll
-          for (int e = 0; e < 8; ++e) d[i][e] *= lin_act_d(act, b[e]);
+          for (int e = 0; e < 8; ++e) d[i][e] *= lin_act_d<ACT>(b[e]);
         }
-      } else if (k < N) {
-        grads(k, d[i]);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) d[i][e] = last && i == it ? tail[e] : 0.f;
       }
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
@@ -296,7 +293,7 @@ __global__ void __launch_bounds__(kDzThreads) k_lin_dz(const void *dy, const voi
       }
     }
     request(m + (int)gridDim.x);
-    if (a16)
+    if (LONG && a16)
       for (int k = SPAN + 8 * tid; k < N; k += 8 * kDzThreads) {
         float a[8];
         grads(k, a);
@@ -315,8 +312,7 @@ __global__ void __launch_bounds__(kDzThreads) k_lin_dz(const void *dy, const voi
       f2 = __uint_as_float((uint32_t)(127 + cut) << 23);
       if (tid == 0) rs[m] = __uint_as_float((uint32_t)(127 - cut) << 23);
     }
-    auto put = [&](int k, const float (&a)[8]) __attribute__((always_inline)) {
-      if (dzo && k < N) dgu_store<DT>(dzo, row, k, N, a);
+    auto put16 = [&](int k, const float (&a)[8]) __attribute__((always_inline)) {
       if (!a16 || k >= np) return;
       gq_half8 x;
 #pragma unroll
@@ -324,25 +320,37 @@ __global__ void __launch_bounds__(kDzThreads) k_lin_dz(const void *dy, const voi
       *reinterpret_cast<gq_half8 *>(a16 + (size_t)m * (size_t)np + k) = x;
     };
 #pragma unroll
-    for (int i = 0; i < kDzRuns; ++i) put(8 * (tid + kDzThreads * i), d[i]);
-    for (int k = SPAN + 8 * tid; k < (a16 ? np : N); k += 8 * kDzThreads) {
-      float a[8] = {};
-      if (k < N) grads(k, a);
-      put(k, a);
-      if (part)
+    for (int i = 0; i < RUNS; ++i) {
+      if (dzo && run(i) + 8 <= N) dgu_store<DT>(dzo, row, run(i), run(i) + 8, d[i]);
+      put16(run(i), d[i]);
+    }
+    if (dzo && last) dgu_store<DT>(dzo, row, kt, N, tail);
+    if (LONG)
+      for (int k = SPAN + 8 * tid; k < (a16 ? np : N); k += 8 * kDzThreads) {
+        float a[8] = {};
+        if (k < N) grads(k, a);
+        if (dzo && k < N) dgu_store<DT>(dzo, row, k, N, a);
+        put16(k, a);
+        if (pr)
 #pragma unroll
-        for (int e = 0; e < 8; ++e)
-          if (k + e < N) pr[k + e] = (add || m != (int)blockIdx.x ? pr[k + e] : 0.f) + a[e];
+          for (int e = 0; e < 8; ++e)
+            if (k + e < N) pr[k + e] = (add || m != (int)blockIdx.x ? pr[k + e] : 0.f) + a[e];
+      }
+  }
+  if (!pr) return;
+#pragma unroll
+  for (int i = 0; i < RUNS; ++i) {
+    if (run(i) + 8 <= N) {
+      FRun32 r;
+      r.v[0] = gq_f4{sum[i][0], sum[i][1], sum[i][2], sum[i][3]};
+      r.v[1] = gq_f4{sum[i][4], sum[i][5], sum[i][6], sum[i][7]};
+      *reinterpret_cast<FRun32 *>(pr + run(i)) = r;
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (run(i) + e < N) pr[run(i) + e] = sum[i][e];
     }
   }
-  if (!part) return;
-#pragma unroll
-  for (int i = 0; i < kDzRuns; ++i)
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const int n = 8 * (tid + kDzThreads * i) + e;
-      if (n < N) pr[n] = sum[i][e];
-    }
 }
 // dbias = the workgroups' sums, in an order of their own (none: zeros): 64 columns a workgroup, wave w adds parts w, w + 16, ...
 constexpr int kDbWaves = 16;
@@ -368,11 +376,25 @@ int launch_dbias(const float *part, float *db, size_t N, int parts, hipStream_t 
 template <int DT>
 int launch_dz(const void *dy, const void *z, void *dz, _Float16 *a16, float *rs, float *part, int add, int wgs, int M, int N,
               int np, int act, hipStream_t s) {
-  hipLaunchKernelGGL(k_lin_dz<DT>, dim3((unsigned)wgs), dim3(kDzThreads), 0, s, dy, z, dz, a16, rs, part, add, M, N, np, act);
+#define GQ_DZ_RUNS(ACT, RUNS) \
+  hipLaunchKernelGGL((k_lin_dz<DT, ACT, RUNS>), dim3((unsigned)wgs), dim3(kDzThreads), 0, s, dy, z, dz, a16, rs, part, add, M, N, np)
+  // (np: whole runs of the fp16 row)
+#define GQ_DZ_ACT(ACT)                                 \
+  do {                                                 \
+    if (np <= 8 * kDzThreads) GQ_DZ_RUNS(ACT, 1);      \
+    else if (np <= 16 * kDzThreads) GQ_DZ_RUNS(ACT, 2); \
+    else GQ_DZ_RUNS(ACT, 4);                           \
+  } while (0)
+  if (act == GQ_ACT_NONE) GQ_DZ_ACT(GQ_ACT_NONE);
+  else if (act == GQ_ACT_RELU) GQ_DZ_ACT(GQ_ACT_RELU);
+  else if (act == GQ_ACT_SILU) GQ_DZ_ACT(GQ_ACT_SILU);
+  else GQ_DZ_ACT(GQ_ACT_GELU_TANH);
+#undef GQ_DZ_ACT
+#undef GQ_DZ_RUNS
   return gq_last_launch();
 }
 
-bool lin_act_valid(int act) { return act >= GQ_ACT_SILU && act <= GQ_ACT_GELU; }
+bool lin_act_valid(int act) { return act >= GQ_ACT_SILU && act <= GQ_ACT_RELU; }
 
 int check_linear(int fmt, const void *w, size_t M, size_t N, size_t K, int act) {
   GQ_TRY(gq_check_shape(fmt, N, K));

@@ -189,6 +189,7 @@ k_lin_rb(const uint8_t *__restrict__ w, uint32_t sc_off, const _Float16 *__restr
           const_cast<uint8_t *>(reinterpret_cast<const uint8_t *>(p)) + (p ? (size_t)m0 * N * ES : 0), (short)0,
           p ? range(ES) : 0, 0x00020000);
     };
+    const LinAct act = lin_act_of(e.act);
     const __amdgpu_buffer_rsrc_t yr = rsrc(e.y), zr = rsrc(e.z), rr = rsrc(e.resid);  // (none: no range)
 #pragma unroll
     for (int i = 0; i < TM; ++i) {
@@ -213,12 +214,19 @@ k_lin_rb(const uint8_t *__restrict__ w, uint32_t sc_off, const _Float16 *__restr
             }
           }
         }
+        gq_f16v &z = acc[i][j];
 #pragma unroll
-        for (int v = 0; v < 16; ++v) {
-          const float z = fmaf(acc[i][j][v], rsv[v], b);
-          if (e.z) front_put<DT>(zr, at(v), e.dt, z);
-          front_put<DT>(yr, at(v), e.dt, lin_act(e.act, z) + res[v]);
+        for (int v = 0; v < 16; ++v) z[v] = fmaf(z[v], rsv[v], b);
+        if (e.z) {
+#pragma unroll
+          for (int v = 0; v < 16; ++v) front_put<DT>(zr, at(v), e.dt, z[v]);
         }
+        if (e.act != GQ_ACT_NONE) {
+#pragma unroll
+          for (int v = 0; v < 16; ++v) z[v] = lin_act_f(act, z[v]);
+        }
+#pragma unroll
+        for (int v = 0; v < 16; ++v) front_put<DT>(yr, at(v), e.dt, z[v] + res[v]);
       }
     }
   };

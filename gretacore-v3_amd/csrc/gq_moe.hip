@@ -336,8 +336,8 @@ GQ_DEV float moe_gu_h(At at, int nl, int m, float f, int act) {
 // Up to 4 tokens of 16-bit x: codes and x as they are, scales in fp32 (gq_rows_frag.h); row j is token j.  h goes out in fp16 (nib:
 // in the nibbles' order) with a power-of-two scale for each 32 of a row, the scale groups of W_down's products; the inverse of block
 // 2 m + i of 128 values to hs[pair][128s][i][m].
-// Workgroup (j, q): 32 columns of the expert that pair q names first.  ROUTE: the choice is made here, by every workgroup for itself (a
-// launch of its own cost XX us more); the first one keeps it.
+// Workgroup (j, q): 32 columns of the expert that pair q names first.  ROUTE: the choice is made here, by every workgroup for itself (8 of
+// 64 experts of 1024 x 2048: 20.5 us the layer, 23.1 with the choice in a launch of its own); the first one keeps it.
 template <int FMT, int XT, int MR, int KS, int PD, bool ROUTE>
 __global__ void __launch_bounds__(64 * KS)
 k_moe_gu_few(const uint8_t *__restrict__ wg, const uint8_t *__restrict__ wu, size_t sc_off, const void *__restrict__ x,

@@ -26,7 +26,7 @@ FORMATS = {"q4_0": FMT_Q4_0, "q8_0": FMT_Q8_0, "q4_k": FMT_Q4_K, "q4_k_ggml": FM
 
 DT_F32, DT_F16, DT_BF16 = 0, 1, 2
 ACT_SILU, ACT_GELU_TANH = 0, 1
-ACT_NONE, ACT_RELU, ACT_GELU = 2, 3, 4  # linear only
+ACT_NONE, ACT_RELU = 2, 3  # linear only
 SCORE_SOFTMAX, SCORE_SIGMOID = 0, 1
 MOE_MAX_TOKENS, MOE_MAX_EXPERTS, MOE_MAX_TOP = 64, 1024, 16
 MAX_BATCH = 16
@@ -575,15 +575,17 @@ def gemv_swiglu_plan(fmt: int, n: int, k: int, batch: int):
 # one given (inputs of other streams are the caller's to order, as for torch's own).  The checks are few
 # attribute reads (a 4-bit GEMV's kernel runs 4 us); the messages are made only when one fails.
 _dts = {}  # torch dtype -> DT_*
-_empty = _current_device = _f32 = None
+_empty = _current_device = _f32 = _i32 = None
 
 
 def _init_torch():
-    global _empty, _current_device, _f32
+    global _empty, _current_device, _f32, _i32
     import torch
-    _f32 = torch.float32
+    _f32, _i32 = torch.float32, torch.int32
     _dts.update({torch.float32: DT_F32, torch.float16: DT_F16, torch.bfloat16: DT_BF16})
     _empty, _current_device = torch.empty, torch.cuda.current_device
+    if torch.cuda.is_available():
+        _stream()  # (initialises _raw_stream)
 
 
 def _on(stream, call, *args):
@@ -774,18 +776,19 @@ def linear(fmt: int, w, x, n: int, k: int, bias=None, act: int = ACT_NONE, resid
     if resid is not None:
         _operand(resid, (m, n), "resid", device, dtype)
     if y is None:
-        y = _empty((m, n), dtype=dtype, device=x.device)
+        y = x.new_empty(m, n, dtype=dtype) if dtype != x.dtype else x.new_empty(m, n)
     else:
         _operand(y, (m, n), "y", device)
     if z is not None:
         _operand(z, (m, n), "z", device, dtype)
     elif save:
-        z = _empty((m, n), dtype=dtype, device=x.device)
+        z = y.new_empty(m, n)
     ws_ptr, ws_n = None, 0
-    if workspace is not None:
+    # (one to four rows of 16-bit x need none)
+    if workspace is not None and (m > 4 or m * (k + 255) > 65536 or x.dtype == _f32):
         ws_ptr, ws_n = _room(workspace, _linear_bytes(False, fmt, m, n, k), device)
     st = load().gq_linear(fmt, w.data_ptr(), x.data_ptr(), _dt(x.dtype), _ptr(bias), bias_dt, act, _ptr(resid), y.data_ptr(),
-                          _dt(dtype), _ptr(z), m, n, k, ws_ptr, ws_n, _stream())
+                          _dt(dtype), _ptr(z), m, n, k, ws_ptr, ws_n, _raw_stream(device))
     if st:
         check(st, "gq_linear")
     return y if z is None else (y, z)
@@ -811,21 +814,21 @@ def linear_bwd(fmt: int, w, dy, z, n: int, k: int, act: int = ACT_NONE, want_dx:
     if dx is not None:
         _operand(dx, (m, k), "dx", device)
     elif want_dx:
-        dx = _empty((m, k), dtype=dx_dtype or dtype, device=dy.device)
+        dx = dy.new_empty(m, k, dtype=dx_dtype or dtype)
     if dz is not None:
         _operand(dz, (m, n), "dz", device, dtype)
     elif want_dz:
-        dz = _empty((m, n), dtype=dtype, device=dy.device)
+        dz = dy.new_empty(m, n)
     if dbias is not None or want_dbias:
         if dbias is None:
-            dbias = _empty((n,), dtype=_f32, device=dy.device)
+            dbias = dy.new_empty(n, dtype=_f32)
         else:
             _operand(dbias, (n,), "dbias", device, _f32)
     ws_ptr, ws_n = None, 0
     if workspace is not None:
         ws_ptr, ws_n = _room(workspace, _linear_bytes(True, fmt, m, n, k), device)
     st = load().gq_linear_bwd(fmt, w.data_ptr(), dy.data_ptr(), _ptr(z), _dt(dtype), act, _ptr(dz), _ptr(dx),
-                              _dt(dx.dtype if dx is not None else dtype), _ptr(dbias), m, n, k, ws_ptr, ws_n, _stream())
+                              _dt(dx.dtype if dx is not None else dtype), _ptr(dbias), m, n, k, ws_ptr, ws_n, _raw_stream(device))
     if st:
         check(st, "gq_linear_bwd")
     return {"dx": dx, "dz": dz, "dbias": dbias}
@@ -857,13 +860,12 @@ def _expert_operands(fmt, gate, up, fmt_down, down, n, k, n_experts, device):
 
 
 def _choice(ids, weights, m, top_k, x, device):
-    import torch
     if ids is None:
-        ids = _empty((m, top_k), dtype=torch.int32, device=x.device)
+        ids = x.new_empty(m, top_k, dtype=_i32)
     else:
-        _operand(ids, (m, top_k), "ids", device, torch.int32)
+        _operand(ids, (m, top_k), "ids", device, _i32)
     if weights is None:
-        weights = _empty((m, top_k), dtype=_f32, device=x.device)
+        weights = x.new_empty(m, top_k, dtype=_f32)
     else:
         _operand(weights, (m, top_k), "weights", device, _f32)
     return ids, weights
@@ -884,7 +886,7 @@ def moe_route(router, x, k: int, n_experts: int, top_k: int, score: int = SCORE_
     if workspace is not None:
         ws_ptr, ws_n = _room(workspace, load().gq_moe_route_workspace_bytes(ctypes.addressof(layer), m), device)
     st = load().gq_moe_route(ctypes.addressof(layer), x.data_ptr(), _dt(x.dtype), ids.data_ptr(), weights.data_ptr(), m, ws_ptr,
-                             ws_n, _stream())
+                             ws_n, _raw_stream(device))
     if st:
         check(st, "gq_moe_route")
     return ids, weights
@@ -931,7 +933,7 @@ def _moe_call(route, fmt, gate, up, fmt_down, down, router, x, n, k, n_experts, 
     if resid is not None:
         _operand(resid, (m, k), "resid", device, dtype)
     if y is None:
-        y = _empty((m, k), dtype=dtype, device=x.device)
+        y = x.new_empty(m, k, dtype=dtype) if dtype != x.dtype else x.new_empty(m, k)
     else:
         _operand(y, (m, k), "y", device)
     layer = MoeLayer(fmt, fmt_down, act, top_k, gate.data_ptr(), up.data_ptr(), down.data_ptr(), n_experts, n, k, _ptr(router),
@@ -942,10 +944,10 @@ def _moe_call(route, fmt, gate, up, fmt_down, down, router, x, n, k, n_experts, 
     at = ctypes.addressof(layer)
     if route:
         st = load().gq_moe_layer(at, x.data_ptr(), _dt(x.dtype), _ptr(resid), y.data_ptr(), _dt(dtype), _ptr(ids), _ptr(weights),
-                                 m, ws_ptr, ws_n, _stream())
+                                 m, ws_ptr, ws_n, _raw_stream(device))
     else:
         st = load().gq_moe_ffn(at, x.data_ptr(), _dt(x.dtype), ids.data_ptr(), weights.data_ptr(), _ptr(resid), y.data_ptr(),
-                               _dt(dtype), m, ws_ptr, ws_n, _stream())
+                               _dt(dtype), m, ws_ptr, ws_n, _raw_stream(device))
     if st:
         check(st, "gq_moe_layer" if route else "gq_moe_ffn")
     return y

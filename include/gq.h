@@ -334,10 +334,9 @@ int gq_w4_gate_up(const void *d_gate, const void *d_up, int group, const void *d
  * after a power-of-two scale per row; up to 64 rows keep the k-quants' d (and dmin) in fp32, more
  * fold them into fp16 weights. */
 #define GQ_ACT_NONE 2 /* z */
-#define GQ_ACT_RELU 3 /* max(z, 0) */
-#define GQ_ACT_GELU 4 /* z Phi(z), Phi the normal distribution; beside these GQ_ACT_SILU and GQ_ACT_GELU_TANH */
-/* A workspace of NULL takes scratch memory of the call's own, as in gq_ffn_gate_up; calls that need none (up to
- * four 4-byte aligned rows of 16-bit x) run without under capture too.  The bytes for M rows are enough for every call of
+#define GQ_ACT_RELU 3 /* max(z, 0); beside these GQ_ACT_SILU and GQ_ACT_GELU_TANH */
+/* A workspace of NULL takes scratch memory of the call's own, as in gq_ffn_gate_up; calls that need none (the rows of
+ * x that go in as they are) run without under capture too.  The bytes for M rows are enough for every call of
  * fewer.  N * 256 outputs stay below 2^31 bytes; K == 0 is refused. */
 size_t gq_linear_workspace_bytes(int fmt, size_t M, size_t N, size_t K);
 int gq_linear(int fmt, const void *d_packed, const void *d_x, int x_dtype, const void *d_bias, int bias_dtype, int act,

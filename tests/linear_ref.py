@@ -12,9 +12,6 @@ def act_grad(act, z):
         return z, torch.ones_like(z)
     if act == gq.ACT_RELU:
         return z.clamp(min=0), (z > 0).double()
-    if act == gq.ACT_GELU:
-        cdf = 0.5 * torch.erfc(-z / math.sqrt(2))
-        return z * cdf, cdf + z * torch.exp(-0.5 * z * z) / math.sqrt(2 * math.pi)
     if act == gq.ACT_SILU:
         s = torch.sigmoid(z)
         return z * s, s + z * s * torch.sigmoid(-z)

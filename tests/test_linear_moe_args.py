@@ -9,7 +9,7 @@ from linear_ref import act_grad
 P = 4096  # a non-null address that no refused or empty call touches
 OK, INVALID, UNSUPPORTED, WORKSPACE = 0, 1, 2, 4
 BIG = (1 << 24) + 32
-ACTS = [gq.ACT_SILU, gq.ACT_GELU_TANH, gq.ACT_NONE, gq.ACT_RELU, gq.ACT_GELU]
+ACTS = [gq.ACT_SILU, gq.ACT_GELU_TANH, gq.ACT_NONE, gq.ACT_RELU]
 
 
 def linear(fmt=gq.FMT_Q4_0, w=P, x=P, xdt=gq.DT_BF16, bias=None, bdt=gq.DT_F32, act=gq.ACT_NONE, resid=None, y=P, dt=gq.DT_BF16,
@@ -24,7 +24,7 @@ def bwd(fmt=gq.FMT_Q4_0, w=P, dy=P, z=P, dt=gq.DT_BF16, act=gq.ACT_RELU, dz=P, d
 
 @pytest.mark.parametrize("call", [linear, bwd])
 @pytest.mark.parametrize("bad,status", [
-    (dict(fmt=3), UNSUPPORTED), (dict(fmt=gq.FMT_F16), UNSUPPORTED), (dict(act=5), UNSUPPORTED), (dict(act=-1), UNSUPPORTED),
+    (dict(fmt=3), UNSUPPORTED), (dict(fmt=gq.FMT_F16), UNSUPPORTED), (dict(act=4), UNSUPPORTED), (dict(act=-1), UNSUPPORTED),
     (dict(xdt=3), UNSUPPORTED), (dict(dt=-1), UNSUPPORTED), (dict(k=33), INVALID), (dict(fmt=gq.FMT_Q4_K, k=128), INVALID),
     (dict(n=BIG), INVALID), (dict(k=BIG), INVALID), (dict(m=BIG), INVALID), (dict(w=None), INVALID), (dict(w=P + 8), INVALID),
     (dict(k=0), INVALID),
