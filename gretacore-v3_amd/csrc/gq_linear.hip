@@ -59,10 +59,11 @@ k_lin_few(const uint8_t *__restrict__ w, size_t sc_off, const void *__restrict__
   const int np = 128 * units, stride = (int)few_lds_stride(np);
   const bool mine = few_mine<FMT>(lane) && (lane & 3) < M;
   const uint32_t x0 = mine ? (uint32_t)((lane & 3) * stride + 32 * g) : (uint32_t)(M * stride), xd = mine ? 256u : 0u;
-  FUnit<FMT> us[PD][R];
-  auto request = [&](int unit, int st) __attribute__((always_inline)) {
+  constexpr int G = kGroup<FMT>;
+  FUnit<FMT> us[PD][R][G];
+  auto request = [&](int group, int st) __attribute__((always_inline)) {
 #pragma unroll
-    for (int t = 0; t < R; ++t) load_unit<FMT>(tl[t], unit, lane, us[st][t]);
+    for (int t = 0; t < R; ++t) load_group<FMT>(tl[t], group, lane, us[st][t]);
   };
   float acc[R][MR] = {};
   uint32_t mg;  // (kept in a register)
@@ -71,11 +72,11 @@ k_lin_few(const uint8_t *__restrict__ w, size_t sc_off, const void *__restrict__
   constexpr uint32_t one = XT == GQ_DT_F16 ? 0x3C003C00u : 0x3F803F80u;
   const gq_u4 ones = {one, one, one, one};
   const gq_f4 zero = {0.f, 0.f, 0.f, 0.f};
-  auto compute = [&](int unit, int st) __attribute__((always_inline)) {
+  auto add = [&](int unit, int st, int p) __attribute__((always_inline)) {
     const uint32_t at = x0 + xd * (uint32_t)unit;
     float s[R][2], mn[R][2];
 #pragma unroll
-    for (int t = 0; t < R; ++t) few_scales<FMT>(us[st][t], unit, g & (NG - 1), s[t], mn[t]);
+    for (int t = 0; t < R; ++t) few_scales<FMT>(us[st][t][p], unit, g & (NG - 1), s[t], mn[t]);
 #pragma unroll
     for (int m = 0; m < 2; ++m) {
       const gq_u4 a0 = few_lds(xs_s, at, m, 0), a1 = few_lds(xs_s, at, m, 1);
@@ -84,7 +85,7 @@ k_lin_few(const uint8_t *__restrict__ w, size_t sc_off, const void *__restrict__
 #pragma unroll
       for (int t = 0; t < R; ++t) {
         gq_u4 b[2];
-        few_codes<FMT, XT>(us[st][t], m, mg, b);
+        few_codes<FMT, XT>(us[st][t][p], m, mg, b);
         const gq_f4 d = few_mfma<XT>(a1, b[1], few_mfma<XT>(a0, b[0], zero));
         const float o = FMT == GQ_FMT_Q4_K ? fmaf(s[t][m], OFF, mn[t][m]) : 0.f;
 #pragma unroll
@@ -95,13 +96,17 @@ k_lin_few(const uint8_t *__restrict__ w, size_t sc_off, const void *__restrict__
       }
     }
   };
+  auto compute = [&](int group, int st) __attribute__((always_inline)) {
+#pragma unroll
+    for (int p = 0; p < G; ++p) add(G * group + p, st, p);
+  };
   LinOut<KS, R, MR> out;
   out.ahead(e, M, N, (int)blockIdx.x);
   // (x's loads go out before the weights': behind them they would wait for theirs)
   few_stage<64 * KS>(x, M, K, np, stride, kNibOrder<FMT>, xs_s, tid,
-                     [&]() __attribute__((always_inline)) { walk_requests<PD, KS>(units, wave, request); });
+                     [&]() __attribute__((always_inline)) { walk_requests<PD, KS>(units / G, wave, request); });
   step_barrier<63>();  // (of LDS alone)
-  walk_computes<PD, KS>(units, wave, request, compute);
+  walk_computes<PD, KS>(units / G, wave, request, compute);
 #pragma unroll
   for (int t = 0; t < R; ++t)
 #pragma unroll
@@ -139,18 +144,19 @@ k_lin_rows(const uint8_t *__restrict__ w, size_t sc_off, const _Float16 *__restr
     const int row = 16 * t + r;
     xo[t] = 2u * ((uint32_t)(row < M ? row : M - 1) * (uint32_t)lda + 16u * (uint32_t)g);  // (rows past M: not stored)
   }
-  FUnit<FMT> us[PD][R];
-  gq_half8 xs[PD][MT][4];
-  auto request = [&](int unit, int st) __attribute__((always_inline)) {
+  constexpr int G = kGroup<FMT>;
+  FUnit<FMT> us[PD][R][G];
+  gq_half8 xs[PD][G][MT][4];
+  auto request = [&](int group, int st) __attribute__((always_inline)) {
 #pragma unroll
-    for (int t = 0; t < R; ++t) load_unit<FMT>(tl[t], unit, lane, us[st][t]);
+    for (int t = 0; t < R; ++t) load_group<FMT>(tl[t], group, lane, us[st][t]);
 #pragma unroll
     for (int t = 0; t < MT; ++t) {
-      const uint32_t o = unit < units ? xo[t] + 256u * (uint32_t)unit : 0xFFFFFF00u;
+      const uint32_t o = G * group < units ? xo[t] + 256u * G * (uint32_t)group : 0xFFFFFC00u;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
+      for (int i = 0; i < 4 * G; ++i) {
         const auto v = __builtin_amdgcn_raw_buffer_load_b128(xr, o + 128u * (i >> 1) + 16u * (i & 1), 0, 0);
-        xs[st][t][i] = __builtin_bit_cast(gq_half8, gq_u4{v[0], v[1], v[2], v[3]});
+        xs[st][i >> 2][t][i & 3] = __builtin_bit_cast(gq_half8, gq_u4{v[0], v[1], v[2], v[3]});
       }
     }
   };
@@ -160,13 +166,15 @@ k_lin_rows(const uint8_t *__restrict__ w, size_t sc_off, const _Float16 *__restr
 #pragma unroll
     for (int i = 0; i < MT; ++i) acc[t][i] = gq_f4{0.f, 0.f, 0.f, 0.f};
   const uint32_t mg = gq_nib_magic();
-  auto compute = [&](int unit, int st) __attribute__((always_inline)) {
+  auto compute = [&](int group, int st) __attribute__((always_inline)) {
 #pragma unroll
-    for (int t = 0; t < R; ++t) rows_add<FMT, MT>(us[st][t], unit, g, mg, xs[st], acc[t]);
+    for (int p = 0; p < G; ++p)
+#pragma unroll
+      for (int t = 0; t < R; ++t) rows_add<FMT, MT>(us[st][t][p], G * group + p, g, mg, xs[st][p], acc[t]);
   };
   LinOut<KS, R, 16 * MT> out;
   out.ahead(e, M, N, (int)blockIdx.x);
-  walk_units<PD, KS>(units, wave, request, compute);
+  walk_units<PD, KS>(units / G, wave, request, compute);
 #pragma unroll
   for (int t = 0; t < R; ++t)
 #pragma unroll
@@ -192,7 +200,7 @@ int launch_few_t(const void *w, const void *x, const float *rs, const LinEpi &e,
   const int units = (int)(gq_kpad(FMT, K) / 128);
   const size_t tiles = gq_tiles(N), lds = few_lds_bytes(M, 128 * (size_t)units);
 #define GQ_FEW(MR, R, KS, PD)                                                                                               \
-  hipLaunchKernelGGL((k_lin_few<FMT, XT, MR, R, KS, PD>), dim3((unsigned)((tiles + (R)-1) / (R))), dim3(64 * (KS)), lds, s,   \
+  hipLaunchKernelGGL((k_lin_few<FMT, XT, MR, R, KS, group_stages<FMT>(PD)>), dim3((unsigned)((tiles + (R)-1) / (R))), dim3(64 * (KS)), lds, s,   \
                      (const uint8_t *)w, gq_sc_plane_offset(FMT, N, K), x, rs, e, M, N, K, (int)gq_chunks(FMT, K), units)
 #define GQ_FEW_M(R, KS, PD)           \
   do {                                \
@@ -211,7 +219,7 @@ int launch_rows_t(const void *w, const _Float16 *a16, int lda, const float *rs, 
   const int units = (int)(gq_kpad(FMT, K) / 128);
   const size_t tiles = gq_tiles(N);
 #define GQ_ROWS(R, KS, PD)                                                                                               \
-  hipLaunchKernelGGL((k_lin_rows<FMT, 1, R, KS, PD>), dim3((unsigned)((tiles + (R)-1) / (R))), dim3(64 * (KS)), 0, s,      \
+  hipLaunchKernelGGL((k_lin_rows<FMT, 1, R, KS, group_stages<FMT>(PD)>), dim3((unsigned)((tiles + (R)-1) / (R))), dim3(64 * (KS)), 0, s,      \
                      (const uint8_t *)w, gq_sc_plane_offset(FMT, N, K), a16, lda, rs, e, M, N, (int)gq_chunks(FMT, K), units)
   // Two tiles share the rows of x where there are workgroups enough; long rows by few waves (16 rows, us by two tiles and 4 waves / one
   // and 8 / one and 4, deeper: 14336 x 4096 Q4_K 15.6 / 22 / 19.6; 4096 x 14336 24.4 / 21.8 / 19.5; 4096 x 4096 Q4_0 9.6 / 8.1 / 8.4)

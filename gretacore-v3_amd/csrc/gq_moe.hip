@@ -373,10 +373,11 @@ k_moe_gu_few(const uint8_t *__restrict__ wg, const uint8_t *__restrict__ wu, siz
   }
   const bool mine = few_mine<FMT>(lane) && (lane & 3) < M;
   const uint32_t x0 = mine ? (uint32_t)((lane & 3) * stride + 32 * g) : (uint32_t)(M * stride), xd = mine ? 256u : 0u;
-  FUnit<FMT> us[PD][T];
-  auto request = [&](int unit, int st) __attribute__((always_inline)) {
+  constexpr int G = kGroup<FMT>;
+  FUnit<FMT> us[PD][T][G];
+  auto request = [&](int group, int st) __attribute__((always_inline)) {
 #pragma unroll
-    for (int t = 0; t < T; ++t) load_unit<FMT>(tl[t], unit, lane, us[st][t]);
+    for (int t = 0; t < T; ++t) load_group<FMT>(tl[t], group, lane, us[st][t]);
   };
   float acc[T][MR] = {};
   uint32_t mg;  // (kept in a register)
@@ -385,11 +386,11 @@ k_moe_gu_few(const uint8_t *__restrict__ wg, const uint8_t *__restrict__ wu, siz
   constexpr uint32_t one = XT == GQ_DT_F16 ? 0x3C003C00u : 0x3F803F80u;
   const gq_u4 ones = {one, one, one, one};
   const gq_f4 zero = {0.f, 0.f, 0.f, 0.f};
-  auto compute = [&](int unit, int st) __attribute__((always_inline)) {
+  auto add = [&](int unit, int st, int p) __attribute__((always_inline)) {
     const uint32_t at = x0 + xd * (uint32_t)unit;
     float s[T][2], mn[T][2];
 #pragma unroll
-    for (int t = 0; t < T; ++t) few_scales<FMT>(us[st][t], unit, g & (NG - 1), s[t], mn[t]);
+    for (int t = 0; t < T; ++t) few_scales<FMT>(us[st][t][p], unit, g & (NG - 1), s[t], mn[t]);
 #pragma unroll
     for (int m = 0; m < 2; ++m) {
       const gq_u4 a0 = few_lds(xs_s, at, m, 0), a1 = few_lds(xs_s, at, m, 1);
@@ -398,7 +399,7 @@ k_moe_gu_few(const uint8_t *__restrict__ wg, const uint8_t *__restrict__ wu, siz
 #pragma unroll
       for (int t = 0; t < T; ++t) {
         gq_u4 b[2];
-        few_codes<FMT, XT>(us[st][t], m, mg, b);
+        few_codes<FMT, XT>(us[st][t][p], m, mg, b);
         const gq_f4 d = few_mfma<XT>(a1, b[1], few_mfma<XT>(a0, b[0], zero));
         const float o = FMT == GQ_FMT_Q4_K ? fmaf(s[t][m], OFF, mn[t][m]) : 0.f;
 #pragma unroll
@@ -409,7 +410,11 @@ k_moe_gu_few(const uint8_t *__restrict__ wg, const uint8_t *__restrict__ wu, siz
       }
     }
   };
-  walk_units<PD, KS>(units, wave, request, compute);
+  auto compute = [&](int group, int st) __attribute__((always_inline)) {
+#pragma unroll
+    for (int p = 0; p < G; ++p) add(G * group + p, st, p);
+  };
+  walk_units<PD, KS>(units / G, wave, request, compute);
 #pragma unroll
   for (int t = 0; t < T; ++t)
 #pragma unroll
@@ -466,27 +471,30 @@ k_moe_gu_rows(const uint8_t *__restrict__ wg, const uint8_t *__restrict__ wu, si
       const_cast<_Float16 *>(a16), (short)0, (int)(2u * (uint32_t)M * (uint32_t)lda), 0x00020000);
   const bool row = r < blk.count;
   const uint32_t xo = row ? 2u * ((uint32_t)(blk.pair[r] / top) * (uint32_t)lda + 16u * (uint32_t)g) : 0u;
-  FUnit<FMT> us[PD][T];
-  gq_half8 xs[PD][1][4];
-  auto request = [&](int unit, int st) __attribute__((always_inline)) {
+  constexpr int G = kGroup<FMT>;
+  FUnit<FMT> us[PD][T][G];
+  gq_half8 xs[PD][G][1][4];
+  auto request = [&](int group, int st) __attribute__((always_inline)) {
 #pragma unroll
-    for (int t = 0; t < T; ++t) load_unit<FMT>(tl[t], unit, lane, us[st][t]);
-    const uint32_t o = row && unit < units ? xo + 256u * (uint32_t)unit : 0xFFFFFF00u;
+    for (int t = 0; t < T; ++t) load_group<FMT>(tl[t], group, lane, us[st][t]);
+    const uint32_t o = row && G * group < units ? xo + 256u * G * (uint32_t)group : 0xFFFFFC00u;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < 4 * G; ++i) {
       const auto v = __builtin_amdgcn_raw_buffer_load_b128(xr, o + 128u * (i >> 1) + 16u * (i & 1), 0, 0);
-      xs[st][0][i] = __builtin_bit_cast(gq_half8, gq_u4{v[0], v[1], v[2], v[3]});
+      xs[st][i >> 2][0][i & 3] = __builtin_bit_cast(gq_half8, gq_u4{v[0], v[1], v[2], v[3]});
     }
   };
   gq_f4 acc[T][1];
 #pragma unroll
   for (int t = 0; t < T; ++t) acc[t][0] = gq_f4{0.f, 0.f, 0.f, 0.f};
   const uint32_t mg = gq_nib_magic();
-  auto compute = [&](int unit, int st) __attribute__((always_inline)) {
+  auto compute = [&](int group, int st) __attribute__((always_inline)) {
 #pragma unroll
-    for (int t = 0; t < T; ++t) rows_add<FMT, 1>(us[st][t], unit, g, mg, xs[st], acc[t]);
+    for (int p = 0; p < G; ++p)
+#pragma unroll
+      for (int t = 0; t < T; ++t) rows_add<FMT, 1>(us[st][t][p], G * group + p, g, mg, xs[st][p], acc[t]);
   };
-  walk_units<PD, KS>(units, wave, request, compute);
+  walk_units<PD, KS>(units / G, wave, request, compute);
 #pragma unroll
   for (int t = 0; t < T; ++t) red[wave][t][lane] = acc[t][0];
   __syncthreads();
@@ -593,36 +601,37 @@ k_moe_down_few(const uint8_t *__restrict__ wd, size_t sc_off, const _Float16 *__
   const uint32_t zero_at = (uint32_t)(P * stride);
   const float2 *f_s = reinterpret_cast<const float2 *>(xs_s + P * stride + 160);
   const int gi = NG == 2 ? g & 1 : g >> 1;  // the 32-block of a step that this lane's sums are of
-  FUnit<FMT> us[PD];
+  constexpr int G = kGroup<FMT>;
+  FUnit<FMT> us[PD][G];
   auto request = [&](const ItemAt &at, int st) __attribute__((always_inline)) {
     const bool on = at.b < nblk;
     const size_t tile = (size_t)__builtin_amdgcn_readlane(expert, on ? at.b : 0) * (size_t)ntiles + blockIdx.x;
-    load_unit<FMT>(ftile<FMT>(wd, sc_off, tile, on ? C : 0), at.u, lane, us[st]);
+    load_group<FMT>(ftile<FMT>(wd, sc_off, tile, on ? C : 0), at.u, lane, us[st]);
   };
   float acc[MR] = {};
   uint32_t mg;  // (kept in a register)
   asm volatile("v_mov_b32 %0, 0x64006400" : "=v"(mg));
   const gq_u4 ones = {0x3C003C00u, 0x3C003C00u, 0x3C003C00u, 0x3C003C00u};
   const gq_f4 zero = {0.f, 0.f, 0.f, 0.f};
-  auto compute = [&](const ItemAt &at, int st) __attribute__((always_inline)) {
-    const int b = at.b, q = p_s[b][MR == 1 ? 0 : lane & 3];
-    const uint32_t xo = mine && q >= 0 ? (uint32_t)(q * stride + 256 * at.u + 32 * g) : zero_at;
+  auto add = [&](int b, int unit, int st, int p) __attribute__((always_inline)) {
+    const int q = p_s[b][MR == 1 ? 0 : lane & 3];
+    const uint32_t xo = mine && q >= 0 ? (uint32_t)(q * stride + 256 * unit + 32 * g) : zero_at;
     float s[2], mn[2];
     float2 f[MR];
 #pragma unroll
     for (int r = 0; r < MR; ++r) {
       const int qr = p_s[b][r];
       const float w = w_s[b][r];
-      f[r] = f_s[2 * (max(qr, 0) * units + at.u) + gi];
+      f[r] = f_s[2 * (max(qr, 0) * units + unit) + gi];
       f[r] = qr < 0 ? make_float2(0.f, 0.f) : make_float2(f[r].x * w, f[r].y * w);  // (a token without the expert)
     }
-    few_scales<FMT>(us[st], at.u, g & (NG - 1), s, mn);
+    few_scales<FMT>(us[st][p], unit, g & (NG - 1), s, mn);
 #pragma unroll
     for (int m = 0; m < 2; ++m) {
       const gq_u4 a0 = few_lds(xs_s, xo, m, 0), a1 = few_lds(xs_s, xo, m, 1);
       const gq_f4 sx = few_mfma<XT>(a1, ones, few_mfma<XT>(a0, ones, zero));
       gq_u4 b[2];
-      few_codes<FMT, XT>(us[st], m, mg, b);
+      few_codes<FMT, XT>(us[st][p], m, mg, b);
       const gq_f4 d = few_mfma<XT>(a1, b[1], few_mfma<XT>(a0, b[0], zero));
       const float o = FMT == GQ_FMT_Q4_K ? fmaf(s[m], OFF, mn[m]) : s[m] * OFF;
 #pragma unroll
@@ -630,16 +639,21 @@ k_moe_down_few(const uint8_t *__restrict__ wd, size_t sc_off, const _Float16 *__
         acc[r] = fmaf(m ? f[r].y : f[r].x, fmaf(s[m], d[r], -o * sx[r]), acc[r]);
     }
   };
+  auto compute = [&](const ItemAt &at, int st) __attribute__((always_inline)) {
+#pragma unroll
+    for (int p = 0; p < G; ++p) add(at.b, G * at.u + p, st, p);
+  };
+  const int groups = units / G;
   ItemAt rq = {0, 0};
-  rq.next(wave, units);
+  rq.next(wave, groups);
   ItemAt first = rq;
   for (int i = tid; i < P * units; i += 64 * KS)  // (of pairs that name no expert too: not used)
     *reinterpret_cast<gq_f4 *>(xs_s + P * stride + 160 + 16 * i) = *reinterpret_cast<const gq_f4 *>(hs + 4 * (size_t)i);
   few_stage<64 * KS>(h, P, N, np, stride, false, xs_s, tid, [&]() __attribute__((always_inline)) {
-    if (nblk > 0) items_requests<PD, KS>(rq, units, request);
+    if (nblk > 0) items_requests<PD, KS>(rq, groups, request);
   });
   step_barrier<63>();  // (of LDS alone)
-  items_computes<PD, KS>(first, rq, nblk, units, request, compute);
+  items_computes<PD, KS>(first, rq, nblk, groups, request, compute);
 #pragma unroll
   for (int r = 0; r < MR; ++r) red[wave][r][lane] = acc[r];
   __syncthreads();
@@ -687,8 +701,9 @@ k_moe_down_rows(const uint8_t *__restrict__ wd, size_t sc_off, const _Float16 *_
   __syncthreads();
   const __amdgpu_buffer_rsrc_t xr = __builtin_amdgcn_make_buffer_rsrc(
       const_cast<_Float16 *>(h16), (short)0, (int)(2u * (uint32_t)P * (uint32_t)ldh), 0x00020000);
-  FUnit<FMT> us[PD][R];
-  gq_half8 xs[PD][1][4];
+  constexpr int G = kGroup<FMT>;
+  FUnit<FMT> us[PD][R][G];
+  gq_half8 xs[PD][G][1][4];
   auto request = [&](const ItemAt &at, int st) __attribute__((always_inline)) {
     const bool on = at.b < nblk;
     const int b = on ? at.b : b0;
@@ -696,14 +711,14 @@ k_moe_down_rows(const uint8_t *__restrict__ wd, size_t sc_off, const _Float16 *_
 #pragma unroll
     for (int t = 0; t < R; ++t) {
       const int tile = (int)blockIdx.x * R + t;  // (clamped: not stored)
-      load_unit<FMT>(ftile<FMT>(wd, sc_off, tile0 + (size_t)min(tile, ntiles - 1), on ? C : 0), at.u, lane, us[st][t]);
+      load_group<FMT>(ftile<FMT>(wd, sc_off, tile0 + (size_t)min(tile, ntiles - 1), on ? C : 0), at.u, lane, us[st][t]);
     }
     const uint32_t q = p_s[16 * b + r];
-    const uint32_t o = on && q != 0xFFFFu ? 2u * (q * (uint32_t)ldh + 16u * (uint32_t)g) + 256u * (uint32_t)at.u : 0xFFFFFF00u;
+    const uint32_t o = on && q != 0xFFFFu ? 2u * (q * (uint32_t)ldh + 16u * (uint32_t)g) + 256u * G * (uint32_t)at.u : 0xFFFFFC00u;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < 4 * G; ++i) {
       const auto v = __builtin_amdgcn_raw_buffer_load_b128(xr, o + 128u * (i >> 1) + 16u * (i & 1), 0, 0);
-      xs[st][0][i] = __builtin_bit_cast(gq_half8, gq_u4{v[0], v[1], v[2], v[3]});
+      xs[st][i >> 2][0][i & 3] = __builtin_bit_cast(gq_half8, gq_u4{v[0], v[1], v[2], v[3]});
     }
   };
   gq_f4 acc[R][1];
@@ -730,13 +745,16 @@ k_moe_down_rows(const uint8_t *__restrict__ wd, size_t sc_off, const _Float16 *_
       cur = at.b;
     }
 #pragma unroll
-    for (int t = 0; t < R; ++t) rows_add<FMT, 1>(us[st][t], at.u, g, mg, xs[st], acc[t]);
+    for (int p = 0; p < G; ++p)
+#pragma unroll
+      for (int t = 0; t < R; ++t) rows_add<FMT, 1>(us[st][t][p], G * at.u + p, g, mg, xs[st][p], acc[t]);
   };
+  const int groups = units / G;
   ItemAt rq = {b0, 0};
-  rq.next(wave, units);
+  rq.next(wave, groups);
   const ItemAt first = rq;
-  items_requests<PD, KS>(rq, units, request);
-  items_computes<PD, KS>(first, rq, nblk, units, request, compute);
+  items_requests<PD, KS>(rq, groups, request);
+  items_computes<PD, KS>(first, rq, nblk, groups, request, compute);
   flush();
   __syncthreads();
   for (int i = tid; i < 16 * R * M; i += 64 * KS) {
@@ -891,7 +909,7 @@ int launch_gu_few_t(const gq_moe &l, const void *x, const float *rs, const Route
                     hipStream_t s) {
   const int N = (int)l.N, K = (int)l.K, units = (int)(gq_kpad(FMT, K) / 128), nib = l.fmt_down == GQ_FMT_Q4_0 || gq_fmt_is_q4k(l.fmt_down);
 #define GQ_GU_R(MR, KS, PD, ROUTE)                                                                                         \
-  hipLaunchKernelGGL((k_moe_gu_few<FMT, XT, MR, KS, PD, ROUTE>), dim3((unsigned)(N / 32), (unsigned)(M * l.top_k)), dim3(64 * (KS)), \
+  hipLaunchKernelGGL((k_moe_gu_few<FMT, XT, MR, KS, group_stages<FMT>(PD), ROUTE>), dim3((unsigned)(N / 32), (unsigned)(M * l.top_k)), dim3(64 * (KS)), \
                      few_lds_bytes(M, 128 * (size_t)units), s, (const uint8_t *)l.gate, (const uint8_t *)l.up,            \
                      gq_sc_plane_offset(FMT, l.n_experts * l.N, K), x, rs, a ? *a : RouteArgs{}, ids, b.h16, b.hs, nib, M, N, K,    \
                      (int)gq_chunks(FMT, K), units, l.act, (int)l.n_experts, l.top_k)
@@ -922,7 +940,7 @@ int launch_gu_t(const gq_moe &l, const void *x, int xt, const float *rs, const R
   const int N = (int)l.N, K = (int)l.K, units = (int)(gq_kpad(FMT, K) / 128), tiles = N / 16;
   // (16 tokens, 8 experts of 14336 x 4096, Q4_0, by one tile 190 us the layer, by two 167; 64 tokens, 128 experts of 768 x 2048, 143 and 128)
   constexpr int R = 2, KS = 4;
-  hipLaunchKernelGGL((k_moe_gu_rows<FMT, R, KS, 2>), dim3((unsigned)((tiles + R - 1) / R), (unsigned)p.maxblk), dim3(64 * KS), 0, s,
+  hipLaunchKernelGGL((k_moe_gu_rows<FMT, R, KS, group_stages<FMT>(2)>), dim3((unsigned)((tiles + R - 1) / R), (unsigned)p.maxblk), dim3(64 * KS), 0, s,
                      (const uint8_t *)l.gate, (const uint8_t *)l.up, gq_sc_plane_offset(FMT, l.n_experts * l.N, K), b.a16, b.lda, rs, p,
                      b.h, M, N, (int)gq_chunks(FMT, K), units, l.act, l.top_k);
   return gq_last_launch();
@@ -936,7 +954,7 @@ int launch_down_t(const gq_moe &l, const int *ids, const float *weights, const M
   if (moe_few(l, M)) {
     const size_t rows = (size_t)M * l.top_k, lds = few_lds_bytes(rows, 128 * (size_t)units) + rows * units * 16;
 #define GQ_DOWN(MR, KS, PD)                                                                                              \
-  hipLaunchKernelGGL((k_moe_down_few<FMT, MR, KS, PD>), dim3(tiles), dim3(64 * (KS)), lds, s, (const uint8_t *)l.down, so, b.h16, b.hs, ids, \
+  hipLaunchKernelGGL((k_moe_down_few<FMT, MR, KS, group_stages<FMT>(PD)>), dim3(tiles), dim3(64 * (KS)), lds, s, (const uint8_t *)l.down, so, b.h16, b.hs, ids, \
                      weights, resid, y, dt, M, N, K, C, units, (int)l.n_experts, l.top_k)
     if (M == 1) GQ_DOWN(1, 16, 2);
     else GQ_DOWN(4, 16, 2);
@@ -947,7 +965,7 @@ int launch_down_t(const gq_moe &l, const int *ids, const float *weights, const M
   // the layer, by two in two parts 152, by four in four parts 147 - 149; 64 tokens, 128 experts of 768 x 2048, 127, 117 and 139 - 159.)
   constexpr int R = 2, KS = 8;
   const size_t P = (size_t)M * l.top_k, lds = (size_t)KS * M * 64 * R + P * 4 + (size_t)p.maxblk * 34 + P + 16;
-  hipLaunchKernelGGL((k_moe_down_rows<FMT, R, KS, 2>), dim3((tiles + R - 1) / R, (unsigned)b.parts), dim3(64 * KS), lds, s,
+  hipLaunchKernelGGL((k_moe_down_rows<FMT, R, KS, group_stages<FMT>(2)>), dim3((tiles + R - 1) / R, (unsigned)b.parts), dim3(64 * KS), lds, s,
                      (const uint8_t *)l.down, so, b.h16, b.ldh, b.hs, p, resid, y, dt, b.parts > 1 ? b.part : nullptr, M, K, C, units,
                      l.top_k, p.maxblk);
   return gq_last_launch();

@@ -55,6 +55,36 @@ GQ_DEV void load_unit(const FTile<FMT> &t, int unit, int lane, FUnit<FMT> &u) {
     u.s[1] = v[1];
   }
 }
+// What a wave loads at a time: a unit, of the k-quants both units of a super-block, whose scales come with one load each (Q4_K three loads for
+// two units in place of four, Q6_K five of eight; a CU's loads count as much as their bytes).
+template <int FMT>
+constexpr int kGroup = kSuper<FMT> ? 2 : 1;
+// stages of a pipeline `units` deep
+template <int FMT>
+constexpr int group_stages(int units) {
+  return units / kGroup<FMT> > 0 ? units / kGroup<FMT> : 1;
+}
+template <int FMT>
+GQ_DEV void load_group(const FTile<FMT> &t, int group, int lane, FUnit<FMT> (&u)[kGroup<FMT>]) {
+  using F = HFmt<FMT>;
+  if constexpr (!kSuper<FMT>) {
+    load_unit<FMT>(t, group, lane, u[0]);
+  } else {
+    const uint32_t c = (uint32_t)group, qo = c * F::QB + 16u * (uint32_t)lane, so = c * F::SB, r = (uint32_t)lane & 15u;
+    u[0].q[0] = ld16_r(t.q, qo);
+    u[1].q[0] = ld16_r(t.q, qo + 1024u);
+    if constexpr (FMT == GQ_FMT_Q4_K) {
+      const auto v = __builtin_amdgcn_raw_buffer_load_b128(t.s, so + 16u * r, 0, 0);
+      u[0].s = u[1].s = gq_u4{v[0], v[1], v[2], v[3]};
+    } else {
+      const gq_u4 h = ld16_r(t.q, qo + 2048u);
+      const auto v = __builtin_amdgcn_raw_buffer_load_b128(t.s, so + 16u * r, 0, 0);
+      u[0].s = gq_u4{h[0], h[1], v[0], v[1]};
+      u[1].s = gq_u4{h[2], h[3], v[2], v[3]};
+      u[0].d = u[1].d = __builtin_amdgcn_raw_buffer_load_b16(t.s, so + 256u + 2u * r, 0, 0);
+    }
+  }
+}
 // Q4_K: scale and min codes of sub-blocks i of the unit's two steps, a byte each (p: the unit's half)
 GQ_DEV void unit_codes_q4k(const FUnit<GQ_FMT_Q4_K> &u, uint32_t p, bool i, uint32_t &sc, uint32_t &mn) {
   const uint32_t w = (i ? u.s[2] : u.s[1]) >> (16u * p), m = u.s[3] >> (16u * p + (i ? 4u : 0u));
