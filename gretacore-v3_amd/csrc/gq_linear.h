@@ -53,7 +53,7 @@ GQ_DEV void lin_put(const LinEpi &e, size_t m, int n, int N, float v, const LinT
 
 }  // namespace
 
-// The tiled kernels (gq_linear_rb.hip): a16 fp16 [M][gq_kpad(K)] in the B fragments' order, rs its row scales (padded by 256), part: room for
+// The tiled kernels (gq_linear_rb.hip): a16 fp16 [M][gq_kpad(K)] in the B fragments' order, rs its row scales (padded by 256; NULL: 1), part: room for
 // parts of K, kLinPartBytes
 int gq_launch_linear_rb(int fmt, const void *w, const _Float16 *a16, const float *rs, const void *epi, float *part, int M, int N, int K,
                         hipStream_t s);

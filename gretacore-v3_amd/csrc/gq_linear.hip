@@ -470,15 +470,19 @@ extern "C" int gq_linear(int fmt, const void *w, const void *x, int x_dtype, con
   _Float16 *a16 = (_Float16 *)ws;
   float *rs = (float *)((uint8_t *)ws + gq_align256(mb * (Kp + 8) * 2));
   const int q4 = fmt == GQ_FMT_Q4_0 || gq_fmt_is_q4k(fmt);
+  // fp16 rows of whole chunks are what the matrix cores take already, but for the 4-bit formats' order
+  const bool plain = x_dtype == GQ_DT_F16 && !q4 && K == Kp && ((uintptr_t)x & 15) == 0;
   if (is_few) {
     GQ_TRY(gq_launch_a_to_f16(x, x_dtype, a16, rs, (int)M, (int)K, (int)K, 0, s));
     return few(a16, GQ_DT_F16, rs);
   }
   float *part = (float *)((uint8_t *)rs + gq_align256((mb + 256) * 4));
   if (M <= kRows) {  // rows 16 bytes longer than a multiple of 4 KiB, where 16 of them would collide
-    const int ld = (int)Kp + 8;
-    GQ_TRY(gq_launch_a_to_f16(x, x_dtype, a16, rs, (int)M, (int)K, ld, q4, s));
-#define GQ_ROWS_F(F) launch_rows_t<F>(w, a16, ld, rs, e, (int)M, (int)N, (int)K, s)
+    const int ld = (int)(plain ? K : Kp + 8);
+    if (!plain) GQ_TRY(gq_launch_a_to_f16(x, x_dtype, a16, rs, (int)M, (int)K, ld, q4, s));
+    const _Float16 *a = plain ? (const _Float16 *)x : a16;
+    const float *f = plain ? nullptr : rs;
+#define GQ_ROWS_F(F) launch_rows_t<F>(w, a, ld, f, e, (int)M, (int)N, (int)K, s)
     if (fmt == GQ_FMT_Q4_0) return GQ_ROWS_F(GQ_FMT_Q4_0);
     if (fmt == GQ_FMT_Q8_0) return GQ_ROWS_F(GQ_FMT_Q8_0);
     if (gq_fmt_is_q6k(fmt)) return GQ_ROWS_F(GQ_FMT_Q6_K);
@@ -488,12 +492,13 @@ extern "C" int gq_linear(int fmt, const void *w, const void *x, int x_dtype, con
   const size_t xs = gq_dtype_size(x_dtype) * K, ys = gq_dtype_size(y_dtype) * N;
   for (size_t m0 = 0; m0 < M; m0 += mb) {
     const int m = (int)(M - m0 < mb ? M - m0 : mb);
-    GQ_TRY(gq_launch_a_to_f16((const uint8_t *)x + m0 * xs, x_dtype, a16, rs, m, (int)K, (int)Kp, q4, s));
+    const _Float16 *a = plain ? (const _Float16 *)x + m0 * K : a16;
+    if (!plain) GQ_TRY(gq_launch_a_to_f16((const uint8_t *)x + m0 * xs, x_dtype, a16, rs, m, (int)K, (int)Kp, q4, s));
     LinEpi b = e;
     b.resid = resid ? (const uint8_t *)resid + m0 * ys : nullptr;
     b.y = (uint8_t *)y + m0 * ys;
     b.z = z ? (uint8_t *)z + m0 * ys : nullptr;
-    GQ_TRY(gq_launch_linear_rb(fmt, w, a16, rs, &b, part, m, (int)N, (int)K, s));
+    GQ_TRY(gq_launch_linear_rb(fmt, w, a, plain ? nullptr : rs, &b, part, m, (int)N, (int)K, s));
   }
   return GQ_OK;
 }

@@ -104,7 +104,8 @@ k_lin_rb(const uint8_t *__restrict__ w, uint32_t sc_off, const _Float16 *__restr
     load_rstep<FMT, NJ>(w, qo, so, s, st[i]);
     __builtin_amdgcn_sched_barrier(0);
   };
-  const gq_f4 rs4 = *reinterpret_cast<const gq_f4 *>(rs + m0 + 4 * (tid % (BM / 4)));  // (padded past M)
+  // (padded past M)
+  const gq_f4 rs4 = rs ? *reinterpret_cast<const gq_f4 *>(rs + m0 + 4 * (tid % (BM / 4))) : gq_f4{1.f, 1.f, 1.f, 1.f};
   prime(B0{});
   prime(B1{});
   if constexpr (PD >= 3) prime(B2{});

@@ -68,6 +68,22 @@ GQ_DEV void moe_convert(const void *x, const MoeConv &c, int m, int K, int lane)
     *reinterpret_cast<gq_half8 *>(c.a16 + (size_t)m * c.lda + k) = h;
   }
 }
+// The sum of a wave's values, in all lanes: rows of 16 by rotations, then the rows
+template <int CTRL>
+GQ_DEV double dpp_d(double v) {
+  const uint64_t b = __builtin_bit_cast(uint64_t, v);
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)b, CTRL, 0xF, 0xF, false);
+  const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(b >> 32), CTRL, 0xF, 0xF, false);
+  return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+GQ_DEV double wave_sum(double v) {
+  v += dpp_d<0x128>(v);  // row_ror 8, 4, 2, 1
+  v += dpp_d<0x124>(v);
+  v += dpp_d<0x122>(v);
+  v += dpp_d<0x121>(v);
+  v += __shfl_xor(v, 16, 64);
+  return v + __shfl_xor(v, 32, 64);
+}
 // Workgroup (e, b): logits of expert e for tokens TOK b .. TOK b + TOK - 1.  Products of two fp32 values are exact in 64 bits.
 // Workgroup (E, b): the conversion of those tokens' rows, a wave a row.
 constexpr int kLogThreads = 256;
@@ -100,9 +116,7 @@ __global__ void __launch_bounds__(kLogThreads) k_moe_logits(const void *__restri
     }
   }
 #pragma unroll
-  for (int o = 32; o > 0; o >>= 1)
-#pragma unroll
-    for (int t = 0; t < TOK; ++t) acc[t] += __shfl_xor(acc[t], o, 64);
+  for (int t = 0; t < TOK; ++t) acc[t] = wave_sum(acc[t]);
   if ((tid & 63) == 0)
 #pragma unroll
     for (int t = 0; t < TOK; ++t) red[tid >> 6][t] = acc[t];
@@ -162,8 +176,7 @@ GQ_DEV void moe_choose(const RouteArgs &a, int m, int E, int top, int lane, int 
     if (!a.renorm || a.bias) {  // (renormalised weights do without the sum over all experts)
 #pragma unroll
       for (int i = 0; i < NE; ++i) sum += l[i] == ninf ? 0.0 : exp(l[i] - lmax);
-#pragma unroll
-      for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
+      sum = wave_sum(sum);
     } else {
       sum = 1.0;
     }
