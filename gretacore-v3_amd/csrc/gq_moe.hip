@@ -823,11 +823,10 @@ int check_moe(const gq_moe *l, size_t M, bool route, bool ffn) {
   return GQ_OK;
 }
 
-// Up to 4 tokens whose rows of x, and of h with their scales, fit LDS (beside 20 KiB of the kernels' own)
+// Up to 4 tokens whose rows of x, and of h with their scales, fit LDS beside the waves' sums (32 KiB of k_moe_gu_few, 18 of k_moe_down_few)
 bool moe_few(const gq_moe &l, size_t M) {
-  constexpr size_t kLds = (160 - 20) * 1024;
   const size_t P = M * (size_t)l.top_k, nk = (gq_kpad(l.fmt, l.K) + 127) & ~(size_t)127, nn = (gq_kpad(l.fmt_down, l.N) + 127) & ~(size_t)127;
-  return M <= (size_t)kMoeFew && few_lds_bytes(M, nk) <= kLds && few_lds_bytes(P, nn) + P * nn / 8 <= kLds;
+  return M <= (size_t)kMoeFew && few_lds_bytes(M, nk) <= (160 - 34) * 1024 && few_lds_bytes(P, nn) + P * nn / 8 <= (160 - 20) * 1024;
 }
 // Where a call's intermediate values lie in its workspace
 struct MoeWs {
