@@ -252,31 +252,49 @@ int launch_rb(const void *w, const _Float16 *a16, const float *rs, const LinEpi 
 }
 template <int FMT>
 int launch_fmt(const void *w, const _Float16 *a16, const float *rs, const LinEpi &e, float *part, int M, int N, int K, hipStream_t s) {
-  auto wgs = [&](int bm, int bn) { return (size_t)((M + bm - 1) / bm) * (size_t)((N + bn - 1) / bn); };
   const int nsteps = (int)(gq_kpad(FMT, K) / BK);  // (even)
-  // parts of K as far as a workgroup a CU and at least four rounds of the groups a part go
-  auto parts = [&](size_t tiles, int kg) {
-    return (int)std::max((size_t)1, std::min({256 / std::max(tiles, (size_t)1), (size_t)(nsteps / (4 * kg)), (size_t)kLinParts}));
+  // The tile and the parts of K whose rounds of the 256 CUs take the least: a round its steps (and what fills its K groups' pipelines) times what
+  // a step takes on a full chip; parts a launch more, and their sums' way to memory and back.  us with the conversion of x, Q4_K / Q8_0, against a
+  // ladder of tiles that are near one workgroup a CU each:
+  //   2048 x 4096 x 14336   239 / -    (250)         128 x 256        900 x 4096 x 14336   120 / 133 (125 / 143; Q4_0, Q6_K)   128 x 128
+  //   2048 x 6144 x 4096    113 / 113  (125 / 122)   256 x 256        300 x 14336 x 4096   53 / 63 (67 / 95; Q4_0, Q6_K)       128 x 256
+  //   509 x 8191 x 4096     - / 46     (48)          128 x 128        200 x 20000 x 1024   24 / 23 (32 / 34)                   128 x 256
+  //   512 x 4096 x 14336    78 / 78    (79 / 77)     in 2, 4 parts    128 x 4096 x 4096    17.7 / 17.1 (19.5 / 20.5)           32 x 64
+  //   128 x 14336 x 4096    26 / 34 (Q4_0, Q6_K: the same) 64 x 128   64 x 4096 x 14336    26 / 29 (24 / 31; Q4_0, Q6_K)       64 x 128, 8 parts
+  // Loads a lane shares between two column blocks of a wave (64 x 256 by 4 waves): 51 against 47 of 509 x 8191 x 4096.
+  float best = 1e30f;
+  int parts = 1;
+  auto takes = [&](int bm, int bn, int kg, float step) {
+    const size_t tiles = (size_t)((M + bm - 1) / bm) * (size_t)((N + bn - 1) / bn);
+    bool better = false;
+    for (int p = 1; p <= kLinParts && (p == 1 || (nsteps >= 4 * kg * p && (size_t)p * M * N * 4 <= kLinPartBytes)); ++p) {
+      const float rounds = (float)((tiles * (size_t)p + 255) / 256);
+      const float t = rounds * (float)((nsteps + p - 1) / p + 4 * kg) * step + (p > 1 ? 4.f + (float)p * (float)M * (float)N * 1.6e-6f : 0.f);
+      if (t >= best) continue;
+      best = t;
+      parts = p;
+      better = true;
+    }
+    return better;
   };
+  // (4 bits: two K groups of 128 x 256, 2048 x 4096 x 14336 Q4_K 237 us, one group 250; Q8_0, Q6_K 1024 x 8192 x 4096 80, 81 and 72, 78)
+  constexpr bool NIB = FMT == GQ_FMT_Q4_0 || FMT == GQ_FMT_Q4_K;
+  int tile = 0;
+  takes(256, 256, 1, 1.65f);
+  if (takes(128, 256, NIB ? 2 : 1, 1.f)) tile = 1;
+  if (takes(128, 128, 2, 0.56f)) tile = 2;
+  if (takes(64, 128, 4, 0.35f)) tile = 3;
+  if (nsteps % 4 == 0 && takes(32, 64, 4, 0.16f)) tile = 4;
 #define GQ_RB(P, ...) launch_rb<FMT, __VA_ARGS__>(w, a16, rs, e, part, P, M, N, K, s)
-  // About one workgroup a CU, by tiles of 256 x 256, 128 x 256, 64 x 256 in two K groups, 64 x 128 in four, 32 x 64 in four, us with the conversion
-  // of x (Q4_K, bf16; the 64-row tiles in two and four groups of M x 4096 x 14336 within 3 %):
-  //   2048 x 4096 x 14336                251 by 128 x 256, one round
-  //   512 x 4096 x 14336 (Q6_K)          86 by 128 x 256 in 4 parts, 101 by 64 x 256 in 2, 98 by 64 x 128
-  //   256 x 14336 x 4096                 46 by 64 x 256 (and by 128 x 128), 53 by 64 x 128
-  //   128 x 14336 x 4096                 39 by 64 x 256, 29 by 64 x 128, 51 by 32 x 64
-  //   256 x 4096 x 14336                 63, 49 by 64 x 128 in 1, 2 parts; 72 by 32 x 64
-  //   64 x 4096 x 14336                  56, 35, 25 by 64 x 128 in 1, 2, 4 parts; 36, 25, 27 by 32 x 64
-  //   64 x 4096 x 4096 (Q4_0)            23, 17, 15.5; 15.2, 13.5, 16.6
-  //   32 x 4096 x 14336                  56, 34, 24; 35, 23, 18.7 (16-row fragments as for fewer rows: 23)
-  //   64 x 14336 x 4096                  25.6 by 64 x 128, 27.8 by 32 x 64
-  if (wgs(256, 256) >= 384) return GQ_RB(1, 256, 8, 1, 3, 1);
-  const size_t wide = wgs(128, 256);
-  if (wide >= 192 || (wide >= 64 && M >= 256 && nsteps >= 128)) return GQ_RB(parts(wide, 1), 128, 8, 1, 4, 1);
-  if (wgs(64, 256) >= 192) return GQ_RB(1, 64, 8, 1, 4, 2);
-  if (nsteps % 4) return GQ_RB(parts(wgs(64, 128), 2), 64, 4, 1, 4, 2);
-  if (M <= 64 && wgs(32, 64) <= 256) return GQ_RB(parts(wgs(32, 64), 4), 32, 2, 1, 4, 4);
-  return GQ_RB(parts(wgs(64, 128), 4), 64, 4, 1, 3, 4);
+  if (tile == 0) return GQ_RB(parts, 256, 8, 1, 3, 1);
+  if (tile == 1) {
+    if constexpr (NIB) return GQ_RB(parts, 128, 8, 1, 3, 2);
+    else return GQ_RB(parts, 128, 8, 1, 4, 1);
+  }
+  if (tile == 2) return GQ_RB(parts, 128, 4, 1, 3, 2);
+  if (tile == 4) return GQ_RB(parts, 32, 2, 1, 4, 4);
+  if (nsteps % 4) return GQ_RB(parts, 64, 4, 1, 4, 2);  // (whole rounds of the groups)
+  return GQ_RB(parts, 64, 4, 1, 3, 4);
 #undef GQ_RB
 }
 

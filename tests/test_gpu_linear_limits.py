@@ -34,7 +34,7 @@ def backward(c, act=0, **kw):
 # formats with blocks of 32: K that is no whole chunk of the layout, and an odd number of them
 @pytest.mark.parametrize("fmt", [O.Q4_0, O.Q8_0])
 @pytest.mark.parametrize("m,n,k", [(1, 16, 32), (3, 33, 608), (4, 40, 96), (14, 70, 416), (20, 65, 160), (50, 65, 4128), (100, 70, 4128),
-                                   (300, 129, 224)])
+                                   (300, 129, 224), (20, 100, 288), (20, 100, 8288), (130, 300, 2144), (130, 9000, 160)])
 def test_short_chunks(dev, fmt, m, n, k):
     for dtype in (torch.float16, torch.bfloat16):
         c = Case(dev, fmt, m, n, k, seed=k, dtype=dtype)
@@ -47,7 +47,8 @@ def test_short_chunks(dev, fmt, m, n, k):
 @pytest.mark.parametrize("m,n,k", [(1, 4099, 4096), (2, 1500, 14336), (4, 300, 16128), (4, 100, 20480), (7, 1030, 8192), (12, 2100, 1024), (16, 14336, 256),
                                    (16, 100, 20480), (24, 600, 14336), (40, 3001, 2048), (40, 17000, 256), (64, 260, 4352), (90, 1500, 2304),
                                    (200, 4100, 1024), (200, 14000, 512), (260, 9000, 8192), (700, 13000, 512), (2050, 520, 512), (1500, 2100, 4096),
-                                   (6000, 4100, 512)])
+                                   (6000, 4100, 512), (200, 20000, 1024), (300, 520, 8192), (65, 20000, 4096), (512, 4100, 14336),
+                                   (130, 14000, 8192)])
 def test_large(dev, fmt, m, n, k):
     c = Case(dev, fmt, m, n, k, seed=n, dtype=torch.bfloat16)
     check_forward(c, 1, *forward(c, 1, save=True), torch.bfloat16)
