@@ -29,6 +29,7 @@ struct MoePlan {
   MoeBlk *blk;  // [maxblk], the blocks that there are first
   float *wsum;  // [pair] the weight (of the first pair of an expert that a token names twice: their sum)
   int maxblk;
+  int *count;  // tokens chosen for (zeroed by k_moe_logits)
 };
 
 // ---- router --------------------------------------------------------------------------
@@ -89,10 +90,11 @@ GQ_DEV double wave_sum(double v) {
 constexpr int kLogThreads = 256;
 template <int XT, int RT, int TOK>
 __global__ void __launch_bounds__(kLogThreads) k_moe_logits(const void *__restrict__ x, const void *__restrict__ wr,
-                                                            double *__restrict__ logits, MoeConv conv, int M, int E, int K) {
+                                                            double *__restrict__ logits, MoeConv conv, int *count, int M, int E, int K) {
   static_assert(TOK <= kLogThreads / 64, "a wave a row");
   __shared__ double red[kLogThreads / 64][TOK];
   const int tid = threadIdx.x, e = blockIdx.x, m0 = TOK * (int)blockIdx.y;
+  if (count && tid == 0 && e == 0 && m0 == 0) *count = 0;
   if (e == E) {
     const int w = tid >> 6;
     if (w < TOK && m0 + w < M) moe_convert<XT>(x, conv, m0 + w, K, tid & 63);
@@ -149,6 +151,11 @@ GQ_DEV uint32_t wave_max(uint32_t v) {
 #undef GQ_DPP_MAX
   return (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
 }
+// Values that another workgroup of the launch reads: past the caches that it does not share
+template <typename V>
+GQ_DEV void st_agent(V *p, V v) { __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+template <typename V>
+GQ_DEV V ld_agent(const V *p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
 GQ_DEV double lane_d(double v, int lane) {  // (lane: the same in all lanes)
   const uint64_t b = __builtin_bit_cast(uint64_t, v);
   const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)b, lane);
@@ -228,7 +235,7 @@ GQ_DEV void moe_choose(const RouteArgs &a, int m, int E, int top, int lane, int 
   }
   if (lane < top) {
     if (ids_s) ids_s[m * top + lane] = id;
-    if (a.ids) a.ids[m * top + lane] = id;
+    if (a.ids) st_agent(a.ids + m * top + lane, id);
   }
   if (!weighed) return;
   double w = id < 0 ? 0.0 : score(mine), total = 0.0;
@@ -239,7 +246,7 @@ GQ_DEV void moe_choose(const RouteArgs &a, int m, int E, int top, int lane, int 
   if (lane < top) {
     const float f = id < 0 ? 0.f : (float)(w * (double)a.scale);
     if (w_s) w_s[m * top + lane] = f;
-    if (a.weights) a.weights[m * top + lane] = f;
+    if (a.weights) st_agent(a.weights + m * top + lane, f);
   }
 }
 
@@ -248,10 +255,22 @@ __global__ void __launch_bounds__(64) k_moe_choose(RouteArgs a, int E, int top) 
   moe_choose<NE>(a, (int)blockIdx.x, E, top, (int)threadIdx.x, nullptr, nullptr);
 }
 
-// ---- plan: one workgroup ------------------------------------------------------------
+// ---- plan ---------------------------------------------------------------------------
 // The choice (NE: experts a lane; 0: ids and weights are given), each expert's pairs in order of their tokens, in blocks of 16.
 // Ids outside 0 .. E - 1 name no expert; an expert that a token names twice gets one pair with both weights.
 constexpr int kPlanThreads = 1024, kBlkRows = 16;
+// Is this workgroup the last of n to arrive at a counter (zero before the launch)?  What the others stored before they came, by st_agent, can
+// be read then, by ld_agent (fences in their place, which write back and drop whole caches: 2 us more).
+GQ_DEV bool arrives_last(int *counter, int n) {
+  __shared__ int last_s;
+  __builtin_amdgcn_s_waitcnt(0x0F70);  // (every wave's own stores have arrived)
+  __syncthreads();
+  if (threadIdx.x == 0)
+    last_s = __hip_atomic_fetch_add(counter, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == n - 1;
+  __syncthreads();
+  return last_s != 0;
+}
+// NE > 0: more tokens than a workgroup has waves are chosen for by a workgroup each, and the last to be done makes the plan.
 template <int NE>
 __global__ void __launch_bounds__(kPlanThreads) k_moe_plan(RouteArgs a, const int *__restrict__ ids, const float *__restrict__ weights,
                                                            MoePlan p, int M, int E, int top) {
@@ -261,13 +280,22 @@ __global__ void __launch_bounds__(kPlanThreads) k_moe_plan(RouteArgs a, const in
   __shared__ uint32_t tok_s[2][kPlanThreads];  // the tokens of an expert, a bit each
   __shared__ float w_s[MP];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, P = M * top;
-  tok_s[0][tid] = tok_s[1][tid] = 0;
   if constexpr (NE > 0) {
-    for (int m = wave; m < M; m += kPlanThreads / 64) moe_choose<NE>(a, m, E, top, lane, id_s, w_s);
+    if (gridDim.x > 1) {
+      if (wave == 0) moe_choose<NE>(a, (int)blockIdx.x, E, top, lane, nullptr, nullptr);
+      if (!arrives_last(p.count, (int)gridDim.x)) return;
+      if (tid < P) {
+        id_s[tid] = ld_agent(a.ids + tid);
+        w_s[tid] = ld_agent(a.weights + tid);
+      }
+    } else if (wave < M) {
+      moe_choose<NE>(a, wave, E, top, lane, id_s, w_s);
+    }
   } else if (tid < P) {
     id_s[tid] = ids[tid];
     w_s[tid] = weights[tid];
   }
+  tok_s[0][tid] = tok_s[1][tid] = 0;
   __syncthreads();
   const int tok = tid / top;
   int id = -1;
@@ -830,7 +858,7 @@ bool moe_few(const gq_moe &l, size_t M) {
 }
 // Where a call's intermediate values lie in its workspace
 struct MoeWs {
-  size_t logits, ids, weights, nblk, blk, wsum, a16, rs, h, h16, hs, part, bytes;
+  size_t logits, ids, weights, count, nblk, blk, wsum, a16, rs, h, h16, hs, part, bytes;
   int maxblk, parts;
 };
 MoeWs moe_ws(const gq_moe &l, size_t M) {
@@ -848,6 +876,7 @@ MoeWs moe_ws(const gq_moe &l, size_t M) {
   w.logits = take(M * l.n_experts * 8);
   w.ids = take(P * 4);
   w.weights = take(P * 4);
+  w.count = take(4);
   w.nblk = take(4);
   w.blk = take((size_t)w.maxblk * sizeof(MoeBlk));
   w.wsum = take(P * 4);
@@ -865,27 +894,27 @@ MoeWs moe_ws(const gq_moe &l, size_t M) {
 }
 
 template <int XT, int RT>
-int launch_logits_t(const gq_moe &l, const void *x, double *logits, const MoeConv &conv, int M, hipStream_t s) {
+int launch_logits_t(const gq_moe &l, const void *x, double *logits, const MoeConv &conv, int *count, int M, hipStream_t s) {
 #define GQ_LOG(TOK)                                                                                                       \
   hipLaunchKernelGGL((k_moe_logits<XT, RT, TOK>), dim3((unsigned)(l.n_experts + (conv.a16 != nullptr)),                  \
                                                        (unsigned)((M + (TOK)-1) / (TOK))),                               \
-                     dim3(kLogThreads), 0, s, x, l.router, logits, conv, M, (int)l.n_experts, (int)l.K)
+                     dim3(kLogThreads), 0, s, x, l.router, logits, conv, count, M, (int)l.n_experts, (int)l.K)
   if (M == 1) GQ_LOG(1);
   else GQ_LOG(4);
 #undef GQ_LOG
   return gq_last_launch();
 }
 template <int XT>
-int launch_logits_x(const gq_moe &l, const void *x, double *logits, const MoeConv &conv, int M, hipStream_t s) {
-  if (l.router_dtype == GQ_DT_F32) return launch_logits_t<XT, GQ_DT_F32>(l, x, logits, conv, M, s);
-  if (l.router_dtype == GQ_DT_F16) return launch_logits_t<XT, GQ_DT_F16>(l, x, logits, conv, M, s);
-  return launch_logits_t<XT, GQ_DT_BF16>(l, x, logits, conv, M, s);
+int launch_logits_x(const gq_moe &l, const void *x, double *logits, const MoeConv &conv, int *count, int M, hipStream_t s) {
+  if (l.router_dtype == GQ_DT_F32) return launch_logits_t<XT, GQ_DT_F32>(l, x, logits, conv, count, M, s);
+  if (l.router_dtype == GQ_DT_F16) return launch_logits_t<XT, GQ_DT_F16>(l, x, logits, conv, count, M, s);
+  return launch_logits_t<XT, GQ_DT_BF16>(l, x, logits, conv, count, M, s);
 }
 int launch_plan(const gq_moe &l, const RouteArgs &a, const int *ids, const float *weights, const MoePlan &plan, int M,
                 hipStream_t s) {
   const int E = (int)l.n_experts;
 #define GQ_PLAN(NE)                                                                                                       \
-  hipLaunchKernelGGL(k_moe_plan<NE>, dim3(1), dim3(kPlanThreads), 0, s, a, ids, weights, plan, M, E, l.top_k)
+  hipLaunchKernelGGL(k_moe_plan<NE>, dim3((NE) > 0 && M > kPlanThreads / 64 ? (unsigned)M : 1u), dim3(kPlanThreads), 0, s, a, ids, weights, plan, M, E, l.top_k)
   if (!a.logits) GQ_PLAN(0);
   else if (E <= 64) GQ_PLAN(1);
   else if (E <= 128) GQ_PLAN(2);
@@ -904,10 +933,10 @@ int launch_choose(const gq_moe &l, const RouteArgs &a, int M, hipStream_t s) {
 #undef GQ_CHOOSE
   return gq_last_launch();
 }
-int launch_logits(const gq_moe &l, const void *x, int xt, double *logits, const MoeConv &conv, int M, hipStream_t s) {
-  if (xt == GQ_DT_F32) return launch_logits_x<GQ_DT_F32>(l, x, logits, conv, M, s);
-  if (xt == GQ_DT_F16) return launch_logits_x<GQ_DT_F16>(l, x, logits, conv, M, s);
-  return launch_logits_x<GQ_DT_BF16>(l, x, logits, conv, M, s);
+int launch_logits(const gq_moe &l, const void *x, int xt, double *logits, const MoeConv &conv, int *count, int M, hipStream_t s) {
+  if (xt == GQ_DT_F32) return launch_logits_x<GQ_DT_F32>(l, x, logits, conv, count, M, s);
+  if (xt == GQ_DT_F16) return launch_logits_x<GQ_DT_F16>(l, x, logits, conv, count, M, s);
+  return launch_logits_x<GQ_DT_BF16>(l, x, logits, conv, count, M, s);
 }
 
 // Intermediate values of a call
@@ -1035,7 +1064,7 @@ struct MoeRoom {
   }
 };
 MoePlan plan_of(const MoeWs &w, uint8_t *ws) {
-  return MoePlan{(int *)(ws + w.nblk), (MoeBlk *)(ws + w.blk), (float *)(ws + w.wsum), w.maxblk};
+  return MoePlan{(int *)(ws + w.nblk), (MoeBlk *)(ws + w.blk), (float *)(ws + w.wsum), w.maxblk, (int *)(ws + w.count)};
 }
 
 }  // namespace
@@ -1060,7 +1089,7 @@ extern "C" int gq_moe_route(const gq_moe *l, const void *x, int x_dtype, int32_t
   MoeRoom room(ws, ws_bytes, M * l->n_experts * 8, s);
   GQ_TRY(room.status);
   double *logits = (double *)room.ptr;
-  GQ_TRY(launch_logits(*l, x, x_dtype, logits, MoeConv{}, (int)M, s));
+  GQ_TRY(launch_logits(*l, x, x_dtype, logits, MoeConv{}, nullptr, (int)M, s));
   return launch_choose(*l, RouteArgs{logits, l->router_bias, ids, weights, l->score, l->renorm, l->scale}, (int)M, s);
 }
 
@@ -1098,15 +1127,11 @@ extern "C" int gq_moe_layer(const gq_moe *l, const void *x, int x_dtype, const v
   if (!ids) ids = (int32_t *)(room.ptr + w.ids);
   if (!weights) weights = (float *)(room.ptr + w.weights);
   RouteArgs a = {(double *)(room.ptr + w.logits), l->router_bias, ids, weights, l->score, l->renorm, l->scale};
-  GQ_TRY(launch_logits(*l, x, x_dtype, (double *)(room.ptr + w.logits), conv, (int)M, s));
-  // The choice, a wave a token: few tokens with the gate and up products, in the plan's workgroup where each of its 16 waves has one at most
-  // (four tokens a wave, 64 of 128 experts: 22 us, against 5 and 5 of two launches), else in a launch of its own.
-  const bool few = moe_few(*l, M), within = few && l->n_experts <= 64 * kFewNE, own = !within && (few || M > kPlanThreads / 64);
-  if (own) GQ_TRY(launch_choose(*l, a, (int)M, s));
-  if (!few) {
-    RouteArgs b = a;
-    if (own) b.logits = nullptr;
-    GQ_TRY(launch_plan(*l, b, ids, weights, plan, (int)M, s));
-  }
+  const bool few = moe_few(*l, M), within = few && l->n_experts <= 64 * kFewNE;
+  GQ_TRY(launch_logits(*l, x, x_dtype, (double *)(room.ptr + w.logits), conv, few ? nullptr : plan.count, (int)M, s));
+  // The choice, a wave a token: few tokens with the gate and up products, else with the plan (four tokens a wave of one workgroup, 64 of 128
+  // experts: 22 us; a workgroup a token, the last of them making the plan, 8, in two launches 5 and 5)
+  if (!few) GQ_TRY(launch_plan(*l, a, ids, weights, plan, (int)M, s));
+  else if (!within) GQ_TRY(launch_choose(*l, a, (int)M, s));
   return moe_products(*l, x, x_dtype, within ? &a : nullptr, ids, weights, plan, mid, resid, y, y_dtype, (int)M, s);
 }
