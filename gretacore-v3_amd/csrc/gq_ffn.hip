@@ -986,9 +986,15 @@ __global__ void __launch_bounds__(64 * WN * KG) k_front_dx(const uint8_t *__rest
       }
     }
 }
-// dx = rs[m] * the parts' sums, in part order (no parts: zeros)
+// dx = rs[m] * the parts' sums, in part order (no parts: zeros).  Workgroups behind its own: a bias gradient, 16 columns each (db: gq_internal.h)
 __global__ void __launch_bounds__(256) k_dx_sum(const float *__restrict__ part, const float *__restrict__ rs, void *__restrict__ y,
-                                                int dt, size_t mk, int K, int parts) {
+                                                int dt, size_t mk, int K, int parts, GqColSums db) {
+  const unsigned own = (unsigned)((mk / 4 + 255) / 256);
+  if (blockIdx.x >= own) {
+    __shared__ double red[16][16];
+    gq_col_sums<16, 16>(db, 16 * (int)(blockIdx.x - own), threadIdx.x & 15, threadIdx.x >> 4, red);
+    return;
+  }
   const size_t i = ((size_t)blockIdx.x * 256 + threadIdx.x) * 4;  // (K % 32 == 0: four of one row)
   if (i >= mk) return;
   gq_f4 v = {0.f, 0.f, 0.f, 0.f};
@@ -1316,10 +1322,10 @@ int launch_dx(const GqDxPlan &p, const void *wg, const void *wu, const _Float16 
   }
 #undef GQ_DX
 }
-int launch_dx_sum(const float *part, const float *rs, void *y, int dt, size_t M, size_t K, int parts, hipStream_t s) {
-  const size_t mk = M * K, wgs = (mk / 4 + 255) / 256;
+int launch_dx_sum(const float *part, const float *rs, void *y, int dt, size_t M, size_t K, int parts, const GqColSums &db, hipStream_t s) {
+  const size_t mk = M * K, wgs = (mk / 4 + 255) / 256 + (size_t)(db.n + 15) / 16;
   GQ_CHECK(wgs <= 0x7FFFFFFFu, GQ_ERR_INVALID_ARGS);  // (one grid dimension)
-  hipLaunchKernelGGL(k_dx_sum, dim3((unsigned)wgs), dim3(256), 0, s, part, rs, y, dt, mk, (int)K, parts);
+  hipLaunchKernelGGL(k_dx_sum, dim3((unsigned)wgs), dim3(256), 0, s, part, rs, y, dt, mk, (int)K, parts, db);
   return gq_last_launch();
 }
 template <int DT>
@@ -1336,16 +1342,16 @@ size_t gq_dx_rs_bytes(const GqDxPlan &p) { return dx_rs_bytes(p); }
 size_t gq_dx_bytes(const GqDxPlan &p, size_t K) { return dx_bytes(p, K); }
 size_t gq_dx_most_bytes(size_t M, size_t N, size_t K, int mats) { return dx_most_bytes(M, N, K, mats); }
 int gq_launch_dx(int fmt, const GqDxPlan &p, const void *w0, const void *w1, const _Float16 *a16, const float *rs, float *part,
-                 void *y, int dt, int M, size_t N, size_t K, hipStream_t s) {
+                 void *y, int dt, int M, size_t N, size_t K, const GqColSums &db, hipStream_t s) {
   void *to = p.parts > 1 ? (void *)part : y;
   if (fmt == GQ_FMT_Q4_0) GQ_TRY(launch_dx<GQ_FMT_Q4_0>(p, w0, w1, a16, rs, to, dt, M, N, K, s));
   else if (fmt == GQ_FMT_Q8_0) GQ_TRY(launch_dx<GQ_FMT_Q8_0>(p, w0, w1, a16, rs, to, dt, M, N, K, s));
   else if (gq_fmt_is_q6k(fmt)) GQ_TRY(launch_dx<GQ_FMT_Q6_K>(p, w0, w1, a16, rs, to, dt, M, N, K, s));
   else GQ_TRY(launch_dx<GQ_FMT_Q4_K>(p, w0, w1, a16, rs, to, dt, M, N, K, s));
-  return p.parts > 1 ? launch_dx_sum(part, rs, y, dt, (size_t)M, K, p.parts, s) : GQ_OK;
+  return p.parts > 1 ? launch_dx_sum(part, rs, y, dt, (size_t)M, K, p.parts, db, s) : GQ_OK;
 }
 int gq_launch_zeros(void *y, int dt, size_t M, size_t K, hipStream_t s) {
-  return launch_dx_sum(nullptr, nullptr, y, dt, M, K, 0, s);
+  return launch_dx_sum(nullptr, nullptr, y, dt, M, K, 0, GqColSums{}, s);
 }
 
 extern "C" size_t gq_ffn_gate_up_bwd_workspace_bytes(int fmt, size_t M, size_t N, size_t K) {
@@ -1361,7 +1367,7 @@ extern "C" int gq_ffn_gate_up_bwd(int fmt, const void *gate, const void *up, con
   if (M == 0 || (!dg && !du && !dx)) return GQ_OK;
   GQ_CHECK(K > 0, GQ_ERR_INVALID_ARGS);
   hipStream_t s = (hipStream_t)stream;
-  if (N == 0) return dx ? launch_dx_sum(nullptr, nullptr, dx, dx_dtype, M, K, 0, s) : GQ_OK;  // (sums of nothing)
+  if (N == 0) return dx ? launch_dx_sum(nullptr, nullptr, dx, dx_dtype, M, K, 0, GqColSums{}, s) : GQ_OK;  // (sums of nothing)
   GQ_CHECK(dh && g && u, GQ_ERR_INVALID_ARGS);
   const GqDxPlan plan = dx_plan(M, N, K, 2);
   const size_t need = dx ? gq_ffn_gate_up_bwd_workspace_bytes(fmt, M, N, K) : 0;
@@ -1382,7 +1388,7 @@ extern "C" int gq_ffn_gate_up_bwd(int fmt, const void *gate, const void *up, con
     else if (dtype == GQ_DT_F16) GQ_TRY(launch_dgu<GQ_DT_F16>(at(dh), at(g), at(u), at(dg), at(du), a16, rs, m, (int)N, (int)plan.np, act, s));
     else GQ_TRY(launch_dgu<GQ_DT_BF16>(at(dh), at(g), at(u), at(dg), at(du), a16, rs, m, (int)N, (int)plan.np, act, s));
     if (!dx) continue;
-    GQ_TRY(gq_launch_dx(fmt, plan, gate, up, a16, rs, part, (uint8_t *)dx + m0 * xs, dx_dtype, m, N, K, s));
+    GQ_TRY(gq_launch_dx(fmt, plan, gate, up, a16, rs, part, (uint8_t *)dx + m0 * xs, dx_dtype, m, N, K, GqColSums{}, s));
   }
   return GQ_OK;
 }

@@ -112,10 +112,16 @@ int gq_launch_split_sum(const float *part, float *c, size_t n, int parts, hipStr
 // Sums over the weights' rows, y[m][k] = sum over n of a0[m][n] W0[n][k] (+ a1[m][n] W1[n][k], mats = 2), of up to mb rows
 // at a time (gq_ffn.hip).  A is fp16 [m][mats * np], each half padded with zeros to np columns, rs its row
 // scales; part: the parts' sums, behind dx_a_bytes and dx_rs_bytes in a workspace of dx_bytes (dx_most_bytes: enough
-// for every call of at most M rows).
+// for every call of at most M rows).  db: sums that the launch which adds parts (parts > 1) does beside them.
 struct GqDxPlan {
   size_t mb, np;
   int shape, parts, sps, mats;
+};
+// Sums of columns to come: db[n] = the sum over p of part[p][n], p < parts (n 0: nothing)
+struct GqColSums {
+  const float *part;
+  float *db;
+  int n, parts;
 };
 GqDxPlan gq_dx_plan(size_t M, size_t N, size_t K, int mats);
 size_t gq_dx_a_bytes(const GqDxPlan &p);
@@ -123,7 +129,7 @@ size_t gq_dx_rs_bytes(const GqDxPlan &p);
 size_t gq_dx_bytes(const GqDxPlan &p, size_t K);
 size_t gq_dx_most_bytes(size_t M, size_t N, size_t K, int mats);
 int gq_launch_dx(int fmt, const GqDxPlan &p, const void *w0, const void *w1, const _Float16 *a16, const float *rs, float *part,
-                 void *y, int dt, int M, size_t N, size_t K, hipStream_t s);
+                 void *y, int dt, int M, size_t N, size_t K, const GqColSums &db, hipStream_t s);
 // zeros [M][K] of an activation dtype (K % 32 == 0)
 int gq_launch_zeros(void *y, int dt, size_t M, size_t K, hipStream_t s);
 // Compute units of the current device (cached per device; 0 without a device).

@@ -450,6 +450,23 @@ GQ_DEV void step_barrier() {
 // waves per SIMD: what a workgroup brings, at least two
 constexpr int front_wpe(int waves) { return waves > 4 ? waves / 4 : 2; }
 
+// Columns n0 .. n0 + COLS - 1 of c, thread (lane, group): GROUPS groups add parts g, g + GROUPS, ... in 64 bits, then the groups in order
+template <int COLS, int GROUPS>
+GQ_DEV void gq_col_sums(const GqColSums &c, int n0, int lane, int group, double (*red)[COLS]) {
+  const int n = n0 + lane;
+  double v = 0.0;
+  if (n < c.n) {
+#pragma unroll 8
+    for (int p = group; p < c.parts; p += GROUPS) v += (double)c.part[(size_t)p * (size_t)c.n + n];
+  }
+  red[group][lane] = v;
+  __syncthreads();
+  if (group > 0 || n >= c.n) return;
+#pragma unroll
+  for (int g = 1; g < GROUPS; ++g) v += red[g][lane];
+  c.db[n] = (float)v;
+}
+
 // 8 values of a row of n from column k on (zeros behind it)
 template <int DT>
 GQ_DEV void dgu_load(const void *p, size_t row, int k, int n, float (&o)[8]) {
