@@ -10,6 +10,7 @@ from __future__ import annotations
 import ctypes
 import functools
 import os
+import struct
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "lib", "libgq.so")
@@ -147,6 +148,10 @@ class MoeLayer(ctypes.Structure):
                 ("gate", _vp), ("up", _vp), ("down", _vp), ("n_experts", _c_size), ("N", _c_size), ("K", _c_size),
                 ("router", _vp), ("router_bias", _vp), ("router_dtype", ctypes.c_int), ("score", ctypes.c_int),
                 ("renorm", ctypes.c_int), ("scale", ctypes.c_float)]
+
+
+# (the same as bytes, in half the time or less: 1.5 us a call; a pointer that is not there: 0)
+_moe_pack = struct.Struct("@4i3P3N2P3if").pack
 
 
 class ChainOp(ctypes.Structure):
@@ -880,12 +885,12 @@ def moe_route(router, x, k: int, n_experts: int, top_k: int, score: int = SCORE_
     m, device = _rows(x, k, "x")
     _router_operands(router, router_bias, n_experts, k, device)
     ids, weights = _choice(ids, weights, m, top_k, x, device)
-    layer = MoeLayer(0, 0, 0, top_k, None, None, None, n_experts, 0, k, router.data_ptr(), _ptr(router_bias), _dt(router.dtype),
-                     score, renorm, scale)
+    layer = _moe_pack(0, 0, 0, top_k, 0, 0, 0, n_experts, 0, k, router.data_ptr(), _ptr(router_bias) or 0, _dt(router.dtype),
+                      score, renorm, scale)
     ws_ptr, ws_n = None, 0
     if workspace is not None:
-        ws_ptr, ws_n = _room(workspace, load().gq_moe_route_workspace_bytes(ctypes.addressof(layer), m), device)
-    st = load().gq_moe_route(ctypes.addressof(layer), x.data_ptr(), _dt(x.dtype), ids.data_ptr(), weights.data_ptr(), m, ws_ptr,
+        ws_ptr, ws_n = _room(workspace, load().gq_moe_route_workspace_bytes(layer, m), device)
+    st = load().gq_moe_route(layer, x.data_ptr(), _dt(x.dtype), ids.data_ptr(), weights.data_ptr(), m, ws_ptr,
                              ws_n, _raw_stream(device))
     if st:
         check(st, "gq_moe_route")
@@ -936,17 +941,16 @@ def _moe_call(route, fmt, gate, up, fmt_down, down, router, x, n, k, n_experts, 
         y = x.new_empty(m, k, dtype=dtype) if dtype != x.dtype else x.new_empty(m, k)
     else:
         _operand(y, (m, k), "y", device)
-    layer = MoeLayer(fmt, fmt_down, act, top_k, gate.data_ptr(), up.data_ptr(), down.data_ptr(), n_experts, n, k, _ptr(router),
-                     _ptr(router_bias), _dt(router.dtype) if router is not None else 0, score, renorm, scale)
+    layer = _moe_pack(fmt, fmt_down, act, top_k, gate.data_ptr(), up.data_ptr(), down.data_ptr(), n_experts, n, k, _ptr(router) or 0,
+                      _ptr(router_bias) or 0, _dt(router.dtype) if router is not None else 0, score, renorm, scale)
     ws_ptr, ws_n = None, 0
     if workspace is not None:
         ws_ptr, ws_n = _room(workspace, _moe_bytes(fmt, fmt_down, m, n, k, n_experts, top_k), device)
-    at = ctypes.addressof(layer)
     if route:
-        st = load().gq_moe_layer(at, x.data_ptr(), _dt(x.dtype), _ptr(resid), y.data_ptr(), _dt(dtype), _ptr(ids), _ptr(weights),
+        st = load().gq_moe_layer(layer, x.data_ptr(), _dt(x.dtype), _ptr(resid), y.data_ptr(), _dt(dtype), _ptr(ids), _ptr(weights),
                                  m, ws_ptr, ws_n, _raw_stream(device))
     else:
-        st = load().gq_moe_ffn(at, x.data_ptr(), _dt(x.dtype), ids.data_ptr(), weights.data_ptr(), _ptr(resid), y.data_ptr(),
+        st = load().gq_moe_ffn(layer, x.data_ptr(), _dt(x.dtype), ids.data_ptr(), weights.data_ptr(), _ptr(resid), y.data_ptr(),
                                _dt(dtype), m, ws_ptr, ws_n, _raw_stream(device))
     if st:
         check(st, "gq_moe_layer" if route else "gq_moe_ffn")
