@@ -331,12 +331,12 @@ int gq_w4_gate_up(const void *d_gate, const void *d_up, int group, const void *d
  * Sums are fp32, bias, activation and residual are applied to them in fp32, and
  * y and z are rounded once.  x and the weights enter the matrix cores as in gq_ffn_gate_up: one to four rows
  * of 16-bit x as they are (of bf16 rows the finite values stay below 2^115), all others rounded to fp16
- * after a power-of-two scale per row; up to 64 rows keep the k-quants' d (and dmin) in fp32, more
- * fold them into fp16 weights. */
+ * after a power-of-two scale per row (fp16 rows of whole 128s, 16-byte aligned, with Q8_0 or Q6_K weights: as they are); up to
+ * 16 rows keep the k-quants' d (and dmin) in fp32, more fold them into fp16 weights. */
 #define GQ_ACT_NONE 2 /* z */
 #define GQ_ACT_RELU 3 /* max(z, 0); beside these GQ_ACT_SILU and GQ_ACT_GELU_TANH */
-/* A workspace of NULL takes scratch memory of the call's own, as in gq_ffn_gate_up; calls that need none (the rows of
- * x that go in as they are) run without under capture too.  The bytes for M rows are enough for every call of
+/* A workspace of NULL takes scratch memory of the call's own, as in gq_ffn_gate_up; calls that need none (one to four rows of 16-bit
+ * x, together up to 65536 values) run without under capture too.  The bytes for M rows are enough for every call of
  * fewer.  N * 256 outputs stay below 2^31 bytes; K == 0 is refused. */
 size_t gq_linear_workspace_bytes(int fmt, size_t M, size_t N, size_t K);
 int gq_linear(int fmt, const void *d_packed, const void *d_x, int x_dtype, const void *d_bias, int bias_dtype, int act,
@@ -386,7 +386,8 @@ int gq_moe_route(const gq_moe *layer, const void *d_x, int x_dtype, int32_t *d_i
  * that another device holds, an empty slot), an expert named twice counts with both weights.  x is [M][K] of
  * x_dtype, y and resid (NULL: none; it may be y) [M][K] of y_dtype, all contiguous.  Sums, h and the weighted sum are
  * fp32, y is rounded once; x and h enter the matrix cores in fp16 after a power-of-two scale per row (one to
- * four tokens: x as it is, h with a scale per row and 128 values), weights as in gq_ffn_gate_up's kernels of few rows. */
+ * four tokens: x of 16 bits as it is, of bf16 the finite values below 2^115, and h with a scale per 32 values), weights as in
+ * gq_ffn_gate_up's kernels of few rows.  y and resid overlap nothing else. */
 int gq_moe_ffn(const gq_moe *layer, const void *d_x, int x_dtype, const int32_t *d_ids, const float *d_weights,
                const void *d_resid, void *d_y, int y_dtype, size_t M, void *d_workspace, size_t workspace_bytes,
                void *stream);

@@ -599,3 +599,15 @@ def test_a_block_decodes(dev, fmt, down):
         one = run(la, t[i:i + 1], top, resid=s[i:i + 1], save=True, workspace=ws)
         assert torch.equal(one[1], ids[i:i + 1]) and torch.equal(one[2], w[i:i + 1])
         check(la, t[i:i + 1], rid[i:i + 1], rw[i:i + 1], 0, s[i:i + 1], one[0])
+
+
+@pytest.mark.parametrize("m", [1, 3, 9, 64])
+def test_no_expert_at_all(dev, m):
+    """Ids that all name none: the residual, or zeros."""
+    la = Layer(dev, O.Q4_K, O.Q8_0, 3, 256, 256, seed=25)
+    x, w = la.x(m, torch.bfloat16), torch.rand(m, 2, generator=la.gen).to(dev)
+    ids = torch.full((m, 2), -1, dtype=torch.int32, device=dev)
+    ids[:, 1] = 3
+    resid = torch.randn(m, 256, generator=la.gen).to(torch.bfloat16).to(dev)
+    assert bool((products(la, x, ids, w) == 0).all())
+    assert torch.equal(products(la, x, ids, w, resid=resid), resid)
