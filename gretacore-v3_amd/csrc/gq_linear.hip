@@ -207,8 +207,11 @@ int launch_few_t(const void *w, const void *x, const float *rs, const LinEpi &e,
     if (M == 1) GQ_FEW(1, R, KS, PD); \
     else GQ_FEW(4, R, KS, PD);        \
   } while (0)
-  // (Q4_K, one row: 4096 x 14336 by one tile 9.6 us, by two 12.5; Q4_0 14336 x 4096 11.1 and 9.0)
-  if (tiles <= 320) GQ_FEW_M(1, 16, 2);
+  // One tile and 16 waves up to a workgroup a CU, 8 waves up to two, then two tiles, which share what is done for x (one row, us by one tile and 16
+  // waves / one and 8 / two and 8: 4096 x 14336 Q4_K 9.3 / 11.7 / 13.7; 5120 x 5120 Q6_K 10.2 / 8.0 / 8.7; 8192 x 8192 Q4_0 11.9 / 9.6 / 10.3;
+  // 14336 x 4096 Q4_K 11.7 / 9.9 / 9.4, Q8_0 13.3 / 12.7 / 13.2)
+  if (tiles <= 256) GQ_FEW_M(1, 16, 2);
+  else if (tiles <= 512) GQ_FEW_M(1, 8, 2);
   else GQ_FEW_M(2, 8, 2);
 #undef GQ_FEW_M
 #undef GQ_FEW
@@ -221,9 +224,12 @@ int launch_rows_t(const void *w, const _Float16 *a16, int lda, const float *rs, 
 #define GQ_ROWS(R, KS, PD)                                                                                               \
   hipLaunchKernelGGL((k_lin_rows<FMT, 1, R, KS, group_stages<FMT>(PD)>), dim3((unsigned)((tiles + (R)-1) / (R))), dim3(64 * (KS)), 0, s,      \
                      (const uint8_t *)w, gq_sc_plane_offset(FMT, N, K), a16, lda, rs, e, M, N, (int)gq_chunks(FMT, K), units)
-  // Two tiles share the rows of x where there are workgroups enough; long rows by few waves (16 rows, us by two tiles and 4 waves / one
-  // and 8 / one and 4, deeper: 14336 x 4096 Q4_K 15.6 / 22 / 19.6; 4096 x 14336 24.4 / 21.8 / 19.5; 4096 x 4096 Q4_0 9.6 / 8.1 / 8.4)
+  // Two tiles share the rows of x (which every workgroup reads whole) where that leaves a workgroup for every other CU; long rows of one tile by few
+  // waves.  16 rows, us by two tiles and 4 waves / two and 8 / one and 8 / one and 4, deeper:
+  //   14336 x 4096 Q4_K 15.2 / 14.5 / 18.6 / 18.8, Q4_0 14.6 / 15.4 / 20.6 / 19.7    6144 x 14336 Q4_K 25.7 / 23.1 / - / 30.6, Q8_0 24.9 / 24.6 / - / 34.3
+  //   4096 x 14336 Q4_K 24.9 / 22.4 / 19.4 / 19.5, Q8_0 23.7 / 23.4 / 20.3 / 19.5    8 rows, 4096 x 4096 Q8_0 8.5 / 8.3 / 6.5 / 6.9
   if (tiles > 512) GQ_ROWS(2, 4, 2);
+  else if (tiles > 256) GQ_ROWS(2, 8, 2);
   else if (units > 64) GQ_ROWS(1, 4, 4);
   else GQ_ROWS(1, 8, 2);
 #undef GQ_ROWS

@@ -44,7 +44,7 @@ def test_short_chunks(dev, fmt, m, n, k):
 
 # few rows of wide and of long matrices, each tile of the rule with K in parts and without, many rows
 @pytest.mark.parametrize("fmt", [O.Q4_0, O.Q8_0, O.Q4_K, O.Q6_K])
-@pytest.mark.parametrize("m,n,k", [(1, 4099, 4096), (2, 1500, 14336), (4, 300, 16128), (4, 100, 20480), (7, 1030, 8192), (12, 2100, 1024), (16, 14336, 256),
+@pytest.mark.parametrize("m,n,k", [(1, 4099, 4096), (1, 9003, 1024), (2, 1500, 14336), (3, 5001, 2048), (11, 5003, 4096), (4, 300, 16128), (4, 100, 20480), (7, 1030, 8192), (12, 2100, 1024), (16, 14336, 256),
                                    (16, 100, 20480), (24, 600, 14336), (40, 3001, 2048), (40, 17000, 256), (64, 260, 4352), (90, 1500, 2304),
                                    (200, 4100, 1024), (200, 14000, 512), (260, 9000, 8192), (700, 13000, 512), (2050, 520, 512), (1500, 2100, 4096),
                                    (6000, 4100, 512), (200, 20000, 1024), (300, 520, 8192), (65, 20000, 4096), (512, 4100, 14336),
