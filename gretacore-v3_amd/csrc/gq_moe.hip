@@ -19,16 +19,17 @@ namespace {
 
 constexpr int kMoeFew = 4;  // tokens that the kernels of few rows take
 
-// A block of an expert's work: up to 16 of its pairs (token * top + slot).  expert -1: no block.
+// A block of an expert's work: up to 16 (with more tokens an expert 32: 2^MoePlan::sh) of its pairs (token * top + slot).  expert -1: no block.
+constexpr int kMoeTiles = 2;  // row tiles of 16 of a block at most
 struct MoeBlk {
   int expert, count;
-  int pair[16];
+  int pair[16 * kMoeTiles];
 };
 struct MoePlan {
   int *nblk;
   MoeBlk *blk;  // [maxblk], the blocks that there are first
   float *wsum;  // [pair] the weight (of the first pair of an expert that a token names twice: their sum)
-  int maxblk;
+  int maxblk, sh;  // 2^sh: rows of a block
   int *count;  // tokens chosen for (zeroed by k_moe_logits)
 };
 
@@ -258,7 +259,7 @@ __global__ void __launch_bounds__(64) k_moe_choose(RouteArgs a, int E, int top) 
 // ---- plan ---------------------------------------------------------------------------
 // The choice (NE: experts a lane; 0: ids and weights are given), each expert's pairs in order of their tokens, in blocks of 16.
 // Ids outside 0 .. E - 1 name no expert; an expert that a token names twice gets one pair with both weights.
-constexpr int kPlanThreads = 1024, kBlkRows = 16;
+constexpr int kPlanThreads = 1024;
 // Is this workgroup the last of n to arrive at a counter (zero before the launch)?  What the others stored before they came, by st_agent, can
 // be read then, by ld_agent (fences in their place, which write back and drop whole caches: 2 us more).
 GQ_DEV bool arrives_last(int *counter, int n) {
@@ -315,7 +316,7 @@ __global__ void __launch_bounds__(kPlanThreads) k_moe_plan(RouteArgs a, const in
     if (id >= 0) atomicOr(&tok_s[tok >> 5][id], 1u << (tok & 31));
   }
   __syncthreads();
-  const int c = __popc(tok_s[0][tid]) + __popc(tok_s[1][tid]), nb = (c + kBlkRows - 1) / kBlkRows;
+  const int c = __popc(tok_s[0][tid]) + __popc(tok_s[1][tid]), nb = (c + (1 << p.sh) - 1) >> p.sh;
   int inc = nb;
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) {
@@ -334,7 +335,7 @@ __global__ void __launch_bounds__(kPlanThreads) k_moe_plan(RouteArgs a, const in
   base_s[tid] = base;
   for (int b = 0; b < nb; ++b) {
     p.blk[base + b].expert = tid;
-    p.blk[base + b].count = min(c - kBlkRows * b, kBlkRows);
+    p.blk[base + b].count = min(c - (b << p.sh), 1 << p.sh);
   }
   for (int b = all + tid; b < p.maxblk; b += kPlanThreads) p.blk[b].expert = -1;
   if (tid == 0) *p.nblk = all;
@@ -342,7 +343,7 @@ __global__ void __launch_bounds__(kPlanThreads) k_moe_plan(RouteArgs a, const in
   if (id >= 0) {
     const uint32_t below = (1u << (tok & 31)) - 1u, w0 = tok_s[0][id], w1 = tok_s[1][id];
     const int rank = tok < 32 ? __popc(w0 & below) : __popc(w0) + __popc(w1 & below);
-    p.blk[base_s[id] + rank / kBlkRows].pair[rank % kBlkRows] = tid;
+    p.blk[base_s[id] + (rank >> p.sh)].pair[rank & ((1 << p.sh) - 1)] = tid;
   }
 }
 
@@ -489,13 +490,13 @@ k_moe_gu_few(const uint8_t *__restrict__ wg, const uint8_t *__restrict__ wu, siz
 }
 
 // More tokens: a block's rows are its pairs, fp16 rows of x gathered, the scale groups folded into the weights.
-template <int FMT, int R, int KS, int PD>
+template <int FMT, int MT, int R, int KS, int PD>
 __global__ void __launch_bounds__(64 * KS)
 k_moe_gu_rows(const uint8_t *__restrict__ wg, const uint8_t *__restrict__ wu, size_t sc_off, const _Float16 *__restrict__ a16,
               int lda, const float *__restrict__ rs, MoePlan p, float *__restrict__ h, int M, int N, int C, int units, int act,
               int top) {
   constexpr int T = 2 * R;
-  __shared__ gq_f4 red[KS][T][64];
+  __shared__ gq_f4 red[KS][T][MT][64];
   const MoeBlk &blk = p.blk[blockIdx.y];
   const int expert = __builtin_amdgcn_readfirstlane(blk.expert);
   if (expert < 0) return;
@@ -510,41 +511,53 @@ k_moe_gu_rows(const uint8_t *__restrict__ wg, const uint8_t *__restrict__ wu, si
   }
   const __amdgpu_buffer_rsrc_t xr = __builtin_amdgcn_make_buffer_rsrc(
       const_cast<_Float16 *>(a16), (short)0, (int)(2u * (uint32_t)M * (uint32_t)lda), 0x00020000);
-  const bool row = r < blk.count;
-  const uint32_t xo = row ? 2u * ((uint32_t)(blk.pair[r] / top) * (uint32_t)lda + 16u * (uint32_t)g) : 0u;
+  bool row[MT];
+  uint32_t xo[MT];
+#pragma unroll
+  for (int t = 0; t < MT; ++t) {
+    row[t] = 16 * t + r < blk.count;
+    xo[t] = row[t] ? 2u * ((uint32_t)(blk.pair[16 * t + r] / top) * (uint32_t)lda + 16u * (uint32_t)g) : 0u;
+  }
   constexpr int G = kGroup<FMT>;
   FUnit<FMT> us[PD][T][G];
-  gq_half8 xs[PD][G][1][4];
+  gq_half8 xs[PD][G][MT][4];
   auto request = [&](int group, int st) __attribute__((always_inline)) {
 #pragma unroll
     for (int t = 0; t < T; ++t) load_group<FMT>(tl[t], group, lane, us[st][t]);
-    const uint32_t o = row && G * group < units ? xo + 256u * G * (uint32_t)group : 0xFFFFFC00u;
 #pragma unroll
-    for (int i = 0; i < 4 * G; ++i) {
-      const auto v = __builtin_amdgcn_raw_buffer_load_b128(xr, o + 128u * (i >> 1) + 16u * (i & 1), 0, 0);
-      xs[st][i >> 2][0][i & 3] = __builtin_bit_cast(gq_half8, gq_u4{v[0], v[1], v[2], v[3]});
+    for (int t = 0; t < MT; ++t) {
+      const uint32_t o = row[t] && G * group < units ? xo[t] + 256u * G * (uint32_t)group : 0xFFFFFC00u;
+#pragma unroll
+      for (int i = 0; i < 4 * G; ++i) {
+        const auto v = __builtin_amdgcn_raw_buffer_load_b128(xr, o + 128u * (i >> 1) + 16u * (i & 1), 0, 0);
+        xs[st][i >> 2][t][i & 3] = __builtin_bit_cast(gq_half8, gq_u4{v[0], v[1], v[2], v[3]});
+      }
     }
   };
-  gq_f4 acc[T][1];
+  gq_f4 acc[T][MT];
 #pragma unroll
-  for (int t = 0; t < T; ++t) acc[t][0] = gq_f4{0.f, 0.f, 0.f, 0.f};
+  for (int t = 0; t < T; ++t)
+#pragma unroll
+    for (int m = 0; m < MT; ++m) acc[t][m] = gq_f4{0.f, 0.f, 0.f, 0.f};
   const uint32_t mg = gq_nib_magic();
   auto compute = [&](int group, int st) __attribute__((always_inline)) {
 #pragma unroll
     for (int p = 0; p < G; ++p)
 #pragma unroll
-      for (int t = 0; t < T; ++t) rows_add<FMT, 1>(us[st][t][p], G * group + p, g, mg, xs[st][p], acc[t]);
+      for (int t = 0; t < T; ++t) rows_add<FMT, MT>(us[st][t][p], G * group + p, g, mg, xs[st][p], acc[t]);
   };
   walk_units<PD, KS>(units / G, wave, request, compute);
 #pragma unroll
-  for (int t = 0; t < T; ++t) red[wave][t][lane] = acc[t][0];
+  for (int t = 0; t < T; ++t)
+#pragma unroll
+    for (int m = 0; m < MT; ++m) red[wave][t][m][lane] = acc[t][m];
   __syncthreads();
   for (int o = threadIdx.x; o < 16 * R * blk.count; o += 64 * KS) {
     const int nl = o % (16 * R), m = o / (16 * R), n = 16 * R * (int)blockIdx.x + nl, q = blk.pair[m];
     if (n >= N) continue;
     h[(size_t)q * N + n] = moe_gu_h<KS, R>(
         [&](int k, int w, int t, int nn, int mm) {
-          return reinterpret_cast<const float *>(&red[k][w * R + t][16 * (mm >> 2) + nn])[mm & 3];
+          return reinterpret_cast<const float *>(&red[k][w * R + t][mm >> 4][4 * (mm & 12) + nn])[mm & 3];
         },
         nl, m, rs[q / top], act);
   }
@@ -714,7 +727,7 @@ k_moe_down_few(const uint8_t *__restrict__ wd, size_t sc_off, const _Float16 *__
 // More tokens: a block's rows are its pairs (fp16 rows of h with a power-of-two scale each); a block's sums go, with the
 // scale's inverse and the expert's weight, to the wave's own sums of the tokens in LDS.  gridDim.y parts of the blocks: their sums go to part
 // [part][M][K] in fp32, which k_moe_sum adds.
-template <int FMT, int R, int KS, int PD>
+template <int FMT, int MT, int R, int KS, int PD>
 __global__ void __launch_bounds__(64 * KS)
 k_moe_down_rows(const uint8_t *__restrict__ wd, size_t sc_off, const _Float16 *__restrict__ h16, int ldh, const float *__restrict__ hs,
                 MoePlan p, const void *resid, void *y, int dt, float *__restrict__ part, int M, int K, int C, int units, int top, int maxblk) {
@@ -722,8 +735,8 @@ k_moe_down_rows(const uint8_t *__restrict__ wd, size_t sc_off, const _Float16 *_
   const int P = M * top;
   float *sum_s = lds;                                                    // [KS][M][16 R]
   float *f_s = sum_s + KS * M * 16 * R;                                    // [P]: weight and scale of a pair
-  uint16_t *p_s = reinterpret_cast<uint16_t *>(f_s + P);                 // [maxblk][16]: pairs, 0xFFFF none
-  uint16_t *e_s = p_s + 16 * maxblk;                                     // [maxblk]
+  uint16_t *p_s = reinterpret_cast<uint16_t *>(f_s + P);                 // [maxblk][16 MT]: pairs, 0xFFFF none
+  uint16_t *e_s = p_s + 16 * MT * maxblk;                                     // [maxblk]
   uint8_t *t_s = reinterpret_cast<uint8_t *>(e_s + maxblk);              // [P]: token of a pair
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int g = lane >> 4, r = lane & 15, ntiles = K / 16;
@@ -734,17 +747,18 @@ k_moe_down_rows(const uint8_t *__restrict__ wd, size_t sc_off, const _Float16 *_
     f_s[i] = p.wsum[i] * hs[i];
     t_s[i] = (uint8_t)(i / top);
   }
-  for (int i = tid; i < 16 * maxblk; i += 64 * KS) {
-    const MoeBlk &b = p.blk[i >> 4];
-    p_s[i] = (i & 15) < b.count ? (uint16_t)b.pair[i & 15] : (uint16_t)0xFFFF;
-    if ((i & 15) == 0) e_s[i >> 4] = (uint16_t)b.expert;
+  for (int i = tid; i < 16 * MT * maxblk; i += 64 * KS) {
+    const int at = i % (16 * MT);
+    const MoeBlk &b = p.blk[i / (16 * MT)];
+    p_s[i] = at < b.count ? (uint16_t)b.pair[at] : (uint16_t)0xFFFF;
+    if (at == 0) e_s[i / (16 * MT)] = (uint16_t)b.expert;
   }
   __syncthreads();
   const __amdgpu_buffer_rsrc_t xr = __builtin_amdgcn_make_buffer_rsrc(
       const_cast<_Float16 *>(h16), (short)0, (int)(2u * (uint32_t)P * (uint32_t)ldh), 0x00020000);
   constexpr int G = kGroup<FMT>;
   FUnit<FMT> us[PD][R][G];
-  gq_half8 xs[PD][G][1][4];
+  gq_half8 xs[PD][G][MT][4];
   auto request = [&](const ItemAt &at, int st) __attribute__((always_inline)) {
     const bool on = at.b < nblk;
     const int b = on ? at.b : b0;
@@ -754,31 +768,40 @@ k_moe_down_rows(const uint8_t *__restrict__ wd, size_t sc_off, const _Float16 *_
       const int tile = (int)blockIdx.x * R + t;  // (clamped: not stored)
       load_group<FMT>(ftile<FMT>(wd, sc_off, tile0 + (size_t)min(tile, ntiles - 1), on ? C : 0), at.u, lane, us[st][t]);
     }
-    const uint32_t q = p_s[16 * b + r];
-    const uint32_t o = on && q != 0xFFFFu ? 2u * (q * (uint32_t)ldh + 16u * (uint32_t)g) + 256u * G * (uint32_t)at.u : 0xFFFFFC00u;
 #pragma unroll
-    for (int i = 0; i < 4 * G; ++i) {
-      const auto v = __builtin_amdgcn_raw_buffer_load_b128(xr, o + 128u * (i >> 1) + 16u * (i & 1), 0, 0);
-      xs[st][i >> 2][0][i & 3] = __builtin_bit_cast(gq_half8, gq_u4{v[0], v[1], v[2], v[3]});
+    for (int t = 0; t < MT; ++t) {
+      const uint32_t q = p_s[16 * (MT * b + t) + r];
+      const uint32_t o = on && q != 0xFFFFu ? 2u * (q * (uint32_t)ldh + 16u * (uint32_t)g) + 256u * G * (uint32_t)at.u : 0xFFFFFC00u;
+#pragma unroll
+      for (int i = 0; i < 4 * G; ++i) {
+        const auto v = __builtin_amdgcn_raw_buffer_load_b128(xr, o + 128u * (i >> 1) + 16u * (i & 1), 0, 0);
+        xs[st][i >> 2][t][i & 3] = __builtin_bit_cast(gq_half8, gq_u4{v[0], v[1], v[2], v[3]});
+      }
     }
   };
-  gq_f4 acc[R][1];
+  gq_f4 acc[R][MT];
 #pragma unroll
-  for (int t = 0; t < R; ++t) acc[t][0] = gq_f4{0.f, 0.f, 0.f, 0.f};
+  for (int t = 0; t < R; ++t)
+#pragma unroll
+    for (int m = 0; m < MT; ++m) acc[t][m] = gq_f4{0.f, 0.f, 0.f, 0.f};
   const uint32_t mg = gq_nib_magic();
   int cur = -1;
   auto flush = [&]() __attribute__((always_inline)) {
     if (cur < 0) return;
 #pragma unroll
-    for (int v = 0; v < 4; ++v) {
-      const uint32_t q = p_s[16 * cur + 4 * g + v];
-      if (q == 0xFFFFu) continue;
-      float *s = sum_s + (wave * M + t_s[q]) * (16 * R) + r;  // (a block's tokens differ)
+    for (int m = 0; m < MT; ++m)
 #pragma unroll
-      for (int t = 0; t < R; ++t) s[16 * t] += f_s[q] * acc[t][0][v];
-    }
+      for (int v = 0; v < 4; ++v) {
+        const uint32_t q = p_s[16 * (MT * cur + m) + 4 * g + v];
+        if (q == 0xFFFFu) continue;
+        float *s = sum_s + (wave * M + t_s[q]) * (16 * R) + r;  // (a block's tokens differ)
 #pragma unroll
-    for (int t = 0; t < R; ++t) acc[t][0] = gq_f4{0.f, 0.f, 0.f, 0.f};
+        for (int t = 0; t < R; ++t) s[16 * t] += f_s[q] * acc[t][m][v];
+      }
+#pragma unroll
+    for (int t = 0; t < R; ++t)
+#pragma unroll
+      for (int m = 0; m < MT; ++m) acc[t][m] = gq_f4{0.f, 0.f, 0.f, 0.f};
   };
   auto compute = [&](const ItemAt &at, int st) __attribute__((always_inline)) {
     if (at.b != cur) {
@@ -788,7 +811,7 @@ k_moe_down_rows(const uint8_t *__restrict__ wd, size_t sc_off, const _Float16 *_
 #pragma unroll
     for (int p = 0; p < G; ++p)
 #pragma unroll
-      for (int t = 0; t < R; ++t) rows_add<FMT, 1>(us[st][t][p], G * at.u + p, g, mg, xs[st][p], acc[t]);
+      for (int t = 0; t < R; ++t) rows_add<FMT, MT>(us[st][t][p], G * at.u + p, g, mg, xs[st][p], acc[t]);
   };
   const int groups = units / G;
   ItemAt rq = {b0, 0};
@@ -856,10 +879,15 @@ bool moe_few(const gq_moe &l, size_t M) {
   const size_t P = M * (size_t)l.top_k, nk = (gq_kpad(l.fmt, l.K) + 127) & ~(size_t)127, nn = (gq_kpad(l.fmt_down, l.N) + 127) & ~(size_t)127;
   return M <= (size_t)kMoeFew && few_lds_bytes(M, nk) <= (160 - 34) * 1024 && few_lds_bytes(P, nn) + P * nn / 8 <= (160 - 20) * 1024;
 }
+// Row tiles of a block: two where an expert has 16 tokens and more if all are taken alike, so that its weights are read and converted for up to 32 of
+// them (us the layer by one / two tiles, Q4_K with Q6_K and Q8_0 with Q4_0: 64 tokens, 2 of 8 of 14336 x 4096, 295 / 279 and 311 / 271; 20 tokens, 4 of 4
+// of 4096 x 4096, 80 / 68 and 83 / 67; with fewer the second tile's loads and products are for nothing: 48 tokens, 2 of 8 of 14336 x 4096, 231 / 271 and 242 / 256;
+// four tiles: 366 - 462 of the first, 212 and 176 of 43 tokens, 4 of 4 of 9984 x 3328, that two do in 189 and 207).
+int moe_tiles(const gq_moe &l, size_t M) { return M * (size_t)l.top_k >= 16 * l.n_experts ? 2 : 1; }
 // Where a call's intermediate values lie in its workspace
 struct MoeWs {
   size_t logits, ids, weights, count, nblk, blk, wsum, a16, rs, h, h16, hs, part, bytes;
-  int maxblk, parts;
+  int maxblk, parts, tiles;
 };
 MoeWs moe_ws(const gq_moe &l, size_t M) {
   MoeWs w;
@@ -872,13 +900,15 @@ MoeWs moe_ws(const gq_moe &l, size_t M) {
   const size_t P = M * (size_t)l.top_k;
   const bool few = moe_few(l, M);
   // (an expert's last block may be short: at most a block an expert beyond whole ones)
-  w.maxblk = (int)(few ? std::min(P, l.n_experts) : std::min(P, l.n_experts + P / 16));
+  w.tiles = few ? 1 : moe_tiles(l, M);
+  const size_t blocks = few ? std::min(P, l.n_experts) : std::min(P, l.n_experts + P / 16);  // (of one tile: the bytes grow with the tokens)
+  w.maxblk = (int)(w.tiles == 1 ? blocks : std::min(P, l.n_experts + P / 32));
   w.logits = take(M * l.n_experts * 8);
   w.ids = take(P * 4);
   w.weights = take(P * 4);
   w.count = take(4);
   w.nblk = take(4);
-  w.blk = take((size_t)w.maxblk * sizeof(MoeBlk));
+  w.blk = take(blocks * sizeof(MoeBlk));
   w.wsum = take(P * 4);
   w.a16 = take(M * (gq_kpad(l.fmt, l.K) + 8) * 2);
   w.rs = take((M + 256) * 4);
@@ -887,7 +917,7 @@ MoeWs moe_ws(const gq_moe &l, size_t M) {
   w.hs = take(few ? P * ((l.N + 127) / 128) * 16 : (P + 256) * 4);
   // W_down's row tiles, two a workgroup, in parts as far as a workgroup a CU goes (64 tokens, 128 experts of 768 x 2048, in 2 / 3 / 4
   // parts: 147 / 127 / 117 us the layer; 37 tokens, 61 of 1376 x 2080, whose four are more than that, 100 / 92 / 98)
-  w.parts = few ? 1 : (int)std::min(std::max((size_t)1, 256 / ((l.K + 31) / 32)), std::min((size_t)8, (size_t)w.maxblk));
+  w.parts = few ? 1 : (int)std::min(std::max((size_t)1, 256 / ((l.K + 31) / 32)), std::min((size_t)8, blocks));
   w.part = take(w.parts > 1 ? w.parts * M * l.K * 4 : 0);
   w.bytes = at;
   return w;
@@ -981,9 +1011,13 @@ int launch_gu_t(const gq_moe &l, const void *x, int xt, const float *rs, const R
   const int N = (int)l.N, K = (int)l.K, units = (int)(gq_kpad(FMT, K) / 128), tiles = N / 16;
   // (16 tokens, 8 experts of 14336 x 4096, Q4_0, by one tile 190 us the layer, by two 167; 64 tokens, 128 experts of 768 x 2048, 143 and 128)
   constexpr int R = 2, KS = 4;
-  hipLaunchKernelGGL((k_moe_gu_rows<FMT, R, KS, group_stages<FMT>(2)>), dim3((unsigned)((tiles + R - 1) / R), (unsigned)p.maxblk), dim3(64 * KS), 0, s,
-                     (const uint8_t *)l.gate, (const uint8_t *)l.up, gq_sc_plane_offset(FMT, l.n_experts * l.N, K), b.a16, b.lda, rs, p,
-                     b.h, M, N, (int)gq_chunks(FMT, K), units, l.act, l.top_k);
+#define GQ_GU_ROWS(MT)                                                                                                                      \
+  hipLaunchKernelGGL((k_moe_gu_rows<FMT, MT, R, KS, group_stages<FMT>(2)>), dim3((unsigned)((tiles + R - 1) / R), (unsigned)p.maxblk), dim3(64 * KS), 0, s, \
+                     (const uint8_t *)l.gate, (const uint8_t *)l.up, gq_sc_plane_offset(FMT, l.n_experts * l.N, K), b.a16, b.lda, rs, p,    \
+                     b.h, M, N, (int)gq_chunks(FMT, K), units, l.act, l.top_k)
+  if (p.sh == 4) GQ_GU_ROWS(1);
+  else GQ_GU_ROWS(2);
+#undef GQ_GU_ROWS
   return gq_last_launch();
 }
 template <int FMT>
@@ -1005,10 +1039,14 @@ int launch_down_t(const gq_moe &l, const int *ids, const float *weights, const M
   // Two tiles a workgroup, which share the rows of h: four of six loads a unit.  (16 tokens, 8 experts of 14336 x 4096, Q4_0, by one tile 167 us
   // the layer, by two in two parts 152, by four in four parts 147 - 149; 64 tokens, 128 experts of 768 x 2048, 127, 117 and 139 - 159.)
   constexpr int R = 2, KS = 8;
-  const size_t P = (size_t)M * l.top_k, lds = (size_t)KS * M * 64 * R + P * 4 + (size_t)p.maxblk * 34 + P + 16;
-  hipLaunchKernelGGL((k_moe_down_rows<FMT, R, KS, group_stages<FMT>(2)>), dim3((tiles + R - 1) / R, (unsigned)b.parts), dim3(64 * KS), lds, s,
-                     (const uint8_t *)l.down, so, b.h16, b.ldh, b.hs, p, resid, y, dt, b.parts > 1 ? b.part : nullptr, M, K, C, units,
-                     l.top_k, p.maxblk);
+  const size_t P = (size_t)M * l.top_k, lds = (size_t)KS * M * 64 * R + P * 4 + (size_t)p.maxblk * ((2u << p.sh) + 2) + P + 16;
+#define GQ_DOWN_ROWS(MT)                                                                                                                   \
+  hipLaunchKernelGGL((k_moe_down_rows<FMT, MT, R, KS, group_stages<FMT>(2)>), dim3((tiles + R - 1) / R, (unsigned)b.parts), dim3(64 * KS), lds, s, \
+                     (const uint8_t *)l.down, so, b.h16, b.ldh, b.hs, p, resid, y, dt, b.parts > 1 ? b.part : nullptr, M, K, C, units,      \
+                     l.top_k, p.maxblk)
+  if (p.sh == 4) GQ_DOWN_ROWS(1);
+  else GQ_DOWN_ROWS(2);
+#undef GQ_DOWN_ROWS
   return gq_last_launch();
 }
 
@@ -1064,7 +1102,7 @@ struct MoeRoom {
   }
 };
 MoePlan plan_of(const MoeWs &w, uint8_t *ws) {
-  return MoePlan{(int *)(ws + w.nblk), (MoeBlk *)(ws + w.blk), (float *)(ws + w.wsum), w.maxblk, (int *)(ws + w.count)};
+  return MoePlan{(int *)(ws + w.nblk), (MoeBlk *)(ws + w.blk), (float *)(ws + w.wsum), w.maxblk, w.tiles == 1 ? 4 : 5, (int *)(ws + w.count)};
 }
 
 }  // namespace
