@@ -611,3 +611,37 @@ def test_no_expert_at_all(dev, m):
     resid = torch.randn(m, 256, generator=la.gen).to(torch.bfloat16).to(dev)
     assert bool((products(la, x, ids, w) == 0).all())
     assert torch.equal(products(la, x, ids, w, resid=resid), resid)
+
+
+@pytest.mark.parametrize("m,e,top", [(64, 1024, 16), (64, 16, 16), (4, 1024, 16)])
+def test_the_most(dev, m, e, top):
+    """As many tokens, experts and experts a token as a call takes."""
+    la = Layer(dev, O.Q4_0, O.Q8_0, e, 32, 64, seed=26)
+    la.router *= 1 / la.size
+    x = la.x(m, torch.float16)
+    y, ids, w = run(la, x, top, save=True)
+    rid, rw = choose(x, la.router, top, 0, True, 1.0, None)
+    assert torch.equal(ids.long(), rid)
+    check(la, x, rid, rw, 0, None, y)
+
+
+@pytest.mark.parametrize("m", [2, 7, 40])
+def test_half_of_the_choice_wanted(dev, m):
+    """ids or weights alone, through the C entry point; y in place of the residual."""
+    import ctypes
+
+    import gq
+    la, lib = Layer(dev, O.Q8_0, O.Q8_0, 9, 64, 96, seed=27), gq.load()
+    la.router *= 1 / la.size
+    x = la.x(m, torch.bfloat16)
+    resid = torch.randn(m, 96, generator=la.gen).to(torch.bfloat16).to(dev)
+    y, ids, w = run(la, x, 3, resid=resid, save=True)
+    layer = gq.MoeLayer(la.fmt, la.fmt_down, 0, 3, *(p.data_ptr() for p in la.packed), 9, 64, 96, la.router.data_ptr(), None, gq.DT_F32, 0, 1, 1.0)
+    for ids2, w2 in ((torch.empty_like(ids), None), (None, torch.empty_like(w)), (None, None)):
+        out = resid.clone()
+        st = lib.gq_moe_layer(ctypes.addressof(layer), x.data_ptr(), gq.DT_BF16, out.data_ptr(), out.data_ptr(), gq.DT_BF16,
+                              ids2.data_ptr() if ids2 is not None else None, w2.data_ptr() if w2 is not None else None, m, None, 0,
+                              torch.cuda.current_stream().cuda_stream)
+        assert st == 0 and torch.equal(out, y)
+        assert ids2 is None or torch.equal(ids2, ids)
+        assert w2 is None or torch.equal(w2, w)
