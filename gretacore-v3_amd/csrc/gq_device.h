@@ -36,6 +36,14 @@ GQ_DEV float gq_scale_h2f(uint32_t h16) { return gq_h2f(h16); }
 GQ_DEV uint32_t gq_h2_bits(gq_half2 v) { return __builtin_bit_cast(uint32_t, v); }
 GQ_DEV gq_half2 gq_bits_h2(uint32_t v) { return __builtin_bit_cast(gq_half2, v); }
 
+GQ_DEV float gq_pow2(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }  // (-126 <= e <= 127)
+// The power of two under which values go to fp16: s = 14 - floor(log2(top)) of their largest magnitude (no NaN), which
+// lands in [2^14, 2^15) whatever its size, so that no finite value overflows.  -114 (an Inf) to 126 (zeros too): 2^s and 2^-s are normal.
+GQ_DEV int gq_fp16_shift(float top) {
+  const int sh = 14 + 127 - (int)((__float_as_uint(top) >> 23) & 0xFFu);
+  return sh > 126 ? 126 : sh;
+}
+
 // 4-bit codes straight to fp16: OR-ing a code into the low mantissa bits of
 // 1024.0 (0x6400) gives 1024 + q.  Of a code-group word (slots 0..3 in the
 // low nibbles of bytes 0..3, slots 4..7 in the high nibbles) four and-or ops

@@ -324,9 +324,8 @@ k_front_rows_px(const uint8_t *__restrict__ wg, const uint8_t *__restrict__ wu, 
         }
       top = fmaxf(top, __shfl_xor(top, 16, 64));
       top = fmaxf(top, __shfl_xor(top, 32, 64));
-      // 2^s, s = 14 - floor(log2(top)) at most 126 (at least -114: both have a normal inverse)
-      const int sh = 14 + 127 - (int)((__float_as_uint(top) >> 23) & 0xFFu), cut = sh > 126 ? 126 : sh;
-      const float f2 = __uint_as_float((uint32_t)(127 + cut) << 23), inv = __uint_as_float((uint32_t)(127 - cut) << 23);
+      const int sh = gq_fp16_shift(top);
+      const float f2 = gq_pow2(sh), inv = gq_pow2(-sh);
 #pragma unroll
       for (int v = 0; v < 4; ++v) back[t][v] = __shfl(inv, 4 * g + v, 64);
 #pragma unroll
@@ -631,9 +630,9 @@ __global__ void __launch_bounds__(kDguThreads) k_front_dgu(const void *dh, const
     __syncthreads();
 #pragma unroll
     for (int w = 0; w < kDguThreads / 64; ++w) top = fmaxf(top, top_s[w]);
-    const int sh = 14 + 127 - (int)((__float_as_uint(top) >> 23) & 0xFFu), cut = sh > 126 ? 126 : sh;
-    f2 = __uint_as_float((uint32_t)(127 + cut) << 23);
-    if (tid == 0) rs[blockIdx.x] = __uint_as_float((uint32_t)(127 - cut) << 23);
+    const int sh = gq_fp16_shift(top);
+    f2 = gq_pow2(sh);
+    if (tid == 0) rs[blockIdx.x] = gq_pow2(-sh);
   }
   auto put16 = [&](int k, const float (&a)[8], const float (&b)[8]) __attribute__((always_inline)) {
     if (!a16 || k >= np) return;

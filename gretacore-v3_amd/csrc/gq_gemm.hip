@@ -833,14 +833,6 @@ GQ_DEV void win_max(float (&m)[NR], int n) {
     for (int r = 0; r < NR; ++r)
       if (r < n) m[r] = fmaxf(m[r], __shfl_xor(m[r], o, 64));
 }
-// s = 14 - floor(log2(amax)) from the exponent field (0 for a zero row, Inf / NaN;
-// clamped so 2^s and 2^-s stay normal floats)
-template <bool WIN>
-GQ_DEV int row_shift(float amax) {
-  const uint32_t eb = (__float_as_uint(amax) >> 23) & 0xFFu;
-  const int sh = (!WIN && eb == 0u) || eb == 0xFFu ? 0 : 14 - ((int)eb - 127);
-  return sh < -100 ? -100 : sh > 100 ? 100 : sh;
-}
 // WIN: a window of 256 k whose largest magnitude is more than 2^20 below the row's is scaled
 // up by 2^t more, t to wsh[window][row] (rows padded to 4), and such a row's rs is negative; the GEMM
 // undoes t around the window.  In any other window an entry down to 2^-9 of its
@@ -848,10 +840,9 @@ GQ_DEV int row_shift(float amax) {
 // (Q6_K with K > 4096 and fp16 weights, whose few-row kernel scales by window.)
 GQ_DEV int win_shift(float amax, float wmax, int sh) {
   const int t = (int)(__float_as_uint(amax) >> 23) - (int)(__float_as_uint(wmax) >> 23);
-  const int top = 100 - sh < 64 ? 100 - sh : 64;
+  const int top = 126 - sh < 64 ? 126 - sh : 64;
   return wmax == 0.f || t <= 20 ? 0 : t < top ? t : top;
 }
-GQ_DEV float pow2f(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }
 
 template <int DT, int RUNS, bool WIN>
 __global__ void __launch_bounds__(kConvThreads) k_a_to_f16(const void *__restrict__ a, _Float16 *__restrict__ o,
@@ -911,14 +902,14 @@ __global__ void __launch_bounds__(kConvThreads) k_a_to_f16(const void *__restric
 #pragma unroll
     for (int w = 0; w < kConvThreads / 64; ++w) amin = fminf(amin, wmin[w]);
   }
-  const int sh = row_shift<WIN>(amax);
-  const float f = pow2f(sh);
-  if (tid == 0) rs[m] = WIN && win_shift(amax, amin, sh) > 0 ? -pow2f(-sh) : pow2f(-sh);
+  const int sh = gq_fp16_shift(amax);
+  const float f = gq_pow2(sh);
+  if (tid == 0) rs[m] = WIN && win_shift(amax, amin, sh) > 0 ? -gq_pow2(-sh) : gq_pow2(-sh);
   auto put = [&](const float(&x)[8], int k0, float wmax) {  // (wmax: of the run's window)
     float fw = f;
     if constexpr (WIN) {
       const int t = win_shift(amax, wmax, sh);
-      fw = pow2f(sh + t);
+      fw = gq_pow2(sh + t);
       if ((tid & 31) == 0) wsh[(size_t)(k0 >> 8) * ((gridDim.x + 3) & ~3u) + m] = (uint8_t)t;
     }
     *reinterpret_cast<gq_half8 *>(o + m * ldo + k0) = conv8(x, fw, q4perm);
@@ -979,9 +970,9 @@ __global__ void __launch_bounds__(256) k_a_to_f16_w(const void *__restrict__ a, 
     amax = fmaxf(amax, __shfl_xor(amax, o2, 64));
     if constexpr (WIN) amin = fminf(amin, __shfl_xor(amin, o2, 64));
   }
-  const int sh = row_shift<WIN>(amax);
-  const float f = pow2f(sh);
-  if (lane == 0) rs[m] = WIN && win_shift(amax, amin, sh) > 0 ? -pow2f(-sh) : pow2f(-sh);
+  const int sh = gq_fp16_shift(amax);
+  const float f = gq_pow2(sh);
+  if (lane == 0) rs[m] = WIN && win_shift(amax, amin, sh) > 0 ? -gq_pow2(-sh) : gq_pow2(-sh);
 #pragma unroll
   for (int r = 0; r < R; ++r) {
     const int k0 = 8 * (lane + 64 * r);
@@ -989,7 +980,7 @@ __global__ void __launch_bounds__(256) k_a_to_f16_w(const void *__restrict__ a, 
     float fw = f;
     if constexpr (WIN) {
       const int t = win_shift(amax, wm[r], sh);
-      fw = pow2f(sh + t);
+      fw = gq_pow2(sh + t);
       if ((lane & 31) == 0) wsh[(size_t)(k0 >> 8) * (((unsigned)M + 3) & ~3u) + m] = (uint8_t)t;
     }
     *reinterpret_cast<gq_half8 *>(o + m * ldo + k0) = conv8(v[r], fw, q4perm);

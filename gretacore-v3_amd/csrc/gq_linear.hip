@@ -322,9 +322,9 @@ __global__ void __launch_bounds__(kDzThreads) k_lin_dz(const void *dy, const voi
       __syncthreads();  // (two buffers: a row's maxima are read before the next row's barrier, the one after writes them)
 #pragma unroll
       for (int w = 0; w < kDzThreads / 64; ++w) top = fmaxf(top, top_s[buf][w]);
-      const int sh = 14 + 127 - (int)((__float_as_uint(top) >> 23) & 0xFFu), cut = sh > 126 ? 126 : sh;
-      f2 = __uint_as_float((uint32_t)(127 + cut) << 23);
-      if (tid == 0) rs[m] = __uint_as_float((uint32_t)(127 - cut) << 23);
+      const int sh = gq_fp16_shift(top);
+      f2 = gq_pow2(sh);
+      if (tid == 0) rs[m] = gq_pow2(-sh);
     }
     auto put16 = [&](int k, const float (&a)[8]) __attribute__((always_inline)) {
       if (!a16 || k >= np) return;

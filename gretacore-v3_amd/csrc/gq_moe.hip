@@ -54,11 +54,9 @@ GQ_DEV void moe_convert(const void *x, const MoeConv &c, int m, int K, int lane)
   }
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
-  // s = 14 - floor(log2(top)) within +-100, 0 for a row of zeros or with an Inf
-  const int eb = (int)((__float_as_uint(top) >> 23) & 0xFFu);
-  const int sh = eb == 0 || eb == 0xFF ? 0 : min(max(14 + 127 - eb, -100), 100);
-  const float f = __uint_as_float((uint32_t)(127 + sh) << 23);
-  if (lane == 0) c.rs[m] = __uint_as_float((uint32_t)(127 - sh) << 23);
+  const int sh = gq_fp16_shift(top);
+  const float f = gq_pow2(sh);
+  if (lane == 0) c.rs[m] = gq_pow2(-sh);
   for (int k = 8 * lane; k < c.lda; k += 512) {
     FRaw<XT> r;
     float v[8];
@@ -476,14 +474,13 @@ k_moe_gu_few(const uint8_t *__restrict__ wg, const uint8_t *__restrict__ wu, siz
   float t = fabsf(v);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) t = fmaxf(t, __shfl_xor(t, o, 32));
-  // 2^s, s = 14 - floor(log2(t)) at most 126 (at least -114: both have a normal inverse)
-  const int sh = 14 + 127 - (int)((__float_as_uint(t) >> 23) & 0xFFu), cut = sh > 126 ? 126 : sh;
+  const int sh = gq_fp16_shift(t);
   const int e = nl & 7, to = nib ? (e & 1 ? 4 + (e >> 1) : e >> 1) : e;
-  h[(size_t)q * N + n0 + (nl & 24) + to] = (_Float16)(v * __uint_as_float((uint32_t)(127 + cut) << 23));
+  h[(size_t)q * N + n0 + (nl & 24) + to] = (_Float16)(v * gq_pow2(sh));
   if (nl == 0) {
     const int c = (n0 >> 5) & 3;
     float *o = hs + ((size_t)q * ((N + 127) / 128) + (n0 >> 7)) * 4;
-    o[2 * (c & 1) + (c >> 1)] = __uint_as_float((uint32_t)(127 - cut) << 23);
+    o[2 * (c & 1) + (c >> 1)] = gq_pow2(-sh);
     if (n0 + 32 == N)
       for (int d = c + 1; d < 4; ++d) o[2 * (d & 1) + (d >> 1)] = 0.f;  // (blocks behind the row)
   }
