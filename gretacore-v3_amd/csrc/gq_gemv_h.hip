@@ -39,12 +39,12 @@ GQ_DEV uint32_t max_half_wave(uint32_t v) {
 
 // Activation range: each batch row's 256-k window (32 runs of 8, one per
 // lane of a 32-lane half) is converted to fp16 after scaling by 2^s, s = 14 -
-// floor(log2(max |x|)) over the window, clamped to [-100, 100] so both 2^s and
+// floor(log2(max |x|)) over the window, from -114 up to 126, so both 2^s and
 // 2^-s are normal floats: the window's largest entry lands in [2^14, 2^15),
 // so no entry overflows fp16 and entries down to 2^-24 of the largest stay
 // normal (also after the 1/16 of the 4-bit formats' high-nibble slots).  An
-// all-zero window gets 2^100 (zeros stay zeros), one holding Inf or NaN
-// 2^-100 (they stay Inf / NaN).  The window's dot products are multiplied by
+// all-zero window gets 2^126 (zeros stay zeros), one holding Inf or NaN
+// 2^-114 (they stay Inf / NaN).  The window's dot products are multiplied by
 // 2^-s (exact) as they are added to the fp32 accumulator.  `in` false: the
 // run is outside the data (its values do not count).  Returns 2^s; *unscale
 // receives 2^-s.
@@ -55,8 +55,8 @@ GQ_DEV float window_scale(const float (&xv)[8], bool in, float *unscale) {
 #pragma unroll
   for (int e = 0; e < 8; ++e) am = fmaxf(am, fabsf(xv[e]));
   const uint32_t eb = max_half_wave(in ? __float_as_uint(am) : 0u) >> 23;
-  // biased exponent of 2^s: 127 + 14 - (eb - 127), clamped to 127 +- 100
-  const uint32_t fe = (uint32_t)min(max(268 - (int)eb, 27), 227);
+  // biased exponent of 2^s: 127 + 14 - (eb - 127)
+  const uint32_t fe = (uint32_t)min(268 - (int)eb, 253);
   *unscale = __uint_as_float((254u - fe) << 23);
   return __uint_as_float(fe << 23);
 }

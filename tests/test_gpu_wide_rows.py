@@ -77,6 +77,29 @@ def test_windows_of_one_row(dev):
     close(c, gq.matmul(O.Q6_K, c.packed, c.x, n, k))
 
 
+# (1, 2 to 8, 9 to 16 rows; K short, of several parts, and more than a workgroup stages at once)
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("m", [1, 2, 8, 13, 16])
+@pytest.mark.parametrize("n,k", [(100, 512), (4096, 4608), (272, 14336)])
+def test_gemv(dev, fmt, m, n, k):
+    import gq
+    c = wide(dev, fmt, m, n, k, torch.float32)
+    close(c, gq.gemv(fmt, c.packed, c.x, n, k, workspace=gq.Workspace(dev)))
+    close(c, gq.matmul(fmt, c.packed, c.x, n, k))
+    for y in gq.gemv_multi(fmt, [(c.packed, n), (c.packed, n)], c.x, k) if m <= 4 else ():  # (which takes no more)
+        close(c, y)
+
+
+@pytest.mark.parametrize("m", [1, 2, 8, 16, 40, 200])
+@pytest.mark.parametrize("n,k", [(100, 512), (272, 4608)])
+def test_fp16_weights(dev, m, n, k):
+    import gq
+    c = wide(dev, O.Q8_0, m, n, k, torch.float32)
+    w = c.w.to(torch.float16)
+    c.w = w.double()
+    close(c, gq.gemm_f16w(w, c.x, n, k))
+
+
 @pytest.mark.parametrize("fmt,down", [(O.Q4_0, O.Q8_0), (O.Q8_0, O.Q4_K), (O.Q4_K, O.Q6_K), (O.Q6_K, O.Q4_0)])
 @pytest.mark.parametrize("m", [1, 4, 5, 64])
 @pytest.mark.parametrize("size", [60, 58, 56])
