@@ -905,11 +905,12 @@ def moe_ffn(fmt: int, gate, up, fmt_down: int, down, x, ids, weights, n: int, k:
     if stream is not None:
         return _on(stream, moe_ffn, fmt, gate, up, fmt_down, down, x, ids, weights, n, k, n_experts, act, resid, y, out_dtype,
                    workspace)
+    if ids is None or weights is None or ids.dim() != 2:
+        raise GQError("ids and weights: [m][top_k] expected")
     m, device = _rows(x, k, "x")
-    if ids.dim() != 2:
-        raise GQError("ids: [m][top_k] expected")
     top_k = ids.shape[1]
-    ids, weights = _choice(ids, weights, m, top_k, x, device)
+    _operand(ids, (m, top_k), "ids", device, _i32)
+    _operand(weights, (m, top_k), "weights", device, _f32)
     return _moe_call(False, fmt, gate, up, fmt_down, down, None, x, n, k, n_experts, top_k, act, 0, False, 1.0, None, resid, y, ids,
                      weights, out_dtype, workspace, m, device)
 
