@@ -789,7 +789,7 @@ def linear(fmt: int, w, x, n: int, k: int, bias=None, act: int = ACT_NONE, resid
     elif save:
         z = y.new_empty(m, n)
     ws_ptr, ws_n = None, 0
-    # (one to four rows of 16-bit x need none)
+    # (one to four rows of 16-bit x, up to 65536 values of them, need none)
     if workspace is not None and (m > 4 or m * (k + 255) > 65536 or x.dtype == _f32):
         ws_ptr, ws_n = _room(workspace, _linear_bytes(False, fmt, m, n, k), device)
     st = load().gq_linear(fmt, w.data_ptr(), x.data_ptr(), _dt(x.dtype), _ptr(bias), bias_dt, act, _ptr(resid), y.data_ptr(),

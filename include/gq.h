@@ -330,9 +330,10 @@ int gq_w4_gate_up(const void *d_gate, const void *d_up, int group, const void *d
  * wanted; gq_linear_bwd takes it).  resid may be y itself; y and z overlap nothing else.
  * Sums are fp32, bias, activation and residual are applied to them in fp32, and
  * y and z are rounded once.  x and the weights enter the matrix cores as in gq_ffn_gate_up: one to four rows
- * of 16-bit x as they are (of bf16 rows the finite values stay below 2^115), all others rounded to fp16
+ * of 16-bit x, up to 65536 values together with K in whole 128s (k-quants 256s), as they are, the scales in fp32: 2e-5 of a product's
+ * row, bf16 2e-6 (of bf16 rows the finite values stay below 2^115); one to four longer rows as the next.  All others are rounded to fp16
  * after a power-of-two scale per row (fp16 rows of whole 128s, 16-byte aligned, with Q8_0 or Q6_K weights: as they are); up to
- * 16 rows keep the k-quants' d (and dmin) in fp32, more fold them into fp16 weights. */
+ * 16 rows keep the k-quants' d (and dmin) in fp32 and round Q4_0 and Q8_0 weights to fp16, 2e-4; more fold them into fp16 weights. */
 #define GQ_ACT_NONE 2 /* z */
 #define GQ_ACT_RELU 3 /* max(z, 0); beside these GQ_ACT_SILU and GQ_ACT_GELU_TANH */
 /* A workspace of NULL takes scratch memory of the call's own, as in gq_ffn_gate_up; calls that need none (one to four rows of 16-bit
@@ -385,9 +386,10 @@ int gq_moe_route(const gq_moe *layer, const void *d_x, int x_dtype, int32_t *d_i
 /* The experts' products for a given choice (the router is not read): ids outside 0 .. n_experts - 1 name no expert (one
  * that another device holds, an empty slot), an expert named twice counts with both weights.  x is [M][K] of
  * x_dtype, y and resid (NULL: none; it may be y) [M][K] of y_dtype, all contiguous.  Sums, h and the weighted sum are
- * fp32, y is rounded once; x and h enter the matrix cores in fp16 after a power-of-two scale per row (one to
- * four tokens: x of 16 bits as it is, of bf16 the finite values below 2^115, and h with a scale per 32 values), weights as in
- * gq_ffn_gate_up's kernels of few rows.  y and resid overlap nothing else. */
+ * fp32, y is rounded once; x and h enter the matrix cores in fp16 after a power-of-two scale per row, weights
+ * as in gq_linear up to 16 rows.  One to four tokens whose rows of x are up to 64000 values together and whose rows of h (top_k a token) up to
+ * 66000, K and N in whole 128s or 256s (two tokens, two experts each, of N = 14336; not three): x of 16 bits as it is, of bf16 the finite values
+ * below 2^115, h with a scale per 32 values, weights' scales in fp32.  y and resid overlap nothing else. */
 int gq_moe_ffn(const gq_moe *layer, const void *d_x, int x_dtype, const int32_t *d_ids, const float *d_weights,
                const void *d_resid, void *d_y, int y_dtype, size_t M, void *d_workspace, size_t workspace_bytes,
                void *stream);

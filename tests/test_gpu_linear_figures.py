@@ -1,14 +1,16 @@
 """The product with its epilogue held to the figures that its documentation gives, path by path.
 
 Tolerances.  An activation z s(p): the sigmoid's argument is off by five and a half half steps of fp32, 3.3e-7 |p| of s, its exponential,
-reciprocal and products by six, 3.6e-7; results below fp32's range are flushed, 1e-30."""
+reciprocal and products by six, 3.6e-7; results below fp32's range are flushed, 1e-30.  Products: figures."""
 import math
 
 import pytest
 import torch
 
+import figures
 import oracle as O
 from linear_ref import act_grad
+from test_gpu_linear import DTYPES, Case
 
 pytestmark = pytest.mark.gpu
 
@@ -37,3 +39,31 @@ def test_both_sides_of_an_activation(dev, act, m):
     rel = 4e-7 * p.abs().clamp(max=100) + 1e-6
     assert bool(((y.double() - f).abs() <= rel * f.abs() + 1e-30).all())
     assert bool(((dz.double() - d).abs() <= rel * (s + (t * dp).abs() * s * torch.sigmoid(-p)) + 2 ** -24 * (t * dp).abs() * s + 1e-30).all())
+
+
+# rows that are few and fit LDS together, the last that do and the first that do not, up to 16, tiles
+@pytest.mark.parametrize("fmt", [O.Q4_0, O.Q8_0, O.Q4_K, O.Q6_K])
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("m,k", [(1, 512), (1, 14336), (1, 65536), (1, 65792), (2, 4096), (2, 32768), (3, 21760), (3, 22016), (4, 1024), (4, 16384), (4, 16640),
+                                 (4, 20480), (5, 512), (11, 4096), (16, 14336), (17, 1024), (60, 4096), (200, 2048)])
+def test_products(dev, fmt, dtype, m, k):
+    import gq
+    n = 160
+    c = Case(dev, fmt, m, n, k, seed=k % 7, dtype=dtype, bias=False, resid=False)
+    y = gq.linear(fmt, c.packed, c.x, n, k, out_dtype=torch.float32)
+    err = (y.double() - figures.taken(c.x) @ c.w.t().contiguous()).norm(dim=1) / figures.terms(c.x, c.w)
+    print(f"share {float(err.max()):.3e} of {figures.linear(fmt, m, k, dtype):.3e}")
+    assert float(err.max()) <= figures.linear(fmt, m, k, dtype), float(err.max())
+
+
+@pytest.mark.parametrize("fmt", [O.Q4_0, O.Q8_0, O.Q4_K, O.Q6_K])
+@pytest.mark.parametrize("m,n,k", [(1, 256, 512), (8, 1000, 1024), (70, 513, 512), (300, 2048, 512)])
+def test_input_gradients(dev, fmt, m, n, k):
+    """dx: dz to fp16 and the weights as in the tiles."""
+    import gq
+    c = Case(dev, fmt, m, n, k, seed=n % 7, dtype=torch.float16)
+    dx = gq.linear_bwd(fmt, c.packed, c.dy, None, n, k, dx_dtype=torch.float32, want_dz=False)["dx"]
+    rows = c.dy.double().norm(dim=1) > 0
+    err = (dx.double() - figures.taken(c.dy.float()) @ c.w).norm(dim=1)[rows] / figures.terms(c.dy, c.w.t())[rows]
+    print(f"share {float(err.max()):.3e} of {figures.tiles(fmt):.3e}")
+    assert float(err.max()) <= figures.tiles(fmt), float(err.max())
