@@ -67,3 +67,60 @@ def test_input_gradients(dev, fmt, m, n, k):
     err = (dx.double() - figures.taken(c.dy.float()) @ c.w).norm(dim=1)[rows] / figures.terms(c.dy, c.w.t())[rows]
     print(f"share {float(err.max()):.3e} of {figures.tiles(fmt):.3e}")
     assert float(err.max()) <= figures.tiles(fmt), float(err.max())
+
+
+@pytest.mark.parametrize("fmt", [O.Q4_0, O.Q8_0, O.Q4_K, O.Q6_K])
+@pytest.mark.parametrize("m,k", [(1, 512), (4, 4096), (5, 512), (16, 4096), (40, 512), (300, 1024)])
+def test_subnormal_fp16_rows(dev, fmt, m, k):
+    """fp16 rows of subnormals alone, and of subnormals beside a 1 (2^14 x / 16, the 4-bit formats' smallest, is still normal), on the paths
+    that convert x and on those that take it as it is: no value is flushed."""
+    import gq
+    n = 160
+    c = Case(dev, fmt, m, n, k, seed=3, dtype=torch.float32, bias=False, resid=False)
+    x = c.x.double() / c.x.double().abs().max() * 2.0 ** -15
+    c.x = x.to(torch.float16)
+    assert float(c.x.abs().max()) < 2.0 ** -14 and int((c.x != 0).sum()) > 0.9 * c.x.numel()
+    for large in (False, True):
+        if large:
+            c.x[:, 3] = 1.0
+        y = gq.linear(fmt, c.packed, c.x, n, k, out_dtype=torch.float32)
+        ref = c.x.double() @ c.w.t().contiguous()
+        err = (y.double() - ref).norm(dim=1)
+        assert bool((err <= figures.linear(fmt, m, k, torch.float16) * figures.terms(c.x, c.w)).all())
+        if not large:
+            assert bool((ref.norm(dim=1) > 0).all())
+
+
+@pytest.mark.parametrize("fmt", [O.Q4_0, O.Q8_0, O.Q4_K, O.Q6_K])
+def test_the_same_again(dev, fmt):
+    """Two calls on the same inputs give the same bits, on every path and for every output."""
+    import gq
+    n, k = 1030, 4096
+    for m in (1, 3, 4, 9, 16, 40, 203, 509):
+        c = Case(dev, fmt, m, n, k, seed=m, dtype=torch.float16)
+        ws = gq.Workspace(dev)
+
+        def call():
+            y, z = gq.linear(fmt, c.packed, c.x, n, k, bias=c.bias, act=1, resid=c.resid, save=True, workspace=ws)
+            return y, z, *gq.linear_bwd(fmt, c.packed, c.dy, c.z, n, k, act=1, want_dbias=True, workspace=ws).values()
+
+        first = [t.clone() for t in call()]
+        for _ in range(3):
+            ws.ensure(1).fill_(0xFF)  # (what a workspace held before is of no account)
+            assert all(torch.equal(a, b) for a, b in zip(first, call()))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_bias_gradient_over_blocks_of_rows(dev, dtype):
+    """More rows than a block of the bias gradient without dx takes (2^20): its last block is of fewer rows than workgroups share."""
+    import gq
+    m, n, k = (1 << 20) + 100, 9, 32
+    gen = torch.Generator(device=dev).manual_seed(4)
+    dy, z = (torch.randn(m, n, generator=gen, device=dev).to(dtype) for _ in range(2))
+    w = gq.repack(O.Q8_0, torch.zeros(gq.gguf_bytes(O.Q8_0, n, k), dtype=torch.uint8, device=dev), n, k)
+    out = gq.linear_bwd(O.Q8_0, w, dy, z, n, k, act=3, want_dx=False, want_dbias=True)
+    dz = dy.double() * (z.double() > 0)
+    assert torch.equal(out["dz"].double(), dz)
+    # (a workgroup adds its 4097 rows in fp32: as many sums that grow as a root, each off by up to half a step; 256 of them are added in 64 bits)
+    err = (out["dbias"].double() - dz.sum(0)).abs()
+    assert bool((err <= 2 ** -24 * 4097 ** 0.5 * 4 * dz.pow(2).sum(0).sqrt() + 2 ** -24 * dz.sum(0).abs()).all())

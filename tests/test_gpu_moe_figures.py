@@ -58,3 +58,21 @@ def test_products_of_experts(dev, fmt, down, dtype, m, e, top, n, k):
     diff = (y.double() - ref).norm(dim=1)
     print(f"share {float((diff / err).max()):.3f}")
     assert bool((diff <= err).all()), (diff / err).tolist()
+
+
+@pytest.mark.parametrize("fmt,down", [(O.Q4_0, O.Q8_0), (O.Q8_0, O.Q4_K), (O.Q4_K, O.Q6_K), (O.Q6_K, O.Q4_0)])
+def test_the_same_again(dev, fmt, down):
+    """Two calls on the same tokens give the same bits, choice and output, whatever the workspace held."""
+    import gq
+    la = Layer(dev, fmt, down, 24, 512, 2048, seed=2)
+    la.router *= 1 / la.size
+    for m in (1, 3, 4, 5, 16, 17, 37, 64):
+        x, ws = la.x(m, torch.bfloat16), gq.Workspace(dev)
+
+        def call():
+            return gq.moe_layer(fmt, *la.packed[:2], down, la.packed[2], la.router, x, la.n, la.k, la.e, 6, save=True, workspace=ws)
+
+        first = [t.clone() for t in call()]
+        for _ in range(3):
+            ws.ensure(1).fill_(0xFF)
+            assert all(torch.equal(a, b) for a, b in zip(first, call()))
