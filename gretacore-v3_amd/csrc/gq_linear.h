@@ -59,6 +59,7 @@ int gq_launch_linear_rb(int fmt, const void *w, const _Float16 *a16, const float
                         hipStream_t s);
 // the epilogue epi of the parts' sums [parts][M][N] (gq_linear.hip)
 int gq_launch_linear_sum(const float *part, const void *epi, int M, int N, int parts, hipStream_t s);
-// Parts are taken only as far as a workgroup a CU goes, each with an fp32 tile of at most 128 x 256 outputs, and at most 8
+// At most 8 parts, chosen by the rounds they make (gq_linear_rb.hip); their sums together fit kLinPartBytes, those of a workgroup a CU with an fp32
+// tile of 128 x 256 outputs each
 constexpr int kLinParts = 8;
 constexpr size_t kLinPartBytes = (size_t)256 * 128 * 256 * 4;

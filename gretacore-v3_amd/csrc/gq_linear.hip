@@ -239,7 +239,8 @@ int launch_rows_t(const void *w, const _Float16 *a16, int lda, const float *rs, 
 // ---- backward ----------------------------------------------------------------------
 // dz = dy act'(z): one pass over dy and z, a workgroup a row at a time (row blockIdx.x, + gridDim.x, ...).  dz goes out in its own
 // type where it is wanted, and, as it is before that rounding, to fp16 with one power-of-two scale per row (the row's
-// largest to [2^14, 2^15); 2^-114 to 2^126), padded with zeros to np columns: the A operand of dx.  The workgroup's rows are summed
+// largest to [2^14, 2^15); 2^-114 to 2^126), padded with zeros to np columns: the A operand of dx, of the matrix cores' types the one
+// with the most bits (2.1e-4 of a row; products of fp32 would leave them).  The workgroup's rows are summed
 // by column into its row of `part` (dbias), which a last kernel adds over the workgroups in their order.  The first RUNS * 4096
 // columns of a row and their sums stay in registers, the rest (RUNS = 4 alone) is computed twice and summed in `part`.  The row's last,
 // ragged run is one thread's, on a path of its own: a launch starts with its code to be fetched, and every unrolled run's

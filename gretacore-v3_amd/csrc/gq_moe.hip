@@ -4,9 +4,10 @@
 //   l[m][e] = sum_k x[m][k] Wr[e][k]                    k_moe_logits, in 64 bits: which of two experts is larger decides the layer
 //   S_m, w_me                                           k_moe_plan: the choice, and the list of each expert's tokens
 //   h_me = act(Wg_e x_m) * (Wu_e x_m)                   k_moe_gu_*: one row of h a (token, expert) pair
-//   y_m = r_m + sum over S_m of w_me Wd_e h_me          k_moe_down_*: a workgroup adds its 16 columns over all experts
+//   y_m = r_m + sum over S_m of w_me Wd_e h_me          k_moe_down_*: a workgroup adds its row tiles' columns (16, more tokens: 32) over all
+//                                                       experts, or over a part of them
 //
-// The weights of the experts taken bound all of it; each is read once for up to 16 of its tokens.
+// The weights of the experts taken bound all of it; each is read once for up to 16 of its tokens, 32 where experts have many (moe_tiles).
 #include <algorithm>
 #include <type_traits>
 
@@ -255,7 +256,7 @@ __global__ void __launch_bounds__(64) k_moe_choose(RouteArgs a, int E, int top) 
 }
 
 // ---- plan ---------------------------------------------------------------------------
-// The choice (NE: experts a lane; 0: ids and weights are given), each expert's pairs in order of their tokens, in blocks of 16.
+// The choice (NE: experts a lane; 0: ids and weights are given), each expert's pairs in order of their tokens, in blocks of 16 or 32 (2^MoePlan::sh).
 // Ids outside 0 .. E - 1 name no expert; an expert that a token names twice gets one pair with both weights.
 constexpr int kPlanThreads = 1024;
 // Is this workgroup the last of n to arrive at a counter (zero before the launch)?  What the others stored before they came, by st_agent, can
@@ -374,7 +375,7 @@ GQ_DEV float moe_gu_h(At at, int nl, int m, float f, int act) {
 }
 
 // Up to 4 tokens of 16-bit x: codes and x as they are, scales in fp32 (gq_rows_frag.h); row j is token j.  h goes out in fp16 (nib:
-// in the nibbles' order) with a power-of-two scale for each 32 of a row, the scale groups of W_down's products; the inverse of block
+// in the nibbles' order; as the matrix cores take it, 2.1e-4 of h) with a power-of-two scale for each 32 of a row, the scale groups of W_down's products; the inverse of block
 // 2 m + i of 128 values to hs[pair][128s][i][m].
 // Workgroup (j, q): 32 columns of the expert that pair q names first.  ROUTE: the choice is made here, by every workgroup for itself (8 of
 // 64 experts of 1024 x 2048: 20.5 us the layer, 23.1 with the choice in a launch of its own); the first one keeps it.
@@ -561,8 +562,9 @@ k_moe_gu_rows(const uint8_t *__restrict__ wg, const uint8_t *__restrict__ wu, si
 }
 
 // ---- down ------------------------------------------------------------------------------
-// A workgroup owns a row tile of every expert's W_down (16 columns of y); its KS waves take the units of all blocks in turn
-// (block by block, unit by unit), so that the sum over a token's experts stays in the workgroup, in one order.
+// A workgroup owns R row tiles of every expert's W_down (16 R columns of y: one tile with few tokens, two with more); its KS waves take the units
+// of all blocks, or of its part of them, in turn (block by block, unit by unit), so that the sum over a token's experts stays in the workgroup,
+// in one order, and parts are added in theirs (k_moe_sum).
 struct ItemAt {
   int b, u;
   GQ_DEV_M void next(int by, int units) {
@@ -1071,7 +1073,7 @@ int moe_products(const gq_moe &l, const void *x, int xt, const RouteArgs *a, con
   else if (gq_fmt_is_q6k(l.fmt)) GQ_TRY(GQ_GU_F(GQ_FMT_Q6_K));
   else GQ_TRY(GQ_GU_F(GQ_FMT_Q4_K));
 #undef GQ_GU_F
-  if (!moe_few(l, M))
+  if (!moe_few(l, M))  // (h as the matrix cores take it, fp16 under a power of two per row: 2.1e-4 of it)
     GQ_TRY(gq_launch_a_to_f16(b.h, GQ_DT_F32, b.h16, b.hs, M * l.top_k, (int)l.N, b.ldh,
                               l.fmt_down == GQ_FMT_Q4_0 || gq_fmt_is_q4k(l.fmt_down), s));
 #define GQ_DOWN_F(F) launch_down_t<F>(l, ids, weights, plan, b, resid, y, dt, M, s)
