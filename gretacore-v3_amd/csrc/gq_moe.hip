@@ -882,6 +882,8 @@ bool moe_few(const gq_moe &l, size_t M) {
 // them (us the layer by one / two tiles, Q4_K with Q6_K and Q8_0 with Q4_0: 64 tokens, 2 of 8 of 14336 x 4096, 295 / 279 and 311 / 271; 20 tokens, 4 of 4
 // of 4096 x 4096, 80 / 68 and 83 / 67; with fewer the second tile's loads and products are for nothing: 48 tokens, 2 of 8 of 14336 x 4096, 231 / 271 and 242 / 256;
 // four tiles: 366 - 462 of the first, 212 and 176 of 43 tokens, 4 of 4 of 9984 x 3328, that two do in 189 and 207).
+// The mean serves uneven choices too, one expert that every token takes, or experts by their rank's inverse: 64 tokens, 8 of 128 of 768 x 2048,
+// 96 / 124 and 93 / 116 (112 / 129 and 106 / 121); 48 tokens, 2 of 8 of 14336 x 4096, 232 / 266 and 226 / 253 (281 / 275 and 273 / 261: 2 and 4 % lost).
 int moe_tiles(const gq_moe &l, size_t M) { return M * (size_t)l.top_k >= 16 * l.n_experts ? 2 : 1; }
 // Where a call's intermediate values lie in its workspace
 struct MoeWs {
