@@ -386,7 +386,6 @@ k_moe_gu_few(const uint8_t *__restrict__ wg, const uint8_t *__restrict__ wu, siz
              int nib, int M, int N, int K, int C, int units, int act, int E, int top) {
   static_assert(KS >= kMoeFew, "a wave a token");
   constexpr int NG = kFewGroups<FMT>, R = 2, T = 2 * R;
-  constexpr float OFF = kFewOff<FMT, XT>;
   __shared__ float red[KS][T][MR][64];
   extern __shared__ __attribute__((aligned(16))) uint8_t xs_s[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -424,36 +423,10 @@ k_moe_gu_few(const uint8_t *__restrict__ wg, const uint8_t *__restrict__ wu, siz
   uint32_t mg;  // (kept in a register)
   if constexpr (XT == GQ_DT_F16) asm volatile("v_mov_b32 %0, 0x64006400" : "=v"(mg));
   else asm volatile("v_mov_b32 %0, 0x43004300" : "=v"(mg));
-  constexpr uint32_t one = XT == GQ_DT_F16 ? 0x3C003C00u : 0x3F803F80u;
-  const gq_u4 ones = {one, one, one, one};
-  const gq_f4 zero = {0.f, 0.f, 0.f, 0.f};
-  auto add = [&](int unit, int st, int p) __attribute__((always_inline)) {
-    const uint32_t at = x0 + xd * (uint32_t)unit;
-    float s[T][2], mn[T][2];
-#pragma unroll
-    for (int t = 0; t < T; ++t) few_scales<FMT>(us[st][t][p], unit, g & (NG - 1), s[t], mn[t]);
-#pragma unroll
-    for (int m = 0; m < 2; ++m) {
-      const gq_u4 a0 = few_lds(xs_s, at, m, 0), a1 = few_lds(xs_s, at, m, 1);
-      gq_f4 sx = zero;
-      if constexpr (OFF != 0.f || FMT == GQ_FMT_Q4_K) sx = few_mfma<XT>(a1, ones, few_mfma<XT>(a0, ones, zero));
-#pragma unroll
-      for (int t = 0; t < T; ++t) {
-        gq_u4 b[2];
-        few_codes<FMT, XT>(us[st][t][p], m, mg, b);
-        const gq_f4 d = few_mfma<XT>(a1, b[1], few_mfma<XT>(a0, b[0], zero));
-        const float o = FMT == GQ_FMT_Q4_K ? fmaf(s[t][m], OFF, mn[t][m]) : 0.f;
-#pragma unroll
-        for (int v = 0; v < MR; ++v) {
-          if constexpr (FMT == GQ_FMT_Q4_K) acc[t][v] = fmaf(s[t][m], d[v], fmaf(-o, sx[v], acc[t][v]));
-          else acc[t][v] = fmaf(s[t][m], OFF != 0.f ? fmaf(-OFF, sx[v], d[v]) : d[v], acc[t][v]);
-        }
-      }
-    }
-  };
   auto compute = [&](int group, int st) __attribute__((always_inline)) {
 #pragma unroll
-    for (int p = 0; p < G; ++p) add(G * group + p, st, p);
+    for (int p = 0; p < G; ++p)
+      few_add<FMT, XT>(us[st], p, G * group + p, g, xs_s, x0 + xd * (uint32_t)(G * group + p), mg, acc);
   };
   walk_units<PD, KS>(units / G, wave, request, compute);
 #pragma unroll

@@ -222,6 +222,17 @@ GQ_DEV void few_scales(const FUnit<FMT> &u, int unit, int i, float (&s)[2], floa
     }
   }
 }
+// acc += what a step's product d, of the codes with their offset, and sum sx of x come to under the scale group's scale and minimum
+template <int FMT, int XT, int MR>
+GQ_DEV void few_scaled(float s, float mn, const gq_f4 &d, const gq_f4 &sx, float (&acc)[MR]) {
+  constexpr float OFF = kFewOff<FMT, XT>;
+  const float o = FMT == GQ_FMT_Q4_K ? fmaf(s, OFF, mn) : 0.f;
+#pragma unroll
+  for (int v = 0; v < MR; ++v) {
+    if constexpr (FMT == GQ_FMT_Q4_K) acc[v] = fmaf(s, d[v], fmaf(-o, sx[v], acc[v]));
+    else acc[v] = fmaf(s, OFF != 0.f ? fmaf(-OFF, sx[v], d[v]) : d[v], acc[v]);
+  }
+}
 // Rows 4 I + j of the operand: quad Q of x in the lane groups of scale group I, the others as in old
 template <int NG, int I, int Q>
 GQ_DEV uint32_t few_quad(uint32_t old, uint32_t src) {
@@ -251,6 +262,28 @@ GQ_DEV bool few_mine(int lane) {  // row lane % 4 is of this lane's scale group
 // operand of step m, half j of the unit whose 128 values start at offset `at` (of lane group 0)
 GQ_DEV gq_u4 few_lds(const uint8_t *xs, uint32_t at, int m, int j) {
   return *reinterpret_cast<const gq_u4 *>(xs + at + 128 * m + 16 * j);
+}
+// acc += unit `unit` of T tiles, us[t][p], times x at `at` of LDS
+template <int FMT, int XT, int T, int MR, int G>
+GQ_DEV void few_add(const FUnit<FMT> (&us)[T][G], int p, int unit, int g, const uint8_t *xs, uint32_t at, uint32_t mg, float (&acc)[T][MR]) {
+  constexpr uint32_t one = XT == GQ_DT_F16 ? 0x3C003C00u : 0x3F803F80u;
+  const gq_u4 ones = {one, one, one, one};
+  const gq_f4 zero = {0.f, 0.f, 0.f, 0.f};
+  float s[T][2], mn[T][2];
+#pragma unroll
+  for (int t = 0; t < T; ++t) few_scales<FMT>(us[t][p], unit, g & (kFewGroups<FMT> - 1), s[t], mn[t]);
+#pragma unroll
+  for (int m = 0; m < 2; ++m) {
+    const gq_u4 a0 = few_lds(xs, at, m, 0), a1 = few_lds(xs, at, m, 1);
+    gq_f4 sx = zero;
+    if constexpr (kFewOff<FMT, XT> != 0.f || FMT == GQ_FMT_Q4_K) sx = few_mfma<XT>(a1, ones, few_mfma<XT>(a0, ones, zero));
+#pragma unroll
+    for (int t = 0; t < T; ++t) {
+      gq_u4 b[2];
+      few_codes<FMT, XT>(us[t][p], m, mg, b);
+      few_scaled<FMT, XT>(s[t][m], mn[t][m], few_mfma<XT>(a1, b[1], few_mfma<XT>(a0, b[0], zero)), sx, acc[t]);
+    }
+  }
 }
 // Copies rows of `n` 16-bit values (n % 32 == 0, row r at src + r * n) to LDS, zeros up to np, nib: in the nibbles' order, by T threads.
 // ahead() is called between the last loads and their stores: what it requests is under way while they are waited for.
