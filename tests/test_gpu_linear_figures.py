@@ -124,3 +124,30 @@ def test_bias_gradient_over_blocks_of_rows(dev, dtype):
     # (a workgroup adds its 4097 rows in fp32: as many sums that grow as a root, each off by up to half a step; 256 of them are added in 64 bits)
     err = (out["dbias"].double() - dz.sum(0)).abs()
     assert bool((err <= 2 ** -24 * 4097 ** 0.5 * 4 * dz.pow(2).sum(0).sqrt() + 2 ** -24 * dz.sum(0).abs()).all())
+
+
+@pytest.mark.parametrize("fmt", [O.Q4_0, O.Q8_0, O.Q4_K, O.Q6_K])
+@pytest.mark.parametrize("n", [1, 3])
+def test_longest_rows(dev, fmt, n):
+    """K = 2^24, the largest: one row, sixteen, and more in blocks of sixteen; its gradient.  (fp32 sums of 2^17 units of 128 terms, one after the
+    other in four waves: 2^-24 256 of them beside the shares.)"""
+    import gq
+    k, m = 1 << 24, 17
+    b = O.gen_weights(fmt, n, k, seed=n)
+    w, packed = torch.from_numpy(O.dequant(fmt, b).reshape(n, k)).to(dev), gq.repack(fmt, torch.from_numpy(b).to(dev), n, k)
+    gen = torch.Generator(device=dev).manual_seed(1)
+    x = torch.randn(m, k, generator=gen, device=dev).to(torch.float16)
+    ws = gq.Workspace(dev, gq.linear_workspace_bytes(fmt, m, n, k))
+    ref = torch.stack([(w.double() * r.double()).sum(1) for r in x])
+    size = torch.stack([(w.double() * r.double()).pow(2).sum(1).sqrt() for r in x])
+    for rows in (1, 16, 17):
+        y = gq.linear(fmt, packed, x[:rows], n, k, out_dtype=torch.float32, workspace=ws)
+        share = 4 * (figures.tiles(fmt) if rows > 16 else figures.rows(fmt)) + 2 ** -16  # (single sums: within four of their deviations)
+        assert bool(((y.double() - ref[:rows]).abs() <= share * size[:rows]).all())
+    dy = torch.randn(3, n, generator=gen, device=dev)
+    dx = gq.linear_bwd(fmt, packed, dy, None, n, k, want_dz=False, workspace=gq.Workspace(dev))["dx"]
+    dz = figures.taken(dy).float()
+    for r in range(3):
+        # (a row's norm, as everywhere: a single weight of Q4_K whose minimum cancels it is 0 with an error of the minimum's half step)
+        want, size = (dz[r, :, None] * w).double().sum(0), (dz[r, :, None] * w).double().norm()
+        assert float((dx[r].double() - want).norm()) <= figures.tiles(fmt) * float(size)
